@@ -11,6 +11,7 @@
 #define XB_ERR_BAD_ROW 8     // a requested row outside [0, tokens)
 #define XB_ERR_SCRATCH 16    // scratch memory that a kernel must find zeroed was not
 #define XB_ERR_BAD_POSITION 32  // a token position outside the position table
+#define XB_ERR_NO_PAGE 64       // a request whose tokens found no free pages
 
 // Element type codes shared with the Python side.
 #define XB_F32 0

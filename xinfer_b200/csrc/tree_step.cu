@@ -1,0 +1,235 @@
+// What a step that verifies trees of drafted tokens does beside its model: the path that the model's own choices confirm, pages and
+// slots for tokens whose number only the device knows, and the accepted tokens' keys and values into those slots.
+#include "common.cuh"
+
+namespace {
+
+// ---- acceptance -------------------------------------------------------------------------------------------------------
+// Request b has the nodes token_start[b] .. token_start[b + 1] - 1; parents[t] is a node's place in its own tree (the root's: -1;
+// a parent comes before its children).  From the root on, the next node of the path is the child of lowest place whose token is
+// targets[its parent], as long as there is one and the path has room.  A warp per request.
+__global__ void tree_accept_kernel(int* accepted, int* path, int* next_tokens, const int* drafted, const int* targets, const int* parents,
+                                   const int* token_start, int requests, int tokens, int width) {
+    const int lane = threadIdx.x & 31, b = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5);
+    if (b >= requests) return;
+    const int first = min(max(token_start[b], 0), tokens), n = min(max(token_start[b + 1], first), tokens) - first;
+    int* mine = path + (size_t)b * width;
+    int len = 0, at = n > 0 ? 0 : -1, last = -1;
+    while (at >= 0 && len < width) {
+        if (lane == 0) mine[len] = first + at;
+        ++len;
+        last = targets[first + at];
+        int next = -1;
+        for (int base = (at + 1) & ~31; base < n && next < 0; base += 32) {
+            const int i = base + lane;
+            const bool fits = i > at && i < n && parents[first + i] == at && drafted[first + i] == last;
+            const unsigned who = __ballot_sync(0xffffffffu, fits);
+            if (who) next = base + __ffs(who) - 1;
+        }
+        at = next;
+    }
+    for (int i = len + lane; i < width; i += 32) mine[i] = -1;
+    if (lane == 0) {
+        accepted[b] = len;
+        next_tokens[b] = last;
+    }
+}
+
+// ---- pages and slots -----------------------------------------------------------------------------------------------------
+// Request b holds ceil(lengths[b] / page_size) pages, the first entries of its row of the block table, and gets new_tokens[b] more
+// tokens; one that has ended (-1) gives its pages back.  Free pages lie in a ring of `ring_size` page ids, `ring[1]` of them from
+// place ring[0] on: pages are taken at its head, in order of the requests, and given back at its end, so nothing that a block reads
+// is written by another and the same call may be made twice.  A request whose pages are not all there gets none and no slots; its
+// length stays.  Every block forms the requests' sums for itself and takes a share of the tokens.
+constexpr int SLOT_THREADS = 256;
+constexpr int SLOT_TOKENS = 1024;               // tokens a block takes at a time
+constexpr int SLOT_REQUESTS = 8192;             // requests of a call: their starts lie in shared memory
+
+struct SlotArgs {
+    long long* slots;              // [capacity]: page * page_size + offset; -1: none
+    int* positions;                // [capacity]
+    int* request;                  // [capacity]: the token's request, -1 behind them all
+    int* token_start;              // [requests + 1]
+    int* lengths_out;              // [requests]
+    int* ring_out;                 // head and count afterwards
+    int* table;                    // [requests, table_stride]
+    int* free_ring;                // [ring_size]
+    const int* ring;               // head, count
+    const int* lengths;            // [requests]
+    const int* new_tokens;         // [requests]
+    int requests, capacity, table_stride, page_size, ring_size;
+    int* err;
+};
+
+struct Sums {
+    int tokens, need, back;
+};
+__device__ __forceinline__ Sums operator+(Sums a, Sums b) { return Sums{a.tokens + b.tokens, a.need + b.need, a.back + b.back}; }
+
+// Exclusive prefix of `mine` over the block's threads; `total` receives the sum.
+__device__ __forceinline__ Sums block_prefix(Sums mine, Sums* of_warps, Sums& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Sums incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const Sums v{__shfl_up_sync(0xffffffffu, incl.tokens, o), __shfl_up_sync(0xffffffffu, incl.need, o), __shfl_up_sync(0xffffffffu, incl.back, o)};
+        if (lane >= o) incl = incl + v;
+    }
+    if (lane == 31) of_warps[warp] = incl;
+    __syncthreads();
+    Sums before{0, 0, 0};
+    total = Sums{0, 0, 0};
+    for (int w = 0; w < SLOT_THREADS / 32; ++w) {
+        if (w < warp) before = before + of_warps[w];
+        total = total + of_warps[w];
+    }
+    return Sums{before.tokens + incl.tokens - mine.tokens, before.need + incl.need - mine.need, before.back + incl.back - mine.back};
+}
+
+__global__ void __launch_bounds__(SLOT_THREADS)
+cache_slots_kernel(const SlotArgs A) {
+    extern __shared__ int starts[];                              // [requests + 1], then [requests]: pages taken before the request's own
+    int* taken_before = starts + A.requests + 1;                 // (-1: the request was not served)
+    __shared__ Sums of_warps[SLOT_THREADS / 32];
+    __shared__ int taken;
+    const int each = (A.requests + SLOT_THREADS - 1) / SLOT_THREADS, b0 = (int)threadIdx.x * each;
+    const int ps = A.page_size, head = (A.ring[0] % A.ring_size + A.ring_size) % A.ring_size, count = min(max(A.ring[1], 0), A.ring_size);
+    // whether the request's pages, those it holds and those it asks for, fit its row of the table; one whose do not asks for none
+    auto fits = [&](int b) { return ((long long)max(A.lengths[b], 0) + max(A.new_tokens[b], 0) + ps - 1) / ps <= A.table_stride; };
+    auto held_by = [&](int b) { return (int)(((long long)max(A.lengths[b], 0) + ps - 1) / ps); };
+    auto sums_of = [&](int b) {
+        const int add = A.new_tokens[b];
+        if (!fits(b)) return Sums{max(add, 0), 0, 0};
+        const int held = held_by(b);
+        if (add < 0) return Sums{0, 0, held};
+        return Sums{add, (int)(((long long)max(A.lengths[b], 0) + add + ps - 1) / ps) - held, 0};
+    };
+    Sums mine{0, 0, 0}, total;
+    for (int b = b0; b < min(b0 + each, A.requests); ++b) mine = mine + sums_of(b);
+    if (threadIdx.x == 0) taken = 0;
+    Sums at = block_prefix(mine, of_warps, total);
+    const bool first_block = blockIdx.x == 0;
+    for (int b = b0; b < min(b0 + each, A.requests); ++b) {
+        const Sums s = sums_of(b);
+        const int len = max(A.lengths[b], 0), add = A.new_tokens[b], held = held_by(b);
+        const bool served = fits(b) && (s.need == 0 || at.need + s.need <= count);
+        starts[b] = at.tokens;
+        taken_before[b] = served ? at.need : -1;
+        if (served && s.need > 0) atomicMax(&taken, at.need + s.need);
+        if (first_block) {
+            A.token_start[b] = at.tokens;
+            A.lengths_out[b] = add < 0 ? 0 : (served ? len + add : len);
+            if (!served) atomicOr(A.err, XB_ERR_NO_PAGE);
+            int* row = A.table + (size_t)b * A.table_stride;
+            if (served)
+                for (int i = 0; i < s.need; ++i) row[held + i] = A.free_ring[(int)(((long long)head + at.need + i) % A.ring_size)];
+            if (total.back + count <= A.ring_size)
+                for (int i = 0; i < s.back; ++i) A.free_ring[(int)(((long long)head + count + at.back + i) % A.ring_size)] = row[i];
+        }
+        at = at + s;
+    }
+    if (threadIdx.x == 0) starts[A.requests] = total.tokens;
+    __syncthreads();
+    if (first_block && threadIdx.x == 0) {
+        A.token_start[A.requests] = total.tokens;
+        A.ring_out[0] = (int)(((long long)head + taken) % A.ring_size);
+        const bool room = total.back + count <= A.ring_size;     // (more pages than the ring was made for: they are not taken back)
+        A.ring_out[1] = count - taken + (room ? total.back : 0);
+        if (!room) atomicOr(A.err, XB_ERR_BAD_PAGE);
+        if (total.tokens > A.capacity) atomicOr(A.err, XB_ERR_BAD_ROW);
+    }
+    for (int base = (int)blockIdx.x * SLOT_TOKENS; base < A.capacity; base += (int)gridDim.x * SLOT_TOKENS)
+        for (int t = base + (int)threadIdx.x; t < min(base + SLOT_TOKENS, A.capacity); t += SLOT_THREADS) {
+            if (t >= total.tokens) {
+                A.slots[t] = -1;
+                A.positions[t] = 0;
+                A.request[t] = -1;
+                continue;
+            }
+            int lo = 0, hi = A.requests;                         // starts[lo] <= t < starts[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (starts[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            const int len = max(A.lengths[lo], 0), pos = len + t - starts[lo], place = pos / ps, held = held_by(lo);
+            long long slot = -1;
+            if (taken_before[lo] >= 0) {
+                const int page = place < held ? A.table[(size_t)lo * A.table_stride + place]
+                                              : A.free_ring[(int)(((long long)head + taken_before[lo] + place - held) % A.ring_size)];
+                if (page >= 0) slot = (long long)page * ps + pos % ps;
+                else atomicOr(A.err, XB_ERR_BAD_PAGE);
+            }
+            A.slots[t] = slot;
+            A.positions[t] = pos;
+            A.request[t] = lo;
+        }
+}
+
+// ---- accepted rows into the cache ------------------------------------------------------------------------------------------
+// Token i of the step (slots[i], the o-th new one of request b = request_of[i], o = i - token_start[b]) is drafted row path[b][o]:
+// its keys and values of every layer go to its slot.  Grid (token, layer); U: the unit of the copy.
+template <typename U>
+__global__ void cache_commit_kernel(const void* const* layers /* [layers][4]: k cache, v cache, new k, new v */, const long long* slots,
+                                    const int* request_of, const int* token_start, const int* path, int requests, int width, int rows, int nkv,
+                                    int units, int page_size, long long num_slots, int* err) {
+    const int i = blockIdx.x;
+    const int b = request_of[i];
+    if (b < 0 || b >= requests) return;
+    const long long slot = slots[i];
+    const int o = i - token_start[b];
+    if (slot < 0 || o < 0 || o >= width) return;
+    const int row = path[(size_t)b * width + o];
+    if (row < 0) return;
+    if (row >= rows || slot >= num_slots) {
+        if (threadIdx.x == 0) atomicOr(err, row >= rows ? XB_ERR_BAD_ROW : XB_ERR_BAD_PAGE);
+        return;
+    }
+    const void* const* mine = layers + 4 * (size_t)blockIdx.y;
+    const long long page = slot / page_size, off = slot % page_size;
+    for (int c = threadIdx.x; c < 2 * nkv * units; c += blockDim.x) {
+        const int what = c / (nkv * units), g = c / units % nkv, u = c % units;
+        const U* src = (const U*)mine[2 + what];
+        U* dst = (U*)mine[what];
+        dst[((page * nkv + g) * page_size + off) * units + u] = src[((long long)row * nkv + g) * units + u];
+    }
+}
+
+}  // namespace
+
+XB_EXPORT int xb_tree_accept(int* accepted, int* path, int* next_tokens, const int* drafted, const int* targets, const int* parents,
+                             const int* token_start, int requests, int tokens, int width, cudaStream_t stream) {
+    if (requests <= 0) return 0;
+    if (width < 1) return (int)cudaErrorInvalidValue;
+    tree_accept_kernel<<<(requests + 3) / 4, 128, 0, stream>>>(accepted, path, next_tokens, drafted, targets, parents, token_start, requests, tokens, width);
+    return xb_launch_status();
+}
+
+XB_EXPORT int xb_cache_slots(long long* slots, int* positions, int* request, int* token_start, int* lengths_out, int* ring_out, int* table, int* free_ring,
+                             const int* ring, const int* lengths, const int* new_tokens, int requests, int capacity, int table_stride, int page_size,
+                             int ring_size, int* err, cudaStream_t stream) {
+    if (requests <= 0) return 0;
+    if (requests > SLOT_REQUESTS || page_size < 1 || ring_size < 1 || table_stride < 1) return (int)cudaErrorInvalidValue;
+    const SlotArgs A{slots, positions, request, token_start, lengths_out, ring_out, table, free_ring, ring, lengths, new_tokens,
+                     requests, capacity, table_stride, page_size, ring_size, err};
+    int blocks = (capacity + SLOT_TOKENS - 1) / SLOT_TOKENS;
+    blocks = blocks < 1 ? 1 : (blocks > 148 ? 148 : blocks);
+    const size_t smem = (2 * (size_t)requests + 1) * 4;
+    static const cudaError_t room = cudaFuncSetAttribute(cache_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * SLOT_REQUESTS + 1) * 4);
+    if (room != cudaSuccess) return (int)room;
+    cache_slots_kernel<<<blocks, SLOT_THREADS, smem, stream>>>(A);
+    return xb_launch_status();
+}
+
+XB_EXPORT int xb_cache_commit(const void* const* layers, int num_layers, const long long* slots, const int* request_of, const int* token_start,
+                              const int* path, int tokens, int requests, int width, int rows, int nkv, int row_bytes, int page_size, long long num_slots,
+                              int* err, cudaStream_t stream) {
+    if (tokens <= 0 || num_layers <= 0 || requests <= 0) return 0;
+    if (num_layers > 65535 || row_bytes < 2 || row_bytes % 2 || page_size < 1) return (int)cudaErrorInvalidValue;
+    const dim3 grid(tokens, num_layers);
+    if (row_bytes % 16 == 0)
+        cache_commit_kernel<uint4><<<grid, 128, 0, stream>>>(layers, slots, request_of, token_start, path, requests, width, rows, nkv, row_bytes / 16, page_size, num_slots, err);
+    else
+        cache_commit_kernel<uint16_t><<<grid, 128, 0, stream>>>(layers, slots, request_of, token_start, path, requests, width, rows, nkv, row_bytes / 2, page_size, num_slots, err);
+    return xb_launch_status();
+}

@@ -107,7 +107,7 @@ def _ok(status: int, what: str, n: int = 1) -> None:
 
 
 # device-side error word -------------------------------------------------------------------------
-ERR_BAD_TOKEN, ERR_BAD_PAGE, ERR_WAIT, ERR_BAD_ROW, ERR_SCRATCH, ERR_BAD_POSITION = 1, 2, 4, 8, 16, 32
+ERR_BAD_TOKEN, ERR_BAD_PAGE, ERR_WAIT, ERR_BAD_ROW, ERR_SCRATCH, ERR_BAD_POSITION, ERR_NO_PAGE = 1, 2, 4, 8, 16, 32, 64
 
 
 def describe_error(word: int) -> str:
@@ -122,6 +122,8 @@ def describe_error(word: int) -> str:
         parts.append("a requested row outside the step's tokens")
     if word & ERR_BAD_POSITION:
         parts.append("a token position outside the position table")
+    if word & ERR_NO_PAGE:
+        parts.append("a request whose tokens found no free pages")
     if word & ERR_SCRATCH:
         parts.append("scratch memory that a kernel must find zeroed was not")
     return "; ".join(parts) or "no error"
@@ -1753,3 +1755,235 @@ def stream_mix(out, x, read, weight, eps, err, *, branch=None, mix=None, write=N
                                     x.stride(0), x.stride(1), _ptr(branch), _ptr(rows), _ptr(read), _ptr(mix), _ptr(write),
                                     _ptr(weight), nrows, n, dim, src, float(eps), float(weight_offset), err.data_ptr(),
                                     _stream()), "stream_mix")
+
+
+# ---- a step that verifies trees of drafted tokens ----------------------------------------------------------------------------
+def _token_rows(t, name: str, dtype, tokens: int, heads: int, d: int) -> int:
+    """Elements between the tokens of ``[tokens, heads, d]`` whose heads are dense; tokens may lie further apart."""
+    try:
+        ok = t.is_cuda and t.dtype == dtype and t.shape == (tokens, heads, d)
+    except AttributeError:
+        ok = False
+    if ok:
+        st, sh, sd = t.stride()
+        if (sd == 1 or d == 1) and (sh == d or heads == 1) and (st >= heads * d or tokens <= 1):
+            return st if tokens > 1 else heads * d
+    if not isinstance(t, torch.Tensor):
+        raise KernelError(f"{name}: expected a tensor, got {type(t).__name__}")
+    raise KernelError(f"{name}: expected a {dtype} CUDA tensor of shape {(tokens, heads, d)} with dense heads, got {t.dtype} {tuple(t.shape)} "
+                      f"with strides {t.stride()} on {t.device}")
+
+
+def tree_attention_scratch(tokens: int, nh: int, nkv: int, d: int, dtype) -> int:
+    """float32 numbers of scratch that ``tree_attention`` takes for that many drafted tokens; 0: none."""
+    return 0
+
+
+def tree_attention(out, q, k_new, v_new, k_cache, v_cache, context, token_start, ancestors, block_table, scale, err, *, scratch=None,
+                   depth=None, window: Optional[int] = None):
+    """Attention of drafted tokens that form a tree per request.  Request b has the tokens ``token_start[b] .. token_start[b + 1]``
+    of ``q`` ``[T, heads, d]`` and ``context[b]`` keys in the cache ``[page, kv_head, slot, d]`` by its row of ``block_table``; the
+    drafted tokens' own keys and values are ``k_new`` and ``v_new`` ``[T, kv_heads, d]``, outside the cache.  Token i sees the cached
+    keys and the drafted tokens of its request whose bits are set in ``ancestors[i]`` (int32 words, the tree's first token the
+    lowest bit; its own bit as well as any).  ``window``: of these, the ones fewer than that many positions before it, by ``depth``
+    (int32: a token's position is the context plus its depth).  A token that sees nothing gets zeros.  ``out``, ``q``, ``k_new``
+    and ``v_new`` have dense heads, their tokens may lie apart.  ``scratch``: float32, ``tree_attention_scratch`` numbers, contents
+    undefined, not shared by calls that may overlap."""
+    T, nh, d = q.shape
+    nkv = k_new.shape[1]
+    dtype = q.dtype
+    code = dtype_code(dtype)
+    if nkv < 1 or nh % nkv:
+        raise KernelError(f"{nh} query heads do not divide into {nkv} key/value heads")
+    if not 1 <= d <= 512:
+        raise KernelError(f"tree_attention takes heads of 1 to 512 channels, not {d}")
+    so, sq = _token_rows(out, "out", dtype, T, nh, d), _token_rows(q, "q", dtype, T, nh, d)
+    sk, sv = _token_rows(k_new, "k_new", dtype, T, nkv, d), _token_rows(v_new, "v_new", dtype, T, nkv, d)
+    _need(k_cache, "k_cache", dtype, (None, nkv, None, d))
+    pages, _, page_size, _ = k_cache.shape
+    _need(v_cache, "v_cache", dtype, (pages, nkv, page_size, d))
+    _need(context, "context", torch.int32)
+    requests = context.numel()
+    _need(token_start, "token_start", torch.int32, (requests + 1,))
+    _need(block_table, "block_table", torch.int32, (requests, None))
+    _need(ancestors, "ancestors", torch.int32, (T, None))
+    _need(err, "err", torch.int32)
+    if window is not None and window < 1:
+        raise KernelError(f"a window of {window} keys")
+    if window is not None and depth is None:
+        raise KernelError("a window goes by the tokens' depths")
+    if depth is not None:
+        _need(depth, "depth", torch.int32, (T,))
+    need = tree_attention_scratch(T, nh, nkv, d, dtype)
+    if need:
+        _need(scratch, "scratch", torch.float32)
+        if scratch.numel() < need:
+            raise KernelError(f"scratch holds {scratch.numel()} numbers, {need} are needed")
+    _ok(kernels_lib().xb_tree_attention(
+        code, out.data_ptr(), q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), context.data_ptr(),
+        token_start.data_ptr(), ancestors.data_ptr(), _ptr(depth), block_table.data_ptr(), so, sq, sk, sv, T, requests, ancestors.shape[1],
+        block_table.shape[1], nh, nkv, d, page_size, pages, int(window or 0), float(scale), err.data_ptr(), _stream()), "tree_attention")
+
+
+def _logit_rows(t, name: str, shape) -> int:
+    if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32 or t.shape != shape
+            or (shape[1] > 1 and t.stride(1) != 1) or (shape[0] > 1 and t.stride(0) < shape[1])):
+        raise KernelError(f"{name}: expected float32 CUDA rows {tuple(shape)} with dense numbers, got "
+                          + (f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__))
+    return t.stride(0) if shape[0] > 1 else shape[1]
+
+
+def logit_rules(out, logits, penalties, history, history_start, prompt_len, *, list_of_row=None, tree=None, bias=None, mask=None, mask_of_row=None):
+    """Penalties for repeated tokens, biases and grammar masks on float32 ``logits`` ``[R, V]``; ``out`` may be the logits themselves.
+    ``penalties`` ``[R, 3]``: repetition (x / p or x * p by the logit's sign, for tokens of the prompt or said since; 1: none),
+    frequency and presence (of tokens said since; 0: none).  Lists of tokens lie one behind another in ``history`` (int32), list i from
+    ``history_start[i]`` to ``history_start[i + 1]``; its first ``prompt_len[i]`` tokens are the prompt.  Row r counts the list
+    ``list_of_row[r]`` (negative: none; default: list r).  ``tree`` = (drafted ``[R]``, ancestors ``[R, words]``, first_row ``[R]``): the
+    row also counts the drafted tokens of the rows ``first_row[r] + i`` for every bit i of its ancestors.  ``bias`` = (start ``[R + 1]``,
+    tokens, values): numbers added to tokens of a row.  ``mask`` ``[M, words of 32 tokens]``: row r keeps only the tokens whose bits
+    are set in row ``mask_of_row[r]`` (negative: all; default: row r).  Tokens outside the vocabulary are passed over."""
+    R, V = logits.shape
+    si, so = _logit_rows(logits, "logits", (R, V)), _logit_rows(out, "out", (R, V))
+    if out.data_ptr() == logits.data_ptr() and si != so:
+        raise KernelError("rows that are changed in place have one stride")
+    _need(penalties, "penalties", torch.float32, (R, 3))
+    _need(history, "history", torch.int32)
+    _need(prompt_len, "prompt_len", torch.int32)
+    lists = prompt_len.numel()
+    _need(history_start, "history_start", torch.int32, (lists + 1,))
+    if list_of_row is not None:
+        _need(list_of_row, "list_of_row", torch.int32, (R,))
+    elif lists != R:
+        raise KernelError(f"{lists} lists for {R} rows need list_of_row")
+    drafted = ancestors = first_row = bias_start = bias_tokens = bias_values = None
+    words = mask_words = masks = 0
+    if tree is not None:
+        drafted, ancestors, first_row = tree
+        _need(drafted, "drafted", torch.int32, (R,))
+        _need(ancestors, "ancestors", torch.int32, (R, None))
+        _need(first_row, "first_row", torch.int32, (R,))
+        words = ancestors.shape[1]
+    if bias is not None:
+        bias_start, bias_tokens, bias_values = bias
+        _need(bias_start, "bias start", torch.int32, (R + 1,))
+        _need(bias_tokens, "bias tokens", torch.int32)
+        _need(bias_values, "bias values", torch.float32, tuple(bias_tokens.shape))
+    if mask is not None:
+        _need(mask, "mask", torch.int32, (None, None))
+        masks, mask_words = mask.shape
+        if mask_words * 32 < V:
+            raise KernelError(f"masks of {mask_words} words do not cover {V} tokens")
+        if mask_of_row is not None:
+            _need(mask_of_row, "mask_of_row", torch.int32, (R,))
+        elif masks != R:
+            raise KernelError(f"{masks} masks for {R} rows need mask_of_row")
+    elif mask_of_row is not None:
+        raise KernelError("mask_of_row without masks")
+    _ok(kernels_lib().xb_logit_rules(
+        out.data_ptr(), logits.data_ptr(), penalties.data_ptr(), history.data_ptr(), history_start.data_ptr(), prompt_len.data_ptr(),
+        _ptr(list_of_row), _ptr(drafted), _ptr(ancestors), _ptr(first_row), _ptr(bias_start), _ptr(bias_tokens), _ptr(bias_values), _ptr(mask),
+        _ptr(mask_of_row), so, si, history.numel(), bias_tokens.numel() if bias is not None else 0, R, lists, V, words, masks, mask_words,
+        _stream()), "logit_rules")
+
+
+def tree_accept(accepted, path, next_tokens, drafted, targets, parents, token_start):
+    """Which drafted tokens the model's own choices confirm.  Node i of request b's tree is token ``token_start[b] + i``;
+    ``parents`` holds a node's place in its tree (-1: the root, which is node 0; a parent comes before its children) and
+    ``targets`` the token that the model chose behind each node.  From the root on the path goes to the child of lowest place whose
+    ``drafted`` token is its parent's target.  ``path`` ``[B, width]`` receives the path's tokens (rows of the step; -1 behind them),
+    ``accepted`` how many they are (at most the width), ``next_tokens`` the target of the last one (-1 for a request without nodes)."""
+    _need(accepted, "accepted", torch.int32)
+    B, T = accepted.numel(), drafted.numel()
+    _need(path, "path", torch.int32, (B, None))
+    _need(next_tokens, "next_tokens", torch.int32, (B,))
+    _need(drafted, "drafted", torch.int32, (T,))
+    _need(targets, "targets", torch.int32, (T,))
+    _need(parents, "parents", torch.int32, (T,))
+    _need(token_start, "token_start", torch.int32, (B + 1,))
+    if path.shape[1] < 1:
+        raise KernelError("a path needs room for its root")
+    _ok(kernels_lib().xb_tree_accept(accepted.data_ptr(), path.data_ptr(), next_tokens.data_ptr(), drafted.data_ptr(), targets.data_ptr(),
+                                     parents.data_ptr(), token_start.data_ptr(), B, T, path.shape[1], _stream()), "tree_accept")
+
+
+SLOT_REQUESTS_MAX = 8192
+
+
+def cache_slots(slots, positions, request_of, token_start, lengths_out, ring_out, block_table, free_ring, ring, lengths, new_tokens,
+                page_size: int, err):
+    """Pages and slots for ``new_tokens[b]`` more tokens of every request, of which only the device knows the number.  Request b
+    holds the pages of its ``lengths[b]`` tokens in the first entries of its row of ``block_table``; -1 new tokens: it has ended and
+    gives them back.  ``free_ring`` holds the free pages' ids, ``ring`` = (place of the first, how many).  Writes the block table's new
+    entries and the pages given back into ``free_ring``; ``ring_out`` and ``lengths_out`` receive the state afterwards (other memory than
+    ``ring`` and ``lengths``, so that a call may be made again); per token in order ``slots`` (int64, page * page_size + place; -1: none),
+    ``positions`` and ``request_of`` (-1 behind the last token), and ``token_start`` ``[B + 1]``.  Requests are served in their order; one
+    whose pages are not all there, or do not fit its row, is left as it was, its slots are -1 and the error word says so."""
+    _need(lengths, "lengths", torch.int32)
+    B = lengths.numel()
+    if B > SLOT_REQUESTS_MAX:
+        raise KernelError(f"{B} requests; a call takes {SLOT_REQUESTS_MAX}")
+    _need(slots, "slots", torch.int64)
+    n = slots.numel()
+    _need(positions, "positions", torch.int32, (n,))
+    _need(request_of, "request_of", torch.int32, (n,))
+    _need(token_start, "token_start", torch.int32, (B + 1,))
+    _need(lengths_out, "lengths_out", torch.int32, (B,))
+    _need(ring_out, "ring_out", torch.int32, (2,))
+    _need(block_table, "block_table", torch.int32, (B, None))
+    _need(free_ring, "free_ring", torch.int32)
+    _need(ring, "ring", torch.int32, (2,))
+    _need(new_tokens, "new_tokens", torch.int32, (B,))
+    _need(err, "err", torch.int32)
+    if page_size < 1 or not free_ring.numel() or not block_table.shape[1]:
+        raise KernelError("pages of at least one token, a ring and a table with room for one page")
+    if ring_out.data_ptr() == ring.data_ptr() or (B and lengths_out.data_ptr() == lengths.data_ptr()):
+        raise KernelError("the state afterwards goes to other memory than the state before")
+    _ok(kernels_lib().xb_cache_slots(
+        slots.data_ptr(), positions.data_ptr(), request_of.data_ptr(), token_start.data_ptr(), lengths_out.data_ptr(), ring_out.data_ptr(),
+        block_table.data_ptr(), free_ring.data_ptr(), ring.data_ptr(), lengths.data_ptr(), new_tokens.data_ptr(), B, n, block_table.shape[1],
+        int(page_size), free_ring.numel(), err.data_ptr(), _stream()), "cache_slots")
+
+
+class CommitTable:
+    """Where every layer's cached and new keys and values lie, for ``cache_commit``; made once (``commit_table``)."""
+
+    def __init__(self, tensors, pointers, shape, rows: int):
+        self.tensors, self.pointers, self.shape, self.rows = tensors, pointers, shape, rows      # (the tensors are kept alive)
+
+
+def commit_table(k_caches, v_caches, k_new, v_new) -> CommitTable:
+    """``k_caches`` and ``v_caches``: per layer ``[page, kv_head, slot, d]``; ``k_new`` and ``v_new``: per layer ``[rows, kv_heads, d]``;
+    all layers alike."""
+    layers = list(zip(k_caches, v_caches, k_new, v_new))
+    if not layers or not len(k_caches) == len(v_caches) == len(k_new) == len(v_new):
+        raise KernelError("commit_table: every layer has a key cache, a value cache, new keys and new values")
+    shape, dtype, rows = tuple(k_caches[0].shape), k_caches[0].dtype, k_new[0].shape[0]
+    dtype_code(dtype)
+    for kc, vc, kn, vn in layers:
+        for name, t, want in (("k_cache", kc, shape), ("v_cache", vc, shape), ("k_new", kn, (rows, shape[1], shape[3])),
+                              ("v_new", vn, (rows, shape[1], shape[3]))):
+            _need(t, name, dtype, want)
+            if t.data_ptr() % 16:
+                raise KernelError(f"{name}: starts off a 16-byte boundary")
+    pointers = torch.tensor([t.data_ptr() for layer in layers for t in layer], dtype=torch.int64).to(k_caches[0].device)
+    return CommitTable(layers, pointers, shape, rows)
+
+
+def cache_commit(table: CommitTable, slots, request_of, token_start, path, err):
+    """The keys and values of accepted tokens go to their slots, in every layer.  Entry i of ``slots`` and ``request_of`` (as
+    ``cache_slots`` wrote them) is token ``i - token_start[b]`` of request b = ``request_of[i]``, whose new row is
+    ``path[b, i - token_start[b]]`` (as ``tree_accept`` wrote it).  Entries without a request, a slot or a row are passed over."""
+    if not isinstance(table, CommitTable):
+        raise KernelError("cache_commit takes a table of commit_table")
+    pages, nkv, page_size, d = table.shape
+    _need(slots, "slots", torch.int64)
+    n = slots.numel()
+    _need(request_of, "request_of", torch.int32, (n,))
+    _need(path, "path", torch.int32, (None, None))
+    B, width = path.shape
+    _need(token_start, "token_start", torch.int32, (B + 1,))
+    _need(err, "err", torch.int32)
+    layers = len(table.tensors)
+    _ok(kernels_lib().xb_cache_commit(
+        table.pointers.data_ptr(), layers, slots.data_ptr(), request_of.data_ptr(), token_start.data_ptr(), path.data_ptr(), n, B, width,
+        table.rows, nkv, d * table.tensors[0][0].element_size(), page_size, pages * page_size, err.data_ptr(), _stream()), "cache_commit")
