@@ -28,7 +28,7 @@ tree_attention_kernel(const TreeArgs A) {
     if (b < 0) return;                       // a row of no request is left as it is
     const int g = h / (A.nh / A.nkv), first = clamp_start(A, A.token_start[b]), n = clamp_start(A, A.token_start[b + 1]) - first;
     const int context = context_of(A, b);
-    const int my_pos = context + (A.depth ? A.depth[t] : 0);
+    const int my_depth = A.window > 0 ? max(0, A.depth[t]) : 0, my_pos = context + my_depth;
     const int lo = A.window > 0 ? max(0, my_pos - A.window + 1) : 0;
     float* qs = q_rows + (size_t)warp * A.d;
     const T* q = (const T*)A.q + (size_t)t * A.q_stride + (size_t)h * A.d;
@@ -46,7 +46,7 @@ tree_attention_kernel(const TreeArgs A) {
         long long row = 0;                   // of the key, in elements of its tensor
         if (drafted) {
             seen = j < n && (A.ancestors[(size_t)t * A.words + (j >> 5)] >> (j & 31) & 1);
-            if (seen && A.window > 0) seen = A.depth[t] - A.depth[first + j] < A.window;
+            if (seen && A.window > 0) seen = my_depth - max(0, A.depth[first + j]) < A.window;
         } else {
             seen = j >= lo && j < context;
             if (seen) {
@@ -105,11 +105,18 @@ int launch(const TreeArgs& A, cudaStream_t stream) {
 XB_EXPORT int xb_tree_attention(int dtype, void* out, const void* q, const void* k_new, const void* v_new, const void* k_cache, const void* v_cache,
                                 const int* context, const int* token_start, const int* ancestors, const int* depth, const int* block_table,
                                 long long out_stride, long long q_stride, long long k_stride, long long v_stride, int tokens, int requests, int words,
-                                int table_stride, int nh, int nkv, int d, int page_size, int num_pages, int window, float scale, int* err,
-                                cudaStream_t stream) {
+                                int table_stride, int nh, int nkv, int d, int page_size, int num_pages, int window, float scale, float* scratch,
+                                int* err, cudaStream_t stream) {
     if (tokens <= 0 || requests <= 0) return 0;
-    if (d < 1 || d > 512 || nkv < 1 || nh % nkv || page_size < 1 || (window > 0 && !depth)) return (int)cudaErrorInvalidValue;
+    if (requests > LINE_REQUESTS || d < 1 || d > 512 || nkv < 1 || nh % nkv || page_size < 1 || (window > 0 && !depth)) return (int)cudaErrorInvalidValue;
     const TreeArgs A{out, q, k_new, v_new, k_cache, v_cache, context, token_start, ancestors, depth, block_table, out_stride, q_stride, k_stride, v_stride,
                      tokens, requests, words, table_stride, nh, nkv, d, page_size, num_pages, window, scale, err};
+    if (dtype == XB_BF16 && scratch && ((uintptr_t)scratch & 15) == 0 && tree_tc_takes(A)) return tree_tc_launch(A, scratch, stream);
     return dtype == XB_F32 ? launch<float>(A, stream) : launch<__nv_bfloat16>(A, stream);
+}
+
+// float32 numbers of scratch for a step of `tokens` drafted tokens (0: none is used)
+XB_EXPORT long long xb_tree_attention_scratch(int dtype, int tokens, int nh, int nkv, int d) {
+    if (dtype != XB_BF16 || tokens <= 0 || nkv <= 0 || nh < nkv) return 0;
+    return line_floats(tokens, nh, nkv, d);
 }

@@ -5,6 +5,7 @@ CPU or through a library: a missing extension or a CPU tensor is an error.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional
 
@@ -1758,6 +1759,9 @@ def stream_mix(out, x, read, weight, eps, err, *, branch=None, mix=None, write=N
 
 
 # ---- a step that verifies trees of drafted tokens ----------------------------------------------------------------------------
+TREE_REQUESTS_MAX = SLOT_REQUESTS_MAX = 8192
+
+
 def _token_rows(t, name: str, dtype, tokens: int, heads: int, d: int) -> int:
     """Elements between the tokens of ``[tokens, heads, d]`` whose heads are dense; tokens may lie further apart."""
     try:
@@ -1774,9 +1778,10 @@ def _token_rows(t, name: str, dtype, tokens: int, heads: int, d: int) -> int:
                       f"with strides {t.stride()} on {t.device}")
 
 
+@functools.lru_cache(maxsize=4096)
 def tree_attention_scratch(tokens: int, nh: int, nkv: int, d: int, dtype) -> int:
     """float32 numbers of scratch that ``tree_attention`` takes for that many drafted tokens; 0: none."""
-    return 0
+    return int(kernels_lib().xb_tree_attention_scratch(dtype_code(dtype), int(tokens), int(nh), int(nkv), int(d)))
 
 
 def tree_attention(out, q, k_new, v_new, k_cache, v_cache, context, token_start, ancestors, block_table, scale, err, *, scratch=None,
@@ -1804,6 +1809,8 @@ def tree_attention(out, q, k_new, v_new, k_cache, v_cache, context, token_start,
     _need(v_cache, "v_cache", dtype, (pages, nkv, page_size, d))
     _need(context, "context", torch.int32)
     requests = context.numel()
+    if requests > TREE_REQUESTS_MAX:
+        raise KernelError(f"{requests} requests; a call takes {TREE_REQUESTS_MAX}")
     _need(token_start, "token_start", torch.int32, (requests + 1,))
     _need(block_table, "block_table", torch.int32, (requests, None))
     _need(ancestors, "ancestors", torch.int32, (T, None))
@@ -1822,7 +1829,7 @@ def tree_attention(out, q, k_new, v_new, k_cache, v_cache, context, token_start,
     _ok(kernels_lib().xb_tree_attention(
         code, out.data_ptr(), q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), context.data_ptr(),
         token_start.data_ptr(), ancestors.data_ptr(), _ptr(depth), block_table.data_ptr(), so, sq, sk, sv, T, requests, ancestors.shape[1],
-        block_table.shape[1], nh, nkv, d, page_size, pages, int(window or 0), float(scale), err.data_ptr(), _stream()), "tree_attention")
+        block_table.shape[1], nh, nkv, d, page_size, pages, int(window or 0), float(scale), _ptr(scratch), err.data_ptr(), _stream()), "tree_attention")
 
 
 def _logit_rows(t, name: str, shape) -> int:
@@ -1904,9 +1911,6 @@ def tree_accept(accepted, path, next_tokens, drafted, targets, parents, token_st
         raise KernelError("a path needs room for its root")
     _ok(kernels_lib().xb_tree_accept(accepted.data_ptr(), path.data_ptr(), next_tokens.data_ptr(), drafted.data_ptr(), targets.data_ptr(),
                                      parents.data_ptr(), token_start.data_ptr(), B, T, path.shape[1], _stream()), "tree_accept")
-
-
-SLOT_REQUESTS_MAX = 8192
 
 
 def cache_slots(slots, positions, request_of, token_start, lengths_out, ring_out, block_table, free_ring, ring, lengths, new_tokens,

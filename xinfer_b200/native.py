@@ -177,7 +177,8 @@ def _declare_kernels(lib):
     _sig(lib, "xb_expert_router", I, [I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, F, P])
     _sig(lib, "xb_attn_decode_tc", I,
          [P, P, P, P, P, P, P, P, I, I, I, I, I, I, L, I, I, I, F, F, F, P, F, I, I, I, I, P, I, P, P])
-    _sig(lib, "xb_tree_attention", I, [I, P, P, P, P, P, P, P, P, P, P, P, L, L, L, L, I, I, I, I, I, I, I, I, I, I, F, P, P])
+    _sig(lib, "xb_tree_attention", I, [I, P, P, P, P, P, P, P, P, P, P, P, L, L, L, L, I, I, I, I, I, I, I, I, I, I, F, P, P, P])
+    _sig(lib, "xb_tree_attention_scratch", L, [I, I, I, I, I])
     _sig(lib, "xb_logit_rules", I, [P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, L, L, L, L, I, I, I, I, I, I, P])
     _sig(lib, "xb_tree_accept", I, [P, P, P, P, P, P, P, I, I, I, P])
     _sig(lib, "xb_cache_slots", I, [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P, P])
