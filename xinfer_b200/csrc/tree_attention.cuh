@@ -47,23 +47,30 @@ __device__ __forceinline__ int request_of(const TreeArgs& A, int t) {
 
 // ---- the line of all jobs' tiles -------------------------------------------------------------------------------------------
 // A job is (request, key/value head, up to job_nodes nodes); its tiles of KT keys are the cached ones from the first that a node sees
-// and the drafted ones.  The line holds all jobs' tiles, request by request; block c takes the units c * share .. (c + 1) * share - 1.
+// and the drafted ones.  The line holds all jobs' tiles, request by request, each as long as it costs: block c takes the tiles that begin
+// in c * share .. (c + 1) * share - 1.
 constexpr int KT = 64;
 constexpr int LINE_BLOCKS = 148;   // a block per SM
 constexpr int LINE_REQUESTS = 8192;
 constexpr int MIN_SHARE = 4;       // tiles that a block takes at least: below that its start and the join cost more than they save
+constexpr int TILE_ROWS = 128;     // rows (node, query head of the group) of a product; a job has up to two such tiles
+constexpr int COST_ONE = 2;        // what a tile of keys costs a job of one tile of rows, and of two: 1,400 and 2,150 cycles measured
+constexpr int COST_TWO = 3;
 
 struct Line {
     int half_nodes, job_nodes;     // nodes of a tile of rows and of a job
-    int blocks, part_rows;         // rows of a part that is kept for the join
-    float* part_o;                 // [blocks][2][part_rows][d]: a block's first segment, if its job began before it, and its last, if its job goes on
+    int part_rows;                 // rows of a part that is kept for the join: a multiple of 8
+    float* part_o;                 // [blocks][2][part_rows / 8][d / 4][8][4]: a block's first segment, if its job began before it, and its last,
+                                   // if its job goes on; four channels of eight rows lie together, as a warp writes and reads them
     float* part_ml;                // [blocks][2][part_rows][2]: maximum and sum
-    int* starts;                   // [requests + 1]: units before each request, then the share
+    int* shared_jobs;              // [blocks][8]: the job that begins in the block and goes on in others
     float* dense;                  // room for q, k_new and v_new as dense rows of bfloat16
 };
 
 struct RequestLine {
-    int first, nodes, context, tile0, old_tiles, tiles, jobs;
+    int first, nodes, context, tile0, old_tiles, tiles, pieces;
+    int per_tile;                  // what a tile costs each of its jobs
+    __device__ __forceinline__ int units(int nkv) const { return nkv * pieces * tiles * per_tile; }
 };
 
 __device__ __forceinline__ RequestLine request_line(const TreeArgs& A, const Line& line, int b) {
@@ -74,78 +81,111 @@ __device__ __forceinline__ RequestLine request_line(const TreeArgs& A, const Lin
     r.tile0 = A.window > 0 ? max(0, r.context - A.window + 1) / KT : 0;    // (the root's window begins first)
     r.old_tiles = max(0, (r.context + KT - 1) / KT - r.tile0);
     r.tiles = r.old_tiles + (r.nodes + KT - 1) / KT;
-    r.jobs = A.nkv * ((r.nodes + line.job_nodes - 1) / line.job_nodes);
+    r.pieces = (r.nodes + line.job_nodes - 1) / line.job_nodes;
+    r.per_tile = r.nodes > line.half_nodes ? COST_TWO : COST_ONE;
     return r;
 }
 
-__device__ __forceinline__ size_t part_row(const Line& line, int block, int which, int row) { return ((size_t)block * 2 + which) * line.part_rows + row; }
-
-struct LineShared {
-    int of_warps[32];
-    int request, before;
-};
-struct LinePlace {
-    int request, before, unit, end;    // the request of the block's first unit, the units before it, the block's units
+// Where a block stands in the line; walked by one warp, whose lanes hold the same values.
+struct Walk {
+    RequestLine r;                 // of request b
+    int b, g, piece;               // the job: request, key/value head, which of their pieces
+    int job, from, end, share;     // where the job begins in the line, the block's range, a block's share
+    int i0, i1;                    // the block's tiles of the job's
 };
 
-// Where this block begins; every thread of the block takes part.  Block 0 writes line.starts.
-__device__ __forceinline__ LinePlace place_in_line(const TreeArgs& A, const Line& line, LineShared& sh) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int each = (A.requests + blockDim.x - 1) / blockDim.x, b0 = (int)threadIdx.x * each, b1 = min(b0 + each, A.requests);
-    auto units = [&](int b) {
-        const RequestLine r = request_line(A, line, b);
-        return r.jobs * r.tiles;
-    };
+// (x > 0) / cost, upwards
+__device__ __forceinline__ int tiles_of_cost(int x, int cost) { return cost == COST_TWO ? (x + COST_TWO - 1) / COST_TWO : (x + COST_ONE - 1) / COST_ONE; }
+
+// The block's place before its first job: every lane sums a run of the requests.
+__device__ __forceinline__ Walk place_in_line(const TreeArgs& A, const Line& line) {
+    const int lane = threadIdx.x & 31, each = (A.requests + 31) / 32, b0 = lane * each, b1 = min(b0 + each, A.requests);
+    Walk w;
     int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += units(b);
+#pragma unroll 1
+    for (int b = b0; b < b1; ++b) {
+        w.r = request_line(A, line, b);
+        mine += w.r.units(A.nkv);
+    }
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += v;
     }
-    if (lane == 31) sh.of_warps[warp] = incl;
-    __syncthreads();
-    int before = incl - mine, total = 0;
-    for (int w = 0; w < warps; ++w) {
-        if (w < warp) before += sh.of_warps[w];
-        total += sh.of_warps[w];
-    }
-    const int share = max(MIN_SHARE, (total + line.blocks - 1) / line.blocks), unit = min((long long)blockIdx.x * share, (long long)total);
-    for (int b = b0; b < b1; ++b) {
-        const int n = units(b);
-        if (unit >= before && unit < before + n) {
-            sh.request = b;
-            sh.before = before;
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    w.share = max(MIN_SHARE * COST_TWO, (total + LINE_BLOCKS - 1) / LINE_BLOCKS);
+    w.from = (int)min((long long)blockIdx.x * w.share, (long long)total);
+    w.end = min(total, w.from + w.share);
+    w.job = w.end;
+    w.b = w.g = w.piece = w.i0 = w.i1 = 0;
+    if (w.from >= w.end) return w;
+    int before = incl - mine, b = b0;
+    const unsigned who = __ballot_sync(0xffffffffu, w.from >= before && w.from < incl);
+    const int owner = __ffs(who) - 1;
+    if (lane == owner) {
+#pragma unroll 1
+        for (; b < b1; ++b) {
+            if (each > 1) w.r = request_line(A, line, b);
+            const int n = w.r.units(A.nkv);
+            if (w.from < before + n) break;
+            before += n;
         }
-        if (blockIdx.x == 0) line.starts[b] = before;
-        before += n;
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) line.starts[A.requests] = share;
-    __syncthreads();
-    return LinePlace{sh.request, sh.before, unit, min(total, unit + share)};
+    w.b = __shfl_sync(0xffffffffu, b, owner);
+    before = __shfl_sync(0xffffffffu, before, owner);
+    w.r = request_line(A, line, w.b);
+    const int length = w.r.tiles * w.r.per_tile, at = (w.from - before) / length;
+    w.g = at / w.r.pieces;
+    w.piece = at % w.r.pieces;
+    w.job = before + at * length;
+    return w;
 }
 
-// host: the scratch in float32 numbers, and its layout
-constexpr int TILE_ROWS = 128;
+// The next job of which the block has a part; false: there is none.  (The first tile that begins at or behind `from` may be the next
+// job's, or the next request's first.)
+__device__ __forceinline__ bool next_segment(const TreeArgs& A, const Line& line, Walk& w, bool first) {
+    for (;; first = false) {
+        if (!first) w.job += w.r.tiles * w.r.per_tile;
+        if (w.job >= w.end) return false;
+        if (!first && ++w.piece == w.r.pieces) {
+            w.piece = 0;
+            if (++w.g == A.nkv) {
+                w.g = 0;
+                do {
+                    if (++w.b >= A.requests) return false;
+                    w.r = request_line(A, line, w.b);
+                } while (w.r.nodes == 0);                          // (a request without nodes has no jobs)
+            }
+        }
+        w.i0 = w.from > w.job ? tiles_of_cost(w.from - w.job, w.r.per_tile) : 0;
+        w.i1 = min(w.r.tiles, tiles_of_cost(w.end - w.job, w.r.per_tile));
+        if (w.i0 < w.i1) return true;
+    }
+}
+
+__device__ __forceinline__ size_t part_row(const Line& line, int block, int which, int row) { return ((size_t)block * 2 + which) * line.part_rows + row; }
+// where four channels of a part's row lie, in float4
+__device__ __forceinline__ size_t part_four(const Line& line, int d, size_t row, int c4) { return ((row >> 3) * (d >> 2) + c4) * 8 + (row & 7); }
+
+// host: the scratch in float32 numbers, and its layout (every part is a multiple of 4 numbers long)
 inline int line_part_rows(int tokens, int group) {
     const int nodes = 2 * (TILE_ROWS / (group < TILE_ROWS ? group : TILE_ROWS));
-    return (tokens < nodes ? tokens : nodes) * group;
+    return ((tokens < nodes ? tokens : nodes) * group + 7) / 8 * 8;
 }
 inline long long line_floats(int tokens, int nh, int nkv, int d) {
-    return (long long)LINE_BLOCKS * 2 * line_part_rows(tokens, nh / nkv) * (d + 2) + LINE_REQUESTS + 4 + ((long long)tokens * (nh + 2 * nkv) * d + 1) / 2;
+    return (long long)LINE_BLOCKS * (2 * line_part_rows(tokens, nh / nkv) * (long long)(d + 2) + 8) + ((long long)tokens * (nh + 2 * nkv) * d + 1) / 2;
 }
 inline Line make_line(const TreeArgs& A, float* scratch) {
     const int G = A.nh / A.nkv;
     Line line;
     line.half_nodes = TILE_ROWS / G;
     line.job_nodes = 2 * line.half_nodes;
-    line.blocks = LINE_BLOCKS;
     line.part_rows = line_part_rows(A.tokens, G);
     line.part_o = scratch;
-    line.part_ml = scratch + (size_t)line.blocks * 2 * line.part_rows * A.d;
-    line.starts = reinterpret_cast<int*>(line.part_ml + (size_t)line.blocks * 2 * line.part_rows * 2);
-    line.dense = reinterpret_cast<float*>(line.starts) + LINE_REQUESTS + 4;      // (every part before it is a multiple of 4 numbers long)
+    line.part_ml = scratch + (size_t)LINE_BLOCKS * 2 * line.part_rows * A.d;
+    line.shared_jobs = reinterpret_cast<int*>(line.part_ml + (size_t)LINE_BLOCKS * 2 * line.part_rows * 2);
+    line.dense = reinterpret_cast<float*>(line.shared_jobs) + LINE_BLOCKS * 8;
     return line;
 }
 

@@ -20,6 +20,8 @@
 #include "tc_common.cuh"
 #include "tree_attention.cuh"
 
+#include <type_traits>
+
 namespace {
 
 using namespace xbtc;
@@ -28,45 +30,7 @@ using namespace xbtree;
 constexpr int RT = TILE_ROWS;              // rows of a tile
 constexpr float RESCALE_STEP = 8.f;        // a row's maximum moves only when it grows by more than 2^8
 constexpr int THREADS = 384;
-__host__ __device__ constexpr int stages(int dp) { return dp <= 64 ? 8 : 5; }
-
-// A block's part of a job.
-struct Segment {
-    int b, g, node0, t0;           // request, key/value head, first node of the job and its row
-    int nodes;                     // of the job (both tiles)
-    int tree0, tree_n, context;    // the request's first node's row, its nodes, its cached keys
-    int tile0, old_tiles;          // the first cached tile, cached tiles from there on
-    int i0, i1, tiles;             // this segment's tiles of the job's
-};
-
-struct Walk {                      // where a role stands in the line
-    int b, before, unit, end;      // request, units before it, the next unit, the block's end
-};
-
-__device__ __forceinline__ bool next_segment(const TreeArgs& A, const Line& line, Walk& w, Segment& s) {
-    if (w.unit >= w.end) return false;
-    RequestLine r = request_line(A, line, w.b);
-    while (w.unit >= w.before + r.jobs * r.tiles) {       // (requests without work have no units)
-        w.before += r.jobs * r.tiles;
-        r = request_line(A, line, ++w.b);
-    }
-    const int job = (w.unit - w.before) / r.tiles, pieces = r.jobs / A.nkv;
-    s.b = w.b;
-    s.g = job / pieces;
-    s.tree0 = r.first;
-    s.tree_n = r.nodes;
-    s.context = r.context;
-    s.node0 = job % pieces * line.job_nodes;
-    s.t0 = r.first + s.node0;
-    s.nodes = min(line.job_nodes, r.nodes - s.node0);
-    s.tile0 = r.tile0;
-    s.old_tiles = r.old_tiles;
-    s.tiles = r.tiles;
-    s.i0 = w.unit - w.before - job * r.tiles;
-    s.i1 = min(r.tiles, s.i0 + w.end - w.unit);
-    w.unit += s.i1 - s.i0;
-    return true;
-}
+__host__ __device__ constexpr int stages(int dp) { return dp <= 64 ? 8 : 4; }
 
 __device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
     uint32_t r;
@@ -93,6 +57,29 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     return d;
 }
 
+// Bounded waits, with the way that is taken when the barrier is not yet there outside the loops' code.
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int* err) { return mbar_wait(bar, parity, err); }
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int* err) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok ? true : wait_long(bar, parity, err);
+}
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* err) { return __all_sync(0xffffffffu, wait(bar, parity, err)); }
+
+// A block's part of a job, as the warp that walks the line tells it the others: a ring of these lies in shared memory.
+struct __align__(16) Segment {
+    int i0, i1, old_tiles, key0;       // tiles of the job from i0 to i1; cached ones; the first cached key that is walked over
+    int context, tree, first, node0;   // cached keys, the request's nodes and the row of the first, the job's first node
+    int nodes, g, b, parts;            // the job's nodes (0: there is no segment any more), key/value head, request, blocks that share the job from here on
+    int deep_lo, whole, pad0, pad1;    // where the deepest node's window begins (0: none); whether this is all of the job
+};
+constexpr int SEGMENTS = 8;
+constexpr int READERS = 11;            // warps that read a segment
+
 template <int DP>
 __global__ void __launch_bounds__(THREADS)
 tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -100,48 +87,70 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                          int ps_shift, float scale_log2) {
     constexpr int HALVES = DP / 64, NS = stages(DP);
     constexpr uint32_t Q_ONE = HALVES * RT * 128, Q_BYTES = 2 * Q_ONE, KV_HALF = KT * 128, KV_BYTES = HALVES * KV_HALF, STAGE_BYTES = 2 * KV_BYTES;
-    constexpr uint32_t BAR_OFF = Q_BYTES + NS * STAGE_BYTES, RING = 8 * NS;
+    constexpr uint32_t BAR_OFF = Q_BYTES + NS * STAGE_BYTES, RING = 8 * NS, OUT_OFF = BAR_OFF + 1024, STATS_OFF = OUT_OFF + 8 * 2048;
+    constexpr uint32_t SEG_OFF = STATS_OFF + 2048;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t base = smem_u32(smem_raw), q_sm = base, kv_sm = base + Q_BYTES, bars = base + BAR_OFF;
     const uint32_t k_full0 = bars, k_empty0 = bars + RING, v_full0 = bars + 2 * RING, v_empty0 = bars + 3 * RING, rest = bars + 4 * RING;
-    const uint32_t s_ready0 = rest, pv_done0 = rest + 32, p_ready0 = rest + 64, q_full = rest + 80, q_empty = rest + 96, looked0 = rest + 104;
-    volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(smem_raw + BAR_OFF + 4 * RING + 120);   // tmem, dead, then the value rows that are
-    volatile uint32_t* odd_rows = words + 2;                                                                // not finite: [4 looks][2 words]
-    LineShared& line_sh = *reinterpret_cast<LineShared*>(smem_raw + BAR_OFF + 512);
+    const uint32_t s_ready0 = rest, pv_done0 = rest + 32, p_ready0 = rest + 64, q_full = rest + 96, q_empty = rest + 104, looked0 = rest + 112,
+                   told = rest + 144, joined = rest + 152, seg_full0 = rest + 160, seg_empty0 = seg_full0 + 8 * SEGMENTS;
+    volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(smem_raw + BAR_OFF + 4 * RING + 160 + 16 * SEGMENTS);   // tmem, -, then the value rows
+    volatile uint32_t* odd_rows = words + 2;                                                                                // that are not finite: [4][2]
+    Segment* const segments = reinterpret_cast<Segment*>(smem_raw + SEG_OFF);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int G = A.nh / A.nkv, half_nodes = line.half_nodes;
+    int* const err = A.err;
 
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < 4 * NS; ++i) mbar_init(bars + 8 * i, 1);
-        for (int i = 0; i < 4; ++i) mbar_init(s_ready0 + 8 * i, 1), mbar_init(pv_done0 + 8 * i, 1);
-        mbar_init(p_ready0, 128);
-        mbar_init(p_ready0 + 8, 128);
-        mbar_init(q_full, 1);
-        mbar_init(q_empty, 1);
-        mbar_init(looked0, 2);
-        mbar_init(looked0 + 8, 2);
-        mbar_init_fence();
+    Walk w;
+    if (warp == 8) {
+        pdl_wait();                // lengths, rows and masks may come from the kernel before
+        w = place_in_line(A, line);
+    } else {
+        if (threadIdx.x == 9 * 32) {
+            for (int i = 0; i < 4 * NS; ++i) mbar_init(bars + 8 * i, 1);
+            for (int i = 0; i < 4; ++i) {
+                mbar_init(s_ready0 + 8 * i, 1);
+                mbar_init(pv_done0 + 8 * i, 1);
+                mbar_init(p_ready0 + 8 * i, 4);        // a warp each
+                mbar_init(looked0 + 8 * i, 2);
+            }
+            mbar_init(q_full, 1);
+            mbar_init(q_empty, 1);
+            mbar_init(told, 8);
+            mbar_init(joined, 8);
+            for (int i = 0; i < SEGMENTS; ++i) mbar_init(seg_full0 + 8 * i, 1), mbar_init(seg_empty0 + 8 * i, READERS);
+            mbar_init_fence();
+        }
+        if (warp == 10) tmem_alloc(const_cast<uint32_t*>(&words[0]), 512);
+        pdl_wait();
     }
-    constexpr uint32_t TMEM_COLS = 512;
-    if (warp == 0) tmem_alloc(const_cast<uint32_t*>(&words[0]), TMEM_COLS);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = words[0];
     pdl_launch_dependents();       // only now: see pdl_launch_dependents on tensor memory
-    pdl_wait();                    // lengths, rows and masks may come from the kernel before
-    if (threadIdx.x == 0) {
-        if (base & 1023u) atomicOr(A.err, XB_ERR_WAIT);                                        // the swizzle needs a 1024-byte aligned window
-        words[1] = (*reinterpret_cast<volatile int*>(A.err) & XB_ERR_WAIT) ? 1u : 0u;          // or an earlier block gave up: do not pile on
-    }
-    const LinePlace at = place_in_line(A, line, line_sh);
-    const Walk start{at.request, at.before, at.unit, words[1] ? at.unit : at.end};
-    const bool out16 = rows_on_16_bytes(A.out, A.out_stride);
-    const int G = A.nh / A.nkv, half_nodes = line.half_nodes;
-    const int box_rows = min(A.page_size, KT);
-    int* err = A.err;
 
+    int seg = 0;                   // segments so far
+    // The next segment from the ring; nodes == 0: there is none, or a wait gave up.
+    auto read_segment = [&]() -> Segment {
+        Segment s;
+        s.nodes = 0;
+        const int at = seg % SEGMENTS;
+        if (wait_warp(seg_full0 + 8 * at, (seg / SEGMENTS) & 1, err)) {
+            const int4* from = reinterpret_cast<const int4*>(segments + at);
+            int4* to = reinterpret_cast<int4*>(&s);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[i] = from[i];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(seg_empty0 + 8 * at);
+        }
+        ++seg;
+        return s;
+    };
+
+    const int box_rows = min(A.page_size, KT);
     if (warp == 8 || warp == 10) {
-        // ---- keys (warp 8) and values (warp 10), a lane per box ----------------------------------------------------------
+        // ---- keys (warp 8, which also walks the line) and values (warp 10), a lane per box --------------------------------------
         const bool is_v = warp == 10;
         const uint32_t full0 = is_v ? v_full0 : k_full0, empty0 = is_v ? v_empty0 : k_empty0;
         const CUtensorMap* map = is_v ? &map_v : &map_k;
@@ -150,13 +159,64 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         int st = 0;
         uint32_t ph = 0;
         bool rounds = false, ok = true;
-        Walk w = start;
-        Segment s;
-        while (ok && next_segment(A, line, w, s)) {
+        if (!is_v) {
+            if (base & 1023u) atomicOr(err, XB_ERR_WAIT);                                  // the swizzle needs a 1024-byte aligned window
+            if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(err) & XB_ERR_WAIT)) w.job = w.end;   // or an earlier block gave up: do not pile on
+        }
+        bool first = true, goes_on = false;
+        while (ok) {
+            Segment s;
+            if (is_v) {
+                s = read_segment();
+                if (!s.nodes) break;
+            } else {
+                const bool more = next_segment(A, line, w, first);
+                first = false;
+                if (more) {
+                    const RequestLine& r = w.r;
+                    s.i0 = w.i0;
+                    s.i1 = w.i1;
+                    s.old_tiles = r.old_tiles;
+                    s.key0 = r.tile0 * KT;
+                    s.context = r.context;
+                    s.tree = r.nodes;
+                    s.first = r.first;
+                    s.node0 = w.piece * line.job_nodes;
+                    s.nodes = min(line.job_nodes, r.nodes - s.node0);
+                    s.g = w.g;
+                    s.b = w.b;
+                    s.whole = w.i1 - w.i0 == r.tiles;
+                    s.parts = w.i0 == 0 && !s.whole ? (w.job + (r.tiles - 1) * r.per_tile) / w.share - (int)blockIdx.x + 1 : 0;
+                    s.deep_lo = 0;
+                    if (A.window > 0) {
+                        int deepest = 0;
+                        for (int i = lane; i < r.nodes; i += 32) deepest = max(deepest, A.depth[r.first + i]);
+                        s.deep_lo = r.context + __reduce_max_sync(0xffffffffu, deepest) - A.window + 1;
+                    }
+                    if (s.parts && lane == 0) *reinterpret_cast<int4*>(line.shared_jobs + blockIdx.x * 8) = make_int4(s.parts, s.first + s.node0, s.nodes, s.g);
+                    goes_on |= s.parts > 0;
+                } else {
+                    s.nodes = 0;
+                    if (!goes_on && lane == 0) line.shared_jobs[blockIdx.x * 8] = 0;
+                }
+                const int at = seg % SEGMENTS;
+                if (seg >= SEGMENTS) ok = wait_warp(seg_empty0 + 8 * at, ((seg / SEGMENTS) - 1) & 1, err);
+                if (!ok) break;
+                if (lane == 0) {
+                    int4* to = reinterpret_cast<int4*>(segments + at);
+                    const int4* from = reinterpret_cast<const int4*>(&s);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) to[i] = from[i];
+                    mbar_arrive(seg_full0 + 8 * at);
+                }
+                __syncwarp();
+                ++seg;
+                if (!more) break;
+            }
             const int* table = A.block_table + (size_t)s.b * A.table_stride;
             auto page_of = [&](int it) -> int {            // the page of this lane's box, -1: nothing to load
                 if (it >= s.i1 || it >= s.old_tiles || lane >= boxes) return -1;
-                const int j = (s.tile0 + it) * KT + bi * box_rows;
+                const int j = s.key0 + it * KT + bi * box_rows;
                 if (j >= s.context) return -1;
                 const int page = table[j >> ps_shift];
                 if (page < 0 || page >= A.num_pages) {
@@ -168,8 +228,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             int page_next = page_of(s.i0);
             for (int it = s.i0; it < s.i1; ++it) {
                 const int page = page_next;
-                if (rounds && !__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * st, ph ^ 1u, err))) {
-                    words[1] = 1;
+                if (rounds && !wait_warp(empty0 + 8 * st, ph ^ 1u, err)) {
                     ok = false;
                     break;
                 }
@@ -179,13 +238,13 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     if (lane == 0) mbar_expect_tx(full0 + 8 * st, nb * box_rows * 128);
                     __syncwarp();
                     if (page >= 0) {
-                        const int j = (s.tile0 + it) * KT + bi * box_rows;
-                        tma_load_2d(dst0 + hf * KV_HALF + bi * box_rows * 128, map, hf * 64, (page * A.nkv + s.g) * A.page_size + (j & (A.page_size - 1)), full0 + 8 * st);
+                        const int j = it * KT + bi * box_rows;             // (key0 is a multiple of the tile, so of the smaller pages too)
+                        tma_load_2d(dst0 + hf * KV_HALF + bi * box_rows * 128, map, hf * 64, (page * A.nkv + s.g) * A.page_size + ((s.key0 + j) & (A.page_size - 1)), full0 + 8 * st);
                     }
                 } else {
                     if (lane == 0) mbar_expect_tx(full0 + 8 * st, KV_BYTES);
                     __syncwarp();
-                    if (lane < HALVES) tma_load_3d(dst0 + lane * KV_HALF, map_new, lane * 64, s.g, s.tree0 + (it - s.old_tiles) * KT, full0 + 8 * st);
+                    if (lane < HALVES) tma_load_3d(dst0 + lane * KV_HALF, map_new, lane * 64, s.g, s.first + (it - s.old_tiles) * KT, full0 + 8 * st);
                 }
                 page_next = page_of(it + 1);
                 if (++st == NS) {
@@ -200,17 +259,17 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const bool leader = lane == 0;
         const uint32_t idesc_s = umma_idesc(KT, 0);
         const uint64_t dq0 = umma_desc(q_sm, 16, 1024), dk0 = umma_desc(kv_sm, 16, 1024);
-        int st = 0, Th[2] = {0, 0}, I = 0;       // ring stage, tiles of either row tile so far, segments so far
+        int st = 0, Th[2] = {0, 0};              // ring stage, tiles of either half so far
         uint32_t ph = 0;
         bool ok = true;
-        Walk w = start;
-        Segment s;
-        while (ok && next_segment(A, line, w, s)) {
-            const int halves = s.nodes > half_nodes ? 2 : 1;
+        while (ok) {
+            const Segment s = read_segment();
+            if (!s.nodes) break;
+            const int halves = s.nodes > half_nodes ? 2 : 1, I = seg - 1;
             if (I > 0) {                         // Q lies where the last one lay: once every product that reads that has completed
                 if (leader) umma_commit(q_empty);
                 __syncwarp();
-                ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (uint32_t)(I - 1) & 1u, err, true));
+                ok = wait_warp(q_empty, (uint32_t)(I - 1) & 1u, err);
                 if (!ok) break;
             }
             if (leader) {
@@ -218,23 +277,22 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 for (int hd = 0; hd < halves; ++hd)
 #pragma unroll
                     for (int hf = 0; hf < HALVES; ++hf)
-                        tma_load_3d(q_sm + hd * Q_ONE + hf * RT * 128, &map_q, hf * 64, s.g * G, s.t0 + hd * half_nodes, q_full);
+                        tma_load_3d(q_sm + hd * Q_ONE + hf * RT * 128, &map_q, hf * 64, s.g * G, s.first + s.node0 + hd * half_nodes, q_full);
             }
             __syncwarp();
-            ok = __all_sync(0xffffffffu, mbar_wait(q_full, (uint32_t)I & 1u, err, true));
-            ++I;
+            ok = wait_warp(q_full, (uint32_t)I & 1u, err);
             for (int it = s.i0; it < s.i1 && ok; ++it) {
-                ok = __all_sync(0xffffffffu, mbar_wait(k_full0 + 8 * st, ph, err, true));
+                ok = wait_warp(k_full0 + 8 * st, ph, err);
                 const uint64_t dk = dk0 + (uint64_t)((st * STAGE_BYTES) >> 4);
 #pragma unroll
                 for (int hd = 0; hd < 2; ++hd) {
-                    if (hd >= halves) break;
+                    if (halves == 1 && ((it - s.i0) & 1) != hd) continue;
                     const int th = Th[hd]++, sb = th & 1;
-                    // these columns held the scores and then P of this row tile's last tile but one: its P V must have read them
-                    ok = ok && (th < 2 || __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * (2 * hd + sb), ((th >> 1) - 1) & 1, err, true)));
+                    // these columns held the scores and then P of this half's last tile but one: its P V must have read them
+                    ok = ok && (th < 2 || wait_warp(pv_done0 + 8 * (2 * hd + sb), ((th >> 1) - 1) & 1, err));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t dq = dq0 + (uint64_t)((hd * Q_ONE) >> 4);
+                    const uint64_t dq = dq0 + (uint64_t)((halves == 1 ? 0u : hd * Q_ONE) >> 4);
                     if (leader) {
 #pragma unroll
                         for (int kk = 0; kk < DP / 16; ++kk) {
@@ -255,7 +313,6 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
             }
         }
-        if (!ok) words[1] = 1;
     } else if (warp == 11) {
         // ---- O += P V of every tile (O starts as zeros, by the softmax threads) -----------------------------------------------
         const bool leader = lane == 0;
@@ -264,18 +321,18 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         int st = 0, Th[2] = {0, 0};
         uint32_t ph = 0;
         bool ok = true;
-        Walk w = start;
-        Segment s;
-        while (ok && next_segment(A, line, w, s)) {
+        while (ok) {
+            const Segment s = read_segment();
+            if (!s.nodes) break;
             const int halves = s.nodes > half_nodes ? 2 : 1;
             for (int it = s.i0; it < s.i1 && ok; ++it) {
-                ok = __all_sync(0xffffffffu, mbar_wait(v_full0 + 8 * st, ph, err, true));
+                ok = wait_warp(v_full0 + 8 * st, ph, err);
                 const uint64_t dv = dv0 + (uint64_t)((st * STAGE_BYTES) >> 4);
 #pragma unroll
                 for (int hd = 0; hd < 2; ++hd) {
-                    if (hd >= halves) break;
+                    if (halves == 1 && ((it - s.i0) & 1) != hd) continue;
                     const int th = Th[hd]++, sb = th & 1;
-                    ok = ok && __all_sync(0xffffffffu, mbar_wait(p_ready0 + 8 * hd, th & 1, err, true));
+                    ok = ok && wait_warp(p_ready0 + 8 * (2 * hd + sb), (th >> 1) & 1, err);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t tp = tmem + (uint32_t)(hd * 128 + sb * 64);
@@ -296,72 +353,79 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
             }
         }
-        if (!ok) words[1] = 1;
     } else {
         // ---- softmax: a row per thread ---------------------------------------------------------------------------------------------
         const int hd = warp >> 2, r = (int)threadIdx.x & 127;
         const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t tmem_s = tmem + (uint32_t)(hd * 128), tmem_o = tmem + (uint32_t)(256 + hd * 128);
-        const uint32_t my_s_ready = s_ready0 + 16 * hd, my_p_ready = p_ready0 + 8 * hd, my_pv_done = pv_done0 + 16 * hd;
+        const uint32_t tmem_s = tmem + (uint32_t)(hd * 128) + lane_addr, tmem_o = tmem + (uint32_t)(256 + hd * 128) + lane_addr;
+        const uint32_t my_s_ready = s_ready0 + 16 * hd, my_p_ready = p_ready0 + 16 * hd, my_pv_done = pv_done0 + 16 * hd;
         const int node_r = r / G, head_r = r % G;
-        const bool warp_rows = (warp & 3) * 32 < half_nodes * G;
-        int T = 0, Th = 0, looks = 0;            // tiles of all segments so far, of this row tile's, tiles that were looked at
+        const int window = A.window;
+        const bool out16 = rows_on_16_bytes(A.out, A.out_stride);
+        // the rows whose results this thread stores, one of every eight of the warp's: their nodes, and where they lie from the job's first on
+        int st_node[4];
+        long long st_at[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int in_half = (warp & 3) * 32 + k * 8 + (lane >> 2);
+            st_node[k] = in_half / G;
+            st_at[k] = st_node[k] * A.out_stride + (in_half % G) * A.d + (lane & 3) * 8;
+        }
+        int T = 0, Th = 0, looks = 0, joins = 0;   // tiles of all segments so far, of this half's, tiles that were looked at, segments of one tile of rows
         bool alive = true;
-        Walk w = start;
-        Segment s;
-        while (alive && next_segment(A, line, w, s)) {
-            const int window = A.window, iters = s.i1 - s.i0;
-            // whether the tile's keys are not seen alike by all rows (the windows of deeper nodes begin later)
-            int deep_lo = 0;                              // where the deepest node's begins
-            if (window > 0) {
-                int deepest = 0;
-                for (int i = lane; i < s.tree_n; i += 32) deepest = max(deepest, A.depth[s.tree0 + i]);
-                deep_lo = s.context + __reduce_max_sync(0xffffffffu, deepest) - window + 1;
-            }
-            auto mixed = [&](int it) { return it >= s.old_tiles || (window > 0 && (s.tile0 + it) * KT < deep_lo); };
-            if (hd == 1 && s.nodes <= half_nodes) {       // a segment of one row tile: the second one's threads sit it out
-                for (int it = s.i0; it < s.i1; ++it) looks += mixed(it) ? 1 : 0;
-                T += iters;
-                continue;
-            }
-            const int node = s.node0 + hd * half_nodes + node_r;         // in its tree
+        while (alive) {
+            const Segment s = read_segment();
+            if (!s.nodes) break;
+            // one tile of rows: both halves work on it, each on every other tile of keys
+            const bool split = s.nodes <= half_nodes;
+            const int half_first = split ? 0 : hd * half_nodes;
+            const int node = s.node0 + half_first + node_r;              // in its tree
             const bool valid = node_r < half_nodes && node < s.node0 + s.nodes;
-            const bool working = warp_rows && __any_sync(0xffffffffu, valid);
-            const int t = s.tree0 + node, h = s.g * G + head_r;
+            const bool working = __any_sync(0xffffffffu, valid);
+            const int t = s.first + node;
             const int my_depth = valid && window > 0 ? max(0, A.depth[t]) : 0;
             const int my_lo = window > 0 ? max(0, s.context + my_depth - window + 1) : 0;
-            const int* my_words = A.ancestors + (size_t)(valid ? t : s.t0) * A.words;
+            const int* my_words = A.ancestors + (size_t)(valid ? t : s.first) * A.words;
             uint32_t word_lo = 0, word_hi = 0;            // of the first drafted tile
             if (valid && s.i1 > s.old_tiles) {
                 word_lo = A.words > 0 ? (uint32_t)my_words[0] : 0u;
                 word_hi = A.words > 1 ? (uint32_t)my_words[1] : 0u;
             }
-            {
+            if (working) {
                 float zero[32];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) zero[i] = 0.f;
 #pragma unroll
-                for (int c0 = 0; c0 < DP; c0 += 32) tmem_st32(tmem_o + lane_addr + c0, zero);
+                for (int c0 = 0; c0 < DP; c0 += 32) tmem_st32(tmem_o + c0, zero);
+                tmem_st_wait();
             }
             float m_ref = -INFINITY, l = 0.f;
-            for (int it = s.i0; it < s.i1; ++it) {
-                const int n_it = it - s.i0, th = Th + n_it, sb = th & 1, gt = T + n_it, st = gt % NS;
-                const bool drafted = it >= s.old_tiles, look = mixed(it);
-                const int key0 = drafted ? (it - s.old_tiles) * KT : (s.tile0 + it) * KT;
-                const int keys = drafted ? s.tree_n : s.context;          // keys from here on belong to nobody
-                const bool edge = look || key0 + KT > keys;
-                // the value rows: zeroed where nobody may see them, and in tiles that are not seen alike where they are not finite
-                if (hd == 0 && edge && r < KT) {
-                    alive = __all_sync(0xffffffffu, mbar_wait(v_full0 + 8 * st, (gt / NS) & 1, err));   // orders these accesses after the copy
+            // cached tiles before `mixed` begin before the deepest node's window does; those from `full` on go beyond the context
+            const int mixed = s.deep_lo > s.key0 ? min(s.old_tiles, (s.deep_lo - s.key0 + KT - 1) / KT) : 0, full = (s.context - s.key0) / KT;
+            // the looks at tiles that not all rows see alike, up to tile `it`
+            auto looks_at = [&](int it) { return looks + min(it, mixed) - min(s.i0, mixed) + max(it, s.old_tiles) - max(s.i0, s.old_tiles); };
+
+            // One tile; EDGE: not all of its keys are seen by all rows.
+            auto tile = [&](auto edge_c, int it, int th) -> bool {
+                constexpr bool EDGE = decltype(edge_c)::value;
+                const int sb = th & 1;
+                const bool drafted = EDGE && it >= s.old_tiles, look = EDGE && (drafted || it < mixed);
+                const int key0 = !EDGE ? 0 : drafted ? (it - s.old_tiles) * KT : s.key0 + it * KT;
+                const int keys = drafted ? s.tree : s.context;            // keys from here on belong to nobody
+                const int n_look = look ? looks_at(it) : 0;
+                if (EDGE && (split || hd == 0) && r < KT) {
+                    // the value rows: zeroed where nobody may see them, and in tiles that are not seen alike where they are not finite
+                    const int gt = T + it - s.i0, st = gt % NS;
+                    const bool here = wait_warp(v_full0 + 8 * st, (gt / NS) & 1, err);     // orders these accesses after the copy
                     uint4* row = reinterpret_cast<uint4*>(smem_raw + Q_BYTES + st * STAGE_BYTES + KV_BYTES + r * 128);
-                    bool drop = key0 + r >= keys || (!drafted && key0 + r < (window > 0 ? max(0, s.context - window + 1) : 0)), odd = false;
+                    bool drop = key0 + r >= keys || (!drafted && window > 0 && key0 + r < s.context - window + 1), odd = false;
                     if (look && !drop) {
 #pragma unroll
                         for (int hf = 0; hf < HALVES; ++hf)
 #pragma unroll
                             for (int c8 = 0; c8 < 8; ++c8) odd |= bf16_not_finite(row[hf * (KV_HALF / 16) + c8]);
                     }
-                    if (alive && (drop || odd)) {
+                    if (here && (drop || odd)) {
 #pragma unroll
                         for (int hf = 0; hf < HALVES; ++hf)
 #pragma unroll
@@ -371,15 +435,12 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     fence_async_shared();          // the zeroed rows: visible to the product
                     __syncwarp();
                     if (look && lane == 0) {
-                        odd_rows[(looks & 3) * 2 + warp] = odd_mask;
-                        mbar_arrive(looked0 + 8 * (looks & 1));
+                        odd_rows[(n_look & 3) * 2 + (warp & 3)] = odd_mask;
+                        mbar_arrive(looked0 + 8 * (n_look & 3));
                     }
-                    if (!alive) break;
+                    if (!here) return false;
                 }
-                if (!__all_sync(0xffffffffu, mbar_wait(my_s_ready + 8 * sb, (th >> 1) & 1, err))) {
-                    alive = false;
-                    break;
-                }
+                if (!wait_warp(my_s_ready + 8 * sb, (th >> 1) & 1, err)) return false;
                 float corr = 1.f;
                 int moved = 0;
                 unsigned long long seen = ~0ull;
@@ -388,8 +449,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     float sc[64];
                     {
                         uint32_t ra[32], rb[32];
-                        tmem_ld32_nowait(tmem_s + sb * 64 + lane_addr, ra);
-                        tmem_ld32_nowait(tmem_s + sb * 64 + lane_addr + 32, rb);
+                        tmem_ld32_nowait(tmem_s + sb * 64, ra);
+                        tmem_ld32_nowait(tmem_s + sb * 64 + 32, rb);
                         tmem_ld_wait();
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
@@ -397,7 +458,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             sc[32 + i] = __uint_as_float(rb[i]);
                         }
                     }
-                    if (edge) {
+                    if (EDGE) {
                         if (drafted) {
                             const int at = key0 / 32;
                             seen = at == 0 ? ((unsigned long long)word_hi << 32 | word_lo) : 0ull;
@@ -408,7 +469,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             if (keys - key0 < 64) seen &= (1ull << (keys - key0)) - 1;
                             if (window > 0)
                                 for (int i = 0; i < min(64, keys - key0); ++i)
-                                    if (my_depth - max(0, A.depth[s.tree0 + key0 + i]) >= window) seen &= ~(1ull << i);
+                                    if (my_depth - max(0, A.depth[s.first + key0 + i]) >= window) seen &= ~(1ull << i);
                         } else {
                             if (keys - key0 < 64) seen = (1ull << (keys - key0)) - 1;
                             if (my_lo > key0) seen = my_lo - key0 < 64 ? seen & (~0ull << (my_lo - key0)) : 0ull;
@@ -427,8 +488,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     const float mx = max3_nan(mx4[0], mx4[1], max3_nan(mx4[2], mx4[3], mx4[3])) * scale_log2;
                     if (!(mx <= m_ref + RESCALE_STEP)) {                 // (a score that is no number makes the row one)
                         corr = m_ref == -INFINITY ? 0.f : ex2(m_ref - mx);
+                        moved = m_ref != -INFINITY && valid;             // (O is zero before)
                         m_ref = mx;
-                        moved = n_it > 0 && valid;
                     }
                     const float m_neg = m_ref == -INFINITY ? 0.f : -m_ref;
                     const f32x2 scale2 = pack2(scale_log2, scale_log2), mneg2 = pack2(m_neg, m_neg);
@@ -443,7 +504,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         for (int i = 0; i < 8; ++i)
                             if ((i & 3) != 3) e[i] = ex2(x[i]);
                         ex2_poly2(x[3], x[7], e[3], e[7]);
-                        if (edge) {                // the polynomial ends at 2^-126: a key that is not seen has no weight at all
+                        if (EDGE) {                // the polynomial ends at 2^-126: a key that is not seen has no weight at all
                             if (x[3] == -INFINITY) e[3] = 0.f;
                             if (x[7] == -INFINITY) e[7] = 0.f;
                         }
@@ -458,44 +519,38 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     unpack2(sum_a, s0, s1);
                     unpack2(sum_b, s2, s3);
                     l = l * corr + ((s0 + s1) + (s2 + s3));
-                    tmem_st32_u(tmem_s + sb * 64 + lane_addr, pk);       // P goes where the scores were
+                    tmem_st32_u(tmem_s + sb * 64, pk);                   // P goes where the scores were
                 }
-                // O is not touched, and this tile not announced, before the last tile's P V has completed: the issuer waits for
-                // announcements by their parity, so none may be two of them ahead
-                if (n_it > 0 && !__all_sync(0xffffffffu, mbar_wait(my_pv_done + 8 * (sb ^ 1), ((th - 1) >> 1) & 1, err))) {
-                    alive = false;
-                    break;
+                // O is touched only when the last tile's P V has completed
+                if (EDGE || __any_sync(0xffffffffu, moved)) {
+                    if (th > Th && !wait_warp(my_pv_done + 8 * (sb ^ 1), ((th - 1) >> 1) & 1, err)) return false;
                 }
                 if (__any_sync(0xffffffffu, moved)) {
                     tc_fence_after();
                     const float f = moved ? corr : 1.f;
-#pragma unroll
+#pragma unroll 1
                     for (int c0 = 0; c0 < DP; c0 += 32) {
                         float o[32];
-                        tmem_ld32(tmem_o + lane_addr + c0, o);
+                        tmem_ld32(tmem_o + c0, o);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] *= f;
-                        tmem_st32(tmem_o + lane_addr + c0, o);
+                        tmem_st32(tmem_o + c0, o);
                     }
                 }
                 tmem_st_wait();
                 if (look) {
-                    if (!__all_sync(0xffffffffu, mbar_wait(looked0 + 8 * (looks & 1), (looks >> 1) & 1, err))) {
-                        alive = false;
-                        break;
-                    }
-                    const uint32_t odd_lo = odd_rows[(looks & 3) * 2], odd_hi = odd_rows[(looks & 3) * 2 + 1];
-                    ++looks;
+                    if (!wait_warp(looked0 + 8 * (n_look & 3), (n_look >> 2) & 1, err)) return false;
+                    const uint32_t odd_lo = odd_rows[(n_look & 3) * 2], odd_hi = odd_rows[(n_look & 3) * 2 + 1];
                     if ((odd_lo | odd_hi) && working) {    // (rare) the same for all lanes
                         tc_fence_after();
                         for (int i = 0; i < 64; ++i) {
                             if (!((i < 32 ? odd_lo >> i : odd_hi >> (i - 32)) & 1u)) continue;
-                            const uint32_t two = tmem_ld1(tmem_s + sb * 64 + lane_addr + (uint32_t)(i >> 1));
+                            const uint32_t two = tmem_ld1(tmem_s + sb * 64 + (uint32_t)(i >> 1));
                             const float p = __uint_as_float((i & 1) ? two & 0xffff0000u : two << 16);
                             const bool mine = valid && (seen >> i & 1ull);
                             const __nv_bfloat16* v;
                             if (drafted) {
-                                v = (const __nv_bfloat16*)A.v_new + (size_t)(s.tree0 + key0 + i) * A.v_stride + (size_t)s.g * A.d;
+                                v = (const __nv_bfloat16*)A.v_new + (size_t)(s.first + key0 + i) * A.v_stride + (size_t)s.g * A.d;
                             } else {
                                 const int j = key0 + i, page = A.block_table[(size_t)s.b * A.table_stride + (j >> ps_shift)];
                                 v = (const __nv_bfloat16*)A.v_cache + (((size_t)page * A.nkv + s.g) * A.page_size + (j & (A.page_size - 1))) * A.d;
@@ -503,115 +558,190 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll 1
                             for (int c0 = 0; c0 < DP; c0 += 32) {
                                 float o[32];
-                                tmem_ld32(tmem_o + lane_addr + c0, o);
+                                tmem_ld32(tmem_o + c0, o);
 #pragma unroll
                                 for (int c = 0; c < 32; ++c)
                                     if (mine && c0 + c < A.d) o[c] = fmaf(p, __bfloat162float(v[c0 + c]), o[c]);
-                                tmem_st32(tmem_o + lane_addr + c0, o);
+                                tmem_st32(tmem_o + c0, o);
                             }
                             tmem_st_wait();
                         }
                     }
                 }
                 tc_fence_before();
-                mbar_arrive(my_p_ready);
-            }
-            // ---- O / l, or this part of a job that blocks share -----------------------------------------------------------------------
-            if (alive) alive = mbar_wait(my_pv_done + 8 * ((Th + iters - 1) & 1), ((Th + iters - 1) >> 1) & 1, err);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(my_p_ready + 8 * sb);
+                return true;
+            };
+            int th = Th;
+            const int step = split ? 2 : 1;
+            for (int it = s.i0 + (split ? hd : 0); it < s.i1 && alive; it += step, ++th)
+                alive = it >= mixed && it < full ? tile(std::false_type{}, it, th) : tile(std::true_type{}, it, th);
+            const int n_it = th - Th;
+            // ---- O / l, or this part of a job that blocks share ---------------------------------------------------------------------
+            Th = th;
+            T += s.i1 - s.i0;
+            looks = looks_at(s.i1);
+            if (alive && n_it > 0) alive = wait_warp(my_pv_done + 8 * ((Th - 1) & 1), ((Th - 1) >> 1) & 1, err);
             alive = __all_sync(0xffffffffu, alive);
+            float f_mine = 1.f, f_other = 0.f;
+            if (split && alive) {
+                // the halves' sums come together: each of them takes half of the channels of both
+                volatile float2* stats = reinterpret_cast<volatile float2*>(smem_raw + STATS_OFF);
+                stats[hd * 128 + r].x = m_ref;
+                stats[hd * 128 + r].y = l;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(told);
+                alive = wait_warp(told, joins & 1, err);
+                tc_fence_after();
+                const float m_o = stats[(hd ^ 1) * 128 + r].x, l_o = stats[(hd ^ 1) * 128 + r].y;
+                const float m_all = max3_nan(m_ref, m_o, m_o);
+                f_mine = m_all == -INFINITY ? 0.f : ex2(m_ref - m_all);
+                f_other = m_all == -INFINITY ? 0.f : ex2(m_o - m_all);
+                l = f_mine * l + f_other * l_o;
+                m_ref = m_all;
+            }
             if (alive && working) {
                 tc_fence_after();
-                const bool whole = iters == s.tiles;
-                const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-                const size_t part = part_row(line, blockIdx.x, s.i0 > 0 ? 0 : 1, (node - s.node0) * G + head_r);
-#pragma unroll
-                for (int c0 = 0; c0 < DP; c0 += 32) {
+                if (s.whole) {
+                    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+                    f_mine *= inv;
+                    f_other *= inv;
+                }
+                const uint32_t o_other = tmem + (uint32_t)(256 + (hd ^ 1) * 128) + lane_addr;
+                const int c_from = split ? hd * (DP / 2) : 0, c_to = min(A.d, split ? c_from + DP / 2 : DP);
+                const size_t part = part_row(line, blockIdx.x, s.i0 > 0 ? 0 : 1, (half_first + node_r) * G + head_r);
+                float4* part_to = reinterpret_cast<float4*>(line.part_o) + part_four(line, A.d, part, c_from / 4);
+                __nv_bfloat16* out_to = (__nv_bfloat16*)A.out + (size_t)(s.first + s.node0 + half_first) * A.out_stride + (size_t)s.g * G * A.d + c_from;
+                uint4* const stage = reinterpret_cast<uint4*>(smem_raw + OUT_OFF + warp * 2048);
+                const int st_nodes = min(half_nodes, s.nodes - half_first);
+#pragma unroll 1
+                for (int c0 = c_from; c0 < c_to; c0 += 32) {
                     float o[32];
-                    tmem_ld32(tmem_o + lane_addr + c0, o);
-                    if (!valid) continue;
-                    if (whole) {
-                        __nv_bfloat16* dst = (__nv_bfloat16*)A.out + (size_t)t * A.out_stride + (size_t)h * A.d;
+                    tmem_ld32(tmem_o + c0, o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] *= f_mine;
+                    if (split) {
+                        float o2[32];
+                        tmem_ld32(o_other + c0, o2);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = fmaf(o2[i], f_other, o[i]);
+                    }
+                    if (s.whole) {
+                        // through shared memory, so that neighbouring lanes write neighbouring addresses: 64 bytes of a row lie in
+                        // four pieces of 16, at places that differ from row to row
+                        __syncwarp();
 #pragma unroll
                         for (int c8 = 0; c8 < 4; ++c8) {
-                            const int c = c0 + c8 * 8;
-                            if (c < A.d) {
-                                uint4 v;
-                                v.x = pack_bf16(o[c8 * 8] * inv, o[c8 * 8 + 1] * inv);
-                                v.y = pack_bf16(o[c8 * 8 + 2] * inv, o[c8 * 8 + 3] * inv);
-                                v.z = pack_bf16(o[c8 * 8 + 4] * inv, o[c8 * 8 + 5] * inv);
-                                v.w = pack_bf16(o[c8 * 8 + 6] * inv, o[c8 * 8 + 7] * inv);
-                                store8(dst + c, v, out16);
-                            }
+                            uint4 v;
+                            v.x = pack_bf16(o[c8 * 8], o[c8 * 8 + 1]);
+                            v.y = pack_bf16(o[c8 * 8 + 2], o[c8 * 8 + 3]);
+                            v.z = pack_bf16(o[c8 * 8 + 4], o[c8 * 8 + 5]);
+                            v.w = pack_bf16(o[c8 * 8 + 6], o[c8 * 8 + 7]);
+                            stage[lane * 4 + (c8 ^ ((lane >> 1) & 3))] = v;
                         }
-                    } else {
-                        float* dst = line.part_o + part * A.d;
+                        __syncwarp();
+                        const bool in = c0 + (lane & 3) * 8 < A.d;
 #pragma unroll
-                        for (int c4 = 0; c4 < 8; ++c4) {
-                            const int c = c0 + c4 * 4;
-                            if (c < A.d) *reinterpret_cast<float4*>(dst + c) = make_float4(o[c4 * 4], o[c4 * 4 + 1], o[c4 * 4 + 2], o[c4 * 4 + 3]);
+                        for (int k = 0; k < 4; ++k) {
+                            const int rr = k * 8 + (lane >> 2);
+                            if (in && st_node[k] < st_nodes) store8(out_to + st_at[k], stage[rr * 4 + ((lane & 3) ^ ((rr >> 1) & 3))], out16);
                         }
+                        out_to += 32;
+                    } else if (valid) {
+#pragma unroll
+                        for (int c4 = 0; c4 < 8; ++c4)
+                            if (c0 + c4 * 4 < A.d) part_to[c4 * 8] = make_float4(o[c4 * 4], o[c4 * 4 + 1], o[c4 * 4 + 2], o[c4 * 4 + 3]);
+                        part_to += 64;
                     }
                 }
-                if (valid && !whole) {
-                    line.part_ml[part * 2] = m_ref;
-                    line.part_ml[part * 2 + 1] = l;
-                }
+                if (valid && !s.whole && !(split && hd)) *reinterpret_cast<float2*>(line.part_ml + part * 2) = make_float2(m_ref, l);
             }
-            T += iters;
-            Th += iters;
+            if (split) {
+                // O is not written again before both halves have read it
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(joined);
+                if (alive) alive = wait_warp(joined, joins & 1, err);
+                tc_fence_after();
+                ++joins;
+            }
         }
-        if (!alive) words[1] = 1;
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) tmem_free(tmem, TMEM_COLS);
+    if (warp == 10) tmem_free(tmem, 512);
 }
 
-// Joins the parts of rows that several blocks shared, in the order of the parts: with M the largest of their maxima,
-// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.  A warp per row.
-__global__ void __launch_bounds__(128)
+// Joins the parts of a job that several blocks shared, in the order of the parts: with M the largest of their maxima,
+// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.  Grid (block that the job begins in, some of its rows); a block takes eight rows at a
+// time, a thread four channels of a row, and requests eight parts at once: the join is a few trips to the L2.
+constexpr int MERGE_Y = 8;
+template <int DP>
+__global__ void __launch_bounds__(DP * 2)
 tree_merge_kernel(const TreeArgs A, const Line line) {
+    __shared__ float factors[LINE_BLOCKS][8], inverse[8];
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int t = (int)(item / A.nh), h = (int)(item % A.nh);
-    if (t >= A.tokens || (*reinterpret_cast<volatile int*>(A.err) & XB_ERR_WAIT)) return;
-    const int b = request_of(A, t);
-    if (b < 0) return;
-    const RequestLine r = request_line(A, line, b);
-    const int share = line.starts[A.requests], G = A.nh / A.nkv, node = t - r.first, piece = node / line.job_nodes;
-    const int unit0 = line.starts[b] + (h / G * (r.jobs / A.nkv) + piece) * r.tiles, c0 = unit0 / share, c1 = (unit0 + r.tiles - 1) / share;
-    if (c0 == c1) return;
-    const int row = (node - piece * line.job_nodes) * G + h % G, parts = c1 - c0 + 1;
-    auto at = [&](int i) { return part_row(line, c0 + i, i > 0 ? 0 : 1, row); };
-    float M = -INFINITY;
-    for (int i = lane; i < parts; i += 32) M = fmaxf(M, __ldcg(line.part_ml + at(i) * 2));
-    M = warp_max(M);
-    const float base = M == -INFINITY ? 0.f : M;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, W = 0.f;
-    const int c = lane * 4;
-    for (int i = 0; i < parts; ++i) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(line.part_ml + at(i) * 2));
-        const float f = exp2f(ml.x - base);
-        W = fmaf(f, ml.y, W);
-        if (c < A.d) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(line.part_o + at(i) * A.d + c));
-            acc[0] = fmaf(f, v.x, acc[0]);
-            acc[1] = fmaf(f, v.y, acc[1]);
-            acc[2] = fmaf(f, v.z, acc[2]);
-            acc[3] = fmaf(f, v.w, acc[3]);
-        }
-    }
-    const float inv = W > 0.f || W != W ? 1.f / W : 0.f;
-    if (c < A.d) {
-        __nv_bfloat16* dst = (__nv_bfloat16*)A.out + (size_t)t * A.out_stride + (size_t)h * A.d + c;
-        if (rows_on_16_bytes(A.out, A.out_stride)) {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
-        } else {
+    const int4 job = *reinterpret_cast<const int4*>(line.shared_jobs + blockIdx.x * 8);     // parts, first node's row, nodes, key/value head
+    const int parts = job.x, G = A.nh / A.nkv, rows = job.z * G, in = threadIdx.x & 7, c4 = threadIdx.x >> 3;
+    if (parts < 2 || (*reinterpret_cast<volatile int*>(A.err) & XB_ERR_WAIT)) return;
+    const bool out16 = rows_on_16_bytes(A.out, A.out_stride);
+    for (int row0 = (int)blockIdx.y * 8; row0 < rows; row0 += MERGE_Y * 8) {
+        const int row = row0 + in;
+        auto at = [&](int i) { return part_row(line, blockIdx.x + i, i > 0 ? 0 : 1, row); };
+        const float4* o = reinterpret_cast<const float4*>(line.part_o);
+        float4 v[8];
+        const bool mine = c4 * 4 < A.d;
+        auto fetch = [&](int i0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) dst[i] = __float2bfloat16_rn(acc[i] * inv);
+            for (int i = 0; i < 8; ++i) v[i] = mine && i0 + i < parts ? __ldcg(o + part_four(line, A.d, at(i0 + i), c4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        fetch(0);
+        if (threadIdx.x < 32) {    // four lanes to a row
+            float M = -INFINITY, W = 0.f;
+            for (int i = c4; i < parts; i += 4) M = fmaxf(M, __ldcg(line.part_ml + at(i) * 2));
+            M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 8));
+            M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
+            if (M == -INFINITY) M = 0.f;
+            for (int i = c4; i < parts; i += 4) {
+                const float2 ml = __ldcg(reinterpret_cast<const float2*>(line.part_ml + at(i) * 2));
+                const float f = exp2f(ml.x - M);
+                factors[i][in] = f;
+                W = fmaf(f, ml.y, W);
+            }
+            W += __shfl_xor_sync(0xffffffffu, W, 8);
+            W += __shfl_xor_sync(0xffffffffu, W, 16);
+            if (c4 == 0) inverse[in] = W > 0.f || W != W ? 1.f / W : 0.f;
         }
+        __syncthreads();
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = 0; i0 < parts; i0 += 8) {
+            if (i0) fetch(i0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float f = i0 + i < parts ? factors[i0 + i][in] : 0.f;
+                acc.x = fmaf(f, v[i].x, acc.x);
+                acc.y = fmaf(f, v[i].y, acc.y);
+                acc.z = fmaf(f, v[i].z, acc.z);
+                acc.w = fmaf(f, v[i].w, acc.w);
+            }
+        }
+        if (mine && row < rows) {
+            const float inv = inverse[in];
+            __nv_bfloat16* dst = (__nv_bfloat16*)A.out + (size_t)(job.y + row / G) * A.out_stride + (size_t)(job.w * G + row % G) * A.d + c4 * 4;
+            const uint2 two = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+            if (out16) {
+                *reinterpret_cast<uint2*>(dst) = two;
+            } else {
+                reinterpret_cast<uint16_t*>(dst)[0] = (uint16_t)two.x;
+                reinterpret_cast<uint16_t*>(dst)[1] = (uint16_t)(two.x >> 16);
+                reinterpret_cast<uint16_t*>(dst)[2] = (uint16_t)two.y;
+                reinterpret_cast<uint16_t*>(dst)[3] = (uint16_t)(two.y >> 16);
+            }
+        }
+        __syncthreads();           // the factors are written anew
     }
 }
 
@@ -633,7 +763,7 @@ __global__ void tree_dense_rows_kernel(__nv_bfloat16* to, const TreeArgs A) {
 template <int DP>
 int launch_tc(const TreeArgs& A, const Line& line, cudaStream_t stream) {
     constexpr int NS = stages(DP);
-    constexpr size_t smem = 2 * (DP / 64) * RT * 128 + NS * 2 * (DP / 64) * KT * 128 + 1024;
+    constexpr size_t smem = 2 * (DP / 64) * RT * 128 + NS * 2 * (DP / 64) * KT * 128 + 1024 + 8 * 2048 + 2048 + SEGMENTS * sizeof(Segment);
     static const cudaError_t room = cudaFuncSetAttribute(tree_attention_tc_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (room != cudaSuccess) return (int)room;
     const int G = A.nh / A.nkv, box_rows = A.page_size < KT ? A.page_size : KT;
@@ -647,9 +777,9 @@ int launch_tc(const TreeArgs& A, const Line& line, cudaStream_t stream) {
     if (!tensor_map_bf16(&mq, A.q, 3, dq, sq, bq) || !tensor_map_2d(&mk, A.k_cache, rows, A.d, box_rows) || !tensor_map_2d(&mv, A.v_cache, rows, A.d, box_rows) ||
         !tensor_map_bf16(&mkn, A.k_new, 3, dn, sk, bn) || !tensor_map_bf16(&mvn, A.v_new, 3, dn, sv, bn))
         return (int)cudaErrorInvalidValue;
-    const int rc = xb_launch(tree_attention_tc_kernel<DP>, dim3(line.blocks), dim3(THREADS), smem, stream, mq, mk, mv, mkn, mvn, A, line, shift, A.scale * 1.4426950408889634f);
+    const int rc = xb_launch(tree_attention_tc_kernel<DP>, dim3(LINE_BLOCKS), dim3(THREADS), smem, stream, mq, mk, mv, mkn, mvn, A, line, shift, A.scale * 1.4426950408889634f);
     if (rc) return rc;
-    return xb_launch(tree_merge_kernel, dim3((unsigned)(((long long)A.tokens * A.nh + 3) / 4)), dim3(128), 0, stream, A, line);
+    return xb_launch(tree_merge_kernel<DP>, dim3(LINE_BLOCKS, line.part_rows / 8 < MERGE_Y ? line.part_rows / 8 : MERGE_Y), dim3(DP * 2), 0, stream, A, line);
 }
 
 }  // namespace
