@@ -56,6 +56,7 @@ constexpr int MIN_SHARE = 4;       // tiles that a block takes at least: below t
 constexpr int TILE_ROWS = 128;     // rows (node, query head of the group) of a product; a job has up to two such tiles
 constexpr int COST_ONE = 2;        // what a tile of keys costs a job of one tile of rows, and of two: 1,400 and 2,150 cycles measured
 constexpr int COST_TWO = 3;
+constexpr int COST_JOB = 8;        // what a job costs beside its tiles: its last, drafted keys and its result
 
 struct Line {
     int half_nodes, job_nodes;     // nodes of a tile of rows and of a job
@@ -70,7 +71,8 @@ struct Line {
 struct RequestLine {
     int first, nodes, context, tile0, old_tiles, tiles, pieces;
     int per_tile;                  // what a tile costs each of its jobs
-    __device__ __forceinline__ int units(int nkv) const { return nkv * pieces * tiles * per_tile; }
+    __device__ __forceinline__ int job_units() const { return tiles * per_tile + COST_JOB; }
+    __device__ __forceinline__ int units(int nkv) const { return nkv * pieces * job_units(); }
 };
 
 __device__ __forceinline__ RequestLine request_line(const TreeArgs& A, const Line& line, int b) {
@@ -135,7 +137,7 @@ __device__ __forceinline__ Walk place_in_line(const TreeArgs& A, const Line& lin
     w.b = __shfl_sync(0xffffffffu, b, owner);
     before = __shfl_sync(0xffffffffu, before, owner);
     w.r = request_line(A, line, w.b);
-    const int length = w.r.tiles * w.r.per_tile, at = (w.from - before) / length;
+    const int length = w.r.job_units(), at = (w.from - before) / length;
     w.g = at / w.r.pieces;
     w.piece = at % w.r.pieces;
     w.job = before + at * length;
@@ -146,7 +148,7 @@ __device__ __forceinline__ Walk place_in_line(const TreeArgs& A, const Line& lin
 // job's, or the next request's first.)
 __device__ __forceinline__ bool next_segment(const TreeArgs& A, const Line& line, Walk& w, bool first) {
     for (;; first = false) {
-        if (!first) w.job += w.r.tiles * w.r.per_tile;
+        if (!first) w.job += w.r.job_units();
         if (w.job >= w.end) return false;
         if (!first && ++w.piece == w.r.pieces) {
             w.piece = 0;

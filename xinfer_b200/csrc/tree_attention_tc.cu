@@ -50,6 +50,14 @@ __device__ __forceinline__ void store8(__nv_bfloat16* dst, const uint4& v, bool 
     }
 }
 
+// Whether one of eight bfloat16 is not finite: times zero it is no number, and stays so in a sum.
+__device__ __forceinline__ bool any_not_finite(const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(w[i]), "r"(0u));
+    return (sum & 0x7fff7fffu) != 0u;
+}
 // The largest of three; one that is no number wins.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float d;
@@ -95,16 +103,20 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const uint32_t s_ready0 = rest, pv_done0 = rest + 32, p_ready0 = rest + 64, q_full = rest + 96, q_empty = rest + 104, looked0 = rest + 112,
                    told = rest + 144, joined = rest + 152, seg_full0 = rest + 160, seg_empty0 = seg_full0 + 8 * SEGMENTS;
     volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(smem_raw + BAR_OFF + 4 * RING + 160 + 16 * SEGMENTS);   // tmem, -, then the value rows
-    volatile uint32_t* odd_rows = words + 2;                                                                                // that are not finite: [4][2]
+    volatile uint32_t* odd_rows = words + 2;                                                                                // that are not finite: [4][warp][2]
     Segment* const segments = reinterpret_cast<Segment*>(smem_raw + SEG_OFF);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = A.nh / A.nkv, half_nodes = line.half_nodes;
     int* const err = A.err;
 
     Walk w;
+    bool gave_up = false;
     if (warp == 8) {
         pdl_wait();                // lengths, rows and masks may come from the kernel before
+        if (base & 1023u) atomicOr(err, XB_ERR_WAIT);                                  // the swizzle needs a 1024-byte aligned window
+        const int word = lane == 0 ? *reinterpret_cast<volatile int*>(err) : 0;        // or an earlier block gave up: do not pile on
         w = place_in_line(A, line);
+        gave_up = __any_sync(0xffffffffu, word & XB_ERR_WAIT);
     } else {
         if (threadIdx.x == 9 * 32) {
             for (int i = 0; i < 4 * NS; ++i) mbar_init(bars + 8 * i, 1);
@@ -112,7 +124,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 mbar_init(s_ready0 + 8 * i, 1);
                 mbar_init(pv_done0 + 8 * i, 1);
                 mbar_init(p_ready0 + 8 * i, 4);        // a warp each
-                mbar_init(looked0 + 8 * i, 2);
+                mbar_init(looked0 + 8 * i, 4);
             }
             mbar_init(q_full, 1);
             mbar_init(q_empty, 1);
@@ -159,10 +171,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         int st = 0;
         uint32_t ph = 0;
         bool rounds = false, ok = true;
-        if (!is_v) {
-            if (base & 1023u) atomicOr(err, XB_ERR_WAIT);                                  // the swizzle needs a 1024-byte aligned window
-            if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(err) & XB_ERR_WAIT)) w.job = w.end;   // or an earlier block gave up: do not pile on
-        }
+        if (gave_up) w.job = w.end;
         bool first = true, goes_on = false;
         while (ok) {
             Segment s;
@@ -413,33 +422,6 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const int key0 = !EDGE ? 0 : drafted ? (it - s.old_tiles) * KT : s.key0 + it * KT;
                 const int keys = drafted ? s.tree : s.context;            // keys from here on belong to nobody
                 const int n_look = look ? looks_at(it) : 0;
-                if (EDGE && (split || hd == 0) && r < KT) {
-                    // the value rows: zeroed where nobody may see them, and in tiles that are not seen alike where they are not finite
-                    const int gt = T + it - s.i0, st = gt % NS;
-                    const bool here = wait_warp(v_full0 + 8 * st, (gt / NS) & 1, err);     // orders these accesses after the copy
-                    uint4* row = reinterpret_cast<uint4*>(smem_raw + Q_BYTES + st * STAGE_BYTES + KV_BYTES + r * 128);
-                    bool drop = key0 + r >= keys || (!drafted && window > 0 && key0 + r < s.context - window + 1), odd = false;
-                    if (look && !drop) {
-#pragma unroll
-                        for (int hf = 0; hf < HALVES; ++hf)
-#pragma unroll
-                            for (int c8 = 0; c8 < 8; ++c8) odd |= bf16_not_finite(row[hf * (KV_HALF / 16) + c8]);
-                    }
-                    if (here && (drop || odd)) {
-#pragma unroll
-                        for (int hf = 0; hf < HALVES; ++hf)
-#pragma unroll
-                            for (int c8 = 0; c8 < 8; ++c8) row[hf * (KV_HALF / 16) + c8] = make_uint4(0, 0, 0, 0);
-                    }
-                    const uint32_t odd_mask = __ballot_sync(0xffffffffu, odd);
-                    fence_async_shared();          // the zeroed rows: visible to the product
-                    __syncwarp();
-                    if (look && lane == 0) {
-                        odd_rows[(n_look & 3) * 2 + (warp & 3)] = odd_mask;
-                        mbar_arrive(looked0 + 8 * (n_look & 3));
-                    }
-                    if (!here) return false;
-                }
                 if (!wait_warp(my_s_ready + 8 * sb, (th >> 1) & 1, err)) return false;
                 float corr = 1.f;
                 int moved = 0;
@@ -521,6 +503,42 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     l = l * corr + ((s0 + s1) + (s2 + s3));
                     tmem_st32_u(tmem_s + sb * 64, pk);                   // P goes where the scores were
                 }
+                if (EDGE && (split || hd == 0)) {
+                    // the value rows: zeroed where nobody may see them, and in tiles that are not seen alike where they are not finite.
+                    // Eight lanes have a row's half, a warp every fourth group of four rows.
+                    const int gt = T + it - s.i0, st = gt % NS;
+                    const bool here = wait_warp(v_full0 + 8 * st, (gt / NS) & 1, err);     // orders these accesses after the copy
+                    unsigned char* const rows = smem_raw + Q_BYTES + st * STAGE_BYTES + KV_BYTES;
+                    const int dead_to = !drafted && window > 0 ? s.context - window + 1 - key0 : 0, dead_from = keys - key0;
+                    uint32_t odd_lo = 0, odd_hi = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int rr = k * 16 + (warp & 3) * 4 + (lane >> 3);
+                        uint4* at = reinterpret_cast<uint4*>(rows + rr * 128 + (lane & 7) * 16);
+                        const bool drop = rr >= dead_from || rr < dead_to;
+                        bool odd = false;
+                        if (look && !drop) {
+#pragma unroll
+                            for (int hf = 0; hf < HALVES; ++hf) odd |= any_not_finite(at[hf * (KV_HALF / 16)]);
+                        }
+                        uint32_t mask = __ballot_sync(0xffffffffu, odd);                   // eight bits to a row
+                        mask = (mask & 0xffu ? 1u : 0u) | (mask & 0xff00u ? 2u : 0u) | (mask & 0xff0000u ? 4u : 0u) | (mask & 0xff000000u ? 8u : 0u);
+                        if (here && (drop || (mask >> (lane >> 3) & 1u))) {
+#pragma unroll
+                            for (int hf = 0; hf < HALVES; ++hf) at[hf * (KV_HALF / 16)] = make_uint4(0, 0, 0, 0);
+                        }
+                        if (k < 2) odd_lo |= mask << (k * 16 + (warp & 3) * 4);
+                        else odd_hi |= mask << ((k - 2) * 16 + (warp & 3) * 4);
+                    }
+                    fence_async_shared();          // the zeroed rows: visible to the product
+                    __syncwarp();
+                    if (look && lane == 0) {
+                        odd_rows[(n_look & 3) * 8 + (warp & 3) * 2] = odd_lo;
+                        odd_rows[(n_look & 3) * 8 + (warp & 3) * 2 + 1] = odd_hi;
+                        mbar_arrive(looked0 + 8 * (n_look & 3));
+                    }
+                    if (!here) return false;
+                }
                 // O is touched only when the last tile's P V has completed
                 if (EDGE || __any_sync(0xffffffffu, moved)) {
                     if (th > Th && !wait_warp(my_pv_done + 8 * (sb ^ 1), ((th - 1) >> 1) & 1, err)) return false;
@@ -540,7 +558,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 tmem_st_wait();
                 if (look) {
                     if (!wait_warp(looked0 + 8 * (n_look & 3), (n_look >> 2) & 1, err)) return false;
-                    const uint32_t odd_lo = odd_rows[(n_look & 3) * 2], odd_hi = odd_rows[(n_look & 3) * 2 + 1];
+                    uint32_t odd_lo = 0, odd_hi = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) odd_lo |= odd_rows[(n_look & 3) * 8 + 2 * i], odd_hi |= odd_rows[(n_look & 3) * 8 + 2 * i + 1];
                     if ((odd_lo | odd_hi) && working) {    // (rare) the same for all lanes
                         tc_fence_after();
                         for (int i = 0; i < 64; ++i) {
