@@ -64,7 +64,8 @@ struct Line {
     float* part_o;                 // [blocks][2][part_rows / 8][d / 4][8][4]: a block's first segment, if its job began before it, and its last,
                                    // if its job goes on; four channels of eight rows lie together, as a warp writes and reads them
     float* part_ml;                // [blocks][2][part_rows][2]: maximum and sum
-    int* shared_jobs;              // [blocks][8]: the job that begins in the block and goes on in others
+    int* shared_jobs;              // [blocks][2][8]: the jobs of these parts: parts (0: there is no such part), block of the first, first node's
+                                   // row, nodes, key/value head
     float* dense;                  // room for q, k_new and v_new as dense rows of bfloat16
 };
 
@@ -176,7 +177,7 @@ inline int line_part_rows(int tokens, int group) {
     return ((tokens < nodes ? tokens : nodes) * group + 7) / 8 * 8;
 }
 inline long long line_floats(int tokens, int nh, int nkv, int d) {
-    return (long long)LINE_BLOCKS * (2 * line_part_rows(tokens, nh / nkv) * (long long)(d + 2) + 8) + ((long long)tokens * (nh + 2 * nkv) * d + 1) / 2;
+    return (long long)LINE_BLOCKS * (2 * line_part_rows(tokens, nh / nkv) * (long long)(d + 2) + 16) + ((long long)tokens * (nh + 2 * nkv) * d + 1) / 2;
 }
 inline Line make_line(const TreeArgs& A, float* scratch) {
     const int G = A.nh / A.nkv;
@@ -187,7 +188,7 @@ inline Line make_line(const TreeArgs& A, float* scratch) {
     line.part_o = scratch;
     line.part_ml = scratch + (size_t)LINE_BLOCKS * 2 * line.part_rows * A.d;
     line.shared_jobs = reinterpret_cast<int*>(line.part_ml + (size_t)LINE_BLOCKS * 2 * line.part_rows * 2);
-    line.dense = reinterpret_cast<float*>(line.shared_jobs) + LINE_BLOCKS * 8;
+    line.dense = reinterpret_cast<float*>(line.shared_jobs) + LINE_BLOCKS * 16;
     return line;
 }
 

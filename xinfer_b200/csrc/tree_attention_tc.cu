@@ -50,6 +50,43 @@ __device__ __forceinline__ void store8(__nv_bfloat16* dst, const uint4& v, bool 
     }
 }
 
+// One lane of the warp, chosen by the hardware.
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t e;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(e));
+    return e;
+}
+// Products issued by one lane of a warp that stays together: their operands are then values of the warp, and an issue takes a few
+// instructions (with the issue in a branch of one lane every operand is moved there, 100 cycles a product).
+__device__ __forceinline__ void umma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "setp.ne.b32 q, %4, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(one) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t one, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(bar), "r"(one) : "memory");
+}
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 // Whether one of eight bfloat16 is not finite: times zero it is no number, and stays so in a sum.
 __device__ __forceinline__ bool any_not_finite(const uint4& v) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -82,8 +119,8 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* er
 struct __align__(16) Segment {
     int i0, i1, old_tiles, key0;       // tiles of the job from i0 to i1; cached ones; the first cached key that is walked over
     int context, tree, first, node0;   // cached keys, the request's nodes and the row of the first, the job's first node
-    int nodes, g, b, parts;            // the job's nodes (0: there is no segment any more), key/value head, request, blocks that share the job from here on
-    int deep_lo, whole, pad0, pad1;    // where the deepest node's window begins (0: none); whether this is all of the job
+    int nodes, g, b, whole;            // the job's nodes (0: there is no segment any more), key/value head, request; whether this is all of the job
+    int deep_lo, pad[3];               // where the deepest node's window begins (0: none)
 };
 constexpr int SEGMENTS = 8;
 constexpr int READERS = 11;            // warps that read a segment
@@ -172,7 +209,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         uint32_t ph = 0;
         bool rounds = false, ok = true;
         if (gave_up) w.job = w.end;
-        bool first = true, goes_on = false;
+        bool first = true;
+        int told_of = 0;           // the parts of shared jobs that the join knows of
         while (ok) {
             Segment s;
             if (is_v) {
@@ -195,18 +233,23 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     s.g = w.g;
                     s.b = w.b;
                     s.whole = w.i1 - w.i0 == r.tiles;
-                    s.parts = w.i0 == 0 && !s.whole ? (w.job + (r.tiles - 1) * r.per_tile) / w.share - (int)blockIdx.x + 1 : 0;
                     s.deep_lo = 0;
                     if (A.window > 0) {
                         int deepest = 0;
                         for (int i = lane; i < r.nodes; i += 32) deepest = max(deepest, A.depth[r.first + i]);
                         s.deep_lo = r.context + __reduce_max_sync(0xffffffffu, deepest) - A.window + 1;
                     }
-                    if (s.parts && lane == 0) *reinterpret_cast<int4*>(line.shared_jobs + blockIdx.x * 8) = make_int4(s.parts, s.first + s.node0, s.nodes, s.g);
-                    goes_on |= s.parts > 0;
+                    if (!s.whole && lane == 0) {       // what the join needs to know
+                        const int which = s.i0 > 0 ? 0 : 1, from = w.job / w.share, to = (w.job + (r.tiles - 1) * r.per_tile) / w.share;
+                        int4* job = reinterpret_cast<int4*>(line.shared_jobs + (blockIdx.x * 2 + which) * 8);
+                        job[0] = make_int4(to - from + 1, from, s.first + s.node0, s.nodes);
+                        job[1].x = s.g;
+                        told_of |= 1 << which;
+                    }
                 } else {
                     s.nodes = 0;
-                    if (!goes_on && lane == 0) line.shared_jobs[blockIdx.x * 8] = 0;
+                    for (int which = 0; which < 2; ++which)
+                        if (lane == 0 && !(told_of >> which & 1)) line.shared_jobs[(blockIdx.x * 2 + which) * 8] = 0;
                 }
                 const int at = seg % SEGMENTS;
                 if (seg >= SEGMENTS) ok = wait_warp(seg_empty0 + 8 * at, ((seg / SEGMENTS) - 1) & 1, err);
@@ -265,7 +308,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
     } else if (warp == 9) {
         // ---- Q, then S = Q K^T of every tile --------------------------------------------------------------------------------
-        const bool leader = lane == 0;
+        const uint32_t one = elected(), tmem_u = uniform(tmem);
         const uint32_t idesc_s = umma_idesc(KT, 0);
         const uint64_t dq0 = umma_desc(q_sm, 16, 1024), dk0 = umma_desc(kv_sm, 16, 1024);
         int st = 0, Th[2] = {0, 0};              // ring stage, tiles of either half so far
@@ -273,15 +316,15 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         bool ok = true;
         while (ok) {
             const Segment s = read_segment();
-            if (!s.nodes) break;
-            const int halves = s.nodes > half_nodes ? 2 : 1, I = seg - 1;
+            const int nodes = uniform(s.nodes), iters = uniform(s.i1 - s.i0);
+            if (!nodes) break;
+            const int halves = nodes > half_nodes ? 2 : 1, I = seg - 1;
             if (I > 0) {                         // Q lies where the last one lay: once every product that reads that has completed
-                if (leader) umma_commit(q_empty);
-                __syncwarp();
+                commit(one, q_empty);
                 ok = wait_warp(q_empty, (uint32_t)(I - 1) & 1u, err);
                 if (!ok) break;
             }
-            if (leader) {
+            if (one) {
                 mbar_expect_tx(q_full, (uint32_t)(halves * HALVES * half_nodes * G * 128));
                 for (int hd = 0; hd < halves; ++hd)
 #pragma unroll
@@ -290,32 +333,28 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
             __syncwarp();
             ok = wait_warp(q_full, (uint32_t)I & 1u, err);
-            for (int it = s.i0; it < s.i1 && ok; ++it) {
+            for (int it = 0; it < iters && ok; ++it) {
                 ok = wait_warp(k_full0 + 8 * st, ph, err);
                 const uint64_t dk = dk0 + (uint64_t)((st * STAGE_BYTES) >> 4);
 #pragma unroll
                 for (int hd = 0; hd < 2; ++hd) {
-                    if (halves == 1 && ((it - s.i0) & 1) != hd) continue;
+                    if (halves == 1 && (it & 1) != hd) continue;
                     const int th = Th[hd]++, sb = th & 1;
                     // these columns held the scores and then P of this half's last tile but one: its P V must have read them
                     ok = ok && (th < 2 || wait_warp(pv_done0 + 8 * (2 * hd + sb), ((th >> 1) - 1) & 1, err));
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t dq = dq0 + (uint64_t)((halves == 1 ? 0u : hd * Q_ONE) >> 4);
-                    if (leader) {
 #pragma unroll
-                        for (int kk = 0; kk < DP / 16; ++kk) {
-                            const uint32_t off = (kk >> 2), inner = (kk & 3) * 32;
-                            umma_bf16(tmem + (uint32_t)(hd * 128 + sb * 64), dq + (uint64_t)((off * RT * 128 + inner) >> 4),
-                                      dk + (uint64_t)((off * KV_HALF + inner) >> 4), idesc_s, kk ? 1u : 0u);
-                        }
-                        umma_commit(s_ready0 + 8 * (2 * hd + sb));
+                    for (int kk = 0; kk < DP / 16; ++kk) {
+                        const uint32_t off = (kk >> 2), inner = (kk & 3) * 32;
+                        umma_ss(one, tmem_u + (uint32_t)(hd * 128 + sb * 64), dq + (uint64_t)((off * RT * 128 + inner) >> 4),
+                                dk + (uint64_t)((off * KV_HALF + inner) >> 4), idesc_s, kk ? 1u : 0u);
                     }
-                    __syncwarp();
+                    commit(one, s_ready0 + 8 * (2 * hd + sb));
                 }
                 if (!ok) break;
-                if (leader) umma_commit(k_empty0 + 8 * st);
-                __syncwarp();
+                commit(one, k_empty0 + 8 * st);
                 if (++st == NS) {
                     st = 0;
                     ph ^= 1u;
@@ -324,7 +363,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
     } else if (warp == 11) {
         // ---- O += P V of every tile (O starts as zeros, by the softmax threads) -----------------------------------------------
-        const bool leader = lane == 0;
+        const uint32_t one = elected(), tmem_u = uniform(tmem);
         const uint32_t idesc_o = umma_idesc(DP, 1);
         const uint64_t dv0 = umma_desc(kv_sm + KV_BYTES, KV_HALF, 1024);
         int st = 0, Th[2] = {0, 0};
@@ -332,30 +371,27 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         bool ok = true;
         while (ok) {
             const Segment s = read_segment();
-            if (!s.nodes) break;
-            const int halves = s.nodes > half_nodes ? 2 : 1;
-            for (int it = s.i0; it < s.i1 && ok; ++it) {
+            const int nodes = uniform(s.nodes), iters = uniform(s.i1 - s.i0);
+            if (!nodes) break;
+            const int halves = nodes > half_nodes ? 2 : 1;
+            for (int it = 0; it < iters && ok; ++it) {
                 ok = wait_warp(v_full0 + 8 * st, ph, err);
                 const uint64_t dv = dv0 + (uint64_t)((st * STAGE_BYTES) >> 4);
 #pragma unroll
                 for (int hd = 0; hd < 2; ++hd) {
-                    if (halves == 1 && ((it - s.i0) & 1) != hd) continue;
+                    if (halves == 1 && (it & 1) != hd) continue;
                     const int th = Th[hd]++, sb = th & 1;
                     ok = ok && wait_warp(p_ready0 + 8 * (2 * hd + sb), (th >> 1) & 1, err);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t tp = tmem + (uint32_t)(hd * 128 + sb * 64);
-                    if (leader) {
+                    const uint32_t tp = tmem_u + (uint32_t)(hd * 128 + sb * 64);
 #pragma unroll
-                        for (int kk = 0; kk < KT / 16; ++kk)
-                            umma_bf16_ta(tmem + (uint32_t)(256 + hd * 128), tp + (uint32_t)(kk * 8), dv + (uint64_t)((kk * 2048) >> 4), idesc_o, 1u);
-                        umma_commit(pv_done0 + 8 * (2 * hd + sb));
-                    }
-                    __syncwarp();
+                    for (int kk = 0; kk < KT / 16; ++kk)
+                        umma_ts(one, tmem_u + (uint32_t)(256 + hd * 128), tp + (uint32_t)(kk * 8), dv + (uint64_t)((kk * 2048) >> 4), idesc_o);
+                    commit(one, pv_done0 + 8 * (2 * hd + sb));
                 }
                 if (!ok) break;
-                if (leader) umma_commit(v_empty0 + 8 * st);
-                __syncwarp();
+                commit(one, v_empty0 + 8 * st);
                 if (++st == NS) {
                     st = 0;
                     ph ^= 1u;
@@ -695,63 +731,55 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 }
 
 // Joins the parts of a job that several blocks shared, in the order of the parts: with M the largest of their maxima,
-// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.  Grid (block that the job begins in, some of its rows); a block takes eight rows at a
-// time, a thread four channels of a row, and requests eight parts at once: the join is a few trips to the L2.
-constexpr int MERGE_Y = 8;
-template <int DP>
-__global__ void __launch_bounds__(DP * 2)
-tree_merge_kernel(const TreeArgs A, const Line line) {
-    __shared__ float factors[LINE_BLOCKS][8], inverse[8];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int4 job = *reinterpret_cast<const int4*>(line.shared_jobs + blockIdx.x * 8);     // parts, first node's row, nodes, key/value head
-    const int parts = job.x, G = A.nh / A.nkv, rows = job.z * G, in = threadIdx.x & 7, c4 = threadIdx.x >> 3;
-    if (parts < 2 || (*reinterpret_cast<volatile int*>(A.err) & XB_ERR_WAIT)) return;
+// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.  Grid (block and which of its parts, MERGE_Y): as many of the job's rows as the part is
+// of the job, so that there are as many blocks at work as there are parts.  A thread has four channels of a row in every group of eight
+// rows and requests eight numbers of four at once: P parts of 8 / P groups.  The join is then a trip or two to the L2.
+constexpr int MERGE_Y = 4;
+constexpr int MERGE_ROWS = 32;     // rows whose factors lie in shared memory
+
+struct MergeJob {
+    int parts, c_first, t0, rows, g, G;
+};
+
+template <int P>
+__device__ __forceinline__ void merge_groups(const TreeArgs& A, const Line& line, const MergeJob& job, const float (*factors)[MERGE_ROWS],
+                                             const float* inverse, int base, int end, int in, int c4) {
+    constexpr int K = 8 / P;
+    const float4* o = reinterpret_cast<const float4*>(line.part_o);
     const bool out16 = rows_on_16_bytes(A.out, A.out_stride);
-    for (int row0 = (int)blockIdx.y * 8; row0 < rows; row0 += MERGE_Y * 8) {
-        const int row = row0 + in;
-        auto at = [&](int i) { return part_row(line, blockIdx.x + i, i > 0 ? 0 : 1, row); };
-        const float4* o = reinterpret_cast<const float4*>(line.part_o);
-        float4 v[8];
-        const bool mine = c4 * 4 < A.d;
-        auto fetch = [&](int i0) {
+    for (int g0 = base; g0 < end; g0 += K) {
+        float4 acc[K];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = mine && i0 + i < parts ? __ldcg(o + part_four(line, A.d, at(i0 + i), c4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        };
-        fetch(0);
-        if (threadIdx.x < 32) {    // four lanes to a row
-            float M = -INFINITY, W = 0.f;
-            for (int i = c4; i < parts; i += 4) M = fmaxf(M, __ldcg(line.part_ml + at(i) * 2));
-            M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 8));
-            M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
-            if (M == -INFINITY) M = 0.f;
-            for (int i = c4; i < parts; i += 4) {
-                const float2 ml = __ldcg(reinterpret_cast<const float2*>(line.part_ml + at(i) * 2));
-                const float f = exp2f(ml.x - M);
-                factors[i][in] = f;
-                W = fmaf(f, ml.y, W);
-            }
-            W += __shfl_xor_sync(0xffffffffu, W, 8);
-            W += __shfl_xor_sync(0xffffffffu, W, 16);
-            if (c4 == 0) inverse[in] = W > 0.f || W != W ? 1.f / W : 0.f;
-        }
-        __syncthreads();
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = 0; i0 < parts; i0 += 8) {
-            if (i0) fetch(i0);
+        for (int k = 0; k < K; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = 0; i0 < job.parts; i0 += P) {
+            float4 v[K][P];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float f = i0 + i < parts ? factors[i0 + i][in] : 0.f;
-                acc.x = fmaf(f, v[i].x, acc.x);
-                acc.y = fmaf(f, v[i].y, acc.y);
-                acc.z = fmaf(f, v[i].z, acc.z);
-                acc.w = fmaf(f, v[i].w, acc.w);
-            }
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const int row = (g0 + k) * 8 + in;
+                    v[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (g0 + k < end && i0 + i < job.parts)
+                        v[k][i] = __ldcg(o + part_four(line, A.d, part_row(line, job.c_first + i0 + i, i0 + i > 0 ? 0 : 1, row), c4));
+                }
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const float f = g0 + k < end && i0 + i < job.parts ? factors[i0 + i][(g0 + k - base) * 8 + in] : 0.f;
+                    acc[k].x = fmaf(f, v[k][i].x, acc[k].x);
+                    acc[k].y = fmaf(f, v[k][i].y, acc[k].y);
+                    acc[k].z = fmaf(f, v[k][i].z, acc[k].z);
+                    acc[k].w = fmaf(f, v[k][i].w, acc[k].w);
+                }
         }
-        if (mine && row < rows) {
-            const float inv = inverse[in];
-            __nv_bfloat16* dst = (__nv_bfloat16*)A.out + (size_t)(job.y + row / G) * A.out_stride + (size_t)(job.w * G + row % G) * A.d + c4 * 4;
-            const uint2 two = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int row = (g0 + k) * 8 + in;
+            if (g0 + k >= end || row >= job.rows) continue;
+            const float inv = inverse[(g0 + k - base) * 8 + in];
+            __nv_bfloat16* dst = (__nv_bfloat16*)A.out + (size_t)(job.t0 + row / job.G) * A.out_stride + (size_t)(job.g * job.G + row % job.G) * A.d + c4 * 4;
+            const uint2 two = make_uint2(pack_bf16(acc[k].x * inv, acc[k].y * inv), pack_bf16(acc[k].z * inv, acc[k].w * inv));
             if (out16) {
                 *reinterpret_cast<uint2*>(dst) = two;
             } else {
@@ -760,6 +788,52 @@ tree_merge_kernel(const TreeArgs A, const Line line) {
                 reinterpret_cast<uint16_t*>(dst)[2] = (uint16_t)two.y;
                 reinterpret_cast<uint16_t*>(dst)[3] = (uint16_t)(two.y >> 16);
             }
+        }
+    }
+}
+
+template <int DP>
+__global__ void __launch_bounds__(DP * 2)
+tree_merge_kernel(const TreeArgs A, const Line line) {
+    __shared__ float factors[LINE_BLOCKS][MERGE_ROWS], inverse[MERGE_ROWS];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int4 told = *reinterpret_cast<const int4*>(line.shared_jobs + blockIdx.x * 8);    // parts, first block, first node's row, nodes
+    const int G = A.nh / A.nkv;
+    const MergeJob job{told.x, told.y, told.z, told.w * G, line.shared_jobs[blockIdx.x * 8 + 4], G};
+    if (job.parts < 2) return;
+    // this block's groups of eight rows
+    const int groups = (job.rows + 7) / 8, shares = job.parts * MERGE_Y, mine = ((int)blockIdx.x / 2 - job.c_first) * MERGE_Y + blockIdx.y;
+    const int g0 = groups * mine / shares, g1 = groups * (mine + 1) / shares;
+    if (g0 >= g1 || (*reinterpret_cast<volatile int*>(A.err) & XB_ERR_WAIT)) return;
+    const int in = threadIdx.x & 7, c4 = threadIdx.x >> 3;
+    const float2* ml = reinterpret_cast<const float2*>(line.part_ml);
+    for (int base = g0; base < g1; base += MERGE_ROWS / 8) {
+        const int end = min(g1, base + MERGE_ROWS / 8);
+        for (int t = threadIdx.x; t < (end - base) * 64; t += DP * 2) {    // eight lanes to a row
+            const int r8 = t >> 3, q = t & 7, row = min(base * 8 + r8, job.rows - 1);
+            auto at = [&](int i) { return ml + part_row(line, job.c_first + i, i > 0 ? 0 : 1, row); };
+            const float2 first = q < job.parts ? __ldcg(at(q)) : make_float2(-INFINITY, 0.f);
+            float M = first.x, W = 0.f;
+            for (int i = q + 8; i < job.parts; i += 8) M = fmaxf(M, __ldcg(at(i)).x);
+#pragma unroll
+            for (int k = 1; k < 8; k <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+            if (M == -INFINITY) M = 0.f;
+            for (int i = q; i < job.parts; i += 8) {
+                const float2 x = i == q ? first : __ldcg(at(i));
+                const float f = exp2f(x.x - M);
+                factors[i][r8] = f;
+                W = fmaf(f, x.y, W);
+            }
+#pragma unroll
+            for (int k = 1; k < 8; k <<= 1) W += __shfl_xor_sync(0xffffffffu, W, k);
+            if (q == 0) inverse[r8] = W > 0.f || W != W ? 1.f / W : 0.f;
+        }
+        __syncthreads();
+        if (c4 * 4 < A.d) {
+            if (job.parts == 2) merge_groups<2>(A, line, job, factors, inverse, base, end, in, c4);
+            else if (job.parts <= 4) merge_groups<4>(A, line, job, factors, inverse, base, end, in, c4);
+            else merge_groups<8>(A, line, job, factors, inverse, base, end, in, c4);
         }
         __syncthreads();           // the factors are written anew
     }
@@ -799,7 +873,7 @@ int launch_tc(const TreeArgs& A, const Line& line, cudaStream_t stream) {
         return (int)cudaErrorInvalidValue;
     const int rc = xb_launch(tree_attention_tc_kernel<DP>, dim3(LINE_BLOCKS), dim3(THREADS), smem, stream, mq, mk, mv, mkn, mvn, A, line, shift, A.scale * 1.4426950408889634f);
     if (rc) return rc;
-    return xb_launch(tree_merge_kernel<DP>, dim3(LINE_BLOCKS, line.part_rows / 8 < MERGE_Y ? line.part_rows / 8 : MERGE_Y), dim3(DP * 2), 0, stream, A, line);
+    return xb_launch(tree_merge_kernel<DP>, dim3(2 * LINE_BLOCKS, MERGE_Y), dim3(DP * 2), 0, stream, A, line);
 }
 
 }  // namespace
