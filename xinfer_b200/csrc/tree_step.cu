@@ -10,6 +10,8 @@ namespace {
 // targets[its parent], as long as there is one and the path has room.  A warp per request.
 __global__ void tree_accept_kernel(int* accepted, int* path, int* next_tokens, const int* drafted, const int* targets, const int* parents,
                                    const int* token_start, int requests, int tokens, int width) {
+    pdl_launch_dependents();
+    pdl_wait();
     const int lane = threadIdx.x & 31, b = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5);
     if (b >= requests) return;
     const int first = min(max(token_start[b], 0), tokens), n = min(max(token_start[b + 1], first), tokens) - first;
@@ -42,7 +44,6 @@ __global__ void tree_accept_kernel(int* accepted, int* path, int* next_tokens, c
 // is written by another and the same call may be made twice.  A request whose pages are not all there gets none and no slots; its
 // length stays.  Every block forms the requests' sums for itself and takes a share of the tokens.
 constexpr int SLOT_THREADS = 256;
-constexpr int SLOT_TOKENS = 1024;               // tokens a block takes at a time
 constexpr int SLOT_REQUESTS = 8192;             // requests of a call: their starts lie in shared memory
 
 struct SlotArgs {
@@ -86,84 +87,100 @@ __device__ __forceinline__ Sums block_prefix(Sums mine, Sums* of_warps, Sums& to
     return Sums{before.tokens + incl.tokens - mine.tokens, before.need + incl.need - mine.need, before.back + incl.back - mine.back};
 }
 
+// The last of `n` runs that begins at or before x, of runs that begin at begin(0) = 0 <= begin(1) <= ...
+template <typename Begin>
+__device__ __forceinline__ int run_of(int x, int n, Begin begin) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (begin(mid) <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
 __global__ void __launch_bounds__(SLOT_THREADS)
 cache_slots_kernel(const SlotArgs A) {
-    extern __shared__ int starts[];                              // [requests + 1], then [requests]: pages taken before the request's own
-    int* taken_before = starts + A.requests + 1;                 // (-1: the request was not served)
+    extern __shared__ int starts[];                              // per request: tokens before it,
+    int* need_before = starts + A.requests + 1;                  // pages taken before it (~ of them: it was not served),
+    int* back_before = need_before + A.requests;                 // pages given back before it
     __shared__ Sums of_warps[SLOT_THREADS / 32];
     __shared__ int taken;
-    const int each = (A.requests + SLOT_THREADS - 1) / SLOT_THREADS, b0 = (int)threadIdx.x * each;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int each = (A.requests + SLOT_THREADS - 1) / SLOT_THREADS, b0 = (int)threadIdx.x * each, b1 = min(b0 + each, A.requests);
     const int ps = A.page_size, head = (A.ring[0] % A.ring_size + A.ring_size) % A.ring_size, count = min(max(A.ring[1], 0), A.ring_size);
     // whether the request's pages, those it holds and those it asks for, fit its row of the table; one whose do not asks for none
-    auto fits = [&](int b) { return ((long long)max(A.lengths[b], 0) + max(A.new_tokens[b], 0) + ps - 1) / ps <= A.table_stride; };
-    auto held_by = [&](int b) { return (int)(((long long)max(A.lengths[b], 0) + ps - 1) / ps); };
-    auto sums_of = [&](int b) {
-        const int add = A.new_tokens[b];
-        if (!fits(b)) return Sums{max(add, 0), 0, 0};
-        const int held = held_by(b);
-        if (add < 0) return Sums{0, 0, held};
-        return Sums{add, (int)(((long long)max(A.lengths[b], 0) + add + ps - 1) / ps) - held, 0};
+    auto fits = [&](int len, int add) { return ((long long)len + max(add, 0) + ps - 1) / ps <= A.table_stride; };
+    auto pages = [&](int len) { return (int)(((long long)len + ps - 1) / ps); };
+    auto sums_of = [&](int len, int add) {
+        if (!fits(len, add)) return Sums{max(add, 0), 0, 0};
+        if (add < 0) return Sums{0, 0, pages(len)};
+        return Sums{add, (int)(((long long)len + add + ps - 1) / ps) - pages(len), 0};
     };
     Sums mine{0, 0, 0}, total;
-    for (int b = b0; b < min(b0 + each, A.requests); ++b) mine = mine + sums_of(b);
+    for (int b = b0; b < b1; ++b) mine = mine + sums_of(max(A.lengths[b], 0), A.new_tokens[b]);
     if (threadIdx.x == 0) taken = 0;
     Sums at = block_prefix(mine, of_warps, total);
     const bool first_block = blockIdx.x == 0;
-    for (int b = b0; b < min(b0 + each, A.requests); ++b) {
-        const Sums s = sums_of(b);
-        const int len = max(A.lengths[b], 0), add = A.new_tokens[b], held = held_by(b);
-        const bool served = fits(b) && (s.need == 0 || at.need + s.need <= count);
+    int most = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int len = max(A.lengths[b], 0), add = A.new_tokens[b];
+        const Sums s = sums_of(len, add);
+        const bool served = fits(len, add) && (s.need == 0 || at.need + s.need <= count);
         starts[b] = at.tokens;
-        taken_before[b] = served ? at.need : -1;
-        if (served && s.need > 0) atomicMax(&taken, at.need + s.need);
+        need_before[b] = served ? at.need : ~at.need;
+        back_before[b] = at.back;
+        if (served && s.need > 0) most = at.need + s.need;
         if (first_block) {
             A.token_start[b] = at.tokens;
             A.lengths_out[b] = add < 0 ? 0 : (served ? len + add : len);
             if (!served) atomicOr(A.err, XB_ERR_NO_PAGE);
-            int* row = A.table + (size_t)b * A.table_stride;
-            if (served)
-                for (int i = 0; i < s.need; ++i) row[held + i] = A.free_ring[(int)(((long long)head + at.need + i) % A.ring_size)];
-            if (total.back + count <= A.ring_size)
-                for (int i = 0; i < s.back; ++i) A.free_ring[(int)(((long long)head + count + at.back + i) % A.ring_size)] = row[i];
         }
         at = at + s;
     }
+    if (most > 0) atomicMax(&taken, most);
     if (threadIdx.x == 0) starts[A.requests] = total.tokens;
     __syncthreads();
+    const bool room = total.back + count <= A.ring_size;         // (more pages than the ring was made for: they are not taken back)
     if (first_block && threadIdx.x == 0) {
         A.token_start[A.requests] = total.tokens;
         A.ring_out[0] = (int)(((long long)head + taken) % A.ring_size);
-        const bool room = total.back + count <= A.ring_size;     // (more pages than the ring was made for: they are not taken back)
         A.ring_out[1] = count - taken + (room ? total.back : 0);
         if (!room) atomicOr(A.err, XB_ERR_BAD_PAGE);
         if (total.tokens > A.capacity) atomicOr(A.err, XB_ERR_BAD_ROW);
     }
-    for (int base = (int)blockIdx.x * SLOT_TOKENS; base < A.capacity; base += (int)gridDim.x * SLOT_TOKENS)
-        for (int t = base + (int)threadIdx.x; t < min(base + SLOT_TOKENS, A.capacity); t += SLOT_THREADS) {
-            if (t >= total.tokens) {
-                A.slots[t] = -1;
-                A.positions[t] = 0;
-                A.request[t] = -1;
-                continue;
-            }
-            int lo = 0, hi = A.requests;                         // starts[lo] <= t < starts[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (starts[mid] <= t) lo = mid;
-                else hi = mid;
-            }
-            const int len = max(A.lengths[lo], 0), pos = len + t - starts[lo], place = pos / ps, held = held_by(lo);
-            long long slot = -1;
-            if (taken_before[lo] >= 0) {
-                const int page = place < held ? A.table[(size_t)lo * A.table_stride + place]
-                                              : A.free_ring[(int)(((long long)head + taken_before[lo] + place - held) % A.ring_size)];
-                if (page >= 0) slot = (long long)page * ps + pos % ps;
-                else atomicOr(A.err, XB_ERR_BAD_PAGE);
-            }
-            A.slots[t] = slot;
-            A.positions[t] = pos;
-            A.request[t] = lo;
+    auto ring_at = [&](int i) { return (int)(((long long)head + i) % A.ring_size); };
+    auto needed = [&](int b) { return need_before[b] < 0 ? ~need_before[b] : need_before[b]; };
+    const int threads = (int)gridDim.x * SLOT_THREADS, me = (int)blockIdx.x * SLOT_THREADS + (int)threadIdx.x;
+    for (int i = me; i < min(taken, total.need); i += threads) { // new entries of the table: the i-th page from the ring's head
+        const int b = run_of(i, A.requests, needed);
+        if (need_before[b] >= 0) A.table[(size_t)b * A.table_stride + pages(max(A.lengths[b], 0)) + i - need_before[b]] = A.free_ring[ring_at(i)];
+    }
+    if (room)
+        for (int i = me; i < total.back; i += threads) {         // pages that are given back
+            const int b = run_of(i, A.requests, [&](int b) { return back_before[b]; });
+            A.free_ring[ring_at(count + i)] = A.table[(size_t)b * A.table_stride + i - back_before[b]];
         }
+    for (int t = me; t < A.capacity; t += threads) {
+        if (t >= total.tokens) {
+            A.slots[t] = -1;
+            A.positions[t] = 0;
+            A.request[t] = -1;
+            continue;
+        }
+        const int b = run_of(t, A.requests, [&](int b) { return starts[b]; });
+        const int len = max(A.lengths[b], 0), pos = len + t - starts[b], place = pos / ps, held = pages(len);
+        long long slot = -1;
+        if (need_before[b] >= 0) {
+            const int page = place < held ? A.table[(size_t)b * A.table_stride + place] : A.free_ring[ring_at(need_before[b] + place - held)];
+            if (page >= 0) slot = (long long)page * ps + pos % ps;
+            else atomicOr(A.err, XB_ERR_BAD_PAGE);
+        }
+        A.slots[t] = slot;
+        A.positions[t] = pos;
+        A.request[t] = b;
+    }
 }
 
 // ---- accepted rows into the cache ------------------------------------------------------------------------------------------
@@ -173,6 +190,8 @@ template <typename U>
 __global__ void cache_commit_kernel(const void* const* layers /* [layers][4]: k cache, v cache, new k, new v */, const long long* slots,
                                     const int* request_of, const int* token_start, const int* path, int requests, int width, int rows, int nkv,
                                     int units, int page_size, long long num_slots, int* err) {
+    pdl_launch_dependents();
+    pdl_wait();
     const int i = blockIdx.x;
     const int b = request_of[i];
     if (b < 0 || b >= requests) return;
@@ -201,8 +220,8 @@ XB_EXPORT int xb_tree_accept(int* accepted, int* path, int* next_tokens, const i
                              const int* token_start, int requests, int tokens, int width, cudaStream_t stream) {
     if (requests <= 0) return 0;
     if (width < 1) return (int)cudaErrorInvalidValue;
-    tree_accept_kernel<<<(requests + 3) / 4, 128, 0, stream>>>(accepted, path, next_tokens, drafted, targets, parents, token_start, requests, tokens, width);
-    return xb_launch_status();
+    return xb_launch(tree_accept_kernel, dim3((requests + 3) / 4), dim3(128), 0, stream, accepted, path, next_tokens, drafted, targets, parents, token_start, requests,
+                     tokens, width);
 }
 
 XB_EXPORT int xb_cache_slots(long long* slots, int* positions, int* request, int* token_start, int* lengths_out, int* ring_out, int* table, int* free_ring,
@@ -212,13 +231,12 @@ XB_EXPORT int xb_cache_slots(long long* slots, int* positions, int* request, int
     if (requests > SLOT_REQUESTS || page_size < 1 || ring_size < 1 || table_stride < 1) return (int)cudaErrorInvalidValue;
     const SlotArgs A{slots, positions, request, token_start, lengths_out, ring_out, table, free_ring, ring, lengths, new_tokens,
                      requests, capacity, table_stride, page_size, ring_size, err};
-    int blocks = (capacity + SLOT_TOKENS - 1) / SLOT_TOKENS;
-    blocks = blocks < 1 ? 1 : (blocks > 148 ? 148 : blocks);
-    const size_t smem = (2 * (size_t)requests + 1) * 4;
-    static const cudaError_t room = cudaFuncSetAttribute(cache_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * SLOT_REQUESTS + 1) * 4);
+    int blocks = (capacity + SLOT_THREADS - 1) / SLOT_THREADS;
+    blocks = blocks < 4 ? 4 : (blocks > 148 ? 148 : blocks);    // (four also where few tokens come: pages are given back beside them)
+    const size_t smem = (3 * (size_t)requests + 1) * 4;
+    static const cudaError_t room = cudaFuncSetAttribute(cache_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * SLOT_REQUESTS + 1) * 4);
     if (room != cudaSuccess) return (int)room;
-    cache_slots_kernel<<<blocks, SLOT_THREADS, smem, stream>>>(A);
-    return xb_launch_status();
+    return xb_launch(cache_slots_kernel, dim3(blocks), dim3(SLOT_THREADS), smem, stream, A);
 }
 
 XB_EXPORT int xb_cache_commit(const void* const* layers, int num_layers, const long long* slots, const int* request_of, const int* token_start,
@@ -227,9 +245,8 @@ XB_EXPORT int xb_cache_commit(const void* const* layers, int num_layers, const l
     if (tokens <= 0 || num_layers <= 0 || requests <= 0) return 0;
     if (num_layers > 65535 || row_bytes < 2 || row_bytes % 2 || page_size < 1) return (int)cudaErrorInvalidValue;
     const dim3 grid(tokens, num_layers);
-    if (row_bytes % 16 == 0)
-        cache_commit_kernel<uint4><<<grid, 128, 0, stream>>>(layers, slots, request_of, token_start, path, requests, width, rows, nkv, row_bytes / 16, page_size, num_slots, err);
-    else
-        cache_commit_kernel<uint16_t><<<grid, 128, 0, stream>>>(layers, slots, request_of, token_start, path, requests, width, rows, nkv, row_bytes / 2, page_size, num_slots, err);
-    return xb_launch_status();
+    auto go = [&](auto kernel, int unit) {
+        return xb_launch(kernel, grid, dim3(128), 0, stream, layers, slots, request_of, token_start, path, requests, width, rows, nkv, row_bytes / unit, page_size, num_slots, err);
+    };
+    return row_bytes % 16 == 0 ? go(cache_commit_kernel<uint4>, 16) : go(cache_commit_kernel<uint16_t>, 2);
 }

@@ -1870,6 +1870,8 @@ def logit_rules(out, logits, penalties, history, history_start, prompt_len, *, l
         _need(ancestors, "ancestors", torch.int32, (R, None))
         _need(first_row, "first_row", torch.int32, (R,))
         words = ancestors.shape[1]
+        if words > 32:
+            raise KernelError(f"ancestors of {words} words: trees of up to 1,024 nodes")
     if bias is not None:
         bias_start, bias_tokens, bias_values = bias
         _need(bias_start, "bias start", torch.int32, (R + 1,))
