@@ -30,85 +30,103 @@ struct RuleArgs {
     const int* mask;               // [masks, mask_words], bit v: token v may follow; null without masks
     const int* mask_of_row;        // [rows], negative: no mask; null: row r has mask r
     long long out_stride, in_stride, history_len, bias_len;
-    int rows, lists, vocab, words, masks, mask_words, rows_per_block;
+    int rows, lists, vocab, words, masks, mask_words;
 };
 
-__device__ __forceinline__ float ruled(float x, unsigned count, float rep, float freq, float pres) {
+// (`inv` is 1 / rep, rounded: a product in place of a quotient is one float32 rounding more, and a sixth of the instructions)
+__device__ __forceinline__ float ruled(float x, unsigned count, float rep, float inv, float freq, float pres) {
     if (count == 0u) return x;
-    x = x > 0.f ? x / rep : x * rep;
+    x *= x > 0.f ? inv : rep;
     const unsigned c = count & ~ASKED;
     if (c) x = x - freq * (float)c - pres;
     return x;
 }
 
-constexpr int ROWS = 16;                        // rows of a block at most: what they need to know lies in shared memory
+constexpr int WARPS = THREADS / 32;
+constexpr int ROWS = 48;                        // rows at a time: what they need to know lies in shared memory
 constexpr int WORDS = 32;                       // words of ancestors: trees of up to 1,024 nodes
+constexpr int BIASES = 384;                     // biases of the rows at a time
+constexpr int STAGES = 2;                       // rows on their way or worked on
 
 struct RowFacts {
-    float rep, freq, pres;
+    float rep, inv, freq, pres;
     int list, mask, first, bias, biases;
 };
+struct Bias {
+    int u;                                      // where in the chunk (-1: elsewhere, or not the first of the row's entries for its token)
+    float value;                                // of all the row's entries for that token
+};
 
-// A block takes 1,024 VECS tokens of the vocabulary of several rows in turn.  The lists' tokens are counted in shared memory, once for
-// rows that follow each other with one list (the nodes of a tree); a row's own path is added before it and taken away behind it.  The
-// next row's logits and mask are on their way meanwhile.  Bound by memory: a logit is read and written once.
+template <int N>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+    if (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(from) : "memory");
+}
+
+constexpr int chunk_of(int vecs) { return 4 * THREADS * vecs; }
+constexpr int mask_room(int vecs) { return WARPS * vecs * 5; }
+constexpr int smem_of(int vecs, int words) { return 4 * (chunk_of(vecs) + STAGES * (chunk_of(vecs) + mask_room(vecs)) + words * (ROWS + 4 * WARPS + 32)); }
+
+// The vocabulary is cut into chunks of 1,024 VECS tokens, and the (chunk, row) pairs, chunk by chunk, into equal shares for as many blocks
+// as the device holds.  The lists' tokens are counted in shared memory, once for rows that follow each other with one list (the nodes of a
+// tree); a row's own path is added before it and taken away behind it.  A warp owns 128 of every 1,024 tokens, with their counts, mask
+// words and biases, so that the warps of a block go through the rows without waiting for each other; each has two more rows on their way.
+// Bound by memory: a logit is read and written once.
 template <int VECS>
-__global__ void __launch_bounds__(THREADS, 4)
+__global__ void __launch_bounds__(THREADS)
 logit_rules_kernel(const RuleArgs A) {
-    constexpr int CHUNK = 4 * THREADS * VECS;
-    __shared__ __align__(16) unsigned count[CHUNK];
+    constexpr int CHUNK = chunk_of(VECS);
+    extern __shared__ __align__(16) unsigned count[];            // [CHUNK], then the stages' logits and their mask words
+    float4* const logits_at = reinterpret_cast<float4*>(count + CHUNK);
+    int* const masks_at = reinterpret_cast<int*>(count + CHUNK + STAGES * CHUNK);          // [STAGES][WARPS][VECS][5]
     __shared__ RowFacts facts[ROWS];
-    __shared__ int paths[ROWS][WORDS], node_at[WORDS * 32];      // the rows' ancestors; where the tree's drafted tokens lie in the chunk, or -1
+    __shared__ Bias biases[BIASES];
+    // the rows' ancestors [ROWS][words]; the nodes whose tokens a warp owns, by `head` [WARPS][4][words]; where the tree's drafted tokens lie
+    // in the chunk, or -1 [words][32]
+    unsigned* const paths = reinterpret_cast<unsigned*>(masks_at + STAGES * mask_room(VECS));
+    unsigned* const own_nodes = paths + ROWS * A.words;
+    int* const node_at = reinterpret_cast<int*>(own_nodes + WARPS * 4 * A.words);
     pdl_launch_dependents();
     pdl_wait();
-    const int lo = (int)blockIdx.x * CHUNK, n = min(CHUNK, A.vocab - lo), tid = threadIdx.x;
-    const int r0 = (int)blockIdx.y * A.rows_per_block, rows = min(A.rows - r0, A.rows_per_block);
-    if (tid < rows) {
-        const int r = r0 + tid;
-        RowFacts f;
-        f.rep = A.penalties[3 * r];
-        f.freq = A.penalties[3 * r + 1];
-        f.pres = A.penalties[3 * r + 2];
-        f.list = A.list_of_row ? A.list_of_row[r] : r;
-        if (f.list < 0 || f.list >= A.lists) f.list = -1;
-        f.mask = A.mask == nullptr ? -1 : (A.mask_of_row ? A.mask_of_row[r] : r);
-        if (f.mask < 0 || f.mask >= A.masks) f.mask = -1;
-        f.first = A.drafted ? A.first_row[r] : 0;
-        f.bias = A.bias_start ? max(0, A.bias_start[r]) : 0;
-        f.biases = A.bias_start ? (int)max(0LL, min((long long)A.bias_start[r + 1], A.bias_len) - f.bias) : 0;
-        facts[tid] = f;
-    }
-    for (int i = tid; i < rows * A.words; i += THREADS) paths[i / A.words][i % A.words] = A.ancestors[(size_t)r0 * A.words + i];
-    __syncthreads();
-    float4 x[VECS];
-    int may_word[VECS];
-    // The row's logits that lie on 16-byte boundaries are taken four at a time, behind `head` (0 to 3) that do not; `whole` of them.
-    int head = 0, whole = 0;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long units = (long long)((A.vocab + CHUNK - 1) / CHUNK) * A.rows;
+    const long long from = units * blockIdx.x / gridDim.x, to = units * (blockIdx.x + 1) / gridDim.x;
+    int lo = 0, n = 0, r0 = 0, rows = 0;       // the chunk's first token, its tokens; rows r0 .. r0 + rows - 1
+    int listed = 0;                            // their biases in `biases` (-1: a row by itself with more than fit)
+    int counted = -2, tree = -1;               // the list that `count` holds (-1: none), the tree that `node_at` does; of this chunk
+
+    // The row's logits that lie on 16-byte boundaries are taken four at a time, behind `head` (0 to 3) that do not; `whole` fours.
+    auto head_of = [&](int k) { return min(n, (int)((16 - ((uintptr_t)(A.logits + (size_t)(r0 + k) * A.in_stride + lo) & 15)) & 15) / 4); };
+    // the warp that has element u of the chunk; the first one has those beside the fours
+    auto owner = [&](int u, int head, int whole) { return u < head || u >= head + 4 * whole ? 0 : (u - head) >> 7 & (WARPS - 1); };
+    // (every row is a group of copies, those behind the last row are empty)
     auto fetch = [&](int k) {
-        const float* in = A.logits + (size_t)(r0 + k) * A.in_stride + lo;
-        head = min(n, (int)((16 - ((uintptr_t)in & 15)) & 15) / 4);
-        whole = (n - head) / 4;
-        const int* mask = facts[k].mask >= 0 ? A.mask + (size_t)facts[k].mask * A.mask_words : nullptr;
+        if (k < rows) {
+            const float* in = A.logits + (size_t)(r0 + k) * A.in_stride + lo;
+            const int head = head_of(k), whole = (n - head) / 4, stage = k % STAGES;
+            float4* to = logits_at + stage * (CHUNK / 4) + tid;
+            const float4* from = reinterpret_cast<const float4*>(in + head) + tid;
 #pragma unroll
-        for (int j = 0; j < VECS; ++j) {
-            const int i = tid + j * THREADS;
-            if (i < whole) {
-                x[j] = __ldcs(reinterpret_cast<const float4*>(in + head) + i);
-                if (mask) may_word[j] = mask[(lo + head + 4 * i) >> 5];
+            for (int j = 0; j < VECS; ++j)
+                if (tid + j * THREADS < whole) copy_async<16>(to + j * THREADS, from + j * THREADS);
+            if (facts[k].mask >= 0 && lane < 5 * VECS) {         // the words of the warp's 128 tokens in each 1,024: four, or five off a word's start
+                const int word = ((lo + head + (lane / 5) * 4 * THREADS + warp * 128) >> 5) + lane % 5;
+                if (word < A.mask_words) copy_async<4>(masks_at + (stage * WARPS + warp) * VECS * 5 + lane, A.mask + (size_t)facts[k].mask * A.mask_words + word);
             }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    // adds `by` to the counts of the drafted tokens on the row's path
-    auto add_path = [&](int k, unsigned by) {
-        for (int i = tid; i < A.words * 32; i += THREADS)
-            if ((paths[k][i >> 5] >> (i & 31) & 1) && node_at[i] >= 0) atomicAdd(&count[node_at[i]], by);
+    // adds `by` to the counts of the drafted tokens on the row's path, the warp's own ones
+    auto add_path = [&](int k, int head, unsigned by) {
+        for (int w = 0; w < A.words; ++w)
+            if ((paths[k * A.words + w] & own_nodes[(warp * 4 + head) * A.words + w]) >> lane & 1) atomicAdd(&count[node_at[w * 32 + lane]], by);
     };
-    fetch(0);
-    int counted = -2, tree = -1;               // the list that `count` holds (-1: none), the tree that `node_at` does
-    for (int k = 0; k < rows; ++k) {
+    auto work = [&](int k) {
         const RowFacts f = facts[k];
-        if (f.list != counted || (A.drafted && f.first != tree)) {
-            __syncthreads();                   // (the last row's path has been taken away)
+        const int head = head_of(k), whole = (n - head) / 4, stage = k % STAGES;
+        if (f.list != counted || (A.drafted && f.first != tree)) {           // (the same for the whole block)
+            __syncthreads();
             if (f.list != counted) {
 #pragma unroll
                 for (int j = 0; j < VECS; ++j) reinterpret_cast<uint4*>(count)[tid + j * THREADS] = make_uint4(0u, 0u, 0u, 0u);
@@ -123,93 +141,195 @@ logit_rules_kernel(const RuleArgs A) {
             if (f.list >= 0 && f.list != counted) {
                 const long long a = max(0, A.history_start[f.list]), z = min((long long)A.history_start[f.list + 1], A.history_len);
                 const long long said = a + A.prompt_len[f.list];
-#pragma unroll 4
-                for (long long i = a + tid; i < z; i += THREADS) {
-                    const unsigned u = (unsigned)(A.history[i] - lo);
+                auto say = [&](int token, long long i) {
+                    const unsigned u = (unsigned)(token - lo);
                     if (u < (unsigned)n) {
                         if (i < said) atomicOr(&count[u], ASKED);
                         else atomicAdd(&count[u], 1u);
                     }
+                };
+                // four tokens at a time from the first 16-byte boundary on
+                const long long a4 = min(z, a + (long long)((16 - ((uintptr_t)(A.history + a) & 15)) & 15) / 4), z4 = z - max(0LL, z - a4) % 4;
+                if (a + tid < a4) say(A.history[a + tid], a + tid);
+                if (z4 >= a4 && z4 + tid < z) say(A.history[z4 + tid], z4 + tid);
+#pragma unroll 4
+                for (long long i = a4 + 4 * tid; i < z4; i += 4 * THREADS) {
+                    const int4 t = *reinterpret_cast<const int4*>(A.history + i);
+                    say(t.x, i);
+                    say(t.y, i + 1);
+                    say(t.z, i + 2);
+                    say(t.w, i + 3);
                 }
             }
+            if (A.drafted && f.first != tree)
+                for (int h = 0; h < 4; ++h)                      // for every way that a row may lie
+                    for (int w = 0; w < A.words; ++w) {
+                        const int u = node_at[w * 32 + lane], head = min(n, h);
+                        const unsigned mine = __ballot_sync(0xffffffffu, u >= 0 && owner(u, head, (n - head) / 4) == warp);
+                        if (lane == 0) own_nodes[(warp * 4 + h) * A.words + w] = mine;
+                    }
+            __syncthreads();
             counted = f.list;
             tree = f.first;
         }
-        if (A.drafted) add_path(k, 1u);
-        const int bias_v = tid < f.biases ? A.bias_tokens[f.bias + tid] : -1;      // on its way while the row is worked on
-        __syncthreads();
-        const int* mask = f.mask >= 0 ? A.mask + (size_t)f.mask * A.mask_words : nullptr;
+        if (A.drafted) add_path(k, head, 1u);
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");      // this row is there
+        __syncwarp();
+        const float4* x = logits_at + stage * (CHUNK / 4) + tid;
+        const int* mask = f.mask >= 0 ? masks_at + (stage * WARPS + warp) * VECS * 5 : nullptr;
+        const int* far_mask = f.mask >= 0 ? A.mask + (size_t)f.mask * A.mask_words : nullptr;
         const float* in = A.logits + (size_t)(r0 + k) * A.in_stride + lo;
         float* out = A.out + (size_t)(r0 + k) * A.out_stride + lo;
         const bool fours = (((uintptr_t)(out + head)) & 15) == 0;
-        // (the few beside the fours)
-        for (int i = tid; i < n - 4 * whole; i += THREADS) {
-            const int u = i < head ? i : i + 4 * whole;
-            const bool may = mask == nullptr || (mask[(lo + u) >> 5] >> ((lo + u) & 31) & 1);
-            out[u] = may ? ruled(in[u], count[u], f.rep, f.freq, f.pres) : -INFINITY;
-        }
-#pragma unroll
-        for (int j = 0; j < VECS; ++j) {
-            const int i = tid + j * THREADS, u = head + 4 * i;
-            if (i >= whole) continue;
-            uint4 c;
-            if (head == 0) c = reinterpret_cast<const uint4*>(count)[i];
-            else c = make_uint4(count[u], count[u + 1], count[u + 2], count[u + 3]);
-            const int shift = (lo + u) & 31;
-            unsigned may = mask ? (unsigned)may_word[j] >> shift : 15u;
-            // four bits that begin in the last three of a word go on in the next one, which is there: a token's word is
-            if (mask && shift > 28) may = __funnelshift_r((unsigned)may_word[j], (unsigned)mask[((lo + u) >> 5) + 1], shift);
-            float4 y = x[j];
+        auto all_four = [&](float4 y, const uint4& c, unsigned may) {
             if (c.x | c.y | c.z | c.w) {
-                y.x = ruled(y.x, c.x, f.rep, f.freq, f.pres);
-                y.y = ruled(y.y, c.y, f.rep, f.freq, f.pres);
-                y.z = ruled(y.z, c.z, f.rep, f.freq, f.pres);
-                y.w = ruled(y.w, c.w, f.rep, f.freq, f.pres);
+                y.x = ruled(y.x, c.x, f.rep, f.inv, f.freq, f.pres);
+                y.y = ruled(y.y, c.y, f.rep, f.inv, f.freq, f.pres);
+                y.z = ruled(y.z, c.z, f.rep, f.inv, f.freq, f.pres);
+                y.w = ruled(y.w, c.w, f.rep, f.inv, f.freq, f.pres);
             }
             if (!(may & 1u)) y.x = -INFINITY;
             if (!(may & 2u)) y.y = -INFINITY;
             if (!(may & 4u)) y.z = -INFINITY;
             if (!(may & 8u)) y.w = -INFINITY;
-            if (fours) {
-                reinterpret_cast<float4*>(out + head)[i] = y;
-            } else {
-                out[u] = y.x;
-                out[u + 1] = y.y;
-                out[u + 2] = y.z;
-                out[u + 3] = y.w;
+            return y;
+        };
+        auto may_say = [&](int u) { return far_mask == nullptr || (far_mask[(lo + u) >> 5] >> ((lo + u) & 31) & 1); };
+        if (head == 0 && fours && n == CHUNK) {
+            // a whole chunk on 16-byte boundaries: the same in a third of the instructions (lo is a multiple of 32)
+            float4* out4 = reinterpret_cast<float4*>(out) + tid;
+            const uint4* count4 = reinterpret_cast<const uint4*>(count) + tid;
+            const int shift = 4 * lane & 31;
+#pragma unroll
+            for (int j = 0; j < VECS; ++j) __stcs(out4 + j * THREADS, all_four(x[j * THREADS], count4[j * THREADS], mask ? (unsigned)mask[j * 5 + (lane >> 3)] >> shift : 15u));
+        } else {
+            if (warp == 0)         // (the few beside the fours)
+                for (int i = lane; i < n - 4 * whole; i += 32) {
+                    const int u = i < head ? i : i + 4 * whole;
+                    out[u] = may_say(u) ? ruled(in[u], count[u], f.rep, f.inv, f.freq, f.pres) : -INFINITY;
+                }
+#pragma unroll
+            for (int j = 0; j < VECS; ++j) {
+                const int i = tid + j * THREADS, u = head + 4 * i;
+                if (i >= whole) continue;
+                uint4 c;
+                if (head == 0) c = reinterpret_cast<const uint4*>(count)[i];
+                else c = make_uint4(count[u], count[u + 1], count[u + 2], count[u + 3]);
+                unsigned may = 15u;
+                if (mask) {            // (four bits that begin in the last three of a word go on in the next one)
+                    const int word = ((lo + u) >> 5) - ((lo + head + j * 4 * THREADS + warp * 128) >> 5), shift = (lo + u) & 31;
+                    may = (unsigned)mask[j * 5 + word] >> shift;
+                    if (shift > 28) may = __funnelshift_r((unsigned)mask[j * 5 + word], (unsigned)mask[j * 5 + word + 1], shift);
+                }
+                const float4 y = all_four(x[j * THREADS], c, may);
+                if (fours) {
+                    reinterpret_cast<float4*>(out + head)[i] = y;
+                } else {
+                    out[u] = y.x;
+                    out[u + 1] = y.y;
+                    out[u + 2] = y.z;
+                    out[u + 3] = y.w;
+                }
             }
         }
-        if (k + 1 < rows) fetch(k + 1);
-        if (!A.drafted && f.biases == 0) continue;
-        __syncthreads();                       // the counts have been read, the row is written
-        if (A.drafted) add_path(k, 0xffffffffu);
-        // a token that several entries name gets their sum, in their order, from the thread of the first
-        for (int i = tid; i < f.biases; i += THREADS) {
-            const int* tokens = A.bias_tokens + f.bias;
-            const int v = i == tid ? bias_v : tokens[i];
-            const unsigned u = (unsigned)(v - lo);
-            if (u >= (unsigned)n) continue;
-            if (mask != nullptr && !(mask[v >> 5] >> (v & 31) & 1)) continue;
-            bool first = true;
-            for (int j = 0; j < i && first; ++j) first = tokens[j] != v;
-            if (!first) continue;
-            float y = out[u];
-            for (int j = i; j < f.biases; ++j)
-                if (tokens[j] == v) y += A.bias_values[f.bias + j];
-            out[u] = y;
+        if (!A.drafted && !A.bias_start) return;
+        __syncwarp();                          // the warp's counts have been read, its part of the row is written
+        if (A.drafted) add_path(k, head, 0xffffffffu);
+        if (listed > 0)
+            for (int i = lane; i < f.biases; i += 32) {
+                const Bias b = biases[f.bias - facts[0].bias + i];
+                if (b.u >= 0 && owner(b.u, head, whole) == warp && may_say(b.u)) out[b.u] += b.value;
+            }
+        if (listed < 0)
+            for (int i = lane; i < f.biases; i += 32) {
+                const int* tokens = A.bias_tokens + f.bias;
+                const int v = tokens[i], u = v - lo;
+                if ((unsigned)u >= (unsigned)n || owner(u, head, whole) != warp || !may_say(u)) continue;
+                bool mine = true;
+                for (int j = 0; j < i && mine; ++j) mine = tokens[j] != v;
+                if (!mine) continue;
+                float sum = 0.f;
+                for (int j = i; j < f.biases; ++j)
+                    if (tokens[j] == v) sum += A.bias_values[f.bias + j];
+                out[u] += sum;
+            }
+        __syncwarp();
+    };
+    for (long long at = from; at < to; at += rows) {
+        r0 = (int)(at % A.rows);
+        rows = (int)min((long long)min(ROWS, A.rows - r0), to - at);
+        if ((int)(at / A.rows) * CHUNK != lo || at == from) {
+            lo = (int)(at / A.rows) * CHUNK;
+            n = min(CHUNK, A.vocab - lo);
+            counted = -2;
+            tree = -1;
+        }
+        listed = 0;
+        if (A.bias_start) {                    // as many rows as have no more biases than there is room for
+            auto biases_to = [&](int r) { return (int)min((long long)max(0, A.bias_start[r]), A.bias_len); };
+            while (rows > 1 && biases_to(r0 + rows) - biases_to(r0) > BIASES) rows = (rows + 1) / 2;
+            listed = max(0, biases_to(r0 + rows) - biases_to(r0));
+            if (listed > BIASES) listed = -1;
+        }
+        __syncthreads();                       // (the rows before are done with)
+        if (tid < rows) {
+            const int r = r0 + tid;
+            RowFacts f;
+            f.rep = A.penalties[3 * r];
+            f.inv = 1.f / f.rep;
+            f.freq = A.penalties[3 * r + 1];
+            f.pres = A.penalties[3 * r + 2];
+            f.list = A.list_of_row ? A.list_of_row[r] : r;
+            if (f.list < 0 || f.list >= A.lists) f.list = -1;
+            f.mask = A.mask == nullptr ? -1 : (A.mask_of_row ? A.mask_of_row[r] : r);
+            if (f.mask < 0 || f.mask >= A.masks) f.mask = -1;
+            f.first = A.drafted ? A.first_row[r] : 0;
+            f.bias = A.bias_start ? max(0, A.bias_start[r]) : 0;
+            f.biases = A.bias_start ? (int)max(0LL, min((long long)A.bias_start[r + 1], A.bias_len) - f.bias) : 0;
+            facts[tid] = f;
+        }
+        for (int i = tid; i < rows * A.words; i += THREADS) paths[i] = A.ancestors[(size_t)r0 * A.words + i];
+        __syncthreads();
+        for (int k = 0; k < STAGES - 1; ++k) fetch(k);
+        if (listed > 0) {
+            // a token that several of a row's entries name gets their sum, in their order, by the first of them
+            for (int i = tid; i < listed; i += THREADS) {
+                const long long e = facts[0].bias + i;
+                const int v = A.bias_tokens[e], u = v - lo;
+                Bias b{-1, 0.f};
+                if ((unsigned)u < (unsigned)n) {
+                    int row = 0;
+                    while (row + 1 < rows && facts[row + 1].bias <= e) ++row;
+                    bool mine = true;
+                    for (long long j = facts[row].bias; j < e && mine; ++j) mine = A.bias_tokens[j] != v;
+                    if (mine) {
+                        b.u = u;
+                        for (long long j = e; j < facts[row].bias + facts[row].biases; ++j)
+                            if (A.bias_tokens[j] == v) b.value += A.bias_values[j];
+                    }
+                }
+                biases[i] = b;
+            }
+            __syncthreads();
+        }
+        for (int k = 0; k < rows; ++k) {
+            work(k);
+            fetch(k + STAGES - 1);             // (into the stage of row k - 1, which this warp alone reads and has read)
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 template <int VECS>
-int launch(RuleArgs A, cudaStream_t stream) {
-    const int chunks = (A.vocab + 4 * THREADS * VECS - 1) / (4 * THREADS * VECS);
-    // rows that share a list are counted once where they follow each other in a block: as many rows to a block as leave eight blocks
-    // for every processor
-    const long long blocks = (long long)chunks * A.rows;
-    A.rows_per_block = (int)(blocks / (148 * 8));
-    A.rows_per_block = A.rows_per_block < 1 ? 1 : (A.rows_per_block > ROWS ? ROWS : A.rows_per_block);
-    return xb_launch(logit_rules_kernel<VECS>, dim3(chunks, (A.rows + A.rows_per_block - 1) / A.rows_per_block), dim3(THREADS), 0, stream, A);
+int launch(const RuleArgs& A, cudaStream_t stream) {
+    const int smem = smem_of(VECS, A.words);
+    int per_sm = 0;
+    cudaError_t rc = cudaFuncSetAttribute(logit_rules_kernel<VECS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of(VECS, WORDS));
+    if (rc == cudaSuccess) rc = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, logit_rules_kernel<VECS>, THREADS, smem);
+    if (rc != cudaSuccess) return (int)rc;
+    const int resident = (per_sm > 0 ? per_sm : 1) * 148;          // blocks that the device holds
+    const long long units = (long long)((A.vocab + chunk_of(VECS) - 1) / chunk_of(VECS)) * A.rows;
+    return xb_launch(logit_rules_kernel<VECS>, dim3((unsigned)(units < resident ? units : resident)), dim3(THREADS), smem, stream, A);
 }
 
 }  // namespace
@@ -222,7 +342,7 @@ XB_EXPORT int xb_logit_rules(float* out, const float* logits, const float* penal
     if (rows <= 0 || vocab <= 0) return 0;
     if (rows > (1 << 20) || words > WORDS || (mask && mask_words < (vocab + 31) / 32)) return (int)cudaErrorInvalidValue;
     const RuleArgs A{out, logits, penalties, history, history_start, prompt_len, list_of_row, drafted, ancestors, first_row, bias_start, bias_tokens,
-                     bias_values, mask, mask_of_row, out_stride, in_stride, history_len, bias_len, rows, lists, vocab, words, masks, mask_words, 1};
+                     bias_values, mask, mask_of_row, out_stride, in_stride, history_len, bias_len, rows, lists, vocab, words, masks, mask_words};
     // chunks of 1,024 tokens while that leaves processors without work, of 4,096 when there are rows enough
     return (long long)rows * vocab < 148LL * 2 * 4096 ? launch<1>(A, stream) : launch<4>(A, stream);
 }
