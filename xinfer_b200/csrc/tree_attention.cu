@@ -11,93 +11,344 @@ namespace {
 
 using namespace xbtree;
 
-constexpr int WARPS = 4;
+// The kernel for float32, and for what the tcgen05 kernel does not take (tree_attention_tc.cu): any head size, group and page.  A job's rows
+// are 32 (node, query head) pairs; a tile is 32 keys.  Scores are formed 2 rows x 4 keys a thread and values summed 4 rows x 4 channels at a
+// time, by float32 multiply-adds from shared memory; a warp forms the softmax of eight rows, a key per lane.  Jobs, tiles and the join are
+// those of the line in tree_attention.cuh, four blocks to a processor.  Bound by the multiply-adds' operands from shared memory: a score
+// or value product reads two numbers of it for every three it forms.
+constexpr int RT = 32, KT = 32, THREADS = 128, LINE_BLOCKS = 4 * 148;
 
-// The simple form, for every type, head size and layout: a warp per (node, head), 32 keys at a time.  A lane scores a key, the
-// warp forms the tile's maximum and sum, then the lanes hold channels and the tile's weights come by shuffle.
-template <typename T, int CH>
-__global__ void __launch_bounds__(WARPS * 32)
-tree_attention_kernel(const TreeArgs A) {
-    extern __shared__ float q_rows[];        // [WARPS][d]
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long item = (long long)blockIdx.x * WARPS + warp;
-    const int t = (int)(item / A.nh), h = (int)(item % A.nh);
-    if (t >= A.tokens) return;
-    const int b = request_of(A, t);
-    T* out = (T*)A.out + (size_t)t * A.out_stride + (size_t)h * A.d;
-    if (b < 0) return;                       // a row of no request is left as it is
-    const int g = h / (A.nh / A.nkv), first = clamp_start(A, A.token_start[b]), n = clamp_start(A, A.token_start[b + 1]) - first;
-    const int context = context_of(A, b);
-    const int my_depth = A.window > 0 ? max(0, A.depth[t]) : 0, my_pos = context + my_depth;
-    const int lo = A.window > 0 ? max(0, my_pos - A.window + 1) : 0;
-    float* qs = q_rows + (size_t)warp * A.d;
-    const T* q = (const T*)A.q + (size_t)t * A.q_stride + (size_t)h * A.d;
-    for (int c = lane; c < A.d; c += 32) qs[c] = to_f32<T>(q[c]);
-    __syncwarp();
-    float m = -INFINITY, l = 0.f, o[CH];
+// Four channels of a row from c on, zeros from d on; `fours`: rows start where four numbers may be read at once (and d is a multiple of 4).
+__device__ __forceinline__ float4 four_of(const float* row, int c, int d, bool fours) {
+    if (fours) return c < d ? *reinterpret_cast<const float4*>(row + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    return make_float4(c < d ? row[c] : 0.f, c + 1 < d ? row[c + 1] : 0.f, c + 2 < d ? row[c + 2] : 0.f, c + 3 < d ? row[c + 3] : 0.f);
+}
+__device__ __forceinline__ float4 four_of(const __nv_bfloat16* row, int c, int d, bool fours) {
+    if (fours) {
+        if (c >= d) return make_float4(0.f, 0.f, 0.f, 0.f);
+        const uint2 v = *reinterpret_cast<const uint2*>(row + c);
+        return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+    }
+    auto at = [&](int i) { return c + i < d ? __bfloat162float(row[c + i]) : 0.f; };
+    return make_float4(at(0), at(1), at(2), at(3));
+}
+__device__ __forceinline__ bool finite(const float4& v) {
+    return fabsf(v.x) <= 3.402823466e38f && fabsf(v.y) <= 3.402823466e38f && fabsf(v.z) <= 3.402823466e38f && fabsf(v.w) <= 3.402823466e38f;
+}
+
+// DP: the head size rounded up; rows of zeros lie behind d.
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS)
+tree_attention_kernel(const TreeArgs A, const Line line) {
+    constexpr int LD = DP + 4, LP = KT + 4, CJ = DP / 64;
+    extern __shared__ __align__(16) float smem[];
+    float* const q_sm = smem;                      // [RT][LD]
+    float* const k_sm = q_sm + RT * LD;            // [KT][LD]
+    float* const v_sm = k_sm + KT * LD;            // [KT][DP]
+    float* const p_sm = v_sm + KT * DP;            // [RT][LP]
+    __shared__ Walk walk;
+    __shared__ float corr[RT], sums[RT], tops[RT];
+    __shared__ unsigned seen_of[RT];
+    // of this tile and the next: where the keys begin in their tensor (-1 nowhere), the keys' depths, the rows' ancestors among the keys
+    __shared__ long long rows_of[2][KT];
+    __shared__ int depths[2][KT], row_depth[RT];
+    __shared__ unsigned masks[2][RT];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = A.nh / A.nkv;
+    const T *q = (const T*)A.q, *k_new = (const T*)A.k_new, *v_new = (const T*)A.v_new, *k_cache = (const T*)A.k_cache, *v_cache = (const T*)A.v_cache;
+    auto on_fours = [](const void* p, long long stride) { return ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0 && stride % 4 == 0; };
+    const bool fours = A.d % 4 == 0 && on_fours(q, A.q_stride) && on_fours(k_new, A.k_stride) && on_fours(v_new, A.v_stride) && on_fours(k_cache, 0) && on_fours(v_cache, 0);
+    if (warp == 0) {
+        const Walk w = place_in_line<KT>(A, line);
+        if (lane == 0) walk = w;
+    }
+    __syncthreads();
+    Walk w = walk;
+    int told_of = 0;
+    for (bool first = true; next_segment<KT>(A, line, w, first); first = false) {
+        const RequestLine& s = w.r;
+        const int row0 = w.piece * RT, rows = min(RT, s.nodes * G - row0);
+        const bool whole = w.i1 - w.i0 == s.tiles;
+        for (int i = tid; i < RT * DP / 4; i += THREADS) {
+            const int r = i / (DP / 4), c = i % (DP / 4) * 4, row = row0 + r;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows) x = four_of(q + (size_t)(s.first + row / G) * A.q_stride + (size_t)(w.g * G + row % G) * A.d, c, A.d, fours);
+            *reinterpret_cast<float4*>(q_sm + r * LD + c) = x;
+        }
+        if (tid < RT) {
+            tops[tid] = -INFINITY;
+            sums[tid] = 0.f;
+        }
+        const int* table = A.block_table + (size_t)w.b * A.table_stride;
+        float o[4][CJ][4];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) o[i] = 0.f;
-    const int* table = A.block_table + (size_t)b * A.table_stride;
-    const int old_tiles = (context + 31) / 32, tiles = old_tiles + (n + 31) / 32;
-    for (int tile = lo / 32; tile < tiles; ++tile) {
-        const bool drafted = tile >= old_tiles;
-        const int j = (drafted ? tile - old_tiles : tile) * 32 + lane;
-        bool seen;
-        long long row = 0;                   // of the key, in elements of its tensor
-        if (drafted) {
-            seen = j < n && (A.ancestors[(size_t)t * A.words + (j >> 5)] >> (j & 31) & 1);
-            if (seen && A.window > 0) seen = my_depth - max(0, A.depth[first + j]) < A.window;
-        } else {
-            seen = j >= lo && j < context;
-            if (seen) {
-                const int page = table[j / A.page_size];
-                if (page < 0 || page >= A.num_pages) {
-                    atomicOr(A.err, XB_ERR_BAD_PAGE);
-                    seen = false;
-                } else {
-                    row = (((long long)page * A.nkv + g) * A.page_size + j % A.page_size) * A.d;
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < CJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[r][j][e] = 0.f;
+        const int o_row = tid / 16 * 4, o_col = tid % 16 * 4;
+        // a window's first key, of the root; keys before it are nobody's
+        const int lo = A.window > 0 ? max(0, s.context - A.window + 1) : 0;
+        auto find_rows = [&](int it) {             // by the first warp, a key and a row to a lane
+            const bool drafted = it >= s.old_tiles;
+            const int key = (drafted ? it - s.old_tiles : s.tile0 + it) * KT + lane;
+            long long at = -1;
+            if (drafted) {
+                if (key < s.nodes) at = s.first + key;
+            } else if (key < s.context && key >= lo) {
+                const int page = table[key / A.page_size];
+                if (page >= 0 && page < A.num_pages) at = (((long long)page * A.nkv + w.g) * A.page_size + key % A.page_size) * A.d;
+                else atomicOr(A.err, XB_ERR_BAD_PAGE);
+            }
+            rows_of[it & 1][lane] = at;
+            if (drafted) {
+                unsigned mask = 0;
+                if (lane < rows && (key >> 5) < A.words) mask = (unsigned)A.ancestors[(size_t)(s.first + (row0 + lane) / G) * A.words + (key >> 5)];
+                masks[it & 1][lane] = mask;
+                depths[it & 1][lane] = A.window > 0 && key < s.nodes ? max(0, A.depth[s.first + key]) : 0;
+            }
+        };
+        if (warp == 0) {
+            row_depth[lane] = A.window > 0 && lane < rows ? max(0, A.depth[s.first + (row0 + lane) / G]) : 0;
+            find_rows(w.i0);
+        }
+        for (int it = w.i0; it < w.i1; ++it) {
+            const bool drafted = it >= s.old_tiles;
+            const int key0 = drafted ? (it - s.old_tiles) * KT : (s.tile0 + it) * KT, keys = min(KT, (drafted ? s.nodes : s.context) - key0);
+            bool odd = false;
+            __syncthreads();                       // the tile before has been read
+#pragma unroll 4
+            for (int i = tid; i < KT * DP / 4; i += THREADS) {
+                const int j = i / (DP / 4), c = i % (DP / 4) * 4;
+                const long long at = rows_of[it & 1][j];
+                float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+                if (at >= 0) {
+                    k = four_of(drafted ? k_new + at * A.k_stride + (size_t)w.g * A.d : k_cache + at, c, A.d, fours);
+                    v = four_of(drafted ? v_new + at * A.v_stride + (size_t)w.g * A.d : v_cache + at, c, A.d, fours);
+                }
+                odd |= !finite(v);
+                *reinterpret_cast<float4*>(k_sm + j * LD + c) = k;
+                *reinterpret_cast<float4*>(v_sm + j * DP + c) = v;
+            }
+            // a value that is not finite may be one that not all rows see: their weights of zero must not meet it
+            const bool some_odd = __syncthreads_or(odd) && (drafted || A.window > 0);
+            if (warp == 0 && it + 1 < w.i1) find_rows(it + 1);
+            {
+                const int r = tid / 8 * 2, j = tid % 8;
+                float sc[2][4] = {};
+#pragma unroll 4
+                for (int c = 0; c < DP; c += 4) {
+                    float4 a[2], b[4];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) a[x] = *reinterpret_cast<const float4*>(q_sm + (r + x) * LD + c);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) b[y] = *reinterpret_cast<const float4*>(k_sm + (j + 8 * y) * LD + c);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            sc[x][y] = fmaf(a[x].x, b[y].x, sc[x][y]);
+                            sc[x][y] = fmaf(a[x].y, b[y].y, sc[x][y]);
+                            sc[x][y] = fmaf(a[x].z, b[y].z, sc[x][y]);
+                            sc[x][y] = fmaf(a[x].w, b[y].w, sc[x][y]);
+                        }
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) p_sm[(r + x) * LP + j + 8 * y] = sc[x][y];
+            }
+            __syncthreads();
+            {
+                // a warp has eight rows, side by side
+                constexpr int R = RT / (THREADS / 32);
+                float x[R], top[R], sum[R];
+                bool seen[R];
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const int r = warp * R + i;
+                    seen[i] = r < rows && lane < keys;
+                    if (drafted) seen[i] = seen[i] && (masks[it & 1][r] >> lane & 1u) && (A.window <= 0 || row_depth[r] - depths[it & 1][lane] < A.window);
+                    else if (A.window > 0) seen[i] = seen[i] && key0 + lane > s.context + row_depth[r] - A.window;
+                    x[i] = seen[i] ? p_sm[r * LP + lane] * A.scale : -INFINITY;
+                    top[i] = x[i];
+                }
+#pragma unroll
+                for (int k = 16; k > 0; k >>= 1)
+#pragma unroll
+                    for (int i = 0; i < R; ++i) {                // (a score that is no number makes the row one)
+                        const float y = __shfl_xor_sync(0xffffffffu, top[i], k);
+                        top[i] = top[i] != top[i] || y != y ? NAN : fmaxf(top[i], y);
+                    }
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const float before = tops[warp * R + i];
+                    top[i] = before != before || top[i] != top[i] ? NAN : fmaxf(before, top[i]);
+                    x[i] = seen[i] ? expf(x[i] - top[i]) : 0.f;  // (a row that sees a key has a largest score)
+                    sum[i] = x[i];
+                    p_sm[(warp * R + i) * LP + lane] = x[i];
+                }
+#pragma unroll
+                for (int k = 16; k > 0; k >>= 1)
+#pragma unroll
+                    for (int i = 0; i < R; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], k);
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const int r = warp * R + i;
+                    const unsigned mask = __ballot_sync(0xffffffffu, seen[i]);
+                    const float before = tops[r];
+                    __syncwarp();
+                    if (lane == 0) {
+                        const float f = before == -INFINITY ? 0.f : expf(before - top[i]);
+                        corr[r] = f;
+                        sums[r] = sums[r] * f + sum[i];
+                        tops[r] = top[i];
+                        seen_of[r] = mask;
+                    }
                 }
             }
-        }
-        const T* k = drafted ? (const T*)A.k_new + (size_t)(first + j) * A.k_stride + (size_t)g * A.d : (const T*)A.k_cache + row;
-        const T* v = drafted ? (const T*)A.v_new + (size_t)(first + j) * A.v_stride + (size_t)g * A.d : (const T*)A.v_cache + row;
-        float s = -INFINITY;
-        if (seen) {
-            s = 0.f;
-            for (int c = 0; c < A.d; ++c) s = fmaf(qs[c], to_f32<T>(k[c]), s);
-            s *= A.scale;
-        }
-        const unsigned live = __ballot_sync(0xffffffffu, seen);
-        if (!live) continue;
-        const float top = fmaxf(m, warp_max(s)), base = top == -INFINITY ? 0.f : top;
-        const float p = seen ? expf(s - base) : 0.f, corr = expf(m - base);
-        l = l * corr + warp_sum(p);
-        m = top;
+            __syncthreads();
 #pragma unroll
-        for (int i = 0; i < CH; ++i) o[i] *= corr;
-        for (unsigned left = live; left; left &= left - 1) {
-            const int who = __ffs(left) - 1;
-            const float w = __shfl_sync(0xffffffffu, p, who);
-            const T* vr = (const T*)__shfl_sync(0xffffffffu, (unsigned long long)v, who);
+            for (int r = 0; r < 4; ++r) {
+                const float f = corr[o_row + r];
 #pragma unroll
-            for (int i = 0; i < CH; ++i)
-                if (lane + 32 * i < A.d) o[i] = fmaf(w, to_f32<T>(vr[lane + 32 * i]), o[i]);
+                for (int j = 0; j < CJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[r][j][e] *= f;
+            }
+            if (!some_odd) {
+#pragma unroll 2
+                for (int key = 0; key < KT; key += 4) {
+                    float4 p[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p[r] = *reinterpret_cast<const float4*>(p_sm + (o_row + r) * LP + key);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+#pragma unroll
+                        for (int j = 0; j < CJ; ++j) {
+                            const float4 v = *reinterpret_cast<const float4*>(v_sm + (key + y) * DP + o_col + 64 * j);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float w = y == 0 ? p[r].x : y == 1 ? p[r].y : y == 2 ? p[r].z : p[r].w;
+                                o[r][j][0] = fmaf(w, v.x, o[r][j][0]);
+                                o[r][j][1] = fmaf(w, v.y, o[r][j][1]);
+                                o[r][j][2] = fmaf(w, v.z, o[r][j][2]);
+                                o[r][j][3] = fmaf(w, v.w, o[r][j][3]);
+                            }
+                        }
+                }
+            } else {
+                for (int key = 0; key < KT; ++key)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (!(seen_of[o_row + r] >> key & 1u)) continue;
+                        const float w = p_sm[(o_row + r) * LP + key];
+#pragma unroll
+                        for (int j = 0; j < CJ; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[r][j][e] = fmaf(w, v_sm[key * DP + o_col + 64 * j + e], o[r][j][e]);
+                    }
+            }
+        }
+        __syncthreads();
+        const int which = w.i0 > 0 ? 0 : 1;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = row0 + o_row + r;
+            if (o_row + r >= rows) continue;
+            const float sum = sums[o_row + r], inv = whole ? (sum > 0.f || sum != sum ? 1.f / sum : 0.f) : 1.f;
+            const size_t part = part_row(line, blockIdx.x, which, o_row + r);
+            T* out = (T*)A.out + (size_t)(s.first + row / G) * A.out_stride + (size_t)(w.g * G + row % G) * A.d;
+#pragma unroll
+            for (int j = 0; j < CJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int c = o_col + 64 * j + e;
+                    if (c >= A.d) continue;
+                    if (whole) out[c] = from_f32<T>(o[r][j][e] * inv);
+                    else line.part_o[part * A.d + c] = o[r][j][e];
+                }
+        }
+        if (!whole) {
+            if (tid < rows) {
+                float* ml = line.part_ml + part_row(line, blockIdx.x, which, tid) * 2;
+                ml[0] = tops[tid];
+                ml[1] = sums[tid];
+            }
+            if (tid == 0) {
+                int from;
+                const int parts = job_parts(w, from);
+                int* job = line.shared_jobs + (blockIdx.x * 2 + which) * 8;
+                job[0] = parts;
+                job[1] = from;
+                job[2] = row0;
+                job[3] = rows;
+                job[4] = w.g;
+                job[5] = s.first;
+            }
+            told_of |= 1 << which;
+        }
+        __syncthreads();                           // what the next job writes has been read
+    }
+    if (tid < 2 && !(told_of >> tid & 1)) line.shared_jobs[(blockIdx.x * 2 + tid) * 8] = 0;
+}
+
+// Joins the parts of a job that several blocks shared, in their order: with M the largest of their maxima,
+// out = sum_i e^(m_i - M) O_i / sum_i e^(m_i - M) l_i.  A block per part, which takes as many of the job's rows; a warp per row.
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+tree_join_kernel(const TreeArgs A, const Line line) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int* job = line.shared_jobs + blockIdx.x * 8;
+    const int parts = job[0], c_first = job[1], row0 = job[2], rows = job[3], g = job[4], first = job[5];
+    if (parts < 2) return;
+    const int mine = (int)blockIdx.x / 2 - c_first, G = A.nh / A.nkv, lane = threadIdx.x & 31;
+    for (int r = rows * mine / parts + (int)(threadIdx.x >> 5); r < rows * (mine + 1) / parts; r += THREADS / 32) {
+        auto at = [&](int i) { return part_row(line, c_first + i, i > 0 ? 0 : 1, r); };
+        float M = -INFINITY, W = 0.f;
+        for (int i = lane; i < parts; i += 32) M = fmaxf(M, __ldcg(line.part_ml + at(i) * 2));
+        M = warp_max(M);
+        if (M == -INFINITY) M = 0.f;
+        for (int i = lane; i < parts; i += 32) W = fmaf(expf(__ldcg(line.part_ml + at(i) * 2) - M), __ldcg(line.part_ml + at(i) * 2 + 1), W);
+        W = warp_sum(W);
+        const float inv = W > 0.f || W != W ? 1.f / W : 0.f;
+        T* out = (T*)A.out + (size_t)(first + (row0 + r) / G) * A.out_stride + (size_t)(g * G + (row0 + r) % G) * A.d;
+        for (int c = lane; c < A.d; c += 32) {
+            float acc = 0.f;
+#pragma unroll 4
+            for (int i = 0; i < parts; ++i) acc = fmaf(expf(__ldcg(line.part_ml + at(i) * 2) - M), __ldcg(line.part_o + at(i) * A.d + c), acc);
+            out[c] = from_f32<T>(acc * inv);
         }
     }
-    const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int i = 0; i < CH; ++i)
-        if (lane + 32 * i < A.d) out[lane + 32 * i] = from_f32<T>(o[i] * inv);
+}
+
+long long scratch_floats(int d) { return line_floats(LINE_BLOCKS, RT, d, 0); }
+
+template <typename T, int DP>
+int launch_dp(const TreeArgs& A, const Line& line, cudaStream_t stream) {
+    constexpr int smem = 4 * (RT * (DP + 4) + KT * (DP + 4) + KT * DP + RT * (KT + 4));
+    const cudaError_t room = cudaFuncSetAttribute(tree_attention_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (room != cudaSuccess) return (int)room;
+    const int rc = xb_launch(tree_attention_kernel<T, DP>, dim3(LINE_BLOCKS), dim3(THREADS), smem, stream, A, line);
+    if (rc) return rc;
+    return xb_launch(tree_join_kernel<T>, dim3(2 * LINE_BLOCKS), dim3(THREADS), 0, stream, A, line);
 }
 
 template <typename T>
-int launch(const TreeArgs& A, cudaStream_t stream) {
-    const unsigned blocks = (unsigned)(((long long)A.tokens * A.nh + WARPS - 1) / WARPS);
-    const size_t smem = (size_t)WARPS * A.d * 4;
-    if (A.d <= 64) tree_attention_kernel<T, 2><<<blocks, WARPS * 32, smem, stream>>>(A);
-    else if (A.d <= 128) tree_attention_kernel<T, 4><<<blocks, WARPS * 32, smem, stream>>>(A);
-    else tree_attention_kernel<T, 16><<<blocks, WARPS * 32, smem, stream>>>(A);
-    return xb_launch_status();
+int launch(const TreeArgs& A, float* scratch, cudaStream_t stream) {
+    Line line;
+    line.two_from = A.tokens;
+    line.row_mul = A.nh / A.nkv;
+    line.row_div = RT;
+    line.part_rows = RT;
+    lay_out(line, LINE_BLOCKS, A.d, scratch);
+    if (A.d <= 64) return launch_dp<T, 64>(A, line, stream);
+    if (A.d <= 128) return launch_dp<T, 128>(A, line, stream);
+    if (A.d <= 256) return launch_dp<T, 256>(A, line, stream);
+    return launch_dp<T, 512>(A, line, stream);
 }
 
 }  // namespace
@@ -111,12 +362,14 @@ XB_EXPORT int xb_tree_attention(int dtype, void* out, const void* q, const void*
     if (requests > LINE_REQUESTS || d < 1 || d > 512 || nkv < 1 || nh % nkv || page_size < 1 || (window > 0 && !depth)) return (int)cudaErrorInvalidValue;
     const TreeArgs A{out, q, k_new, v_new, k_cache, v_cache, context, token_start, ancestors, depth, block_table, out_stride, q_stride, k_stride, v_stride,
                      tokens, requests, words, table_stride, nh, nkv, d, page_size, num_pages, window, scale, err};
-    if (dtype == XB_BF16 && scratch && ((uintptr_t)scratch & 15) == 0 && tree_tc_takes(A)) return tree_tc_launch(A, scratch, stream);
-    return dtype == XB_F32 ? launch<float>(A, stream) : launch<__nv_bfloat16>(A, stream);
+    if (!scratch || ((uintptr_t)scratch & 15)) return (int)cudaErrorInvalidValue;
+    if (dtype == XB_BF16 && tree_tc_takes(A)) return tree_tc_launch(A, scratch, stream);
+    return dtype == XB_F32 ? launch<float>(A, scratch, stream) : launch<__nv_bfloat16>(A, scratch, stream);
 }
 
-// float32 numbers of scratch for a step of `tokens` drafted tokens (0: none is used)
+// float32 numbers of scratch, on a 16-byte boundary, for a step of `tokens` drafted tokens: enough for either kernel
 XB_EXPORT long long xb_tree_attention_scratch(int dtype, int tokens, int nh, int nkv, int d) {
-    if (dtype != XB_BF16 || tokens <= 0 || nkv <= 0 || nh < nkv) return 0;
-    return line_floats(tokens, nh, nkv, d);
+    if (tokens <= 0 || nkv <= 0 || nh < nkv || d < 1) return 4;
+    const long long any = scratch_floats(d), tc = dtype == XB_BF16 ? tree_tc_scratch(tokens, nh, nkv, d) : 0;
+    return any > tc ? any : tc;
 }

@@ -46,26 +46,25 @@ __device__ __forceinline__ int request_of(const TreeArgs& A, int t) {
 }
 
 // ---- the line of all jobs' tiles -------------------------------------------------------------------------------------------
-// A job is (request, key/value head, up to job_nodes nodes); its tiles of KT keys are the cached ones from the first that a node sees
-// and the drafted ones.  The line holds all jobs' tiles, request by request, each as long as it costs: block c takes the tiles that begin
-// in c * share .. (c + 1) * share - 1.
-constexpr int KT = 64;
-constexpr int LINE_BLOCKS = 148;   // a block per SM
+// A job is (request, key/value head, some of the rows that a node and a query head of the group make); its tiles of KT keys are the cached
+// ones from the first that a node sees and the drafted ones.  The line holds all jobs' tiles, request by request, each as long as it
+// costs: block c takes the tiles that begin in c * share .. (c + 1) * share - 1, whatever the lengths are, so that blocks finish together and
+// nobody has to know the lengths on the host.
 constexpr int LINE_REQUESTS = 8192;
-constexpr int MIN_SHARE = 4;       // tiles that a block takes at least: below that its start and the join cost more than they save
-constexpr int TILE_ROWS = 128;     // rows (node, query head of the group) of a product; a job has up to two such tiles
 constexpr int COST_ONE = 2;        // what a tile of keys costs a job of one tile of rows, and of two: 1,400 and 2,150 cycles measured
 constexpr int COST_TWO = 3;
 constexpr int COST_JOB = 8;        // what a job costs beside its tiles: its last, drafted keys and its result
+constexpr int MIN_SHARE = 4;       // tiles that a block takes at least: below that its start and the join cost more than they save
 
 struct Line {
-    int half_nodes, job_nodes;     // nodes of a tile of rows and of a job
-    int part_rows;                 // rows of a part that is kept for the join: a multiple of 8
-    float* part_o;                 // [blocks][2][part_rows / 8][d / 4][8][4]: a block's first segment, if its job began before it, and its last,
-                                   // if its job goes on; four channels of eight rows lie together, as a warp writes and reads them
+    int row_mul, row_div;          // a request's jobs of a head: nodes * row_mul / row_div, upwards
+    int two_from;                  // jobs of more nodes have two tiles of rows
+    int part_rows;                 // rows of a part that is kept for the join
+    float* part_o;                 // [blocks][2][part_rows][d]: a block's first segment, if its job began before it, and its last, if its job
+                                   // goes on; how rows and channels lie is each kernel's own
     float* part_ml;                // [blocks][2][part_rows][2]: maximum and sum
-    int* shared_jobs;              // [blocks][2][8]: the jobs of these parts: parts (0: there is no such part), block of the first, first node's
-                                   // row, nodes, key/value head
+    int* shared_jobs;              // [blocks][2][8]: the jobs of these parts: parts (0: there is no such part), block of the first, first row
+                                   // or node, rows or nodes, key/value head, request
     float* dense;                  // room for q, k_new and v_new as dense rows of bfloat16
 };
 
@@ -76,6 +75,7 @@ struct RequestLine {
     __device__ __forceinline__ int units(int nkv) const { return nkv * pieces * job_units(); }
 };
 
+template <int KT>
 __device__ __forceinline__ RequestLine request_line(const TreeArgs& A, const Line& line, int b) {
     RequestLine r;
     r.first = clamp_start(A, A.token_start[b]);
@@ -84,8 +84,8 @@ __device__ __forceinline__ RequestLine request_line(const TreeArgs& A, const Lin
     r.tile0 = A.window > 0 ? max(0, r.context - A.window + 1) / KT : 0;    // (the root's window begins first)
     r.old_tiles = max(0, (r.context + KT - 1) / KT - r.tile0);
     r.tiles = r.old_tiles + (r.nodes + KT - 1) / KT;
-    r.pieces = (r.nodes + line.job_nodes - 1) / line.job_nodes;
-    r.per_tile = r.nodes > line.half_nodes ? COST_TWO : COST_ONE;
+    r.pieces = (r.nodes * line.row_mul + line.row_div - 1) / line.row_div;
+    r.per_tile = r.nodes > line.two_from ? COST_TWO : COST_ONE;
     return r;
 }
 
@@ -101,13 +101,14 @@ struct Walk {
 __device__ __forceinline__ int tiles_of_cost(int x, int cost) { return cost == COST_TWO ? (x + COST_TWO - 1) / COST_TWO : (x + COST_ONE - 1) / COST_ONE; }
 
 // The block's place before its first job: every lane sums a run of the requests.
+template <int KT>
 __device__ __forceinline__ Walk place_in_line(const TreeArgs& A, const Line& line) {
     const int lane = threadIdx.x & 31, each = (A.requests + 31) / 32, b0 = lane * each, b1 = min(b0 + each, A.requests);
     Walk w;
     int mine = 0;
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
-        w.r = request_line(A, line, b);
+        w.r = request_line<KT>(A, line, b);
         mine += w.r.units(A.nkv);
     }
     int incl = mine;
@@ -117,7 +118,7 @@ __device__ __forceinline__ Walk place_in_line(const TreeArgs& A, const Line& lin
         if (lane >= o) incl += v;
     }
     const int total = __shfl_sync(0xffffffffu, incl, 31);
-    w.share = max(MIN_SHARE * COST_TWO, (total + LINE_BLOCKS - 1) / LINE_BLOCKS);
+    w.share = max(MIN_SHARE * COST_TWO, (total + (int)gridDim.x - 1) / (int)gridDim.x);
     w.from = (int)min((long long)blockIdx.x * w.share, (long long)total);
     w.end = min(total, w.from + w.share);
     w.job = w.end;
@@ -129,7 +130,7 @@ __device__ __forceinline__ Walk place_in_line(const TreeArgs& A, const Line& lin
     if (lane == owner) {
 #pragma unroll 1
         for (; b < b1; ++b) {
-            if (each > 1) w.r = request_line(A, line, b);
+            if (each > 1) w.r = request_line<KT>(A, line, b);
             const int n = w.r.units(A.nkv);
             if (w.from < before + n) break;
             before += n;
@@ -137,7 +138,7 @@ __device__ __forceinline__ Walk place_in_line(const TreeArgs& A, const Line& lin
     }
     w.b = __shfl_sync(0xffffffffu, b, owner);
     before = __shfl_sync(0xffffffffu, before, owner);
-    w.r = request_line(A, line, w.b);
+    w.r = request_line<KT>(A, line, w.b);
     const int length = w.r.job_units(), at = (w.from - before) / length;
     w.g = at / w.r.pieces;
     w.piece = at % w.r.pieces;
@@ -147,6 +148,7 @@ __device__ __forceinline__ Walk place_in_line(const TreeArgs& A, const Line& lin
 
 // The next job of which the block has a part; false: there is none.  (The first tile that begins at or behind `from` may be the next
 // job's, or the next request's first.)
+template <int KT>
 __device__ __forceinline__ bool next_segment(const TreeArgs& A, const Line& line, Walk& w, bool first) {
     for (;; first = false) {
         if (!first) w.job += w.r.job_units();
@@ -157,7 +159,7 @@ __device__ __forceinline__ bool next_segment(const TreeArgs& A, const Line& line
                 w.g = 0;
                 do {
                     if (++w.b >= A.requests) return false;
-                    w.r = request_line(A, line, w.b);
+                    w.r = request_line<KT>(A, line, w.b);
                 } while (w.r.nodes == 0);                          // (a request without nodes has no jobs)
             }
         }
@@ -167,33 +169,26 @@ __device__ __forceinline__ bool next_segment(const TreeArgs& A, const Line& line
     }
 }
 
-__device__ __forceinline__ size_t part_row(const Line& line, int block, int which, int row) { return ((size_t)block * 2 + which) * line.part_rows + row; }
-// where four channels of a part's row lie, in float4
-__device__ __forceinline__ size_t part_four(const Line& line, int d, size_t row, int c4) { return ((row >> 3) * (d >> 2) + c4) * 8 + (row & 7); }
+// In how many blocks the job's tiles begin, and the first of them.
+__device__ __forceinline__ int job_parts(const Walk& w, int& first) {
+    first = w.job / w.share;
+    return (w.job + (w.r.tiles - 1) * w.r.per_tile) / w.share - first + 1;
+}
 
-// host: the scratch in float32 numbers, and its layout (every part is a multiple of 4 numbers long)
-inline int line_part_rows(int tokens, int group) {
-    const int nodes = 2 * (TILE_ROWS / (group < TILE_ROWS ? group : TILE_ROWS));
-    return ((tokens < nodes ? tokens : nodes) * group + 7) / 8 * 8;
-}
-inline long long line_floats(int tokens, int nh, int nkv, int d) {
-    return (long long)LINE_BLOCKS * (2 * line_part_rows(tokens, nh / nkv) * (long long)(d + 2) + 16) + ((long long)tokens * (nh + 2 * nkv) * d + 1) / 2;
-}
-inline Line make_line(const TreeArgs& A, float* scratch) {
-    const int G = A.nh / A.nkv;
-    Line line;
-    line.half_nodes = TILE_ROWS / G;
-    line.job_nodes = 2 * line.half_nodes;
-    line.part_rows = line_part_rows(A.tokens, G);
+__device__ __forceinline__ size_t part_row(const Line& line, int block, int which, int row) { return ((size_t)block * 2 + which) * line.part_rows + row; }
+
+// host: the layout of a line's scratch, in float32 numbers (every part is a multiple of 4 numbers long)
+inline long long line_floats(int blocks, int part_rows, int d, long long dense) { return (long long)blocks * 2 * (part_rows * (long long)(d + 2) + 8) + dense; }
+inline void lay_out(Line& line, int blocks, int d, float* scratch) {
     line.part_o = scratch;
-    line.part_ml = scratch + (size_t)LINE_BLOCKS * 2 * line.part_rows * A.d;
-    line.shared_jobs = reinterpret_cast<int*>(line.part_ml + (size_t)LINE_BLOCKS * 2 * line.part_rows * 2);
-    line.dense = reinterpret_cast<float*>(line.shared_jobs) + LINE_BLOCKS * 16;
-    return line;
+    line.part_ml = scratch + (size_t)blocks * 2 * line.part_rows * d;
+    line.shared_jobs = reinterpret_cast<int*>(line.part_ml + (size_t)blocks * 2 * line.part_rows * 2);
+    line.dense = reinterpret_cast<float*>(line.shared_jobs) + (size_t)blocks * 16;
 }
 
 // tree_attention_tc.cu
 bool tree_tc_takes(const TreeArgs& A);
+long long tree_tc_scratch(int tokens, int nh, int nkv, int d);
 int tree_tc_launch(const TreeArgs& A, float* scratch, cudaStream_t stream);
 
 }  // namespace xbtree

@@ -5,10 +5,9 @@
 // ones first, then the drafted ones, with a running maximum and sum per row (one thread a row) and O in tensor memory.
 // Which rows see a drafted key is a bit per key: the row's words of ancestors.
 //
-// The tiles of all jobs, in order of the requests, are one line that is cut into equal shares, one per block: blocks finish together
-// whatever the lengths are, and nobody has to know the lengths on the host.  A job that several blocks share leaves an unnormalised O with
-// its maximum and sum per block; tree_merge_kernel joins them in their order.  Every block forms the line for itself, from two numbers
-// per request.
+// The tiles of all jobs are one line that is cut into equal shares, one per block (tree_attention.cuh).  A job that several blocks share
+// leaves an unnormalised O with its maximum and sum per block; tree_merge_kernel joins them in their order.  One warp of a block forms the
+// line, from three numbers per request, and tells the others of the block's parts of jobs.
 //
 // Per tile: S = Q K^T by warp 9, P = 2^(S - m) by warps 0..3 (first row tile) and 4..7 (second), in the tensor memory of S, O += P V by
 // warp 11; warps 8 and 10 fetch keys and values, by page boxes from the cache and by boxes of 64 rows from the drafted rows.
@@ -27,7 +26,9 @@ namespace {
 using namespace xbtc;
 using namespace xbtree;
 
-constexpr int RT = TILE_ROWS;              // rows of a tile
+constexpr int RT = 128;                    // rows of a tile
+constexpr int KT = 64;                     // keys of a tile
+constexpr int LINE_BLOCKS = 148;           // a block per SM
 constexpr float RESCALE_STEP = 8.f;        // a row's maximum moves only when it grows by more than 2^8
 constexpr int THREADS = 384;
 __host__ __device__ constexpr int stages(int dp) { return dp <= 64 ? 8 : 4; }
@@ -49,6 +50,9 @@ __device__ __forceinline__ void store8(__nv_bfloat16* dst, const uint4& v, bool 
         for (int i = 0; i < 8; ++i) reinterpret_cast<uint16_t*>(dst)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
     }
 }
+
+// where four channels of a part's row lie, in float4: those of eight rows together, as a warp writes and reads them
+__device__ __forceinline__ size_t part_four(const Line& line, int d, size_t row, int c4) { return ((row >> 3) * (d >> 2) + c4) * 8 + (row & 7); }
 
 // One lane of the warp, chosen by the hardware.
 __device__ __forceinline__ uint32_t elected() {
@@ -143,7 +147,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     volatile uint32_t* odd_rows = words + 2;                                                                                // that are not finite: [4][warp][2]
     Segment* const segments = reinterpret_cast<Segment*>(smem_raw + SEG_OFF);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int G = A.nh / A.nkv, half_nodes = line.half_nodes;
+    const int G = A.nh / A.nkv, half_nodes = line.two_from;
     int* const err = A.err;
 
     Walk w;
@@ -152,7 +156,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         pdl_wait();                // lengths, rows and masks may come from the kernel before
         if (base & 1023u) atomicOr(err, XB_ERR_WAIT);                                  // the swizzle needs a 1024-byte aligned window
         const int word = lane == 0 ? *reinterpret_cast<volatile int*>(err) : 0;        // or an earlier block gave up: do not pile on
-        w = place_in_line(A, line);
+        w = place_in_line<KT>(A, line);
         gave_up = __any_sync(0xffffffffu, word & XB_ERR_WAIT);
     } else {
         if (threadIdx.x == 9 * 32) {
@@ -217,7 +221,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 s = read_segment();
                 if (!s.nodes) break;
             } else {
-                const bool more = next_segment(A, line, w, first);
+                const bool more = next_segment<KT>(A, line, w, first);
                 first = false;
                 if (more) {
                     const RequestLine& r = w.r;
@@ -228,8 +232,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     s.context = r.context;
                     s.tree = r.nodes;
                     s.first = r.first;
-                    s.node0 = w.piece * line.job_nodes;
-                    s.nodes = min(line.job_nodes, r.nodes - s.node0);
+                    s.node0 = w.piece * line.row_div;
+                    s.nodes = min(line.row_div, r.nodes - s.node0);
                     s.g = w.g;
                     s.b = w.b;
                     s.whole = w.i1 - w.i0 == r.tiles;
@@ -240,9 +244,11 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         s.deep_lo = r.context + __reduce_max_sync(0xffffffffu, deepest) - A.window + 1;
                     }
                     if (!s.whole && lane == 0) {       // what the join needs to know
-                        const int which = s.i0 > 0 ? 0 : 1, from = w.job / w.share, to = (w.job + (r.tiles - 1) * r.per_tile) / w.share;
+                        const int which = s.i0 > 0 ? 0 : 1;
+                        int from;
+                        const int parts = job_parts(w, from);
                         int4* job = reinterpret_cast<int4*>(line.shared_jobs + (blockIdx.x * 2 + which) * 8);
-                        job[0] = make_int4(to - from + 1, from, s.first + s.node0, s.nodes);
+                        job[0] = make_int4(parts, from, s.first + s.node0, s.nodes);
                         job[1].x = s.g;
                         told_of |= 1 << which;
                     }
@@ -867,7 +873,7 @@ int launch_tc(const TreeArgs& A, const Line& line, cudaStream_t stream) {
     const long long rows = (long long)A.num_pages * A.nkv * A.page_size;
     const long long dq[3] = {A.d, A.nh, A.tokens}, dn[3] = {A.d, A.nkv, A.tokens};
     const long long sq[2] = {A.d, A.q_stride}, sk[2] = {A.d, A.k_stride}, sv[2] = {A.d, A.v_stride};
-    const int bq[3] = {64, G, line.half_nodes}, bn[3] = {64, 1, KT};
+    const int bq[3] = {64, G, line.two_from}, bn[3] = {64, 1, KT};
     if (!tensor_map_bf16(&mq, A.q, 3, dq, sq, bq) || !tensor_map_2d(&mk, A.k_cache, rows, A.d, box_rows) || !tensor_map_2d(&mv, A.v_cache, rows, A.d, box_rows) ||
         !tensor_map_bf16(&mkn, A.k_new, 3, dn, sk, bn) || !tensor_map_bf16(&mvn, A.v_new, 3, dn, sv, bn))
         return (int)cudaErrorInvalidValue;
@@ -885,9 +891,23 @@ bool tree_tc_takes(const TreeArgs& A) {
            ((long long)A.num_pages + 1) * A.nkv * A.page_size < (1LL << 31) && rows_on_16_bytes(A.k_cache, 0) && rows_on_16_bytes(A.v_cache, 0);
 }
 
+static int part_rows_of(int tokens, int group) {
+    const int nodes = 2 * (RT / (group < RT ? group : RT));
+    return ((tokens < nodes ? tokens : nodes) * group + 7) / 8 * 8;
+}
+
+long long tree_tc_scratch(int tokens, int nh, int nkv, int d) {
+    return line_floats(LINE_BLOCKS, part_rows_of(tokens, nh / nkv), d, ((long long)tokens * (nh + 2 * nkv) * d + 1) / 2);
+}
+
 int tree_tc_launch(const TreeArgs& given, float* scratch, cudaStream_t stream) {
     TreeArgs A = given;
-    const Line line = make_line(A, scratch);
+    Line line;
+    line.two_from = RT / (A.nh / A.nkv);
+    line.row_mul = 1;
+    line.row_div = 2 * line.two_from;
+    line.part_rows = part_rows_of(A.tokens, A.nh / A.nkv);
+    lay_out(line, LINE_BLOCKS, A.d, scratch);
     if (!rows_on_16_bytes(A.q, A.q_stride) || !rows_on_16_bytes(A.k_new, A.k_stride) || !rows_on_16_bytes(A.v_new, A.v_stride)) {
         __nv_bfloat16* dense = reinterpret_cast<__nv_bfloat16*>(line.dense);
         const int rc = xb_launch(tree_dense_rows_kernel, dim3(A.tokens), dim3(256), 0, stream, dense, A);
