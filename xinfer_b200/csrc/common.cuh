@@ -109,6 +109,20 @@ __device__ __forceinline__ float gate_mul_any(int act, float g, float u, float p
 // Last CUDA error of a launch as an int for the caller (0 = ok).
 static inline int xb_launch_status() { return (int)cudaGetLastError(); }
 
+// Dynamic shared memory above the default, asked for once per kernel and device: `done` is a static word of the caller, a bit per device
+// (two threads that ask at once ask twice, which does no harm).
+template <typename... KArgs>
+static inline int xb_more_smem(void (*kernel)(KArgs...), int bytes, unsigned long long* done) {
+    int dev = 0;
+    cudaError_t rc = cudaGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (rc == cudaSuccess && !(*done & bit)) {
+        rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (rc == cudaSuccess) *done |= bit;
+    }
+    return (int)rc;
+}
+
 // Programmatic dependent launch: a kernel launched through xb_launch may be scheduled while the
 // kernel before it in the stream is still running; it calls pdl_wait() before it touches anything
 // that kernel may have written (or still reads), and pdl_launch_dependents() as early as it likes

@@ -323,11 +323,11 @@ logit_rules_kernel(const RuleArgs A) {
 template <int VECS>
 int launch(const RuleArgs& A, cudaStream_t stream) {
     const int smem = smem_of(VECS, A.words);
-    int per_sm = 0;
-    cudaError_t rc = cudaFuncSetAttribute(logit_rules_kernel<VECS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of(VECS, WORDS));
-    if (rc == cudaSuccess) rc = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, logit_rules_kernel<VECS>, THREADS, smem);
-    if (rc != cudaSuccess) return (int)rc;
-    const int resident = (per_sm > 0 ? per_sm : 1) * 148;          // blocks that the device holds
+    static unsigned long long roomy = 0;
+    if (const int rc = xb_more_smem(logit_rules_kernel<VECS>, smem_of(VECS, WORDS), &roomy)) return rc;
+    // as many blocks as the device holds: 228 KB of shared memory a processor, of which every block takes its own, the static arrays and 1 KB
+    const int per_sm = (228 * 1024) / (smem + (int)(ROWS * sizeof(RowFacts) + BIASES * sizeof(Bias)) + 1024);
+    const int resident = (per_sm < 1 ? 1 : (per_sm > 8 ? 8 : per_sm)) * 148;
     const long long units = (long long)((A.vocab + chunk_of(VECS) - 1) / chunk_of(VECS)) * A.rows;
     return xb_launch(logit_rules_kernel<VECS>, dim3((unsigned)(units < resident ? units : resident)), dim3(THREADS), smem, stream, A);
 }

@@ -13,7 +13,7 @@ using namespace xbtree;
 
 // The kernel for float32, and for what the tcgen05 kernel does not take (tree_attention_tc.cu): any head size, group and page.  A job's rows
 // are 32 (node, query head) pairs; a tile is 32 keys.  Scores are formed 2 rows x 4 keys a thread and values summed 4 rows x 4 channels at a
-// time, by float32 multiply-adds from shared memory; a warp forms the softmax of eight rows, a key per lane.  Jobs, tiles and the join are
+// time, by float32 multiply-adds from shared memory; four lanes form the softmax of a row, eight keys each.  Jobs, tiles and the join are
 // those of the line in tree_attention.cuh, four blocks to a processor.  Bound by the multiply-adds' operands from shared memory: a score
 // or value product reads two numbers of it for every three it forms.
 constexpr int RT = 32, KT = 32, THREADS = 128, LINE_BLOCKS = 4 * 148;
@@ -32,6 +32,12 @@ __device__ __forceinline__ float4 four_of(const __nv_bfloat16* row, int c, int d
     auto at = [&](int i) { return c + i < d ? __bfloat162float(row[c + i]) : 0.f; };
     return make_float4(at(0), at(1), at(2), at(3));
 }
+// The larger of two; one that is no number wins.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 __device__ __forceinline__ bool finite(const float4& v) {
     return fabsf(v.x) <= 3.402823466e38f && fabsf(v.y) <= 3.402823466e38f && fabsf(v.z) <= 3.402823466e38f && fabsf(v.w) <= 3.402823466e38f;
 }
@@ -49,10 +55,8 @@ tree_attention_kernel(const TreeArgs A, const Line line) {
     __shared__ Walk walk;
     __shared__ float corr[RT], sums[RT], tops[RT];
     __shared__ unsigned seen_of[RT];
-    // of this tile and the next: where the keys begin in their tensor (-1 nowhere), the keys' depths, the rows' ancestors among the keys
-    __shared__ long long rows_of[2][KT];
-    __shared__ int depths[2][KT], row_depth[RT];
-    __shared__ unsigned masks[2][RT];
+    __shared__ long long rows_of[2][KT];           // of this tile and the next: where the keys begin in their tensor (-1: nowhere)
+    __shared__ int depths[2][KT];                  // and their depths
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = A.nh / A.nkv;
@@ -91,29 +95,41 @@ tree_attention_kernel(const TreeArgs A, const Line line) {
         const int o_row = tid / 16 * 4, o_col = tid % 16 * 4;
         // a window's first key, of the root; keys before it are nobody's
         const int lo = A.window > 0 ? max(0, s.context - A.window + 1) : 0;
-        auto find_rows = [&](int it) {             // by the first warp, a key and a row to a lane
+        // What a tile needs to know, of its keys by the first warp, a key to a lane, and of a row by the row's lanes: asked for while another
+        // tile is worked on, then written down.
+        const int my_row = tid >> 2, my_t = s.first + (row0 + min(my_row, rows - 1)) / G;
+        const int my_depth = A.window > 0 ? max(0, A.depth[my_t]) : 0;
+        int asked_page = 0, asked_depth = 0;
+        unsigned asked_mask = 0;
+        auto first_key = [&](int it) { return (it >= s.old_tiles ? it - s.old_tiles : s.tile0 + it) * KT; };
+        auto ask = [&](int it) {
+            const int key = first_key(it) + lane;
             const bool drafted = it >= s.old_tiles;
-            const int key = (drafted ? it - s.old_tiles : s.tile0 + it) * KT + lane;
-            long long at = -1;
+            asked_mask = 0;
+            if (drafted && key / KT < A.words) asked_mask = (unsigned)A.ancestors[(size_t)my_t * A.words + key / KT];
+            if (warp > 0) return;
+            asked_page = asked_depth = 0;
             if (drafted) {
+                if (A.window > 0 && key < s.nodes) asked_depth = max(0, A.depth[s.first + key]);
+            } else if (key < s.context && key >= lo) {
+                asked_page = table[key / A.page_size];
+            }
+        };
+        auto write_down = [&](int it) {            // (the first warp)
+            const int key = first_key(it) + lane;
+            long long at = -1;
+            if (it >= s.old_tiles) {
                 if (key < s.nodes) at = s.first + key;
             } else if (key < s.context && key >= lo) {
-                const int page = table[key / A.page_size];
-                if (page >= 0 && page < A.num_pages) at = (((long long)page * A.nkv + w.g) * A.page_size + key % A.page_size) * A.d;
+                if (asked_page >= 0 && asked_page < A.num_pages) at = (((long long)asked_page * A.nkv + w.g) * A.page_size + key % A.page_size) * A.d;
                 else atomicOr(A.err, XB_ERR_BAD_PAGE);
             }
             rows_of[it & 1][lane] = at;
-            if (drafted) {
-                unsigned mask = 0;
-                if (lane < rows && (key >> 5) < A.words) mask = (unsigned)A.ancestors[(size_t)(s.first + (row0 + lane) / G) * A.words + (key >> 5)];
-                masks[it & 1][lane] = mask;
-                depths[it & 1][lane] = A.window > 0 && key < s.nodes ? max(0, A.depth[s.first + key]) : 0;
-            }
+            depths[it & 1][lane] = asked_depth;
         };
-        if (warp == 0) {
-            row_depth[lane] = A.window > 0 && lane < rows ? max(0, A.depth[s.first + (row0 + lane) / G]) : 0;
-            find_rows(w.i0);
-        }
+        ask(w.i0);
+        unsigned my_mask = asked_mask;
+        if (warp == 0) write_down(w.i0);
         for (int it = w.i0; it < w.i1; ++it) {
             const bool drafted = it >= s.old_tiles;
             const int key0 = drafted ? (it - s.old_tiles) * KT : (s.tile0 + it) * KT, keys = min(KT, (drafted ? s.nodes : s.context) - key0);
@@ -134,7 +150,7 @@ tree_attention_kernel(const TreeArgs A, const Line line) {
             }
             // a value that is not finite may be one that not all rows see: their weights of zero must not meet it
             const bool some_odd = __syncthreads_or(odd) && (drafted || A.window > 0);
-            if (warp == 0 && it + 1 < w.i1) find_rows(it + 1);
+            if (it + 1 < w.i1) ask(it + 1);
             {
                 const int r = tid / 8 * 2, j = tid % 8;
                 float sc[2][4] = {};
@@ -162,51 +178,54 @@ tree_attention_kernel(const TreeArgs A, const Line line) {
             }
             __syncthreads();
             {
-                // a warp has eight rows, side by side
-                constexpr int R = RT / (THREADS / 32);
-                float x[R], top[R], sum[R];
-                bool seen[R];
+                // which keys of the tile the row sees
+                unsigned m = keys < 32 ? (1u << keys) - 1u : 0xffffffffu;
+                if (my_row >= rows) m = 0;
+                const int q8 = (tid & 3) * 8;
+                if (drafted) {
+                    m &= my_mask;
+                    if (A.window > 0)
 #pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    const int r = warp * R + i;
-                    seen[i] = r < rows && lane < keys;
-                    if (drafted) seen[i] = seen[i] && (masks[it & 1][r] >> lane & 1u) && (A.window <= 0 || row_depth[r] - depths[it & 1][lane] < A.window);
-                    else if (A.window > 0) seen[i] = seen[i] && key0 + lane > s.context + row_depth[r] - A.window;
-                    x[i] = seen[i] ? p_sm[r * LP + lane] * A.scale : -INFINITY;
-                    top[i] = x[i];
+                        for (int i = 0; i < 8; ++i)
+                            if (my_depth - depths[it & 1][q8 + i] >= A.window) m &= ~(1u << (q8 + i));
+                } else if (A.window > 0) {
+                    const int from = s.context + my_depth - A.window + 1 - key0;
+                    if (from > 0) m = from < 32 ? m & (0xffffffffu << from) : 0u;
                 }
+                float* p = p_sm + my_row * LP + q8;
+                float x[8], top = -INFINITY;
+                *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+                *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + 4);
 #pragma unroll
-                for (int k = 16; k > 0; k >>= 1)
-#pragma unroll
-                    for (int i = 0; i < R; ++i) {                // (a score that is no number makes the row one)
-                        const float y = __shfl_xor_sync(0xffffffffu, top[i], k);
-                        top[i] = top[i] != top[i] || y != y ? NAN : fmaxf(top[i], y);
-                    }
-#pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    const float before = tops[warp * R + i];
-                    top[i] = before != before || top[i] != top[i] ? NAN : fmaxf(before, top[i]);
-                    x[i] = seen[i] ? expf(x[i] - top[i]) : 0.f;  // (a row that sees a key has a largest score)
-                    sum[i] = x[i];
-                    p_sm[(warp * R + i) * LP + lane] = x[i];
+                for (int i = 0; i < 8; ++i) {
+                    x[i] = m >> (q8 + i) & 1u ? x[i] * A.scale : -INFINITY;
+                    top = max_nan(top, x[i]);
                 }
+                const float before = tops[my_row];
+                top = max_nan(top, before);        // (a score that is no number makes the row one)
+                top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float base = top == -INFINITY ? 0.f : top;
+                float sum = 0.f;
 #pragma unroll
-                for (int k = 16; k > 0; k >>= 1)
-#pragma unroll
-                    for (int i = 0; i < R; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], k);
-#pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    const int r = warp * R + i;
-                    const unsigned mask = __ballot_sync(0xffffffffu, seen[i]);
-                    const float before = tops[r];
-                    __syncwarp();
-                    if (lane == 0) {
-                        const float f = before == -INFINITY ? 0.f : expf(before - top[i]);
-                        corr[r] = f;
-                        sums[r] = sums[r] * f + sum[i];
-                        tops[r] = top[i];
-                        seen_of[r] = mask;
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    x[i] = expf(x[i] - base);
+                    sum += x[i];
+                }
+                *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(x);
+                *reinterpret_cast<float4*>(p + 4) = *reinterpret_cast<const float4*>(x + 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                // (with a window the row's lanes have each looked at their own keys)
+                unsigned seen = m & 0xffu << q8;
+                seen |= __shfl_xor_sync(0xffffffffu, seen, 1);
+                seen |= __shfl_xor_sync(0xffffffffu, seen, 2);
+                if ((tid & 3) == 0) {
+                    const float f = expf(before - base);
+                    corr[my_row] = f;
+                    sums[my_row] = sums[my_row] * f + sum;
+                    tops[my_row] = top;
+                    seen_of[my_row] = seen;
                 }
             }
             __syncthreads();
@@ -218,6 +237,8 @@ tree_attention_kernel(const TreeArgs A, const Line line) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[r][j][e] *= f;
             }
+            my_mask = asked_mask;
+            if (warp == 0 && it + 1 < w.i1) write_down(it + 1);
             if (!some_odd) {
 #pragma unroll 2
                 for (int key = 0; key < KT; key += 4) {
@@ -296,10 +317,12 @@ tree_attention_kernel(const TreeArgs A, const Line line) {
 }
 
 // Joins the parts of a job that several blocks shared, in their order: with M the largest of their maxima,
-// out = sum_i e^(m_i - M) O_i / sum_i e^(m_i - M) l_i.  A block per part, which takes as many of the job's rows; a warp per row.
-template <typename T>
+// out = sum_i e^(m_i - M) O_i / sum_i e^(m_i - M) l_i.  A block per part, which takes as many of the job's rows; a warp per row, a part's factor
+// per lane, then the row's channels of eight parts at once.
+template <typename T, int DP>
 __global__ void __launch_bounds__(THREADS)
 tree_join_kernel(const TreeArgs A, const Line line) {
+    constexpr int C = DP / 32, P = C >= 8 ? 2 : 16 / C;
     pdl_launch_dependents();
     pdl_wait();
     const int* job = line.shared_jobs + blockIdx.x * 8;
@@ -308,20 +331,37 @@ tree_join_kernel(const TreeArgs A, const Line line) {
     const int mine = (int)blockIdx.x / 2 - c_first, G = A.nh / A.nkv, lane = threadIdx.x & 31;
     for (int r = rows * mine / parts + (int)(threadIdx.x >> 5); r < rows * (mine + 1) / parts; r += THREADS / 32) {
         auto at = [&](int i) { return part_row(line, c_first + i, i > 0 ? 0 : 1, r); };
-        float M = -INFINITY, W = 0.f;
+        float M = -INFINITY, W = 0.f, acc[C] = {};
         for (int i = lane; i < parts; i += 32) M = fmaxf(M, __ldcg(line.part_ml + at(i) * 2));
         M = warp_max(M);
         if (M == -INFINITY) M = 0.f;
-        for (int i = lane; i < parts; i += 32) W = fmaf(expf(__ldcg(line.part_ml + at(i) * 2) - M), __ldcg(line.part_ml + at(i) * 2 + 1), W);
+        for (int base = 0; base < parts; base += 32) {
+            float f = 0.f;
+            if (base + lane < parts) {
+                f = expf(__ldcg(line.part_ml + at(base + lane) * 2) - M);
+                W = fmaf(f, __ldcg(line.part_ml + at(base + lane) * 2 + 1), W);
+            }
+            for (int i0 = 0; i0 < min(32, parts - base); i0 += P) {
+                float v[P][C];
+#pragma unroll
+                for (int i = 0; i < P; ++i)
+#pragma unroll
+                    for (int k = 0; k < C; ++k)
+                        v[i][k] = base + i0 + i < parts && lane + 32 * k < A.d ? __ldcg(line.part_o + at(base + i0 + i) * A.d + lane + 32 * k) : 0.f;
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const float fi = __shfl_sync(0xffffffffu, f, (i0 + i) & 31);
+#pragma unroll
+                    for (int k = 0; k < C; ++k) acc[k] = fmaf(fi, v[i][k], acc[k]);
+                }
+            }
+        }
         W = warp_sum(W);
         const float inv = W > 0.f || W != W ? 1.f / W : 0.f;
         T* out = (T*)A.out + (size_t)(first + (row0 + r) / G) * A.out_stride + (size_t)(g * G + (row0 + r) % G) * A.d;
-        for (int c = lane; c < A.d; c += 32) {
-            float acc = 0.f;
-#pragma unroll 4
-            for (int i = 0; i < parts; ++i) acc = fmaf(expf(__ldcg(line.part_ml + at(i) * 2) - M), __ldcg(line.part_o + at(i) * A.d + c), acc);
-            out[c] = from_f32<T>(acc * inv);
-        }
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+            if (lane + 32 * k < A.d) out[lane + 32 * k] = from_f32<T>(acc[k] * inv);
     }
 }
 
@@ -330,17 +370,18 @@ long long scratch_floats(int d) { return line_floats(LINE_BLOCKS, RT, d, 0); }
 template <typename T, int DP>
 int launch_dp(const TreeArgs& A, const Line& line, cudaStream_t stream) {
     constexpr int smem = 4 * (RT * (DP + 4) + KT * (DP + 4) + KT * DP + RT * (KT + 4));
-    const cudaError_t room = cudaFuncSetAttribute(tree_attention_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (room != cudaSuccess) return (int)room;
+    static unsigned long long roomy = 0;
+    if (const int rc = xb_more_smem(tree_attention_kernel<T, DP>, smem, &roomy)) return rc;
     const int rc = xb_launch(tree_attention_kernel<T, DP>, dim3(LINE_BLOCKS), dim3(THREADS), smem, stream, A, line);
     if (rc) return rc;
-    return xb_launch(tree_join_kernel<T>, dim3(2 * LINE_BLOCKS), dim3(THREADS), 0, stream, A, line);
+    return xb_launch(tree_join_kernel<T, DP>, dim3(2 * LINE_BLOCKS), dim3(THREADS), 0, stream, A, line);
 }
 
 template <typename T>
 int launch(const TreeArgs& A, float* scratch, cudaStream_t stream) {
     Line line;
     line.two_from = A.tokens;
+    line.min_share = 3 * COST_ONE;
     line.row_mul = A.nh / A.nkv;
     line.row_div = RT;
     line.part_rows = RT;

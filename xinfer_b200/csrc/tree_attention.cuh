@@ -53,12 +53,12 @@ __device__ __forceinline__ int request_of(const TreeArgs& A, int t) {
 constexpr int LINE_REQUESTS = 8192;
 constexpr int COST_ONE = 2;        // what a tile of keys costs a job of one tile of rows, and of two: 1,400 and 2,150 cycles measured
 constexpr int COST_TWO = 3;
-constexpr int COST_JOB = 8;        // what a job costs beside its tiles: its last, drafted keys and its result
-constexpr int MIN_SHARE = 4;       // tiles that a block takes at least: below that its start and the join cost more than they save
+constexpr int COST_JOB = 12;       // what a job costs beside its tiles: its last, drafted keys and its result
 
 struct Line {
     int row_mul, row_div;          // a request's jobs of a head: nodes * row_mul / row_div, upwards
     int two_from;                  // jobs of more nodes have two tiles of rows
+    int min_share;                 // what a block takes at least: below that its start and the join cost more than they save
     int part_rows;                 // rows of a part that is kept for the join
     float* part_o;                 // [blocks][2][part_rows][d]: a block's first segment, if its job began before it, and its last, if its job
                                    // goes on; how rows and channels lie is each kernel's own
@@ -118,7 +118,7 @@ __device__ __forceinline__ Walk place_in_line(const TreeArgs& A, const Line& lin
         if (lane >= o) incl += v;
     }
     const int total = __shfl_sync(0xffffffffu, incl, 31);
-    w.share = max(MIN_SHARE * COST_TWO, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    w.share = max(line.min_share, (total + (int)gridDim.x - 1) / (int)gridDim.x);
     w.from = (int)min((long long)blockIdx.x * w.share, (long long)total);
     w.end = min(total, w.from + w.share);
     w.job = w.end;

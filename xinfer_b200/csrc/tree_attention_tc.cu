@@ -864,8 +864,8 @@ template <int DP>
 int launch_tc(const TreeArgs& A, const Line& line, cudaStream_t stream) {
     constexpr int NS = stages(DP);
     constexpr size_t smem = 2 * (DP / 64) * RT * 128 + NS * 2 * (DP / 64) * KT * 128 + 1024 + 8 * 2048 + 2048 + SEGMENTS * sizeof(Segment);
-    static const cudaError_t room = cudaFuncSetAttribute(tree_attention_tc_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (room != cudaSuccess) return (int)room;
+    static unsigned long long roomy = 0;
+    if (const int rc = xb_more_smem(tree_attention_tc_kernel<DP>, (int)smem, &roomy)) return rc;
     const int G = A.nh / A.nkv, box_rows = A.page_size < KT ? A.page_size : KT;
     int shift = 0;
     while ((1 << shift) < A.page_size) ++shift;
@@ -904,6 +904,7 @@ int tree_tc_launch(const TreeArgs& given, float* scratch, cudaStream_t stream) {
     TreeArgs A = given;
     Line line;
     line.two_from = RT / (A.nh / A.nkv);
+    line.min_share = 8;
     line.row_mul = 1;
     line.row_div = 2 * line.two_from;
     line.part_rows = part_rows_of(A.tokens, A.nh / A.nkv);

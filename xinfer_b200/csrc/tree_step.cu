@@ -234,8 +234,9 @@ XB_EXPORT int xb_cache_slots(long long* slots, int* positions, int* request, int
     int blocks = (capacity + SLOT_THREADS - 1) / SLOT_THREADS;
     blocks = blocks < 4 ? 4 : (blocks > 148 ? 148 : blocks);    // (four also where few tokens come: pages are given back beside them)
     const size_t smem = (3 * (size_t)requests + 1) * 4;
-    static const cudaError_t room = cudaFuncSetAttribute(cache_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * SLOT_REQUESTS + 1) * 4);
-    if (room != cudaSuccess) return (int)room;
+    static unsigned long long roomy = 0;
+    if (smem > 48 * 1024)
+        if (const int rc = xb_more_smem(cache_slots_kernel, (3 * SLOT_REQUESTS + 1) * 4, &roomy)) return rc;
     return xb_launch(cache_slots_kernel, dim3(blocks), dim3(SLOT_THREADS), smem, stream, A);
 }
 

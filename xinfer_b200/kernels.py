@@ -1765,13 +1765,14 @@ TREE_REQUESTS_MAX = SLOT_REQUESTS_MAX = 8192
 def _token_rows(t, name: str, dtype, tokens: int, heads: int, d: int) -> int:
     """Elements between the tokens of ``[tokens, heads, d]`` whose heads are dense; tokens may lie further apart."""
     try:
-        ok = t.is_cuda and t.dtype == dtype and t.shape == (tokens, heads, d)
+        if t.is_cuda and t.dtype == dtype and t.shape == (tokens, heads, d):
+            if t.is_contiguous():
+                return heads * d
+            st, sh, sd = t.stride()
+            if (sd == 1 or d == 1) and (sh == d or heads == 1) and (st >= heads * d or tokens <= 1):
+                return st if tokens > 1 else heads * d
     except AttributeError:
-        ok = False
-    if ok:
-        st, sh, sd = t.stride()
-        if (sd == 1 or d == 1) and (sh == d or heads == 1) and (st >= heads * d or tokens <= 1):
-            return st if tokens > 1 else heads * d
+        pass
     if not isinstance(t, torch.Tensor):
         raise KernelError(f"{name}: expected a tensor, got {type(t).__name__}")
     raise KernelError(f"{name}: expected a {dtype} CUDA tensor of shape {(tokens, heads, d)} with dense heads, got {t.dtype} {tuple(t.shape)} "
