@@ -2,7 +2,8 @@
 
 Public entry points, in the manner of the reference's Python package (xinfer.pyi):
 ``Engine(EngineConfig, dtype)`` with ``generate_sync`` / ``generate_stream``, ``SamplingParams``,
-``GenerationOutput``; plus ``ModelRunner.step`` for callers that drive steps themselves.
+``GenerationOutput``; plus ``ModelRunner.step`` for callers that drive steps themselves, and ``TreeDecoder`` for decoding
+that verifies drafted tokens.
 """
 from .config import EngineConfig, GenerationConfig, Qwen3Config, ConfigError, register_architecture
 
@@ -17,6 +18,9 @@ def __getattr__(name):
     if name == "SamplingParams":
         from .sampling import SamplingParams
         return SamplingParams
+    if name in ("TreeDecoder", "LogitRules", "lookup_draft"):
+        from .engine import tree_decode
+        return getattr(tree_decode, name)
     if name in ("ModelRunner", "StepInput", "StepError"):
         from .engine import runner
         return getattr(runner, name)
@@ -24,4 +28,5 @@ def __getattr__(name):
 
 
 __all__ = ["EngineConfig", "GenerationConfig", "Qwen3Config", "ConfigError", "register_architecture", "Engine",
-           "GenerationOutput", "StreamItem", "SamplingParams", "ModelRunner", "StepInput", "StepError"]
+           "GenerationOutput", "StreamItem", "SamplingParams", "ModelRunner", "StepInput", "StepError", "TreeDecoder",
+           "LogitRules", "lookup_draft"]

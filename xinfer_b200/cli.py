@@ -3,6 +3,7 @@ src/server/mod.rs:706-904): the same names and meanings where the reference has 
 
     python -m xinfer_b200 --m DIR --prompts "1,2,3|4,5,6" --max-tokens 32
     python -m xinfer_b200 --m DIR --batch 8 --prompt-len 128 --max-tokens 64 --ignore-eos
+    python -m xinfer_b200 --m DIR --prompts "1,2,3" --max-tokens 32 --draft-nodes 16      (verify drafted trees)
     python -m xinfer_b200 --random CONFIG.json --seed 0 --m DIR      (write a random-weight folder)
 
 Prompts are token ids (``|`` between prompts as in the reference, ``,`` between ids); with
@@ -49,6 +50,9 @@ def build_parser() -> argparse.ArgumentParser:
                     help="debug: fill every cache page that is given back with NaN before the next step")
     ap.add_argument("--disable-run-ahead", action="store_true",
                     help="wait for every step's tokens before the next step is decided")
+    ap.add_argument("--draft-nodes", type=int, metavar="N",
+                    help="decode with trees of up to N tokens per request and step, drafted from the text so far (all prompts at once)")
+    ap.add_argument("--repetition-penalty", type=float, help="with --draft-nodes: divides or multiplies the logits of tokens seen before")
     ap.add_argument("--random", metavar="CONFIG_JSON", help="write a random-weight model folder to --m from this config and --seed, then exit")
     ap.add_argument("--store-dtype", default="bf16", help="dtype of the tensors --random writes (bf16 or f32)")
     return ap
@@ -117,6 +121,21 @@ def main(argv: Optional[List[str]] = None) -> int:
     engine = Engine(econfig, args.dtype)
     print(f"model loaded in {time.time() - t0:.1f} s; cache holds {engine.runner.kv_cache_tokens()} tokens", file=sys.stderr)
     params = SamplingParams(max_tokens=args.max_tokens, ignore_eos=args.ignore_eos)
+    if args.draft_nodes:
+        from . import LogitRules, TreeDecoder
+        params.seed = args.seed
+        if engine.generation_cfg is not None:
+            params = engine.generation_cfg.fill(params)
+        decoder = TreeDecoder(engine.runner, max_nodes=args.draft_nodes, eos_token_ids=engine.eos_token_ids)
+        t0 = time.time()
+        texts = decoder.generate(prompts, params, rules=LogitRules(args.repetition_penalty or 1.0))
+        for i, (p, t) in enumerate(zip(prompts, texts)):
+            print(f"[seq {i}] prompt {len(p)} tokens -> {len(t)} tokens: " + ",".join(str(x) for x in t))
+        print(f"{sum(len(t) for t in texts)} tokens in {decoder.steps} steps and {time.time() - t0:.2f}s; "
+              f"{decoder.confirmed} of {decoder.drafted} drafted tokens confirmed")
+        return 0
+    if args.repetition_penalty:
+        raise SystemExit("--repetition-penalty goes with --draft-nodes")
     outs = engine.generate_sync(params, prompts)
     for o in outs:
         print(f"[seq {o.seq_id}] prompt {o.prompt_length} tokens -> {o.decoded_length} tokens ({o.finish_reason}): "

@@ -306,7 +306,7 @@ __global__ void qk_norm_rope_write_kernel(
     long long kv_row = -1;
     if (write_kv && req_of_token[t] >= 0) {  // request -1 marks a padding token
         const int b = req_of_token[t];
-        const int page = block_table[(size_t)b * table_stride + pos / page_size];
+        const int page = write_kv == 2 ? t : block_table[(size_t)b * table_stride + pos / page_size];    // 2: rows [tokens, nkv, d], pages of one slot
         if (page < 0 || page >= num_pages) {
             if (threadIdx.x == 0) atomicOr(err, XB_ERR_BAD_PAGE);
         } else {

@@ -41,10 +41,10 @@ struct QkArgs {
     const float* sin_t;
     const int* positions;          // [tokens]
     const int* req_of_token;       // [tokens]; < 0: padding, nothing is cached
-    const int* block_table;        // [requests, table_stride]
+    const int* block_table;        // [requests, table_stride]; not read where rows are written
     int table_stride, nh, nkv, d, rot, interleaved, page_size, num_pages, max_pos;
     float eps;
-    int write_kv;
+    int write_kv;                  // 0: keys and values are not written; 1: to their pages; 2: to row t of [tokens, nkv, d] (pages of one slot)
 };
 
 // What a lane needs beside the values: fetched from what the host sent before the step's first
@@ -69,7 +69,7 @@ __device__ __forceinline__ QkItem qk_prepare(const QkArgs& A, int t, int h, int 
         if (is_q) {
             it.dst = A.q_out + ((size_t)t * A.nh + h) * A.d;
         } else if (A.write_kv && A.req_of_token[t] >= 0) {
-            const int page = A.block_table[(size_t)A.req_of_token[t] * A.table_stride + pos / A.page_size];
+            const int page = A.write_kv == 2 ? t : A.block_table[(size_t)A.req_of_token[t] * A.table_stride + pos / A.page_size];
             if (page < 0 || page >= A.num_pages) {
                 atomicOr(err, XB_ERR_BAD_PAGE);
             } else {

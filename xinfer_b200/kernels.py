@@ -308,8 +308,19 @@ def rope_table(cos_t, sin_t, inv_freq):
     _ok(kernels_lib().xb_rope_table(cos_t.data_ptr(), sin_t.data_ptr(), inv_freq.data_ptr(), max_pos, half, _stream()), "rope_table")
 
 
+def qk_norm_rope_rows(q_out, k_out, v_out, qkv, q_w, k_w, cos_t, sin_t, positions, req_of_token, nh, nkv, d, rot, interleaved, eps, err):
+    """``qk_norm_rope_write`` with keys and values into rows ``[T, nkv, d]`` of their own instead of pages: the same numbers."""
+    T = qkv.shape[0]
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        _need(t, name, qkv.dtype, (T, nkv, d))
+    rows = (T, nkv, 1, d)                # pages of one slot, a token's own
+    qk_norm_rope_write(q_out, k_out.view(rows), v_out.view(rows), qkv, q_w, k_w, cos_t, sin_t, positions, req_of_token, req_of_token, 0, nh, nkv, d, rot,
+                       interleaved, eps, 2, err)
+
+
 def qk_norm_rope_write(q_out, k_cache, v_cache, qkv, q_w, k_w, cos_t, sin_t, positions, req_of_token,
                        block_table, table_stride, nh, nkv, d, rot, interleaved, eps, write_kv, err):
+    """``write_kv``: whether keys and values go to their pages (2: page t is token t's, see ``qk_norm_rope_rows``)."""
     T = qkv.shape[0]
     _need(qkv, "qkv", None, (T, (nh + 2 * nkv) * d))
     _need(q_out, "q_out", qkv.dtype, (T, nh, d))
@@ -331,14 +342,14 @@ def qk_norm_rope_write(q_out, k_cache, v_cache, qkv, q_w, k_w, cos_t, sin_t, pos
         _ok(kernels_lib().xb_qk_norm_rope_write_bf16(
             q_out.data_ptr(), _ptr(k_cache), _ptr(v_cache), qkv.data_ptr(), _ptr(q_w), _ptr(k_w), _ptr(cos_t), _ptr(sin_t),
             positions.data_ptr(), req_of_token.data_ptr(), block_table.data_ptr(), int(table_stride), T, nh, nkv, d, rot,
-            int(bool(interleaved)), page_size, num_pages, max_pos, float(eps), int(bool(write_kv)), err.data_ptr(),
+            int(bool(interleaved)), page_size, num_pages, max_pos, float(eps), int(write_kv), err.data_ptr(),
             _stream()), "qk_norm_rope_write_bf16")
         return
     _ok(kernels_lib().xb_qk_norm_rope_write(
         dtype_code(qkv.dtype), q_out.data_ptr(), _ptr(k_cache), _ptr(v_cache), qkv.data_ptr(), _ptr(q_w), _ptr(k_w),
         _ptr(cos_t), _ptr(sin_t), positions.data_ptr(), req_of_token.data_ptr(), block_table.data_ptr(),
         int(table_stride), T, nh, nkv, d, rot, int(bool(interleaved)), page_size, num_pages, max_pos, float(eps),
-        int(bool(write_kv)), err.data_ptr(), _stream()), "qk_norm_rope_write")
+        int(write_kv), err.data_ptr(), _stream()), "qk_norm_rope_write")
 
 
 def attention_plain(out, q, k_cache, v_cache, positions, req_of_token, block_table, table_stride, window, scale, err, *,

@@ -75,7 +75,7 @@ class DenseLayers:
         return DenseLayers(layers, gemm_ex) if gemm_ex is not None else None
 
     def takes(self, ctx: StepContext, caches: List[Optional[LayerCache]]) -> bool:
-        if not (ENABLED and kernels.vectorized and gemm_backend._enabled and attention_backend._enabled and attention_backend.PREFILL_TC
+        if ctx.tree is not None or not (ENABLED and kernels.vectorized and gemm_backend._enabled and attention_backend._enabled and attention_backend.PREFILL_TC
                 and attention_backend.DECODE_TC) or gemm_backend.FUSE_EPILOGUES or tracing.ENABLED \
                 or not _torch_calls_the_library():
             return False

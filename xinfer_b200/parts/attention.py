@@ -62,6 +62,8 @@ class Attention(Mixer):
         return PagedCacheNeed.keys_and_values(self.spec.num_kv_heads, self.spec.head_dim, self.spec.window)
 
     def prepare_step(self, ctx: StepContext, cache: LayerCache) -> None:
+        if ctx.tree is not None:
+            return
         from . import attention_backend
         s = self.spec
         attention_backend.prepare_step(ctx, self.dtype, s.num_heads, s.num_kv_heads, s.head_dim, cache.page_size, s.window,
@@ -75,6 +77,8 @@ class Attention(Mixer):
         rot = self.position.rotary() if self.position is not None else None
         q = ws.get("attn.q", (T, nh, d), self.dtype)
         table, stride = ctx.tables[cache.group], ctx.strides[cache.group]
+        if ctx.tree is not None:
+            return self._forward_tree(x, q, rot, table.view(-1, stride), ctx, cache)
         head_args = (self.q_norm, self.k_norm, rot.cos if rot else None, rot.sin if rot else None, ctx.positions,
                      ctx.req_of_token, table, stride, nh, nkv, d, rot.rotary_dim if rot else 0,
                      rot.interleaved if rot else False, s.qk_norm_eps, writes_cache, ctx.err)
@@ -92,6 +96,26 @@ class Attention(Mixer):
         o = ws.get("attn.o", (T, nh, d), self.dtype)
         from . import attention_backend
         attention_backend.attend(o, q, cache, ctx, table, stride, s.window, s.scale)
+        out = ws.get("attn.out", (T, s.hidden), self.dtype)
+        linear(out, o.view(T, nh * d), self.w_o, ctx.err)
+        return out
+
+    def _forward_tree(self, x, q, rot, table, ctx: StepContext, cache: LayerCache):
+        """The same over a tree of drafted tokens: their keys and values stay in rows of their own, and each sees the cached keys and
+        its own path."""
+        s, ws, tree = self.spec, ctx.workspace, ctx.tree
+        if self.position is not None and rot is None:
+            raise ValueError("drafted tokens need rotary tables or no positions")
+        T, nh, nkv, d = x.shape[0], s.num_heads, s.num_kv_heads, s.head_dim
+        qkv = ws.get("attn.qkv", (T, (nh + 2 * nkv) * d), self.dtype)
+        linear(qkv, x, self.w_qkv, ctx.err)
+        k_new, v_new = cache["k_new"][:T], cache["v_new"][:T]
+        kernels.qk_norm_rope_rows(q, k_new, v_new, qkv, self.q_norm, self.k_norm, rot.cos if rot else None, rot.sin if rot else None, ctx.positions,
+                                  ctx.req_of_token, nh, nkv, d, rot.rotary_dim if rot else 0, rot.interleaved if rot else False, s.qk_norm_eps, ctx.err)
+        o = ws.get("attn.o", (T, nh, d), self.dtype)
+        scratch = ws.get("attn.tree", (kernels.tree_attention_scratch(T, nh, nkv, d, self.dtype),), torch.float32)
+        kernels.tree_attention(o, q, k_new, v_new, cache["k"], cache["v"], tree.context, tree.token_start, tree.ancestors, table, s.scale, ctx.err,
+                               scratch=scratch, depth=tree.depth, window=s.window)
         out = ws.get("attn.out", (T, s.hidden), self.dtype)
         linear(out, o.view(T, nh * d), self.w_o, ctx.err)
         return out

@@ -86,6 +86,18 @@ class Workspace:
 
 
 @dataclass
+class TreeStep:
+    """A step whose tokens are drafted and form a tree per request: nothing of it goes to the cache until the model's own choices have
+    confirmed it.  Mixers keep the step's keys and values in rows of their own (``k_new`` and ``v_new`` beside the pages of their
+    ``LayerCache``); a token's position is its request's context plus its depth."""
+
+    context: torch.Tensor      # int32 [B]: cached tokens of each request
+    token_start: torch.Tensor  # int32 [B + 1]: its first token
+    ancestors: torch.Tensor    # int32 [T, words]: bit i, lowest first: node i of the token's own tree lies on its path (itself among them)
+    depth: torch.Tensor        # int32 [T]
+
+
+@dataclass
 class StepContext:
     """Everything a part may know about the running step."""
 
@@ -126,6 +138,8 @@ class StepContext:
     # the type in which a mixer or feed-forward that can choose hands its result to the residual stream
     # (float32 where the model keeps a float32 stream); None: the engine's dtype
     branch_dtype: Optional[torch.dtype] = None
+    # the step verifies drafted tokens
+    tree: Optional[TreeStep] = None
 
     def longest_portion(self) -> int:
         """Tokens of the entry that brings most (a replayed step brings one of each)."""
