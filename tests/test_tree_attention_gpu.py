@@ -251,3 +251,90 @@ def test_refusals():
         with pytest.raises(k.KernelError):
             k.tree_attention(**{**args, **change})
     assert int(err) == 0
+
+
+MORE = [  # as above
+    ([3, 0, 1, 7, 20] * 20, [0, 50, 130, 64, 9] * 20, 8, 2, 64, 16, None), ([2, 1, 0] * 30, [700, 3, 40] * 30, 4, 4, 128, 32, 33), ([1] * 70, list(range(70)), 4, 1, 32, 8, None),
+    ([5, 9], [30, 300], 4, 2, 16, 16, None), ([2, 1], [40, 500], 128, 1, 64, 16, None), ([3], [100], 130, 1, 64, 16, None), ([10, 3], [700, 255], 8, 2, 128, 256, None),
+    ([1024], [33], 2, 1, 64, 16, None), ([300, 1], [10, 1000], 8, 4, 64, 16, 40), ([12], [9000], 2, 2, 128, 16, None)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nodes,contexts,nh,nkv,d,ps,window", MORE)
+def test_more_against_64_bits(nodes, contexts, nh, nkv, d, ps, window, dtype):
+    test_against_64_bits(nodes, contexts, nh, nkv, d, ps, window, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("what", ["key", "value"])
+def test_cached_rows_that_are_not_numbers_reach_every_node(dtype, what):
+    s = Step([40, 5], [200, 90], 8, 2, 128, 16, dtype)
+    clean = s.run()
+    at = s.table[0, 150 // 16], 1, 150 % 16
+    (s.kc if what == "key" else s.vc)[at] = float("nan")
+    out = s.run()
+    assert torch.isnan(out[:40, 4:]).all() and torch.equal(out[:, :4], clean[:, :4]) and torch.equal(out[40:], clean[40:]) and int(s.err) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_scores_that_are_large(dtype):
+    """Scores of several hundred, of either sign: the running maximum moves from tile to tile."""
+    s = Step([20, 6], [300, 64], 8, 2, 64, 16, dtype, sharp=120.0)
+    s.check(s.run())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_captured_call_follows_its_inputs(dtype):
+    """The lengths and masks are the device's: one graph serves other requests of the same shapes."""
+    from xinfer_b200 import kernels as k
+    steps = [Step(n, c, 8, 2, 128, 16, dtype, seed=i, words=2) for i, (n, c) in enumerate((([30, 2], [300, 40]), ([1, 31], [0, 320]), ([16, 16], [170, 171])))]
+    names = ("q", "kn", "vn", "kc", "vc", "ancestors", "table")
+    pages, width = max(s.kc.shape[0] for s in steps), max(s.table.shape[1] for s in steps)
+
+    def fitted(s):
+        grow = lambda t: torch.cat([t, torch.full((pages - t.shape[0], *t.shape[1:]), float("nan"), dtype=t.dtype)])  # noqa: E731
+        table = torch.zeros(2, width, dtype=torch.int32)
+        table[:, :s.table.shape[1]] = s.table
+        return [s.q, s.kn, s.vn, grow(s.kc), grow(s.vc), s.ancestors, table]
+
+    at = dict(zip(names, (t.to(DEV) for t in fitted(steps[0]))))
+    context, start = i32(steps[0].contexts), i32([int(x) for x in steps[0].start])
+    out, err = torch.zeros(32, 8, 128, dtype=dtype, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    scratch = torch.empty(k.tree_attention_scratch(32, 8, 2, 128, dtype), device=DEV)
+    call = lambda: k.tree_attention(out, at["q"], at["kn"], at["vn"], at["kc"], at["vc"], context, start, at["ancestors"], at["table"],  # noqa: E731
+                                    steps[0].scale, err, scratch=scratch)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+        call()                     # one behind another on the same scratch
+    for s in steps + steps[:1]:
+        for name, t in zip(names, fitted(s)):
+            at[name].copy_(t)
+        context.copy_(i32(s.contexts))
+        start.copy_(i32([int(x) for x in s.start]))
+        out.fill_(7.0)
+        graph.replay()
+        s.check(out)
+        assert torch.equal(out, s.run()) and int(err) == 0
+
+
+def test_more_refusals():
+    from xinfer_b200 import kernels as k
+    dtype = torch.bfloat16
+    q, kn = torch.zeros(4, 8, 64, dtype=dtype, device=DEV), torch.zeros(4, 2, 64, dtype=dtype, device=DEV)
+    cache = torch.zeros(2, 2, 16, 64, dtype=dtype, device=DEV)
+    need = k.tree_attention_scratch(4, 8, 2, 64, dtype)
+    room = torch.empty(need + 4, device=DEV)
+    args = dict(out=torch.empty_like(q), q=q, k_new=kn, v_new=kn, k_cache=cache, v_cache=cache, context=i32([20]), token_start=i32([0, 4]), ancestors=i32([[1]] * 4),
+                block_table=i32([[0, 1]]), scale=1.0, err=i32([0]), scratch=room[:need])
+    k.tree_attention(**args)
+    wide = torch.zeros(2, 2, 1 << 20, 64, dtype=dtype, device=DEV)
+    for change in (dict(scratch=room[:need - 1]), dict(scratch=room[1:need + 1]), dict(scratch=None), dict(scratch=room.bfloat16()),
+                   dict(k_new=kn[:, :0], v_new=kn[:, :0]), dict(context=i32([0] * 8193)),
+                   # requests whose tiles together might be more than 32 bits count
+                   dict(k_cache=wide, v_cache=wide, context=i32([0] * 4000), token_start=i32([0] * 4001), block_table=torch.zeros(4000, 64, dtype=torch.int32, device=DEV))):
+        with pytest.raises(k.KernelError):
+            k.tree_attention(**{**args, **change})
+    assert int(args["err"]) == 0

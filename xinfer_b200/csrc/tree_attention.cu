@@ -404,6 +404,9 @@ XB_EXPORT int xb_tree_attention(int dtype, void* out, const void* q, const void*
     const TreeArgs A{out, q, k_new, v_new, k_cache, v_cache, context, token_start, ancestors, depth, block_table, out_stride, q_stride, k_stride, v_stride,
                      tokens, requests, words, table_stride, nh, nkv, d, page_size, num_pages, window, scale, err};
     if (!scratch || ((uintptr_t)scratch & 15)) return (int)cudaErrorInvalidValue;
+    // the longest line that these shapes allow is counted in 32 bits
+    const double jobs = (double)nkv * ((double)tokens * (nh / nkv) / RT + requests), tiles = (double)table_stride * page_size / KT + (double)tokens / KT + 2;
+    if (jobs * (tiles * COST_TWO + COST_JOB) >= 2147483648.0) return (int)cudaErrorInvalidValue;
     if (dtype == XB_BF16 && tree_tc_takes(A)) return tree_tc_launch(A, scratch, stream);
     return dtype == XB_F32 ? launch<float>(A, scratch, stream) : launch<__nv_bfloat16>(A, scratch, stream);
 }

@@ -142,7 +142,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const uint32_t base = smem_u32(smem_raw), q_sm = base, kv_sm = base + Q_BYTES, bars = base + BAR_OFF;
     const uint32_t k_full0 = bars, k_empty0 = bars + RING, v_full0 = bars + 2 * RING, v_empty0 = bars + 3 * RING, rest = bars + 4 * RING;
     const uint32_t s_ready0 = rest, pv_done0 = rest + 32, p_ready0 = rest + 64, q_full = rest + 96, q_empty = rest + 104, looked0 = rest + 112,
-                   told = rest + 144, joined = rest + 152, seg_full0 = rest + 160, seg_empty0 = seg_full0 + 8 * SEGMENTS;
+                   told = rest + 144, joined = rest + 152, seg_full0 = rest + 160, seg_empty0 = seg_full0 + 8 * SEGMENTS,
+                   drained = seg_empty0 + 8 * SEGMENTS + 136;    // (behind the words)
     volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(smem_raw + BAR_OFF + 4 * RING + 160 + 16 * SEGMENTS);   // tmem, -, then the value rows
     volatile uint32_t* odd_rows = words + 2;                                                                                // that are not finite: [4][warp][2]
     Segment* const segments = reinterpret_cast<Segment*>(smem_raw + SEG_OFF);
@@ -171,6 +172,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             mbar_init(q_empty, 1);
             mbar_init(told, 8);
             mbar_init(joined, 8);
+            mbar_init(drained, 1);
+            mbar_init(drained + 8, 1);
             for (int i = 0; i < SEGMENTS; ++i) mbar_init(seg_full0 + 8 * i, 1), mbar_init(seg_empty0 + 8 * i, READERS);
             mbar_init_fence();
         }
@@ -312,6 +315,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
             }
         }
+        // nothing of this warp's is on its way when the block ends, however it ends
+        for (int i = 0; i < NS; ++i)
+            if (rounds || i < st) wait_warp(full0 + 8 * i, i < st ? ph : ph ^ 1u, err);
     } else if (warp == 9) {
         // ---- Q, then S = Q K^T of every tile --------------------------------------------------------------------------------
         const uint32_t one = elected(), tmem_u = uniform(tmem);
@@ -367,6 +373,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
             }
         }
+        commit(one, drained);                    // no product is at work when the tensor memory is freed, however the block ends
+        wait_warp(drained, 0, err);
     } else if (warp == 11) {
         // ---- O += P V of every tile (O starts as zeros, by the softmax threads) -----------------------------------------------
         const uint32_t one = elected(), tmem_u = uniform(tmem);
@@ -404,6 +412,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
             }
         }
+        commit(one, drained + 8);
+        wait_warp(drained + 8, 0, err);
     } else {
         // ---- softmax: a row per thread ---------------------------------------------------------------------------------------------
         const int hd = warp >> 2, r = (int)threadIdx.x & 127;

@@ -1838,6 +1838,8 @@ def tree_attention(out, q, k_new, v_new, k_cache, v_cache, context, token_start,
         _need(scratch, "scratch", torch.float32)
         if scratch.numel() < need:
             raise KernelError(f"scratch holds {scratch.numel()} numbers, {need} are needed")
+        if scratch.data_ptr() % 16:
+            raise KernelError("scratch starts off a 16-byte boundary")
     _ok(kernels_lib().xb_tree_attention(
         code, out.data_ptr(), q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), context.data_ptr(),
         token_start.data_ptr(), ancestors.data_ptr(), _ptr(depth), block_table.data_ptr(), so, sq, sk, sv, T, requests, ancestors.shape[1],
