@@ -140,3 +140,63 @@ def test_refusals():
                    dict(mask=i32([[1, 1]]), mask_of_row=i32([0]))):
         with pytest.raises(k.KernelError):
             k.logit_rules(**{**args, **change})
+
+
+def case_of_rows(rng, R, vocab, lists, list_of_row, paths=None, biases=None):
+    logits = (rng.normal(size=(R, vocab)) * 3).astype(np.float32)
+    pen = np.stack([rng.choice([1.0, 1.3, 0.8], R), rng.choice([0.0, 0.5], R), rng.choice([0.0, 0.7], R)], 1).astype(np.float32)
+    prompt = [len(t) // 3 for t in lists]
+    biases = biases or [[] for _ in range(R)]
+    ref, bound = reference(logits, pen, lists, prompt, list_of_row, paths or [[]] * R, biases, [None] * R)
+    return logits, pen, prompt, ref, bound
+
+
+@pytest.mark.parametrize("vocab", [600, 5003, 70001])
+@pytest.mark.parametrize("counts", [[700, 3], [100] * 20, [384, 1, 385, 0, 384], [0] * 60 + [90] * 9])
+def test_many_biases(vocab, counts):
+    """More than a block keeps at a time, of one row or of several, with tokens that are named more than once: their sum, in its order."""
+    rng = np.random.default_rng(vocab + len(counts))
+    R = len(counts)
+    biases = [[(int(v), float(a)) for v, a in zip(rng.integers(-1, min(vocab, 2000) + 1, m), np.round(rng.normal(size=m), 2).astype(np.float32))] for m in counts]
+    logits, pen, prompt, ref, bound = case_of_rows(rng, R, vocab, [[1, 2, 2, 5]] * R, list(range(R)), biases=biases)
+    got = call(logits, pen, [[1, 2, 2, 5]] * R, prompt, list(range(R)), None, None, None, biases, None, None).double().cpu().numpy()
+    # (the entries of a token are summed by themselves first: each of its roundings is of a number no larger than all their sizes together)
+    for r, row in enumerate(biases):
+        for v in {v for v, _ in row if 0 <= v < vocab}:
+            mine = [abs(a) for w, a in row if w == v]
+            bound[r, v] += 2.0 ** -23 * len(mine) * sum(mine)
+    assert (np.abs(got - ref) <= bound).all()
+
+
+@pytest.mark.parametrize("nodes,vocab", [([60, 60], 3001), ([700], 900), ([1024], 64), ([33, 1, 100], 20000), ([50] * 5, 1024)])
+def test_large_trees_of_rows_that_share_a_list(nodes, vocab):
+    rng = np.random.default_rng(sum(nodes))
+    words = -(-max(nodes) // 32)
+    drafted, masks, first, paths, list_of_row = [], [], [], [], []
+    for b, n in enumerate(nodes):
+        _, _, on = tree(rng, n)
+        toks = rng.integers(-1, min(vocab, 6), n)
+        paths += [[int(toks[i]) for i in np.flatnonzero(on[r])] for r in range(n)]
+        first += [len(drafted)] * n
+        drafted += toks.tolist()
+        masks.append(words_of(on, words))
+        list_of_row += [b] * n
+    lists = [rng.integers(0, min(vocab, 10), 50).tolist() for _ in nodes]
+    logits, pen, prompt, ref, bound = case_of_rows(rng, len(drafted), vocab, lists, list_of_row, paths)
+    got = call(logits, pen, lists, prompt, list_of_row, first, drafted, torch.cat(masks), None, None, None).double().cpu().numpy()
+    assert (np.abs(got - ref) <= bound).all()
+
+
+def test_places_that_make_no_sense_reach_nothing():
+    """Starts that do not ascend, lists, rows and masks that are not there: what they name is passed over."""
+    from xinfer_b200 import kernels as k
+    x = torch.randn(3, 500, device=DEV)
+    values = torch.ones(5, device=DEV)
+    for starts in ([0, 1000, 5, 5], [0, 5, 0, 0], [-7, 2, 10 ** 9, 2], [5, 0, 0, 0]):
+        out = torch.full_like(x, 9.0)
+        k.logit_rules(out, x, torch.tensor([[1.0, 0.0, 0.0]] * 3, device=DEV), i32([1, 2]), i32([0, 2 ** 30]), i32([-5]), list_of_row=i32([0, 7, -9]),
+                      tree=(i32([1, 2, 3]), i32([[-1], [-1], [-1]]), i32([-3, 2, 10 ** 9])), bias=(i32(starts), i32([0, 1, 2, 3, 4]), values))
+        for r in range(3):
+            # what lies outside the ascending part is not said by the rule, but every number is the logit or the logit and its bias
+            there = (out[r] == x[r]) | (out[r] == x[r] + 1.0)
+            assert bool(there.all()) and bool((out[r, 5:] == x[r, 5:]).all())

@@ -228,3 +228,27 @@ def test_refusals():
             k.commit_table(*bad)
     with pytest.raises(k.KernelError):
         k.cache_commit(None, s["slots"], s["request_of"], s["token_start"], i32([[0]]), err)
+
+
+@pytest.mark.parametrize("most", [2 ** 31 - 1, 2 ** 30, 10 ** 6])
+def test_slots_for_numbers_of_tokens_that_nobody_has(most):
+    """Requests that ask for more than their rows hold get nothing, however much it is together; the one beside them gets its slots
+    where the tokens before it leave room."""
+    from xinfer_b200 import kernels as k
+    rng = np.random.default_rng(9)
+    c = Cache(rng, [3, 5, 9, 2], 8, 20, 4)
+    pages = [list(row) for row in c.rows]
+    got = run_slots(c, [4, most, most, 3], 12)
+    assert got["err"] == k.ERR_NO_PAGE | k.ERR_BAD_ROW
+    assert got["lengths"] == [7, 5, 9, 5] and got["slots"] == [pages[0][0] * 8 + i for i in range(3, 7)] + [-1] * 8
+    assert got["start"] == [0, 4, min(4 + most, 2 ** 31 - 1), min(4 + 2 * most, 2 ** 31 - 1), min(7 + 2 * most, 2 ** 31 - 1)]
+    assert got["req"] == [0] * 4 + [1] * 8 and got["ring"][1] == 20
+
+
+def test_slots_of_the_most_requests():
+    rng = np.random.default_rng(10)
+    from xinfer_b200 import kernels as k
+    B = k.SLOT_REQUESTS_MAX
+    new = rng.choice([0, 1, 2, 9, -1], B).tolist()
+    lengths = rng.integers(0, 40, B).tolist()
+    check_slots(Cache(rng, lengths, 16, 3000, 5), new)

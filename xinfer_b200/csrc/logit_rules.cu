@@ -286,6 +286,10 @@ logit_rules_kernel(const RuleArgs A) {
             f.first = A.drafted ? A.first_row[r] : 0;
             f.bias = A.bias_start ? max(0, A.bias_start[r]) : 0;
             f.biases = A.bias_start ? (int)max(0LL, min((long long)A.bias_start[r + 1], A.bias_len) - f.bias) : 0;
+            if (listed >= 0) {                 // (starts that do not ascend: no further than what is listed)
+                const int before = A.bias_start ? f.bias - max(0, A.bias_start[r0]) : 0;
+                f.biases = before < 0 ? 0 : max(0, min(f.biases, listed - before));
+            }
             facts[tid] = f;
         }
         for (int i = tid; i < rows * A.words; i += THREADS) paths[i] = A.ancestors[(size_t)r0 * A.words + i];

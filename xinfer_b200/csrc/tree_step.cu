@@ -63,7 +63,8 @@ struct SlotArgs {
 };
 
 struct Sums {
-    int tokens, need, back;
+    long long tokens;              // (a request may ask for any number)
+    int need, back;
 };
 __device__ __forceinline__ Sums operator+(Sums a, Sums b) { return Sums{a.tokens + b.tokens, a.need + b.need, a.back + b.back}; }
 
@@ -118,6 +119,7 @@ cache_slots_kernel(const SlotArgs A) {
         if (add < 0) return Sums{0, 0, pages(len)};
         return Sums{add, (int)(((long long)len + add + ps - 1) / ps) - pages(len), 0};
     };
+    auto start_of = [](long long tokens) { return (int)min(tokens, 0x7fffffffLL); };
     Sums mine{0, 0, 0}, total;
     for (int b = b0; b < b1; ++b) mine = mine + sums_of(max(A.lengths[b], 0), A.new_tokens[b]);
     if (threadIdx.x == 0) taken = 0;
@@ -128,23 +130,23 @@ cache_slots_kernel(const SlotArgs A) {
         const int len = max(A.lengths[b], 0), add = A.new_tokens[b];
         const Sums s = sums_of(len, add);
         const bool served = fits(len, add) && (s.need == 0 || at.need + s.need <= count);
-        starts[b] = at.tokens;
+        starts[b] = start_of(at.tokens);
         need_before[b] = served ? at.need : ~at.need;
         back_before[b] = at.back;
         if (served && s.need > 0) most = at.need + s.need;
         if (first_block) {
-            A.token_start[b] = at.tokens;
+            A.token_start[b] = start_of(at.tokens);
             A.lengths_out[b] = add < 0 ? 0 : (served ? len + add : len);
             if (!served) atomicOr(A.err, XB_ERR_NO_PAGE);
         }
         at = at + s;
     }
     if (most > 0) atomicMax(&taken, most);
-    if (threadIdx.x == 0) starts[A.requests] = total.tokens;
+    if (threadIdx.x == 0) starts[A.requests] = start_of(total.tokens);
     __syncthreads();
     const bool room = total.back + count <= A.ring_size;         // (more pages than the ring was made for: they are not taken back)
     if (first_block && threadIdx.x == 0) {
-        A.token_start[A.requests] = total.tokens;
+        A.token_start[A.requests] = start_of(total.tokens);
         A.ring_out[0] = (int)(((long long)head + taken) % A.ring_size);
         A.ring_out[1] = count - taken + (room ? total.back : 0);
         if (!room) atomicOr(A.err, XB_ERR_BAD_PAGE);
@@ -228,7 +230,8 @@ XB_EXPORT int xb_cache_slots(long long* slots, int* positions, int* request, int
                              const int* ring, const int* lengths, const int* new_tokens, int requests, int capacity, int table_stride, int page_size,
                              int ring_size, int* err, cudaStream_t stream) {
     if (requests <= 0) return 0;
-    if (requests > SLOT_REQUESTS || page_size < 1 || ring_size < 1 || table_stride < 1) return (int)cudaErrorInvalidValue;
+    if (requests > SLOT_REQUESTS || page_size < 1 || ring_size < 1 || table_stride < 1 || (long long)requests * table_stride > 0x7fffffffLL)
+        return (int)cudaErrorInvalidValue;
     const SlotArgs A{slots, positions, request, token_start, lengths_out, ring_out, table, free_ring, ring, lengths, new_tokens,
                      requests, capacity, table_stride, page_size, ring_size, err};
     int blocks = (capacity + SLOT_THREADS - 1) / SLOT_THREADS;
