@@ -3,8 +3,10 @@
 * ``libxinfer_b200_kernels.so``: every ``.cu`` file of this folder, compiled by nvcc for sm_100a.
 * ``libxinfer_b200_host.so``: the host runtime (``host/*.cpp``: page pools, block tables, request
   slots, scheduler), compiled by g++; it needs no CUDA and also serves the CPU-only tests.
+* ``xinfer_b200_wrap.so``: a Python module (``python/*.cpp``) with the checks and calls of wrappers, compiled by g++
+  against torch's headers.
 
-Both land in ``csrc/_build`` next to a stamp of the sources' hash, so a changed source rebuilds
+All land in ``csrc/_build`` next to a stamp of the sources' hash, so a changed source rebuilds
 and an unchanged one loads at once.  A line is printed now and then while compiling.
 """
 from __future__ import annotations
@@ -151,8 +153,30 @@ def build_host() -> str:
     return _build("libxinfer_b200_host.so", sources, cc, ld, flags, "host runtime")
 
 
+def build_wrap() -> str:
+    import sysconfig
+
+    import torch
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if not cxx:
+        raise BuildError("no C++ compiler (g++) found: the wrappers' module cannot be compiled")
+    root = os.path.dirname(torch.__file__)
+    flags = [f for f in CXX_FLAGS if f != "-Wall"] + [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f'-DBUILT_FOR_TORCH="{torch.__version__}"']
+    include = ["-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               "-isystem", sysconfig.get_paths()["include"]]
+
+    def cc(src, obj):
+        return [cxx, *flags, *include, "-c", src, "-o", obj]
+
+    def ld(objs, out):
+        return [cxx, "-shared", "-o", out, *objs, "-L", os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+
+    return _build("xinfer_b200_wrap.so", _sources("python", ".cpp"), cc, ld, flags, "checks and calls of wrappers")
+
+
 def build_all() -> None:
     build_host()
+    build_wrap()
     build_kernels()
 
 

@@ -123,6 +123,30 @@ static inline int xb_more_smem(void (*kernel)(KArgs...), int bytes, unsigned lon
     return (int)rc;
 }
 
+// An entry point whose arguments come as words of 64 bits: pointers and whole numbers as they are, real numbers as doubles.
+#include <cstring>
+#include <type_traits>
+#include <utility>
+template <typename T>
+static inline T xb_from_word(long long w) {
+    if constexpr (std::is_pointer<T>::value) {
+        return reinterpret_cast<T>(w);
+    } else if constexpr (std::is_floating_point<T>::value) {
+        double d;
+        memcpy(&d, &w, sizeof d);
+        return (T)d;
+    } else {
+        return (T)w;
+    }
+}
+template <typename... P, size_t... I>
+static inline int xb_by_words(int (*f)(P...), const long long* words, std::index_sequence<I...>) { return f(xb_from_word<P>(words[I])...); }
+template <typename... P>
+static inline int xb_by_words(int (*f)(P...), const long long* words, int n) {
+    if (n != (int)sizeof...(P)) return (int)cudaErrorInvalidValue;
+    return xb_by_words(f, words, std::index_sequence_for<P...>{});
+}
+
 // Programmatic dependent launch: a kernel launched through xb_launch may be scheduled while the
 // kernel before it in the stream is still running; it calls pdl_wait() before it touches anything
 // that kernel may have written (or still reads), and pdl_launch_dependents() as early as it likes

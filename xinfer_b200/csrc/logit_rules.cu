@@ -338,11 +338,11 @@ int launch(const RuleArgs& A, cudaStream_t stream) {
 
 }  // namespace
 
-XB_EXPORT int xb_logit_rules(float* out, const float* logits, const float* penalties, const int* history, const int* history_start, const int* prompt_len,
-                             const int* list_of_row, const int* drafted, const int* ancestors, const int* first_row, const int* bias_start,
-                             const int* bias_tokens, const float* bias_values, const int* mask, const int* mask_of_row, long long out_stride,
-                             long long in_stride, long long history_len, long long bias_len, int rows, int lists, int vocab, int words, int masks,
-                             int mask_words, cudaStream_t stream) {
+static int logit_rules(float* out, const float* logits, const float* penalties, const int* history, const int* history_start, const int* prompt_len,
+                       const int* list_of_row, const int* drafted, const int* ancestors, const int* first_row, const int* bias_start,
+                       const int* bias_tokens, const float* bias_values, const int* mask, const int* mask_of_row, long long out_stride,
+                       long long in_stride, long long history_len, long long bias_len, int rows, int lists, int vocab, int words, int masks,
+                       int mask_words, cudaStream_t stream) {
     if (rows <= 0 || vocab <= 0) return 0;
     if (rows > (1 << 20) || words > WORDS || (mask && mask_words < (vocab + 31) / 32)) return (int)cudaErrorInvalidValue;
     const RuleArgs A{out, logits, penalties, history, history_start, prompt_len, list_of_row, drafted, ancestors, first_row, bias_start, bias_tokens,
@@ -350,3 +350,4 @@ XB_EXPORT int xb_logit_rules(float* out, const float* logits, const float* penal
     // chunks of 1,024 tokens while that leaves processors without work, of 4,096 when there are rows enough
     return (long long)rows * vocab < 148LL * 2 * 4096 ? launch<1>(A, stream) : launch<4>(A, stream);
 }
+XB_EXPORT int xb_logit_rules(const long long* words, int n) { return xb_by_words(logit_rules, words, n); }

@@ -394,11 +394,11 @@ int launch(const TreeArgs& A, float* scratch, cudaStream_t stream) {
 
 }  // namespace
 
-XB_EXPORT int xb_tree_attention(int dtype, void* out, const void* q, const void* k_new, const void* v_new, const void* k_cache, const void* v_cache,
-                                const int* context, const int* token_start, const int* ancestors, const int* depth, const int* block_table,
-                                long long out_stride, long long q_stride, long long k_stride, long long v_stride, int tokens, int requests, int words,
-                                int table_stride, int nh, int nkv, int d, int page_size, int num_pages, int window, float scale, float* scratch,
-                                int* err, cudaStream_t stream) {
+static int tree_attention(int dtype, void* out, const void* q, const void* k_new, const void* v_new, const void* k_cache, const void* v_cache,
+                          const int* context, const int* token_start, const int* ancestors, const int* depth, const int* block_table,
+                          long long out_stride, long long q_stride, long long k_stride, long long v_stride, int tokens, int requests, int words,
+                          int table_stride, int nh, int nkv, int d, int page_size, int num_pages, int window, float scale, float* scratch,
+                          int* err, cudaStream_t stream) {
     if (tokens <= 0 || requests <= 0) return 0;
     if (requests > LINE_REQUESTS || d < 1 || d > 512 || nkv < 1 || nh % nkv || page_size < 1 || (window > 0 && !depth)) return (int)cudaErrorInvalidValue;
     const TreeArgs A{out, q, k_new, v_new, k_cache, v_cache, context, token_start, ancestors, depth, block_table, out_stride, q_stride, k_stride, v_stride,
@@ -410,6 +410,7 @@ XB_EXPORT int xb_tree_attention(int dtype, void* out, const void* q, const void*
     if (dtype == XB_BF16 && tree_tc_takes(A)) return tree_tc_launch(A, scratch, stream);
     return dtype == XB_F32 ? launch<float>(A, scratch, stream) : launch<__nv_bfloat16>(A, scratch, stream);
 }
+XB_EXPORT int xb_tree_attention(const long long* words, int n) { return xb_by_words(tree_attention, words, n); }
 
 // float32 numbers of scratch, on a 16-byte boundary, for a step of `tokens` drafted tokens: enough for either kernel
 XB_EXPORT long long xb_tree_attention_scratch(int dtype, int tokens, int nh, int nkv, int d) {

@@ -218,17 +218,18 @@ __global__ void cache_commit_kernel(const void* const* layers /* [layers][4]: k 
 
 }  // namespace
 
-XB_EXPORT int xb_tree_accept(int* accepted, int* path, int* next_tokens, const int* drafted, const int* targets, const int* parents,
-                             const int* token_start, int requests, int tokens, int width, cudaStream_t stream) {
+static int tree_accept(int* accepted, int* path, int* next_tokens, const int* drafted, const int* targets, const int* parents,
+                       const int* token_start, int requests, int tokens, int width, cudaStream_t stream) {
     if (requests <= 0) return 0;
     if (width < 1) return (int)cudaErrorInvalidValue;
     return xb_launch(tree_accept_kernel, dim3((requests + 3) / 4), dim3(128), 0, stream, accepted, path, next_tokens, drafted, targets, parents, token_start, requests,
                      tokens, width);
 }
+XB_EXPORT int xb_tree_accept(const long long* words, int n) { return xb_by_words(tree_accept, words, n); }
 
-XB_EXPORT int xb_cache_slots(long long* slots, int* positions, int* request, int* token_start, int* lengths_out, int* ring_out, int* table, int* free_ring,
-                             const int* ring, const int* lengths, const int* new_tokens, int requests, int capacity, int table_stride, int page_size,
-                             int ring_size, int* err, cudaStream_t stream) {
+static int cache_slots(long long* slots, int* positions, int* request, int* token_start, int* lengths_out, int* ring_out, int* table, int* free_ring,
+                       const int* ring, const int* lengths, const int* new_tokens, int requests, int capacity, int table_stride, int page_size,
+                       int ring_size, int* err, cudaStream_t stream) {
     if (requests <= 0) return 0;
     if (requests > SLOT_REQUESTS || page_size < 1 || ring_size < 1 || table_stride < 1 || (long long)requests * table_stride > 0x7fffffffLL)
         return (int)cudaErrorInvalidValue;
@@ -242,10 +243,11 @@ XB_EXPORT int xb_cache_slots(long long* slots, int* positions, int* request, int
         if (const int rc = xb_more_smem(cache_slots_kernel, (3 * SLOT_REQUESTS + 1) * 4, &roomy)) return rc;
     return xb_launch(cache_slots_kernel, dim3(blocks), dim3(SLOT_THREADS), smem, stream, A);
 }
+XB_EXPORT int xb_cache_slots(const long long* words, int n) { return xb_by_words(cache_slots, words, n); }
 
-XB_EXPORT int xb_cache_commit(const void* const* layers, int num_layers, const long long* slots, const int* request_of, const int* token_start,
-                              const int* path, int tokens, int requests, int width, int rows, int nkv, int row_bytes, int page_size, long long num_slots,
-                              int* err, cudaStream_t stream) {
+static int cache_commit(const void* const* layers, int num_layers, const long long* slots, const int* request_of, const int* token_start,
+                        const int* path, int tokens, int requests, int width, int rows, int nkv, int row_bytes, int page_size, long long num_slots,
+                        int* err, cudaStream_t stream) {
     if (tokens <= 0 || num_layers <= 0 || requests <= 0) return 0;
     if (num_layers > 65535 || row_bytes < 2 || row_bytes % 2 || page_size < 1) return (int)cudaErrorInvalidValue;
     const dim3 grid(tokens, num_layers);
@@ -254,3 +256,4 @@ XB_EXPORT int xb_cache_commit(const void* const* layers, int num_layers, const l
     };
     return row_bytes % 16 == 0 ? go(cache_commit_kernel<uint4>, 16) : go(cache_commit_kernel<uint16_t>, 2);
 }
+XB_EXPORT int xb_cache_commit(const long long* words, int n) { return xb_by_words(cache_commit, words, n); }

@@ -12,7 +12,7 @@ from typing import Optional
 import numpy as np
 import torch
 
-from .native import kernels_lib
+from .native import entry_point, kernels_lib, wrap_module
 
 F32, BF16 = 0, 1
 
@@ -1773,20 +1773,43 @@ def stream_mix(out, x, read, weight, eps, err, *, branch=None, mix=None, write=N
 TREE_REQUESTS_MAX = SLOT_REQUESTS_MAX = 8192
 
 
-def _token_rows(t, name: str, dtype, tokens: int, heads: int, d: int) -> int:
+# Checks and calls in native code, loaded at the first use (csrc/python/wrap.cpp): ``_check`` is ``_need``, ``_rows`` looks at rows that may
+# lie apart, ``_call`` calls an entry point of the kernels.
+def _load_wrap() -> None:
+    global _check, _rows, _call
+    module = wrap_module()
+    module.on_failure(_need_failed)
+    _check, _rows, _call = module.check, module.rows, module.call
+
+
+def _check(*args):
+    _load_wrap()
+    return _check(*args)
+
+
+def _rows(*args):
+    _load_wrap()
+    return _rows(*args)
+
+
+def _call(*args):
+    _load_wrap()
+    return _call(*args)
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str) -> int:
+    return entry_point(name)
+
+
+def _token_rows(t, name: str, dtype, shape) -> int:
     """Elements between the tokens of ``[tokens, heads, d]`` whose heads are dense; tokens may lie further apart."""
-    try:
-        if t.is_cuda and t.dtype == dtype and t.shape == (tokens, heads, d):
-            if t.is_contiguous():
-                return heads * d
-            st, sh, sd = t.stride()
-            if (sd == 1 or d == 1) and (sh == d or heads == 1) and (st >= heads * d or tokens <= 1):
-                return st if tokens > 1 else heads * d
-    except AttributeError:
-        pass
+    row = _rows(t, dtype, shape)
+    if row is not None:
+        return row
     if not isinstance(t, torch.Tensor):
         raise KernelError(f"{name}: expected a tensor, got {type(t).__name__}")
-    raise KernelError(f"{name}: expected a {dtype} CUDA tensor of shape {(tokens, heads, d)} with dense heads, got {t.dtype} {tuple(t.shape)} "
+    raise KernelError(f"{name}: expected a {dtype} CUDA tensor of shape {shape} with dense heads, got {t.dtype} {tuple(t.shape)} "
                       f"with strides {t.stride()} on {t.device}")
 
 
@@ -1814,44 +1837,44 @@ def tree_attention(out, q, k_new, v_new, k_cache, v_cache, context, token_start,
         raise KernelError(f"{nh} query heads do not divide into {nkv} key/value heads")
     if not 1 <= d <= 512:
         raise KernelError(f"tree_attention takes heads of 1 to 512 channels, not {d}")
-    so, sq = _token_rows(out, "out", dtype, T, nh, d), _token_rows(q, "q", dtype, T, nh, d)
-    sk, sv = _token_rows(k_new, "k_new", dtype, T, nkv, d), _token_rows(v_new, "v_new", dtype, T, nkv, d)
-    _need(k_cache, "k_cache", dtype, (None, nkv, None, d))
+    of_q, of_k = (T, nh, d), (T, nkv, d)
+    so, sq = _token_rows(out, "out", dtype, of_q), _token_rows(q, "q", dtype, of_q)
+    sk, sv = _token_rows(k_new, "k_new", dtype, of_k), _token_rows(v_new, "v_new", dtype, of_k)
+    _check(k_cache, "k_cache", dtype, (None, nkv, None, d))
     pages, _, page_size, _ = k_cache.shape
-    _need(v_cache, "v_cache", dtype, (pages, nkv, page_size, d))
-    _need(context, "context", torch.int32)
+    _check(v_cache, "v_cache", dtype, (pages, nkv, page_size, d))
+    _check(context, "context", torch.int32, None)
     requests = context.numel()
     if requests > TREE_REQUESTS_MAX:
         raise KernelError(f"{requests} requests; a call takes {TREE_REQUESTS_MAX}")
-    _need(token_start, "token_start", torch.int32, (requests + 1,))
-    _need(block_table, "block_table", torch.int32, (requests, None))
-    _need(ancestors, "ancestors", torch.int32, (T, None))
-    _need(err, "err", torch.int32)
+    _check(token_start, "token_start", torch.int32, (requests + 1,))
+    _check(block_table, "block_table", torch.int32, (requests, None))
+    _check(ancestors, "ancestors", torch.int32, (T, None))
+    _check(err, "err", torch.int32, None)
     if window is not None and window < 1:
         raise KernelError(f"a window of {window} keys")
     if window is not None and depth is None:
         raise KernelError("a window goes by the tokens' depths")
     if depth is not None:
-        _need(depth, "depth", torch.int32, (T,))
+        _check(depth, "depth", torch.int32, (T,))
     need = tree_attention_scratch(T, nh, nkv, d, dtype)
     if need:
-        _need(scratch, "scratch", torch.float32)
+        _check(scratch, "scratch", torch.float32, None)
         if scratch.numel() < need:
             raise KernelError(f"scratch holds {scratch.numel()} numbers, {need} are needed")
         if scratch.data_ptr() % 16:
             raise KernelError("scratch starts off a 16-byte boundary")
-    _ok(kernels_lib().xb_tree_attention(
-        code, out.data_ptr(), q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), context.data_ptr(),
-        token_start.data_ptr(), ancestors.data_ptr(), _ptr(depth), block_table.data_ptr(), so, sq, sk, sv, T, requests, ancestors.shape[1],
-        block_table.shape[1], nh, nkv, d, page_size, pages, int(window or 0), float(scale), _ptr(scratch), err.data_ptr(), _stream()), "tree_attention")
+    _ok(_call(_entry("xb_tree_attention"), code, out, q, k_new, v_new, k_cache, v_cache, context, token_start, ancestors, depth, block_table, so, sq, sk, sv,
+              T, requests, ancestors.shape[1], block_table.shape[1], nh, nkv, d, page_size, pages, int(window or 0), float(scale), scratch, err, _stream()),
+        "tree_attention")
 
 
 def _logit_rows(t, name: str, shape) -> int:
-    if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32 or t.shape != shape
-            or (shape[1] > 1 and t.stride(1) != 1) or (shape[0] > 1 and t.stride(0) < shape[1])):
-        raise KernelError(f"{name}: expected float32 CUDA rows {tuple(shape)} with dense numbers, got "
+    row = _rows(t, torch.float32, shape)
+    if row is None:
+        raise KernelError(f"{name}: expected float32 CUDA rows {shape} with dense numbers, got "
                           + (f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__))
-    return t.stride(0) if shape[0] > 1 else shape[1]
+    return row
 
 
 def logit_rules(out, logits, penalties, history, history_start, prompt_len, *, list_of_row=None, tree=None, bias=None, mask=None, mask_of_row=None):
@@ -1867,46 +1890,44 @@ def logit_rules(out, logits, penalties, history, history_start, prompt_len, *, l
     si, so = _logit_rows(logits, "logits", (R, V)), _logit_rows(out, "out", (R, V))
     if out.data_ptr() == logits.data_ptr() and si != so:
         raise KernelError("rows that are changed in place have one stride")
-    _need(penalties, "penalties", torch.float32, (R, 3))
-    _need(history, "history", torch.int32)
-    _need(prompt_len, "prompt_len", torch.int32)
+    _check(penalties, "penalties", torch.float32, (R, 3))
+    _check(history, "history", torch.int32, None)
+    _check(prompt_len, "prompt_len", torch.int32, None)
     lists = prompt_len.numel()
-    _need(history_start, "history_start", torch.int32, (lists + 1,))
+    _check(history_start, "history_start", torch.int32, (lists + 1,))
     if list_of_row is not None:
-        _need(list_of_row, "list_of_row", torch.int32, (R,))
+        _check(list_of_row, "list_of_row", torch.int32, (R,))
     elif lists != R:
         raise KernelError(f"{lists} lists for {R} rows need list_of_row")
     drafted = ancestors = first_row = bias_start = bias_tokens = bias_values = None
     words = mask_words = masks = 0
     if tree is not None:
         drafted, ancestors, first_row = tree
-        _need(drafted, "drafted", torch.int32, (R,))
-        _need(ancestors, "ancestors", torch.int32, (R, None))
-        _need(first_row, "first_row", torch.int32, (R,))
+        _check(drafted, "drafted", torch.int32, (R,))
+        _check(ancestors, "ancestors", torch.int32, (R, None))
+        _check(first_row, "first_row", torch.int32, (R,))
         words = ancestors.shape[1]
         if words > 32:
             raise KernelError(f"ancestors of {words} words: trees of up to 1,024 nodes")
     if bias is not None:
         bias_start, bias_tokens, bias_values = bias
-        _need(bias_start, "bias start", torch.int32, (R + 1,))
-        _need(bias_tokens, "bias tokens", torch.int32)
-        _need(bias_values, "bias values", torch.float32, tuple(bias_tokens.shape))
+        _check(bias_start, "bias start", torch.int32, (R + 1,))
+        _check(bias_tokens, "bias tokens", torch.int32, None)
+        _check(bias_values, "bias values", torch.float32, tuple(bias_tokens.shape))
     if mask is not None:
-        _need(mask, "mask", torch.int32, (None, None))
+        _check(mask, "mask", torch.int32, (None, None))
         masks, mask_words = mask.shape
         if mask_words * 32 < V:
             raise KernelError(f"masks of {mask_words} words do not cover {V} tokens")
         if mask_of_row is not None:
-            _need(mask_of_row, "mask_of_row", torch.int32, (R,))
+            _check(mask_of_row, "mask_of_row", torch.int32, (R,))
         elif masks != R:
             raise KernelError(f"{masks} masks for {R} rows need mask_of_row")
     elif mask_of_row is not None:
         raise KernelError("mask_of_row without masks")
-    _ok(kernels_lib().xb_logit_rules(
-        out.data_ptr(), logits.data_ptr(), penalties.data_ptr(), history.data_ptr(), history_start.data_ptr(), prompt_len.data_ptr(),
-        _ptr(list_of_row), _ptr(drafted), _ptr(ancestors), _ptr(first_row), _ptr(bias_start), _ptr(bias_tokens), _ptr(bias_values), _ptr(mask),
-        _ptr(mask_of_row), so, si, history.numel(), bias_tokens.numel() if bias is not None else 0, R, lists, V, words, masks, mask_words,
-        _stream()), "logit_rules")
+    _ok(_call(_entry("xb_logit_rules"), out, logits, penalties, history, history_start, prompt_len, list_of_row, drafted, ancestors, first_row, bias_start,
+              bias_tokens, bias_values, mask, mask_of_row, so, si, history.numel(), bias_tokens.numel() if bias is not None else 0, R, lists, V, words, masks,
+              mask_words, _stream()), "logit_rules")
 
 
 def tree_accept(accepted, path, next_tokens, drafted, targets, parents, token_start):
@@ -1915,18 +1936,17 @@ def tree_accept(accepted, path, next_tokens, drafted, targets, parents, token_st
     ``targets`` the token that the model chose behind each node.  From the root on the path goes to the child of lowest place whose
     ``drafted`` token is its parent's target.  ``path`` ``[B, width]`` receives the path's tokens (rows of the step; -1 behind them),
     ``accepted`` how many they are (at most the width), ``next_tokens`` the target of the last one (-1 for a request without nodes)."""
-    _need(accepted, "accepted", torch.int32)
+    _check(accepted, "accepted", torch.int32, None)
     B, T = accepted.numel(), drafted.numel()
-    _need(path, "path", torch.int32, (B, None))
-    _need(next_tokens, "next_tokens", torch.int32, (B,))
-    _need(drafted, "drafted", torch.int32, (T,))
-    _need(targets, "targets", torch.int32, (T,))
-    _need(parents, "parents", torch.int32, (T,))
-    _need(token_start, "token_start", torch.int32, (B + 1,))
+    _check(path, "path", torch.int32, (B, None))
+    _check(next_tokens, "next_tokens", torch.int32, (B,))
+    _check(drafted, "drafted", torch.int32, (T,))
+    _check(targets, "targets", torch.int32, (T,))
+    _check(parents, "parents", torch.int32, (T,))
+    _check(token_start, "token_start", torch.int32, (B + 1,))
     if path.shape[1] < 1:
         raise KernelError("a path needs room for its root")
-    _ok(kernels_lib().xb_tree_accept(accepted.data_ptr(), path.data_ptr(), next_tokens.data_ptr(), drafted.data_ptr(), targets.data_ptr(),
-                                     parents.data_ptr(), token_start.data_ptr(), B, T, path.shape[1], _stream()), "tree_accept")
+    _ok(_call(_entry("xb_tree_accept"), accepted, path, next_tokens, drafted, targets, parents, token_start, B, T, path.shape[1], _stream()), "tree_accept")
 
 
 def cache_slots(slots, positions, request_of, token_start, lengths_out, ring_out, block_table, free_ring, ring, lengths, new_tokens,
@@ -1938,30 +1958,28 @@ def cache_slots(slots, positions, request_of, token_start, lengths_out, ring_out
     ``ring`` and ``lengths``, so that a call may be made again); per token in order ``slots`` (int64, page * page_size + place; -1: none),
     ``positions`` and ``request_of`` (-1 behind the last token), and ``token_start`` ``[B + 1]``.  Requests are served in their order; one
     whose pages are not all there, or do not fit its row, is left as it was, its slots are -1 and the error word says so."""
-    _need(lengths, "lengths", torch.int32)
+    _check(lengths, "lengths", torch.int32, None)
     B = lengths.numel()
     if B > SLOT_REQUESTS_MAX:
         raise KernelError(f"{B} requests; a call takes {SLOT_REQUESTS_MAX}")
-    _need(slots, "slots", torch.int64)
+    _check(slots, "slots", torch.int64, None)
     n = slots.numel()
-    _need(positions, "positions", torch.int32, (n,))
-    _need(request_of, "request_of", torch.int32, (n,))
-    _need(token_start, "token_start", torch.int32, (B + 1,))
-    _need(lengths_out, "lengths_out", torch.int32, (B,))
-    _need(ring_out, "ring_out", torch.int32, (2,))
-    _need(block_table, "block_table", torch.int32, (B, None))
-    _need(free_ring, "free_ring", torch.int32)
-    _need(ring, "ring", torch.int32, (2,))
-    _need(new_tokens, "new_tokens", torch.int32, (B,))
-    _need(err, "err", torch.int32)
+    _check(positions, "positions", torch.int32, (n,))
+    _check(request_of, "request_of", torch.int32, (n,))
+    _check(token_start, "token_start", torch.int32, (B + 1,))
+    _check(lengths_out, "lengths_out", torch.int32, (B,))
+    _check(ring_out, "ring_out", torch.int32, (2,))
+    _check(block_table, "block_table", torch.int32, (B, None))
+    _check(free_ring, "free_ring", torch.int32, None)
+    _check(ring, "ring", torch.int32, (2,))
+    _check(new_tokens, "new_tokens", torch.int32, (B,))
+    _check(err, "err", torch.int32, None)
     if page_size < 1 or not free_ring.numel() or not block_table.shape[1]:
         raise KernelError("pages of at least one token, a ring and a table with room for one page")
     if ring_out.data_ptr() == ring.data_ptr() or (B and lengths_out.data_ptr() == lengths.data_ptr()):
         raise KernelError("the state afterwards goes to other memory than the state before")
-    _ok(kernels_lib().xb_cache_slots(
-        slots.data_ptr(), positions.data_ptr(), request_of.data_ptr(), token_start.data_ptr(), lengths_out.data_ptr(), ring_out.data_ptr(),
-        block_table.data_ptr(), free_ring.data_ptr(), ring.data_ptr(), lengths.data_ptr(), new_tokens.data_ptr(), B, n, block_table.shape[1],
-        int(page_size), free_ring.numel(), err.data_ptr(), _stream()), "cache_slots")
+    _ok(_call(_entry("xb_cache_slots"), slots, positions, request_of, token_start, lengths_out, ring_out, block_table, free_ring, ring, lengths, new_tokens,
+              B, n, block_table.shape[1], int(page_size), free_ring.numel(), err, _stream()), "cache_slots")
 
 
 class CommitTable:
@@ -1969,6 +1987,7 @@ class CommitTable:
 
     def __init__(self, tensors, pointers, shape, rows: int):
         self.tensors, self.pointers, self.shape, self.rows = tensors, pointers, shape, rows      # (the tensors are kept alive)
+        self.row_bytes = shape[3] * tensors[0][0].element_size()
 
 
 def commit_table(k_caches, v_caches, k_new, v_new) -> CommitTable:
@@ -1982,7 +2001,7 @@ def commit_table(k_caches, v_caches, k_new, v_new) -> CommitTable:
     for kc, vc, kn, vn in layers:
         for name, t, want in (("k_cache", kc, shape), ("v_cache", vc, shape), ("k_new", kn, (rows, shape[1], shape[3])),
                               ("v_new", vn, (rows, shape[1], shape[3]))):
-            _need(t, name, dtype, want)
+            _check(t, name, dtype, want)
             if t.data_ptr() % 16:
                 raise KernelError(f"{name}: starts off a 16-byte boundary")
     pointers = torch.tensor([t.data_ptr() for layer in layers for t in layer], dtype=torch.int64).to(k_caches[0].device)
@@ -1996,14 +2015,12 @@ def cache_commit(table: CommitTable, slots, request_of, token_start, path, err):
     if not isinstance(table, CommitTable):
         raise KernelError("cache_commit takes a table of commit_table")
     pages, nkv, page_size, d = table.shape
-    _need(slots, "slots", torch.int64)
+    _check(slots, "slots", torch.int64, None)
     n = slots.numel()
-    _need(request_of, "request_of", torch.int32, (n,))
-    _need(path, "path", torch.int32, (None, None))
+    _check(request_of, "request_of", torch.int32, (n,))
+    _check(path, "path", torch.int32, (None, None))
     B, width = path.shape
-    _need(token_start, "token_start", torch.int32, (B + 1,))
-    _need(err, "err", torch.int32)
-    layers = len(table.tensors)
-    _ok(kernels_lib().xb_cache_commit(
-        table.pointers.data_ptr(), layers, slots.data_ptr(), request_of.data_ptr(), token_start.data_ptr(), path.data_ptr(), n, B, width,
-        table.rows, nkv, d * table.tensors[0][0].element_size(), page_size, pages * page_size, err.data_ptr(), _stream()), "cache_commit")
+    _check(token_start, "token_start", torch.int32, (B + 1,))
+    _check(err, "err", torch.int32, None)
+    _ok(_call(_entry("xb_cache_commit"), table.pointers, len(table.tensors), slots, request_of, token_start, path, n, B, width, table.rows, nkv,
+              table.row_bytes, page_size, pages * page_size, err, _stream()), "cache_commit")

@@ -1,4 +1,4 @@
-"""Loads the two native libraries (building them at first use) and declares their C signatures.
+"""Loads the native libraries (building them at first use) and declares their C signatures.
 
 There is no fallback: if the kernels cannot be built or loaded the engine raises.
 """
@@ -11,6 +11,7 @@ from ctypes import (POINTER, c_char_p, c_float, c_int, c_int32, c_longlong, c_vo
 _lock = threading.Lock()
 _host = None
 _kernels = None
+_wrap = None
 
 _I32P = POINTER(c_int32)
 _I64P = POINTER(c_longlong)
@@ -40,6 +41,29 @@ def kernels_lib():
             _declare_kernels(lib)
             _kernels = lib
     return _kernels
+
+
+def wrap_module():
+    """Checks of tensors and calls of kernels for wrappers (a Python module of its own; torch has to be imported before)."""
+    global _wrap
+    if _wrap is not None:
+        return _wrap
+    with _lock:
+        if _wrap is None:
+            import importlib.util
+
+            import torch  # noqa: F401  (its libraries are what the module is linked with)
+            from .csrc.build import build_wrap
+            spec = importlib.util.spec_from_file_location("xinfer_b200_wrap", build_wrap())
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            _wrap = module
+    return _wrap
+
+
+def entry_point(name: str) -> int:
+    """The address of an entry point that takes its arguments as words, for ``wrap_module().call``."""
+    return ctypes.cast(getattr(kernels_lib(), name), c_void_p).value
 
 
 def _sig(lib, name, restype, argtypes):
@@ -177,9 +201,4 @@ def _declare_kernels(lib):
     _sig(lib, "xb_expert_router", I, [I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, F, P])
     _sig(lib, "xb_attn_decode_tc", I,
          [P, P, P, P, P, P, P, P, I, I, I, I, I, I, L, I, I, I, F, F, F, P, F, I, I, I, I, P, I, P, P])
-    _sig(lib, "xb_tree_attention", I, [I, P, P, P, P, P, P, P, P, P, P, P, L, L, L, L, I, I, I, I, I, I, I, I, I, I, F, P, P, P])
     _sig(lib, "xb_tree_attention_scratch", L, [I, I, I, I, I])
-    _sig(lib, "xb_logit_rules", I, [P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, L, L, L, L, I, I, I, I, I, I, P])
-    _sig(lib, "xb_tree_accept", I, [P, P, P, P, P, P, P, I, I, I, P])
-    _sig(lib, "xb_cache_slots", I, [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P, P])
-    _sig(lib, "xb_cache_commit", I, [P, I, P, P, P, P, I, I, I, I, I, I, I, L, P, P])
