@@ -246,15 +246,6 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         for (int i = lane; i < r.nodes; i += 32) deepest = max(deepest, A.depth[r.first + i]);
                         s.deep_lo = r.context + __reduce_max_sync(0xffffffffu, deepest) - A.window + 1;
                     }
-                    if (!s.whole && lane == 0) {       // what the join needs to know
-                        const int which = s.i0 > 0 ? 0 : 1;
-                        int from;
-                        const int parts = job_parts(w, from);
-                        int4* job = reinterpret_cast<int4*>(line.shared_jobs + (blockIdx.x * 2 + which) * 8);
-                        job[0] = make_int4(parts, from, s.first + s.node0, s.nodes);
-                        job[1].x = s.g;
-                        told_of |= 1 << which;
-                    }
                 } else {
                     s.nodes = 0;
                     for (int which = 0; which < 2; ++which)
@@ -274,21 +265,29 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 ++seg;
                 if (!more) break;
             }
+            // 32 entries of the block table at a time, a lane each, and the next 32 on their way; a tile's entries lie in one such run
             const int* table = A.block_table + (size_t)s.b * A.table_stride;
-            auto page_of = [&](int it) -> int {            // the page of this lane's box, -1: nothing to load
-                if (it >= s.i1 || it >= s.old_tiles || lane >= boxes) return -1;
-                const int j = s.key0 + it * KT + bi * box_rows;
-                if (j >= s.context) return -1;
-                const int page = table[j >> ps_shift];
-                if (page < 0 || page >= A.num_pages) {
-                    atomicOr(err, XB_ERR_BAD_PAGE);
-                    return A.num_pages;                    // behind the last page: the box reads as zeros
-                }
-                return page;
-            };
-            int page_next = page_of(s.i0);
+            const int entries = (min(s.context, s.key0 + min(s.i1, s.old_tiles) * KT) + A.page_size - 1) >> ps_shift;
+            int entry0 = (s.key0 + s.i0 * KT) >> ps_shift;
+            auto entry = [&](int i) { return i < entries ? table[i] : 0; };
+            int run = entry(entry0 + lane), next_run = entry(entry0 + 32 + lane);
             for (int it = s.i0; it < s.i1; ++it) {
-                const int page = page_next;
+                int page = -1;                             // of this lane's box, -1: nothing to load
+                if (it < s.old_tiles) {
+                    const int at = (s.key0 + it * KT) >> ps_shift;
+                    if (at - entry0 >= 32) {
+                        run = next_run;
+                        entry0 += 32;
+                        next_run = entry(entry0 + 32 + lane);
+                    }
+                    page = __shfl_sync(0xffffffffu, run, (at - entry0 + bi) & 31);
+                    if (lane >= boxes || s.key0 + it * KT + bi * box_rows >= s.context) {
+                        page = -1;
+                    } else if (page < 0 || page >= A.num_pages) {
+                        atomicOr(err, XB_ERR_BAD_PAGE);
+                        page = A.num_pages;                // behind the last page: the box reads as zeros
+                    }
+                }
                 if (rounds && !wait_warp(empty0 + 8 * st, ph ^ 1u, err)) {
                     ok = false;
                     break;
@@ -307,12 +306,20 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     __syncwarp();
                     if (lane < HALVES) tma_load_3d(dst0 + lane * KV_HALF, map_new, lane * 64, s.g, s.first + (it - s.old_tiles) * KT, full0 + 8 * st);
                 }
-                page_next = page_of(it + 1);
                 if (++st == NS) {
                     st = 0;
                     ph ^= 1u;
                     rounds = true;
                 }
+            }
+            if (!is_v && !s.whole && lane == 0) {          // what the join needs to know
+                const int which = s.i0 > 0 ? 0 : 1;
+                int from;
+                const int parts = job_parts(w, from);
+                int4* job = reinterpret_cast<int4*>(line.shared_jobs + (blockIdx.x * 2 + which) * 8);
+                job[0] = make_int4(parts, from, s.first + s.node0, s.nodes);
+                job[1].x = s.g;
+                told_of |= 1 << which;
             }
         }
         // nothing of this warp's is on its way when the block ends, however it ends
