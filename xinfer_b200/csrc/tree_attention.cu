@@ -283,14 +283,19 @@ tree_attention_kernel(const TreeArgs A, const Line line) {
             const size_t part = part_row(line, blockIdx.x, which, o_row + r);
             T* out = (T*)A.out + (size_t)(s.first + row / G) * A.out_stride + (size_t)(w.g * G + row % G) * A.d;
 #pragma unroll
-            for (int j = 0; j < CJ; ++j)
+            for (int j = 0; j < CJ; ++j) {
+                const int c0 = o_col + 64 * j;
+                if (!whole && A.d % 4 == 0) {
+                    if (c0 < A.d) *reinterpret_cast<float4*>(line.part_o + part * A.d + c0) = make_float4(o[r][j][0], o[r][j][1], o[r][j][2], o[r][j][3]);
+                    continue;
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int c = o_col + 64 * j + e;
-                    if (c >= A.d) continue;
-                    if (whole) out[c] = from_f32<T>(o[r][j][e] * inv);
-                    else line.part_o[part * A.d + c] = o[r][j][e];
+                    if (c0 + e >= A.d) continue;
+                    if (whole) out[c0 + e] = from_f32<T>(o[r][j][e] * inv);
+                    else line.part_o[part * A.d + c0 + e] = o[r][j][e];
                 }
+            }
         }
         if (!whole) {
             if (tid < rows) {
@@ -316,53 +321,156 @@ tree_attention_kernel(const TreeArgs A, const Line line) {
     if (tid < 2 && !(told_of >> tid & 1)) line.shared_jobs[(blockIdx.x * 2 + tid) * 8] = 0;
 }
 
-// Joins the parts of a job that several blocks shared, in their order: with M the largest of their maxima,
-// out = sum_i e^(m_i - M) O_i / sum_i e^(m_i - M) l_i.  A block per part, which takes as many of the job's rows; a warp per row, a part's factor
-// per lane, then the row's channels of eight parts at once.
-template <typename T, int DP>
-__global__ void __launch_bounds__(THREADS)
-tree_join_kernel(const TreeArgs A, const Line line) {
-    constexpr int C = DP / 32, P = C >= 8 ? 2 : 16 / C;
-    pdl_launch_dependents();
-    pdl_wait();
-    const int* job = line.shared_jobs + blockIdx.x * 8;
-    const int parts = job[0], c_first = job[1], row0 = job[2], rows = job[3], g = job[4], first = job[5];
-    if (parts < 2) return;
-    const int mine = (int)blockIdx.x / 2 - c_first, G = A.nh / A.nkv, lane = threadIdx.x & 31;
-    for (int r = rows * mine / parts + (int)(threadIdx.x >> 5); r < rows * (mine + 1) / parts; r += THREADS / 32) {
-        auto at = [&](int i) { return part_row(line, c_first + i, i > 0 ? 0 : 1, r); };
-        float M = -INFINITY, W = 0.f, acc[C] = {};
-        for (int i = lane; i < parts; i += 32) M = fmaxf(M, __ldcg(line.part_ml + at(i) * 2));
-        M = warp_max(M);
-        if (M == -INFINITY) M = 0.f;
-        for (int base = 0; base < parts; base += 32) {
-            float f = 0.f;
-            if (base + lane < parts) {
-                f = expf(__ldcg(line.part_ml + at(base + lane) * 2) - M);
-                W = fmaf(f, __ldcg(line.part_ml + at(base + lane) * 2 + 1), W);
-            }
-            for (int i0 = 0; i0 < min(32, parts - base); i0 += P) {
-                float v[P][C];
+// Joins the parts of a job that several blocks shared, in an order that does not change: with M the largest of their maxima,
+// out = sum_i e^(m_i - M) O_i / sum_i e^(m_i - M) l_i.  A block per part, which takes as many of the job's rows.  Bound by trips to the L2: a warp
+// has eight pieces of rows on their way, of several rows where a job has few parts, and asks for them before it forms their factors; of a job
+// of more than eight parts the block's warps take a row together, every fourth part each.
+constexpr int JOIN_WARPS = THREADS / 32, JOIN_TOGETHER = 8;
+
+struct JoinJob {
+    int parts, c_first, row0, rows, g, first, G;
+};
+
+// `V` numbers of a row from c on (a row's numbers lie on its own, d a multiple of V or not).
+template <int V>
+__device__ __forceinline__ void piece_of(float* to, const float* row, int c, int d) {
+    if (d % V == 0) {
+        if constexpr (V == 4) {
+            const float4 x = c < d ? __ldcg(reinterpret_cast<const float4*>(row + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+        } else {
+            const float2 x = c < d ? __ldcg(reinterpret_cast<const float2*>(row + c)) : make_float2(0.f, 0.f);
+            to[0] = x.x, to[1] = x.y;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) to[e] = c + e < d ? __ldcg(row + c + e) : 0.f;
+    }
+}
+
+// P parts of R rows at a time by a warp; TOGETHER: one row by all warps.
+template <typename T, int DP, int P, bool TOGETHER>
+__device__ __forceinline__ void join_rows(const TreeArgs& A, const Line& line, const JoinJob& job, int r0, int r1) {
+    constexpr int V = DP >= 128 ? 4 : 2, K = DP / (32 * V), R = TOGETHER || 8 / (P * K) < 1 ? 1 : 8 / (P * K), STEP = TOGETHER ? JOIN_WARPS : 1;
+    __shared__ float factors[TOGETHER ? LINE_BLOCKS : 1], warps_max[JOIN_WARPS], warps_sum[JOIN_WARPS], others[TOGETHER ? JOIN_WARPS : 1][TOGETHER ? DP : 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part0 = TOGETHER ? warp : 0;
+    auto at = [&](int i, int r) { return part_row(line, job.c_first + i, i > 0 ? 0 : 1, r); };
+    const float2* const ml = reinterpret_cast<const float2*>(line.part_ml);
+    for (int base = TOGETHER ? r0 : r0 + warp * R; base < r1; base += TOGETHER ? 1 : JOIN_WARPS * R) {
+        float v[R][P][K][V];
+        auto request = [&](int i0) {
+#pragma unroll
+            for (int x = 0; x < R; ++x)
 #pragma unroll
                 for (int i = 0; i < P; ++i)
 #pragma unroll
-                    for (int k = 0; k < C; ++k)
-                        v[i][k] = base + i0 + i < parts && lane + 32 * k < A.d ? __ldcg(line.part_o + at(base + i0 + i) * A.d + lane + 32 * k) : 0.f;
+                    for (int k = 0; k < K; ++k) {
+                        const int part = i0 + i * STEP;
 #pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    const float fi = __shfl_sync(0xffffffffu, f, (i0 + i) & 31);
+                        for (int e = 0; e < V; ++e) v[x][i][k][e] = 0.f;
+                        if (part < job.parts && base + x < r1) piece_of<V>(v[x][i][k], line.part_o + at(part, base + x) * A.d, (lane + 32 * k) * V, A.d);
+                    }
+        };
+        request(part0);
+        float f[R], W[R];                          // of the lane's part (not TOGETHER); of the row
+        if constexpr (TOGETHER) {
+            float M = -INFINITY, mine = 0.f;
+            for (int i = threadIdx.x; i < job.parts; i += THREADS) M = fmaxf(M, __ldcg(ml + at(i, base)).x);
+            M = warp_max(M);
+            if (lane == 0) warps_max[warp] = M;
+            __syncthreads();
 #pragma unroll
-                    for (int k = 0; k < C; ++k) acc[k] = fmaf(fi, v[i][k], acc[k]);
-                }
+            for (int w = 0; w < JOIN_WARPS; ++w) M = fmaxf(M, warps_max[w]);
+            if (M == -INFINITY) M = 0.f;
+            for (int i = threadIdx.x; i < job.parts; i += THREADS) {
+                const float2 x = __ldcg(ml + at(i, base));
+                const float e = expf(x.x - M);
+                factors[i] = e;
+                mine = fmaf(e, x.y, mine);
+            }
+            mine = warp_sum(mine);
+            if (lane == 0) warps_sum[warp] = mine;
+            __syncthreads();
+            W[0] = 0.f;
+#pragma unroll
+            for (int w = 0; w < JOIN_WARPS; ++w) W[0] += warps_sum[w];
+        } else {
+#pragma unroll
+            for (int x = 0; x < R; ++x) {
+                const float2 mine = lane < job.parts && base + x < r1 ? __ldcg(ml + at(lane, base + x)) : make_float2(-INFINITY, 0.f);
+                float M = warp_max(mine.x);
+                if (M == -INFINITY) M = 0.f;
+                f[x] = expf(mine.x - M);
+                W[x] = warp_sum(f[x] * mine.y);
             }
         }
-        W = warp_sum(W);
-        const float inv = W > 0.f || W != W ? 1.f / W : 0.f;
-        T* out = (T*)A.out + (size_t)(first + (row0 + r) / G) * A.out_stride + (size_t)(g * G + (row0 + r) % G) * A.d;
+        float acc[R][K][V];
 #pragma unroll
-        for (int k = 0; k < C; ++k)
-            if (lane + 32 * k < A.d) out[lane + 32 * k] = from_f32<T>(acc[k] * inv);
+        for (int x = 0; x < R; ++x)
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[x][k][e] = 0.f;
+        for (int i0 = part0; i0 < job.parts; i0 += P * STEP) {
+            if (i0 > part0) request(i0);
+#pragma unroll
+            for (int x = 0; x < R; ++x)
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const int part = i0 + i * STEP;
+                    float fi;
+                    if constexpr (TOGETHER) fi = part < job.parts ? factors[part] : 0.f;
+                    else fi = __shfl_sync(0xffffffffu, f[x], part & 31);
+#pragma unroll
+                    for (int k = 0; k < K; ++k)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) acc[x][k][e] = fmaf(fi, v[x][i][k][e], acc[x][k][e]);
+                }
+        }
+        if constexpr (TOGETHER) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) others[warp][(lane + 32 * k) * V + e] = acc[0][k][e];
+            __syncthreads();
+        }
+#pragma unroll
+        for (int x = 0; x < R; ++x) {
+            const int row = job.row0 + base + x;
+            if (base + x >= r1) continue;
+            const float inv = W[x] > 0.f || W[x] != W[x] ? 1.f / W[x] : 0.f;
+            T* out = (T*)A.out + (size_t)(job.first + row / job.G) * A.out_stride + (size_t)(job.g * job.G + row % job.G) * A.d;
+            if constexpr (TOGETHER) {
+                for (int c = threadIdx.x; c < A.d; c += THREADS) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int w = 0; w < JOIN_WARPS; ++w) sum += others[w][c];
+                    out[c] = from_f32<T>(sum * inv);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if ((lane + 32 * k) * V + e < A.d) out[(lane + 32 * k) * V + e] = from_f32<T>(acc[x][k][e] * inv);
+            }
+        }
+        if constexpr (TOGETHER) __syncthreads();   // what the next row writes has been read
     }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS)
+tree_join_kernel(const TreeArgs A, const Line line) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int* job_at = line.shared_jobs + blockIdx.x * 8;
+    const JoinJob job{job_at[0], job_at[1], job_at[2], job_at[3], job_at[4], job_at[5], A.nh / A.nkv};
+    if (job.parts < 2) return;
+    const int mine = (int)blockIdx.x / 2 - job.c_first, r0 = job.rows * mine / job.parts, r1 = job.rows * (mine + 1) / job.parts;
+    if (job.parts > JOIN_TOGETHER) join_rows<T, DP, 8, true>(A, line, job, r0, r1);
+    else if (job.parts > 2) join_rows<T, DP, 4, false>(A, line, job, r0, r1);
+    else join_rows<T, DP, 2, false>(A, line, job, r0, r1);
 }
 
 long long scratch_floats(int d) { return line_floats(LINE_BLOCKS, RT, d, 0); }
@@ -381,7 +489,9 @@ template <typename T>
 int launch(const TreeArgs& A, float* scratch, cudaStream_t stream) {
     Line line;
     line.two_from = A.tokens;
-    line.min_share = 3 * COST_ONE;
+    // A tile a block while there are blocks enough: a tile takes 3 us of a block by itself, the join of its part half a microsecond.  One, two
+    // and three tiles measured: 13.8, 18.7 and 21.0 us (8 nodes, 16 heads of 64 channels, 600 keys), 38.2, 38.2 and 48.0 (16 nodes, 4,096 keys).
+    line.min_share = COST_ONE;
     line.row_mul = A.nh / A.nkv;
     line.row_div = RT;
     line.part_rows = RT;
