@@ -74,12 +74,6 @@ tree_attention_kernel(const TreeArgs A, const Line line) {
         const RequestLine& s = w.r;
         const int row0 = w.piece * RT, rows = min(RT, s.nodes * G - row0);
         const bool whole = w.i1 - w.i0 == s.tiles;
-        for (int i = tid; i < RT * DP / 4; i += THREADS) {
-            const int r = i / (DP / 4), c = i % (DP / 4) * 4, row = row0 + r;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < rows) x = four_of(q + (size_t)(s.first + row / G) * A.q_stride + (size_t)(w.g * G + row % G) * A.d, c, A.d, fours);
-            *reinterpret_cast<float4*>(q_sm + r * LD + c) = x;
-        }
         if (tid < RT) {
             tops[tid] = -INFINITY;
             sums[tid] = 0.f;
@@ -128,6 +122,13 @@ tree_attention_kernel(const TreeArgs A, const Line line) {
             depths[it & 1][lane] = asked_depth;
         };
         ask(w.i0);
+#pragma unroll 4
+        for (int i = tid; i < RT * DP / 4; i += THREADS) {
+            const int r = i / (DP / 4), c = i % (DP / 4) * 4, row = row0 + r;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows) x = four_of(q + (size_t)(s.first + row / G) * A.q_stride + (size_t)(w.g * G + row % G) * A.d, c, A.d, fours);
+            *reinterpret_cast<float4*>(q_sm + r * LD + c) = x;
+        }
         unsigned my_mask = asked_mask;
         if (warp == 0) write_down(w.i0);
         for (int it = w.i0; it < w.i1; ++it) {
@@ -135,7 +136,7 @@ tree_attention_kernel(const TreeArgs A, const Line line) {
             const int key0 = drafted ? (it - s.old_tiles) * KT : (s.tile0 + it) * KT, keys = min(KT, (drafted ? s.nodes : s.context) - key0);
             bool odd = false;
             __syncthreads();                       // the tile before has been read
-#pragma unroll 4
+#pragma unroll 8
             for (int i = tid; i < KT * DP / 4; i += THREADS) {
                 const int j = i / (DP / 4), c = i % (DP / 4) * 4;
                 const long long at = rows_of[it & 1][j];
@@ -469,6 +470,7 @@ tree_join_kernel(const TreeArgs A, const Line line) {
     if (job.parts < 2) return;
     const int mine = (int)blockIdx.x / 2 - job.c_first, r0 = job.rows * mine / job.parts, r1 = job.rows * (mine + 1) / job.parts;
     if (job.parts > JOIN_TOGETHER) join_rows<T, DP, 8, true>(A, line, job, r0, r1);
+    else if (job.parts > 4) join_rows<T, DP, 8, false>(A, line, job, r0, r1);
     else if (job.parts > 2) join_rows<T, DP, 4, false>(A, line, job, r0, r1);
     else join_rows<T, DP, 2, false>(A, line, job, r0, r1);
 }
