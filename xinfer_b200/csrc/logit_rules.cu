@@ -35,26 +35,26 @@ struct RuleArgs {
 
 // (`inv` is 1 / rep, rounded: a product in place of a quotient is one float32 rounding more, and a sixth of the instructions)
 __device__ __forceinline__ float ruled(float x, unsigned count, float rep, float inv, float freq, float pres) {
-    if (count == 0u) return x;
-    x *= x > 0.f ? inv : rep;
     const unsigned c = count & ~ASKED;
-    if (c) x = x - freq * (float)c - pres;
-    return x;
+    const float y = x * (x > 0.f ? inv : rep), z = c ? y - freq * (float)c - pres : y;      // (no branch: a warp nearly always has such a token)
+    return count ? z : x;
 }
 
 constexpr int WARPS = THREADS / 32;
 constexpr int ROWS = 48;                        // rows at a time: what they need to know lies in shared memory
 constexpr int WORDS = 32;                       // words of ancestors: trees of up to 1,024 nodes
-constexpr int BIASES = 384;                     // biases of the rows at a time
+constexpr int BIASES = 192;                     // biases of these rows that lie in the chunk
 constexpr int STAGES = 2;                       // rows on their way or worked on
 
-struct RowFacts {
+struct __align__(16) RowFacts {
     float rep, inv, freq, pres;
     int list, mask, first, bias, biases;
+    unsigned biased;                            // a bit per warp that has tokens with biases
 };
 struct Bias {
-    int u;                                      // where in the chunk (-1: elsewhere, or not the first of the row's entries for its token)
-    float value;                                // of all the row's entries for that token
+    int at, entry;                              // row << 16 | where in the chunk; which entry it is
+    float value;                                // of all the row's entries for that token, in their order; in the first of them
+    int first;                                  // whether it is that
 };
 
 template <int N>
@@ -74,7 +74,7 @@ constexpr int smem_of(int vecs, int words) { return 4 * (chunk_of(vecs) + STAGES
 // words and biases, so that the warps of a block go through the rows without waiting for each other; each has two more rows on their way.
 // Bound by memory: a logit is read and written once.
 template <int VECS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 4)
 logit_rules_kernel(const RuleArgs A) {
     constexpr int CHUNK = chunk_of(VECS);
     extern __shared__ __align__(16) unsigned count[];            // [CHUNK], then the stages' logits and their mask words
@@ -82,6 +82,7 @@ logit_rules_kernel(const RuleArgs A) {
     int* const masks_at = reinterpret_cast<int*>(count + CHUNK + STAGES * CHUNK);          // [STAGES][WARPS][VECS][5]
     __shared__ RowFacts facts[ROWS];
     __shared__ Bias biases[BIASES];
+    __shared__ int found;
     // the rows' ancestors [ROWS][words]; the nodes whose tokens a warp owns, by `head` [WARPS][4][words]; where the tree's drafted tokens lie
     // in the chunk, or -1 [words][32]
     unsigned* const paths = reinterpret_cast<unsigned*>(masks_at + STAGES * mask_room(VECS));
@@ -93,13 +94,16 @@ logit_rules_kernel(const RuleArgs A) {
     const long long units = (long long)((A.vocab + CHUNK - 1) / CHUNK) * A.rows;
     const long long from = units * blockIdx.x / gridDim.x, to = units * (blockIdx.x + 1) / gridDim.x;
     int lo = 0, n = 0, r0 = 0, rows = 0;       // the chunk's first token, its tokens; rows r0 .. r0 + rows - 1
-    int listed = 0;                            // their biases in `biases` (-1: a row by itself with more than fit)
+    int listed = 0;                            // their biases in `biases` (-1: of a row by itself, more than fit)
+    unsigned nodes_here = 0;                   // a bit per `head` at which the warp has drafted tokens of the tree
     int counted = -2, tree = -1;               // the list that `count` holds (-1: none), the tree that `node_at` does; of this chunk
 
     // The row's logits that lie on 16-byte boundaries are taken four at a time, behind `head` (0 to 3) that do not; `whole` fours.
-    auto head_of = [&](int k) { return min(n, (int)((16 - ((uintptr_t)(A.logits + (size_t)(r0 + k) * A.in_stride + lo) & 15)) & 15) / 4); };
+    const bool on_fours = ((uintptr_t)A.logits & 15) == 0 && A.in_stride % 4 == 0;             // then there are none of these anywhere
+    auto head_of = [&](int k) { return on_fours ? 0 : min(n, (int)((16 - ((uintptr_t)(A.logits + (size_t)(r0 + k) * A.in_stride + lo) & 15)) & 15) / 4); };
     // the warp that has element u of the chunk; the first one has those beside the fours
     auto owner = [&](int u, int head, int whole) { return u < head || u >= head + 4 * whole ? 0 : (u - head) >> 7 & (WARPS - 1); };
+    const int mask_word = (((lane / 5) * 4 * THREADS + warp * 128) >> 5) + lane % 5;
     // (every row is a group of copies, those behind the last row are empty)
     auto fetch = [&](int k) {
         if (k < rows) {
@@ -111,7 +115,7 @@ logit_rules_kernel(const RuleArgs A) {
             for (int j = 0; j < VECS; ++j)
                 if (tid + j * THREADS < whole) copy_async<16>(to + j * THREADS, from + j * THREADS);
             if (facts[k].mask >= 0 && lane < 5 * VECS) {         // the words of the warp's 128 tokens in each 1,024: four, or five off a word's start
-                const int word = ((lo + head + (lane / 5) * 4 * THREADS + warp * 128) >> 5) + lane % 5;
+                const int word = (lo >> 5) + mask_word;          // (a head of up to three tokens stays in the word)
                 if (word < A.mask_words) copy_async<4>(masks_at + (stage * WARPS + warp) * VECS * 5 + lane, A.mask + (size_t)facts[k].mask * A.mask_words + word);
             }
         }
@@ -161,18 +165,22 @@ logit_rules_kernel(const RuleArgs A) {
                     say(t.w, i + 3);
                 }
             }
-            if (A.drafted && f.first != tree)
+            if (A.drafted && f.first != tree) {
+                nodes_here = 0;
                 for (int h = 0; h < 4; ++h)                      // for every way that a row may lie
                     for (int w = 0; w < A.words; ++w) {
                         const int u = node_at[w * 32 + lane], head = min(n, h);
                         const unsigned mine = __ballot_sync(0xffffffffu, u >= 0 && owner(u, head, (n - head) / 4) == warp);
                         if (lane == 0) own_nodes[(warp * 4 + h) * A.words + w] = mine;
+                        if (mine) nodes_here |= 1u << h;
                     }
+            }
             __syncthreads();
             counted = f.list;
             tree = f.first;
         }
-        if (A.drafted) add_path(k, head, 1u);
+        const bool said_here = nodes_here >> head & 1u, biased_here = f.biased >> warp & 1u;
+        if (said_here) add_path(k, head, 1u);
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");      // this row is there
         __syncwarp();
         const float4* x = logits_at + stage * (CHUNK / 4) + tid;
@@ -232,13 +240,14 @@ logit_rules_kernel(const RuleArgs A) {
                 }
             }
         }
-        if (!A.drafted && !A.bias_start) return;
+        if (!said_here && !biased_here) return;
         __syncwarp();                          // the warp's counts have been read, its part of the row is written
-        if (A.drafted) add_path(k, head, 0xffffffffu);
-        if (listed > 0)
-            for (int i = lane; i < f.biases; i += 32) {
-                const Bias b = biases[f.bias - facts[0].bias + i];
-                if (b.u >= 0 && owner(b.u, head, whole) == warp && may_say(b.u)) out[b.u] += b.value;
+        if (said_here) add_path(k, head, 0xffffffffu);
+        if (biased_here && listed > 0)
+            for (int i = lane; i < listed; i += 32) {
+                const Bias b = biases[i];
+                const int u = b.at & 0xffff;
+                if (b.first && b.at >> 16 == k && owner(u, head, whole) == warp && may_say(u)) out[u] += b.value;
             }
         if (listed < 0)
             for (int i = lane; i < f.biases; i += 32) {
@@ -253,7 +262,6 @@ logit_rules_kernel(const RuleArgs A) {
                     if (tokens[j] == v) sum += A.bias_values[f.bias + j];
                 out[u] += sum;
             }
-        __syncwarp();
     };
     for (long long at = from; at < to; at += rows) {
         r0 = (int)(at % A.rows);
@@ -263,13 +271,6 @@ logit_rules_kernel(const RuleArgs A) {
             n = min(CHUNK, A.vocab - lo);
             counted = -2;
             tree = -1;
-        }
-        listed = 0;
-        if (A.bias_start) {                    // as many rows as have no more biases than there is room for
-            auto biases_to = [&](int r) { return (int)min((long long)max(0, A.bias_start[r]), A.bias_len); };
-            while (rows > 1 && biases_to(r0 + rows) - biases_to(r0) > BIASES) rows = (rows + 1) / 2;
-            listed = max(0, biases_to(r0 + rows) - biases_to(r0));
-            if (listed > BIASES) listed = -1;
         }
         __syncthreads();                       // (the rows before are done with)
         if (tid < rows) {
@@ -284,36 +285,84 @@ logit_rules_kernel(const RuleArgs A) {
             f.mask = A.mask == nullptr ? -1 : (A.mask_of_row ? A.mask_of_row[r] : r);
             if (f.mask < 0 || f.mask >= A.masks) f.mask = -1;
             f.first = A.drafted ? A.first_row[r] : 0;
-            f.bias = A.bias_start ? max(0, A.bias_start[r]) : 0;
+            f.bias = A.bias_start ? (int)min((long long)max(0, A.bias_start[r]), A.bias_len) : 0;
             f.biases = A.bias_start ? (int)max(0LL, min((long long)A.bias_start[r + 1], A.bias_len) - f.bias) : 0;
-            if (listed >= 0) {                 // (starts that do not ascend: no further than what is listed)
-                const int before = A.bias_start ? f.bias - max(0, A.bias_start[r0]) : 0;
-                f.biases = before < 0 ? 0 : max(0, min(f.biases, listed - before));
-            }
+            f.biased = 0u;
             facts[tid] = f;
         }
         for (int i = tid; i < rows * A.words; i += THREADS) paths[i] = A.ancestors[(size_t)r0 * A.words + i];
+        if (tid == 0) found = 0;
         __syncthreads();
         for (int k = 0; k < STAGES - 1; ++k) fetch(k);
+        listed = 0;
+        while (A.bias_start) {
+            // what the rows' entries say of tokens in the chunk; of fewer rows if that is more than there is room for
+            const int first = facts[0].bias, entries = max(0, facts[rows - 1].bias + facts[rows - 1].biases - first);
+            for (int i = tid; i < entries; i += THREADS) {
+                const int u = A.bias_tokens[first + i] - lo;
+                if ((unsigned)u >= (unsigned)n) continue;
+                int row = 0, to_row = rows;        // (the last row that begins at or before the entry; rows without entries begin where the next does)
+                while (to_row - row > 1) {
+                    const int mid = (row + to_row) >> 1;
+                    if (facts[mid].bias - first <= i) row = mid;
+                    else to_row = mid;
+                }
+                const int at = facts[row].bias - first;
+                if (i < at || i >= at + facts[row].biases) continue;        // (starts that do not ascend)
+                const int slot = atomicAdd(&found, 1);
+                if (slot < BIASES) biases[slot] = Bias{row << 16 | u, i, A.bias_values[first + i], 1};
+            }
+            __syncthreads();
+            listed = found;
+            if (listed <= BIASES) break;
+            if (rows == 1) {
+                listed = -1;
+                break;
+            }
+            rows = (rows + 1) / 2;
+            __syncthreads();
+            if (tid == 0) found = 0;
+            __syncthreads();
+        }
+        if (listed < 0) {
+            if (tid == 0) facts[0].biased = 0xffffffffu;
+            __syncthreads();
+        }
         if (listed > 0) {
             // a token that several of a row's entries name gets their sum, in their order, by the first of them
-            for (int i = tid; i < listed; i += THREADS) {
-                const long long e = facts[0].bias + i;
-                const int v = A.bias_tokens[e], u = v - lo;
-                Bias b{-1, 0.f};
-                if ((unsigned)u < (unsigned)n) {
-                    int row = 0;
-                    while (row + 1 < rows && facts[row + 1].bias <= e) ++row;
-                    bool mine = true;
-                    for (long long j = facts[row].bias; j < e && mine; ++j) mine = A.bias_tokens[j] != v;
-                    if (mine) {
-                        b.u = u;
-                        for (long long j = e; j < facts[row].bias + facts[row].biases; ++j)
-                            if (A.bias_tokens[j] == v) b.value += A.bias_values[j];
-                    }
+            float sums[(BIASES + THREADS - 1) / THREADS];
+#pragma unroll
+            for (int x = 0; x < (BIASES + THREADS - 1) / THREADS; ++x) {
+                const int i = tid + x * THREADS;
+                if (i >= listed) continue;
+                const Bias b = biases[i];
+                int next = 0x7fffffff;             // the earliest entry behind b for the same token
+                bool mine = true;
+                for (int j = 0; j < listed; ++j) {
+                    if (biases[j].at != b.at) continue;
+                    if (biases[j].entry < b.entry) mine = false;
+                    else if (biases[j].entry > b.entry) next = min(next, biases[j].entry);
                 }
-                biases[i] = b;
+                sums[x] = b.value;
+                while (mine && next != 0x7fffffff) {
+                    int after = 0x7fffffff;
+                    for (int j = 0; j < listed; ++j) {
+                        if (biases[j].at != b.at) continue;
+                        if (biases[j].entry == next) sums[x] += biases[j].value;
+                        else if (biases[j].entry > next) after = min(after, biases[j].entry);
+                    }
+                    next = after;
+                }
+                biases[i].first = mine;
+                if (mine) {
+                    const int row = b.at >> 16, head = head_of(row);
+                    atomicOr(&facts[row].biased, 1u << owner(b.at & 0xffff, head, (n - head) / 4));
+                }
             }
+            __syncthreads();                       // (the values have been read)
+#pragma unroll
+            for (int x = 0; x < (BIASES + THREADS - 1) / THREADS; ++x)
+                if (tid + x * THREADS < listed) biases[tid + x * THREADS].value = sums[x];
             __syncthreads();
         }
         for (int k = 0; k < rows; ++k) {
