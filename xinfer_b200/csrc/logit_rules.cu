@@ -71,8 +71,11 @@ constexpr int smem_of(int vecs, int words) { return 4 * (chunk_of(vecs) + STAGES
 // The vocabulary is cut into chunks of 1,024 VECS tokens, and the (chunk, row) pairs, chunk by chunk, into equal shares for as many blocks
 // as the device holds.  The lists' tokens are counted in shared memory, once for rows that follow each other with one list (the nodes of a
 // tree); a row's own path is added before it and taken away behind it.  A warp owns 128 of every 1,024 tokens, with their counts, mask
-// words and biases, so that the warps of a block go through the rows without waiting for each other; each has two more rows on their way.
-// Bound by memory: a logit is read and written once.
+// words and biases, so that the warps of a block go through the rows without waiting for each other; each has its next row on its way.
+// Bound by memory: a logit is read and written once.  512 rows of 151,936 with masks, biases and 8 histories of up to 4,096: 131 us, 4.75 TB/s (a
+// copy of as many bytes takes 97); the rest is the blocks' start (a history is counted by every block that meets it) and four blocks a
+// processor for want of shared memory.  With the next two rows on their way and three blocks 140 us, in chunks of 2,048 150 to 165.  A single
+// row of 151,936: 5.7 us, of which the launch and one trip for each of facts, history and logits are nearly all.
 template <int VECS>
 __global__ void __launch_bounds__(THREADS, 4)
 logit_rules_kernel(const RuleArgs A) {
@@ -378,9 +381,9 @@ int launch(const RuleArgs& A, cudaStream_t stream) {
     const int smem = smem_of(VECS, A.words);
     static unsigned long long roomy = 0;
     if (const int rc = xb_more_smem(logit_rules_kernel<VECS>, smem_of(VECS, WORDS), &roomy)) return rc;
-    // as many blocks as the device holds: 228 KB of shared memory a processor, of which every block takes its own, the static arrays and 1 KB
+    // as many blocks as the device holds: 228 KB of shared memory a processor, of which every block takes its own, the static arrays and 1 KB; four by their registers
     const int per_sm = (228 * 1024) / (smem + (int)(ROWS * sizeof(RowFacts) + BIASES * sizeof(Bias)) + 1024);
-    const int resident = (per_sm < 1 ? 1 : (per_sm > 8 ? 8 : per_sm)) * 148;
+    const int resident = (per_sm < 1 ? 1 : (per_sm > 4 ? 4 : per_sm)) * 148;
     const long long units = (long long)((A.vocab + chunk_of(VECS) - 1) / chunk_of(VECS)) * A.rows;
     return xb_launch(logit_rules_kernel<VECS>, dim3((unsigned)(units < resident ? units : resident)), dim3(THREADS), smem, stream, A);
 }
@@ -396,7 +399,8 @@ static int logit_rules(float* out, const float* logits, const float* penalties, 
     if (rows > (1 << 20) || words > WORDS || (mask && mask_words < (vocab + 31) / 32)) return (int)cudaErrorInvalidValue;
     const RuleArgs A{out, logits, penalties, history, history_start, prompt_len, list_of_row, drafted, ancestors, first_row, bias_start, bias_tokens,
                      bias_values, mask, mask_of_row, out_stride, in_stride, history_len, bias_len, rows, lists, vocab, words, masks, mask_words};
-    // chunks of 1,024 tokens while that leaves processors without work, of 4,096 when there are rows enough
-    return (long long)rows * vocab < 148LL * 2 * 4096 ? launch<1>(A, stream) : launch<4>(A, stream);
+    // Chunks of 1,024 tokens while those of 4,096 would leave half of the processors without work.  Small and large chunks measured: one row of
+    // 151,936 5.7 and 6.15 us, of 256,000 with 20,000 said 13.9 and 16.4; three rows of 151,936 6.9 and 6.4, four 8.4 and 6.7, seven 10.8 and 7.9.
+    return (long long)rows * vocab < 148LL * 2048 ? launch<1>(A, stream) : launch<4>(A, stream);
 }
 XB_EXPORT int xb_logit_rules(const long long* words, int n) { return xb_by_words(logit_rules, words, n); }
