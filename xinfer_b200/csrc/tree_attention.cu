@@ -14,8 +14,10 @@ using namespace xbtree;
 // The kernel for float32, and for what the tcgen05 kernel does not take (tree_attention_tc.cu): any head size, group and page.  A job's rows
 // are 32 (node, query head) pairs; a tile is 32 keys.  Scores are formed 2 rows x 4 keys a thread and values summed 4 rows x 4 channels at a
 // time, by float32 multiply-adds from shared memory; four lanes form the softmax of a row, eight keys each.  Jobs, tiles and the join are
-// those of the line in tree_attention.cuh, four blocks to a processor.  Bound by the multiply-adds' operands from shared memory: a score
-// or value product reads two numbers of it for every three it forms.
+// those of the line in tree_attention.cuh, four blocks to a processor.  Bound by the multiply-adds and their operands from shared memory (six
+// reads of four numbers for 32 multiply-adds): 8 trees of 64 nodes at up to 1,024 keys (32 heads over 8 of 128) 178 us, of which 5.6 GFLOP at
+// the multiply-adds' rate are 75; 32 of 16 at up to 2,000 305 us.  Few tokens are bound by trips: three trees of 13 at 777 keys with a window (10
+// heads over 5 of 48) 17 us: 2.2 until the first job is known, 1.2 pages and queries, 1.3 the tile, 2.1 its products, 0.7 the part, then the join.
 constexpr int RT = 32, KT = 32, THREADS = 128, LINE_BLOCKS = 4 * 148;
 
 // Four channels of a row from c on, zeros from d on; `fours`: rows start where four numbers may be read at once (and d is a multiple of 4).
@@ -325,7 +327,8 @@ tree_attention_kernel(const TreeArgs A, const Line line) {
 // Joins the parts of a job that several blocks shared, in an order that does not change: with M the largest of their maxima,
 // out = sum_i e^(m_i - M) O_i / sum_i e^(m_i - M) l_i.  A block per part, which takes as many of the job's rows.  Bound by trips to the L2: a warp
 // has eight pieces of rows on their way, of several rows where a job has few parts, and asks for them before it forms their factors; of a job
-// of more than eight parts the block's warps take a row together, every fourth part each.
+// of more than eight parts the block's warps take a row together, every fourth part each.  3 us for 15 jobs in 7 parts, 4.5 us for 8 jobs in 65
+// parts (a warp a row, four parts on their way: 4 and 11 us).
 constexpr int JOIN_WARPS = THREADS / 32, JOIN_TOGETHER = 8;
 
 struct JoinJob {

@@ -16,6 +16,19 @@
 // A value that a row does not see must not reach it, whatever it holds, but a product takes 0 * inf for NaN.  In tiles that not all rows
 // see alike (drafted keys, the edge of a window) the value rows are looked at: those that hold an infinity or NaN are zeroed for the
 // product, and the rows that do see them add their share to O by hand.  Value rows that nobody sees are zeroed too.
+//
+// What bounds it, and what it measured (bfloat16, 32 heads over 8 of 128 channels, pages of 16; both kernels, calls in a row):
+//   48 trees of 24 nodes, up to 32,768 keys   391 us, 5.6 TB/s: the cache's bytes (tiles of one row tile take 1,350 cycles, the memory's rate).
+//                                             Calls for seconds on end run into the power limit: 415 to 470 us
+//   64 trees of 8, up to 4,096                84 us, 4.6 TB/s: the same, with a job's start every 28 tiles
+//   32 trees of 64, up to 8,192               113 us: jobs of two row tiles take about 2,000 cycles a tile of keys: exponentials (a quarter of them
+//                                             by a polynomial), maxima and conversions of 64 scores a thread, two such warps to an issue slot
+//   8 trees of 64, up to 4,096                33 us: 5 until the first scores, 14 of tiles, 2.4 to write the parts (19 MB at the L2's rate), 2.3
+//                                             until the join's blocks are there, 7 of join
+//   1 tree of 16, 1,024 keys (16 heads)       13.6 us: a chain of trips to memory.  In cycles: lengths 1,300, the place in the line 1,350, the
+//                                             first segment 1,650, pages and the first tile 1,300, then four tiles, the part and the join
+// A block reads 32 KB a tile with at least three tiles on their way, so boxes of both halves of a page (half as many copies) were no faster, and
+// 5 % slower where memory is the bound.
 #include "tc_common.cuh"
 #include "tree_attention.cuh"
 
@@ -756,7 +769,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 // Joins the parts of a job that several blocks shared, in the order of the parts: with M the largest of their maxima,
 // out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.  Grid (block and which of its parts, MERGE_Y): as many of the job's rows as the part is
 // of the job, so that there are as many blocks at work as there are parts.  A thread has four channels of a row in every group of eight
-// rows and requests eight numbers of four at once: P parts of 8 / P groups.  The join is then a trip or two to the L2.
+// rows and requests eight numbers of four at once: P parts of 8 / P groups.  Bound by trips to the L2 (the told job, maxima and sums, the
+// parts): 7 us for 64 jobs of 256 rows in 211 parts (27 MB), 2.5 us for 8 jobs of 32 rows.  Two blocks a part with twice the work, more
+// blocks a processor, or the parts asked for before the factors: 1 to 8 % longer.
 constexpr int MERGE_Y = 4;
 constexpr int MERGE_ROWS = 32;     // rows whose factors lie in shared memory
 
