@@ -190,19 +190,22 @@ cache_slots_kernel(const SlotArgs A) {
 
 // ---- accepted rows into the cache ------------------------------------------------------------------------------------------
 // Token i of the step (slots[i], the o-th new one of request b = request_of[i], o = i - token_start[b]) is drafted row path[b][o]:
-// its keys and values of every layer go to its slot.  Grid (token, layer): 128 threads copy the 2 x 2 KB of 8 heads of 128 channels with one
-// read of 16 bytes each in flight.  Bound by memory: 452 accepted tokens in 36 layers (133 MB read and written) 27.5 us, with a cold L2 35; four in
-// 28 layers 2.4 us.  U: the unit of the copy, two bytes where a head's row is no multiple of 16.
+// its keys and values of every layer go to its slot.  Grid (token, some layers); U: the unit of the copy, two bytes where a head's row is no
+// multiple of 16.  A block finds its token's row and slot by four trips to memory, so it copies several layers where there are blocks
+// enough, with four units a thread on their way.  Bound by memory and these trips: 452 accepted tokens in 36 layers (133 MB read and written) 25
+// us, with a cold L2 33 (a copy of as many bytes takes 20); four in 28 layers 2.8 us.
+constexpr int COMMIT_THREADS = 256, COMMIT_AHEAD = 4;
 template <typename U>
-__global__ void cache_commit_kernel(const void* const* layers /* [layers][4]: k cache, v cache, new k, new v */, const long long* slots,
-                                    const int* request_of, const int* token_start, const int* path, int requests, int width, int rows, int nkv,
-                                    int units, int page_size, long long num_slots, int* err) {
+__global__ void __launch_bounds__(COMMIT_THREADS)
+cache_commit_kernel(const void* const* layers /* [layers][4]: k cache, v cache, new k, new v */, int num_layers, int layers_each, const long long* slots,
+                    const int* request_of, const int* token_start, const int* path, int requests, int width, int rows, int nkv,
+                    int units, int page_size, long long num_slots, int* err) {
     pdl_launch_dependents();
     pdl_wait();
     const int i = blockIdx.x;
     const int b = request_of[i];
-    if (b < 0 || b >= requests) return;
     const long long slot = slots[i];
+    if (b < 0 || b >= requests) return;
     const int o = i - token_start[b];
     if (slot < 0 || o < 0 || o >= width) return;
     const int row = path[(size_t)b * width + o];
@@ -211,13 +214,20 @@ __global__ void cache_commit_kernel(const void* const* layers /* [layers][4]: k 
         if (threadIdx.x == 0) atomicOr(err, row >= rows ? XB_ERR_BAD_ROW : XB_ERR_BAD_PAGE);
         return;
     }
-    const void* const* mine = layers + 4 * (size_t)blockIdx.y;
     const long long page = slot / page_size, off = slot % page_size;
-    for (int c = threadIdx.x; c < 2 * nkv * units; c += blockDim.x) {
+    const int l0 = blockIdx.y * layers_each, l1 = min(l0 + layers_each, num_layers);
+    for (int c = threadIdx.x; c < 2 * nkv * units; c += COMMIT_THREADS) {
         const int what = c / (nkv * units), g = c / units % nkv, u = c % units;
-        const U* src = (const U*)mine[2 + what];
-        U* dst = (U*)mine[what];
-        dst[((page * nkv + g) * page_size + off) * units + u] = src[((long long)row * nkv + g) * units + u];
+        const long long to = ((page * nkv + g) * page_size + off) * units + u, from = ((long long)row * nkv + g) * units + u;
+        for (int l = l0; l < l1; l += COMMIT_AHEAD) {
+            U v[COMMIT_AHEAD];
+#pragma unroll
+            for (int k = 0; k < COMMIT_AHEAD; ++k)
+                if (l + k < l1) v[k] = ((const U*)layers[4 * (l + k) + 2 + what])[from];
+#pragma unroll
+            for (int k = 0; k < COMMIT_AHEAD; ++k)
+                if (l + k < l1) ((U*)const_cast<void*>(layers[4 * (l + k) + what]))[to] = v[k];
+        }
     }
 }
 
@@ -255,9 +265,15 @@ static int cache_commit(const void* const* layers, int num_layers, const long lo
                         int* err, cudaStream_t stream) {
     if (tokens <= 0 || num_layers <= 0 || requests <= 0) return 0;
     if (num_layers > 65535 || row_bytes < 2 || row_bytes % 2 || page_size < 1) return (int)cudaErrorInvalidValue;
-    const dim3 grid(tokens, num_layers);
+    // Layers of a block: as many as leave four blocks a processor, up to 16.  One layer a block and this rule: 1,000 tokens of 24 layers (4 heads of
+    // 64) 26.4 and 10.3 us, 452 of 36 (8 of 128) 28.0 and 25.4, 100 of 36 7.7 and 5.6, 30 of 28 in float32 7.1 and 5.1; eight blocks a processor: 6.3
+    // and 6.9 for the last two, 24.8 for 452.
+    const long long share = (long long)tokens * num_layers / (148 * 4);
+    const int each = share < 1 ? 1 : (share > 16 ? 16 : (int)share);
+    const dim3 grid(tokens, (num_layers + each - 1) / each);
     auto go = [&](auto kernel, int unit) {
-        return xb_launch(kernel, grid, dim3(128), 0, stream, layers, slots, request_of, token_start, path, requests, width, rows, nkv, row_bytes / unit, page_size, num_slots, err);
+        return xb_launch(kernel, grid, dim3(COMMIT_THREADS), 0, stream, layers, num_layers, each, slots, request_of, token_start, path, requests, width, rows, nkv,
+                         row_bytes / unit, page_size, num_slots, err);
     };
     return row_bytes % 16 == 0 ? go(cache_commit_kernel<uint4>, 16) : go(cache_commit_kernel<uint16_t>, 2);
 }
