@@ -892,6 +892,18 @@ __global__ void tree_dense_rows_kernel(__nv_bfloat16* to, const TreeArgs A) {
     }
 }
 
+// A bfloat16 tensor of `RANK` dimensions, innermost first, `strides` elements apart, through boxes in the 128-byte swizzle.
+template <int RANK>
+bool map_of(CUtensorMap* out, const void* ptr, const long long (&dims)[RANK], const long long (&strides)[RANK - 1], const int (&box)[RANK]) {
+    const EncodeTiledFn fn = encode_fn();
+    cuuint64_t dim[RANK], stride[RANK - 1];
+    cuuint32_t boxes[RANK], each[RANK];
+    for (int i = 0; i < RANK; ++i) dim[i] = (cuuint64_t)dims[i], boxes[i] = (cuuint32_t)box[i], each[i] = 1;
+    for (int i = 0; i + 1 < RANK; ++i) stride[i] = (cuuint64_t)strides[i] * 2;
+    return fn && fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, RANK, const_cast<void*>(ptr), dim, stride, boxes, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int DP>
 int launch_tc(const TreeArgs& A, const Line& line, cudaStream_t stream) {
     constexpr int NS = stages(DP);
@@ -903,11 +915,9 @@ int launch_tc(const TreeArgs& A, const Line& line, cudaStream_t stream) {
     while ((1 << shift) < A.page_size) ++shift;
     CUtensorMap mq, mk, mv, mkn, mvn;
     const long long rows = (long long)A.num_pages * A.nkv * A.page_size;
-    const long long dq[3] = {A.d, A.nh, A.tokens}, dn[3] = {A.d, A.nkv, A.tokens};
-    const long long sq[2] = {A.d, A.q_stride}, sk[2] = {A.d, A.k_stride}, sv[2] = {A.d, A.v_stride};
-    const int bq[3] = {64, G, line.two_from}, bn[3] = {64, 1, KT};
-    if (!tensor_map_bf16(&mq, A.q, 3, dq, sq, bq) || !tensor_map_2d(&mk, A.k_cache, rows, A.d, box_rows) || !tensor_map_2d(&mv, A.v_cache, rows, A.d, box_rows) ||
-        !tensor_map_bf16(&mkn, A.k_new, 3, dn, sk, bn) || !tensor_map_bf16(&mvn, A.v_new, 3, dn, sv, bn))
+    if (!map_of<3>(&mq, A.q, {A.d, A.nh, A.tokens}, {A.d, A.q_stride}, {64, G, line.two_from}) || !map_of<2>(&mk, A.k_cache, {A.d, rows}, {A.d}, {64, box_rows}) ||
+        !map_of<2>(&mv, A.v_cache, {A.d, rows}, {A.d}, {64, box_rows}) || !map_of<3>(&mkn, A.k_new, {A.d, A.nkv, A.tokens}, {A.d, A.k_stride}, {64, 1, KT}) ||
+        !map_of<3>(&mvn, A.v_new, {A.d, A.nkv, A.tokens}, {A.d, A.v_stride}, {64, 1, KT}))
         return (int)cudaErrorInvalidValue;
     const int rc = xb_launch(tree_attention_tc_kernel<DP>, dim3(LINE_BLOCKS), dim3(THREADS), smem, stream, mq, mk, mv, mkn, mvn, A, line, shift, A.scale * 1.4426950408889634f);
     if (rc) return rc;
