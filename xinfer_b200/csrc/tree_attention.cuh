@@ -51,7 +51,7 @@ __device__ __forceinline__ int request_of(const TreeArgs& A, int t) {
 // costs: block c takes the tiles that begin in c * share .. (c + 1) * share - 1, whatever the lengths are, so that blocks finish together and
 // nobody has to know the lengths on the host.
 constexpr int LINE_REQUESTS = 8192;
-constexpr int COST_ONE = 2;        // what a tile of keys costs a job of one tile of rows, and of two: 1,400 and 2,150 cycles measured
+constexpr int COST_ONE = 2;        // what a tile of keys costs a job of one tile of rows, and of two: 1,350 and 2,000 cycles measured
 constexpr int COST_TWO = 3;
 constexpr int COST_JOB = 12;       // what a job costs beside its tiles: its last, drafted keys and its result
 
@@ -73,6 +73,10 @@ struct RequestLine {
     int per_tile;                  // what a tile costs each of its jobs
     __device__ __forceinline__ int job_units() const { return tiles * per_tile + COST_JOB; }
     __device__ __forceinline__ int units(int nkv) const { return nkv * pieces * job_units(); }
+    __device__ __forceinline__ RequestLine of_lane(int l) const {
+        auto from = [&](int v) { return __shfl_sync(0xffffffffu, v, l); };
+        return RequestLine{from(first), from(nodes), from(context), from(tile0), from(old_tiles), from(tiles), from(pieces), from(per_tile)};
+    }
 };
 
 template <int KT>
@@ -127,18 +131,23 @@ __device__ __forceinline__ Walk place_in_line(const TreeArgs& A, const Line& lin
     int before = incl - mine, b = b0;
     const unsigned who = __ballot_sync(0xffffffffu, w.from >= before && w.from < incl);
     const int owner = __ffs(who) - 1;
-    if (lane == owner) {
+    if (each > 1) {
+        if (lane == owner) {
 #pragma unroll 1
-        for (; b < b1; ++b) {
-            if (each > 1) w.r = request_line<KT>(A, line, b);
-            const int n = w.r.units(A.nkv);
-            if (w.from < before + n) break;
-            before += n;
+            for (; b < b1; ++b) {
+                w.r = request_line<KT>(A, line, b);
+                const int n = w.r.units(A.nkv);
+                if (w.from < before + n) break;
+                before += n;
+            }
         }
+        w.b = __shfl_sync(0xffffffffu, b, owner);
+        w.r = request_line<KT>(A, line, w.b);
+    } else {                           // a lane has one request: the owner's, without another trip
+        w.b = owner;
+        w.r = w.r.of_lane(owner);
     }
-    w.b = __shfl_sync(0xffffffffu, b, owner);
     before = __shfl_sync(0xffffffffu, before, owner);
-    w.r = request_line<KT>(A, line, w.b);
     const int length = w.r.job_units(), at = (w.from - before) / length;
     w.g = at / w.r.pieces;
     w.piece = at % w.r.pieces;

@@ -25,7 +25,7 @@
 //                                             by a polynomial), maxima and conversions of 64 scores a thread, two such warps to an issue slot
 //   8 trees of 64, up to 4,096                33 us: 5 until the first scores, 14 of tiles, 2.4 to write the parts (19 MB at the L2's rate), 2.3
 //                                             until the join's blocks are there, 7 of join
-//   1 tree of 16, 1,024 keys (16 heads)       13.6 us: a chain of trips to memory.  In cycles: lengths 1,300, the place in the line 1,350, the
+//   1 tree of 16, 1,024 keys (16 heads)       13.6 us: a chain of trips to memory.  In cycles: lengths 1,300, the place in the line 1,000, the
 //                                             first segment 1,650, pages and the first tile 1,300, then four tiles, the part and the join
 // A block reads 32 KB a tile with at least three tiles on their way, so boxes of both halves of a page (half as many copies) were no faster, and
 // 5 % slower where memory is the bound.
