@@ -200,3 +200,42 @@ def test_places_that_make_no_sense_reach_nothing():
             # what lies outside the ascending part is not said by the rule, but every number is the logit or the logit and its bias
             there = (out[r] == x[r]) | (out[r] == x[r] + 1.0)
             assert bool(there.all()) and bool((out[r, 5:] == x[r, 5:]).all())
+
+
+def edge_tokens(vocab):
+    """Tokens around the places where one warp's tokens end and the next one's begin, and those around the chunks' ends."""
+    at = [e + i for e in range(128, vocab, 128) for i in range(-2, 4)] + [c + i for c in range(1024, vocab, 1024) for i in range(-4, 1)] + [vocab - 1 - i for i in range(4)]
+    return np.array(sorted({t for t in at if 0 <= t < vocab}))
+
+
+@pytest.mark.parametrize("vocab,gap,trees", [(3001, 0, 2), (3001, 2, 2), (40001, 0, 2), (40001, 1, 2), (50257, 0, 8), (3001, 3, 2), (331, 0, 3)])
+def test_paths_of_rows_that_start_at_different_places(vocab, gap, trees):
+    """Rows of a tree that start anywhere modulo 16 bytes: a warp's share of the tokens moves from row to row, the counts do not."""
+    from xinfer_b200 import kernels as k
+    rng = np.random.default_rng(vocab + gap)
+    nodes, R = 60, 60 * trees
+    few = np.concatenate([np.arange(126, 132), np.arange(254, 260)])
+    near = edge_tokens(vocab)
+    drafted, masks, paths = [], [], []
+    for b in range(trees):
+        _, _, on = tree(rng, nodes)
+        toks = np.where(rng.random(nodes) < 0.6, rng.choice(few, nodes), rng.choice(near, nodes))
+        drafted += toks.tolist()
+        paths += [[int(toks[i]) for i in np.flatnonzero(on[r])] for r in range(nodes)]
+        masks.append(words_of(on, 2))
+    first, list_of_row = np.repeat(np.arange(trees) * nodes, nodes), np.repeat(np.arange(trees) // 2, nodes)
+    lists = [rng.choice(near, 40).tolist() for _ in range((trees + 1) // 2)]
+    logits, pen, prompt, ref, bound = case_of_rows(rng, R, vocab, lists, list_of_row.tolist(), paths)
+    wide = torch.zeros(R, vocab + gap, device=DEV)
+    wide[:, :vocab] = torch.tensor(logits, device=DEV)
+    x, out = wide[:, :vocab], torch.full((R, vocab), 99.0, device=DEV)
+    args = (torch.tensor(pen, device=DEV), i32(np.concatenate(lists)), i32(np.concatenate([[0], np.cumsum([len(t) for t in lists])])), i32(prompt))
+    more = dict(list_of_row=i32(list_of_row), tree=(i32(drafted), torch.cat(masks).to(DEV), i32(first)))
+    k.logit_rules(out, x, *args, **more)
+    assert (np.abs(out.double().cpu().numpy() - ref) <= bound).all()
+    again = torch.empty_like(out)
+    for _ in range(50):
+        k.logit_rules(again, x, *args, **more)
+        assert torch.equal(again, out)
+    k.logit_rules(x, x, *args, **more)                     # in place
+    assert torch.equal(x, out) and bool((wide[:, vocab:] == 0.0).all())

@@ -72,6 +72,8 @@ constexpr int smem_of(int vecs, int words) { return 4 * (chunk_of(vecs) + STAGES
 // as the device holds.  The lists' tokens are counted in shared memory, once for rows that follow each other with one list (the nodes of a
 // tree); a row's own path is added before it and taken away behind it.  A warp owns 128 of every 1,024 tokens, with their counts, mask
 // words and biases, so that the warps of a block go through the rows without waiting for each other; each has its next row on its way.
+// Which 128 these are goes by where a row starts, so rows of trees that do not all start alike on 16 bytes have a barrier between them: a
+// count that one warp raises for its row may be another one's in the next (512 rows of 151,935 so: 150 us).
 // Bound by memory: a logit is read and written once.  512 rows of 151,936 with masks, biases and 8 histories of up to 4,096: 131 us, 4.75 TB/s (a
 // copy of as many bytes takes 97); the rest is the blocks' start (a history is counted by every block that meets it) and four blocks a
 // processor for want of shared memory.  With the next two rows on their way and three blocks 140 us, in chunks of 2,048 150 to 165.  A single
@@ -103,6 +105,7 @@ logit_rules_kernel(const RuleArgs A) {
 
     // The row's logits that lie on 16-byte boundaries are taken four at a time, behind `head` (0 to 3) that do not; `whole` fours.
     const bool on_fours = ((uintptr_t)A.logits & 15) == 0 && A.in_stride % 4 == 0;             // then there are none of these anywhere
+    const bool owners_move = A.drafted && A.in_stride % 4 != 0;                                // `head` differs from row to row
     auto head_of = [&](int k) { return on_fours ? 0 : min(n, (int)((16 - ((uintptr_t)(A.logits + (size_t)(r0 + k) * A.in_stride + lo) & 15)) & 15) / 4); };
     // the warp that has element u of the chunk; the first one has those beside the fours
     auto owner = [&](int u, int head, int whole) { return u < head || u >= head + 4 * whole ? 0 : (u - head) >> 7 & (WARPS - 1); };
@@ -369,6 +372,7 @@ logit_rules_kernel(const RuleArgs A) {
             __syncthreads();
         }
         for (int k = 0; k < rows; ++k) {
+            if (owners_move && k > 0) __syncthreads();     // the row before has taken its path's counts away, whosever they are now
             work(k);
             fetch(k + STAGES - 1);             // (into the stage of row k - 1, which this warp alone reads and has read)
         }
