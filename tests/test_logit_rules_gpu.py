@@ -239,3 +239,19 @@ def test_paths_of_rows_that_start_at_different_places(vocab, gap, trees):
         assert torch.equal(again, out)
     k.logit_rules(x, x, *args, **more)                     # in place
     assert torch.equal(x, out) and bool((wide[:, vocab:] == 0.0).all())
+
+
+@pytest.mark.parametrize("vocab", [3004, 50_000, 700_001])
+@pytest.mark.parametrize("none", [-1, -2, -33, -1025])
+def test_rows_whose_tree_begins_before_the_first_row(vocab, none):
+    """Node i is row first_row + i where there is one, whatever first_row is; in every chunk of the vocabulary."""
+    rng = np.random.default_rng(vocab - none)
+    R = 9
+    drafted = rng.choice(np.array([1, 5, 1030, 1031, 2050, 3003, vocab // 2, vocab - 1]) % vocab, R)
+    first = np.array([none, none, none, 2, 2, none, none, 2 ** 31 - 1, none])
+    on = rng.random((R, 64)) < 0.5
+    paths = [[int(drafted[first[r] + i]) for i in range(64) if on[r, i] and 0 <= first[r] + i < R] for r in range(R)]
+    lists = [rng.integers(0, vocab, 30).tolist()]
+    logits, pen, prompt, ref, bound = case_of_rows(rng, R, vocab, lists, [0] * R, paths)
+    got = call(logits, pen, lists, prompt, [0] * R, first, drafted, words_of(on, 2), None, None, None).double().cpu().numpy()
+    assert (np.abs(got - ref) <= bound).all()

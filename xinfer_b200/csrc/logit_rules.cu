@@ -43,6 +43,7 @@ __device__ __forceinline__ float ruled(float x, unsigned count, float rep, float
 constexpr int WARPS = THREADS / 32;
 constexpr int ROWS = 48;                        // rows at a time: what they need to know lies in shared memory
 constexpr int WORDS = 32;                       // words of ancestors: trees of up to 1,024 nodes
+constexpr int NO_TREE = -32 * WORDS - 1;        // no row's tree: one that begins so far before the first row has no node, and all such are one
 constexpr int BIASES = 192;                     // biases of these rows that lie in the chunk
 constexpr int STAGES = 2;                       // rows on their way or worked on
 
@@ -101,7 +102,7 @@ logit_rules_kernel(const RuleArgs A) {
     int lo = 0, n = 0, r0 = 0, rows = 0;       // the chunk's first token, its tokens; rows r0 .. r0 + rows - 1
     int listed = 0;                            // their biases in `biases` (-1: of a row by itself, more than fit)
     unsigned nodes_here = 0;                   // a bit per `head` at which the warp has drafted tokens of the tree
-    int counted = -2, tree = -1;               // the list that `count` holds (-1: none), the tree that `node_at` does; of this chunk
+    int counted = -2, tree = NO_TREE;          // the list that `count` holds (-1: none), the tree that `node_at` does; of this chunk
 
     // The row's logits that lie on 16-byte boundaries are taken four at a time, behind `head` (0 to 3) that do not; `whole` fours.
     const bool on_fours = ((uintptr_t)A.logits & 15) == 0 && A.in_stride % 4 == 0;             // then there are none of these anywhere
@@ -276,7 +277,7 @@ logit_rules_kernel(const RuleArgs A) {
             lo = (int)(at / A.rows) * CHUNK;
             n = min(CHUNK, A.vocab - lo);
             counted = -2;
-            tree = -1;
+            tree = NO_TREE;
         }
         __syncthreads();                       // (the rows before are done with)
         if (tid < rows) {
@@ -290,7 +291,7 @@ logit_rules_kernel(const RuleArgs A) {
             if (f.list < 0 || f.list >= A.lists) f.list = -1;
             f.mask = A.mask == nullptr ? -1 : (A.mask_of_row ? A.mask_of_row[r] : r);
             if (f.mask < 0 || f.mask >= A.masks) f.mask = -1;
-            f.first = A.drafted ? A.first_row[r] : 0;
+            f.first = A.drafted ? max(A.first_row[r], NO_TREE + 1) : 0;
             f.bias = A.bias_start ? (int)min((long long)max(0, A.bias_start[r]), A.bias_len) : 0;
             f.biases = A.bias_start ? (int)max(0LL, min((long long)A.bias_start[r + 1], A.bias_len) - f.bias) : 0;
             f.biased = 0u;
