@@ -338,3 +338,17 @@ def test_more_refusals():
         with pytest.raises(k.KernelError):
             k.tree_attention(**{**args, **change})
     assert int(args["err"]) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("window", [None, 30])
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-41, -1e-41, 0.125])
+def test_any_scale(dtype, window, scale):
+    """A factor of zero weighs all keys that are seen alike, one below zero those of opposite queries; what is not seen stays out."""
+    s = Step([33, 70, 1], [100, 700, 64], 8, 2, 64, 16, dtype)
+    s.scale = scale
+    out = s.run(window)
+    assert int(s.err) == 0
+    if scale < 0:                          # (the bound goes by the products' sizes)
+        s.q, s.scale = -s.q, -scale
+    s.check(out, window)

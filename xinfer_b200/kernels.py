@@ -1827,7 +1827,8 @@ def tree_attention(out, q, k_new, v_new, k_cache, v_cache, context, token_start,
     keys and the drafted tokens of its request whose bits are set in ``ancestors[i]`` (int32 words, the tree's first token the
     lowest bit; its own bit as well as any).  ``window``: of these, the ones fewer than that many positions before it, by ``depth``
     (int32: a token's position is the context plus its depth).  A token that sees nothing gets zeros.  ``out``, ``q``, ``k_new``
-    and ``v_new`` have dense heads, their tokens may lie apart.  ``scratch``: float32, ``tree_attention_scratch`` numbers, contents
+    and ``v_new`` have dense heads, their tokens may lie apart.  ``scale`` may be any number (in bfloat16 the tensor cores take those above
+    zero).  ``scratch``: float32, ``tree_attention_scratch`` numbers, contents
     undefined, not shared by calls that may overlap."""
     T, nh, d = q.shape
     nkv = k_new.shape[1]
