@@ -352,3 +352,16 @@ def test_any_scale(dtype, window, scale):
     if scale < 0:                          # (the bound goes by the products' sizes)
         s.q, s.scale = -s.q, -scale
     s.check(out, window)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("width", [0, 2])
+def test_a_cache_without_pages(dtype, width):
+    """Trees behind nothing at all: no page has been made yet."""
+    from xinfer_b200 import kernels as k
+    s = Step([20, 70], [0, 0], 8, 2, 64, 16, dtype)
+    s.kc, s.vc, s.table = s.kc[:0], s.vc[:0], torch.full((2, width), -1, dtype=torch.int32)
+    s.check(s.run())
+    assert int(s.err) == 0
+    s.contexts = [5, 0]
+    assert torch.isfinite(s.run()).all() and int(s.err) == k.ERR_BAD_PAGE

@@ -929,10 +929,11 @@ int launch_tc(const TreeArgs& A, const Line& line, cudaStream_t stream) {
 namespace xbtree {
 
 // (Unseen keys are set to -inf before the scores are scaled, so the factor has to be above zero, and by so much that no product with it is
-// taken for zero; the other kernel scales first.)
+// taken for zero; the other kernel scales first.  A cache without pages has no tensor map.)
 bool tree_tc_takes(const TreeArgs& A) {
-    return A.scale >= 1.17549435e-38f && A.d % 16 == 0 && A.d >= 16 && A.d <= 128 && A.nh / A.nkv <= RT && A.page_size >= 8 && (A.page_size & (A.page_size - 1)) == 0 &&
-           ((long long)A.num_pages + 1) * A.nkv * A.page_size < (1LL << 31) && rows_on_16_bytes(A.k_cache, 0) && rows_on_16_bytes(A.v_cache, 0);
+    return A.scale >= 1.17549435e-38f && A.d % 16 == 0 && A.d >= 16 && A.d <= 128 && A.nh / A.nkv <= RT && A.page_size >= 8 &&
+           (A.page_size & (A.page_size - 1)) == 0 && A.num_pages > 0 && ((long long)A.num_pages + 1) * A.nkv * A.page_size < (1LL << 31) &&
+           rows_on_16_bytes(A.k_cache, 0) && rows_on_16_bytes(A.v_cache, 0);
 }
 
 static int part_rows_of(int tokens, int group) {
