@@ -1,4 +1,8 @@
 """Acceptance of drafted tokens, slots from lengths on the device and the commit of accepted rows, against plain loops."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -252,3 +256,16 @@ def test_slots_of_the_most_requests():
     new = rng.choice([0, 1, 2, 9, -1], B).tolist()
     lengths = rng.integers(0, 40, B).tolist()
     check_slots(Cache(rng, lengths, 16, 3000, 5), new)
+
+
+@pytest.mark.parametrize("requests", [4083, 4084, 4095, 4096])
+def test_slots_of_as_many_requests_as_fill_the_memory_that_needs_no_asking(requests):
+    """In a process of its own: a larger call before it has asked for more shared memory, for all calls after it."""
+    code = ("import sys; sys.path[:0] = sys.argv[1:3]\n"
+            "import numpy as np, test_tree_step_gpu as t\n"
+            f"rng = np.random.default_rng({requests})\n"
+            f"lengths, new = rng.integers(0, 40, {requests}).tolist(), rng.choice([0, 1, 2, 9, -1], {requests}).tolist()\n"
+            "t.check_slots(t.Cache(rng, lengths, 16, 3000, 5), new)\n")
+    here = os.path.dirname(os.path.abspath(__file__))
+    done = subprocess.run([sys.executable, "-c", code, here, os.path.dirname(here)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]

@@ -252,10 +252,9 @@ static int cache_slots(long long* slots, int* positions, int* request, int* toke
                      requests, capacity, table_stride, page_size, ring_size, err};
     int blocks = (capacity + SLOT_THREADS - 1) / SLOT_THREADS;
     blocks = blocks < 4 ? 4 : (blocks > 148 ? 148 : blocks);    // (four also where few tokens come: pages are given back beside them)
-    const size_t smem = (3 * (size_t)requests + 1) * 4;
+    const size_t smem = (3 * (size_t)requests + 1) * 4;         // (with the kernel's own arrays above the default from 4,084 requests on)
     static unsigned long long roomy = 0;
-    if (smem > 48 * 1024)
-        if (const int rc = xb_more_smem(cache_slots_kernel, (3 * SLOT_REQUESTS + 1) * 4, &roomy)) return rc;
+    if (const int rc = xb_more_smem(cache_slots_kernel, (3 * SLOT_REQUESTS + 1) * 4, &roomy)) return rc;
     return xb_launch(cache_slots_kernel, dim3(blocks), dim3(SLOT_THREADS), smem, stream, A);
 }
 XB_EXPORT int xb_cache_slots(const long long* words, int n) { return xb_by_words(cache_slots, words, n); }
