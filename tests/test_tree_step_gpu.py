@@ -269,3 +269,23 @@ def test_slots_of_as_many_requests_as_fill_the_memory_that_needs_no_asking(reque
     here = os.path.dirname(os.path.abspath(__file__))
     done = subprocess.run([sys.executable, "-c", code, here, os.path.dirname(here)], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("new", [9, 10, 20, 2 ** 31 - 1])
+def test_slots_of_lengths_at_the_end_of_32_bits(new):
+    """A length that 32 bits do not hold is refused like one that its row of the table does not hold; the largest one is served."""
+    from xinfer_b200 import kernels as k
+    rng = np.random.default_rng(11)
+    n, ps = 2 ** 31 - 10, 2 ** 30
+    c = Cache(rng, [n, 7], ps, 4, 5)
+    rows = [list(r) for r in c.rows]
+    got = run_slots(c, [new, 2], 24)
+    at = [rows[0][1] * ps + i - ps for i in range(n, n + 9)]
+    beside = [rows[1][0] * ps + 7, rows[1][0] * ps + 8]
+    if new == 9:
+        assert got["err"] == 0 and got["lengths"] == [2 ** 31 - 1, 9] and got["slots"] == at + beside + [-1] * 13 and got["pos"][:11] == list(range(n, n + 9)) + [7, 8]
+    else:
+        mine = min(new, 24)
+        assert got["err"] == k.ERR_NO_PAGE | (k.ERR_BAD_ROW if new > 24 else 0) and got["lengths"] == [n, 9]
+        assert got["slots"] == ([-1] * mine + beside + [-1] * 24)[:24] and got["pos"][:mine] == [min(i, 2 ** 31 - 1) for i in range(n, n + mine)]
+    assert got["ring"][1] == 4 and got["start"] == [0, new, min(new + 2, 2 ** 31 - 1)]

@@ -114,8 +114,12 @@ cache_slots_kernel(const SlotArgs A) {
     pdl_wait();
     const int each = (A.requests + SLOT_THREADS - 1) / SLOT_THREADS, b0 = (int)threadIdx.x * each, b1 = min(b0 + each, A.requests);
     const int ps = A.page_size, head = (A.ring[0] % A.ring_size + A.ring_size) % A.ring_size, count = min(max(A.ring[1], 0), A.ring_size);
-    // whether the request's pages, those it holds and those it asks for, fit its row of the table; one whose do not asks for none
-    auto fits = [&](int len, int add) { return ((long long)len + max(add, 0) + ps - 1) / ps <= A.table_stride; };
+    // whether the request's pages, those it holds and those it asks for, fit its row of the table, and its length 32 bits; one whose do not
+    // asks for none
+    auto fits = [&](int len, int add) {
+        const long long all = (long long)len + max(add, 0);
+        return all <= 0x7fffffffLL && (all + ps - 1) / ps <= A.table_stride;
+    };
     auto pages = [&](int len) { return (int)(((long long)len + ps - 1) / ps); };
     auto sums_of = [&](int len, int add) {
         if (!fits(len, add)) return Sums{max(add, 0), 0, 0};
@@ -175,9 +179,9 @@ cache_slots_kernel(const SlotArgs A) {
             continue;
         }
         const int b = run_of(t, A.requests, [&](int b) { return starts[b]; });
-        const int len = max(A.lengths[b], 0), pos = len + t - starts[b], place = pos / ps, held = pages(len);
+        const int len = max(A.lengths[b], 0), pos = (int)min((long long)len + (t - starts[b]), 0x7fffffffLL), place = pos / ps, held = pages(len);
         long long slot = -1;
-        if (need_before[b] >= 0) {
+        if (need_before[b] >= 0) {                               // (then its positions are all below its new length)
             const int page = place < held ? A.table[(size_t)b * A.table_stride + place] : A.free_ring[ring_at(need_before[b] + place - held)];
             if (page >= 0) slot = (long long)page * ps + pos % ps;
             else atomicOr(A.err, XB_ERR_BAD_PAGE);
