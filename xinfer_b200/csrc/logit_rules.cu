@@ -45,7 +45,6 @@ constexpr int ROWS = 48;                        // rows at a time: what they nee
 constexpr int WORDS = 32;                       // words of ancestors: trees of up to 1,024 nodes
 constexpr int NO_TREE = -32 * WORDS - 1;        // no row's tree: one that begins so far before the first row has no node, and all such are one
 constexpr int BIASES = 192;                     // biases of these rows that lie in the chunk
-constexpr int STAGES = 2;                       // rows on their way or worked on
 
 struct __align__(16) RowFacts {
     float rep, inv, freq, pres;
@@ -67,31 +66,32 @@ __device__ __forceinline__ void copy_async(void* to, const void* from) {
 
 constexpr int chunk_of(int vecs) { return 4 * THREADS * vecs; }
 constexpr int mask_room(int vecs) { return WARPS * vecs * 5; }
-constexpr int smem_of(int vecs, int words) { return 4 * (chunk_of(vecs) + STAGES * (chunk_of(vecs) + mask_room(vecs)) + words * (ROWS + 4 * WARPS + 32)); }
+constexpr int smem_of(int vecs, int words) { return 4 * (2 * chunk_of(vecs) + mask_room(vecs) + words * (ROWS + 4 * WARPS + 32)); }
 
 // The vocabulary is cut into chunks of 1,024 VECS tokens, and the (chunk, row) pairs, chunk by chunk, into equal shares for as many blocks
 // as the device holds.  The lists' tokens are counted in shared memory, once for rows that follow each other with one list (the nodes of a
 // tree); a row's own path is added before it and taken away behind it.  A warp owns 128 of every 1,024 tokens, with their counts, mask
-// words and biases, so that the warps of a block go through the rows without waiting for each other; each has its next row on its way.
-// Which 128 these are goes by where a row starts, so rows of trees that do not all start alike on 16 bytes have a barrier between them: a
-// count that one warp raises for its row may be another one's in the next (512 rows of 151,935 so: 150 us).
+// words and biases, so that the warps of a block go through the rows without waiting for each other: while one waits for its next row, others
+// work.  Which 128 these are goes by where a row starts, so rows of trees that do not all start alike on 16 bytes have a barrier between
+// them: a count that one warp raises for its row may be another one's in the next.
 // Bound by memory: a logit is read and written once.  512 rows of 151,936 with masks, biases and 8 histories of up to 4,096: 131 us, 4.75 TB/s (a
 // copy of as many bytes takes 97); the rest is the blocks' start (a history is counted by every block that meets it) and four blocks a
-// processor for want of shared memory.  With the next two rows on their way and three blocks 140 us, in chunks of 2,048 150 to 165.  A single
-// row of 151,936: 5.7 us, of which the launch and one trip for each of facts, history and logits are nearly all.
+// processor for want of registers.  Asking for a row before the one in front of it is worked on, into room of its own, takes 139 us: the
+// blocks already have 64 KB a processor on their way, and more reads between the writes slow both.  512 rows of 151,935, 143 us.  A single
+// row of 151,936: 5.6 us, of which the launch and one trip for each of facts, history and logits are nearly all.
 template <int VECS>
 __global__ void __launch_bounds__(THREADS, 4)
 logit_rules_kernel(const RuleArgs A) {
     constexpr int CHUNK = chunk_of(VECS);
-    extern __shared__ __align__(16) unsigned count[];            // [CHUNK], then the stages' logits and their mask words
+    extern __shared__ __align__(16) unsigned count[];            // [CHUNK], then a row's logits and its mask words
     float4* const logits_at = reinterpret_cast<float4*>(count + CHUNK);
-    int* const masks_at = reinterpret_cast<int*>(count + CHUNK + STAGES * CHUNK);          // [STAGES][WARPS][VECS][5]
+    int* const masks_at = reinterpret_cast<int*>(count + 2 * CHUNK);                       // [WARPS][VECS][5]
     __shared__ RowFacts facts[ROWS];
     __shared__ Bias biases[BIASES];
     __shared__ int found;
     // the rows' ancestors [ROWS][words]; the nodes whose tokens a warp owns, by `head` [WARPS][4][words]; where the tree's drafted tokens lie
     // in the chunk, or -1 [words][32]
-    unsigned* const paths = reinterpret_cast<unsigned*>(masks_at + STAGES * mask_room(VECS));
+    unsigned* const paths = reinterpret_cast<unsigned*>(masks_at + mask_room(VECS));
     unsigned* const own_nodes = paths + ROWS * A.words;
     int* const node_at = reinterpret_cast<int*>(own_nodes + WARPS * 4 * A.words);
     pdl_launch_dependents();
@@ -111,20 +111,17 @@ logit_rules_kernel(const RuleArgs A) {
     // the warp that has element u of the chunk; the first one has those beside the fours
     auto owner = [&](int u, int head, int whole) { return u < head || u >= head + 4 * whole ? 0 : (u - head) >> 7 & (WARPS - 1); };
     const int mask_word = (((lane / 5) * 4 * THREADS + warp * 128) >> 5) + lane % 5;
-    // (every row is a group of copies, those behind the last row are empty)
     auto fetch = [&](int k) {
-        if (k < rows) {
-            const float* in = A.logits + (size_t)(r0 + k) * A.in_stride + lo;
-            const int head = head_of(k), whole = (n - head) / 4, stage = k % STAGES;
-            float4* to = logits_at + stage * (CHUNK / 4) + tid;
-            const float4* from = reinterpret_cast<const float4*>(in + head) + tid;
+        const float* in = A.logits + (size_t)(r0 + k) * A.in_stride + lo;
+        const int head = head_of(k), whole = (n - head) / 4;
+        float4* to = logits_at + tid;
+        const float4* from = reinterpret_cast<const float4*>(in + head) + tid;
 #pragma unroll
-            for (int j = 0; j < VECS; ++j)
-                if (tid + j * THREADS < whole) copy_async<16>(to + j * THREADS, from + j * THREADS);
-            if (facts[k].mask >= 0 && lane < 5 * VECS) {         // the words of the warp's 128 tokens in each 1,024: four, or five off a word's start
-                const int word = (lo >> 5) + mask_word;          // (a head of up to three tokens stays in the word)
-                if (word < A.mask_words) copy_async<4>(masks_at + (stage * WARPS + warp) * VECS * 5 + lane, A.mask + (size_t)facts[k].mask * A.mask_words + word);
-            }
+        for (int j = 0; j < VECS; ++j)
+            if (tid + j * THREADS < whole) copy_async<16>(to + j * THREADS, from + j * THREADS);
+        if (facts[k].mask >= 0 && lane < 5 * VECS) {             // the words of the warp's 128 tokens in each 1,024: four, or five off a word's start
+            const int word = (lo >> 5) + mask_word;              // (a head of up to three tokens stays in the word)
+            if (word < A.mask_words) copy_async<4>(masks_at + warp * VECS * 5 + lane, A.mask + (size_t)facts[k].mask * A.mask_words + word);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -135,7 +132,7 @@ logit_rules_kernel(const RuleArgs A) {
     };
     auto work = [&](int k) {
         const RowFacts f = facts[k];
-        const int head = head_of(k), whole = (n - head) / 4, stage = k % STAGES;
+        const int head = head_of(k), whole = (n - head) / 4;
         if (f.list != counted || (A.drafted && f.first != tree)) {           // (the same for the whole block)
             __syncthreads();
             if (f.list != counted) {
@@ -188,10 +185,10 @@ logit_rules_kernel(const RuleArgs A) {
         }
         const bool said_here = nodes_here >> head & 1u, biased_here = f.biased >> warp & 1u;
         if (said_here) add_path(k, head, 1u);
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");      // this row is there
+        asm volatile("cp.async.wait_group 0;" ::: "memory");     // this row is there
         __syncwarp();
-        const float4* x = logits_at + stage * (CHUNK / 4) + tid;
-        const int* mask = f.mask >= 0 ? masks_at + (stage * WARPS + warp) * VECS * 5 : nullptr;
+        const float4* x = logits_at + tid;
+        const int* mask = f.mask >= 0 ? masks_at + warp * VECS * 5 : nullptr;
         const int* far_mask = f.mask >= 0 ? A.mask + (size_t)f.mask * A.mask_words : nullptr;
         const float* in = A.logits + (size_t)(r0 + k) * A.in_stride + lo;
         float* out = A.out + (size_t)(r0 + k) * A.out_stride + lo;
@@ -300,7 +297,7 @@ logit_rules_kernel(const RuleArgs A) {
         for (int i = tid; i < rows * A.words; i += THREADS) paths[i] = A.ancestors[(size_t)r0 * A.words + i];
         if (tid == 0) found = 0;
         __syncthreads();
-        for (int k = 0; k < STAGES - 1; ++k) fetch(k);
+        fetch(0);
         listed = 0;
         while (A.bias_start) {
             // what the rows' entries say of tokens in the chunk; of fewer rows if that is more than there is room for
@@ -375,10 +372,10 @@ logit_rules_kernel(const RuleArgs A) {
         for (int k = 0; k < rows; ++k) {
             if (owners_move && k > 0) __syncthreads();     // the row before has taken its path's counts away, whosever they are now
             work(k);
-            fetch(k + STAGES - 1);             // (into the stage of row k - 1, which this warp alone reads and has read)
+            __syncwarp();                      // (the row lies where the warp's part of this one does)
+            if (k + 1 < rows) fetch(k + 1);
         }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 template <int VECS>
