@@ -1,4 +1,6 @@
 """Generation with drafted trees: the tokens of decoding one by one, whatever is drafted."""
+import dataclasses
+
 import numpy as np
 import pytest
 import torch
@@ -187,3 +189,45 @@ def test_rows_instead_of_pages_hold_the_same_numbers():
         k.qk_norm_rope_rows(q2, kn, vn, qkv, w, w, cos, sin, pos, req, nh, nkv, d, d, False, 1e-6, err)
         at = torch.arange(9), slice(None), pos.long().cpu()
         assert torch.equal(q, q2) and torch.equal(kn.cpu(), kc.cpu()[at]) and torch.equal(vn.cpu(), vc.cpu()[at]) and int(err) == 0
+
+
+def tokens_of_steps(runner):
+    """How many tokens each of the model's steps brings, from now on."""
+    counts, forward = [], runner.model.forward
+    runner.model.forward = lambda ctx, *a: (counts.append(ctx.num_tokens), forward(ctx, *a))[1]
+    return counts
+
+
+def test_prompts_go_through_the_model_in_steps_of_bounded_size(model_folders):
+    from xinfer_b200 import SamplingParams, TreeDecoder
+    folder = model_folders("A", torch.float32)
+    prompts = prompts_for("A", [430 + i for i in range(20)])
+    runner = runner_of(folder, "f32", "A", num_blocks=20 * 32, max_num_seqs=20)
+    counts = tokens_of_steps(runner)
+    decoder = TreeDecoder(runner, max_nodes=8)
+    p = SamplingParams(max_tokens=6, ignore_eos=True, temperature=0.7)
+    outs = decoder.generate(prompts, p)
+    assert max(counts) <= 8192 and sum(n for n in counts if n > 160) == sum(len(x) for x in prompts)
+    one = dataclasses.replace(p, seed=7)
+    assert decoder.generate(prompts[7:8], one) == outs[7:8]
+
+
+@pytest.mark.parametrize("batched,chunk", [(7, 100), (64, 5), (64, 64), (1, 1), (13, 13), (90, 41)])
+def test_prompts_in_portions_of_any_size(batched, chunk, model_folders):
+    from xinfer_b200 import LogitRules, SamplingParams, TreeDecoder
+    folder = model_folders("C", torch.float32)
+    cfg, w = plain.load_folder(folder)
+    prompts = prompts_for("C", [5, 40, 17, 1])
+    want = [plain.generate(cfg, w, p, 8) for p in prompts]
+    runner = runner_of(folder, "f32", "C")
+    counts = tokens_of_steps(runner)
+    decoder = TreeDecoder(runner, max_nodes=4, max_num_batched_tokens=batched, prefill_chunk_size=chunk)
+    params = SamplingParams(temperature=0.0, max_tokens=8, ignore_eos=True)
+    assert decoder.generate(prompts, params, draft=lambda t: ([], [])) == want
+    steps = counts[:len(counts) - decoder.steps]
+    assert sum(steps) == 63 and max(steps) <= batched
+    rules = LogitRules(1.2, {3: 0.5})
+    assert decoder.generate(prompts, params, rules=rules) == TreeDecoder(runner, max_nodes=4).generate(prompts, params, rules=rules)
+    for limits in (dict(max_num_batched_tokens=0), dict(prefill_chunk_size=0)):
+        with pytest.raises(ValueError):
+            TreeDecoder(runner, **limits)

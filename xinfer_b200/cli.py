@@ -126,7 +126,8 @@ def main(argv: Optional[List[str]] = None) -> int:
         params.seed = args.seed
         if engine.generation_cfg is not None:
             params = engine.generation_cfg.fill(params)
-        decoder = TreeDecoder(engine.runner, max_nodes=args.draft_nodes, eos_token_ids=engine.eos_token_ids)
+        decoder = TreeDecoder(engine.runner, max_nodes=args.draft_nodes, eos_token_ids=engine.eos_token_ids,
+                              max_num_batched_tokens=args.max_num_batched_tokens, prefill_chunk_size=args.prefill_chunk_size)
         t0 = time.time()
         texts = decoder.generate(prompts, params, rules=LogitRules(args.repetition_penalty or 1.0))
         for i, (p, t) in enumerate(zip(prompts, texts)):

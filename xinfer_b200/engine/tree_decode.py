@@ -111,12 +111,17 @@ class _Request:
 
 class TreeDecoder:
     """Generates with drafted trees over a runner's model and page tensors.  The runner must have no open requests, and none are opened
-    while this decoder generates.  Models whose layers all are grouped-query attention (Qwen3's)."""
+    while this decoder generates.  Models whose layers all are grouped-query attention (Qwen3's).  Prompts go through the model in steps
+    of up to ``max_num_batched_tokens``, in portions of up to ``prefill_chunk_size`` (``EngineConfig``'s limits)."""
 
-    def __init__(self, runner: ModelRunner, *, max_nodes: int = 32, max_depth: int = 12, eos_token_ids=None):
+    def __init__(self, runner: ModelRunner, *, max_nodes: int = 32, max_depth: int = 12, eos_token_ids=None,
+                 max_num_batched_tokens: int = 8192, prefill_chunk_size: int = 8192):
         self.runner, self.max_nodes, self.max_depth = runner, int(max_nodes), int(max_depth)
         if not 1 <= self.max_nodes <= 1024 or not 1 <= self.max_depth:
             raise ValueError("trees of 1 to 1,024 nodes, paths of at least one")
+        self.max_batched, self.prefill_chunk = int(max_num_batched_tokens), int(prefill_chunk_size)
+        if self.max_batched < 1 or self.prefill_chunk < 1:
+            raise ValueError("steps and portions of at least one token")
         plan = runner.plan
         mixers = [runner.model.blocks[run.block].mixer for run in plan.runs]
         if any(type(m) is not Attention for m in mixers) or any(run.cache_from is not None for run in plan.runs) or runner.has_state \
@@ -171,15 +176,19 @@ class TreeDecoder:
         return out
 
     # ---- one step of the model ------------------------------------------------------------------------------------------
-    def _forward(self, token_ids, positions, request_of, start, rows, counts, context: np.ndarray, tree: Optional[TreeStep], starts=None) -> torch.Tensor:
+    def _forward(self, token_ids, positions, request_of, start, rows, counts, context: np.ndarray, tree: Optional[TreeStep], starts=None,
+                 table=None) -> torch.Tensor:
+        """``rows`` None: no logits are wanted."""
         r, B = self.runner, len(counts)
+        table = self.table[:B] if table is None else table
         q_start = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
         T = int(q_start[-1])
         ctx = StepContext(
             dtype=r.dtype, device=r.device, num_tokens=T, num_entries=B, token_ids=token_ids, positions=positions[:T], req_of_token=request_of[:T],
-            q_start=start, start_pos=starts if starts is not None else tree.context, slots=start, logit_rows=rows, num_logit_rows=rows.numel(),
-            tables=[self.table[:B].reshape(-1)], strides=[self.width], err=r.err, workspace=r.workspace, h_q_start=q_start, h_start_pos=context,
-            real_tokens=T, real_entries=B, max_context=int((context + counts).max()), tree=tree)
+            q_start=start, start_pos=starts if starts is not None else tree.context, slots=start,
+            logit_rows=start if rows is None else rows, num_logit_rows=0 if rows is None else rows.numel(), tables=[table.reshape(-1)],
+            strides=[self.width], err=r.err, workspace=r.workspace, h_q_start=q_start, h_start_pos=context, real_tokens=T,
+            real_entries=B, max_context=int((context + counts).max()), tree=tree)
         return r.model.forward(ctx, self.caches, r.layer_states)
 
     def _choose(self, logits: torch.Tensor, requests: List[_Request], counts, parents, drafted, depth, on, facts, rules: LogitRules) -> torch.Tensor:
@@ -252,7 +261,7 @@ class TreeDecoder:
             requests.append(_Request(p, len(p), sp, (b if sp.seed is None else int(sp.seed)) & 0xFFFFFFFFFFFFFFFF, sp.max_tokens or 16384))
         try:
             self._reset()
-            self._prompt_step(requests, rules)
+            self._prompt_steps(requests, rules)
             while not all(q.done for q in requests):
                 self._tree_step(requests, draft, rules)
         except BaseException:
@@ -274,19 +283,46 @@ class TreeDecoder:
             if q.done:
                 return
 
-    def _prompt_step(self, requests: List[_Request], rules: LogitRules) -> None:
-        counts = np.array([q.prompt for q in requests], np.int32)
-        total = int(counts.sum())
-        tokens, new, rows = self._send(np.concatenate([q.tokens for q in requests]), counts, np.cumsum(counts) - 1)
-        before = self.lengths[0][: len(requests)].clone()
-        _, positions, request_of, start = self._slots(new, total)
-        logits = self._forward(tokens, positions, request_of, start, rows, counts, np.zeros(len(requests), np.int32), None, before)
-        chosen = self._choose(logits, requests, np.ones(len(requests), int), None, None, np.zeros(len(requests), int), None, (None, None, None), rules)
-        got = torch.cat([chosen, self.runner.err]).cpu().numpy()
+    def _prompt_steps(self, requests: List[_Request], rules: LogitRules) -> None:
+        """Every prompt, in the requests' order, and the first token of each.  A step takes as many whole prompts as it has room for and
+        a portion of one that is longer than that."""
+        at, B = 0, len(requests)
+        while at < B:
+            counts: List[int] = []
+            room = self.max_batched
+            while room and at + len(counts) < B:
+                q = requests[at + len(counts)]
+                counts.append(min(q.prompt - q.cached, self.prefill_chunk, room))
+                room -= counts[-1]
+                if q.cached + counts[-1] < q.prompt:
+                    break
+            at += self._prompt_step(requests, at, np.array(counts, np.int32), rules)
+
+    def _prompt_step(self, requests: List[_Request], at: int, counts: np.ndarray, rules: LogitRules) -> int:
+        """The next ``counts`` tokens of the prompts from request ``at`` on; returns how many of them have come to their end."""
+        B, n = len(requests), len(counts)
+        mine = requests[at:at + n]
+        ends = [q.cached + int(c) == q.prompt for q, c in zip(mine, counts)]
+        ended = [q for q, e in zip(mine, ends) if e]               # (all of them, or all but the last)
+        all_new = np.zeros(B, np.int32)
+        all_new[at:at + n] = counts
+        context = np.array([q.cached for q in mine], np.int32)
+        tokens, new, rows = self._send(np.concatenate([q.tokens[q.cached:q.cached + int(c)] for q, c in zip(mine, counts)]), all_new,
+                                       (np.cumsum(counts) - 1)[:len(ended)])
+        before = self.lengths[0][at:at + n].clone()
+        _, positions, request_of, start = self._slots(new, int(counts.sum()))
+        logits = self._forward(tokens, positions, request_of - at, start[at:at + n + 1].clone(), rows if ended else None, counts, context, None, before,
+                               self.table[at:at + n])
+        got = [self.runner.err]
+        if ended:
+            got.insert(0, self._choose(logits, ended, np.ones(len(ended), int), None, None, np.zeros(len(ended), int), None, (None, None, None), rules))
+        got = torch.cat(got).cpu().numpy()
         self.runner.raise_on(int(got[-1]))
-        for q, t in zip(requests, got[:-1]):
-            q.cached = q.prompt
+        for q, c in zip(mine, counts):
+            q.cached += int(c)
+        for q, t in zip(ended, got[:-1]):
             self._append(q, [t])
+        return len(ended)
 
     def _tree_step(self, requests: List[_Request], draft: Draft, rules: LogitRules) -> None:
         B, limit = len(requests), self.runner.max_model_len
