@@ -231,3 +231,19 @@ def test_prompts_in_portions_of_any_size(batched, chunk, model_folders):
     for limits in (dict(max_num_batched_tokens=0), dict(prefill_chunk_size=0)):
         with pytest.raises(ValueError):
             TreeDecoder(runner, **limits)
+
+
+def test_the_command_line_draws_alike_with_and_without_drafts(model_folders, capsys):
+    """Every prompt has the seed that the engine gives it, so equal prompts draw different tokens, and drafts change none of them."""
+    from xinfer_b200 import cli
+    folder = model_folders("A", torch.float32)
+    args = ["--m", folder, "--dtype", "f32", "--prompts", "5,17,3,5", "--batch", "3", "--max-tokens", "12", "--ignore-eos", "--temperature", "0.9", "--num-blocks", "64",
+            "--max-model-len", "128"]
+
+    def texts(*more):
+        assert cli.main(args + list(more)) == 0
+        return [line.rsplit(": ", 1)[1] for line in capsys.readouterr().out.splitlines() if line.startswith("[seq ")]
+
+    for seed in ([], ["--seed", "5"]):
+        plainly = texts(*seed)
+        assert len(plainly) == len(set(plainly)) == 3 and texts("--draft-nodes", "8", *seed) == plainly

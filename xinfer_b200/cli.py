@@ -14,6 +14,7 @@ reference's two figures: prompt tokens per second and decoded tokens per second
 from __future__ import annotations
 
 import argparse
+import dataclasses
 import json
 import sys
 import time
@@ -123,13 +124,14 @@ def main(argv: Optional[List[str]] = None) -> int:
     params = SamplingParams(max_tokens=args.max_tokens, ignore_eos=args.ignore_eos)
     if args.draft_nodes:
         from . import LogitRules, TreeDecoder
-        params.seed = args.seed
         if engine.generation_cfg is not None:
             params = engine.generation_cfg.fill(params)
+        # (the seeds of the engine's first requests: what is drawn is the same with and without drafts)
+        per = [dataclasses.replace(params, seed=engine.request_seed(params, i)) for i in range(len(prompts))]
         decoder = TreeDecoder(engine.runner, max_nodes=args.draft_nodes, eos_token_ids=engine.eos_token_ids,
                               max_num_batched_tokens=args.max_num_batched_tokens, prefill_chunk_size=args.prefill_chunk_size)
         t0 = time.time()
-        texts = decoder.generate(prompts, params, rules=LogitRules(args.repetition_penalty or 1.0))
+        texts = decoder.generate(prompts, per, rules=LogitRules(args.repetition_penalty or 1.0))
         for i, (p, t) in enumerate(zip(prompts, texts)):
             print(f"[seq {i}] prompt {len(p)} tokens -> {len(t)} tokens: " + ",".join(str(x) for x in t))
         print(f"{sum(len(t) for t in texts)} tokens in {decoder.steps} steps and {time.time() - t0:.2f}s; "

@@ -179,9 +179,13 @@ class Engine:
         seq_id = self._next_id
         self._next_id += 1
         self.scheduler.add(seq_id, prompt, max_tokens, params.ignore_eos, params.stop_token_ids)
-        seed = params.seed if params.seed is not None else (self.seed * 0x9E3779B97F4A7C15 + seq_id + 1)
-        self._live[seq_id] = _Live(params, int(seed) & 0xFFFFFFFFFFFFFFFF, len(prompt), time.time())
+        self._live[seq_id] = _Live(params, self.request_seed(params, seq_id), len(prompt), time.time())
         return seq_id
+
+    def request_seed(self, params: SamplingParams, seq_id: int) -> int:
+        """What request ``seq_id`` draws with: its own seed, or one made of the engine's."""
+        seed = params.seed if params.seed is not None else (self.seed * 0x9E3779B97F4A7C15 + seq_id + 1)
+        return int(seed) & 0xFFFFFFFFFFFFFFFF
 
     # ---- one iteration --------------------------------------------------------------------------------
     def step(self) -> List[int]:
