@@ -48,3 +48,20 @@ def test_the_command_line_knows_the_options():
     from xinfer_b200.cli import build_parser
     args = build_parser().parse_args(["--m", "x", "--draft-nodes", "8", "--repetition-penalty", "1.1"])
     assert args.draft_nodes == 8 and args.repetition_penalty == 1.1
+
+
+@pytest.mark.parametrize("rules", [dict(repetition_penalty=0.0), dict(repetition_penalty=-1.5), dict(repetition_penalty=float("nan")), dict(repetition_penalty=float("inf")),
+                                   dict(repetition_penalty=1e-45), dict(bias={3: float("nan")})])
+def test_rules_that_make_no_sense_are_refused(rules):
+    from xinfer_b200.engine.tree_decode import LogitRules
+    with pytest.raises(ValueError):
+        LogitRules(**rules).validate()
+    LogitRules(0.5, {3: -float("inf"), 10 ** 6: 2.0}).validate()
+
+
+@pytest.mark.parametrize("args", [["--repetition-penalty", "1.1"], ["--repetition-penalty", "0"], ["--draft-nodes", "0"], ["--draft-nodes", "-3"], ["--draft-nodes", "2000"],
+                                  ["--draft-nodes", "8", "--repetition-penalty", "0"], ["--draft-nodes", "8", "--repetition-penalty", "-2"]])
+def test_the_command_line_refuses_options_before_it_loads_a_model(args):
+    from xinfer_b200.cli import main
+    with pytest.raises(SystemExit, match="--repetition-penalty|--draft-nodes"):
+        main(["--m", "/nowhere", "--prompts", "1,2", *args])

@@ -78,6 +78,12 @@ def main(argv: Optional[List[str]] = None) -> int:
         raise SystemExit("--m <model folder> is required")
     if args.cpu:
         raise SystemExit("--cpu: this engine runs on a B200 only; there is no CPU path")
+    if args.draft_nodes is not None and not 1 <= args.draft_nodes <= 1024:
+        raise SystemExit(f"--draft-nodes {args.draft_nodes}: trees have 1 to 1,024 tokens")
+    if args.repetition_penalty is not None and args.draft_nodes is None:
+        raise SystemExit("--repetition-penalty goes with --draft-nodes")
+    if args.repetition_penalty is not None and not args.repetition_penalty > 0.0:
+        raise SystemExit(f"--repetition-penalty {args.repetition_penalty}: a number above 0 (1: none)")
     device = "cuda:0"
     if args.device_ids:
         ids = [x for x in args.device_ids.split(",") if x != ""]
@@ -122,7 +128,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     engine = Engine(econfig, args.dtype)
     print(f"model loaded in {time.time() - t0:.1f} s; cache holds {engine.runner.kv_cache_tokens()} tokens", file=sys.stderr)
     params = SamplingParams(max_tokens=args.max_tokens, ignore_eos=args.ignore_eos)
-    if args.draft_nodes:
+    if args.draft_nodes is not None:
         from . import LogitRules, TreeDecoder
         if engine.generation_cfg is not None:
             params = engine.generation_cfg.fill(params)
@@ -131,14 +137,12 @@ def main(argv: Optional[List[str]] = None) -> int:
         decoder = TreeDecoder(engine.runner, max_nodes=args.draft_nodes, eos_token_ids=engine.eos_token_ids,
                               max_num_batched_tokens=args.max_num_batched_tokens, prefill_chunk_size=args.prefill_chunk_size)
         t0 = time.time()
-        texts = decoder.generate(prompts, per, rules=LogitRules(args.repetition_penalty or 1.0))
+        texts = decoder.generate(prompts, per, rules=LogitRules(1.0 if args.repetition_penalty is None else args.repetition_penalty))
         for i, (p, t) in enumerate(zip(prompts, texts)):
             print(f"[seq {i}] prompt {len(p)} tokens -> {len(t)} tokens: " + ",".join(str(x) for x in t))
         print(f"{sum(len(t) for t in texts)} tokens in {decoder.steps} steps and {time.time() - t0:.2f}s; "
               f"{decoder.confirmed} of {decoder.drafted} drafted tokens confirmed")
         return 0
-    if args.repetition_penalty:
-        raise SystemExit("--repetition-penalty goes with --draft-nodes")
     outs = engine.generate_sync(params, prompts)
     for o in outs:
         print(f"[seq {o.seq_id}] prompt {o.prompt_length} tokens -> {o.decoded_length} tokens ({o.finish_reason}): "

@@ -38,6 +38,13 @@ class LogitRules:
     bias: Dict[int, float] = dataclasses.field(default_factory=dict)
     allowed: Optional[Callable[[List[int]], Optional[np.ndarray]]] = None
 
+    def validate(self) -> None:
+        tiny, most = np.finfo(np.float32).tiny, np.finfo(np.float32).max      # (logits are divided by it in float32)
+        if not tiny <= self.repetition_penalty <= most:
+            raise ValueError(f"repetition_penalty must be a number above 0, got {self.repetition_penalty}")
+        if any(x != x for x in self.bias.values()):
+            raise ValueError("a bias that is no number")
+
     def active(self) -> bool:
         return self.repetition_penalty != 1.0 or bool(self.bias) or self.allowed is not None
 
@@ -243,6 +250,7 @@ class TreeDecoder:
         if self.runner.cache.live_requests():
             raise StepError("the runner has open requests: their pages are the host's")
         rules = rules or LogitRules()
+        rules.validate()
         draft = draft or lookup_draft(self.max_nodes - 1, self.max_depth - 1)
         if not prompts:
             return []
