@@ -33,18 +33,6 @@ __device__ __forceinline__ int context_of(const TreeArgs& A, int b) {
     return c < 0 ? 0 : (int)(c > most ? most : c);
 }
 
-// The request that token t belongs to: the last one that starts at or before it; -1 for a token behind them all.
-__device__ __forceinline__ int request_of(const TreeArgs& A, int t) {
-    if (t < A.token_start[0] || t >= A.token_start[A.requests]) return -1;
-    int lo = 0, hi = A.requests;             // token_start[lo] <= t < token_start[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (A.token_start[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-
 // ---- the line of all jobs' tiles -------------------------------------------------------------------------------------------
 // A job is (request, key/value head, some of the rows that a node and a query head of the group make); its tiles of KT keys are the cached
 // ones from the first that a node sees and the drafted ones.  The line holds all jobs' tiles, request by request, each as long as it
