@@ -45,7 +45,7 @@ __global__ void tree_accept_kernel(int* accepted, int* path, int* next_tokens, c
 // place ring[0] on: pages are taken at its head, in order of the requests, and given back at its end, so nothing that a block reads
 // is written by another and the same call may be made twice.  A request whose pages are not all there gets none and no slots; its
 // length stays.  Every block forms the requests' sums for itself and takes a share of the tokens: nothing waits for another block, and one
-// launch does it.  Bound by trips (lengths, then a token's page): 5.3 us for 64 requests of 6 tokens, 5.7 us for 32 of 2,048 (1.9 MB written).
+// launch does it.  Bound by trips (lengths, then a token's page): 5.0 us for 64 requests of 6 tokens, 5.5 us for 32 of 2,048 (1.9 MB written).
 constexpr int SLOT_THREADS = 256;
 constexpr int SLOT_REQUESTS = 8192;             // requests of a call: their starts lie in shared memory
 
@@ -114,17 +114,14 @@ cache_slots_kernel(const SlotArgs A) {
     pdl_wait();
     const int each = (A.requests + SLOT_THREADS - 1) / SLOT_THREADS, b0 = (int)threadIdx.x * each, b1 = min(b0 + each, A.requests);
     const int ps = A.page_size, head = (A.ring[0] % A.ring_size + A.ring_size) % A.ring_size, count = min(max(A.ring[1], 0), A.ring_size);
+    auto pages = [&](int len) { return (int)(((unsigned)len + (unsigned)(ps - 1)) / (unsigned)ps); };       // (the sum is below 2^32)
     // whether the request's pages, those it holds and those it asks for, fit its row of the table, and its length 32 bits; one whose do not
     // asks for none
-    auto fits = [&](int len, int add) {
-        const long long all = (long long)len + max(add, 0);
-        return all <= 0x7fffffffLL && (all + ps - 1) / ps <= A.table_stride;
-    };
-    auto pages = [&](int len) { return (int)(((long long)len + ps - 1) / ps); };
+    auto fits = [&](int len, int add) { return max(add, 0) <= 0x7fffffff - len && pages(len + max(add, 0)) <= A.table_stride; };
     auto sums_of = [&](int len, int add) {
         if (!fits(len, add)) return Sums{max(add, 0), 0, 0};
         if (add < 0) return Sums{0, 0, pages(len)};
-        return Sums{add, (int)(((long long)len + add + ps - 1) / ps) - pages(len), 0};
+        return Sums{add, pages(len + add) - pages(len), 0};
     };
     auto start_of = [](long long tokens) { return (int)min(tokens, 0x7fffffffLL); };
     Sums mine{0, 0, 0}, total;
@@ -179,7 +176,7 @@ cache_slots_kernel(const SlotArgs A) {
             continue;
         }
         const int b = run_of(t, A.requests, [&](int b) { return starts[b]; });
-        const int len = max(A.lengths[b], 0), pos = (int)min((long long)len + (t - starts[b]), 0x7fffffffLL), place = pos / ps, held = pages(len);
+        const int len = max(A.lengths[b], 0), pos = len + min(t - starts[b], 0x7fffffff - len), place = pos / ps, held = pages(len);
         long long slot = -1;
         if (need_before[b] >= 0) {                               // (then its positions are all below its new length)
             const int page = place < held ? A.table[(size_t)b * A.table_stride + place] : A.free_ring[ring_at(need_before[b] + place - held)];
