@@ -76,9 +76,9 @@ constexpr int smem_of(int vecs, int words) { return 4 * (2 * chunk_of(vecs) + ma
 // them: a count that one warp raises for its row may be another one's in the next.
 // Bound by memory: a logit is read and written once.  512 rows of 151,936 with masks, biases and 8 histories of up to 4,096: 131 us, 4.75 TB/s (a
 // copy of as many bytes takes 97); the rest is the blocks' start (a history is counted by every block that meets it) and four blocks a
-// processor for want of registers.  Asking for a row before the one in front of it is worked on, into room of its own, takes 139 us: the
-// blocks already have 64 KB a processor on their way, and more reads between the writes slow both.  512 rows of 151,935, 143 us.  A single
-// row of 151,936: 5.6 us, of which the launch and one trip for each of facts, history and logits are nearly all.
+// processor for want of registers.  In chunks of 2,048: 152 us.  Asking for a row before the one in front of it is worked on, into room of its
+// own: 139 us; the blocks already have 64 KB a processor on their way, and more reads between the writes slow both.  512 rows of 151,935: 143
+// us.  A single row of 151,936: 5.6 us, of which the launch and one trip for each of facts, history and logits are nearly all.
 template <int VECS>
 __global__ void __launch_bounds__(THREADS, 4)
 logit_rules_kernel(const RuleArgs A) {
@@ -402,7 +402,7 @@ static int logit_rules(float* out, const float* logits, const float* penalties, 
     const RuleArgs A{out, logits, penalties, history, history_start, prompt_len, list_of_row, drafted, ancestors, first_row, bias_start, bias_tokens,
                      bias_values, mask, mask_of_row, out_stride, in_stride, history_len, bias_len, rows, lists, vocab, words, masks, mask_words};
     // Chunks of 1,024 tokens while those of 4,096 would leave half of the processors without work.  Small and large chunks measured: one row of
-    // 151,936 5.7 and 6.15 us, of 256,000 with 20,000 said 13.9 and 16.4; three rows of 151,936 6.9 and 6.4, four 8.4 and 6.7, seven 10.8 and 7.9.
+    // 151,936 5.6 and 5.9 us, of 256,000 with 20,000 said 13.9 and 16.5; three rows of 151,936 6.8 and 6.3, four 8.2 and 6.6, seven 10.8 and 7.7.
     return (long long)rows * vocab < 148LL * 2048 ? launch<1>(A, stream) : launch<4>(A, stream);
 }
 XB_EXPORT int xb_logit_rules(const long long* words, int n) { return xb_by_words(logit_rules, words, n); }

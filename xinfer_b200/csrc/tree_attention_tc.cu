@@ -19,11 +19,11 @@
 //
 // What bounds it, and what it measured (bfloat16, 32 heads over 8 of 128 channels, pages of 16; both kernels, calls in a row):
 //   48 trees of 24 nodes, up to 32,768 keys   391 us, 5.6 TB/s: the cache's bytes (tiles of one row tile take 1,350 cycles, the memory's rate).
-//                                             Calls for seconds on end run into the power limit: 415 to 470 us
+//                                             Calls for seconds on end run into the power limit: at 1,450 MHz the cycles a tile are the bound, 466 us
 //   64 trees of 8, up to 4,096                84 us, 4.6 TB/s: the same, with a job's start every 28 tiles
 //   32 trees of 64, up to 8,192               113 us: jobs of two row tiles take about 2,000 cycles a tile of keys: exponentials (a quarter of them
 //                                             by a polynomial), maxima and conversions of 64 scores a thread, two such warps to an issue slot
-//   8 trees of 64, up to 4,096                33 us: 5 until the first scores, 14 of tiles, 2.4 to write the parts (19 MB at the L2's rate), 2.3
+//   8 trees of 64, up to 4,096                33 to 35 us: 5 until the first scores, 14 of tiles, 2.4 to write the parts (19 MB at the L2's rate), 2.3
 //                                             until the join's blocks are there, 7 of join
 //   1 tree of 16, 1,024 keys (16 heads)       13.6 us: a chain of trips to memory.  In cycles: lengths 1,300, the place in the line 1,000, the
 //                                             first segment 1,650, pages and the first tile 1,300, then four tiles, the part and the join
