@@ -1958,7 +1958,8 @@ def cache_slots(slots, positions, request_of, token_start, lengths_out, ring_out
     entries and the pages given back into ``free_ring``; ``ring_out`` and ``lengths_out`` receive the state afterwards (other memory than
     ``ring`` and ``lengths``, so that a call may be made again); per token in order ``slots`` (int64, page * page_size + place; -1: none),
     ``positions`` and ``request_of`` (-1 behind the last token), and ``token_start`` ``[B + 1]``.  Requests are served in their order; one
-    whose pages are not all there, or do not fit its row, is left as it was, its slots are -1 and the error word says so."""
+    whose pages are not all there, or do not fit its row, or whose length 32 bits do not hold, is left as it was, its slots are -1 and the
+    error word says so."""
     _check(lengths, "lengths", torch.int32, None)
     B = lengths.numel()
     if B > SLOT_REQUESTS_MAX:
