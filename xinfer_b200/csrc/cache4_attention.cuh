@@ -1,0 +1,44 @@
+// What the kernels of attention over a cache of 4-bit codes share (cache4_attention.cu says what they compute).
+#pragma once
+#include "codes4.cuh"
+
+namespace xb4 {
+
+struct AttendArgs {
+    void* out;                     // [tokens, nh, d], tokens `out_stride` elements apart; q alike
+    const void* q;
+    const uint8_t* k_cache;        // [pages, nkv, page_size * row_bytes(d)]
+    const uint8_t* v_cache;
+    const int* lengths;            // [requests]: tokens with the step's own
+    const int* token_start;        // [requests + 1]
+    const int* block_table;        // [requests, table_stride]
+    long long out_stride, q_stride;
+    int tokens, requests, table_stride, nh, nkv, d, page_size, num_pages, window;
+    float scale;
+    int* err;
+};
+
+constexpr int REQUESTS_MAX = 8192;
+constexpr long long KEYS_MOST = 0x7fff0000;      // keys that a row of the table may hold: their numbers, rounded up to tiles, are 32 bits
+
+// A request of the step.  Its token i stands at position first_pos + i and sees the keys up to there, of these the last `window`.
+struct Request {
+    int first, nodes;              // its tokens in the step
+    int first_pos;
+    int keys;                      // keys that lie in the table's row
+};
+__device__ __forceinline__ Request request_of(const AttendArgs& A, int b) {
+    Request r;
+    r.first = min(max(A.token_start[b], 0), A.tokens);               // (starts outside the tokens count as the nearest bound)
+    r.nodes = max(0, min(max(A.token_start[b + 1], 0), A.tokens) - r.first);
+    const int len = A.lengths[b];
+    const long long most = (long long)A.table_stride * A.page_size;
+    if (len > most && r.nodes > 0) atomicOr(A.err, XB_ERR_BAD_PAGE);
+    r.keys = len < 0 ? 0 : (int)(len > most ? most : len);
+    r.first_pos = max(len, 0) - r.nodes;
+    return r;
+}
+// The first key that a token at `pos` sees.
+__device__ __forceinline__ int first_seen(const AttendArgs& A, int pos) { return A.window > 0 ? max(0, pos - A.window + 1) : 0; }
+
+}  // namespace xb4

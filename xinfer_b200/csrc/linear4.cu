@@ -1,0 +1,97 @@
+// Products of a step's rows with a weight in 4 bits: y[t, n] = sum_k x[t, k] (m + s code)[n, k], groups of 32, 64 or 128 columns (codes4.cuh).
+//
+// The weight lies in tiles of 16 rows and 128 columns, a tile's bytes together: 1,024 bytes of codes, then per row the words of its groups.
+// Lane 4 g + t of a warp has rows g and g + 8 (two pieces of 16 bytes, 512 bytes apart) and in them the columns 32 j + 8 t + e of word j: as an
+// MMA's lanes take them, each word's columns in one group whatever the group's size.  Column e of a word lies in its half byte 4 (e & 1) +
+// e / 2, so that a mask takes out a pair of neighbours.  Rows and columns beyond the weight have codes and words of zeros.
+#include "codes4.cuh"
+
+namespace {
+
+using namespace xb4;
+
+struct LinearArgs {
+    void* out;                     // [tokens, rows], rows `out_stride` elements apart
+    const void* x;                 // [tokens, columns], rows `x_stride` elements apart
+    const uint8_t* weight;         // [row tiles, column tiles, tile bytes]
+    long long out_stride, x_stride;
+    int tokens, rows, columns, per_row;      // per_row: groups of a tile's row (4, 2, 1)
+};
+
+// Any type and size: a block per tile of rows and eight tokens, its warps take the column tiles in turn.  Products and sums in float32.
+constexpr int ANY_WARPS = 8, ANY_TOKENS = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(ANY_WARPS * 32)
+linear4_any_kernel(const LinearArgs A) {
+    __shared__ float part[ANY_WARPS][ANY_TOKENS][TILE_ROWS];
+    pdl_overlap_few();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int col_tiles = (A.columns + TILE_COLS - 1) / TILE_COLS, tile_bytes = TILE_CODES + TILE_ROWS * A.per_row * 4;
+    const int t0 = blockIdx.y * ANY_TOKENS, many = min(ANY_TOKENS, A.tokens - t0);
+    const uint8_t* line = A.weight + (long long)blockIdx.x * col_tiles * tile_bytes;
+    const T* x = static_cast<const T*>(A.x) + t0 * A.x_stride;
+    float acc[ANY_TOKENS][2] = {};
+    for (int ct = warp; ct < col_tiles; ct += ANY_WARPS) {
+        const uint8_t* tile = line + (long long)ct * tile_bytes;
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(tile + TILE_CODES);
+        const uint4 a = reinterpret_cast<const uint4*>(tile)[lane], b = reinterpret_cast<const uint4*>(tile)[32 + lane];
+        const uint32_t lo[4] = {a.x, a.y, a.z, a.w}, hi[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int grp = j * A.per_row / 4;
+            const uint32_t wlo = words[g * A.per_row + grp], whi = words[(g + 8) * A.per_row + grp];
+            const int c0 = ct * TILE_COLS + j * 32 + t * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (c0 + e >= A.columns) break;
+                const int shift = 4 * ((e & 1) * 4 + e / 2);
+                const float w0 = value_of((lo[j] >> shift) & 15, wlo), w1 = value_of((hi[j] >> shift) & 15, whi);
+#pragma unroll
+                for (int i = 0; i < ANY_TOKENS; ++i)
+                    if (i < many) {
+                        const float v = to_f32<T>(x[i * A.x_stride + c0 + e]);
+                        acc[i][0] = fmaf(v, w0, acc[i][0]);
+                        acc[i][1] = fmaf(v, w1, acc[i][1]);
+                    }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ANY_TOKENS; ++i)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float v = acc[i][r];
+            v += __shfl_xor_sync(0xffffffffu, v, 1);
+            v += __shfl_xor_sync(0xffffffffu, v, 2);
+            if (t == 0) part[warp][i][g + 8 * r] = v;
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < many * TILE_ROWS; i += ANY_WARPS * 32) {
+        const int tok = i / TILE_ROWS, row = i % TILE_ROWS, n = blockIdx.x * TILE_ROWS + row;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < ANY_WARPS; ++w) v += part[w][tok][row];
+        if (n < A.rows) static_cast<T*>(A.out)[(t0 + tok) * A.out_stride + n] = from_f32<T>(v);
+    }
+}
+
+template <typename T>
+int launch_any(const LinearArgs& A, cudaStream_t stream) {
+    const dim3 grid((A.rows + TILE_ROWS - 1) / TILE_ROWS, (A.tokens + ANY_TOKENS - 1) / ANY_TOKENS);
+    return xb_launch_few(linear4_any_kernel<T>, grid, dim3(ANY_WARPS * 32), 0, stream, A);
+}
+
+}  // namespace
+
+static int linear4(int dtype, void* out, const void* x, const uint8_t* weight, long long out_stride, long long x_stride, int tokens, int rows, int columns,
+                   int group, float* scratch, cudaStream_t stream) {
+    if (tokens <= 0 || rows <= 0) return 0;
+    if (columns < 1 || (group != 32 && group != 64 && group != 128) || tokens > 65535 * ANY_TOKENS) return (int)cudaErrorInvalidValue;
+    const LinearArgs A{out, x, weight, out_stride, x_stride, tokens, rows, columns, TILE_COLS / group};
+    return dtype == XB_F32 ? launch_any<float>(A, stream) : launch_any<__nv_bfloat16>(A, stream);
+}
+XB_EXPORT int xb_linear4(const long long* words, int n) { return xb_by_words(linear4, words, n); }
+
+// float32 numbers of scratch for such a product
+XB_EXPORT long long xb_linear4_scratch(int dtype, int tokens, int rows, int columns) { return 0; }

@@ -90,6 +90,25 @@ PyObject* rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// elsewhere(device, tensors or None...): the place of the first tensor that is not on the CUDA device of that number; None if there is none.
+PyObject* elsewhere(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n < 1) {
+        PyErr_SetString(PyExc_TypeError, "elsewhere(device, tensors...)");
+        return nullptr;
+    }
+    return guarded([&]() -> PyObject* {
+        const long long device = PyLong_AsLongLong(args[0]);
+        if (device == -1 && PyErr_Occurred()) return nullptr;
+        for (Py_ssize_t i = 1; i < n; ++i) {
+            if (args[i] == Py_None) continue;
+            if (!THPVariable_Check(args[i])) return PyLong_FromSsize_t(i - 1);
+            const at::Tensor& t = THPVariable_Unpack(args[i]);
+            if (!t.is_cuda() || t.get_device() != device) return PyLong_FromSsize_t(i - 1);
+        }
+        Py_RETURN_NONE;
+    });
+}
+
 // call(entry, arguments...): an entry point that takes its arguments as words of 64 bits (xb_by_words).  A tensor is its address, None is
 // the null pointer, a float the bits of a double.  Its status is the result.
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -140,6 +159,7 @@ PyCFunction method(F f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<
 
 PyMethodDef methods[] = {{"check", method(check), METH_FASTCALL, "check(tensor, name, dtype, shape)"},
                          {"rows", method(rows), METH_FASTCALL, "rows(tensor, dtype, shape)"},
+                         {"elsewhere", method(elsewhere), METH_FASTCALL, "elsewhere(device, tensors...)"},
                          {"call", method(call), METH_FASTCALL, "call(entry, arguments...)"},
                          {"on_failure", on_failure, METH_O, "on_failure(function)"},
                          {nullptr, nullptr, 0, nullptr}};

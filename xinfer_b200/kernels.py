@@ -2026,3 +2026,173 @@ def cache_commit(table: CommitTable, slots, request_of, token_start, path, err):
     _check(err, "err", torch.int32, None)
     _ok(_call(_entry("xb_cache_commit"), table.pointers, len(table.tensors), slots, request_of, token_start, path, n, B, width, table.rows, nkv,
               table.row_bytes, page_size, pages * page_size, err, _stream()), "cache_commit")
+
+
+# ---- a decoding step whose cache and weights are held in 4 bits --------------------------------------------------------------------
+# Groups of consecutive numbers with a scale s and a least value m in bfloat16, a number is m + s * code with codes 0 .. 15:
+# s = (largest - least) / 15, code = round((x - m) / s).  A group with a number that is not finite reads as NaN.
+CACHE4_GROUP = 32                  # channels of a head that share a scale; a head's last group may be shorter
+CACHE4_DIM_MAX = 256
+
+
+def _here(*tensors) -> None:
+    """The kernels run on the current device: tensors of another one are an error."""
+    device = torch.cuda.current_device() if _raw_stream is None else _device_index()
+    at = wrap_module().elsewhere(device, *tensors)
+    if at is not None:
+        raise KernelError(f"a tensor on {tensors[at].device}: the call runs on the current device, cuda:{device}")
+
+
+def cache4_page_bytes(page_size: int, d: int) -> int:
+    """Bytes that a page of ``page_size`` tokens of one key/value head of ``d`` channels takes in 4 bits: 20 for every group of 32 channels of a
+    token.  They are the codes of every group, 16 bytes for each slot (channel 2 i of the group in the low half of byte i), then for every slot the
+    (s, m) pairs of its groups."""
+    if not 1 <= d <= CACHE4_DIM_MAX or page_size < 1:
+        raise KernelError(f"pages of {page_size} tokens with heads of {d} channels: of one token at least, and 1 to {CACHE4_DIM_MAX} channels")
+    return int(page_size) * 20 * (-(-int(d) // CACHE4_GROUP))
+
+
+def _cache4(k_cache, v_cache, page_size: int, nkv, d: int) -> tuple:
+    """Checks the pages ``[pages, kv_heads, bytes]`` and gives (pages, kv_heads)."""
+    _check(k_cache, "k_cache", torch.uint8, (None, nkv, cache4_page_bytes(page_size, d)))
+    _check(v_cache, "v_cache", torch.uint8, tuple(k_cache.shape))
+    if k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+        raise KernelError("a cache starts off a 16-byte boundary")
+    return k_cache.shape[0], k_cache.shape[1]
+
+
+def cache4_write(q_out, k_cache, v_cache, qkv, positions, slots, page_size: int, err, *, q_norm=None, k_norm=None, eps: float = 1e-6, cos=None, sin=None,
+                 interleaved: bool = False, values=None):
+    """Norms and rotation of a step's queries and keys, its keys and values into 4-bit pages ``[page, kv_head, bytes]`` (``cache4_page_bytes``).
+    ``qkv`` ``[T, (heads + 2 kv_heads) * d]`` (rows may lie apart) holds a token's query heads, key heads and value heads; ``q_out`` ``[T, heads, d]``
+    receives the queries.  ``q_norm``, ``k_norm`` (float32 ``[d]``): root mean square norms per head.  ``cos``, ``sin`` (float32
+    ``[positions, rot / 2]``): the first rot channels of queries and keys turn by the angles of the token's ``positions`` (int32), in
+    pairs of halves or (``interleaved``) of neighbours.  ``slots`` (int64, as ``cache_slots`` writes them): page * page_size + place; a token
+    with -1 is not cached.  Tokens of one call have slots of their own.  ``values`` = (k, v), bfloat16 ``[T, kv_heads, d]``: the rows as the cache
+    gives them back, of every token, for kernels that read keys and values from rows.  Slots outside the cache, and positions outside the table of
+    a token that is cached, are reported in ``err``."""
+    T, nh, d = q_out.shape
+    dtype = qkv.dtype
+    code = dtype_code(dtype)
+    pages, nkv = _cache4(k_cache, v_cache, page_size, None, d)
+    if nkv < 1:
+        raise KernelError("a cache without heads")
+    _check(q_out, "q_out", dtype, (T, nh, d))
+    row = _rows(qkv, dtype, (T, (nh + 2 * nkv) * d))
+    if row is None:
+        raise KernelError(f"qkv: expected {dtype} CUDA rows {(T, (nh + 2 * nkv) * d)} with dense numbers, got {qkv.dtype} {tuple(qkv.shape)} with strides {qkv.stride()}")
+    _check(positions, "positions", torch.int32, (T,))
+    _check(slots, "slots", torch.int64, (T,))
+    _check(err, "err", torch.int32, None)
+    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if t is not None:
+            _check(t, name, torch.float32, (d,))
+    rot = most = 0
+    if (cos is None) != (sin is None):
+        raise KernelError("a rotation takes cosines and sines")
+    if cos is not None:
+        _check(cos, "cos", torch.float32, (None, None))
+        _check(sin, "sin", torch.float32, tuple(cos.shape))
+        most, rot = cos.shape[0], 2 * cos.shape[1]
+        if most < 1 or rot < 2 or rot > d:
+            raise KernelError(f"a table of {most} positions and {rot} channels for heads of {d}")
+    k_values = v_values = None
+    if values is not None:
+        k_values, v_values = values
+        _check(k_values, "values", torch.bfloat16, (T, nkv, d))
+        _check(v_values, "values", torch.bfloat16, (T, nkv, d))
+    _here(q_out, k_cache, v_cache, qkv, positions, slots, err, q_norm, k_norm, cos, sin, k_values, v_values)
+    _ok(_call(_entry("xb_cache4_write"), code, q_out, k_cache, v_cache, qkv, q_norm, k_norm, cos, sin, positions, slots, k_values, v_values, row,
+              pages * int(page_size), T, nh, nkv, d, rot, int(bool(interleaved)), int(page_size), most, float(eps), err, _stream()), "cache4_write")
+
+
+@functools.lru_cache(maxsize=4096)
+def cache4_attention_scratch(tokens: int, requests: int, nh: int, nkv: int, d: int, dtype, longest: Optional[int] = None) -> int:
+    """float32 numbers of scratch that ``cache4_attention`` takes for such a step; 0: none."""
+    longest = _longest(longest, tokens, 1)
+    return int(kernels_lib().xb_cache4_attention_scratch(dtype_code(dtype), int(tokens), int(requests), int(nh), int(nkv), int(d), longest))
+
+
+def cache4_attention(out, q, k_cache, v_cache, lengths, token_start, block_table, page_size: int, scale, err, *, scratch=None, window: Optional[int] = None,
+                     longest: Optional[int] = None):
+    """Attention of a step's tokens over 4-bit pages ``[page, kv_head, bytes]`` that hold their own keys and values already (``cache4_write``).
+    Request b has the tokens ``token_start[b] .. token_start[b + 1]`` of ``q`` ``[T, heads, d]``, the last ones of its ``lengths[b]`` (int32): a token
+    sees the keys up to its own position, of these the last ``window``, by its request's row of ``block_table``.  One that sees nothing
+    gets zeros; rows behind the last request's stay as they are.  ``out`` and ``q`` have dense heads, their tokens may lie apart.  ``scratch``: float32,
+    ``cache4_attention_scratch`` numbers, contents undefined, not shared by calls that may overlap.  ``longest``: tokens of the request that
+    brings most, as far as the host knows it (1 for a decoding step); the form of the kernels goes by it, never what they compute."""
+    T, nh, d = q.shape
+    dtype = q.dtype
+    code = dtype_code(dtype)
+    pages, nkv = _cache4(k_cache, v_cache, page_size, None, d)
+    if nkv < 1 or nh < 1 or nh % nkv:
+        raise KernelError(f"{nh} query heads do not divide into {nkv} key/value heads")
+    shape = (T, nh, d)
+    so, sq = _token_rows(out, "out", dtype, shape), _token_rows(q, "q", dtype, shape)
+    _check(lengths, "lengths", torch.int32, None)
+    requests = lengths.numel()
+    if requests > TREE_REQUESTS_MAX:
+        raise KernelError(f"{requests} requests; a call takes {TREE_REQUESTS_MAX}")
+    _check(token_start, "token_start", torch.int32, (requests + 1,))
+    _check(block_table, "block_table", torch.int32, (requests, None))
+    _check(err, "err", torch.int32, None)
+    if block_table.shape[1] * page_size > 0x7fff0000:
+        raise KernelError(f"a table of {block_table.shape[1]} pages of {page_size} tokens: keys are counted in 32 bits")
+    if window is not None and window < 1:
+        raise KernelError(f"a window of {window} keys")
+    if longest is not None and longest < 1:
+        raise KernelError(f"a longest request of {longest} tokens")
+    longest = _longest(longest, T, 1)
+    need = cache4_attention_scratch(T, requests, nh, nkv, d, dtype, longest)
+    if need:
+        _check(scratch, "scratch", torch.float32, None)
+        if scratch.numel() < need:
+            raise KernelError(f"scratch holds {scratch.numel()} numbers, {need} are needed")
+        if scratch.data_ptr() % 16:
+            raise KernelError("scratch starts off a 16-byte boundary")
+    _here(out, q, k_cache, v_cache, lengths, token_start, block_table, err, scratch)
+    _ok(_call(_entry("xb_cache4_attention"), code, out, q, k_cache, v_cache, lengths, token_start, block_table, so, sq, T, requests, block_table.shape[1], nh, nkv,
+              d, int(page_size), pages, int(window or 0), longest, float(scale), scratch if need else None, err, _stream()), "cache4_attention")
+
+
+def linear4_shape(rows: int, columns: int, group: int) -> tuple:
+    """The shape of a weight ``[rows, columns]`` in 4 bits (``weights.pack4``): uint8 ``[row tiles, column tiles, bytes]``, tiles of 16 rows and 128
+    columns, 1,024 bytes of codes and a (s, m) pair for every ``group`` (32, 64 or 128) columns of a row."""
+    if group not in (32, 64, 128) or rows < 1 or columns < 1:
+        raise KernelError(f"a weight of {rows} rows and {columns} columns in groups of {group}: groups have 32, 64 or 128 columns")
+    return -(-int(rows) // 16), -(-int(columns) // 128), 1024 + 16 * (128 // group) * 4
+
+
+@functools.lru_cache(maxsize=4096)
+def linear4_scratch(tokens: int, rows: int, columns: int, dtype) -> int:
+    """float32 numbers of scratch that ``linear4`` takes for such a product; 0: none."""
+    return int(kernels_lib().xb_linear4_scratch(dtype_code(dtype), int(tokens), int(rows), int(columns)))
+
+
+def linear4(out, x, weight, *, scratch=None):
+    """``out[t, n] = sum_k x[t, k] * W[n, k]`` for rows ``x`` ``[T, columns]`` and a weight in 4 bits (``weights.pack4``); sums in float32, rounded once.
+    ``out`` is ``[T, rows]`` of x's type; rows of both may lie apart.  ``scratch``: float32, ``linear4_scratch`` numbers, contents undefined, not shared by calls that
+    may overlap."""
+    T, columns = x.shape
+    rows = out.shape[1] if out.dim() == 2 else 0
+    dtype = x.dtype
+    code = dtype_code(dtype)
+    at = _rows(x, dtype, (T, columns)), _rows(out, dtype, (T, rows))
+    if None in at or rows < 1 or columns < 1:
+        raise KernelError(f"out and x: expected CUDA rows of one type with dense numbers, got {out.dtype} {tuple(out.shape)} with strides {out.stride()} and "
+                          f"{x.dtype} {tuple(x.shape)} with strides {x.stride()}")
+    _check(weight, "weight", torch.uint8, (-(-rows // 16), -(-columns // 128), None))
+    group = {1024 + 16 * (128 // g) * 4: g for g in (32, 64, 128)}.get(weight.shape[2])
+    if group is None:
+        raise KernelError(f"weight: tiles of {weight.shape[2]} bytes belong to no group of 32, 64 or 128 columns")
+    if weight.data_ptr() % 16:
+        raise KernelError("weight: starts off a 16-byte boundary")
+    need = linear4_scratch(T, rows, columns, dtype)
+    if need:
+        _check(scratch, "scratch", torch.float32, None)
+        if scratch.numel() < need:
+            raise KernelError(f"scratch holds {scratch.numel()} numbers, {need} are needed")
+        if scratch.data_ptr() % 16:
+            raise KernelError("scratch starts off a 16-byte boundary")
+    _here(out, x, weight, scratch)
+    _ok(_call(_entry("xb_linear4"), code, out, x, weight, at[1], at[0], T, rows, columns, group, scratch if need else None, _stream()), "linear4")
