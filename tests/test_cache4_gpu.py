@@ -432,8 +432,9 @@ def test_refusals():
     from xinfer_b200 import kernels as k
     a = Attend([1, 2], [30, 40], 4, 2, 64, BF)
     caches, lengths, start, table = a.tensors()
+    room = k.cache4_attention_scratch(a.q.shape[0], 2, 4, 2, 64, BF) + 4
     good = dict(out=a.out, q=a.q, k_cache=caches[0], v_cache=caches[1], lengths=lengths, token_start=start, block_table=table, page_size=16, scale=0.1, err=a.err,
-                scratch=torch.zeros(1 << 16, device=DEV))
+                scratch=torch.zeros(room, device=DEV))
 
     def refused(**change):
         with pytest.raises(k.KernelError):
@@ -442,7 +443,7 @@ def test_refusals():
     k.cache4_attention(**good)
     refused(out=a.out.float()), refused(q=a.q.half()), refused(k_cache=caches[0].int()), refused(v_cache=caches[1][:-1]), refused(lengths=lengths.long())
     refused(token_start=start[:-1]), refused(block_table=table[:1]), refused(page_size=8), refused(page_size=0), refused(window=0), refused(longest=0)
-    refused(q=a.q[:, :3], out=a.out[:, :3]), refused(scratch=torch.zeros(4, device=DEV)), refused(scratch=torch.zeros(1 << 16, device=DEV)[1:]), refused(err=a.err.long())
+    refused(q=a.q[:, :3], out=a.out[:, :3]), refused(scratch=torch.zeros(4, device=DEV)), refused(scratch=torch.zeros(room, device=DEV)[1:]), refused(err=a.err.long())
     refused(lengths=lengths.cpu()), refused(q=a.q.cpu()), refused(block_table=table.expand(2, table.shape[1])[:, ::2])
     w = Write(3, 4, 2, 64, BF, 16)
     base = dict(q_out=w.q_out, k_cache=w.caches[0], v_cache=w.caches[1], qkv=w.qkv, positions=w.positions, slots=w.slots, page_size=16, err=w.err, cos=w.cos, sin=w.sin)

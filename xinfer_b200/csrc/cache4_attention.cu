@@ -1,7 +1,7 @@
 // Attention of a step's tokens over a paged cache of 4-bit codes (codes4.cuh): token i of request b, at position lengths[b] - nodes + i, gets
 //   sum_j softmax_j(scale q . k_j) v_j   over the keys j up to its position, of these the last `window`; zeros if it sees none.
 // The step's own keys are in the cache already.  A page outside the pool is reported and its keys are not seen.
-#include "cache4_attention.cuh"
+#include "cache4_attention_mma.h"
 
 namespace {
 
@@ -236,6 +236,7 @@ static int cache4_attention(int dtype, void* out, const void* q, const uint8_t* 
     if ((long long)table_stride * page_size > KEYS_MOST || (long long)tokens * nh > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     const AttendArgs A{out, q, k_cache, v_cache, lengths, token_start, block_table, out_stride, q_stride, tokens, requests, table_stride, nh, nkv, d, page_size,
                        num_pages, window, scale, err};
+    if (dtype == XB_BF16 && mma_takes(A)) return mma_launch(A, longest, scratch, stream);
     return dtype == XB_F32 ? launch_any<float>(A, longest, scratch, stream) : launch_any<__nv_bfloat16>(A, longest, scratch, stream);
 }
 XB_EXPORT int xb_cache4_attention(const long long* words, int n) { return xb_by_words(cache4_attention, words, n); }
@@ -244,5 +245,6 @@ XB_EXPORT int xb_cache4_attention(const long long* words, int n) { return xb_by_
 XB_EXPORT long long xb_cache4_attention_scratch(int dtype, int tokens, int requests, int nh, int nkv, int d, int longest) {
     if (tokens <= 0 || requests <= 0 || nkv <= 0 || nh < nkv || d < 1) return 0;
     const AnyGrid g = any_grid(requests, nh, nkv, longest);
-    return g.splits == 1 ? 0 : (long long)g.splits * tokens * nh * (d + 2);
+    const long long any = g.splits == 1 ? 0 : (long long)g.splits * tokens * nh * (d + 2), mma = dtype == XB_BF16 && mma_takes(d) ? mma_scratch(nh, nkv, d, longest) : 0;
+    return any > mma ? any : mma;                      // (the pages are not known here: enough for either kernel)
 }

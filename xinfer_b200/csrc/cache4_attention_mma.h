@@ -1,0 +1,12 @@
+// Few rows of a key/value head over 4-bit pages, in bfloat16 (cache4_attention_mma.cu).
+#pragma once
+#include "cache4_attention.cuh"
+
+namespace xb4 {
+
+bool mma_takes(int d);                        // whether it has a form for such heads
+bool mma_takes(const AttendArgs& A);
+long long mma_scratch(int nh, int nkv, int d, int longest);        // float32 numbers, on a 16-byte boundary
+int mma_launch(const AttendArgs& A, int longest, float* scratch, cudaStream_t stream);
+
+}  // namespace xb4
