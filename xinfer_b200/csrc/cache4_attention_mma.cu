@@ -12,9 +12,9 @@
 //           larger than that of a probability times a value; the second sum is float32.  8 sum(p s) is a product with a constant operand.
 // The softmax's reference is a number per column that moves only when a score is more than 2^8 above it.
 //
-// The tiles (64 keys) of all jobs are one line cut into equal shares, one a block, whatever the lengths are; a block's four warps take a quarter of
-// its tiles of a job each, fetch them into rings of their own with bulk copies, and join in shared memory.  Parts of a job that several
-// blocks share are joined by a second kernel in their order.
+// The tiles (32 keys) of all jobs are one line cut into equal shares, one a warp, whatever the lengths are: warps of a block have nothing to do with each
+// other.  A warp fetches its keys and values into a ring of its own with bulk copies.  Parts of a job that several warps share are joined by a
+// second kernel in their order.
 #include "cache4_attention_mma.h"
 #include "tc_common.cuh"
 
@@ -23,38 +23,33 @@ namespace {
 using namespace xb4;
 using xbtc::smem_u32;
 
-constexpr int KT = 64;                     // keys of a tile of the line
-constexpr int STEP = 16;                   // keys of a warp's step
+constexpr int STEP = 16;                   // keys of a step
+constexpr int STAGE_STEPS = 2;             // steps that are fetched together
+constexpr int KT = STEP * STAGE_STEPS;     // keys of a tile of the line
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int COST_TILE = 2, COST_JOB = 2; // a job's start and end take about as long as a tile
+constexpr int COST_JOB = 3;                // a job's start and end take about as long as three tiles
 constexpr float RESCALE_STEP = 8.f;
 constexpr int JOB_WORDS = 8;
 
-__host__ __device__ constexpr int per_sm(int nt, int ng) { return nt == 1 && ng <= 4 ? 4 : (nt == 1 || ng <= 4 ? 2 : 1); }
+__host__ __device__ constexpr int per_sm(int nt, int ng) { return nt == 1 && ng <= 4 ? 4 : 2; }
 __host__ __device__ constexpr int blocks_of(int nt, int ng) { return 148 * per_sm(nt, ng); }
-__host__ __device__ constexpr int stages(int ng) { return ng <= 2 ? 8 : (ng <= 4 ? 5 : 4); }
-__host__ __device__ constexpr int stage_bytes(int ng) { return 2 * STEP * 20 * ng; }
-// a warp's result in shared memory: [rows][channels + 4], then the rows' maxima and sums
-__host__ __device__ constexpr int result_floats(int nt, int ng) { return 8 * nt * (32 * ng + 4) + 16 * nt; }
-__host__ __device__ constexpr int smem_bytes(int nt, int ng) {
-    const int ring = WARPS * stages(ng) * stage_bytes(ng), joined = WARPS * result_floats(nt, ng) * 4;
-    return (ring > joined ? ring : joined) + WARPS * stages(ng) * 8;
-}
+__host__ __device__ constexpr int stages(int ng) { return ng <= 2 ? 4 : 2; }
+__host__ __device__ constexpr int stage_bytes(int ng) { return STAGE_STEPS * 2 * STEP * 20 * ng; }
+__host__ __device__ constexpr int smem_bytes(int ng) { return WARPS * stages(ng) * (stage_bytes(ng) + 8); }
 
 struct Line {
-    float* part_o;                 // [blocks][2][rows][d]: a block's first segment, if its job began before it, and its last, if its job goes on
-    float* part_ml;                // [blocks][2][rows][2]: maximum and sum
-    int* jobs;                     // [blocks][2][8]: parts (0: there is no such part), block of the first, first row, rows, key/value head, request
-    int min_share;
+    float* part_o;                 // [warps][2][rows][d]: a warp's first segment, if its job began before it, and its last, if its job goes on
+    float* part_ml;                // [warps][2][rows][2]: maximum and sum
+    int* jobs;                     // [warps][2][8]: parts (0: there is no such part), warp of the first, first row, rows, key/value head, request
 };
 
 struct Walk {
     Request r;
     int b, g, piece;               // the job: request, key/value head, which of their pieces of rows
     int tile0, tiles, pieces;      // of the request
-    int job, from, end, share;     // where the job begins in the line, the block's range, a block's share
-    int i0, i1;                    // the block's tiles of the job's
-    __device__ __forceinline__ int job_units() const { return tiles * COST_TILE + COST_JOB; }
+    int job, from, end, share;     // where the job begins in the line, the warp's range, a warp's share
+    int i0, i1;                    // the warp's tiles of the job's
+    __device__ __forceinline__ int job_units() const { return tiles + COST_JOB; }
 };
 
 template <int ROWS>
@@ -67,9 +62,9 @@ __device__ __forceinline__ void set_request(const AttendArgs& A, Walk& w, int b)
     w.tiles = max(1, (w.r.keys + KT - 1) / KT - w.tile0);
 }
 
-// The block's place in the line before its first job; every warp of the block finds it for itself.
+// The warp's place in the line before its first job.
 template <int ROWS>
-__device__ __forceinline__ bool place_in_line(const AttendArgs& A, const Line& line, Walk& w) {
+__device__ __forceinline__ bool place_in_line(const AttendArgs& A, const Line& line, int me, int warps, Walk& w) {
     const int lane = threadIdx.x & 31, each = (A.requests + 31) / 32, b0 = lane * each, b1 = min(b0 + each, A.requests);
     int mine = 0;
 #pragma unroll 1
@@ -84,8 +79,8 @@ __device__ __forceinline__ bool place_in_line(const AttendArgs& A, const Line& l
         if (lane >= o) incl += v;
     }
     const int total = __shfl_sync(0xffffffffu, incl, 31);
-    w.share = max(line.min_share, (total + (int)gridDim.x - 1) / (int)gridDim.x);
-    w.from = (int)min((long long)blockIdx.x * w.share, (long long)total);
+    w.share = (total + warps - 1) / warps;
+    w.from = (int)min((long long)me * w.share, (long long)total);
     w.end = min(total, w.from + w.share);
     if (w.from >= w.end) return false;
     int before = incl - mine, b = b0;
@@ -108,7 +103,7 @@ __device__ __forceinline__ bool place_in_line(const AttendArgs& A, const Line& l
     return true;
 }
 
-// The next job of which the block has tiles: those that begin in its share.
+// The next job of which the warp has tiles: those that begin in its share.
 template <int ROWS>
 __device__ __forceinline__ bool next_segment(const AttendArgs& A, Walk& w, bool first) {
     for (;; first = false) {
@@ -126,8 +121,8 @@ __device__ __forceinline__ bool next_segment(const AttendArgs& A, Walk& w, bool 
                 }
             }
         }
-        w.i0 = w.from > w.job ? (w.from - w.job + COST_TILE - 1) / COST_TILE : 0;
-        w.i1 = min(w.tiles, (w.end - w.job + COST_TILE - 1) / COST_TILE);
+        w.i0 = max(0, w.from - w.job);
+        w.i1 = min(w.tiles, w.end - w.job);
         if (w.i0 < w.i1) return true;
     }
 }
@@ -150,20 +145,73 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the same without a sum before it
+__device__ __forceinline__ void mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void ldmatrix_x2(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x2_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+}
+// The halves of a word that are infinities or no numbers become zero.
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
+    return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t packed) {        // what bfloat16 rounding left of a and b
+    return xbtc::pack_bf16(a - scale_of(packed), b - least_of(packed));
+}
 
 constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
 constexpr float BACK = 6.18970019642690137449e26f;       // 2^89: 2^133 of the codes over 2^44 of the probabilities
-constexpr float UP = 17592186044416.f;                   // 2^44
+constexpr float UP = 44.f, DOWN = 0x1p-44f;
+constexpr float TOP = UP + RESCALE_STEP;
+
+// The words of the groups of two keys, eight apart.
+template <int NG>
+__device__ __forceinline__ void load_words(uint32_t at, uint32_t (&w)[2][NG]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t key = at + 8 * h * NG * 4;
+        if constexpr (NG % 4 == 0) {
+#pragma unroll
+            for (int n = 0; n < NG; n += 4)
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[h][n]), "=r"(w[h][n + 1]), "=r"(w[h][n + 2]), "=r"(w[h][n + 3]) : "r"(key + n * 4) : "memory");
+        } else {
+#pragma unroll
+            for (int n = 0; n < NG; ++n) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[h][n]) : "r"(key + n * 4) : "memory");
+        }
+    }
+}
+
+// Eight channels of a query (zeros behind the head).
+__device__ __forceinline__ void load_query(const __nv_bfloat16* q, int c, int d, bool on16, float (&x)[8]) {
+    if (on16 && c + 8 <= d) {
+        const uint4 v = *reinterpret_cast<const uint4*>(q + c);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = c + e < d ? __bfloat162float(q[c + e]) : 0.f;
+    }
+}
 
 template <int NT, int NG>
 __global__ void __launch_bounds__(THREADS, per_sm(NT, NG))
 cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
     extern __shared__ __align__(128) char mem[];
-    constexpr int ROWS = 8 * NT, STAGES = stages(NG), STAGE = stage_bytes(NG), HALF = STAGE / 2, CODES = NG * STEP * 16, DP = 32 * NG;
+    constexpr int ROWS = 8 * NT, STAGES = stages(NG), STAGE = stage_bytes(NG), HALF = 20 * NG * STEP, CODES = NG * STEP * 16, DP = 32 * NG;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gi = lane >> 2, ti = lane & 3;
-    const int group = A.nh / A.nkv, ps = A.page_size, piece_keys = ps % STEP == 0 ? STEP : STEP / 2;
+    const int group = A.nh / A.nkv, ps = A.page_size;
+    const bool by16 = ps % STEP == 0;                      // a step's keys lie in one page; else in two
     const uint32_t ring = smem_u32(mem) + warp * STAGES * STAGE;
-    const uint32_t bars = smem_u32(mem) + smem_bytes(NT, NG) - WARPS * STAGES * 8 + warp * STAGES * 8;
+    const uint32_t bars = smem_u32(mem) + WARPS * STAGES * STAGE + warp * STAGES * 8;
+    // (shares one behind another lie in different blocks, so that few of them are spread over the processors)
+    const int warps = (int)gridDim.x * WARPS, me = warp * (int)gridDim.x + (int)blockIdx.x;
+    constexpr bool BY_WORDS = NG % 4 == 0;                 // a key's words are rows that ldmatrix takes
     if (lane == 0) {
         for (int i = 0; i < STAGES; ++i) xbtc::mbar_init(bars + 8 * i, 1);
         xbtc::mbar_init_fence();
@@ -171,46 +219,96 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
     __syncwarp();
     pdl_launch_dependents();
     pdl_wait();
-    if (threadIdx.x < 2) line.jobs[((size_t)blockIdx.x * 2 + threadIdx.x) * JOB_WORDS] = 0;
+    if (lane < 2) line.jobs[((size_t)me * 2 + lane) * JOB_WORDS] = 0;
+    __syncwarp();
     Walk w;
-    if (!place_in_line<ROWS>(A, line, w)) return;
+    if (!place_in_line<ROWS>(A, line, me, warps, w)) return;
     const long long page_bytes = (long long)ps * 20 * NG;
-    uint32_t issued = 0, taken = 0;            // steps of this warp's ring, over all segments
-    bool failed = false;                       // a copy never came: nothing is waited for any more
+    const bool q16 = ((uintptr_t)A.q & 15) == 0 && A.q_stride % 8 == 0 && A.d % 8 == 0;
+    const bool out8 = ((uintptr_t)A.out & 7) == 0 && A.out_stride % 4 == 0 && A.d % 4 == 0;
+    uint32_t put_slot = 0, take_slot = 0, take_parity = 0; // of this warp's ring, over all segments
+    bool failed = false;                                   // a copy never came: nothing is fetched any more
     for (bool first = true; next_segment<ROWS>(A, w, first); first = false) {
         const int row0 = w.piece * ROWS, rows = min(ROWS, w.r.nodes * group - row0);
         const int pos0 = w.r.first_pos + row0 / group, pos1 = w.r.first_pos + (row0 + rows - 1) / group;
-        const int low1 = first_seen(A, pos1);
-        // this warp's steps of the segment, and of these the ones with keys that some row sees
-        const int steps = (w.i1 - w.i0) * (KT / STEP), s0 = (w.tile0 + w.i0) * (KT / STEP);
+        // keys from `all0` on and below `all1` are seen by all rows
+        const int all0 = first_seen(A, pos1), all1 = min(pos0 + 1, w.r.keys);
+        // the segment's steps, of these the ones with keys that some row sees
         const int seen0 = first_seen(A, pos0) / STEP, seen1 = (min(pos1 + 1, w.r.keys) + STEP - 1) / STEP;
-        const int from = max(s0 + steps * warp / WARPS, seen0), to = failed ? from : min(s0 + steps * (warp + 1) / WARPS, seen1);
+        const int from = max((w.tile0 + w.i0) * STAGE_STEPS, seen0), to = failed ? from : min((w.tile0 + w.i1) * STAGE_STEPS, seen1);
         const int* table = A.block_table + (long long)w.b * A.table_stride;
         const uint8_t* k_pages = A.k_cache + w.g * page_bytes;
         const uint8_t* v_pages = A.v_cache + w.g * page_bytes;
+
+        // ---- fetching: a stage holds two steps, each its keys' codes as [group][key][16 bytes] and words as [key][group], then its values'
+        int ids = -1, ids_from = -1, put = from;           // a lane holds the page of one of 32 pieces (keys that lie in one page),
+        unsigned have = 0;                                 // and this which of them there are
+        unsigned none_of = 0;                              // eight bits a stage, the last one lowest: pieces without a page
+        auto issue = [&]() {
+            const int shift = by16 ? 0 : 1, at = (put - from) << shift, in_use = min(STAGE_STEPS, to - put) << shift;
+            if ((at & ~31) != ids_from) {
+                ids_from = at & ~31;
+                const int key = (from << 4) + ((ids_from + lane) << (4 - shift));
+                ids = -1;
+                if (key < to * STEP && key < w.r.keys) {
+                    ids = table[key / ps];
+                    if (ids < 0 || ids >= A.num_pages) {
+                        atomicOr(A.err, XB_ERR_BAD_PAGE);
+                        ids = -1;
+                    }
+                }
+                have = __ballot_sync(0xffffffffu, ids >= 0);
+            }
+            const uint32_t bar = bars + 8 * put_slot, dst = ring + put_slot * STAGE;
+            // piece i of the stage is lane (at & 31) + i of ids
+            const unsigned there = have >> (at & 31) & ((1u << in_use) - 1);
+            none_of = none_of << 8 | (~there & 0xffu);
+            if (lane == 0) xbtc::mbar_expect_tx(bar, __popc(there) * (by16 ? 2 * HALF : HALF));
+            __syncwarp();
+            if (ps == STEP) {                              // whole pages
+                const int id = __shfl_sync(0xffffffffu, ids, (at & 31) + (lane >> 1 & 1));
+                if (lane < 4 && (there >> (lane >> 1) & 1))
+                    bulk_copy(dst + lane * HALF, (lane & 1 ? v_pages : k_pages) + (long long)id * A.nkv * page_bytes, HALF, bar);
+            } else {
+                const int each = 2 * (NG + 1), keys = by16 ? STEP : STEP / 2;      // copies of a piece
+#pragma unroll 1
+                for (int i = lane; i < ((in_use * each + 31) & ~31); i += 32) {
+                    const int piece = min(i / each, 3), n = i % each % (NG + 1), v = i % each / (NG + 1), id = __shfl_sync(0xffffffffu, ids, (at & 31) + piece);
+                    if (i >= in_use * each || !(there >> piece & 1)) continue;
+                    const int key = put * STEP + piece * keys, slot = key % ps, half = by16 ? 0 : piece & 1;
+                    const uint8_t* src = (v ? v_pages : k_pages) + (long long)id * A.nkv * page_bytes;
+                    src += n < NG ? ((long long)n * ps + slot) * 16 : (long long)ps * 16 * NG + slot * NG * 4;
+                    const uint32_t to_smem = dst + (2 * (piece >> shift) + v) * HALF + (n < NG ? n * STEP * 16 + half * 128 : CODES + half * 8 * NG * 4);
+                    bulk_copy(to_smem, src, n < NG ? keys * 16 : keys * NG * 4, bar);
+                }
+            }
+            put_slot = put_slot + 1 == STAGES ? 0 : put_slot + 1;
+            put += STAGE_STEPS;
+        };
+        for (int i = 0; i < STAGES && put < to; ++i) issue();
+
         // ---- queries: columns of S^T; column gi of column tile j is row 8 j + gi
         uint32_t qf[NT][NG][4];
-        float qsum[NT][NG][2], c1[NT][2];
+        float qsum[NT][NG][2], c1[NT][2];                  // the columns' sums per group: as numbers, or in two parts as an operand beside the words
+        uint32_t qw[NT][4];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int row = j * 8 + gi;
-            const bool live = row < rows;
-            const long long t = w.r.first + (row0 + (live ? row : 0)) / group;
-            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(A.q) + t * A.q_stride + (long long)(w.g * group + (row0 + (live ? row : 0)) % group) * A.d;
+            const int row = min(j * 8 + gi, rows - 1);     // (columns without a row repeat the last one's)
+            const long long t = w.r.first + (row0 + row) / group;
+            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(A.q) + t * A.q_stride + (long long)(w.g * group + (row0 + row) % group) * A.d;
             float x[NG][8], top = 0.f;
 #pragma unroll
-            for (int n = 0; n < NG; ++n)
+            for (int n = 0; n < NG; ++n) {
+                load_query(q, 32 * n + 8 * ti, A.d, q16, x[n]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int c = 32 * n + 8 * ti + e;
-                    x[n][e] = live && c < A.d ? __bfloat162float(q[c]) : 0.f;
-                    top = max_nan(top, fabsf(x[n][e]));
-                }
+                for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(x[n][e]));
+            }
             top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // the power of two that brings the row's largest number to 2^119 .. 2^120 (any for rows of zeros and of numbers that are not finite)
-            const int e2 = top > 0.f && top < INFINITY ? 120 - (ilogbf(top) + 1) : 120;
-            const float f1 = ldexpf(1.f, e2 / 2), f2 = ldexpf(1.f, e2 - e2 / 2);
+            // the power of two that brings the row's largest number to 2^119 .. 2^120 (any for rows of zeros and of numbers that are not finite;
+            // exponents of numbers below 2^-126 count as 2^-127's, which is no less exact)
+            const int expo = (int)(__float_as_uint(top) >> 23), e2 = expo < 255 && top > 0.f ? 246 - max(expo, 1) : 120;
+            const float f1 = __uint_as_float((uint32_t)(127 + e2 / 2) << 23), f2 = __uint_as_float((uint32_t)(127 + e2 - e2 / 2) << 23);
             float sums[NG];
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
@@ -228,327 +326,324 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                 sums[n] = sum * 0x1p-33f;
             }
+            if constexpr (BY_WORDS) {                      // in front of s: zero; in front of m: 16 bits of the sum in two parts
+#pragma unroll
+                for (int h = 0; h < NG / 4; ++h) {
+                    const float sum = ti == 0 ? sums[4 * h] : (ti == 1 ? sums[4 * h + 1] : (ti == 2 ? sums[4 * h + 2] : sums[4 * h + 3]));
+                    const uint32_t high = xbtc::pack_bf16(0.f, sum);
+                    qw[j][2 * h] = high;
+                    qw[j][2 * h + 1] = xbtc::pack_bf16(0.f, sum - least_of(high));
+                }
+            }
             // what the lane's columns 2 ti and 2 ti + 1 of S^T need
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int from_lane = (2 * ti + e) * 4;
+                if constexpr (!BY_WORDS) {
 #pragma unroll
-                for (int n = 0; n < NG; ++n) qsum[j][n][e] = __shfl_sync(0xffffffffu, sums[n], from_lane);
+                    for (int n = 0; n < NG; ++n) qsum[j][n][e] = __shfl_sync(0xffffffffu, sums[n], from_lane);
+                }
                 const float back = ldexpf(A.scale * 1.4426950408889634f, 133 - __shfl_sync(0xffffffffu, e2, from_lane));
                 c1[j][e] = fminf(fmaxf(back, -3.0e38f), 3.0e38f);      // (queries near 2^128: a sum of zero stays one)
             }
         }
-        float o[NT][2 * NG][4] = {}, eight[NT][4] = {}, rest[NT][NG][2] = {}, ref[NT][2], l[NT][2] = {};
+        // `base`: 44 minus a column's reference; an infinity before there is one, which makes every score one above it
+        float o[NT][2 * NG][4] = {}, eight[NT][4] = {}, base[NT][2], l[NT][2] = {};
+        float rest[NT][BY_WORDS ? 1 : NG][2] = {}, both[NT][4] = {};       // sums of p (m + 8 s) per group; of p s and p m in rows 2 group and 2 group + 1
 #pragma unroll
-        for (int j = 0; j < NT; ++j) ref[j][0] = ref[j][1] = -INFINITY;
+        for (int j = 0; j < NT; ++j) base[j][0] = base[j][1] = INFINITY;
 
-        // ---- fetching: a step's codes as [group][key][16 bytes], its words as [key][group]; keys, then values
-        int ids = -1, ids_from = -1, put = from;           // a lane holds the page of one of 32 pieces
-        unsigned long long bad = 0;                        // two bits a step, of the last 32: pieces without a page
-        auto issue = [&]() {
-            // (all lanes)
-            const int pieces_a_step = STEP / piece_keys, at = (put - from) * pieces_a_step;
-            if (at / 32 * 32 != ids_from) {
-                ids_from = at / 32 * 32;
-                const long long key = (long long)from * STEP + (long long)(ids_from + lane) * piece_keys;
-                ids = -1;
-                if (key < (long long)to * STEP && key < w.r.keys) {
-                    ids = table[key / ps];
-                    if (ids < 0 || ids >= A.num_pages) {
-                        atomicOr(A.err, XB_ERR_BAD_PAGE);
-                        ids = -1;
-                    }
+        for (int s = from; s < to; s += STAGE_STEPS) {
+            const bool ok = xbtc::mbar_wait(bars + 8 * take_slot, take_parity, A.err, true);
+            if (!__all_sync(0xffffffffu, ok)) {            // (reported: what comes out then does not count)
+                failed = true;
+                for (int i = s + STAGE_STEPS; i < put; i += STAGE_STEPS) {
+                    take_slot = take_slot + 1 == STAGES ? 0 : take_slot + 1;
+                    if (take_slot == 0) take_parity ^= 1;
+                    xbtc::mbar_wait(bars + 8 * take_slot, take_parity, A.err);
                 }
-            }
-            const uint32_t bar = bars + 8 * (issued % STAGES), dst = ring + issued % STAGES * STAGE;
-            const int id0 = __shfl_sync(0xffffffffu, ids, at & 31), id1 = pieces_a_step == 2 ? __shfl_sync(0xffffffffu, ids, (at & 31) + 1) : id0;
-            const unsigned none = (id0 < 0 ? 1u : 0u) | (id1 < 0 ? 2u : 0u);
-            bad = bad << 2 | none;
-            const int key0 = put * STEP;
-            if (pieces_a_step == 1) {
-                if (lane == 0) xbtc::mbar_expect_tx(bar, none ? 0 : STAGE);
-                __syncwarp();
-                if (!none) {
-                    const long long page = (long long)id0 * A.nkv * page_bytes;
-                    if (ps == STEP) {
-                        if (lane < 2) bulk_copy(dst + lane * HALF, (lane ? v_pages : k_pages) + page, HALF, bar);
-                    } else if (lane < 2 * (NG + 1)) {
-                        const int n = lane % (NG + 1), slot = key0 % ps;
-                        const uint8_t* src = (lane > NG ? v_pages : k_pages) + page;
-                        src += n < NG ? ((long long)n * ps + slot) * 16 : (long long)ps * 16 * NG + slot * NG * 4;
-                        bulk_copy(dst + (lane > NG ? HALF : 0) + n * STEP * 16, src, n < NG ? STEP * 16 : STEP * NG * 4, bar);
-                    }
-                }
-            } else {
-                const int there = (id0 < 0 ? 0 : 1) + (id1 < 0 ? 0 : 1);
-                if (lane == 0) xbtc::mbar_expect_tx(bar, there * (STAGE / 2));
-                __syncwarp();
-                for (int i = lane; i < 4 * (NG + 1); i += 32) {
-                    const int half = i & 1, n = (i >> 1) % (NG + 1), v = (i >> 1) / (NG + 1), id = half ? id1 : id0;
-                    if (id < 0) continue;
-                    const int slot = (key0 + half * 8) % ps;
-                    const uint8_t* src = (v ? v_pages : k_pages) + (long long)id * A.nkv * page_bytes;
-                    src += n < NG ? ((long long)n * ps + slot) * 16 : (long long)ps * 16 * NG + slot * NG * 4;
-                    const uint32_t to_smem = dst + v * HALF + (n < NG ? n * STEP * 16 + half * 128 : CODES + half * 8 * NG * 4);
-                    bulk_copy(to_smem, src, n < NG ? 128 : 8 * NG * 4, bar);
-                }
-            }
-            ++issued;
-            ++put;
-        };
-        for (int i = 0; i < STAGES && put < to; ++i) issue();
-
-        for (int s = from; s < to; ++s) {
-            const uint32_t at = ring + taken % STAGES * STAGE;
-            failed = !__all_sync(0xffffffffu, xbtc::mbar_wait(bars + 8 * (taken % STAGES), taken / STAGES & 1, A.err, true));
-            if (failed) {
-                while (++taken < issued) xbtc::mbar_wait(bars + 8 * (taken % STAGES), taken / STAGES & 1, A.err);
                 break;
             }
-            const unsigned none = (unsigned)(bad >> (2 * (put - 1 - s))) & 3u;
-            const int key0 = s * STEP;
-            // ---- scores
-            float x[NT][4] = {};
-            {
-                const uint32_t row = at + (lane & 15) * 16 + (lane >> 4) * STEP * 16;      // matrices: keys 0..7 and 8..15 of a group, then of the next
-                uint32_t wd[2][NG];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t words = at + CODES + (gi + 8 * h) * NG * 4;
-                    if constexpr (NG % 4 == 0) {
-#pragma unroll
-                        for (int n = 0; n < NG; n += 4)
-                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(wd[h][n]), "=r"(wd[h][n + 1]), "=r"(wd[h][n + 2]), "=r"(wd[h][n + 3]) : "r"(words + n * 4) : "memory");
-                    } else {
-#pragma unroll
-                        for (int n = 0; n < NG; ++n) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(wd[h][n]) : "r"(words + n * 4) : "memory");
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < NG; n += 2) {
-                    uint32_t c[4];
-                    ldmatrix_x4(n + 1 < NG ? row + n * STEP * 16 : at + (lane & 15) * 16 + n * STEP * 16, c);
-#pragma unroll
-                    for (int u = 0; u < 2 && n + u < NG; ++u) {
-                        const uint32_t a = c[2 * u], b = c[2 * u + 1], a8 = a >> 8, b8 = b >> 8;
-                        const float sa = scale_of(wd[0][n + u]), ma = least_of(wd[0][n + u]), sb = scale_of(wd[1][n + u]), mb = least_of(wd[1][n + u]);
+            const int ahead = (put - s) / STAGE_STEPS - 1;           // stages issued behind this one
+            const unsigned none = none_of >> (8 * ahead);
+            auto step = [&](auto masks, const int sub, const unsigned lost) {
+                constexpr bool MASKED = decltype(masks)::value;            // some row does not see all of the step's keys
+                const uint32_t at = ring + take_slot * STAGE + sub * 2 * HALF;
+                const int key0 = (s + sub) * STEP;
+                // ---- scores
+                float x[NT][4] = {};
+                {
+                    uint32_t wd[2][NG];
+                    load_words<NG>(at + CODES + gi * NG * 4, wd);
+                    if constexpr (BY_WORDS) {
+                        uint32_t c[4];
+                        if constexpr (NG == 4) ldmatrix_x2(at + CODES + (lane & 15) * 16, c);
+                        else ldmatrix_x4(at + CODES + (lane & 15) * 32 + (lane >> 4) * 16, c);
 #pragma unroll
                         for (int j = 0; j < NT; ++j) {
-                            float d[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma(d, a & LOW, b & LOW, a & HIGH, b & HIGH, qf[j][n + u][0], qf[j][n + u][1]);
-                            mma(d, a8 & LOW, b8 & LOW, a8 & HIGH, b8 & HIGH, qf[j][n + u][2], qf[j][n + u][3]);
-                            x[j][0] = fmaf(sa, d[0], fmaf(ma, qsum[j][n + u][0], x[j][0]));
-                            x[j][1] = fmaf(sa, d[1], fmaf(ma, qsum[j][n + u][1], x[j][1]));
-                            x[j][2] = fmaf(sb, d[2], fmaf(mb, qsum[j][n + u][0], x[j][2]));
-                            x[j][3] = fmaf(sb, d[3], fmaf(mb, qsum[j][n + u][1], x[j][3]));
+                            if constexpr (NG == 4) {
+                                mma0(x[j], c[0], c[1], c[0], c[1], qw[j][0], qw[j][1]);
+                            } else {
+                                mma0(x[j], c[0], c[1], c[2], c[3], qw[j][0], qw[j][2]);
+                                mma(x[j], c[0], c[1], c[2], c[3], qw[j][1], qw[j][3]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NG; n += 2) {
+                        uint32_t c[4];                     // keys 0..7 and 8..15 of a group, then of the next
+                        ldmatrix_x4(at + (lane & 15) * 16 + (n + 1 < NG ? lane >> 4 : 0) * STEP * 16 + n * STEP * 16, c);
+#pragma unroll
+                        for (int u = 0; u < 2 && n + u < NG; ++u) {
+                            const uint32_t a = c[2 * u], b = c[2 * u + 1], a8 = a >> 8, b8 = b >> 8;
+                            const float sa = scale_of(wd[0][n + u]), sb = scale_of(wd[1][n + u]);
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) {
+                                float d[4];
+                                mma0(d, a & LOW, b & LOW, a & HIGH, b & HIGH, qf[j][n + u][0], qf[j][n + u][1]);
+                                mma(d, a8 & LOW, b8 & LOW, a8 & HIGH, b8 & HIGH, qf[j][n + u][2], qf[j][n + u][3]);
+                                if constexpr (!BY_WORDS) {
+                                    const float ma = least_of(wd[0][n + u]), mb = least_of(wd[1][n + u]);
+                                    x[j][0] = fmaf(ma, qsum[j][n + u][0], x[j][0]);
+                                    x[j][1] = fmaf(ma, qsum[j][n + u][1], x[j][1]);
+                                    x[j][2] = fmaf(mb, qsum[j][n + u][0], x[j][2]);
+                                    x[j][3] = fmaf(mb, qsum[j][n + u][1], x[j][3]);
+                                }
+                                x[j][0] = fmaf(sa, d[0], x[j][0]);
+                                x[j][1] = fmaf(sa, d[1], x[j][1]);
+                                x[j][2] = fmaf(sb, d[2], x[j][2]);
+                                x[j][3] = fmaf(sb, d[3], x[j][3]);
+                            }
                         }
                     }
                 }
-            }
-            // ---- probabilities: element e of x is key gi + 8 (e / 2), column 2 ti + e % 2
-            const bool masked = none || key0 < low1 || key0 + STEP - 1 > min(pos0, w.r.keys - 1);
-            uint32_t seen = 0xffffffffu;                   // bit 4 j + e
-            if (masked) {
-                seen = 0;
+                // ---- probabilities times 2^44: element e of x is key gi + 8 (e / 2), column 2 ti + e % 2
+                uint32_t seen = 0xffffffffu;               // bit 4 j + e
+                if constexpr (MASKED) {
+                    seen = 0;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = key0 + gi + 8 * (e >> 1), row = min(j * 8 + 2 * ti + (e & 1), rows - 1), pos = w.r.first_pos + (row0 + row) / group;
+                            const bool is = !(lost >> (e >> 1) & 1) && key < w.r.keys && key <= pos && key >= first_seen(A, pos);
+                            seen |= is ? 1u << (4 * j + e) : 0u;
+                        }
+                }
+                bool higher = false;
+                float p[NT][4];
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int key = key0 + gi + 8 * (e >> 1), row = min(j * 8 + 2 * ti + (e & 1), rows - 1), pos = w.r.first_pos + (row0 + row) / group;
-                        const bool there = !(none & (e >> 1 && piece_keys != STEP ? 2u : 1u));
-                        if (there && key < w.r.keys && key <= pos && key >= first_seen(A, pos)) seen |= 1u << (4 * j + e);
+                        p[j][e] = fmaf(x[j][e], c1[j][e & 1], base[j][e & 1]);
+                        higher |= !(p[j][e] <= TOP);       // (a score that is no number is one too)
                     }
-            }
-            bool higher = false;
+                if (__any_sync(0xffffffffu, higher)) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+                    for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[j][e] *= c1[j][e & 1];
-                    if (!(seen >> (4 * j + e) & 1)) x[j][e] = -INFINITY;
-                    higher |= !(x[j][e] <= ref[j][e & 1] + RESCALE_STEP);       // (a score that is no number is one too)
+                        for (int e = 0; e < 2; ++e) {
+                            const float x0 = seen >> (4 * j + e) & 1 ? x[j][e] * c1[j][e] : -INFINITY, x1 = seen >> (4 * j + e + 2) & 1 ? x[j][e + 2] * c1[j][e] : -INFINITY;
+                            float top = max_nan(x0, x1);
+                            top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                            top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                            top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                            const float now = UP - top;
+                            if (!(now >= base[j][e])) {    // (smaller, or no number)
+                                const float f = base[j][e] == INFINITY ? 0.f : xbtc::ex2(now - base[j][e]);
+                                base[j][e] = now;
+                                l[j][e] *= f;
+                                eight[j][e] *= f, eight[j][e + 2] *= f;
+#pragma unroll
+                                for (int n = 0; n < (BY_WORDS ? 0 : NG); ++n) rest[j][n][e] *= f;
+                                both[j][e] *= f, both[j][e + 2] *= f;
+#pragma unroll
+                                for (int n = 0; n < 2 * NG; ++n) o[j][n][e] *= f, o[j][n][e + 2] *= f;
+                            }
+                            p[j][e] = base[j][e] == INFINITY ? -INFINITY : fmaf(x[j][e], c1[j][e], base[j][e]);
+                            p[j][e + 2] = base[j][e] == INFINITY ? -INFINITY : fmaf(x[j][e + 2], c1[j][e], base[j][e]);
+                        }
                 }
-            if (__any_sync(0xffffffffu, higher)) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float top = max_nan(x[j][e], x[j][e + 2]);
-                        top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                        top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                        top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                        const float now = max_nan(ref[j][e], top), f = ref[j][e] == -INFINITY ? 0.f : xbtc::ex2(ref[j][e] - now);
-                        if (now != ref[j][e]) {
-                            ref[j][e] = now;
-                            l[j][e] *= f;
-                            eight[j][e] *= f, eight[j][e + 2] *= f;
+                    for (int e = 0; e < 4; ++e) p[j][e] = xbtc::ex2(p[j][e]);
+                if constexpr (MASKED) {
 #pragma unroll
-                            for (int n = 0; n < NG; ++n) rest[j][n][e] *= f;
+                    for (int j = 0; j < NT; ++j)
 #pragma unroll
-                            for (int n = 0; n < 2 * NG; ++n) o[j][n][e] *= f, o[j][n][e + 2] *= f;
+                        for (int e = 0; e < 4; ++e)
+                            if (!(seen >> (4 * j + e) & 1)) p[j][e] = 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) l[j][0] += p[j][0] + p[j][2], l[j][1] += p[j][1] + p[j][3];
+                // ---- values
+                {
+                    uint32_t wd[2][NG];
+                    load_words<NG>(at + HALF + CODES + gi * NG * 4, wd);
+                    // (what a row does not see must not reach it, whatever it is: zero times no number is no number)
+                    if constexpr (BY_WORDS) {
+                        uint32_t c[4];
+                        if constexpr (NG == 4) ldmatrix_x2_t(at + HALF + CODES + (lane & 15) * 16, c);
+                        else ldmatrix_x4_t(at + HALF + CODES + (lane & 15) * 32 + (lane >> 4) * 16, c);
+                        if constexpr (MASKED) {            // those who see words that are no numbers get one by p s
+#pragma unroll
+                            for (int i = 0; i < NG / 2; ++i) c[i] = finite_halves(c[i]);
                         }
-                    }
-            }
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float base = ref[j][e & 1] == -INFINITY ? 0.f : ref[j][e & 1];
-                    x[j][e] = xbtc::ex2(x[j][e] - base);
-                    l[j][e & 1] += x[j][e];
-                }
-            // ---- values
-            {
-                const uint32_t row = at + HALF + (lane & 15) * 16 + (lane >> 4) * STEP * 16;
-                uint32_t wd[2][NG];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t words = at + HALF + CODES + (gi + 8 * h) * NG * 4;
-                    if constexpr (NG % 4 == 0) {
-#pragma unroll
-                        for (int n = 0; n < NG; n += 4)
-                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(wd[h][n]), "=r"(wd[h][n + 1]), "=r"(wd[h][n + 2]), "=r"(wd[h][n + 3]) : "r"(words + n * 4) : "memory");
-                    } else {
-#pragma unroll
-                        for (int n = 0; n < NG; ++n) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(wd[h][n]) : "r"(words + n * 4) : "memory");
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < NG; n += 2) {
-                    uint32_t c[4];
-                    ldmatrix_x4_t(n + 1 < NG ? row + n * STEP * 16 : at + HALF + (lane & 15) * 16 + n * STEP * 16, c);
-#pragma unroll
-                    for (int u = 0; u < 2 && n + u < NG; ++u) {
-                        const uint32_t a = c[2 * u], b = c[2 * u + 1], a8 = a >> 8, b8 = b >> 8;
-                        const float sa = scale_of(wd[0][n + u]) * UP, sb = scale_of(wd[1][n + u]) * UP;
-                        const float ma = fmaf(scale_of(wd[0][n + u]), 8.f, least_of(wd[0][n + u])), mb = fmaf(scale_of(wd[1][n + u]), 8.f, least_of(wd[1][n + u]));
-                        const uint32_t mine = gi == n + u ? 0x00080008u : 0u;          // 8 2^-133 in the group's row
 #pragma unroll
                         for (int j = 0; j < NT; ++j) {
-                            float y[4] = {x[j][0] * sa, x[j][1] * sa, x[j][2] * sb, x[j][3] * sb}, z[4] = {x[j][0] * ma, x[j][1] * ma, x[j][2] * mb, x[j][3] * mb};
-                            if (masked) {                  // what is not seen adds nothing, whatever its scale is
+                            const uint32_t h0 = xbtc::pack_bf16(p[j][0], p[j][1]), h1 = xbtc::pack_bf16(p[j][2], p[j][3]);
+                            const uint32_t r0 = pack_rest(p[j][0], p[j][1], h0), r1 = pack_rest(p[j][2], p[j][3], h1);
+                            const uint32_t p0 = transposed(h0), p1 = transposed(h1), q0 = transposed(r0), q1 = transposed(r1);
+                            mma(both[j], c[0], NG == 4 ? 0u : c[2], c[1], NG == 4 ? 0u : c[3], p0, p1);
+                            mma(both[j], c[0], NG == 4 ? 0u : c[2], c[1], NG == 4 ? 0u : c[3], q0, q1);
+                        }
+                    }
 #pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    if (!(seen >> (4 * j + e) & 1)) y[e] = z[e] = 0.f;
+                    for (int n = 0; n < NG; n += 2) {
+                        uint32_t c[4];
+                        ldmatrix_x4_t(at + HALF + (lane & 15) * 16 + (n + 1 < NG ? lane >> 4 : 0) * STEP * 16 + n * STEP * 16, c);
+#pragma unroll
+                        for (int u = 0; u < 2 && n + u < NG; ++u) {
+                            const uint32_t a = c[2 * u], b = c[2 * u + 1], a8 = a >> 8, b8 = b >> 8;
+                            const float sa = scale_of(wd[0][n + u]), sb = scale_of(wd[1][n + u]);
+                            const uint32_t mine = gi == n + u ? 0x00080008u : 0u;          // 8 2^-133 in the group's row
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) {
+                                float y[4] = {p[j][0] * sa, p[j][1] * sa, p[j][2] * sb, p[j][3] * sb};
+                                if constexpr (MASKED) {
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        const uint32_t word = wd[e >> 1][n + u];
+                                        y[e] = !(seen >> (4 * j + e) & 1) ? 0.f : (finite_halves(word) == word ? y[e] : __uint_as_float(0x7fffffffu));
+                                    }
+                                }
+                                if constexpr (!BY_WORDS) {
+                                    const float ma = fmaf(sa, 8.f, least_of(wd[0][n + u])), mb = fmaf(sb, 8.f, least_of(wd[1][n + u]));
+                                    if constexpr (!MASKED) {
+                                        rest[j][n + u][0] = fmaf(p[j][0], ma, fmaf(p[j][2], mb, rest[j][n + u][0]));
+                                        rest[j][n + u][1] = fmaf(p[j][1], ma, fmaf(p[j][3], mb, rest[j][n + u][1]));
+                                    } else {
+#pragma unroll
+                                        for (int e = 0; e < 4; ++e)
+                                            if (seen >> (4 * j + e) & 1) rest[j][n + u][e & 1] = fmaf(p[j][e], e < 2 ? ma : mb, rest[j][n + u][e & 1]);
+                                    }
+                                }
+                                const uint32_t p0 = transposed(xbtc::pack_bf16(y[0], y[1])), p1 = transposed(xbtc::pack_bf16(y[2], y[3]));
+                                mma(o[j][2 * (n + u)], a & LOW, a & HIGH, b & LOW, b & HIGH, p0, p1);
+                                mma(o[j][2 * (n + u) + 1], a8 & LOW, a8 & HIGH, b8 & LOW, b8 & HIGH, p0, p1);
+                                mma(eight[j], mine, 0u, mine, 0u, p0, p1);
                             }
-                            rest[j][n + u][0] += z[0] + z[2];
-                            rest[j][n + u][1] += z[1] + z[3];
-                            const uint32_t p0 = transposed(xbtc::pack_bf16(y[0], y[1])), p1 = transposed(xbtc::pack_bf16(y[2], y[3]));
-                            mma(o[j][2 * (n + u)], a & LOW, a & HIGH, b & LOW, b & HIGH, p0, p1);
-                            mma(o[j][2 * (n + u) + 1], a8 & LOW, a8 & HIGH, b8 & LOW, b8 & HIGH, p0, p1);
-                            mma(eight[j], mine, 0u, mine, 0u, p0, p1);
                         }
                     }
                 }
+            };
+#pragma unroll 1
+            for (int sub = 0; sub < STAGE_STEPS && s + sub < to; ++sub) {
+                const unsigned lost = by16 ? (none >> sub & 1) * 3u : none >> (2 * sub) & 3u;
+                const int key0 = (s + sub) * STEP;
+                if (lost || key0 < all0 || key0 + STEP > all1) step(std::true_type(), sub, lost);
+                else step(std::false_type(), sub, 0u);
             }
             __syncwarp();
-            ++taken;
+            take_slot = take_slot + 1 == STAGES ? 0 : take_slot + 1;
+            if (take_slot == 0) take_parity ^= 1;
             if (put < to) issue();
         }
-        // ---- the warps' results, joined by the block
-        __syncthreads();                                   // (the rings are empty: results may lie there)
-        float* mine = reinterpret_cast<float*>(mem) + warp * result_floats(NT, NG);
-        if (failed)
-            for (int j = 0; j < NT; ++j) l[j][0] = l[j][1] = 0.f, ref[j][0] = ref[j][1] = -INFINITY;
+        // ---- the segment's result: whole rows, or a part
+        const bool whole = w.i0 == 0 && w.i1 == w.tiles;
+        const size_t part = (size_t)me * 2 + (w.from > w.job ? 0 : 1);
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+                const int row = j * 8 + 2 * ti + e;
                 float sum = l[j][e];
 #pragma unroll
                 for (int s = 4; s < 32; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-                float* to_row = mine + (j * 8 + 2 * ti + e) * (DP + 4);
-                float* ml = mine + ROWS * (DP + 4) + (j * 8 + 2 * ti + e) * 2;
-                if (gi == 0) ml[0] = ref[j][e], ml[1] = sum;
+                sum *= DOWN;
+                const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+                const long long t = w.r.first + (row0 + min(row, rows - 1)) / group;
+                __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + t * A.out_stride + (long long)(w.g * group + (row0 + row) % group) * A.d;
 #pragma unroll
                 for (int n = 0; n < NG; ++n) {
-                    float r = rest[j][n][e];
+                    float r;
+                    if constexpr (BY_WORDS) {
+                        const float s8 = __shfl_sync(0xffffffffu, both[j][e + (n >= 4 ? 2 : 0)], (2 * n & 7) * 4 + ti);
+                        r = fmaf(8.f, s8, __shfl_sync(0xffffffffu, both[j][e + (n >= 4 ? 2 : 0)], ((2 * n & 7) + 1) * 4 + ti));
+                    } else {
+                        r = rest[j][n][e];
 #pragma unroll
-                    for (int s = 4; s < 32; s <<= 1) r += __shfl_xor_sync(0xffffffffu, r, s);
+                        for (int s = 4; s < 32; s <<= 1) r += __shfl_xor_sync(0xffffffffu, r, s);
+                    }
+                    r *= DOWN;
                     const float minus = __shfl_sync(0xffffffffu, eight[j][e], n * 4 + ti);
-                    float4 v;
-                    v.x = fmaf(o[j][2 * n][e] - minus, BACK, r);
-                    v.y = fmaf(o[j][2 * n][e + 2] * 0.0625f - minus, BACK, r);
-                    v.z = fmaf(o[j][2 * n + 1][e] - minus, BACK, r);
-                    v.w = fmaf(o[j][2 * n + 1][e + 2] * 0.0625f - minus, BACK, r);
-                    *reinterpret_cast<float4*>(to_row + 32 * n + 4 * gi) = v;
-                }
-            }
-        __syncthreads();
-        {
-            const bool whole = w.i0 == 0 && w.i1 == w.tiles;
-            const int which = w.from > w.job ? 0 : 1;
-            const size_t part = (size_t)blockIdx.x * 2 + which;
-            const float* all = reinterpret_cast<const float*>(mem);
-            constexpr int FLOATS = result_floats(NT, NG);
-            for (int i = threadIdx.x; i < rows * (DP / 4); i += THREADS) {
-                const int row = i / (DP / 4), c = i % (DP / 4) * 4;
-                float top = -INFINITY, f[WARPS], total = 0.f;
+                    const float v[4] = {fmaf(o[j][2 * n][e] - minus, BACK, r) * inv, fmaf(o[j][2 * n][e + 2] * 0.0625f - minus, BACK, r) * inv,
+                                        fmaf(o[j][2 * n + 1][e] - minus, BACK, r) * inv, fmaf(o[j][2 * n + 1][e + 2] * 0.0625f - minus, BACK, r) * inv};
+                    const int c = 32 * n + 4 * gi;
+                    if (row >= rows) continue;
+                    if (!whole) {
+                        *reinterpret_cast<float4*>(line.part_o + (part * ROWS + row) * DP + c) = make_float4(v[0], v[1], v[2], v[3]);
+                    } else if (out8) {
+                        if (c < A.d) *reinterpret_cast<uint2*>(out + c) = make_uint2(xbtc::pack_bf16(v[0], v[1]), xbtc::pack_bf16(v[2], v[3]));
+                    } else {
 #pragma unroll
-                for (int k = 0; k < WARPS; ++k) top = max_nan(top, all[k * FLOATS + ROWS * (DP + 4) + row * 2]);
-                float4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < WARPS; ++k) {
-                    const float ref_k = all[k * FLOATS + ROWS * (DP + 4) + row * 2];
-                    f[k] = ref_k == -INFINITY ? 0.f : xbtc::ex2(ref_k - top);
-                    if (ref_k == -INFINITY) continue;
-                    total = fmaf(f[k], all[k * FLOATS + ROWS * (DP + 4) + row * 2 + 1], total);
-                    const float4 u = *reinterpret_cast<const float4*>(all + k * FLOATS + row * (DP + 4) + c);
-                    v.x = fmaf(f[k], u.x, v.x), v.y = fmaf(f[k], u.y, v.y), v.z = fmaf(f[k], u.z, v.z), v.w = fmaf(f[k], u.w, v.w);
+                        for (int i = 0; i < 4; ++i)
+                            if (c + i < A.d) out[c + i] = __float2bfloat16_rn(v[i]);
+                    }
                 }
-                if (whole) {
-                    const long long t = w.r.first + (row0 + row) / group;
-                    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + t * A.out_stride + (long long)(w.g * group + (row0 + row) % group) * A.d;
-                    const float inv = total == 0.f ? 0.f : 1.f / total;
-                    const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (c + e < A.d) out[c + e] = __float2bfloat16_rn(y[e]);
-                } else {
-                    *reinterpret_cast<float4*>(line.part_o + (part * ROWS + row) * DP + c) = v;
-                    if (c == 0) line.part_ml[(part * ROWS + row) * 2] = top, line.part_ml[(part * ROWS + row) * 2 + 1] = total;
-                }
+                // (minus infinity: there is nothing)
+                if (!whole && gi == 0 && row < rows) *reinterpret_cast<float2*>(line.part_ml + (part * ROWS + row) * 2) = make_float2(UP - base[j][e], sum);
             }
-            if (!whole && threadIdx.x == 0) {
-                int* job = line.jobs + part * JOB_WORDS;
-                const int first_block = w.job / w.share, last = (w.job + (w.tiles - 1) * COST_TILE) / w.share;
-                job[1] = first_block, job[2] = row0, job[3] = rows, job[4] = w.g, job[5] = w.b;
-                job[0] = last - first_block + 1;
-            }
+        if (!whole && lane == 0) {
+            int* job = line.jobs + part * JOB_WORDS;
+            const int first_warp = w.job / w.share, last = (w.job + w.tiles - 1) / w.share;
+            job[1] = first_warp, job[2] = row0, job[3] = rows, job[4] = w.g, job[5] = w.b;
+            job[0] = last - first_warp + 1;
         }
-        xbtc::fence_async_shared();
-        __syncthreads();                                   // (the next segment's copies may write where the results lay)
     }
 }
 
-// A job's parts, joined in the order of the line: the blocks that left them share its numbers.
+// A job's parts, joined in the order of the line: a warp for every part takes its share of the job's numbers, four to eight lanes each where the
+// parts are many.
 template <int NT, int NG>
 __global__ void __launch_bounds__(THREADS)
 cache4_attention_join_kernel(const AttendArgs A, const Line line) {
     constexpr int ROWS = 8 * NT, DP = 32 * NG, FOURS = DP / 4;
     pdl_launch_dependents();
     pdl_wait();
-    const int* job = line.jobs + (size_t)blockIdx.x * JOB_WORDS;
-    const int parts = job[0];
+    const int lane = threadIdx.x & 31, entry = (int)blockIdx.x * WARPS + ((int)threadIdx.x >> 5);
+    const int* job = line.jobs + (size_t)entry * JOB_WORDS;
+    const int4 head = *reinterpret_cast<const int4*>(job);
+    const int parts = head.x;
     if (parts < 1) return;
-    const int first = job[1], row0 = job[2], rows = job[3], g = job[4], group = A.nh / A.nkv;
+    const int first = head.y, row0 = head.z, rows = head.w, g = job[4], group = A.nh / A.nkv;
     const Request r = request_of(A, job[5]);
-    const int mine = (int)blockIdx.x / 2 - first, total = rows * FOURS;
-    auto part_of = [&](int i) { return (size_t)(first + i) * 2 + (i == 0 ? 1 : 0); };     // (the first part is its block's last segment)
-    for (int i = total * mine / parts + (int)threadIdx.x; i < total * (mine + 1) / parts; i += THREADS) {
-        const int row = i / FOURS, c = i % FOURS * 4;
+    const int mine = entry / 2 - first, total = rows * FOURS;
+    auto part_of = [&](int i) { return (size_t)(first + i) * 2 + (i == 0 ? 1 : 0); };     // (the first part is its warp's last segment)
+    const int lanes = parts > 4 ? 8 : 1, sub = lane & (lanes - 1), lo = (int)((long long)total * mine / parts), hi = (int)((long long)total * (mine + 1) / parts);
+    for (int i0 = lo; i0 < hi; i0 += 32 / lanes) {
+        const int i = min(i0 + lane / lanes, hi - 1), row = i / FOURS, c = i % FOURS * 4;
         float top = -INFINITY, sum = 0.f;
-        for (int k = 0; k < parts; ++k) top = max_nan(top, line.part_ml[(part_of(k) * ROWS + row) * 2]);
+        for (int k = sub; k < parts; k += lanes) top = max_nan(top, line.part_ml[(part_of(k) * ROWS + row) * 2]);
+        for (int s = 1; s < lanes; s <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, s));
         float4 v = {0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < parts; ++k) {
+#pragma unroll 4
+        for (int k = sub; k < parts; k += lanes) {
             const size_t at = part_of(k) * ROWS + row;
-            const float ref = line.part_ml[at * 2];
-            if (ref == -INFINITY) continue;
-            const float f = xbtc::ex2(ref - top);
+            const float2 ml = *reinterpret_cast<const float2*>(line.part_ml + at * 2);
             const float4 u = *reinterpret_cast<const float4*>(line.part_o + at * DP + c);
-            sum = fmaf(f, line.part_ml[at * 2 + 1], sum);
+            const float f = ml.x == -INFINITY ? 0.f : xbtc::ex2(ml.x - top);       // (parts of nothing hold zeros)
+            sum = fmaf(f, ml.y, sum);
             v.x = fmaf(f, u.x, v.x), v.y = fmaf(f, u.y, v.y), v.z = fmaf(f, u.z, v.z), v.w = fmaf(f, u.w, v.w);
         }
+        for (int s = 1; s < lanes; s <<= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, s);
+            v.x += __shfl_xor_sync(0xffffffffu, v.x, s), v.y += __shfl_xor_sync(0xffffffffu, v.y, s);
+            v.z += __shfl_xor_sync(0xffffffffu, v.z, s), v.w += __shfl_xor_sync(0xffffffffu, v.w, s);
+        }
+        if (sub || i0 + lane / lanes >= hi) continue;
         const long long t = r.first + (row0 + row) / group;
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + t * A.out_stride + (long long)(g * group + (row0 + row) % group) * A.d;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -561,36 +656,36 @@ cache4_attention_join_kernel(const AttendArgs A, const Line line) {
 
 template <int NT, int NG>
 long long scratch_of() {
-    return (long long)blocks_of(NT, NG) * 2 * (8 * NT * (32 * NG + 2) + JOB_WORDS);
+    return (long long)blocks_of(NT, NG) * WARPS * 2 * (8 * NT * (32 * NG + 2) + JOB_WORDS);
 }
 
 template <int NT, int NG>
 int launch(const AttendArgs& A, float* scratch, cudaStream_t stream) {
-    constexpr int blocks = blocks_of(NT, NG);
+    constexpr int blocks = blocks_of(NT, NG), parts = blocks * WARPS * 2;
     Line line;
     line.part_o = scratch;
-    line.part_ml = scratch + (size_t)blocks * 2 * 8 * NT * 32 * NG;
-    line.jobs = reinterpret_cast<int*>(line.part_ml + (size_t)blocks * 2 * 8 * NT * 2);
-    line.min_share = COST_TILE;
+    line.part_ml = scratch + (size_t)parts * 8 * NT * 32 * NG;
+    line.jobs = reinterpret_cast<int*>(line.part_ml + (size_t)parts * 8 * NT * 2);
     static unsigned long long roomy = 0;
-    if (const int rc = xb_more_smem(cache4_attention_mma_kernel<NT, NG>, smem_bytes(NT, NG), &roomy)) return rc;
-    const int rc = xb_launch(cache4_attention_mma_kernel<NT, NG>, dim3(blocks), dim3(THREADS), smem_bytes(NT, NG), stream, A, line);
+    if (const int rc = xb_more_smem(cache4_attention_mma_kernel<NT, NG>, smem_bytes(NG), &roomy)) return rc;
+    const int rc = xb_launch(cache4_attention_mma_kernel<NT, NG>, dim3(blocks), dim3(THREADS), smem_bytes(NG), stream, A, line);
     if (rc) return rc;
-    return xb_launch(cache4_attention_join_kernel<NT, NG>, dim3(2 * blocks), dim3(THREADS), 0, stream, A, line);
+    return xb_launch(cache4_attention_join_kernel<NT, NG>, dim3(parts / WARPS), dim3(THREADS), 0, stream, A, line);
 }
 
+// Eight rows a job where no request brings more, else sixteen; heads of 256 channels always eight, whose sums alone are 64 registers a thread.
 template <typename F>
 auto by_form(int rows, int groups, F f) {
-    auto with = [&](auto nt) {
-        switch (groups) {
-            case 1: return f(nt, std::integral_constant<int, 1>());
-            case 2: return f(nt, std::integral_constant<int, 2>());
-            case 3: return f(nt, std::integral_constant<int, 3>());
-            case 4: return f(nt, std::integral_constant<int, 4>());
-            default: return f(nt, std::integral_constant<int, 8>());
-        }
-    };
-    return rows <= 8 ? with(std::integral_constant<int, 1>()) : with(std::integral_constant<int, 2>());
+    const std::integral_constant<int, 1> one{};
+    const std::integral_constant<int, 2> two{};
+    auto with = [&](auto ng) { return rows <= 8 ? f(one, ng) : f(two, ng); };
+    switch (groups) {
+        case 1: return with(std::integral_constant<int, 1>());
+        case 2: return with(std::integral_constant<int, 2>());
+        case 3: return with(std::integral_constant<int, 3>());
+        case 4: return with(std::integral_constant<int, 4>());
+        default: return f(one, std::integral_constant<int, 8>());
+    }
 }
 
 int rows_of(int nh, int nkv, int longest) {
@@ -606,7 +701,7 @@ bool mma_takes(int d) { return groups_of(d) <= 4 || groups_of(d) == 8; }
 bool mma_takes(const AttendArgs& A) {
     // the longest line that these shapes allow is counted in 32 bits
     const double jobs = (double)A.nkv * ((double)A.tokens * (A.nh / A.nkv) / 8 + A.requests), tiles = (double)A.table_stride * A.page_size / KT + 2;
-    return mma_takes(A.d) && A.page_size % 8 == 0 && A.num_pages > 0 && jobs * (tiles * COST_TILE + COST_JOB) < 2147483648.0;
+    return mma_takes(A.d) && A.page_size % 8 == 0 && A.num_pages > 0 && jobs * (tiles + COST_JOB) < 2147483648.0;
 }
 long long mma_scratch(int nh, int nkv, int d, int longest) {
     return by_form(rows_of(nh, nkv, longest), groups_of(d), [](auto nt, auto ng) { return scratch_of<decltype(nt)::value, decltype(ng)::value>(); });
