@@ -4,21 +4,13 @@
 // Lane 4 g + t of a warp has rows g and g + 8 (two pieces of 16 bytes, 512 bytes apart) and in them the columns 32 j + 8 t + e of word j: as an
 // MMA's lanes take them, each word's columns in one group whatever the group's size.  Column e of a word lies in its half byte 4 (e & 1) +
 // e / 2, so that a mask takes out a pair of neighbours.  Rows and columns beyond the weight have codes and words of zeros.
-#include "codes4.cuh"
+#include "linear4.h"
 
 namespace {
 
 using namespace xb4;
 
-struct LinearArgs {
-    void* out;                     // [tokens, rows], rows `out_stride` elements apart
-    const void* x;                 // [tokens, columns], rows `x_stride` elements apart
-    const uint8_t* weight;         // [row tiles, column tiles, tile bytes]
-    long long out_stride, x_stride;
-    int tokens, rows, columns, per_row;      // per_row: groups of a tile's row (4, 2, 1)
-};
-
-// Any type and size: a block per tile of rows and eight tokens, its warps take the column tiles in turn.  Products and sums in float32.
+// float32: a block per tile of rows and eight tokens, its warps take the column tiles in turn.  Products and sums in float32.
 constexpr int ANY_WARPS = 8, ANY_TOKENS = 8;
 
 template <typename T>
@@ -85,11 +77,12 @@ int launch_any(const LinearArgs& A, cudaStream_t stream) {
 }  // namespace
 
 static int linear4(int dtype, void* out, const void* x, const uint8_t* weight, long long out_stride, long long x_stride, int tokens, int rows, int columns,
-                   int group, float* scratch, cudaStream_t stream) {
+                   int group, float* scratch, int* err, cudaStream_t stream) {
     if (tokens <= 0 || rows <= 0) return 0;
     if (columns < 1 || (group != 32 && group != 64 && group != 128) || tokens > 65535 * ANY_TOKENS) return (int)cudaErrorInvalidValue;
     const LinearArgs A{out, x, weight, out_stride, x_stride, tokens, rows, columns, TILE_COLS / group};
-    return dtype == XB_F32 ? launch_any<float>(A, stream) : launch_any<__nv_bfloat16>(A, stream);
+    if (dtype == XB_F32) return launch_any<float>(A, stream);
+    return A.tokens > 16 && linear4_tc_takes(A) ? linear4_tc(A, err, stream) : linear4_mma(A, stream);
 }
 XB_EXPORT int xb_linear4(const long long* words, int n) { return xb_by_words(linear4, words, n); }
 

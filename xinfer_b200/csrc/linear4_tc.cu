@@ -1,0 +1,300 @@
+// Products of many rows with a weight in 4 bits, in bfloat16 on the 5th-generation tensor cores (linear4.cu says what is computed and how a weight
+// lies).
+//
+// D[128 rows of the weight, up to 256 tokens] in tensor memory.  Sixteen warps take eight rows each of a column tile out of their codes, into the
+// shared-memory operand (128-byte swizzle); one thread fetches the tokens' columns by TMA, one issues the products.  A number of the weight
+// becomes m + s code rounded to bfloat16 once, as a weight in bfloat16 would be: the bits of a code under a mask are the bfloat16 c 2^-133 (16 times that
+// in the next four bits), so that one multiply-add of two numbers, by s 2^64 and m 2^-69, gives them both times 2^-69, which the sums are
+// multiplied by at the end.  Scales may be up to 2^60.
+// K is split over a cluster's blocks where the row tiles alone do not fill the processors; their sums meet through distributed shared memory in
+// rank order.
+#include "linear4.h"
+#include "tc_common.cuh"
+
+namespace {
+
+using namespace xb4;
+using namespace xbtc;
+
+constexpr int ROWS = 128, CODE_WARPS = 16, THREADS = (CODE_WARPS + 2) * 32;
+constexpr int A_BYTES = ROWS * TILE_COLS * 2, ATOM = ROWS * 128;       // an atom: 64 columns
+constexpr int TOKENS_MOST = 256, STAGES_MOST = 4, AHEAD = 4;
+constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
+constexpr uint32_t UP = 0x5f805f80u, UP16 = 0x5d805d80u, DOWN = 0x1d001d00u;       // 2^64, 2^60, 2^-69, twice
+constexpr float BACK = 0x1p69f;
+
+struct TcArgs {
+    LinearArgs a;
+    int mp, stages, tiles_per_split;       // tokens of a tile, padded
+    int* err;
+};
+
+__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t fma_bf16(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float of_rank(uint32_t addr, uint32_t rank) {
+    uint32_t remote;
+    float v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
+    return v;
+}
+
+// What a lane takes of a column tile: 32 codes of a row, and the row's words.
+template <int PER>
+struct Codes {
+    uint4 c;
+    uint32_t w[PER];
+};
+
+// grid: (row blocks, splits, token blocks); cluster (1, splits, 1)
+template <int PER>
+__global__ void __launch_bounds__(THREADS, 1)
+linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const TcArgs T) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * STAGES_MOST + 1];
+    __shared__ uint32_t s_tmem;
+    const LinearArgs& A = T.a;
+    constexpr int TILE = TILE_CODES + TILE_ROWS * PER * 4;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;       // (the swizzle repeats every 1024 bytes)
+    float* sums = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)));
+    const uint32_t x_atom = (uint32_t)T.mp * 128, stage_bytes = A_BYTES + 2 * x_atom;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mp = T.mp, stages = T.stages;
+    const int row_tiles = (A.rows + TILE_ROWS - 1) / TILE_ROWS, col_tiles = (A.columns + TILE_COLS - 1) / TILE_COLS;
+    const int from = blockIdx.y * T.tiles_per_split, iters = max(0, min(col_tiles - from, T.tiles_per_split));
+    const int t0 = blockIdx.z * mp, many = min(mp, A.tokens - t0);
+    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[STAGES_MOST]), accum = smem_u32(&bars[2 * STAGES_MOST]);
+    const uint32_t tmem_cols = mp < 32 ? 32u : (uint32_t)mp;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(full0 + 8 * s, CODE_WARPS + 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        mbar_init(accum, 1);
+        mbar_init_fence();
+    }
+    if (warp == CODE_WARPS) tmem_alloc(&s_tmem, tmem_cols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    pdl_launch_dependents();       // only now: see pdl_launch_dependents on tensor memory
+
+    if (warp < CODE_WARPS) {
+        // ---- codes to numbers: row 16 (warp / 2) + 8 (warp % 2) + g of the block; a weight is nobody's result, so nothing is waited for
+        const int g = lane >> 2, t = lane & 3, half = warp & 1;
+        const uint8_t* line = A.weight + ((long long)min((int)blockIdx.x * 8 + (warp >> 1), row_tiles - 1) * col_tiles + from) * TILE;     // (behind the last row: it again)
+        auto fetch = [&](Codes<PER>& to, int it) {
+            const uint8_t* tile = line + (long long)min(it, iters - 1) * TILE;
+            to.c = *reinterpret_cast<const uint4*>(tile + half * 512 + lane * 16);
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(tile + TILE_CODES) + (half * 8 + g) * PER;
+            if constexpr (PER == 4) {
+                const uint4 v = *reinterpret_cast<const uint4*>(w);
+                to.w[0] = v.x, to.w[1] = v.y, to.w[2] = v.z, to.w[3] = v.w;
+            } else if constexpr (PER == 2) {
+                const uint2 v = *reinterpret_cast<const uint2*>(w);
+                to.w[0] = v.x, to.w[1] = v.y;
+            } else {
+                to.w[0] = *w;
+            }
+        };
+        Codes<PER> have[AHEAD];
+        if (iters > 0) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) fetch(have[i], i);
+        }
+        // where the lane's eight numbers of word j go: odd rows take the words of a pair the other way round, so that eight lanes meet all banks
+        const int odd = g & 1;
+        const uint32_t row_at = (uint32_t)((warp >> 1) * 16 + half * 8 + g) * 128;
+        const uint32_t first_at = row_at + (uint32_t)(((odd * 4 + t) ^ g) << 4), second_at = row_at + (uint32_t)((((odd ^ 1) * 4 + t) ^ g) << 4);
+        int s = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int it0 = 0; it0 < iters && ok; it0 += AHEAD) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int it = it0 + i;
+                if (it >= iters || !ok) break;
+                if (it >= stages) ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, phase ^ 1u, T.err, true));
+                if (!ok) break;
+                const uint32_t to = base + s * stage_bytes;
+                const uint32_t cw[4] = {have[i].c.x, have[i].c.y, have[i].c.z, have[i].c.w};
+#pragma unroll
+                for (int p = 0; p < 2; ++p)                // words 2 p and 2 p + 1: an atom
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const uint32_t u = (q ^ odd) ? cw[2 * p + 1] : cw[2 * p], u8 = u >> 8;
+                        const uint32_t w = PER == 4 ? ((q ^ odd) ? have[i].w[2 * p + 1 < PER ? 2 * p + 1 : 0] : have[i].w[2 * p < PER ? 2 * p : 0]) : have[i].w[PER == 2 ? p : 0];
+                        const uint32_t sc = __byte_perm(w, w, 0x1010), m = times(__byte_perm(w, w, 0x3232), DOWN), s1 = times(sc, UP), s16 = times(sc, UP16);
+                        uint4 v;
+                        v.x = fma_bf16(u & LOW, s1, m), v.y = fma_bf16(u & HIGH, s16, m), v.z = fma_bf16(u8 & LOW, s1, m), v.w = fma_bf16(u8 & HIGH, s16, m);
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + p * ATOM + (q == 0 ? first_at : second_at)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+                    }
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full0 + 8 * s);
+                fetch(have[i], it + AHEAD);
+                if (++s == stages) {
+                    s = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+    } else if (threadIdx.x == CODE_WARPS * 32) {
+        // ---- the tokens' columns
+        pdl_wait();
+        int s = 0;
+        uint32_t phase = 0;
+        for (int it = 0; it < iters; ++it) {
+            if (it >= stages && !mbar_wait(empty0 + 8 * s, phase ^ 1u, T.err)) break;
+            const uint32_t dst = base + s * stage_bytes + A_BYTES;
+            mbar_expect_tx(full0 + 8 * s, 2 * x_atom);
+            tma_load_2d(dst, &map_x, (from + it) * TILE_COLS, t0, full0 + 8 * s);
+            tma_load_2d(dst + x_atom, &map_x, (from + it) * TILE_COLS + 64, t0, full0 + 8 * s);
+            if (++s == stages) {
+                s = 0;
+                phase ^= 1u;
+            }
+        }
+    } else if (threadIdx.x == (CODE_WARPS + 1) * 32) {
+        // ---- products
+        const uint32_t idesc = umma_idesc(mp);
+        int s = 0;
+        uint32_t phase = 0;
+        for (int it = 0; it < iters; ++it) {
+            if (!mbar_wait(full0 + 8 * s, phase, T.err)) {     // (reported; copies that are still on their way are waited for once more)
+                for (int i = 0; i < stages; ++i) mbar_wait(full0 + 8 * i, i < s ? phase ^ 1u : phase, T.err);
+                break;
+            }
+            tc_fence_after();
+            const uint32_t a = base + s * stage_bytes;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const uint64_t adesc = umma_desc(a + p * ATOM), bdesc = umma_desc(a + A_BYTES + p * x_atom);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) umma_bf16(tmem, adesc + (uint64_t)(kk * 2), bdesc + (uint64_t)(kk * 2), idesc, (it | p | kk) ? 1u : 0u);
+            }
+            umma_commit(empty0 + 8 * s);
+            if (++s == stages) {
+                s = 0;
+                phase ^= 1u;
+            }
+        }
+        umma_commit(accum);
+    }
+    __syncwarp();
+    pdl_wait();                    // nothing of the kernel before may still read what is written below
+    const uint32_t csize = cluster_size(), crank = cluster_rank();
+    const int n0 = blockIdx.x * ROWS;
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out);
+    const bool ready = mbar_wait(accum, 0, T.err) && iters > 0;
+    tc_fence_after();
+    if (warp < CODE_WARPS) {
+        // warps of a quarter of the rows share the tokens
+        const int row = (warp & 3) * 32 + lane;
+        for (int c0 = (warp >> 2) * 16; c0 < mp; c0 += (CODE_WARPS / 4) * 16) {
+            float v[16];
+            if (ready) {
+                tmem_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c0, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = 0.f;
+            }
+            if (csize == 1) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (c0 + i < many && n0 + row < A.rows) out[(long long)(t0 + c0 + i) * A.out_stride + n0 + row] = __float2bfloat16_rn(v[i] * BACK);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sums[(c0 + i) * ROWS + row] = v[i] * BACK;
+            }
+        }
+    }
+    if (csize > 1) {
+        cluster_sync();            // every block of the cluster has written its sums
+        const int total = many * ROWS, per = (total + (int)csize - 1) / (int)csize, end = min(total, ((int)crank + 1) * per);
+        for (int e = (int)crank * per + (int)threadIdx.x; e < end; e += THREADS) {
+            float v = 0.f;
+            for (uint32_t r = 0; r < csize; ++r) v += of_rank(base + (uint32_t)e * 4u, r);
+            const int n = n0 + e % ROWS;
+            if (n < A.rows) out[(long long)(t0 + e / ROWS) * A.out_stride + n] = __float2bfloat16_rn(v);
+        }
+        cluster_sync();            // nobody leaves while its sums are read
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == CODE_WARPS) tmem_free(tmem, tmem_cols);
+}
+
+// [tokens, columns] through boxes of 64 columns and `box` tokens, 128-byte swizzle; what lies outside is zero.
+bool map_of(CUtensorMap* map, const LinearArgs& A, int box) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)A.columns, (cuuint64_t)A.tokens}, strides[1] = {(cuuint64_t)A.x_stride * 2};
+    const cuuint32_t boxes[2] = {64, (cuuint32_t)box}, steps[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(A.x), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int PER>
+int launch(const LinearArgs& A, int* err, cudaStream_t stream) {
+    TcArgs T{A, 32, 0, 0, err};
+    while (T.mp < A.tokens && T.mp < TOKENS_MOST) T.mp *= 2;
+    const int blocks = (A.rows + ROWS - 1) / ROWS, col_tiles = (A.columns + TILE_COLS - 1) / TILE_COLS, token_blocks = (A.tokens + T.mp - 1) / T.mp;
+    // blocks enough for the processors, four column tiles each at least
+    int splits = 1;
+    while (splits < 8 && (long long)blocks * token_blocks * splits * 2 <= 148 && col_tiles / (splits * 2) >= 4) splits *= 2;
+    T.tiles_per_split = (col_tiles + splits - 1) / splits;
+    const int stage_bytes = A_BYTES + 2 * T.mp * 128;
+    T.stages = 200 * 1024 / stage_bytes < STAGES_MOST ? 200 * 1024 / stage_bytes : STAGES_MOST;
+    const int smem = T.stages * stage_bytes + 1024;        // (the sums, 512 bytes a token, fit the stages)
+    CUtensorMap map;
+    if (!map_of(&map, A, T.mp)) return (int)cudaErrorInvalidValue;
+    static unsigned long long roomy = 0;
+    if (const int rc = xb_more_smem(linear4_tc_kernel<PER>, 201 * 1024, &roomy)) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks, splits, token_blocks);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = splits;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = xb_pdl_enabled() ? 2 : 1;
+    const cudaError_t rc = cudaLaunchKernelEx(&cfg, linear4_tc_kernel<PER>, map, T);
+    return rc != cudaSuccess ? (int)rc : xb_launch_status();
+}
+
+}  // namespace
+
+namespace xb4 {
+
+bool linear4_tc_takes(const LinearArgs& A) { return ((uintptr_t)A.x & 15) == 0 && A.x_stride % 8 == 0; }
+int linear4_tc(const LinearArgs& A, int* err, cudaStream_t stream) {
+    return A.per_row == 4 ? launch<4>(A, err, stream) : (A.per_row == 2 ? launch<2>(A, err, stream) : launch<1>(A, err, stream));
+}
+
+}  // namespace xb4

@@ -2195,4 +2195,5 @@ def linear4(out, x, weight, *, scratch=None):
         if scratch.data_ptr() % 16:
             raise KernelError("scratch starts off a 16-byte boundary")
     _here(out, x, weight, scratch)
-    _ok(_call(_entry("xb_linear4"), code, out, x, weight, at[1], at[0], T, rows, columns, group, scratch if need else None, _stream()), "linear4")
+    _ok(_call(_entry("xb_linear4"), code, out, x, weight, at[1], at[0], T, rows, columns, group, scratch if need else None, own_err_word().data_ptr(),
+              _stream()), "linear4")
