@@ -31,8 +31,8 @@ __device__ __forceinline__ uint8_t* page_of(const WriteArgs& A, uint8_t* cache, 
     return cache + (slot / A.page_size * A.nkv + g) * ((long long)A.page_size * xb4::row_bytes(A.d));
 }
 
-// Any head of up to 512 channels: a warp per (token, head), a group's channels one to a lane.
-constexpr int ANY_WARPS = 8, ANY_MOST = 512;
+// Any head: a warp per (token, head), a group's channels one to a lane.
+constexpr int ANY_WARPS = 8, ANY_MOST = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(ANY_WARPS * 32)
@@ -107,8 +107,183 @@ cache4_write_any_kernel(const WriteArgs A) {
     }
 }
 
+// Heads of a multiple of 8 channels, up to 256, whose rotation pairs whole vectors of 8 (halves of a multiple of 8) or neighbours: a lane has 8
+// channels, LPH lanes a head, so a group's 32 channels are four lanes.  A warp takes one token and `each` times 32 / LPH of its heads, and keeps the
+// token's angles.
+constexpr int VEC_WARPS = 8;
+
 template <typename T>
-int launch_any(const WriteArgs& A, cudaStream_t stream) {
+__device__ __forceinline__ void load8(const T* x, float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        const uint4 u = *reinterpret_cast<const uint4*>(x);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    } else {
+        const float4 a = reinterpret_cast<const float4*>(x)[0], b = reinterpret_cast<const float4*>(x)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+}
+__device__ __forceinline__ uint32_t pack2bf(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* x, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(x) = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
+    } else {
+        reinterpret_cast<float4*>(x)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(x)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+}
+
+template <typename T, int LPH>
+__global__ void __launch_bounds__(VEC_WARPS * 32)
+cache4_write_kernel(const WriteArgs A, int each) {
+    constexpr int HEADS = 32 / LPH;
+    pdl_overlap_few();
+    const int lane = threadIdx.x & 31, li = lane & (LPH - 1), sub = lane / LPH, heads = A.nh + 2 * A.nkv, d = A.d;
+    const int per_token = (heads + HEADS * each - 1) / (HEADS * each);
+    const long long job = (long long)blockIdx.x * VEC_WARPS + (threadIdx.x >> 5);
+    const int t = (int)(job / per_token), h0 = (int)(job % per_token) * HEADS * each + sub;
+    if (t >= A.tokens) return;
+    const bool active = li * 8 < d;
+    const int c0 = active ? li * 8 : 0, groups = xb4::groups_of(d);
+    const T* row = static_cast<const T*>(A.qkv) + t * A.row_stride + c0;
+    float next[8];
+    if (h0 < heads) load8(row + (long long)h0 * d, next);
+    const long long slot = A.slots[t];
+    const bool kept = slot >= 0 && slot < A.num_slots;
+    const int place = kept ? (int)(slot % A.page_size) : 0;
+    const long long page_bytes = (long long)A.page_size * xb4::row_bytes(d), page = kept ? slot / A.page_size * A.nkv * page_bytes : 0;
+    // the token's angles: of the vector's pair in the other half, or of its own four pairs
+    const int half = A.rot / 16;                   // vectors of a half
+    const bool turns = A.cos_t && active && c0 < A.rot, upper = turns && !A.interleaved && li >= half;
+    float cs[8], sn[8];
+    if (A.cos_t) {
+        const int at = A.positions[t];
+        if (lane == 0 && slot >= 0 && (at < 0 || at >= A.max_pos)) atomicOr(A.err, XB_ERR_BAD_POSITION);
+        const long long from = (long long)min(max(at, 0), A.max_pos - 1) * (A.rot / 2) + (!turns ? 0 : (A.interleaved ? c0 / 2 : (upper ? c0 - half * 8 : c0)));
+        const float4 a = *reinterpret_cast<const float4*>(A.cos_t + from), b = *reinterpret_cast<const float4*>(A.sin_t + from);
+        cs[0] = a.x, cs[1] = a.y, cs[2] = a.z, cs[3] = a.w, sn[0] = b.x, sn[1] = b.y, sn[2] = b.z, sn[3] = b.w;
+        if (!A.interleaved) {
+            const float4 e = *reinterpret_cast<const float4*>(A.cos_t + from + 4), f = *reinterpret_cast<const float4*>(A.sin_t + from + 4);
+            cs[4] = e.x, cs[5] = e.y, cs[6] = e.z, cs[7] = e.w, sn[4] = f.x, sn[5] = f.y, sn[6] = f.z, sn[7] = f.w;
+        }
+    }
+    if (lane == 0 && slot >= A.num_slots) atomicOr(A.err, XB_ERR_BAD_PAGE);
+#pragma unroll 1
+    for (int i = 0; i < each; ++i) {
+        const int h = h0 + i * HEADS;
+        const bool there = h < heads, is_q = h < A.nh, is_k = !is_q && h < A.nh + A.nkv;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = there && active ? next[e] : 0.f;
+        if (i + 1 < each && h + HEADS < heads) load8(row + (long long)(h + HEADS) * d, next);
+        const float* w = is_q ? A.q_w : (is_k ? A.k_w : nullptr);
+        if (A.q_w || A.k_w) {                      // (the lanes of a warp sum together, whatever their heads are)
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+#pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, LPH);
+            if (w) {
+                const float inv = rsqrtf(ss / (float)d + A.eps);
+                float wv[8];
+                load8(w + c0, wv);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * wv[e];
+            }
+        }
+        if (A.cos_t) {
+            const bool turn = turns && (is_q || is_k);
+            if (A.interleaved) {
+                if (turn) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x0 = v[2 * e], x1 = v[2 * e + 1];
+                        v[2 * e] = x0 * cs[e] - x1 * sn[e];
+                        v[2 * e + 1] = x0 * sn[e] + x1 * cs[e];
+                    }
+                }
+            } else {
+                const int other = (lane & ~(LPH - 1)) + (!turns ? li : (upper ? li - half : li + half));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = __shfl_sync(0xffffffffu, v[e], other);
+                    if (turn) v[e] = upper ? x * sn[e] + v[e] * cs[e] : v[e] * cs[e] - x * sn[e];
+                }
+            }
+        }
+        if (is_q) {
+            if (there && active) store8(static_cast<T*>(A.q_out) + ((long long)t * A.nh + h) * d + c0, v);
+        }
+        if (__all_sync(0xffffffffu, is_q || !there)) continue;
+        const int g = is_k ? h - A.nh : h - A.nh - A.nkv;
+        float lo = active ? v[0] : INFINITY, hi = active ? v[0] : -INFINITY;       // (a last group may be shorter)
+#pragma unroll
+        for (int e = 1; e < 8; ++e) lo = active ? xb4::min_nan(lo, v[e]) : lo, hi = active ? xb4::max_nan(hi, v[e]) : hi;
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            lo = xb4::min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = xb4::max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const bool mine = there && !is_q;
+        if (mine && li < 4 * groups) {
+            const uint32_t word = xb4::word_of(lo, hi);
+            const float s = xb4::scale_of(word), m = xb4::least_of(word), inv = 1.f / s;
+            uint32_t codes = 0;
+            float c[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                // The quotient by a reciprocal is off by at most 3 units of 2^-24; next to a half it is formed again, correctly rounded.
+                float q = (v[e] - m) * inv;
+                c[e] = rintf(q);
+                if (fabsf(fabsf(q - c[e]) - 0.5f) < 1e-5f) c[e] = rintf((v[e] - m) / s);
+                c[e] = s > 0.f ? fminf(fmaxf(c[e], 0.f), 15.f) : 0.f;
+                codes |= (uint32_t)c[e] << (4 * e);
+            }
+            __nv_bfloat16* values = is_k ? A.k_values : A.v_values;
+            if (values && active) {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = fmaf(s, c[e], m);
+                store8(values + ((long long)t * A.nkv + g) * d + c0, y);
+            }
+            if (kept) {
+                uint8_t* to = (is_k ? A.k_cache : A.v_cache) + page + g * page_bytes;
+                reinterpret_cast<uint32_t*>(to + ((long long)(li >> 2) * A.page_size + place) * xb4::GROUP_BYTES)[li & 3] = active ? codes : 0u;
+                if ((li & 3) == 0) reinterpret_cast<uint32_t*>(to + (long long)groups * A.page_size * xb4::GROUP_BYTES)[place * groups + (li >> 2)] = word;
+            }
+        }
+    }
+}
+
+template <typename T, int LPH>
+int launch_vec(const WriteArgs& A, cudaStream_t stream) {
+    // as many heads a warp as leave every processor 32 warps
+    const int heads = A.nh + 2 * A.nkv, together = 32 / LPH;
+    int each = 1;
+    while (each < 8 && (long long)A.tokens * heads / (together * each * 2) >= 148 * 32) each *= 2;
+    const long long jobs = (long long)A.tokens * ((heads + together * each - 1) / (together * each));
+    return xb_launch_few(cache4_write_kernel<T, LPH>, dim3((unsigned)((jobs + VEC_WARPS - 1) / VEC_WARPS)), dim3(VEC_WARPS * 32), 0, stream, A, each);
+}
+
+template <typename T>
+bool vec_takes(const WriteArgs& A) {
+    auto on16 = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
+    return A.d % 8 == 0 && A.d <= 256 && A.row_stride * sizeof(T) % 16 == 0 && on16(A.qkv) && on16(A.q_out) && on16(A.q_w) && on16(A.k_w) && on16(A.k_values) && on16(A.v_values) &&
+           on16(A.cos_t) && on16(A.sin_t) && (!A.cos_t || A.rot % (A.interleaved ? 8 : 16) == 0);
+}
+
+template <typename T>
+int launch(const WriteArgs& A, cudaStream_t stream) {
+    if (vec_takes<T>(A)) {
+        if (A.d <= 32) return launch_vec<T, 4>(A, stream);
+        if (A.d <= 64) return launch_vec<T, 8>(A, stream);
+        return A.d <= 128 ? launch_vec<T, 16>(A, stream) : launch_vec<T, 32>(A, stream);
+    }
     const long long jobs = (long long)A.tokens * (A.nh + 2 * A.nkv);
     return xb_launch_few(cache4_write_any_kernel<T>, dim3((unsigned)((jobs + ANY_WARPS - 1) / ANY_WARPS)), dim3(ANY_WARPS * 32), 0, stream, A);
 }
@@ -124,6 +299,6 @@ static int cache4_write(int dtype, void* q_out, uint8_t* k_cache, uint8_t* v_cac
     if ((long long)tokens * (nh + 2 * nkv) > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     const WriteArgs A{q_out, k_cache, v_cache, qkv, q_w, k_w, rot ? cos_t : nullptr, sin_t, positions, slots, k_values, v_values, row_stride, num_slots, tokens, nh, nkv,
                       d, rot, interleaved, page_size, max_pos, eps, err};
-    return dtype == XB_F32 ? launch_any<float>(A, stream) : launch_any<__nv_bfloat16>(A, stream);
+    return dtype == XB_F32 ? launch<float>(A, stream) : launch<__nv_bfloat16>(A, stream);
 }
 XB_EXPORT int xb_cache4_write(const long long* words, int n) { return xb_by_words(cache4_write, words, n); }
