@@ -96,7 +96,9 @@ cache4_write_any_kernel(const WriteArgs A) {
             lo = xb4::min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
             hi = xb4::max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
-        const uint32_t word = xb4::word_of(lo, hi), code = xb4::code_of(v, word);
+        const uint32_t word = xb4::word_of(lo, hi);
+        const float s = xb4::scale_of(word);
+        const uint32_t code = (uint32_t)xb4::code_of(v, s, xb4::least_of(word), xb4::reciprocal(s));
         if (values && c < d) values[c] = __float2bfloat16_rn(xb4::value_of(code, word));
         uint32_t eight = code << (4 * (lane & 7));
 #pragma unroll
@@ -173,6 +175,9 @@ cache4_write_kernel(const WriteArgs A, int each) {
         }
     }
     if (lane == 0 && slot >= A.num_slots) atomicOr(A.err, XB_ERR_BAD_PAGE);
+    const float* had = nullptr;                    // the norm's weights that the lane holds
+    float wv[8];
+    const float one_over_d = 1.f / (float)d;
 #pragma unroll 1
     for (int i = 0; i < each; ++i) {
         const int h = h0 + i * HEADS;
@@ -181,17 +186,17 @@ cache4_write_kernel(const WriteArgs A, int each) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = there && active ? next[e] : 0.f;
         if (i + 1 < each && h + HEADS < heads) load8(row + (long long)(h + HEADS) * d, next);
-        const float* w = is_q ? A.q_w : (is_k ? A.k_w : nullptr);
         if (A.q_w || A.k_w) {                      // (the lanes of a warp sum together, whatever their heads are)
+            const float* w = is_q ? A.q_w : (is_k ? A.k_w : nullptr);
+            if (w && w != had) load8(w + c0, wv);
+            had = w;
             float ss = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
 #pragma unroll
             for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, LPH);
             if (w) {
-                const float inv = rsqrtf(ss / (float)d + A.eps);
-                float wv[8];
-                load8(w + c0, wv);
+                const float inv = rsqrtf(ss * one_over_d + A.eps);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * wv[e];
             }
@@ -221,9 +226,10 @@ cache4_write_kernel(const WriteArgs A, int each) {
         }
         if (__all_sync(0xffffffffu, is_q || !there)) continue;
         const int g = is_k ? h - A.nh : h - A.nh - A.nkv;
-        float lo = active ? v[0] : INFINITY, hi = active ? v[0] : -INFINITY;       // (a last group may be shorter)
+        float lo = v[0], hi = v[0];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) lo = active ? xb4::min_nan(lo, v[e]) : lo, hi = active ? xb4::max_nan(hi, v[e]) : hi;
+        for (int e = 1; e < 8; ++e) lo = xb4::min_nan(lo, v[e]), hi = xb4::max_nan(hi, v[e]);
+        if (!active) lo = INFINITY, hi = -INFINITY;        // (a last group may be shorter)
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) {
             lo = xb4::min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
@@ -232,16 +238,12 @@ cache4_write_kernel(const WriteArgs A, int each) {
         const bool mine = there && !is_q;
         if (mine && li < 4 * groups) {
             const uint32_t word = xb4::word_of(lo, hi);
-            const float s = xb4::scale_of(word), m = xb4::least_of(word), inv = 1.f / s;
+            const float s = xb4::scale_of(word), m = xb4::least_of(word), inv = xb4::reciprocal(s);
             uint32_t codes = 0;
             float c[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                // The quotient by a reciprocal is off by at most 3 units of 2^-24; next to a half it is formed again, correctly rounded.
-                float q = (v[e] - m) * inv;
-                c[e] = rintf(q);
-                if (fabsf(fabsf(q - c[e]) - 0.5f) < 1e-5f) c[e] = rintf((v[e] - m) / s);
-                c[e] = s > 0.f ? fminf(fmaxf(c[e], 0.f), 15.f) : 0.f;
+                c[e] = xb4::code_of(v[e], s, m, inv);
                 codes |= (uint32_t)c[e] << (4 * e);
             }
             __nv_bfloat16* values = is_k ? A.k_values : A.v_values;

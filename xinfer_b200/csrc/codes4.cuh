@@ -35,16 +35,29 @@ __device__ __forceinline__ float min_nan(float a, float b) {
     return d;
 }
 
+// a / b by a reciprocal of b and one step of correction (Markstein: the remainder a - q b is exact, so what it adds rounds the quotient
+// correctly): halves of whole numbers come out exactly.  `inv` may be off by a unit of its last place.
+__device__ __forceinline__ float corrected(float a, float b, float inv) {
+    const float q = a * inv;
+    return fmaf(fmaf(-q, b, a), inv, q);
+}
+__device__ __forceinline__ float reciprocal(float s) {
+    float r;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
+    return r;
+}
+
 // The group's word from its least and largest number.
 __device__ __forceinline__ uint32_t word_of(float lo, float hi) {
-    const __nv_bfloat16 s = __float2bfloat16_rn((hi - lo) / 15.f), m = __float2bfloat16_rn(lo);
+    const __nv_bfloat16 s = __float2bfloat16_rn(corrected(hi - lo, 15.f, 1.f / 15.f)), m = __float2bfloat16_rn(lo);
     const uint32_t su = __bfloat16_as_ushort(s), mu = __bfloat16_as_ushort(m);
     return (su & 0x7f80u) == 0x7f80u || (mu & 0x7f80u) == 0x7f80u ? 0x7fff7fffu : su | (mu << 16);
 }
-// A number's code in a group with that word.  The quotient is rounded correctly: bfloat16 numbers have the codes that the formula gives.
-__device__ __forceinline__ uint32_t code_of(float x, uint32_t word) {
-    const float s = scale_of(word), c = rintf((x - least_of(word)) / s);
-    return s > 0.f ? (uint32_t)fminf(fmaxf(c, 0.f), 15.f) : 0u;
+// A number's code in a group of that scale and least value, as a whole float32 number; `inv` is the scale's reciprocal.  Where the scale is zero or no
+// number the quotient is no number, or none that counts, and the code is zero.
+__device__ __forceinline__ float code_of(float x, float s, float m, float inv) {
+    const float q = fminf(fmaxf(corrected(x - m, s, inv), 0.f), 15.f);
+    return (q + 12582912.f) - 12582912.f;          // 1.5 * 2^23: rounded to a whole number, halves to even
 }
 __device__ __forceinline__ float value_of(uint32_t code, uint32_t word) { return fmaf(scale_of(word), (float)code, least_of(word)); }
 
