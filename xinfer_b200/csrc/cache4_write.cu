@@ -140,92 +140,113 @@ __device__ __forceinline__ void store8(T* x, const float (&v)[8]) {
     }
 }
 
-template <typename T, int LPH>
-__global__ void __launch_bounds__(VEC_WARPS * 32)
+constexpr int TURN_NONE = 0, TURN_HALVES = 1, TURN_PAIRS = 2;
+
+template <typename T, int LPH, int TURN>
+__global__ void __launch_bounds__(VEC_WARPS * 32, 4)
 cache4_write_kernel(const WriteArgs A, int each) {
     constexpr int HEADS = 32 / LPH;
     pdl_overlap_few();
-    const int lane = threadIdx.x & 31, li = lane & (LPH - 1), sub = lane / LPH, heads = A.nh + 2 * A.nkv, d = A.d;
-    const int per_token = (heads + HEADS * each - 1) / (HEADS * each);
-    const long long job = (long long)blockIdx.x * VEC_WARPS + (threadIdx.x >> 5);
-    const int t = (int)(job / per_token), h0 = (int)(job % per_token) * HEADS * each + sub;
+    const int lane = threadIdx.x & 31, li = lane & (LPH - 1), sub = lane / LPH, d = A.d;
+    // a token's jobs: some for its query heads, then some for its keys and values
+    const int q_jobs = (A.nh + HEADS * each - 1) / (HEADS * each), kv_jobs = (2 * A.nkv + HEADS * each - 1) / (HEADS * each);
+    const unsigned job = blockIdx.x * VEC_WARPS + (threadIdx.x >> 5);
+    const int t = (int)(job / (unsigned)(q_jobs + kv_jobs)), of_token = (int)(job % (unsigned)(q_jobs + kv_jobs));
     if (t >= A.tokens) return;
-    const bool active = li * 8 < d;
+    const bool is_q = of_token < q_jobs, active = li * 8 < d;
+    const int count = is_q ? A.nh : 2 * A.nkv, h0 = (is_q ? of_token : of_token - q_jobs) * HEADS * each + sub;
     const int c0 = active ? li * 8 : 0, groups = xb4::groups_of(d);
-    const T* row = static_cast<const T*>(A.qkv) + t * A.row_stride + c0;
+    const T* heads = static_cast<const T*>(A.qkv) + t * A.row_stride + c0 + (is_q ? 0 : (long long)A.nh * d);
+    const int steps = min(each, (count - (h0 - sub) + HEADS - 1) / HEADS);
     float next[8];
-    if (h0 < heads) load8(row + (long long)h0 * d, next);
-    const long long slot = A.slots[t];
-    const bool kept = slot >= 0 && slot < A.num_slots;
-    const int place = kept ? (int)(slot % A.page_size) : 0;
-    const long long page_bytes = (long long)A.page_size * xb4::row_bytes(d), page = kept ? slot / A.page_size * A.nkv * page_bytes : 0;
-    // the token's angles: of the vector's pair in the other half, or of its own four pairs
+    load8(heads + min(h0, count - 1) * d, next);
+    // the token's angles: of the vector's pair in the other half (the sine with its sign), or of its own four pairs
     const int half = A.rot / 16;                   // vectors of a half
-    const bool turns = A.cos_t && active && c0 < A.rot, upper = turns && !A.interleaved && li >= half;
-    float cs[8], sn[8];
-    if (A.cos_t) {
+    const bool turns = TURN != TURN_NONE && active && c0 < A.rot, upper = TURN == TURN_HALVES && li >= half;
+    const int other = (lane & ~(LPH - 1)) + (!turns ? li : (upper ? li - half : li + half));
+    float cs[TURN == TURN_PAIRS ? 4 : 8], sn[TURN == TURN_PAIRS ? 4 : 8];
+    const long long slot = A.slots[t];
+    if constexpr (TURN != TURN_NONE) {
         const int at = A.positions[t];
         if (lane == 0 && slot >= 0 && (at < 0 || at >= A.max_pos)) atomicOr(A.err, XB_ERR_BAD_POSITION);
-        const long long from = (long long)min(max(at, 0), A.max_pos - 1) * (A.rot / 2) + (!turns ? 0 : (A.interleaved ? c0 / 2 : (upper ? c0 - half * 8 : c0)));
-        const float4 a = *reinterpret_cast<const float4*>(A.cos_t + from), b = *reinterpret_cast<const float4*>(A.sin_t + from);
-        cs[0] = a.x, cs[1] = a.y, cs[2] = a.z, cs[3] = a.w, sn[0] = b.x, sn[1] = b.y, sn[2] = b.z, sn[3] = b.w;
-        if (!A.interleaved) {
-            const float4 e = *reinterpret_cast<const float4*>(A.cos_t + from + 4), f = *reinterpret_cast<const float4*>(A.sin_t + from + 4);
-            cs[4] = e.x, cs[5] = e.y, cs[6] = e.z, cs[7] = e.w, sn[4] = f.x, sn[5] = f.y, sn[6] = f.z, sn[7] = f.w;
+        const long long from = (long long)min(max(at, 0), A.max_pos - 1) * (A.rot / 2) + (!turns ? 0 : (TURN == TURN_PAIRS ? c0 / 2 : (upper ? c0 - half * 8 : c0)));
+        if constexpr (TURN == TURN_PAIRS) {
+            const float4 a = *reinterpret_cast<const float4*>(A.cos_t + from), b = *reinterpret_cast<const float4*>(A.sin_t + from);
+            cs[0] = a.x, cs[1] = a.y, cs[2] = a.z, cs[3] = a.w, sn[0] = b.x, sn[1] = b.y, sn[2] = b.z, sn[3] = b.w;
+        } else {
+            load8(A.cos_t + from, cs);
+            load8(A.sin_t + from, sn);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sn[e] = upper ? sn[e] : -sn[e];
         }
     }
-    if (lane == 0 && slot >= A.num_slots) atomicOr(A.err, XB_ERR_BAD_PAGE);
-    const float* had = nullptr;                    // the norm's weights that the lane holds
+    const float* w = is_q ? A.q_w : A.k_w;
     float wv[8];
+    if (w) load8(w + c0, wv);
     const float one_over_d = 1.f / (float)d;
-#pragma unroll 1
-    for (int i = 0; i < each; ++i) {
-        const int h = h0 + i * HEADS;
-        const bool there = h < heads, is_q = h < A.nh, is_k = !is_q && h < A.nh + A.nkv;
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = there && active ? next[e] : 0.f;
-        if (i + 1 < each && h + HEADS < heads) load8(row + (long long)(h + HEADS) * d, next);
-        if (A.q_w || A.k_w) {                      // (the lanes of a warp sum together, whatever their heads are)
-            const float* w = is_q ? A.q_w : (is_k ? A.k_w : nullptr);
-            if (w && w != had) load8(w + c0, wv);
-            had = w;
+    // norm and rotation of a lane's channels (`wanted`: whether this head is normed and turned; the lanes of a warp exchange all the same)
+    auto prepare = [&](float (&v)[8], bool wanted) {
+        if (w) {
             float ss = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+            for (int e = 0; e < 8; ++e) ss += active ? v[e] * v[e] : 0.f;
 #pragma unroll
             for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, LPH);
-            if (w) {
-                const float inv = rsqrtf(ss * one_over_d + A.eps);
+            const float inv = rsqrtf(ss * one_over_d + A.eps);
+            if (wanted) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * wv[e];
             }
         }
-        if (A.cos_t) {
-            const bool turn = turns && (is_q || is_k);
-            if (A.interleaved) {
-                if (turn) {
+        if constexpr (TURN == TURN_PAIRS) {
+            if (turns && wanted) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x0 = v[2 * e], x1 = v[2 * e + 1];
-                        v[2 * e] = x0 * cs[e] - x1 * sn[e];
-                        v[2 * e + 1] = x0 * sn[e] + x1 * cs[e];
-                    }
-                }
-            } else {
-                const int other = (lane & ~(LPH - 1)) + (!turns ? li : (upper ? li - half : li + half));
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float x = __shfl_sync(0xffffffffu, v[e], other);
-                    if (turn) v[e] = upper ? x * sn[e] + v[e] * cs[e] : v[e] * cs[e] - x * sn[e];
+                for (int e = 0; e < 4; ++e) {
+                    const float x0 = v[2 * e], x1 = v[2 * e + 1];
+                    v[2 * e] = x0 * cs[e] - x1 * sn[e];
+                    v[2 * e + 1] = x0 * sn[e] + x1 * cs[e];
                 }
             }
+        } else if constexpr (TURN == TURN_HALVES) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __shfl_sync(0xffffffffu, v[e], other);
+            if (turns && wanted) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = fmaf(x[e], sn[e], v[e] * cs[e]);
+            }
         }
-        if (is_q) {
-            if (there && active) store8(static_cast<T*>(A.q_out) + ((long long)t * A.nh + h) * d + c0, v);
+    };
+    if (is_q) {
+        T* out = static_cast<T*>(A.q_out) + (long long)t * A.nh * d + c0;
+#pragma unroll 2
+        for (int i = 0; i < steps; ++i) {
+            const int h = h0 + i * HEADS;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = next[e];
+            load8(heads + min(h + HEADS, count - 1) * d, next);
+            prepare(v, true);
+            if (h < count && active) store8(out + h * d, v);
         }
-        if (__all_sync(0xffffffffu, is_q || !there)) continue;
-        const int g = is_k ? h - A.nh : h - A.nh - A.nkv;
+        return;
+    }
+    if (lane == 0 && slot >= A.num_slots) atomicOr(A.err, XB_ERR_BAD_PAGE);
+    const bool kept = slot >= 0 && slot < A.num_slots;
+    const int place = kept ? (int)(slot % A.page_size) : 0;
+    const long long page_bytes = (long long)A.page_size * xb4::row_bytes(d), page = kept ? slot / A.page_size * A.nkv * page_bytes : 0;
+    // where the lane's eight codes and its group's word go in a page; a lane behind the head writes the codes that fill its last group
+    const int code_at = (int)((long long)(li >> 2) * A.page_size + place) * xb4::GROUP_BYTES + (li & 3) * 4, word_at = groups * A.page_size * xb4::GROUP_BYTES + (place * groups + (li >> 2)) * 4;
+    const bool writes = kept && li < 4 * groups;
+#pragma unroll 1
+    for (int i = 0; i < steps; ++i) {
+        const int h = h0 + i * HEADS;
+        const bool is_k = h < A.nkv;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = next[e];
+        load8(heads + min(h + HEADS, count - 1) * d, next);
+        prepare(v, is_k);
         float lo = v[0], hi = v[0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) lo = xb4::min_nan(lo, v[e]), hi = xb4::max_nan(hi, v[e]);
@@ -235,47 +256,41 @@ cache4_write_kernel(const WriteArgs A, int each) {
             lo = xb4::min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
             hi = xb4::max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
-        const bool mine = there && !is_q;
-        if (mine && li < 4 * groups) {
-            const uint32_t word = xb4::word_of(lo, hi);
-            const float s = xb4::scale_of(word), m = xb4::least_of(word), inv = xb4::reciprocal(s);
-            uint32_t codes = 0;
-            float c[8];
+        const uint32_t word = xb4::word_of(lo, hi);
+        const float s = xb4::scale_of(word), m = xb4::least_of(word), inv = xb4::reciprocal(s);
+        uint32_t codes = 0;
+        float y[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                c[e] = xb4::code_of(v[e], s, m, inv);
-                codes |= (uint32_t)c[e] << (4 * e);
-            }
-            __nv_bfloat16* values = is_k ? A.k_values : A.v_values;
-            if (values && active) {
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = fmaf(s, c[e], m);
-                store8(values + ((long long)t * A.nkv + g) * d + c0, y);
-            }
-            if (kept) {
-                uint8_t* to = (is_k ? A.k_cache : A.v_cache) + page + g * page_bytes;
-                reinterpret_cast<uint32_t*>(to + ((long long)(li >> 2) * A.page_size + place) * xb4::GROUP_BYTES)[li & 3] = active ? codes : 0u;
-                if ((li & 3) == 0) reinterpret_cast<uint32_t*>(to + (long long)groups * A.page_size * xb4::GROUP_BYTES)[place * groups + (li >> 2)] = word;
-            }
+        for (int e = 0; e < 8; ++e) {
+            const float c = xb4::code_of(v[e], s, m, inv);
+            codes |= (uint32_t)c << (4 * e);
+            y[e] = fmaf(s, c, m);
         }
+        if (h >= count) continue;
+        const int g = is_k ? h : h - A.nkv;
+        __nv_bfloat16* values = is_k ? A.k_values : A.v_values;
+        if (values && active) store8(values + ((long long)t * A.nkv + g) * d + c0, y);
+        uint8_t* to = (is_k ? A.k_cache : A.v_cache) + page + g * page_bytes;
+        if (writes) *reinterpret_cast<uint32_t*>(to + code_at) = active ? codes : 0u;
+        if (writes && (li & 3) == 0) *reinterpret_cast<uint32_t*>(to + word_at) = word;
     }
 }
 
 template <typename T, int LPH>
 int launch_vec(const WriteArgs& A, cudaStream_t stream) {
     // as many heads a warp as leave every processor 32 warps
-    const int heads = A.nh + 2 * A.nkv, together = 32 / LPH;
+    const int together = 32 / LPH;
     int each = 1;
-    while (each < 8 && (long long)A.tokens * heads / (together * each * 2) >= 148 * 32) each *= 2;
-    const long long jobs = (long long)A.tokens * ((heads + together * each - 1) / (together * each));
-    return xb_launch_few(cache4_write_kernel<T, LPH>, dim3((unsigned)((jobs + VEC_WARPS - 1) / VEC_WARPS)), dim3(VEC_WARPS * 32), 0, stream, A, each);
+    while (each < 8 && (long long)A.tokens * (A.nh + 2 * A.nkv) / (together * each * 2) >= 148 * 32) each *= 2;
+    const long long jobs = (long long)A.tokens * ((A.nh + together * each - 1) / (together * each) + (2 * A.nkv + together * each - 1) / (together * each));
+    auto go = [&](auto kernel) { return xb_launch_few(kernel, dim3((unsigned)((jobs + VEC_WARPS - 1) / VEC_WARPS)), dim3(VEC_WARPS * 32), 0, stream, A, each); };
+    return !A.cos_t ? go(cache4_write_kernel<T, LPH, TURN_NONE>) : (A.interleaved ? go(cache4_write_kernel<T, LPH, TURN_PAIRS>) : go(cache4_write_kernel<T, LPH, TURN_HALVES>));
 }
 
 template <typename T>
 bool vec_takes(const WriteArgs& A) {
     auto on16 = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
-    return A.d % 8 == 0 && A.d <= 256 && A.row_stride * sizeof(T) % 16 == 0 && on16(A.qkv) && on16(A.q_out) && on16(A.q_w) && on16(A.k_w) && on16(A.k_values) && on16(A.v_values) &&
+    return A.d % 8 == 0 && A.d <= 256 && (long long)A.page_size * xb4::row_bytes(A.d) < 0x7fffffffLL && A.row_stride * sizeof(T) % 16 == 0 && on16(A.qkv) && on16(A.q_out) && on16(A.q_w) && on16(A.k_w) && on16(A.k_values) && on16(A.v_values) &&
            on16(A.cos_t) && on16(A.sin_t) && (!A.cos_t || A.rot % (A.interleaved ? 8 : 16) == 0);
 }
 
