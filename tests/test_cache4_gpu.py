@@ -265,6 +265,8 @@ class Attend:
                     allowed = HALF[self.dtype] * np.abs(want) + (2 * (d + 16) * 2.0 ** -23 * steps + (64 + seen.sum() / 16) * 2.0 ** -23) * size
                     if self.dtype == BF:       # the probabilities' rounding, by themselves and times a group's scale, for both parts of m + s code
                         allowed = allowed + 2 * 2.0 ** -8 * (p @ parts[page, :, j % self.ps][seen, g])
+                        if n * (nh // nkv) >= 64:      # many rows: keys are rounded to float16 (2^-11 of themselves, in every product of a score), values to bfloat16
+                            allowed = allowed + (2 * 2.0 ** -11 * min(1.0, float((p * (np.abs(kk) @ np.abs(q[t, h]))).sum() * abs(self.scale))) + 2.0 ** -8) * size
                     off = np.abs(got[t, h] - want)
                     assert np.all(off <= allowed), (b, i, h, (off / allowed).max())
         assert np.all(got[self.start[-1]:] == 9)               # rows behind the last request
@@ -387,7 +389,7 @@ def test_what_is_not_seen_does_not_matter(d, ps, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("longest", [1, 3])
+@pytest.mark.parametrize("longest", [1, 3, 60])
 def test_graphs_and_streams(longest, dtype):
     from xinfer_b200 import kernels as k
     a, other = (Attend([1, longest, 1], c, 8, 2, 128, dtype, seed=3) for c in ([900, 33, 128], [5, 333, 600]))
@@ -426,6 +428,62 @@ def test_graphs_and_streams(longest, dtype):
         graph.replay()
         graph.replay()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("news,d,ps", [([1, 2], 128, 8), ([1, 100], 128, 8), ([1, 100], 64, 16), ([3, 70], 48, 5)])
+def test_pages_that_a_window_has_left_behind(news, d, ps, dtype):
+    """Their entries of the table are gone: nobody reads them and nothing is reported."""
+    a = Attend(news, [300, 333], 4, 2, d, dtype, ps=ps, window=37)
+    for b, length in enumerate(a.lengths):
+        a.table[b, :max(0, length - news[b] - 37 + 1) // ps] = -1
+    good = a.table.copy()
+    a.run()
+    a.table = np.maximum(good, 0)
+    a.check()
+
+
+@pytest.mark.parametrize("news,contexts,nh,nkv,d,window", [([200], [0], 4, 1, 128, None), ([64, 300], [700, 90], 8, 2, 128, None), ([130, 1, 70, 0, 2], [65, 500, 3, 8, 1000], 6, 2, 96, None),
+                                                           ([90], [1000], 8, 8, 64, 100), ([257, 65], [31, 64], 3, 1, 32, 300), ([100, 5], [128, 900], 5, 1, 80, 77), ([80], [50], 2, 1, 256, None),
+                                                           ([500] * 3, [3000, 10, 600], 16, 8, 48, None)])
+@pytest.mark.parametrize("ps", [16, 4, 24])
+def test_portions_of_prompts(news, contexts, nh, nkv, d, window, ps):
+    a = Attend(news, contexts, nh, nkv, d, BF, ps=ps, window=window)
+    a.run()
+    a.check()
+
+
+@pytest.mark.parametrize("d,ps,window", [(128, 16, 40), (64, 8, None), (96, 16, 200)])
+def test_portions_do_not_meet_what_they_do_not_see(d, ps, window):
+    """As above for tokens of a portion: a key of NaN reaches its own token and those behind it, a value's group of NaN its channels there."""
+    a = Attend([150, 3], [200, 45], 4, 2, d, BF, ps=ps, window=window)
+    want = a.run().clone()
+    groups = -(-d // 32)
+    words = [data[..., groups * ps * 16:].reshape(a.pages, 2, ps, groups, 4) for data in a.data]
+    for w in words:                              # behind the end
+        for b, length in enumerate(a.lengths):
+            for j in range(length, -(-length // ps) * ps):
+                w[a.table[b, j // ps], :, j % ps] = 0xFF
+    assert torch.equal(a.run(), want)
+    j = 310                                      # token 110 of the first request
+    words[1][a.table[0, j // ps], 1, j % ps, 1] = 0xFF
+    got = a.run()
+    last = min(150, 110 + (window or 1000))
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[110:last, 2:, 32:64] = True
+    assert bool(torch.isnan(got[bad]).all()) and torch.equal(got[~bad], want[~bad])
+    words[1][a.table[0, j // ps], 1, j % ps, 1] = 0
+    words[0][a.table[0, j // ps], 0, j % ps] = 0xFF
+    got = a.run()
+    assert bool(torch.isnan(got[110:last, :2]).all()) and torch.equal(got[:110], want[:110]) and torch.equal(got[last:150, :2], want[last:150, :2])
+    assert torch.equal(got[150:], want[150:])
+
+
+@pytest.mark.parametrize("size", [1e-6, 1e-3, 1e3, 1e6])
+def test_magnitudes_of_portions(size):
+    a = Attend([100], [137], 8, 2, 128, BF, size=size, scale=0.1 / size)
+    a.run()
+    a.check()
 
 
 def test_refusals():

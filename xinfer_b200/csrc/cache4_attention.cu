@@ -2,6 +2,7 @@
 //   sum_j softmax_j(scale q . k_j) v_j   over the keys j up to its position, of these the last `window`; zeros if it sees none.
 // The step's own keys are in the cache already.  A page outside the pool is reported and its keys are not seen.
 #include "cache4_attention_mma.h"
+#include "cache4_attention_tc.h"
 
 namespace {
 
@@ -234,9 +235,21 @@ static int cache4_attention(int dtype, void* out, const void* q, const uint8_t* 
     if (tokens <= 0 || requests <= 0) return 0;
     if (requests > REQUESTS_MAX || d < 1 || d > DIM_MOST || nkv < 1 || nh < nkv || nh % nkv || page_size < 1) return (int)cudaErrorInvalidValue;
     if ((long long)table_stride * page_size > KEYS_MOST || (long long)tokens * nh > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-    const AttendArgs A{out, q, k_cache, v_cache, lengths, token_start, block_table, out_stride, q_stride, tokens, requests, table_stride, nh, nkv, d, page_size,
-                       num_pages, window, scale, err};
-    if (dtype == XB_BF16 && mma_takes(A)) return mma_launch(A, longest, scratch, stream);
+    AttendArgs A{out, q, k_cache, v_cache, lengths, token_start, block_table, out_stride, q_stride, tokens, requests, table_stride, nh, nkv, d, page_size,
+                       num_pages, window, 0, 0x7fffffff, scale, err};
+    if (dtype == XB_BF16 && tc_takes(A, longest)) {
+        // requests of few rows beside those of many have the kernel for few: 64 single tokens at up to 4,096 keys beside a portion of 512 (both forms read the lengths on the device)
+        const bool both = mma_takes(A);
+        if (both) {
+            A.rows_from = TC_ROWS;
+            const int rc = tc_launch(A, scratch, stream);
+            if (rc) return rc;
+            A.rows_from = 0, A.rows_to = TC_ROWS;
+            return mma_launch(A, TC_ROWS, scratch + tc_scratch(d), stream);
+        }
+        return tc_launch(A, scratch, stream);
+    }
+    if (dtype == XB_BF16 && mma_takes(A)) return mma_launch(A, (nh / nkv) * (long long)longest > TC_ROWS ? TC_ROWS : (nh / nkv) * longest, scratch, stream);
     return dtype == XB_F32 ? launch_any<float>(A, longest, scratch, stream) : launch_any<__nv_bfloat16>(A, longest, scratch, stream);
 }
 XB_EXPORT int xb_cache4_attention(const long long* words, int n) { return xb_by_words(cache4_attention, words, n); }
@@ -245,6 +258,9 @@ XB_EXPORT int xb_cache4_attention(const long long* words, int n) { return xb_by_
 XB_EXPORT long long xb_cache4_attention_scratch(int dtype, int tokens, int requests, int nh, int nkv, int d, int longest) {
     if (tokens <= 0 || requests <= 0 || nkv <= 0 || nh < nkv || d < 1) return 0;
     const AnyGrid g = any_grid(requests, nh, nkv, longest);
-    const long long any = g.splits == 1 ? 0 : (long long)g.splits * tokens * nh * (d + 2), mma = dtype == XB_BF16 && mma_takes(d) ? mma_scratch(nh, nkv, d, longest) : 0;
-    return any > mma ? any : mma;                      // (the pages are not known here: enough for either kernel)
+    // (pages and scale are not known here: enough for any of the kernels)
+    const long long any = g.splits == 1 ? 0 : (long long)g.splits * tokens * nh * (d + 2);
+    const bool tc = dtype == XB_BF16 && tc_takes(nh, nkv, d, longest);
+    const long long rows = (long long)(nh / nkv) * longest, few = dtype == XB_BF16 && mma_takes(d) ? mma_scratch(d, rows > TC_ROWS ? TC_ROWS : (int)rows) : 0, both = few + (tc ? tc_scratch(d) : 0);
+    return any > both ? any : both;
 }

@@ -14,6 +14,7 @@ struct AttendArgs {
     const int* block_table;        // [requests, table_stride]
     long long out_stride, q_stride;
     int tokens, requests, table_stride, nh, nkv, d, page_size, num_pages, window;
+    int rows_from, rows_to;        // requests of other numbers of rows (tokens times query heads of a key/value head) are another kernel's
     float scale;
     int* err;
 };
@@ -36,6 +37,8 @@ __device__ __forceinline__ Request request_of(const AttendArgs& A, int b) {
     if (len > most && r.nodes > 0) atomicOr(A.err, XB_ERR_BAD_PAGE);
     r.keys = len < 0 ? 0 : (int)(len > most ? most : len);
     r.first_pos = max(len, 0) - r.nodes;
+    const int rows = r.nodes * (A.nh / A.nkv);
+    if (rows < A.rows_from || rows >= A.rows_to) r.nodes = 0;
     return r;
 }
 // The first key that a token at `pos` sees.

@@ -234,7 +234,7 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
         // keys from `all0` on and below `all1` are seen by all rows
         const int all0 = first_seen(A, pos1), all1 = min(pos0 + 1, w.r.keys);
         // the segment's steps, of these the ones with keys that some row sees
-        const int seen0 = first_seen(A, pos0) / STEP, seen1 = (min(pos1 + 1, w.r.keys) + STEP - 1) / STEP;
+        const int first_key = first_seen(A, pos0), seen0 = first_key / STEP, seen1 = (min(pos1 + 1, w.r.keys) + STEP - 1) / STEP;
         const int from = max((w.tile0 + w.i0) * STAGE_STEPS, seen0), to = failed ? from : min((w.tile0 + w.i1) * STAGE_STEPS, seen1);
         const int* table = A.block_table + (long long)w.b * A.table_stride;
         const uint8_t* k_pages = A.k_cache + w.g * page_bytes;
@@ -250,7 +250,8 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
                 ids_from = at & ~31;
                 const int key = (from << 4) + ((ids_from + lane) << (4 - shift));
                 ids = -1;
-                if (key < to * STEP && key < w.r.keys) {
+                // (pieces in front of the first row's window: their pages may have been given back)
+                if (key < to * STEP && key < w.r.keys && key + (STEP >> shift) > first_key) {
                     ids = table[key / ps];
                     if (ids < 0 || ids >= A.num_pages) {
                         atomicOr(A.err, XB_ERR_BAD_PAGE);
@@ -688,11 +689,6 @@ auto by_form(int rows, int groups, F f) {
     }
 }
 
-int rows_of(int nh, int nkv, int longest) {
-    const long long r = (long long)(nh / nkv) * longest;
-    return r > 1 << 20 ? 1 << 20 : (int)r;
-}
-
 }  // namespace
 
 namespace xb4 {
@@ -703,12 +699,11 @@ bool mma_takes(const AttendArgs& A) {
     const double jobs = (double)A.nkv * ((double)A.tokens * (A.nh / A.nkv) / 8 + A.requests), tiles = (double)A.table_stride * A.page_size / KT + 2;
     return mma_takes(A.d) && A.page_size % 8 == 0 && A.num_pages > 0 && jobs * (tiles + COST_JOB) < 2147483648.0;
 }
-long long mma_scratch(int nh, int nkv, int d, int longest) {
-    return by_form(rows_of(nh, nkv, longest), groups_of(d), [](auto nt, auto ng) { return scratch_of<decltype(nt)::value, decltype(ng)::value>(); });
+long long mma_scratch(int d, int rows) {
+    return by_form(rows, groups_of(d), [](auto nt, auto ng) { return scratch_of<decltype(nt)::value, decltype(ng)::value>(); });
 }
-int mma_launch(const AttendArgs& A, int longest, float* scratch, cudaStream_t stream) {
-    return by_form(rows_of(A.nh, A.nkv, longest), groups_of(A.d),
-                   [&](auto nt, auto ng) { return launch<decltype(nt)::value, decltype(ng)::value>(A, scratch, stream); });
+int mma_launch(const AttendArgs& A, int rows, float* scratch, cudaStream_t stream) {
+    return by_form(rows, groups_of(A.d), [&](auto nt, auto ng) { return launch<decltype(nt)::value, decltype(ng)::value>(A, scratch, stream); });
 }
 
 }  // namespace xb4

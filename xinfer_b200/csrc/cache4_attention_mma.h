@@ -6,7 +6,8 @@ namespace xb4 {
 
 bool mma_takes(int d);                        // whether it has a form for such heads
 bool mma_takes(const AttendArgs& A);
-long long mma_scratch(int nh, int nkv, int d, int longest);        // float32 numbers, on a 16-byte boundary
-int mma_launch(const AttendArgs& A, int longest, float* scratch, cudaStream_t stream);
+// `rows`: of the request that has most, as far as it is known (64 of more)
+long long mma_scratch(int d, int rows);        // float32 numbers, on a 16-byte boundary
+int mma_launch(const AttendArgs& A, int rows, float* scratch, cudaStream_t stream);
 
 }  // namespace xb4

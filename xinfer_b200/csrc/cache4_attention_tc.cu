@@ -1,0 +1,769 @@
+// Attention over 4-bit pages for many rows of a key/value head (portions of prompts, bfloat16) on the 5th-generation tensor cores
+// (cache4_attention.cu says what is computed).
+//
+// A job is (request, key/value head, up to two tiles of 128 rows): the rows are (token, query head of the group) pairs.  Two warps take tiles of 64 keys
+// and values out of their codes, once for the 256 rows, into operands in shared memory (128-byte swizzle); S = Q K^T by warp 10, P = 2^(S - m) by a
+// thread per row in warps 0..3 and 4..7, in the tensor memory of S, O += P V by warp 11.
+//
+// Keys and queries are products of float16: 11 digits of m + s code, where bfloat16's 8 would move scores by as much as probabilities' rounding does
+// afterwards.  float16's range is made up for by powers of two: one per row of Q, one for every 32 keys of a tile, by which the scores are
+// multiplied back in float32.  Values and probabilities are bfloat16: a value is one multiply-add of the code's bits under a mask
+// (c 2^-133; 16 times that in the next four bits), 2^-69 times its size, which the result is multiplied back by.  Values' scales may be up to 2^60.
+// A group's word that is no number is zero in the operand; rows that see its key get no number in the group's channels at the end, the others nothing.
+//
+// The tiles of all jobs are one line cut into equal shares, one a block; parts of a job that blocks share are joined by a second kernel in their order.
+#include <cuda_fp16.h>
+
+#include "cache4_attention_tc.h"
+#include "tc_common.cuh"
+
+namespace {
+
+using namespace xb4;
+using namespace xbtc;
+
+constexpr int RT = 128, ROWS = 2 * RT, KT = 64;
+constexpr int BLOCKS = 148, THREADS = 384, NS = 3;
+constexpr int COST_JOB = 3;                // a job's start and end take about as long as three tiles
+constexpr float RESCALE_STEP = 8.f;
+constexpr int JOB_WORDS = 8, INFOS = 8;    // (a tile's facts are read at most NS + 2 tiles after they are written)
+constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
+constexpr uint32_t V_UP = 0x5f805f80u, V_UP16 = 0x5d805d80u, V_DOWN = 0x1d001d00u;     // bfloat16 2^64, 2^60, 2^-69, twice
+constexpr float BACK = 0x1p69f;
+
+struct Line {
+    float* part_o;                 // [blocks][2][256][DP]: a block's first segment, if its job began before it, and its last, if its job goes on
+    float* part_ml;                // [blocks][2][256][2]
+    int* jobs;                     // [blocks][2][8]: parts (0: there is no such part), block of the first, first row, rows, key/value head, request
+};
+
+// What the softmax needs to know of a tile of keys, and of its values.
+struct Info {
+    float f[2];                    // what the scores of the tile's halves are multiplied by
+    unsigned there[2];             // keys that lie in a page
+    unsigned odd[2];               // keys whose values have a group that is no number,
+    unsigned char groups[KT];      // and which groups
+};
+
+struct Walk {
+    Request r;
+    int b, g, piece, pieces;
+    int tile0, tiles;              // of the job
+    int job, from, end, share;
+    int i0, i1;
+};
+
+// First row, keys and tiles of a request's piece of rows.
+__device__ __forceinline__ void set_piece(const AttendArgs& A, Walk& w) {
+    const int group = A.nh / A.nkv, row0 = w.piece * ROWS, rows = min(ROWS, w.r.nodes * group - row0);
+    const int pos0 = w.r.first_pos + row0 / group, pos1 = w.r.first_pos + (row0 + rows - 1) / group;
+    w.tile0 = first_seen(A, pos0) / KT;
+    w.tiles = max(1, (min(pos1 + 1, w.r.keys) + KT - 1) / KT - w.tile0);       // (rows that see no key are written all the same)
+}
+__device__ __forceinline__ void set_request(const AttendArgs& A, Walk& w, int b) {
+    w.b = b;
+    w.r = request_of(A, b);
+    w.pieces = (w.r.nodes * (A.nh / A.nkv) + ROWS - 1) / ROWS;
+}
+__device__ __forceinline__ int head_units(const AttendArgs& A, Walk& w) {
+    int sum = 0;
+#pragma unroll 1
+    for (w.piece = 0; w.piece < w.pieces; ++w.piece) {
+        set_piece(A, w);
+        sum += w.tiles + COST_JOB;
+    }
+    return sum;
+}
+
+__device__ __forceinline__ bool place_in_line(const AttendArgs& A, Walk& w) {
+    const int lane = threadIdx.x & 31, each = (A.requests + 31) / 32, b0 = lane * each, b1 = min(b0 + each, A.requests);
+    int mine = 0;
+#pragma unroll 1
+    for (int b = b0; b < b1; ++b) {
+        set_request(A, w, b);
+        mine += A.nkv * head_units(A, w);
+    }
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    w.share = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+    w.from = (int)min((long long)blockIdx.x * w.share, (long long)total);
+    w.end = min(total, w.from + w.share);
+    if (w.from >= w.end) return false;
+    int before = incl - mine, b = b0;
+    const int owner = __ffs(__ballot_sync(0xffffffffu, w.from >= before && w.from < incl)) - 1;
+    if (lane == owner) {
+#pragma unroll 1
+        for (; b < b1; ++b) {
+            set_request(A, w, b);
+            const int n = A.nkv * head_units(A, w);
+            if (w.from < before + n) break;
+            before += n;
+        }
+    }
+    set_request(A, w, __shfl_sync(0xffffffffu, b, owner));
+    before = __shfl_sync(0xffffffffu, before, owner);
+    const int units = head_units(A, w);
+    w.g = (w.from - before) / units;
+    w.job = before + w.g * units;
+    for (w.piece = 0;; ++w.piece) {
+        set_piece(A, w);
+        if (w.from < w.job + w.tiles + COST_JOB) break;
+        w.job += w.tiles + COST_JOB;
+    }
+    return true;
+}
+
+// The next job of which the block has tiles: those that begin in its share.
+__device__ __forceinline__ bool next_segment(const AttendArgs& A, Walk& w, bool first) {
+    for (;; first = false) {
+        if (!first) {
+            w.job += w.tiles + COST_JOB;
+            if (w.job >= w.end) return false;
+            if (++w.piece == w.pieces) {
+                w.piece = 0;
+                if (++w.g == A.nkv) {
+                    w.g = 0;
+                    do {
+                        if (w.b + 1 >= A.requests) return false;
+                        set_request(A, w, w.b + 1);
+                    } while (w.pieces == 0);
+                }
+            }
+            set_piece(A, w);
+        }
+        w.i0 = max(0, w.from - w.job);
+        w.i1 = min(w.tiles, w.end - w.job);
+        if (w.i0 < w.i1) return true;
+    }
+}
+
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t e;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(e));
+    return e;
+}
+// Products issued by one lane of a warp that stays together.
+__device__ __forceinline__ void umma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "setp.ne.b32 q, %4, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(one) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t one, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(bar), "r"(one) : "memory");
+}
+// D float32, A and B float16, both K-major, M = 128, N = n
+__device__ __forceinline__ uint32_t idesc_f16(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int* err) { return mbar_wait(bar, parity, err); }
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* err) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return __all_sync(0xffffffffu, ok ? true : wait_long(bar, parity, err));
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t fma_bf16(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t fma_f16(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t add_f16(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ void store16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ bool half_not_finite(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }       // -126 <= e <= 127
+
+// A key's words.
+template <int NG>
+__device__ __forceinline__ void load_words(const uint8_t* at, uint32_t (&w)[NG]) {
+    if constexpr (NG == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(at);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+#pragma unroll
+        for (int n = 0; n < NG; ++n) w[n] = reinterpret_cast<const uint32_t*>(at)[n];
+    }
+}
+
+template <int NG>
+__global__ void __launch_bounds__(THREADS, 1)
+cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2) {
+    constexpr int DP = NG <= 2 ? 64 : 128, HALVES = DP / 64;
+    constexpr uint32_t Q_ONE = HALVES * RT * 128, KV_HALF = KT * 128, KV_BYTES = HALVES * KV_HALF, STAGE_BYTES = 2 * KV_BYTES;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long bars[4 * NS + 16];
+    __shared__ uint32_t s_tmem;
+    __shared__ Info infos[INFOS];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, q_sm = base, kv_sm = base + 2 * Q_ONE;
+    const uint32_t bar0 = smem_u32(bars), k_full0 = bar0, k_empty0 = bar0 + 8 * NS, v_full0 = bar0 + 16 * NS, v_empty0 = bar0 + 24 * NS, rest = bar0 + 32 * NS;
+    const uint32_t s_ready0 = rest, pv_done0 = rest + 32, p_ready0 = rest + 64, q_ready0 = rest + 96, drained0 = rest + 112;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = A.nh / A.nkv, ps = A.page_size;
+    int* const err = A.err;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 4 * NS; ++i) mbar_init(bar0 + 8 * i, 1);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(s_ready0 + 8 * i, 1);
+            mbar_init(pv_done0 + 8 * i, 1);
+            mbar_init(p_ready0 + 8 * i, 4);        // a warp each
+        }
+        for (int i = 0; i < 2; ++i) mbar_init(q_ready0 + 8 * i, 4), mbar_init(drained0 + 8 * i, 1);
+        mbar_init_fence();
+    }
+    if (warp == 11) tmem_alloc(&s_tmem, 512);
+    if (NG * 32 < DP)                              // channels that no group has: zeros for good (the products of Q and K go over them)
+        for (uint32_t i = threadIdx.x * 16; i < NS * STAGE_BYTES; i += THREADS * 16) store16(kv_sm + i, 0, 0, 0, 0);
+    fence_async_shared();
+    pdl_wait();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    pdl_launch_dependents();       // only now: see pdl_launch_dependents on tensor memory
+    if (threadIdx.x < 2) line.jobs[(blockIdx.x * 2 + threadIdx.x) * JOB_WORDS] = 0;
+    Walk w;
+    const bool any = place_in_line(A, w);
+    const long long page_bytes = (long long)ps * 20 * NG;
+
+    if (warp == 8 || warp == 9) {
+        // ---- codes to operands: warp 8 keys, warp 9 values; a lane has the keys `lane` and `lane + 32` of a tile
+        const bool is_v = warp == 9;
+        const uint32_t full0 = is_v ? v_full0 : k_full0, empty0 = is_v ? v_empty0 : k_empty0;
+        int st = 0, done = 0;
+        uint32_t ph = 0;
+        bool ok = any;
+        for (bool first = true; ok && next_segment(A, w, first); first = false) {
+            const int* table = A.block_table + (long long)w.b * A.table_stride;
+            const uint8_t* pages = (is_v ? A.v_cache : A.k_cache) + w.g * page_bytes;
+            const uint8_t* v_pages = A.v_cache + w.g * page_bytes;
+            const int first_key = first_seen(A, w.r.first_pos + w.piece * ROWS / group);       // (pages in front of it may have been given back)
+            // pages of a tile's keys two tiles ahead, codes and words one
+            auto page_of = [&](int it, int h) {
+                const int key = (w.tile0 + it) * KT + lane + 32 * h;
+                return it < w.i1 && key < w.r.keys && key >= first_key ? table[key / ps] : -1;
+            };
+            uint4 codes[2][NG];
+            uint32_t words[2][NG], beside[2][NG];
+            bool there[2];
+            auto fetch = [&](int it, const int (&ids)[2]) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int key = (w.tile0 + it) * KT + lane + 32 * h, slot = key % ps;
+                    there[h] = ids[h] >= 0 && ids[h] < A.num_pages;
+                    if (!there[h] && key < w.r.keys && key >= first_key) atomicOr(err, XB_ERR_BAD_PAGE);
+                    if (there[h]) {
+                        const long long page = (long long)ids[h] * A.nkv * page_bytes;
+#pragma unroll
+                        for (int n = 0; n < NG; ++n) codes[h][n] = *reinterpret_cast<const uint4*>(pages + page + ((long long)n * ps + slot) * 16);
+                        load_words<NG>(pages + page + (long long)ps * 16 * NG + slot * NG * 4, words[h]);
+                        if (!is_v) load_words<NG>(v_pages + page + (long long)ps * 16 * NG + slot * NG * 4, beside[h]);
+                    }
+                }
+            };
+            int ids[2] = {page_of(w.i0, 0), page_of(w.i0, 1)};
+            fetch(w.i0, ids);
+            ids[0] = page_of(w.i0 + 1, 0), ids[1] = page_of(w.i0 + 1, 1);
+            for (int it = w.i0; it < w.i1; ++it, ++done) {
+                if (done >= NS && !wait_warp(empty0 + 8 * st, ph ^ 1u, err)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t to = kv_sm + st * STAGE_BYTES + (is_v ? KV_BYTES : 0u);
+                Info& info = infos[done % INFOS];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int key = lane + 32 * h;
+                    const uint32_t row = to + key * 128;
+                    if (is_v) {
+#pragma unroll
+                        for (int n = 0; n < NG; ++n) {
+                            uint32_t wd = there[h] ? words[h][n] : 0u;
+                            if (half_not_finite(wd)) wd = 0;
+                            const uint32_t s = __byte_perm(wd, wd, 0x1010), m = times(__byte_perm(wd, wd, 0x3232), V_DOWN), s1 = times(s, V_UP), s16 = times(s, V_UP16);
+                            const uint32_t c[4] = {codes[h][n].x, codes[h][n].y, codes[h][n].z, codes[h][n].w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                // a word's numbers lie as c0 c4, c1 c5, c2 c6, c3 c7: neighbours come together by permutations
+                                const uint32_t u8 = c[i] >> 8;
+                                const uint32_t a = fma_bf16(c[i] & LOW, s1, m), b = fma_bf16(c[i] & HIGH, s16, m), x = fma_bf16(u8 & LOW, s1, m), y = fma_bf16(u8 & HIGH, s16, m);
+                                store16(row + (n >> 1) * KV_HALF + ((((n & 1) * 4 + i) ^ (key & 7)) << 4), __byte_perm(a, b, 0x5410), __byte_perm(x, y, 0x5410), __byte_perm(a, b, 0x7632),
+                                        __byte_perm(x, y, 0x7632));
+                            }
+                        }
+                    } else {
+                        // the power of two that brings the largest number that these 32 keys can hold below 2^15
+                        float most = 0.f;
+                        unsigned odd = 0;
+#pragma unroll
+                        for (int n = 0; n < NG; ++n) {
+                            const uint32_t wd = there[h] ? words[h][n] : 0u;
+                            if (!half_not_finite(wd)) most = fmaxf(most, fmaf(15.f, fabsf(scale_of(wd)), fabsf(least_of(wd))));
+                            if (there[h] && half_not_finite(beside[h][n])) odd |= 1u << n;
+                        }
+                        const int expo = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23);
+                        const int e = min(expo == 0 ? 0 : 141 - expo, 100);            // (k below 2^(expo - 126))
+                        const float f = power_of_two(e);
+                        const unsigned are = __ballot_sync(0xffffffffu, there[h]), odds = __ballot_sync(0xffffffffu, odd != 0);
+                        info.groups[key] = (unsigned char)odd;
+                        if (lane == 0) info.f[h] = power_of_two(-e), info.there[h] = are, info.odd[h] = odds;
+#pragma unroll
+                        for (int n = 0; n < NG; ++n) {
+                            const uint32_t wd = there[h] ? words[h][n] : 0u;
+                            const float s = scale_of(wd) * f, m = least_of(wd) * f;
+                            const uint32_t s2 = pack_f16(s, s), m2 = pack_f16(m, m);
+                            const uint32_t c[4] = {codes[h][n].x, codes[h][n].y, codes[h][n].z, codes[h][n].w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                // (1,024 + c and 1,024 + 16 c are float16 numbers with the code's bits)
+                                const uint32_t u8 = c[i] >> 8;
+                                const uint32_t a = fma_f16(add_f16((c[i] & LOW) | 0x64006400u, 0xe400e400u), s2, m2), b = fma_f16(fma_f16((c[i] & HIGH) | 0x64006400u, 0x2c002c00u, 0xd400d400u), s2, m2);
+                                const uint32_t x = fma_f16(add_f16((u8 & LOW) | 0x64006400u, 0xe400e400u), s2, m2), y = fma_f16(fma_f16((u8 & HIGH) | 0x64006400u, 0x2c002c00u, 0xd400d400u), s2, m2);
+                                store16(row + (n >> 1) * KV_HALF + ((((n & 1) * 4 + i) ^ (key & 7)) << 4), __byte_perm(a, b, 0x5410), __byte_perm(x, y, 0x5410), __byte_perm(a, b, 0x7632),
+                                        __byte_perm(x, y, 0x7632));
+                            }
+                        }
+                    }
+                }
+                if (it + 1 < w.i1) {
+                    fetch(it + 1, ids);
+                    ids[0] = page_of(it + 2, 0), ids[1] = page_of(it + 2, 1);
+                }
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full0 + 8 * st);
+                if (++st == NS) {
+                    st = 0;
+                    ph ^= 1u;
+                }
+            }
+        }
+    } else if (warp == 10) {
+        // ---- S = Q K^T of every tile
+        const uint32_t one = elected(), tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint32_t idesc = idesc_f16(KT);
+        const uint64_t dq0 = umma_desc(q_sm, 16, 1024), dk0 = umma_desc(kv_sm, 16, 1024);
+        int st = 0, Th[2] = {0, 0}, I = 0, I1 = 0;
+        uint32_t ph = 0;
+        bool ok = any;
+        for (bool first = true; ok && next_segment(A, w, first); first = false, ++I) {
+            const int halves = w.r.nodes * group - w.piece * ROWS > RT ? 2 : 1;
+            ok = wait_warp(q_ready0, I & 1, err);
+            if (halves == 2) ok = ok && wait_warp(q_ready0 + 8, I1++ & 1, err);
+            for (int it = w.i0; it < w.i1 && ok; ++it) {
+                ok = wait_warp(k_full0 + 8 * st, ph, err);
+                const uint64_t dk = dk0 + (uint64_t)((st * STAGE_BYTES) >> 4);
+                for (int hd = 0; hd < halves && ok; ++hd) {
+                    const int th = Th[hd]++, sb = th & 1;
+                    // these columns held the scores and then P of this half's last tile but one: its P V must have read them
+                    ok = th < 2 || wait_warp(pv_done0 + 8 * (2 * hd + sb), ((th >> 1) - 1) & 1, err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t dq = dq0 + (uint64_t)((hd * Q_ONE) >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < DP / 16; ++kk) {
+                        const uint32_t off = (kk >> 2), inner = (kk & 3) * 32;
+                        umma_ss(one, tmem_u + (uint32_t)(hd * 128 + sb * 64), dq + (uint64_t)((off * RT * 128 + inner) >> 4), dk + (uint64_t)((off * KV_HALF + inner) >> 4), idesc, kk ? 1u : 0u);
+                    }
+                    commit(one, s_ready0 + 8 * (2 * hd + sb));
+                }
+                if (!ok) break;
+                commit(one, k_empty0 + 8 * st);
+                if (++st == NS) {
+                    st = 0;
+                    ph ^= 1u;
+                }
+            }
+        }
+        commit(one, drained0);                   // no product is at work when the tensor memory is freed, however the block ends
+        wait_warp(drained0, 0, err);
+    } else if (warp == 11) {
+        // ---- O += P V of every tile (O starts as zeros, by the softmax threads)
+        const uint32_t one = elected(), tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint32_t idesc = umma_idesc(DP, 1);
+        const uint64_t dv0 = umma_desc(kv_sm + KV_BYTES, KV_HALF, 1024);
+        int st = 0, Th[2] = {0, 0};
+        uint32_t ph = 0;
+        bool ok = any;
+        for (bool first = true; ok && next_segment(A, w, first); first = false) {
+            const int halves = w.r.nodes * group - w.piece * ROWS > RT ? 2 : 1;
+            for (int it = w.i0; it < w.i1 && ok; ++it) {
+                ok = wait_warp(v_full0 + 8 * st, ph, err);
+                const uint64_t dv = dv0 + (uint64_t)((st * STAGE_BYTES) >> 4);
+                for (int hd = 0; hd < halves && ok; ++hd) {
+                    const int th = Th[hd]++, sb = th & 1;
+                    ok = wait_warp(p_ready0 + 8 * (2 * hd + sb), (th >> 1) & 1, err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t tp = tmem_u + (uint32_t)(hd * 128 + sb * 64);
+#pragma unroll
+                    for (int kk = 0; kk < KT / 16; ++kk)
+                        umma_ts(one, tmem_u + (uint32_t)(256 + hd * 128), tp + (uint32_t)(kk * 8), dv + (uint64_t)((kk * 2048) >> 4), idesc);
+                    commit(one, pv_done0 + 8 * (2 * hd + sb));
+                }
+                if (!ok) break;
+                commit(one, v_empty0 + 8 * st);
+                if (++st == NS) {
+                    st = 0;
+                    ph ^= 1u;
+                }
+            }
+        }
+        commit(one, drained0 + 8);
+        wait_warp(drained0 + 8, 0, err);
+    } else {
+        // ---- softmax: a row per thread
+        const int hd = warp >> 2, r = (int)threadIdx.x & 127;
+        const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tmem_s = tmem + (uint32_t)(hd * 128) + lane_addr, tmem_o = tmem + (uint32_t)(256 + hd * 128) + lane_addr;
+        const uint32_t my_s_ready = s_ready0 + 16 * hd, my_p_ready = p_ready0 + 16 * hd, my_pv_done = pv_done0 + 16 * hd;
+        const bool q16 = ((uintptr_t)A.q & 15) == 0 && A.q_stride % 8 == 0 && A.d % 8 == 0, out16 = ((uintptr_t)A.out & 15) == 0 && A.out_stride % 8 == 0 && A.d % 8 == 0;
+        int T = 0, Th = 0;                       // tiles of all segments so far, of this half's
+        bool alive = any;
+        for (bool first = true; alive && next_segment(A, w, first); first = false) {
+            const int row0 = w.piece * ROWS, rows = min(ROWS, w.r.nodes * group - row0);
+            if (rows <= hd * RT) {               // there is no second tile of rows
+                T += w.i1 - w.i0;
+                continue;
+            }
+            const int row = hd * RT + r;
+            const bool valid = row < rows;
+            const int of_request = row0 + min(row, rows - 1), pos = w.r.first_pos + of_request / group;
+            const int lo = first_seen(A, pos), hi = min(pos + 1, w.r.keys);              // the keys that the row sees
+            const long long t = w.r.first + of_request / group;
+            const int head = w.g * group + of_request % group;
+            // Q: the last tile's scores of the last segment are there, so nothing reads what lies there
+            float c1;
+            {
+                const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(A.q) + t * A.q_stride + (long long)head * A.d;
+                auto load = [&](int c, float (&x)[8]) {
+                    if (q16 && c + 8 <= A.d) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(q + c);
+                        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = c + e < A.d ? __bfloat162float(q[c + e]) : 0.f;
+                    }
+                };
+                float top = 0.f;
+#pragma unroll 4
+                for (int c = 0; c < DP; c += 8) {
+                    float x[8];
+                    load(c, x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(x[e]));
+                }
+                // the power of two that brings the row's largest number to 2^13 .. 2^14
+                const int expo = (int)(__float_as_uint(top) >> 23), e2 = expo < 255 && expo > 0 ? 140 - expo : 0;
+                const float f1 = power_of_two(e2 / 2), f2 = power_of_two(e2 - e2 / 2);
+                c1 = scale_log2 / f1 / f2;
+#pragma unroll 2
+                for (int c = 0; c < DP; c += 8) {
+                    float x[8];
+                    load(c, x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = x[e] * f1 * f2;
+                    store16(q_sm + hd * Q_ONE + (c >> 6) * (RT * 128) + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4), pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]),
+                            pack_f16(x[6], x[7]));
+                }
+                float zero[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) zero[i] = 0.f;
+#pragma unroll
+                for (int c0 = 0; c0 < DP; c0 += 32) tmem_st32(tmem_o + c0, zero);
+                tmem_st_wait();
+                fence_async_shared();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_ready0 + 8 * hd);
+            }
+            float m_ref = -INFINITY, l = 0.f;
+            unsigned poison = 0;                 // groups of channels that are no number
+            // keys from all0 on and below all1 are seen by all rows of the job
+            const int pos0 = w.r.first_pos + row0 / group, pos1 = w.r.first_pos + (row0 + rows - 1) / group;
+            const int all0 = first_seen(A, pos1), all1 = min(pos0 + 1, w.r.keys);
+            for (int it = w.i0; it < w.i1; ++it, ++Th) {
+                const int sb = Th & 1, key0 = (w.tile0 + it) * KT;
+                if (!wait_warp(my_s_ready + 8 * sb, (Th >> 1) & 1, err)) {
+                    alive = false;
+                    break;
+                }
+                tc_fence_after();
+                const volatile Info& info = infos[(T + it - w.i0) % INFOS];
+                float sc[64];
+                {
+                    uint32_t ra[32], rb[32];
+                    tmem_ld32_nowait(tmem_s + sb * 64, ra);
+                    tmem_ld32_nowait(tmem_s + sb * 64 + 32, rb);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        sc[i] = __uint_as_float(ra[i]);
+                        sc[32 + i] = __uint_as_float(rb[i]);
+                    }
+                }
+                const unsigned t0 = info.there[0], t1 = info.there[1], o0 = info.odd[0], o1 = info.odd[1];
+                const float ca = fminf(fmaxf(c1 * info.f[0], 1.2e-38f), 3.0e38f), cb = fminf(fmaxf(c1 * info.f[1], 1.2e-38f), 3.0e38f);      // (a sum of zero stays one, and one of a key that is not seen)
+                const bool edge = key0 < all0 || key0 + KT > all1 || (t0 & t1) != 0xffffffffu || (o0 | o1);
+                bool dead3 = false;              // (keys that are not seen have no weight at all, by the polynomial either)
+                unsigned long long seen = ~0ull;
+                if (edge) {
+                    seen = (unsigned long long)t1 << 32 | t0;
+                    if (hi - key0 < 64) seen &= hi > key0 ? (1ull << (hi - key0)) - 1 : 0ull;
+                    if (lo > key0) seen = lo - key0 < 64 ? seen & (~0ull << (lo - key0)) : 0ull;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) sc[i] = (seen >> i & 1ull) ? sc[i] : -INFINITY;
+                    dead3 = true;
+                    unsigned long long odd = ((unsigned long long)o1 << 32 | o0) & seen;
+                    while (odd) {
+                        poison |= info.groups[__ffsll((long long)odd) - 1];
+                        odd &= odd - 1;
+                    }
+                }
+                float mx[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        m4[0] = max3_nan(m4[0], sc[h * 32 + i], sc[h * 32 + i + 1]);
+                        m4[1] = max3_nan(m4[1], sc[h * 32 + i + 2], sc[h * 32 + i + 3]);
+                        m4[2] = max3_nan(m4[2], sc[h * 32 + i + 4], sc[h * 32 + i + 5]);
+                        m4[3] = max3_nan(m4[3], sc[h * 32 + i + 6], sc[h * 32 + i + 7]);
+                    }
+                    mx[h] = max3_nan(m4[0], m4[1], max3_nan(m4[2], m4[3], m4[3])) * (h ? cb : ca);
+                }
+                const float top = max_nan(mx[0], mx[1]);
+                float corr = 1.f;
+                bool moved = false;
+                if (!(top <= m_ref + RESCALE_STEP)) {                    // (a score that is no number makes the row one)
+                    corr = m_ref == -INFINITY ? 0.f : ex2(m_ref - top);
+                    moved = m_ref != -INFINITY && valid;                 // (O is zero before)
+                    m_ref = top;
+                }
+                const float m_neg = m_ref == -INFINITY ? 0.f : -m_ref;
+                const f32x2 mneg2 = pack2(m_neg, m_neg);
+                f32x2 sum_a = pack2(0.f, 0.f), sum_b = pack2(0.f, 0.f);
+                uint32_t pk[32];
+#pragma unroll
+                for (int c8 = 0; c8 < 8; ++c8) {
+                    const f32x2 scale2 = c8 < 4 ? pack2(ca, ca) : pack2(cb, cb);
+                    float x[8], e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) unpack2(fma2(pack2(sc[c8 * 8 + i], sc[c8 * 8 + i + 1]), scale2, mneg2), x[i], x[i + 1]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if ((i & 3) != 3) e[i] = ex2(x[i]);
+                    ex2_poly2(x[3], x[7], e[3], e[7]);
+                    if (dead3) {
+                        if (x[3] == -INFINITY) e[3] = 0.f;
+                        if (x[7] == -INFINITY) e[7] = 0.f;
+                    }
+                    sum_a = add2(sum_a, add2(pack2(e[0], e[1]), pack2(e[2], e[3])));
+                    sum_b = add2(sum_b, add2(pack2(e[4], e[5]), pack2(e[6], e[7])));
+                    pk[c8 * 4] = pack_bf16(e[0], e[1]);
+                    pk[c8 * 4 + 1] = pack_bf16(e[2], e[3]);
+                    pk[c8 * 4 + 2] = pack_bf16(e[4], e[5]);
+                    pk[c8 * 4 + 3] = pack_bf16(e[6], e[7]);
+                }
+                float s0, s1, s2, s3;
+                unpack2(sum_a, s0, s1);
+                unpack2(sum_b, s2, s3);
+                l = l * corr + ((s0 + s1) + (s2 + s3));
+                tmem_st32_u(tmem_s + sb * 64, pk);                       // P goes where the scores were
+                // O is touched only when the last tile's P V has completed
+                if (__any_sync(0xffffffffu, moved)) {
+                    if (it > w.i0 && !wait_warp(my_pv_done + 8 * (sb ^ 1), ((Th - 1) >> 1) & 1, err)) {
+                        alive = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const float f = moved ? corr : 1.f;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < DP; c0 += 32) {
+                        float o[32];
+                        tmem_ld32(tmem_o + c0, o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] *= f;
+                        tmem_st32(tmem_o + c0, o);
+                    }
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(my_p_ready + 8 * sb);
+            }
+            T += w.i1 - w.i0;
+            // ---- O / l, or this part of a job that blocks share
+            if (alive) alive = wait_warp(my_pv_done + 8 * ((Th - 1) & 1), ((Th - 1) >> 1) & 1, err);
+            if (!alive) break;
+            tc_fence_after();
+            const bool whole = w.i0 == 0 && w.i1 == w.tiles;
+            const size_t part = (size_t)blockIdx.x * 2 + (w.from > w.job ? 0 : 1);
+            const float f = whole ? (l > 0.f || l != l ? BACK / l : 0.f) : BACK;
+            float* part_to = line.part_o + (part * ROWS + row) * DP;
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + t * A.out_stride + (long long)head * A.d;
+#pragma unroll 1
+            for (int c0 = 0; c0 < min(DP, NG * 32); c0 += 32) {
+                float o[32];
+                tmem_ld32(tmem_o + c0, o);
+                const bool bad = poison >> (c0 / 32) & 1u;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = bad ? __uint_as_float(0x7fffffffu) : o[i] * f;
+                if (!valid) continue;
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(part_to + c0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                } else if (out16) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+                        if (c0 + i < A.d) *reinterpret_cast<uint4*>(out + c0 + i) = make_uint4(pack_bf16(o[i], o[i + 1]), pack_bf16(o[i + 2], o[i + 3]), pack_bf16(o[i + 4], o[i + 5]), pack_bf16(o[i + 6], o[i + 7]));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (c0 + i < A.d) out[c0 + i] = __float2bfloat16_rn(o[i]);
+                }
+            }
+            if (!whole && valid) *reinterpret_cast<float2*>(line.part_ml + (part * ROWS + row) * 2) = make_float2(m_ref, l);
+            if (!whole && threadIdx.x == 0) {
+                int* job = line.jobs + part * JOB_WORDS;
+                const int first_block = w.job / w.share, last = (w.job + w.tiles - 1) / w.share;
+                job[1] = first_block, job[2] = row0, job[3] = rows, job[4] = w.g, job[5] = w.b;
+                job[0] = last - first_block + 1;
+            }
+            tc_fence_before();                   // (O has been read before it is written again)
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 11) tmem_free(tmem, 512);
+}
+
+// A job's parts, joined in the order of the line: every part's blocks take a share of the job's numbers.
+constexpr int JOIN_THREADS = 256, JOIN_BLOCKS = 4;
+
+template <int NG>
+__global__ void __launch_bounds__(JOIN_THREADS)
+cache4_attention_tc_join_kernel(const AttendArgs A, const Line line) {
+    constexpr int DP = NG <= 2 ? 64 : 128, FOURS = NG * 8;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int* job = line.jobs + (size_t)blockIdx.x * JOB_WORDS;
+    const int4 head = *reinterpret_cast<const int4*>(job);
+    const int parts = head.x;
+    if (parts < 1) return;
+    const int first = head.y, row0 = head.z, rows = head.w, g = job[4], group = A.nh / A.nkv;
+    const Request r = request_of(A, job[5]);
+    const int mine = ((int)blockIdx.x / 2 - first) * JOIN_BLOCKS + (int)blockIdx.y, shares = parts * JOIN_BLOCKS, total = rows * FOURS;
+    auto part_of = [&](int i) { return (size_t)(first + i) * 2 + (i == 0 ? 1 : 0); };     // (the first part is its block's last segment)
+    for (int i = (int)((long long)total * mine / shares) + (int)threadIdx.x; i < (int)((long long)total * (mine + 1) / shares); i += JOIN_THREADS) {
+        const int row = i / FOURS, c = i % FOURS * 4;
+        float top = -INFINITY, sum = 0.f;
+        for (int k = 0; k < parts; ++k) top = max_nan(top, line.part_ml[(part_of(k) * ROWS + row) * 2]);
+        float4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int k = 0; k < parts; ++k) {
+            const size_t at = part_of(k) * ROWS + row;
+            const float2 ml = *reinterpret_cast<const float2*>(line.part_ml + at * 2);
+            const float4 u = *reinterpret_cast<const float4*>(line.part_o + at * DP + c);
+            const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+            sum = fmaf(f, ml.y, sum);
+            v.x = fmaf(f, u.x, v.x), v.y = fmaf(f, u.y, v.y), v.z = fmaf(f, u.z, v.z), v.w = fmaf(f, u.w, v.w);
+        }
+        const long long t = r.first + (row0 + row) / group;
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + t * A.out_stride + (long long)(g * group + (row0 + row) % group) * A.d;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < A.d) out[c + e] = __float2bfloat16_rn(y[e]);
+    }
+}
+
+constexpr int dp_of(int d) { return d <= 64 ? 64 : 128; }
+
+template <int NG>
+int launch(const AttendArgs& A, float* scratch, cudaStream_t stream) {
+    constexpr int DP = NG <= 2 ? 64 : 128, smem = (DP / 64) * (2 * RT * 128 + NS * 2 * KT * 128) + 1024;
+    Line line;
+    line.part_o = scratch;
+    line.part_ml = scratch + (size_t)BLOCKS * 2 * ROWS * DP;
+    line.jobs = reinterpret_cast<int*>(line.part_ml + (size_t)BLOCKS * 2 * ROWS * 2);
+    static unsigned long long roomy = 0;
+    if (const int rc = xb_more_smem(cache4_attention_tc_kernel<NG>, smem, &roomy)) return rc;
+    const int rc = xb_launch(cache4_attention_tc_kernel<NG>, dim3(BLOCKS), dim3(THREADS), smem, stream, A, line, A.scale * 1.4426950408889634f);
+    if (rc) return rc;
+    return xb_launch(cache4_attention_tc_join_kernel<NG>, dim3(2 * BLOCKS, JOIN_BLOCKS), dim3(JOIN_THREADS), 0, stream, A, line);
+}
+
+}  // namespace
+
+namespace xb4 {
+
+bool tc_takes(int nh, int nkv, int d, int longest) { return d <= 128 && (long long)longest * (nh / nkv) >= TC_ROWS; }
+bool tc_takes(const AttendArgs& A, int longest) {
+    // the longest line that these shapes allow is counted in 32 bits
+    const double jobs = (double)A.nkv * ((double)A.tokens * (A.nh / A.nkv) / ROWS + A.requests), tiles = (double)A.table_stride * A.page_size / KT + 2;
+    return tc_takes(A.nh, A.nkv, A.d, longest) && A.scale > 0.f && A.num_pages > 0 && (long long)A.page_size * row_bytes(A.d) % 16 == 0 && jobs * (tiles + COST_JOB) < 2147483648.0;
+}
+long long tc_scratch(int d) { return (long long)BLOCKS * 2 * (ROWS * (dp_of(d) + 2) + JOB_WORDS); }
+int tc_launch(const AttendArgs& A, float* scratch, cudaStream_t stream) {
+    switch (groups_of(A.d)) {
+        case 1: return launch<1>(A, scratch, stream);
+        case 2: return launch<2>(A, scratch, stream);
+        case 3: return launch<3>(A, scratch, stream);
+        default: return launch<4>(A, scratch, stream);
+    }
+}
+
+}  // namespace xb4
