@@ -263,10 +263,12 @@ class Attend:
                     # a score is a chain of d products and as many parts of a group; both it and the maximum enter an exponential
                     steps = np.abs(kk).max() * np.abs(q[t, h]).sum() * abs(self.scale)
                     allowed = HALF[self.dtype] * np.abs(want) + (2 * (d + 16) * 2.0 ** -23 * steps + (64 + seen.sum() / 16) * 2.0 ** -23) * size
-                    if self.dtype == BF:       # the probabilities' rounding, by themselves and times a group's scale, for both parts of m + s code
+                    if self.dtype == BF and n * (nh // nkv) >= 64 and d <= 128 and self.scale > 0:
+                        # many rows: float16 operands.  A probability and a value are off by 2^-11 of themselves (values by 2^-25 of the largest at least),
+                        # a key by that in every product of a score
+                        allowed = allowed + (2 + 2 * float((p * (np.abs(kk) @ np.abs(q[t, h]))).sum() * self.scale)) * 2.0 ** -11 * size + 2.0 ** -25 * np.abs(vv).max()
+                    elif self.dtype == BF:     # the probabilities' rounding, by themselves and times a group's scale, for both parts of m + s code
                         allowed = allowed + 2 * 2.0 ** -8 * (p @ parts[page, :, j % self.ps][seen, g])
-                        if n * (nh // nkv) >= 64:      # many rows: keys are rounded to float16 (2^-11 of themselves, in every product of a score), values to bfloat16
-                            allowed = allowed + (2 * 2.0 ** -11 * min(1.0, float((p * (np.abs(kk) @ np.abs(q[t, h]))).sum() * abs(self.scale))) + 2.0 ** -8) * size
                     off = np.abs(got[t, h] - want)
                     assert np.all(off <= allowed), (b, i, h, (off / allowed).max())
         assert np.all(got[self.start[-1]:] == 9)               # rows behind the last request

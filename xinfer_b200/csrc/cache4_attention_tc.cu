@@ -5,10 +5,10 @@
 // and values out of their codes, once for the 256 rows, into operands in shared memory (128-byte swizzle); S = Q K^T by warp 10, P = 2^(S - m) by a
 // thread per row in warps 0..3 and 4..7, in the tensor memory of S, O += P V by warp 11.
 //
-// Keys and queries are products of float16: 11 digits of m + s code, where bfloat16's 8 would move scores by as much as probabilities' rounding does
-// afterwards.  float16's range is made up for by powers of two: one per row of Q, one for every 32 keys of a tile, by which the scores are
-// multiplied back in float32.  Values and probabilities are bfloat16: a value is one multiply-add of the code's bits under a mask
-// (c 2^-133; 16 times that in the next four bits), 2^-69 times its size, which the result is multiplied back by.  Values' scales may be up to 2^60.
+// All operands are float16: 11 digits of m + s code and of a probability, where bfloat16's 8 would each move the result as much as its own rounding
+// does.  float16's range is made up for by powers of two that are undone in float32: one per row of Q; one for every 32 keys of a tile, by which the
+// scores are multiplied; one for the values of a job, which moves (with O, as for a new maximum) only when a tile's may be over 16 times larger
+// than the ones before.  Numbers 2^25 times smaller than the largest value lose digits.  Probabilities are held 2^6 times their size.
 // A group's word that is no number is zero in the operand; rows that see its key get no number in the group's channels at the end, the others nothing.
 //
 // The tiles of all jobs are one line cut into equal shares, one a block; parts of a job that blocks share are joined by a second kernel in their order.
@@ -28,8 +28,8 @@ constexpr int COST_JOB = 3;                // a job's start and end take about a
 constexpr float RESCALE_STEP = 8.f;
 constexpr int JOB_WORDS = 8, INFOS = 8;    // (a tile's facts are read at most NS + 2 tiles after they are written)
 constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
-constexpr uint32_t V_UP = 0x5f805f80u, V_UP16 = 0x5d805d80u, V_DOWN = 0x1d001d00u;     // bfloat16 2^64, 2^60, 2^-69, twice
-constexpr float BACK = 0x1p69f;
+constexpr float P_UP = 6.f;
+constexpr int RAW = 3;                     // tiles whose codes are on their way
 
 struct Line {
     float* part_o;                 // [blocks][2][256][DP]: a block's first segment, if its job began before it, and its last, if its job goes on
@@ -39,7 +39,8 @@ struct Line {
 
 // What the softmax needs to know of a tile of keys, and of its values.
 struct Info {
-    float f[2];                    // what the scores of the tile's halves are multiplied by
+    float f[2];                    // what the scores of the tile's halves are multiplied by,
+    float v_back;                  // and what is formed of its values
     unsigned there[2];             // keys that lie in a page
     unsigned odd[2];               // keys whose values have a group that is no number,
     unsigned char groups[KT];      // and which groups
@@ -192,16 +193,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-__device__ __forceinline__ uint32_t fma_bf16(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t d;
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
 __device__ __forceinline__ uint32_t fma_f16(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t d;
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
@@ -223,17 +214,35 @@ __device__ __forceinline__ void store16(uint32_t at, uint32_t a, uint32_t b, uin
 __device__ __forceinline__ bool half_not_finite(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }       // -126 <= e <= 127
 
-// A key's words.
+// Copies of a key's words to shared memory, and from there.
 template <int NG>
-__device__ __forceinline__ void load_words(const uint8_t* at, uint32_t (&w)[NG]) {
+__device__ __forceinline__ void copy_words(uint32_t dst, const uint8_t* src) {
     if constexpr (NG == 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(at);
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     } else {
 #pragma unroll
-        for (int n = 0; n < NG; ++n) w[n] = reinterpret_cast<const uint32_t*>(at)[n];
+        for (int n = 0; n < NG; ++n) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4 * n), "l"(src + 4 * n) : "memory");
     }
 }
+template <int NG>
+__device__ __forceinline__ void load_words(uint32_t at, uint32_t (&w)[NG]) {
+    if constexpr (NG == 4) {
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    } else {
+#pragma unroll
+        for (int n = 0; n < NG; ++n) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[n]) : "r"(at + 4 * n) : "memory");
+    }
+}
+// Eight numbers m + s code from a word, in their order.  (1,024 + c and 1,024 + 16 c are float16 numbers with the code's bits.)
+__device__ __forceinline__ void store_word(uint32_t at, uint32_t c, uint32_t s2, uint32_t m2) {
+    const uint32_t u8 = c >> 8;
+    const uint32_t a = fma_f16(add_f16((c & LOW) | 0x64006400u, 0xe400e400u), s2, m2), b = fma_f16(fma_f16((c & HIGH) | 0x64006400u, 0x2c002c00u, 0xd400d400u), s2, m2);
+    const uint32_t x = fma_f16(add_f16((u8 & LOW) | 0x64006400u, 0xe400e400u), s2, m2), y = fma_f16(fma_f16((u8 & HIGH) | 0x64006400u, 0x2c002c00u, 0xd400d400u), s2, m2);
+    // (they come as 0 4, 1 5, 2 6, 3 7)
+    store16(at, __byte_perm(a, b, 0x5410), __byte_perm(x, y, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(x, y, 0x7632));
+}
+// What a group's numbers stay below in size; nothing if it is no number.
+__device__ __forceinline__ float most_of(uint32_t word) { return half_not_finite(word) ? 0.f : fmaf(15.f, fabsf(scale_of(word)), fabsf(least_of(word))); }
 
 template <int NG>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -244,7 +253,8 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
     __shared__ __align__(8) unsigned long long bars[4 * NS + 16];
     __shared__ uint32_t s_tmem;
     __shared__ Info infos[INFOS];
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, q_sm = base, kv_sm = base + 2 * Q_ONE;
+    constexpr uint32_t RAW_CODES = NG * KT * 16, RAW_WORDS = KT * NG * 4, RAW_K = RAW_CODES + 2 * RAW_WORDS, RAW_V = RAW_CODES + RAW_WORDS;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, q_sm = base, kv_sm = base + 2 * Q_ONE, raw_sm = kv_sm + NS * STAGE_BYTES;
     const uint32_t bar0 = smem_u32(bars), k_full0 = bar0, k_empty0 = bar0 + 8 * NS, v_full0 = bar0 + 16 * NS, v_empty0 = bar0 + 24 * NS, rest = bar0 + 32 * NS;
     const uint32_t s_ready0 = rest, pv_done0 = rest + 32, p_ready0 = rest + 64, q_ready0 = rest + 96, drained0 = rest + 112;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = A.nh / A.nkv, ps = A.page_size;
@@ -286,33 +296,71 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
             const uint8_t* pages = (is_v ? A.v_cache : A.k_cache) + w.g * page_bytes;
             const uint8_t* v_pages = A.v_cache + w.g * page_bytes;
             const int first_key = first_seen(A, w.r.first_pos + w.piece * ROWS / group);       // (pages in front of it may have been given back)
-            // pages of a tile's keys two tiles ahead, codes and words one
-            auto page_of = [&](int it, int h) {
-                const int key = (w.tile0 + it) * KT + lane + 32 * h;
-                return it < w.i1 && key < w.r.keys && key >= first_key ? table[key / ps] : -1;
-            };
-            uint4 codes[2][NG];
-            uint32_t words[2][NG], beside[2][NG];
-            bool there[2];
-            auto fetch = [&](int it, const int (&ids)[2]) {
+            const uint32_t raw0 = raw_sm + (is_v ? RAW * RAW_K : 0u), raw_bytes = is_v ? RAW_V : RAW_K;
+            int ids[2], asked = w.i0, slot_in = 0, slot_out = 0;       // tiles asked for, their places in the ring
+            unsigned have = 0;                                         // two bits a tile, the last asked for lowest
+            auto look = [&](int it) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int key = (w.tile0 + it) * KT + lane + 32 * h, slot = key % ps;
-                    there[h] = ids[h] >= 0 && ids[h] < A.num_pages;
-                    if (!there[h] && key < w.r.keys && key >= first_key) atomicOr(err, XB_ERR_BAD_PAGE);
-                    if (there[h]) {
-                        const long long page = (long long)ids[h] * A.nkv * page_bytes;
-#pragma unroll
-                        for (int n = 0; n < NG; ++n) codes[h][n] = *reinterpret_cast<const uint4*>(pages + page + ((long long)n * ps + slot) * 16);
-                        load_words<NG>(pages + page + (long long)ps * 16 * NG + slot * NG * 4, words[h]);
-                        if (!is_v) load_words<NG>(v_pages + page + (long long)ps * 16 * NG + slot * NG * 4, beside[h]);
-                    }
+                    const int key = (w.tile0 + it) * KT + lane + 32 * h;
+                    ids[h] = it < w.i1 && key < w.r.keys && key >= first_key ? table[key / ps] : -1;
                 }
             };
-            int ids[2] = {page_of(w.i0, 0), page_of(w.i0, 1)};
-            fetch(w.i0, ids);
-            ids[0] = page_of(w.i0 + 1, 0), ids[1] = page_of(w.i0 + 1, 1);
+            auto ask = [&]() {
+                have <<= 2;
+                if (asked < w.i1) {
+                    const uint32_t to = raw0 + slot_in * raw_bytes;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int key = (w.tile0 + asked) * KT + lane + 32 * h, slot = key % ps;
+                        if (ids[h] >= 0 && ids[h] < A.num_pages) {
+                            have |= 1u << h;
+                            const uint8_t* page = pages + (long long)ids[h] * A.nkv * page_bytes;
+#pragma unroll
+                            for (int n = 0; n < NG; ++n)
+                                asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to + (n * KT + lane + 32 * h) * 16), "l"(page + ((long long)n * ps + slot) * 16) : "memory");
+                            const long long words = (long long)ps * 16 * NG + slot * NG * 4;
+                            copy_words<NG>(to + RAW_CODES + (lane + 32 * h) * NG * 4, page + words);
+                            if (!is_v) copy_words<NG>(to + RAW_CODES + RAW_WORDS + (lane + 32 * h) * NG * 4, v_pages + (long long)ids[h] * A.nkv * page_bytes + words);
+                        } else if (key < w.r.keys && key >= first_key) {
+                            atomicOr(err, XB_ERR_BAD_PAGE);
+                        }
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                ++asked;
+                slot_in = slot_in + 1 == RAW ? 0 : slot_in + 1;
+                look(asked);
+            };
+            look(asked);
+#pragma unroll
+            for (int i = 0; i < RAW - 1; ++i) ask();
+            int v_expo = 0;                                            // the values' power of two: their largest lies below 2^(v_expo - 126)
+            float v_down = 1.f;
             for (int it = w.i0; it < w.i1; ++it, ++done) {
+                ask();
+                asm volatile("cp.async.wait_group %0;" ::"n"(RAW - 1) : "memory");     // (a lane reads what it has copied itself)
+                const unsigned there = have >> (2 * (RAW - 1));
+                const uint32_t raw = raw0 + slot_out * raw_bytes;
+                slot_out = slot_out + 1 == RAW ? 0 : slot_out + 1;
+                uint32_t words[2][NG], beside[2][NG];                  // the warp's own, and the values' (warp 9: the same)
+                float most = 0.f;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    load_words<NG>(raw + RAW_CODES + (lane + 32 * h) * NG * 4, words[h]);
+                    if (!is_v) load_words<NG>(raw + RAW_CODES + RAW_WORDS + (lane + 32 * h) * NG * 4, beside[h]);
+#pragma unroll
+                    for (int n = 0; n < NG; ++n) {
+                        if (!(there >> h & 1u)) words[h][n] = beside[h][n] = 0u;
+                        most = fmaxf(most, most_of(is_v ? words[h][n] : beside[h][n]));
+                    }
+                }
+                // both warps find the same power of two for the values
+                const int expo_v = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23);
+                if (v_expo == 0 || expo_v > v_expo + 4) {
+                    v_expo = max(expo_v, 1);
+                    v_down = power_of_two(min(137 - v_expo, 100));     // below 2^11, so that up to 2^15 are no reason for another
+                }
                 if (done >= NS && !wait_warp(empty0 + 8 * st, ph ^ 1u, err)) {
                     ok = false;
                     break;
@@ -323,59 +371,32 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                 for (int h = 0; h < 2; ++h) {
                     const int key = lane + 32 * h;
                     const uint32_t row = to + key * 128;
-                    if (is_v) {
-#pragma unroll
-                        for (int n = 0; n < NG; ++n) {
-                            uint32_t wd = there[h] ? words[h][n] : 0u;
-                            if (half_not_finite(wd)) wd = 0;
-                            const uint32_t s = __byte_perm(wd, wd, 0x1010), m = times(__byte_perm(wd, wd, 0x3232), V_DOWN), s1 = times(s, V_UP), s16 = times(s, V_UP16);
-                            const uint32_t c[4] = {codes[h][n].x, codes[h][n].y, codes[h][n].z, codes[h][n].w};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                // a word's numbers lie as c0 c4, c1 c5, c2 c6, c3 c7: neighbours come together by permutations
-                                const uint32_t u8 = c[i] >> 8;
-                                const uint32_t a = fma_bf16(c[i] & LOW, s1, m), b = fma_bf16(c[i] & HIGH, s16, m), x = fma_bf16(u8 & LOW, s1, m), y = fma_bf16(u8 & HIGH, s16, m);
-                                store16(row + (n >> 1) * KV_HALF + ((((n & 1) * 4 + i) ^ (key & 7)) << 4), __byte_perm(a, b, 0x5410), __byte_perm(x, y, 0x5410), __byte_perm(a, b, 0x7632),
-                                        __byte_perm(x, y, 0x7632));
-                            }
-                        }
-                    } else {
+                    float f = v_down;
+                    if (!is_v) {
                         // the power of two that brings the largest number that these 32 keys can hold below 2^15
-                        float most = 0.f;
+                        float top = 0.f;
                         unsigned odd = 0;
 #pragma unroll
                         for (int n = 0; n < NG; ++n) {
-                            const uint32_t wd = there[h] ? words[h][n] : 0u;
-                            if (!half_not_finite(wd)) most = fmaxf(most, fmaf(15.f, fabsf(scale_of(wd)), fabsf(least_of(wd))));
-                            if (there[h] && half_not_finite(beside[h][n])) odd |= 1u << n;
+                            top = fmaxf(top, most_of(words[h][n]));
+                            if (half_not_finite(beside[h][n])) odd |= 1u << n;
                         }
-                        const int expo = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23);
-                        const int e = min(expo == 0 ? 0 : 141 - expo, 100);            // (k below 2^(expo - 126))
-                        const float f = power_of_two(e);
-                        const unsigned are = __ballot_sync(0xffffffffu, there[h]), odds = __ballot_sync(0xffffffffu, odd != 0);
+                        const int expo = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), e = min(expo == 0 ? 0 : 141 - expo, 100);
+                        f = power_of_two(e);
+                        const unsigned are = __ballot_sync(0xffffffffu, there >> h & 1u), odds = __ballot_sync(0xffffffffu, odd != 0);
                         info.groups[key] = (unsigned char)odd;
-                        if (lane == 0) info.f[h] = power_of_two(-e), info.there[h] = are, info.odd[h] = odds;
-#pragma unroll
-                        for (int n = 0; n < NG; ++n) {
-                            const uint32_t wd = there[h] ? words[h][n] : 0u;
-                            const float s = scale_of(wd) * f, m = least_of(wd) * f;
-                            const uint32_t s2 = pack_f16(s, s), m2 = pack_f16(m, m);
-                            const uint32_t c[4] = {codes[h][n].x, codes[h][n].y, codes[h][n].z, codes[h][n].w};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                // (1,024 + c and 1,024 + 16 c are float16 numbers with the code's bits)
-                                const uint32_t u8 = c[i] >> 8;
-                                const uint32_t a = fma_f16(add_f16((c[i] & LOW) | 0x64006400u, 0xe400e400u), s2, m2), b = fma_f16(fma_f16((c[i] & HIGH) | 0x64006400u, 0x2c002c00u, 0xd400d400u), s2, m2);
-                                const uint32_t x = fma_f16(add_f16((u8 & LOW) | 0x64006400u, 0xe400e400u), s2, m2), y = fma_f16(fma_f16((u8 & HIGH) | 0x64006400u, 0x2c002c00u, 0xd400d400u), s2, m2);
-                                store16(row + (n >> 1) * KV_HALF + ((((n & 1) * 4 + i) ^ (key & 7)) << 4), __byte_perm(a, b, 0x5410), __byte_perm(x, y, 0x5410), __byte_perm(a, b, 0x7632),
-                                        __byte_perm(x, y, 0x7632));
-                            }
-                        }
+                        if (lane == 0) info.f[h] = power_of_two(-e), info.there[h] = are, info.odd[h] = odds, info.v_back = 1.f / v_down;
                     }
-                }
-                if (it + 1 < w.i1) {
-                    fetch(it + 1, ids);
-                    ids[0] = page_of(it + 2, 0), ids[1] = page_of(it + 2, 1);
+#pragma unroll
+                    for (int n = 0; n < NG; ++n) {
+                        uint32_t wd = words[h][n], c[4];
+                        if (is_v && half_not_finite(wd)) wd = 0;
+                        const float s = scale_of(wd) * f, m = least_of(wd) * f;
+                        const uint32_t s2 = pack_f16(s, s), m2 = pack_f16(m, m);
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(raw + (n * KT + key) * 16) : "memory");
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) store_word(row + (n >> 1) * KV_HALF + ((((n & 1) * 4 + i) ^ (key & 7)) << 4), c[i], s2, m2);
+                    }
                 }
                 fence_async_shared();
                 __syncwarp();
@@ -385,6 +406,8 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                     ph ^= 1u;
                 }
             }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncwarp();
         }
     } else if (warp == 10) {
         // ---- S = Q K^T of every tile
@@ -428,7 +451,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
     } else if (warp == 11) {
         // ---- O += P V of every tile (O starts as zeros, by the softmax threads)
         const uint32_t one = elected(), tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
-        const uint32_t idesc = umma_idesc(DP, 1);
+        const uint32_t idesc = idesc_f16(DP) | 1u << 16;       // V lies channel by channel along its rows
         const uint64_t dv0 = umma_desc(kv_sm + KV_BYTES, KV_HALF, 1024);
         int st = 0, Th[2] = {0, 0};
         uint32_t ph = 0;
@@ -527,7 +550,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_ready0 + 8 * hd);
             }
-            float m_ref = -INFINITY, l = 0.f;
+            float m_ref = -INFINITY, l = 0.f, v_back = 0.f;
             unsigned poison = 0;                 // groups of channels that are no number
             // keys from all0 on and below all1 are seen by all rows of the job
             const int pos0 = w.r.first_pos + row0 / group, pos1 = w.r.first_pos + (row0 + rows - 1) / group;
@@ -552,6 +575,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                         sc[32 + i] = __uint_as_float(rb[i]);
                     }
                 }
+                const float v_now = info.v_back;
                 const unsigned t0 = info.there[0], t1 = info.there[1], o0 = info.odd[0], o1 = info.odd[1];
                 const float ca = fminf(fmaxf(c1 * info.f[0], 1.2e-38f), 3.0e38f), cb = fminf(fmaxf(c1 * info.f[1], 1.2e-38f), 3.0e38f);      // (a sum of zero stays one, and one of a key that is not seen)
                 const bool edge = key0 < all0 || key0 + KT > all1 || (t0 & t1) != 0xffffffffu || (o0 | o1);
@@ -591,7 +615,12 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                     moved = m_ref != -INFINITY && valid;                 // (O is zero before)
                     m_ref = top;
                 }
-                const float m_neg = m_ref == -INFINITY ? 0.f : -m_ref;
+                float f_o = corr;                // O's part: it is also in another power of two from now on
+                if (v_now != v_back) {           // (the same for all)
+                    if (v_back != 0.f) f_o *= v_back / v_now, moved = true;
+                    v_back = v_now;
+                }
+                const float m_neg = m_ref == -INFINITY ? 0.f : P_UP - m_ref;
                 const f32x2 mneg2 = pack2(m_neg, m_neg);
                 f32x2 sum_a = pack2(0.f, 0.f), sum_b = pack2(0.f, 0.f);
                 uint32_t pk[32];
@@ -611,10 +640,10 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                     }
                     sum_a = add2(sum_a, add2(pack2(e[0], e[1]), pack2(e[2], e[3])));
                     sum_b = add2(sum_b, add2(pack2(e[4], e[5]), pack2(e[6], e[7])));
-                    pk[c8 * 4] = pack_bf16(e[0], e[1]);
-                    pk[c8 * 4 + 1] = pack_bf16(e[2], e[3]);
-                    pk[c8 * 4 + 2] = pack_bf16(e[4], e[5]);
-                    pk[c8 * 4 + 3] = pack_bf16(e[6], e[7]);
+                    pk[c8 * 4] = pack_f16(e[0], e[1]);
+                    pk[c8 * 4 + 1] = pack_f16(e[2], e[3]);
+                    pk[c8 * 4 + 2] = pack_f16(e[4], e[5]);
+                    pk[c8 * 4 + 3] = pack_f16(e[6], e[7]);
                 }
                 float s0, s1, s2, s3;
                 unpack2(sum_a, s0, s1);
@@ -628,7 +657,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                         break;
                     }
                     tc_fence_after();
-                    const float f = moved ? corr : 1.f;
+                    const float f = moved ? f_o : 1.f;
 #pragma unroll 1
                     for (int c0 = 0; c0 < DP; c0 += 32) {
                         float o[32];
@@ -650,7 +679,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
             tc_fence_after();
             const bool whole = w.i0 == 0 && w.i1 == w.tiles;
             const size_t part = (size_t)blockIdx.x * 2 + (w.from > w.job ? 0 : 1);
-            const float f = whole ? (l > 0.f || l != l ? BACK / l : 0.f) : BACK;
+            const float f = whole ? (l > 0.f || l != l ? v_back / l : 0.f) : v_back;
             float* part_to = line.part_o + (part * ROWS + row) * DP;
             __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + t * A.out_stride + (long long)head * A.d;
 #pragma unroll 1
@@ -734,7 +763,7 @@ constexpr int dp_of(int d) { return d <= 64 ? 64 : 128; }
 
 template <int NG>
 int launch(const AttendArgs& A, float* scratch, cudaStream_t stream) {
-    constexpr int DP = NG <= 2 ? 64 : 128, smem = (DP / 64) * (2 * RT * 128 + NS * 2 * KT * 128) + 1024;
+    constexpr int DP = NG <= 2 ? 64 : 128, smem = (DP / 64) * (2 * RT * 128 + NS * 2 * KT * 128) + RAW * (2 * NG * KT * 16 + 3 * KT * NG * 4) + 1024;
     Line line;
     line.part_o = scratch;
     line.part_ml = scratch + (size_t)BLOCKS * 2 * ROWS * DP;
