@@ -1,12 +1,12 @@
 // Attention over 4-bit pages for many rows of a key/value head (portions of prompts, bfloat16) on the 5th-generation tensor cores
 // (cache4_attention.cu says what is computed).
 //
-// A job is (request, key/value head, up to two tiles of 128 rows): the rows are (token, query head of the group) pairs.  Two warps take tiles of 64 keys
-// and values out of their codes, once for the 256 rows, into operands in shared memory (128-byte swizzle); S = Q K^T by warp 10, P = 2^(S - m) by a
-// thread per row in warps 0..3 and 4..7, in the tensor memory of S, O += P V by warp 11.
+// A job is (request, key/value head, up to two tiles of 128 rows): the rows are (token, query head of the group) pairs.  Eight warps take tiles of 64
+// keys (8..11) and values (12..15) out of their codes, once for the 256 rows, into operands in shared memory (128-byte swizzle); S = Q K^T is
+// issued by warp 8, P = 2^(S - m) formed by a thread per row in warps 0..3 and 4..7, in the tensor memory of S, O += P V issued by warp 12.
 //
 // All operands are float16: 11 digits of m + s code and of a probability, where bfloat16's 8 would each move the result as much as its own rounding
-// does.  float16's range is made up for by powers of two that are undone in float32: one per row of Q; one for every 32 keys of a tile, by which the
+// does.  float16's range is made up for by powers of two that are undone in float32: one per row of Q; one for every 16 keys of a tile, by which the
 // scores are multiplied; one for the values of a job, which moves (with O, as for a new maximum) only when a tile's may be over 16 times larger
 // than the ones before.  Numbers 2^25 times smaller than the largest value lose digits.  Probabilities are held 2^6 times their size.
 // A group's word that is no number is zero in the operand; rows that see its key get no number in the group's channels at the end, the others nothing.
@@ -23,7 +23,8 @@ using namespace xb4;
 using namespace xbtc;
 
 constexpr int RT = 128, ROWS = 2 * RT, KT = 64;
-constexpr int BLOCKS = 148, THREADS = 384, NS = 3;
+constexpr int BLOCKS = 148, THREADS = 512, NS = 3, LEAD = NS - 1;      // tiles that codes are taken out ahead of their products
+constexpr int SOFTMAX_REGS = 168, CODE_REGS = 88;      // of 128 at launch: 2 * 168 + 2 * 88 = 4 * 128
 constexpr int COST_JOB = 3;                // a job's start and end take about as long as three tiles
 constexpr float RESCALE_STEP = 8.f;
 constexpr int JOB_WORDS = 8, INFOS = 8;    // (a tile's facts are read at most NS + 2 tiles after they are written)
@@ -39,10 +40,10 @@ struct Line {
 
 // What the softmax needs to know of a tile of keys, and of its values.
 struct Info {
-    float f[2];                    // what the scores of the tile's halves are multiplied by,
+    float f[4];                    // what the scores of every 16 keys are multiplied by,
     float v_back;                  // and what is formed of its values
-    unsigned there[2];             // keys that lie in a page
-    unsigned odd[2];               // keys whose values have a group that is no number,
+    unsigned short there[4];       // keys that lie in a page
+    unsigned short odd[4];         // keys whose values have a group that is no number,
     unsigned char groups[KT];      // and which groups
 };
 
@@ -178,16 +179,8 @@ __device__ __forceinline__ void commit(uint32_t one, uint32_t bar) {
 }
 // D float32, A and B float16, both K-major, M = 128, N = n
 __device__ __forceinline__ uint32_t idesc_f16(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
-__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int* err) { return mbar_wait(bar, parity, err); }
-__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* err) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return __all_sync(0xffffffffu, ok ? true : wait_long(bar, parity, err));
-}
+
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* err) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, true)); }
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float d;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -253,14 +246,14 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
     __shared__ __align__(8) unsigned long long bars[4 * NS + 16];
     __shared__ uint32_t s_tmem;
     __shared__ Info infos[INFOS];
-    constexpr uint32_t RAW_CODES = NG * KT * 16, RAW_WORDS = KT * NG * 4, RAW_K = RAW_CODES + 2 * RAW_WORDS, RAW_V = RAW_CODES + RAW_WORDS;
+    constexpr uint32_t RAW_CODES = NG * KT * 16, RAW_BYTES = RAW_CODES + KT * NG * 4;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, q_sm = base, kv_sm = base + 2 * Q_ONE, raw_sm = kv_sm + NS * STAGE_BYTES;
     const uint32_t bar0 = smem_u32(bars), k_full0 = bar0, k_empty0 = bar0 + 8 * NS, v_full0 = bar0 + 16 * NS, v_empty0 = bar0 + 24 * NS, rest = bar0 + 32 * NS;
     const uint32_t s_ready0 = rest, pv_done0 = rest + 32, p_ready0 = rest + 64, q_ready0 = rest + 96, drained0 = rest + 112;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = A.nh / A.nkv, ps = A.page_size;
     int* const err = A.err;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 4 * NS; ++i) mbar_init(bar0 + 8 * i, 1);
+        for (int i = 0; i < NS; ++i) mbar_init(k_full0 + 8 * i, 4), mbar_init(k_empty0 + 8 * i, 1), mbar_init(v_full0 + 8 * i, 4), mbar_init(v_empty0 + 8 * i, 1);
         for (int i = 0; i < 4; ++i) {
             mbar_init(s_ready0 + 8 * i, 1);
             mbar_init(pv_done0 + 8 * i, 1);
@@ -269,7 +262,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
         for (int i = 0; i < 2; ++i) mbar_init(q_ready0 + 8 * i, 4), mbar_init(drained0 + 8 * i, 1);
         mbar_init_fence();
     }
-    if (warp == 11) tmem_alloc(&s_tmem, 512);
+    if (warp == 8) tmem_alloc(&s_tmem, 512);
     if (NG * 32 < DP)                              // channels that no group has: zeros for good (the products of Q and K go over them)
         for (uint32_t i = threadIdx.x * 16; i < NS * STAGE_BYTES; i += THREADS * 16) store16(kv_sm + i, 0, 0, 0, 0);
     fence_async_shared();
@@ -284,206 +277,217 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
     const bool any = place_in_line(A, w);
     const long long page_bytes = (long long)ps * 20 * NG;
 
-    if (warp == 8 || warp == 9) {
-        // ---- codes to operands: warp 8 keys, warp 9 values; a lane has the keys `lane` and `lane + 32` of a tile
-        const bool is_v = warp == 9;
-        const uint32_t full0 = is_v ? v_full0 : k_full0, empty0 = is_v ? v_empty0 : k_empty0;
-        int st = 0, done = 0;
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CODE_REGS));
+        // ---- codes to operands, a quarter of a tile's keys a warp (two lanes a key: the first and the second half of its groups), and the products
+        const bool is_v = warp >= 12, leads = warp == 8 || warp == 12;
+        const int quarter = warp & 3, key = quarter * 16 + (lane & 15), part = lane >> 4;
+        constexpr int GP = (NG + 1) / 2;           // groups of a lane, at most
+        const int n0 = part * GP, n1 = min(NG, n0 + GP);
+        const uint32_t full0 = is_v ? v_full0 : k_full0, empty0 = is_v ? v_empty0 : k_empty0, raw0 = raw_sm + (is_v ? RAW * RAW_BYTES : 0u);
+        const uint32_t one = elected(), tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint32_t idesc_s = idesc_f16(KT), idesc_o = idesc_f16(DP) | 1u << 16;        // (V lies channel by channel along its rows)
+        const uint64_t dq0 = umma_desc(q_sm, 16, 1024), dk0 = umma_desc(kv_sm, 16, 1024), dv0 = umma_desc(kv_sm + KV_BYTES, KV_HALF, 1024);
+        int st = 0, done = 0;                      // ring stage and tiles of the codes
         uint32_t ph = 0;
+        int out_st = 0, Th[2] = {0, 0}, I = 0, I1 = 0;     // of the products
+        uint32_t out_ph = 0;
         bool ok = any;
-        for (bool first = true; ok && next_segment(A, w, first); first = false) {
+        for (bool first = true; ok && next_segment(A, w, first); first = false, ++I) {
             const int* table = A.block_table + (long long)w.b * A.table_stride;
             const uint8_t* pages = (is_v ? A.v_cache : A.k_cache) + w.g * page_bytes;
             const uint8_t* v_pages = A.v_cache + w.g * page_bytes;
             const int first_key = first_seen(A, w.r.first_pos + w.piece * ROWS / group);       // (pages in front of it may have been given back)
-            const uint32_t raw0 = raw_sm + (is_v ? RAW * RAW_K : 0u), raw_bytes = is_v ? RAW_V : RAW_K;
+            const int halves = w.r.nodes * group - w.piece * ROWS > RT ? 2 : 1;
+            // pages of the keys lane and lane + 32 of a tile, and the words of their values: every warp finds the same power of two for the values
             int ids[2], asked = w.i0, slot_in = 0, slot_out = 0;       // tiles asked for, their places in the ring
-            unsigned have = 0;                                         // two bits a tile, the last asked for lowest
+            unsigned have = 0;                                         // whether the lane's key is there, a bit a tile, the last asked for lowest
+            float most[RAW];                                           // what the values of the tiles asked for stay below, the last one first,
+            unsigned odd = 0;                                          // and their groups that are no numbers: eight bits a tile, four a key
+#pragma unroll
+            for (int i = 0; i < RAW; ++i) most[i] = 0.f;
             auto look = [&](int it) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int key = (w.tile0 + it) * KT + lane + 32 * h;
-                    ids[h] = it < w.i1 && key < w.r.keys && key >= first_key ? table[key / ps] : -1;
+                    const int k = (w.tile0 + it) * KT + lane + 32 * h;
+                    ids[h] = -1;
+                    if (it < w.i1 && k < w.r.keys && k >= first_key) {
+                        const int id = table[k / ps];
+                        if (id >= 0 && id < A.num_pages) ids[h] = id;
+                        else atomicOr(err, XB_ERR_BAD_PAGE);
+                    }
                 }
             };
+            uint32_t vw[2][NG];
             auto ask = [&]() {
-                have <<= 2;
-                if (asked < w.i1) {
-                    const uint32_t to = raw0 + slot_in * raw_bytes;
+                const int id = __shfl_sync(0xffffffffu, quarter & 2 ? ids[1] : ids[0], (quarter & 1) * 16 + (lane & 15));
+                have = have << 1 | (id >= 0 ? 1u : 0u);
+                if (id >= 0) {
+                    const int slot = ((w.tile0 + asked) * KT + key) % ps;
+                    const uint32_t to = raw0 + slot_in * RAW_BYTES;
+                    const uint8_t* page = pages + (long long)id * A.nkv * page_bytes;
+                    for (int n = n0; n < n1; ++n)
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to + (n * KT + key) * 16), "l"(page + ((long long)n * ps + slot) * 16) : "memory");
+                    if (part == 0) copy_words<NG>(to + RAW_CODES + key * NG * 4, page + (long long)ps * 16 * NG + slot * NG * 4);
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int key = (w.tile0 + asked) * KT + lane + 32 * h, slot = key % ps;
-                        if (ids[h] >= 0 && ids[h] < A.num_pages) {
-                            have |= 1u << h;
-                            const uint8_t* page = pages + (long long)ids[h] * A.nkv * page_bytes;
+                for (int h = 0; h < 2; ++h) {
+                    const int k = (w.tile0 + asked) * KT + lane + 32 * h;
 #pragma unroll
-                            for (int n = 0; n < NG; ++n)
-                                asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to + (n * KT + lane + 32 * h) * 16), "l"(page + ((long long)n * ps + slot) * 16) : "memory");
-                            const long long words = (long long)ps * 16 * NG + slot * NG * 4;
-                            copy_words<NG>(to + RAW_CODES + (lane + 32 * h) * NG * 4, page + words);
-                            if (!is_v) copy_words<NG>(to + RAW_CODES + RAW_WORDS + (lane + 32 * h) * NG * 4, v_pages + (long long)ids[h] * A.nkv * page_bytes + words);
-                        } else if (key < w.r.keys && key >= first_key) {
-                            atomicOr(err, XB_ERR_BAD_PAGE);
+                    for (int n = 0; n < NG; ++n) vw[h][n] = 0u;
+                    if (ids[h] >= 0) {
+                        const uint32_t* from = reinterpret_cast<const uint32_t*>(v_pages + (long long)ids[h] * A.nkv * page_bytes + (long long)ps * 16 * NG + k % ps * NG * 4);
+                        if constexpr (NG == 4) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(from);
+                            vw[h][0] = v.x, vw[h][1] = v.y, vw[h][2] = v.z, vw[h][3] = v.w;
+                        } else {
+#pragma unroll
+                            for (int n = 0; n < NG; ++n) vw[h][n] = from[n];
                         }
                     }
                 }
-                asm volatile("cp.async.commit_group;" ::: "memory");
                 ++asked;
                 slot_in = slot_in + 1 == RAW ? 0 : slot_in + 1;
                 look(asked);
             };
+            auto shift_most = [&]() {              // (the words of the tile asked for last have come by now)
+                float m = 0.f;
+                odd <<= 8;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int n = 0; n < NG; ++n) {
+                        m = fmaxf(m, most_of(vw[h][n]));
+                        if (half_not_finite(vw[h][n])) odd |= 1u << (4 * h + n);
+                    }
+#pragma unroll
+                for (int i = RAW - 1; i > 0; --i) most[i] = most[i - 1];
+                most[0] = m;
+            };
             look(asked);
 #pragma unroll
-            for (int i = 0; i < RAW - 1; ++i) ask();
-            int v_expo = 0;                                            // the values' power of two: their largest lies below 2^(v_expo - 126)
-            float v_down = 1.f;
-            for (int it = w.i0; it < w.i1; ++it, ++done) {
+            for (int i = 0; i < RAW - 1; ++i) {
                 ask();
-                asm volatile("cp.async.wait_group %0;" ::"n"(RAW - 1) : "memory");     // (a lane reads what it has copied itself)
-                const unsigned there = have >> (2 * (RAW - 1));
-                const uint32_t raw = raw0 + slot_out * raw_bytes;
-                slot_out = slot_out + 1 == RAW ? 0 : slot_out + 1;
-                uint32_t words[2][NG], beside[2][NG];                  // the warp's own, and the values' (warp 9: the same)
-                float most = 0.f;
+                shift_most();
+            }
+            int v_expo = 0;                        // the values' power of two: their largest lies below 2^(v_expo - 126)
+            float v_down = 1.f, v_back = 1.f;
+            const int tiles = w.i1 - w.i0;
+            for (int step = 0; step < tiles + (leads ? LEAD : 0); ++step) {
+                if (step < tiles) {
+                    ask();
+                    asm volatile("cp.async.wait_group %0;" ::"n"(RAW - 1) : "memory");
+                    __syncwarp();
+                    const bool there = have >> (RAW - 1) & 1u;
+                    const uint32_t raw = raw0 + slot_out * RAW_BYTES;
+                    slot_out = slot_out + 1 == RAW ? 0 : slot_out + 1;
+                    uint32_t words[NG];
+                    load_words<NG>(raw + RAW_CODES + key * NG * 4, words);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    load_words<NG>(raw + RAW_CODES + (lane + 32 * h) * NG * 4, words[h]);
-                    if (!is_v) load_words<NG>(raw + RAW_CODES + RAW_WORDS + (lane + 32 * h) * NG * 4, beside[h]);
-#pragma unroll
-                    for (int n = 0; n < NG; ++n) {
-                        if (!(there >> h & 1u)) words[h][n] = beside[h][n] = 0u;
-                        most = fmaxf(most, most_of(is_v ? words[h][n] : beside[h][n]));
+                    for (int n = 0; n < NG; ++n)
+                        if (!there) words[n] = 0u;
+                    // (the tile's values were asked for RAW - 1 tiles ago)
+                    const int expo_v = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(most[RAW - 2])) >> 23);
+                    if (v_expo == 0 || expo_v > v_expo + 4) {
+                        v_expo = max(expo_v, 1);
+                        const int e = min(137 - v_expo, 100);          // below 2^11, so that up to 2^15 are no reason for another
+                        v_down = power_of_two(e), v_back = power_of_two(-e);
                     }
-                }
-                // both warps find the same power of two for the values
-                const int expo_v = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23);
-                if (v_expo == 0 || expo_v > v_expo + 4) {
-                    v_expo = max(expo_v, 1);
-                    v_down = power_of_two(min(137 - v_expo, 100));     // below 2^11, so that up to 2^15 are no reason for another
-                }
-                if (done >= NS && !wait_warp(empty0 + 8 * st, ph ^ 1u, err)) {
-                    ok = false;
-                    break;
-                }
-                const uint32_t to = kv_sm + st * STAGE_BYTES + (is_v ? KV_BYTES : 0u);
-                Info& info = infos[done % INFOS];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int key = lane + 32 * h;
-                    const uint32_t row = to + key * 128;
+                    if (done >= NS && !wait_warp(empty0 + 8 * st, ph ^ 1u, err)) {
+                        ok = false;
+                        break;
+                    }
                     float f = v_down;
                     if (!is_v) {
-                        // the power of two that brings the largest number that these 32 keys can hold below 2^15
+                        // the power of two that brings the largest number that these 16 keys can hold below 2^15
+                        Info& info = infos[done % INFOS];
                         float top = 0.f;
-                        unsigned odd = 0;
 #pragma unroll
-                        for (int n = 0; n < NG; ++n) {
-                            top = fmaxf(top, most_of(words[h][n]));
-                            if (half_not_finite(beside[h][n])) odd |= 1u << n;
-                        }
+                        for (int n = 0; n < NG; ++n) top = fmaxf(top, most_of(words[n]));
                         const int expo = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), e = min(expo == 0 ? 0 : 141 - expo, 100);
                         f = power_of_two(e);
-                        const unsigned are = __ballot_sync(0xffffffffu, there >> h & 1u), odds = __ballot_sync(0xffffffffu, odd != 0);
-                        info.groups[key] = (unsigned char)odd;
-                        if (lane == 0) info.f[h] = power_of_two(-e), info.there[h] = are, info.odd[h] = odds, info.v_back = 1.f / v_down;
+                        const unsigned are = __ballot_sync(0xffffffffu, there);
+                        const unsigned odd_now = __shfl_sync(0xffffffffu, odd >> (8 * (RAW - 2)), (quarter & 1) * 16 + (lane & 15)) >> (2 * (quarter & 2)) & 15u;
+                        const unsigned odds = __ballot_sync(0xffffffffu, odd_now != 0);
+                        if (part == 0) info.groups[key] = (unsigned char)odd_now;
+                        if (lane == 0) info.f[quarter] = power_of_two(-e), info.there[quarter] = (unsigned short)are, info.odd[quarter] = (unsigned short)odds;
+                        if (warp == 8 && lane == 0) info.v_back = v_back;
                     }
+                    const uint32_t row = kv_sm + st * STAGE_BYTES + (is_v ? KV_BYTES : 0u) + key * 128;
 #pragma unroll
-                    for (int n = 0; n < NG; ++n) {
-                        uint32_t wd = words[h][n], c[4];
-                        if (is_v && half_not_finite(wd)) wd = 0;
-                        const float s = scale_of(wd) * f, m = least_of(wd) * f;
-                        const uint32_t s2 = pack_f16(s, s), m2 = pack_f16(m, m);
-                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(raw + (n * KT + key) * 16) : "memory");
+                    for (int g = 0; g < GP; ++g) {
+                        const int n = n0 + g;
+                        if (n < n1) {
+                            uint32_t wd = GP == 1 ? (part ? words[NG - 1] : words[0]) : (part ? words[min(GP + g, NG - 1)] : words[g]), c[4];
+                            if (is_v && half_not_finite(wd)) wd = 0;
+                            const float s = scale_of(wd) * f, m = least_of(wd) * f;
+                            const uint32_t s2 = pack_f16(s, s), m2 = pack_f16(m, m);
+                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(raw + (n * KT + key) * 16) : "memory");
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) store_word(row + (n >> 1) * KV_HALF + ((((n & 1) * 4 + i) ^ (key & 7)) << 4), c[i], s2, m2);
+                            for (int i = 0; i < 4; ++i) store_word(row + (n >> 1) * KV_HALF + ((((n & 1) * 4 + i) ^ (key & 7)) << 4), c[i], s2, m2);
+                        }
+                    }
+                    shift_most();
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full0 + 8 * st);
+                    ++done;
+                    if (++st == NS) {
+                        st = 0;
+                        ph ^= 1u;
                     }
                 }
-                fence_async_shared();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full0 + 8 * st);
-                if (++st == NS) {
-                    st = 0;
-                    ph ^= 1u;
+                if (!leads || step < LEAD) continue;
+                // ---- the products of the tile LEAD steps back
+                if (step == LEAD && !is_v) {
+                    ok = wait_warp(q_ready0, I & 1, err);
+                    if (halves == 2) ok = wait_warp(q_ready0 + 8, I1++ & 1, err) && ok;
+                }
+                ok = ok && wait_warp(full0 + 8 * out_st, out_ph, err);
+                for (int hd = 0; hd < halves && ok; ++hd) {
+                    const int th = Th[hd]++, sb = th & 1;
+                    if (!is_v) {
+                        // these columns held the scores and then P of this half's last tile but one: its P V must have read them
+                        ok = th < 2 || wait_warp(pv_done0 + 8 * (2 * hd + sb), ((th >> 1) - 1) & 1, err);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t dq = dq0 + (uint64_t)((hd * Q_ONE) >> 4), dk = dk0 + (uint64_t)((out_st * STAGE_BYTES) >> 4);
+#pragma unroll
+                        for (int kk = 0; kk < DP / 16; ++kk) {
+                            const uint32_t off = (kk >> 2), inner = (kk & 3) * 32;
+                            umma_ss(one, tmem_u + (uint32_t)(hd * 128 + sb * 64), dq + (uint64_t)((off * RT * 128 + inner) >> 4), dk + (uint64_t)((off * KV_HALF + inner) >> 4), idesc_s, kk ? 1u : 0u);
+                        }
+                        commit(one, s_ready0 + 8 * (2 * hd + sb));
+                    } else {
+                        ok = wait_warp(p_ready0 + 8 * (2 * hd + sb), (th >> 1) & 1, err);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t tp = tmem_u + (uint32_t)(hd * 128 + sb * 64);
+                        const uint64_t dv = dv0 + (uint64_t)((out_st * STAGE_BYTES) >> 4);
+#pragma unroll
+                        for (int kk = 0; kk < KT / 16; ++kk)
+                            umma_ts(one, tmem_u + (uint32_t)(256 + hd * 128), tp + (uint32_t)(kk * 8), dv + (uint64_t)((kk * 2048) >> 4), idesc_o);
+                        commit(one, pv_done0 + 8 * (2 * hd + sb));
+                    }
+                }
+                if (!ok) break;
+                commit(one, empty0 + 8 * out_st);
+                if (++out_st == NS) {
+                    out_st = 0;
+                    out_ph ^= 1u;
                 }
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncwarp();
         }
-    } else if (warp == 10) {
-        // ---- S = Q K^T of every tile
-        const uint32_t one = elected(), tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
-        const uint32_t idesc = idesc_f16(KT);
-        const uint64_t dq0 = umma_desc(q_sm, 16, 1024), dk0 = umma_desc(kv_sm, 16, 1024);
-        int st = 0, Th[2] = {0, 0}, I = 0, I1 = 0;
-        uint32_t ph = 0;
-        bool ok = any;
-        for (bool first = true; ok && next_segment(A, w, first); first = false, ++I) {
-            const int halves = w.r.nodes * group - w.piece * ROWS > RT ? 2 : 1;
-            ok = wait_warp(q_ready0, I & 1, err);
-            if (halves == 2) ok = ok && wait_warp(q_ready0 + 8, I1++ & 1, err);
-            for (int it = w.i0; it < w.i1 && ok; ++it) {
-                ok = wait_warp(k_full0 + 8 * st, ph, err);
-                const uint64_t dk = dk0 + (uint64_t)((st * STAGE_BYTES) >> 4);
-                for (int hd = 0; hd < halves && ok; ++hd) {
-                    const int th = Th[hd]++, sb = th & 1;
-                    // these columns held the scores and then P of this half's last tile but one: its P V must have read them
-                    ok = th < 2 || wait_warp(pv_done0 + 8 * (2 * hd + sb), ((th >> 1) - 1) & 1, err);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t dq = dq0 + (uint64_t)((hd * Q_ONE) >> 4);
-#pragma unroll
-                    for (int kk = 0; kk < DP / 16; ++kk) {
-                        const uint32_t off = (kk >> 2), inner = (kk & 3) * 32;
-                        umma_ss(one, tmem_u + (uint32_t)(hd * 128 + sb * 64), dq + (uint64_t)((off * RT * 128 + inner) >> 4), dk + (uint64_t)((off * KV_HALF + inner) >> 4), idesc, kk ? 1u : 0u);
-                    }
-                    commit(one, s_ready0 + 8 * (2 * hd + sb));
-                }
-                if (!ok) break;
-                commit(one, k_empty0 + 8 * st);
-                if (++st == NS) {
-                    st = 0;
-                    ph ^= 1u;
-                }
-            }
+        if (leads) {                               // no product is at work when the tensor memory is freed, however the block ends
+            commit(one, drained0 + (is_v ? 8 : 0));
+            wait_warp(drained0 + (is_v ? 8 : 0), 0, err);
         }
-        commit(one, drained0);                   // no product is at work when the tensor memory is freed, however the block ends
-        wait_warp(drained0, 0, err);
-    } else if (warp == 11) {
-        // ---- O += P V of every tile (O starts as zeros, by the softmax threads)
-        const uint32_t one = elected(), tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
-        const uint32_t idesc = idesc_f16(DP) | 1u << 16;       // V lies channel by channel along its rows
-        const uint64_t dv0 = umma_desc(kv_sm + KV_BYTES, KV_HALF, 1024);
-        int st = 0, Th[2] = {0, 0};
-        uint32_t ph = 0;
-        bool ok = any;
-        for (bool first = true; ok && next_segment(A, w, first); first = false) {
-            const int halves = w.r.nodes * group - w.piece * ROWS > RT ? 2 : 1;
-            for (int it = w.i0; it < w.i1 && ok; ++it) {
-                ok = wait_warp(v_full0 + 8 * st, ph, err);
-                const uint64_t dv = dv0 + (uint64_t)((st * STAGE_BYTES) >> 4);
-                for (int hd = 0; hd < halves && ok; ++hd) {
-                    const int th = Th[hd]++, sb = th & 1;
-                    ok = wait_warp(p_ready0 + 8 * (2 * hd + sb), (th >> 1) & 1, err);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t tp = tmem_u + (uint32_t)(hd * 128 + sb * 64);
-#pragma unroll
-                    for (int kk = 0; kk < KT / 16; ++kk)
-                        umma_ts(one, tmem_u + (uint32_t)(256 + hd * 128), tp + (uint32_t)(kk * 8), dv + (uint64_t)((kk * 2048) >> 4), idesc);
-                    commit(one, pv_done0 + 8 * (2 * hd + sb));
-                }
-                if (!ok) break;
-                commit(one, v_empty0 + 8 * st);
-                if (++st == NS) {
-                    st = 0;
-                    ph ^= 1u;
-                }
-            }
-        }
-        commit(one, drained0 + 8);
-        wait_warp(drained0 + 8, 0, err);
     } else {
         // ---- softmax: a row per thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
         const int hd = warp >> 2, r = (int)threadIdx.x & 127;
         const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tmem_s = tmem + (uint32_t)(hd * 128) + lane_addr, tmem_o = tmem + (uint32_t)(256 + hd * 128) + lane_addr;
@@ -576,8 +580,11 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                     }
                 }
                 const float v_now = info.v_back;
-                const unsigned t0 = info.there[0], t1 = info.there[1], o0 = info.odd[0], o1 = info.odd[1];
-                const float ca = fminf(fmaxf(c1 * info.f[0], 1.2e-38f), 3.0e38f), cb = fminf(fmaxf(c1 * info.f[1], 1.2e-38f), 3.0e38f);      // (a sum of zero stays one, and one of a key that is not seen)
+                const unsigned t0 = info.there[0] | (unsigned)info.there[1] << 16, t1 = info.there[2] | (unsigned)info.there[3] << 16;
+                const unsigned o0 = info.odd[0] | (unsigned)info.odd[1] << 16, o1 = info.odd[2] | (unsigned)info.odd[3] << 16;
+                float cf[4];                     // (a sum of zero stays one, and one of a key that is not seen)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) cf[i] = fminf(fmaxf(c1 * info.f[i], 1.2e-38f), 3.0e38f);
                 const bool edge = key0 < all0 || key0 + KT > all1 || (t0 & t1) != 0xffffffffu || (o0 | o1);
                 bool dead3 = false;              // (keys that are not seen have no weight at all, by the polynomial either)
                 unsigned long long seen = ~0ull;
@@ -594,20 +601,17 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                         odd &= odd - 1;
                     }
                 }
-                float mx[2];
+                float top = -INFINITY;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                for (int h = 0; h < 4; ++h) {
+                    float m2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        m4[0] = max3_nan(m4[0], sc[h * 32 + i], sc[h * 32 + i + 1]);
-                        m4[1] = max3_nan(m4[1], sc[h * 32 + i + 2], sc[h * 32 + i + 3]);
-                        m4[2] = max3_nan(m4[2], sc[h * 32 + i + 4], sc[h * 32 + i + 5]);
-                        m4[3] = max3_nan(m4[3], sc[h * 32 + i + 6], sc[h * 32 + i + 7]);
+                    for (int i = 0; i < 16; i += 4) {
+                        m2[0] = max3_nan(m2[0], sc[h * 16 + i], sc[h * 16 + i + 1]);
+                        m2[1] = max3_nan(m2[1], sc[h * 16 + i + 2], sc[h * 16 + i + 3]);
                     }
-                    mx[h] = max3_nan(m4[0], m4[1], max3_nan(m4[2], m4[3], m4[3])) * (h ? cb : ca);
+                    top = max_nan(top, max_nan(m2[0], m2[1]) * cf[h]);
                 }
-                const float top = max_nan(mx[0], mx[1]);
                 float corr = 1.f;
                 bool moved = false;
                 if (!(top <= m_ref + RESCALE_STEP)) {                    // (a score that is no number makes the row one)
@@ -626,7 +630,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                 uint32_t pk[32];
 #pragma unroll
                 for (int c8 = 0; c8 < 8; ++c8) {
-                    const f32x2 scale2 = c8 < 4 ? pack2(ca, ca) : pack2(cb, cb);
+                    const f32x2 scale2 = pack2(cf[c8 / 2], cf[c8 / 2]);
                     float x[8], e[8];
 #pragma unroll
                     for (int i = 0; i < 8; i += 2) unpack2(fma2(pack2(sc[c8 * 8 + i], sc[c8 * 8 + i + 1]), scale2, mneg2), x[i], x[i + 1]);
@@ -715,7 +719,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 11) tmem_free(tmem, 512);
+    if (warp == 8) tmem_free(tmem, 512);
 }
 
 // A job's parts, joined in the order of the line: every part's blocks take a share of the job's numbers.
@@ -763,7 +767,7 @@ constexpr int dp_of(int d) { return d <= 64 ? 64 : 128; }
 
 template <int NG>
 int launch(const AttendArgs& A, float* scratch, cudaStream_t stream) {
-    constexpr int DP = NG <= 2 ? 64 : 128, smem = (DP / 64) * (2 * RT * 128 + NS * 2 * KT * 128) + RAW * (2 * NG * KT * 16 + 3 * KT * NG * 4) + 1024;
+    constexpr int DP = NG <= 2 ? 64 : 128, smem = (DP / 64) * (2 * RT * 128 + NS * 2 * KT * 128) + RAW * 2 * (NG * KT * 16 + KT * NG * 4) + 1024;
     Line line;
     line.part_o = scratch;
     line.part_ml = scratch + (size_t)BLOCKS * 2 * ROWS * DP;
