@@ -1,14 +1,14 @@
 // Attention over 4-bit pages for many rows of a key/value head (portions of prompts, bfloat16) on the 5th-generation tensor cores
 // (cache4_attention.cu says what is computed).
 //
-// A job is (request, key/value head, up to two tiles of 128 rows): the rows are (token, query head of the group) pairs.  Eight warps take tiles of 64
-// keys (8..11) and values (12..15) out of their codes, once for the 256 rows, into operands in shared memory (128-byte swizzle); S = Q K^T is
-// issued by warp 8, P = 2^(S - m) formed by a thread per row in warps 0..3 and 4..7, in the tensor memory of S, O += P V issued by warp 12.
+// A job is (request, key/value head, up to two tiles of 128 rows): the rows are (token, query head of the group) pairs.  Warps 8..11 take tiles of 64
+// keys and values out of their codes, once for the 256 rows, into operands in shared memory (128-byte swizzle); S = Q K^T is issued by warp 12,
+// P = 2^(S - m) formed by a thread per row in warps 0..3 and 4..7, in the tensor memory of S, O += P V issued by warp 13.
 //
 // All operands are float16: 11 digits of m + s code and of a probability, where bfloat16's 8 would each move the result as much as its own rounding
 // does.  float16's range is made up for by powers of two that are undone in float32: one per row of Q; one for every 16 keys of a tile, by which the
-// scores are multiplied; one for the values of a job, which moves (with O, as for a new maximum) only when a tile's may be over 16 times larger
-// than the ones before.  Numbers 2^25 times smaller than the largest value lose digits.  Probabilities are held 2^6 times their size.
+// scores are multiplied; one for every 16 values, by which probabilities are multiplied, relative to the largest so far (which moves O as a new
+// maximum does).  Numbers 2^25 times smaller than the largest value lose digits.  Probabilities are held 2^6 times their size.
 // A group's word that is no number is zero in the operand; rows that see its key get no number in the group's channels at the end, the others nothing.
 //
 // The tiles of all jobs are one line cut into equal shares, one a block; parts of a job that blocks share are joined by a second kernel in their order.
@@ -23,8 +23,7 @@ using namespace xb4;
 using namespace xbtc;
 
 constexpr int RT = 128, ROWS = 2 * RT, KT = 64;
-constexpr int BLOCKS = 148, THREADS = 512, NS = 3, LEAD = NS - 1;      // tiles that codes are taken out ahead of their products
-constexpr int SOFTMAX_REGS = 168, CODE_REGS = 88;      // of 128 at launch: 2 * 168 + 2 * 88 = 4 * 128
+constexpr int BLOCKS = 148, THREADS = 576, NS = 3;
 constexpr int COST_JOB = 3;                // a job's start and end take about as long as three tiles
 constexpr float RESCALE_STEP = 8.f;
 constexpr int JOB_WORDS = 8, INFOS = 8;    // (a tile's facts are read at most NS + 2 tiles after they are written)
@@ -38,10 +37,10 @@ struct Line {
     int* jobs;                     // [blocks][2][8]: parts (0: there is no such part), block of the first, first row, rows, key/value head, request
 };
 
-// What the softmax needs to know of a tile of keys, and of its values.
+// What the softmax needs to know of a tile's keys and values.
 struct Info {
-    float f[4];                    // what the scores of every 16 keys are multiplied by,
-    float v_back;                  // and what is formed of its values
+    float k_back[4];               // what the scores of every 16 keys are multiplied by,
+    float v_back[4];               // and what comes of every 16 values
     unsigned short there[4];       // keys that lie in a page
     unsigned short odd[4];         // keys whose values have a group that is no number,
     unsigned char groups[KT];      // and which groups
@@ -181,6 +180,16 @@ __device__ __forceinline__ void commit(uint32_t one, uint32_t bar) {
 __device__ __forceinline__ uint32_t idesc_f16(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
 
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* err) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, true)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ void tmem_st16_u(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float d;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -205,6 +214,7 @@ __device__ __forceinline__ void store16(uint32_t at, uint32_t a, uint32_t b, uin
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 __device__ __forceinline__ bool half_not_finite(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
+__device__ __forceinline__ int exponent_of(float power) { return (int)(__float_as_uint(power) >> 23) - 127; }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }       // -126 <= e <= 127
 
 // Copies of a key's words to shared memory, and from there.
@@ -234,9 +244,6 @@ __device__ __forceinline__ void store_word(uint32_t at, uint32_t c, uint32_t s2,
     // (they come as 0 4, 1 5, 2 6, 3 7)
     store16(at, __byte_perm(a, b, 0x5410), __byte_perm(x, y, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(x, y, 0x7632));
 }
-// What a group's numbers stay below in size; nothing if it is no number.
-__device__ __forceinline__ float most_of(uint32_t word) { return half_not_finite(word) ? 0.f : fmaf(15.f, fabsf(scale_of(word)), fabsf(least_of(word))); }
-
 template <int NG>
 __global__ void __launch_bounds__(THREADS, 1)
 cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2) {
@@ -277,217 +284,177 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
     const bool any = place_in_line(A, w);
     const long long page_bytes = (long long)ps * 20 * NG;
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CODE_REGS));
-        // ---- codes to operands, a quarter of a tile's keys a warp (two lanes a key: the first and the second half of its groups), and the products
-        const bool is_v = warp >= 12, leads = warp == 8 || warp == 12;
+    if (warp >= 8 && warp < 16) {
+        const bool is_v = warp >= 12;
+        const uint32_t full0 = is_v ? v_full0 : k_full0, empty0 = is_v ? v_empty0 : k_empty0, raw0 = raw_sm + (is_v ? RAW * RAW_BYTES : 0u);
+        // ---- codes to operands: a quarter of a tile's keys (warps 8..11) or values a warp, two lanes a key (the first and the second half of its groups)
         const int quarter = warp & 3, key = quarter * 16 + (lane & 15), part = lane >> 4;
         constexpr int GP = (NG + 1) / 2;           // groups of a lane, at most
-        const int n0 = part * GP, n1 = min(NG, n0 + GP);
-        const uint32_t full0 = is_v ? v_full0 : k_full0, empty0 = is_v ? v_empty0 : k_empty0, raw0 = raw_sm + (is_v ? RAW * RAW_BYTES : 0u);
-        const uint32_t one = elected(), tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
-        const uint32_t idesc_s = idesc_f16(KT), idesc_o = idesc_f16(DP) | 1u << 16;        // (V lies channel by channel along its rows)
-        const uint64_t dq0 = umma_desc(q_sm, 16, 1024), dk0 = umma_desc(kv_sm, 16, 1024), dv0 = umma_desc(kv_sm + KV_BYTES, KV_HALF, 1024);
-        int st = 0, done = 0;                      // ring stage and tiles of the codes
+        const int n0 = part * GP, n1 = min(NG, n0 + GP), quo = KT / ps, rem = KT % ps;
+        int st = 0, done = 0;                      // ring stage, tiles
         uint32_t ph = 0;
-        int out_st = 0, Th[2] = {0, 0}, I = 0, I1 = 0;     // of the products
-        uint32_t out_ph = 0;
         bool ok = any;
-        for (bool first = true; ok && next_segment(A, w, first); first = false, ++I) {
+        for (bool first = true; ok && next_segment(A, w, first); first = false) {
             const int* table = A.block_table + (long long)w.b * A.table_stride;
             const uint8_t* pages = (is_v ? A.v_cache : A.k_cache) + w.g * page_bytes;
-            const uint8_t* v_pages = A.v_cache + w.g * page_bytes;
             const int first_key = first_seen(A, w.r.first_pos + w.piece * ROWS / group);       // (pages in front of it may have been given back)
-            const int halves = w.r.nodes * group - w.piece * ROWS > RT ? 2 : 1;
-            // pages of the keys lane and lane + 32 of a tile, and the words of their values: every warp finds the same power of two for the values
-            int ids[2], asked = w.i0, slot_in = 0, slot_out = 0;       // tiles asked for, their places in the ring
-            unsigned have = 0;                                         // whether the lane's key is there, a bit a tile, the last asked for lowest
-            float most[RAW];                                           // what the values of the tiles asked for stay below, the last one first,
-            unsigned odd = 0;                                          // and their groups that are no numbers: eight bits a tile, four a key
-#pragma unroll
-            for (int i = 0; i < RAW; ++i) most[i] = 0.f;
-            auto look = [&](int it) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int k = (w.tile0 + it) * KT + lane + 32 * h;
-                    ids[h] = -1;
-                    if (it < w.i1 && k < w.r.keys && k >= first_key) {
-                        const int id = table[k / ps];
-                        if (id >= 0 && id < A.num_pages) ids[h] = id;
-                        else atomicOr(err, XB_ERR_BAD_PAGE);
-                    }
-                }
-            };
-            uint32_t vw[2][NG];
+            // the lane's key: its place in the table and in its page, kept up by sums
+            int k = (w.tile0 + w.i0) * KT + key, at = k / ps, slot = k % ps, asked = w.i0, slot_in = 0, slot_out = 0;       // tiles asked for, their places in the ring
+            unsigned have = 0;                     // whether the key is there, a bit a tile, the last asked for lowest
+            auto look = [&]() { return asked < w.i1 && k < w.r.keys && k >= first_key ? table[at] : -1; };
+            int id = look();
             auto ask = [&]() {
-                const int id = __shfl_sync(0xffffffffu, quarter & 2 ? ids[1] : ids[0], (quarter & 1) * 16 + (lane & 15));
-                have = have << 1 | (id >= 0 ? 1u : 0u);
-                if (id >= 0) {
-                    const int slot = ((w.tile0 + asked) * KT + key) % ps;
+                const bool there = id >= 0 && id < A.num_pages;
+                if (!there && asked < w.i1 && k < w.r.keys && k >= first_key) atomicOr(err, XB_ERR_BAD_PAGE);
+                have = have << 1 | (there ? 1u : 0u);
+                if (there) {
                     const uint32_t to = raw0 + slot_in * RAW_BYTES;
-                    const uint8_t* page = pages + (long long)id * A.nkv * page_bytes;
-                    for (int n = n0; n < n1; ++n)
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to + (n * KT + key) * 16), "l"(page + ((long long)n * ps + slot) * 16) : "memory");
-                    if (part == 0) copy_words<NG>(to + RAW_CODES + key * NG * 4, page + (long long)ps * 16 * NG + slot * NG * 4);
+                    const uint8_t* from = pages + (long long)id * A.nkv * page_bytes;
+#pragma unroll
+                    for (int g = 0; g < GP; ++g)
+                        if (n0 + g < n1)
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to + ((n0 + g) * KT + key) * 16), "l"(from + ((n0 + g) * ps + slot) * 16) : "memory");
+                    if (part == 0) copy_words<NG>(to + RAW_CODES + key * NG * 4, from + ps * 16 * NG + slot * NG * 4);
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int k = (w.tile0 + asked) * KT + lane + 32 * h;
-#pragma unroll
-                    for (int n = 0; n < NG; ++n) vw[h][n] = 0u;
-                    if (ids[h] >= 0) {
-                        const uint32_t* from = reinterpret_cast<const uint32_t*>(v_pages + (long long)ids[h] * A.nkv * page_bytes + (long long)ps * 16 * NG + k % ps * NG * 4);
-                        if constexpr (NG == 4) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(from);
-                            vw[h][0] = v.x, vw[h][1] = v.y, vw[h][2] = v.z, vw[h][3] = v.w;
-                        } else {
-#pragma unroll
-                            for (int n = 0; n < NG; ++n) vw[h][n] = from[n];
-                        }
-                    }
-                }
+                k += KT;
+                slot += rem;
+                at += quo;
+                if (slot >= ps) slot -= ps, ++at;
                 ++asked;
                 slot_in = slot_in + 1 == RAW ? 0 : slot_in + 1;
-                look(asked);
+                id = look();
             };
-            auto shift_most = [&]() {              // (the words of the tile asked for last have come by now)
-                float m = 0.f;
-                odd <<= 8;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int n = 0; n < NG; ++n) {
-                        m = fmaxf(m, most_of(vw[h][n]));
-                        if (half_not_finite(vw[h][n])) odd |= 1u << (4 * h + n);
-                    }
-#pragma unroll
-                for (int i = RAW - 1; i > 0; --i) most[i] = most[i - 1];
-                most[0] = m;
-            };
-            look(asked);
-#pragma unroll
-            for (int i = 0; i < RAW - 1; ++i) {
+            for (int i = 0; i < RAW - 1; ++i) ask();
+            for (int it = w.i0; it < w.i1; ++it) {
                 ask();
-                shift_most();
-            }
-            int v_expo = 0;                        // the values' power of two: their largest lies below 2^(v_expo - 126)
-            float v_down = 1.f, v_back = 1.f;
-            const int tiles = w.i1 - w.i0;
-            for (int step = 0; step < tiles + (leads ? LEAD : 0); ++step) {
-                if (step < tiles) {
-                    ask();
-                    asm volatile("cp.async.wait_group %0;" ::"n"(RAW - 1) : "memory");
-                    __syncwarp();
-                    const bool there = have >> (RAW - 1) & 1u;
-                    const uint32_t raw = raw0 + slot_out * RAW_BYTES;
-                    slot_out = slot_out + 1 == RAW ? 0 : slot_out + 1;
-                    uint32_t words[NG];
-                    load_words<NG>(raw + RAW_CODES + key * NG * 4, words);
+                asm volatile("cp.async.wait_group %0;" ::"n"(RAW - 1) : "memory");
+                __syncwarp();
+                const bool there = have >> (RAW - 1) & 1u;
+                const uint32_t raw = raw0 + slot_out * RAW_BYTES;
+                slot_out = slot_out + 1 == RAW ? 0 : slot_out + 1;
+                uint32_t words[NG];
+                load_words<NG>(raw + RAW_CODES + key * NG * 4, words);
+                // the power of two that brings the largest number that these 16 keys or values can hold below 2^15
+                float top = 0.f;
+                unsigned odd = 0;
 #pragma unroll
-                    for (int n = 0; n < NG; ++n)
-                        if (!there) words[n] = 0u;
-                    // (the tile's values were asked for RAW - 1 tiles ago)
-                    const int expo_v = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(most[RAW - 2])) >> 23);
-                    if (v_expo == 0 || expo_v > v_expo + 4) {
-                        v_expo = max(expo_v, 1);
-                        const int e = min(137 - v_expo, 100);          // below 2^11, so that up to 2^15 are no reason for another
-                        v_down = power_of_two(e), v_back = power_of_two(-e);
-                    }
-                    if (done >= NS && !wait_warp(empty0 + 8 * st, ph ^ 1u, err)) {
-                        ok = false;
-                        break;
-                    }
-                    float f = v_down;
-                    if (!is_v) {
-                        // the power of two that brings the largest number that these 16 keys can hold below 2^15
-                        Info& info = infos[done % INFOS];
-                        float top = 0.f;
-#pragma unroll
-                        for (int n = 0; n < NG; ++n) top = fmaxf(top, most_of(words[n]));
-                        const int expo = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), e = min(expo == 0 ? 0 : 141 - expo, 100);
-                        f = power_of_two(e);
-                        const unsigned are = __ballot_sync(0xffffffffu, there);
-                        const unsigned odd_now = __shfl_sync(0xffffffffu, odd >> (8 * (RAW - 2)), (quarter & 1) * 16 + (lane & 15)) >> (2 * (quarter & 2)) & 15u;
-                        const unsigned odds = __ballot_sync(0xffffffffu, odd_now != 0);
-                        if (part == 0) info.groups[key] = (unsigned char)odd_now;
-                        if (lane == 0) info.f[quarter] = power_of_two(-e), info.there[quarter] = (unsigned short)are, info.odd[quarter] = (unsigned short)odds;
-                        if (warp == 8 && lane == 0) info.v_back = v_back;
-                    }
-                    const uint32_t row = kv_sm + st * STAGE_BYTES + (is_v ? KV_BYTES : 0u) + key * 128;
-#pragma unroll
-                    for (int g = 0; g < GP; ++g) {
-                        const int n = n0 + g;
-                        if (n < n1) {
-                            uint32_t wd = GP == 1 ? (part ? words[NG - 1] : words[0]) : (part ? words[min(GP + g, NG - 1)] : words[g]), c[4];
-                            if (is_v && half_not_finite(wd)) wd = 0;
-                            const float s = scale_of(wd) * f, m = least_of(wd) * f;
-                            const uint32_t s2 = pack_f16(s, s), m2 = pack_f16(m, m);
-                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(raw + (n * KT + key) * 16) : "memory");
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) store_word(row + (n >> 1) * KV_HALF + ((((n & 1) * 4 + i) ^ (key & 7)) << 4), c[i], s2, m2);
-                        }
-                    }
-                    shift_most();
-                    fence_async_shared();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(full0 + 8 * st);
-                    ++done;
-                    if (++st == NS) {
-                        st = 0;
-                        ph ^= 1u;
-                    }
+                for (int n = 0; n < NG; ++n) {
+                    if (!there) words[n] = 0u;
+                    const bool strange = half_not_finite(words[n]);
+                    top = fmaxf(top, strange ? 0.f : fmaf(15.f, fabsf(scale_of(words[n])), fabsf(least_of(words[n]))));
+                    if (strange && is_v) odd |= 1u << n, words[n] = 0u;
                 }
-                if (!leads || step < LEAD) continue;
-                // ---- the products of the tile LEAD steps back
-                if (step == LEAD && !is_v) {
-                    ok = wait_warp(q_ready0, I & 1, err);
-                    if (halves == 2) ok = wait_warp(q_ready0 + 8, I1++ & 1, err) && ok;
-                }
-                ok = ok && wait_warp(full0 + 8 * out_st, out_ph, err);
-                for (int hd = 0; hd < halves && ok; ++hd) {
-                    const int th = Th[hd]++, sb = th & 1;
-                    if (!is_v) {
-                        // these columns held the scores and then P of this half's last tile but one: its P V must have read them
-                        ok = th < 2 || wait_warp(pv_done0 + 8 * (2 * hd + sb), ((th >> 1) - 1) & 1, err);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint64_t dq = dq0 + (uint64_t)((hd * Q_ONE) >> 4), dk = dk0 + (uint64_t)((out_st * STAGE_BYTES) >> 4);
-#pragma unroll
-                        for (int kk = 0; kk < DP / 16; ++kk) {
-                            const uint32_t off = (kk >> 2), inner = (kk & 3) * 32;
-                            umma_ss(one, tmem_u + (uint32_t)(hd * 128 + sb * 64), dq + (uint64_t)((off * RT * 128 + inner) >> 4), dk + (uint64_t)((off * KV_HALF + inner) >> 4), idesc_s, kk ? 1u : 0u);
-                        }
-                        commit(one, s_ready0 + 8 * (2 * hd + sb));
-                    } else {
-                        ok = wait_warp(p_ready0 + 8 * (2 * hd + sb), (th >> 1) & 1, err);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t tp = tmem_u + (uint32_t)(hd * 128 + sb * 64);
-                        const uint64_t dv = dv0 + (uint64_t)((out_st * STAGE_BYTES) >> 4);
-#pragma unroll
-                        for (int kk = 0; kk < KT / 16; ++kk)
-                            umma_ts(one, tmem_u + (uint32_t)(256 + hd * 128), tp + (uint32_t)(kk * 8), dv + (uint64_t)((kk * 2048) >> 4), idesc_o);
-                        commit(one, pv_done0 + 8 * (2 * hd + sb));
-                    }
-                }
+                const int expo = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), e = expo == 0 ? 100 : min(141 - expo, 100);
+                const float f = power_of_two(e);
+                const unsigned bits = __ballot_sync(0xffffffffu, is_v ? odd != 0 : there);
+                if (done >= NS) ok = wait_warp(empty0 + 8 * st, ph ^ 1u, err);
                 if (!ok) break;
-                commit(one, empty0 + 8 * out_st);
-                if (++out_st == NS) {
-                    out_st = 0;
-                    out_ph ^= 1u;
+                Info& info = infos[done % INFOS];
+                if (lane == 0) (is_v ? info.v_back : info.k_back)[quarter] = power_of_two(-e), (is_v ? info.odd : info.there)[quarter] = (unsigned short)bits;
+                if (is_v && bits && part == 0) info.groups[key] = (unsigned char)odd;
+                const uint32_t row = kv_sm + st * STAGE_BYTES + (is_v ? KV_BYTES : 0u) + key * 128;
+#pragma unroll
+                for (int g = 0; g < GP; ++g) {
+                    const int n = n0 + g;
+                    if (n < n1) {
+                        const uint32_t wd = part ? words[min(GP + g, NG - 1)] : words[g];
+                        uint32_t c[4];
+                        const float sc = scale_of(wd) * f, m = least_of(wd) * f;
+                        const uint32_t s2 = pack_f16(sc, sc), m2 = pack_f16(m, m);
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(raw + (n * KT + key) * 16) : "memory");
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) store_word(row + (n >> 1) * KV_HALF + ((((n & 1) * 4 + i) ^ (key & 7)) << 4), c[i], s2, m2);
+                    }
+                }
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full0 + 8 * st);
+                ++done;
+                if (++st == NS) {
+                    st = 0;
+                    ph ^= 1u;
                 }
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncwarp();
         }
-        if (leads) {                               // no product is at work when the tensor memory is freed, however the block ends
-            commit(one, drained0 + (is_v ? 8 : 0));
-            wait_warp(drained0 + (is_v ? 8 : 0), 0, err);
+    } else if (warp == 16) {
+        // ---- S = Q K^T of every tile
+        const uint32_t one = elected(), tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint32_t idesc = idesc_f16(KT);
+        const uint64_t dq0 = umma_desc(q_sm, 16, 1024), dk0 = umma_desc(kv_sm, 16, 1024);
+        int st = 0, Th[2] = {0, 0}, I = 0, I1 = 0;
+        uint32_t ph = 0;
+        bool ok = any;
+        for (bool first = true; ok && next_segment(A, w, first); first = false, ++I) {
+            const int halves = w.r.nodes * group - w.piece * ROWS > RT ? 2 : 1;
+            ok = wait_warp(q_ready0, I & 1, err);
+            if (halves == 2) ok = ok && wait_warp(q_ready0 + 8, I1++ & 1, err);
+            for (int it = w.i0; it < w.i1 && ok; ++it) {
+                ok = wait_warp(k_full0 + 8 * st, ph, err);
+                const uint64_t dk = dk0 + (uint64_t)((st * STAGE_BYTES) >> 4);
+                for (int hd = 0; hd < halves && ok; ++hd) {
+                    const int th = Th[hd]++, sb = th & 1;
+                    // these columns held the scores and then P of this half's last tile but one: its P V must have read them
+                    ok = th < 2 || wait_warp(pv_done0 + 8 * (2 * hd + sb), ((th >> 1) - 1) & 1, err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t dq = dq0 + (uint64_t)((hd * Q_ONE) >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < DP / 16; ++kk) {
+                        const uint32_t off = (kk >> 2), inner = (kk & 3) * 32;
+                        umma_ss(one, tmem_u + (uint32_t)(hd * 128 + sb * 64), dq + (uint64_t)((off * RT * 128 + inner) >> 4), dk + (uint64_t)((off * KV_HALF + inner) >> 4), idesc, kk ? 1u : 0u);
+                    }
+                    commit(one, s_ready0 + 8 * (2 * hd + sb));
+                }
+                if (!ok) break;
+                commit(one, k_empty0 + 8 * st);
+                if (++st == NS) {
+                    st = 0;
+                    ph ^= 1u;
+                }
+            }
         }
+        commit(one, drained0);                   // no product is at work when the tensor memory is freed, however the block ends
+        wait_warp(drained0, 0, err);
+    } else if (warp == 17) {
+        // ---- O += P V of every tile (O starts as zeros, by the softmax threads)
+        const uint32_t one = elected(), tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint32_t idesc = idesc_f16(DP) | 1u << 16;       // V lies channel by channel along its rows
+        const uint64_t dv0 = umma_desc(kv_sm + KV_BYTES, KV_HALF, 1024);
+        int st = 0, Th[2] = {0, 0};
+        uint32_t ph = 0;
+        bool ok = any;
+        for (bool first = true; ok && next_segment(A, w, first); first = false) {
+            const int halves = w.r.nodes * group - w.piece * ROWS > RT ? 2 : 1;
+            for (int it = w.i0; it < w.i1 && ok; ++it) {
+                ok = wait_warp(v_full0 + 8 * st, ph, err);
+                const uint64_t dv = dv0 + (uint64_t)((st * STAGE_BYTES) >> 4);
+                for (int hd = 0; hd < halves && ok; ++hd) {
+                    const int th = Th[hd]++, sb = th & 1;
+                    ok = wait_warp(p_ready0 + 8 * (2 * hd + sb), (th >> 1) & 1, err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t tp = tmem_u + (uint32_t)(hd * 128 + sb * 64);
+#pragma unroll
+                    for (int kk = 0; kk < KT / 16; ++kk)
+                        umma_ts(one, tmem_u + (uint32_t)(256 + hd * 128), tp + (uint32_t)(kk * 8), dv + (uint64_t)((kk * 2048) >> 4), idesc);
+                    commit(one, pv_done0 + 8 * (2 * hd + sb));
+                }
+                if (!ok) break;
+                commit(one, v_empty0 + 8 * st);
+                if (++st == NS) {
+                    st = 0;
+                    ph ^= 1u;
+                }
+            }
+        }
+        commit(one, drained0 + 8);
+        wait_warp(drained0 + 8, 0, err);
     } else {
         // ---- softmax: a row per thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
         const int hd = warp >> 2, r = (int)threadIdx.x & 127;
         const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tmem_s = tmem + (uint32_t)(hd * 128) + lane_addr, tmem_o = tmem + (uint32_t)(256 + hd * 128) + lane_addr;
@@ -554,7 +521,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_ready0 + 8 * hd);
             }
-            float m_ref = -INFINITY, l = 0.f, v_back = 0.f;
+            float m_ref = -INFINITY, l = 0.f, v_back = 0.f, v_down = 0.f;
             unsigned poison = 0;                 // groups of channels that are no number
             // keys from all0 on and below all1 are seen by all rows of the job
             const int pos0 = w.r.first_pos + row0 / group, pos1 = w.r.first_pos + (row0 + rows - 1) / group;
@@ -567,50 +534,56 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                 }
                 tc_fence_after();
                 const volatile Info& info = infos[(T + it - w.i0) % INFOS];
-                float sc[64];
-                {
-                    uint32_t ra[32], rb[32];
-                    tmem_ld32_nowait(tmem_s + sb * 64, ra);
-                    tmem_ld32_nowait(tmem_s + sb * 64 + 32, rb);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        sc[i] = __uint_as_float(ra[i]);
-                        sc[32 + i] = __uint_as_float(rb[i]);
-                    }
+                const int vst = (T + it - w.i0) % NS;
+                if (!wait_warp(v_full0 + 8 * vst, ((T + it - w.i0) / NS) & 1, err)) {      // (what is known of the values)
+                    alive = false;
+                    break;
                 }
-                const float v_now = info.v_back;
                 const unsigned t0 = info.there[0] | (unsigned)info.there[1] << 16, t1 = info.there[2] | (unsigned)info.there[3] << 16;
                 const unsigned o0 = info.odd[0] | (unsigned)info.odd[1] << 16, o1 = info.odd[2] | (unsigned)info.odd[3] << 16;
-                float cf[4];                     // (a sum of zero stays one, and one of a key that is not seen)
+                float cf[4], vf[4], v_most = v_back;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) cf[i] = fminf(fmaxf(c1 * info.f[i], 1.2e-38f), 3.0e38f);
+                for (int i = 0; i < 4; ++i) {
+                    cf[i] = fminf(fmaxf(c1 * info.k_back[i], 1.2e-38f), 3.0e38f);          // (a sum of zero stays one, and one of a key that is not seen)
+                    vf[i] = info.v_back[i];
+                    v_most = fmaxf(v_most, vf[i]);
+                }
                 const bool edge = key0 < all0 || key0 + KT > all1 || (t0 & t1) != 0xffffffffu || (o0 | o1);
-                bool dead3 = false;              // (keys that are not seen have no weight at all, by the polynomial either)
                 unsigned long long seen = ~0ull;
                 if (edge) {
                     seen = (unsigned long long)t1 << 32 | t0;
                     if (hi - key0 < 64) seen &= hi > key0 ? (1ull << (hi - key0)) - 1 : 0ull;
                     if (lo > key0) seen = lo - key0 < 64 ? seen & (~0ull << (lo - key0)) : 0ull;
-#pragma unroll
-                    for (int i = 0; i < 64; ++i) sc[i] = (seen >> i & 1ull) ? sc[i] : -INFINITY;
-                    dead3 = true;
                     unsigned long long odd = ((unsigned long long)o1 << 32 | o0) & seen;
                     while (odd) {
                         poison |= info.groups[__ffsll((long long)odd) - 1];
                         odd &= odd - 1;
                     }
                 }
+                // twice over the scores, 32 at a time, so that they need not stay in registers: the largest, then the exponentials
+                auto scores = [&](int half, float (&sc)[32]) {
+                    tmem_ld32(tmem_s + sb * 64 + half * 32, sc);
+                    if (edge) {
+                        const unsigned mine = (unsigned)(seen >> (32 * half));
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sc[i] = (mine >> i & 1u) ? sc[i] : -INFINITY;
+                    }
+                };
                 float top = -INFINITY;
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    float m2[2] = {-INFINITY, -INFINITY};
+                for (int half = 0; half < 2; ++half) {
+                    float sc[32];
+                    scores(half, sc);
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        m2[0] = max3_nan(m2[0], sc[h * 16 + i], sc[h * 16 + i + 1]);
-                        m2[1] = max3_nan(m2[1], sc[h * 16 + i + 2], sc[h * 16 + i + 3]);
+                    for (int h = 0; h < 2; ++h) {
+                        float m2[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            m2[0] = max3_nan(m2[0], sc[h * 16 + i], sc[h * 16 + i + 1]);
+                            m2[1] = max3_nan(m2[1], sc[h * 16 + i + 2], sc[h * 16 + i + 3]);
+                        }
+                        top = max_nan(top, max_nan(m2[0], m2[1]) * cf[2 * half + h]);
                     }
-                    top = max_nan(top, max_nan(m2[0], m2[1]) * cf[h]);
                 }
                 float corr = 1.f;
                 bool moved = false;
@@ -620,40 +593,45 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                     m_ref = top;
                 }
                 float f_o = corr;                // O's part: it is also in another power of two from now on
-                if (v_now != v_back) {           // (the same for all)
-                    if (v_back != 0.f) f_o *= v_back / v_now, moved = true;
-                    v_back = v_now;
+                if (v_most != v_back) {          // (the same for all)
+                    if (v_back != 0.f) f_o *= v_back * power_of_two(-exponent_of(v_most)), moved = true;
+                    v_back = v_most;
+                    v_down = power_of_two(-exponent_of(v_most));
                 }
                 const float m_neg = m_ref == -INFINITY ? 0.f : P_UP - m_ref;
                 const f32x2 mneg2 = pack2(m_neg, m_neg);
                 f32x2 sum_a = pack2(0.f, 0.f), sum_b = pack2(0.f, 0.f);
-                uint32_t pk[32];
 #pragma unroll
-                for (int c8 = 0; c8 < 8; ++c8) {
-                    const f32x2 scale2 = pack2(cf[c8 / 2], cf[c8 / 2]);
-                    float x[8], e[8];
+                for (int half = 0; half < 2; ++half) {
+                    float sc[32];
+                    uint32_t pk[16];
+                    scores(half, sc);
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2) unpack2(fma2(pack2(sc[c8 * 8 + i], sc[c8 * 8 + i + 1]), scale2, mneg2), x[i], x[i + 1]);
+                    for (int c8 = 0; c8 < 4; ++c8) {
+                        const f32x2 scale2 = pack2(cf[2 * half + c8 / 2], cf[2 * half + c8 / 2]);
+                        const float of_v = vf[2 * half + c8 / 2] * v_down;
+                        float e[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if ((i & 3) != 3) e[i] = ex2(x[i]);
-                    ex2_poly2(x[3], x[7], e[3], e[7]);
-                    if (dead3) {
-                        if (x[3] == -INFINITY) e[3] = 0.f;
-                        if (x[7] == -INFINITY) e[7] = 0.f;
+                        for (int i = 0; i < 8; i += 2) {
+                            float x0, x1;
+                            unpack2(fma2(pack2(sc[c8 * 8 + i], sc[c8 * 8 + i + 1]), scale2, mneg2), x0, x1);
+                            e[i] = ex2(x0), e[i + 1] = ex2(x1);
+                        }
+                        sum_a = add2(sum_a, add2(pack2(e[0], e[1]), pack2(e[2], e[3])));
+                        sum_b = add2(sum_b, add2(pack2(e[4], e[5]), pack2(e[6], e[7])));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float p0, p1;
+                            unpack2(mul2(pack2(e[2 * i], e[2 * i + 1]), pack2(of_v, of_v)), p0, p1);
+                            pk[c8 * 4 + i] = pack_f16(p0, p1);
+                        }
                     }
-                    sum_a = add2(sum_a, add2(pack2(e[0], e[1]), pack2(e[2], e[3])));
-                    sum_b = add2(sum_b, add2(pack2(e[4], e[5]), pack2(e[6], e[7])));
-                    pk[c8 * 4] = pack_f16(e[0], e[1]);
-                    pk[c8 * 4 + 1] = pack_f16(e[2], e[3]);
-                    pk[c8 * 4 + 2] = pack_f16(e[4], e[5]);
-                    pk[c8 * 4 + 3] = pack_f16(e[6], e[7]);
+                    tmem_st16_u(tmem_s + sb * 64 + half * 16, pk);       // P goes where scores were that have been read
                 }
                 float s0, s1, s2, s3;
                 unpack2(sum_a, s0, s1);
                 unpack2(sum_b, s2, s3);
                 l = l * corr + ((s0 + s1) + (s2 + s3));
-                tmem_st32_u(tmem_s + sb * 64, pk);                       // P goes where the scores were
                 // O is touched only when the last tile's P V has completed
                 if (__any_sync(0xffffffffu, moved)) {
                     if (it > w.i0 && !wait_warp(my_pv_done + 8 * (sb ^ 1), ((Th - 1) >> 1) & 1, err)) {
