@@ -241,15 +241,16 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
         const uint8_t* v_pages = A.v_cache + w.g * page_bytes;
 
         // ---- fetching: a stage holds two steps, each its keys' codes as [group][key][16 bytes] and words as [key][group], then its values'
-        int ids = -1, ids_from = -1, put = from;           // a lane holds the page of one of 32 pieces (keys that lie in one page),
+        long long page_at = 0;                             // a lane holds the place of one of 32 pieces' pages (pieces: keys that lie in one page),
         unsigned have = 0;                                 // and this which of them there are
+        int ids_from = -1, put = from;
         unsigned none_of = 0;                              // eight bits a stage, the last one lowest: pieces without a page
         auto issue = [&]() {
             const int shift = by16 ? 0 : 1, at = (put - from) << shift, in_use = min(STAGE_STEPS, to - put) << shift;
             if ((at & ~31) != ids_from) {
                 ids_from = at & ~31;
                 const int key = (from << 4) + ((ids_from + lane) << (4 - shift));
-                ids = -1;
+                int ids = -1;
                 // (pieces in front of the first row's window: their pages may have been given back)
                 if (key < to * STEP && key < w.r.keys && key + (STEP >> shift) > first_key) {
                     ids = table[key / ps];
@@ -259,6 +260,7 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
                     }
                 }
                 have = __ballot_sync(0xffffffffu, ids >= 0);
+                page_at = (long long)ids * A.nkv * page_bytes;
             }
             const uint32_t bar = bars + 8 * put_slot, dst = ring + put_slot * STAGE;
             // piece i of the stage is lane (at & 31) + i of ids
@@ -267,17 +269,17 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
             if (lane == 0) xbtc::mbar_expect_tx(bar, __popc(there) * (by16 ? 2 * HALF : HALF));
             __syncwarp();
             if (ps == STEP) {                              // whole pages
-                const int id = __shfl_sync(0xffffffffu, ids, (at & 31) + (lane >> 1 & 1));
-                if (lane < 4 && (there >> (lane >> 1) & 1))
-                    bulk_copy(dst + lane * HALF, (lane & 1 ? v_pages : k_pages) + (long long)id * A.nkv * page_bytes, HALF, bar);
+                const long long page = __shfl_sync(0xffffffffu, page_at, (at & 31) + (lane >> 1 & 1));
+                if (lane < 4 && (there >> (lane >> 1) & 1)) bulk_copy(dst + lane * HALF, (lane & 1 ? v_pages : k_pages) + page, HALF, bar);
             } else {
                 const int each = 2 * (NG + 1), keys = by16 ? STEP : STEP / 2;      // copies of a piece
 #pragma unroll 1
                 for (int i = lane; i < ((in_use * each + 31) & ~31); i += 32) {
-                    const int piece = min(i / each, 3), n = i % each % (NG + 1), v = i % each / (NG + 1), id = __shfl_sync(0xffffffffu, ids, (at & 31) + piece);
+                    const int piece = min(i / each, 3), n = i % each % (NG + 1), v = i % each / (NG + 1);
+                    const long long page = __shfl_sync(0xffffffffu, page_at, (at & 31) + piece);
                     if (i >= in_use * each || !(there >> piece & 1)) continue;
                     const int key = put * STEP + piece * keys, slot = key % ps, half = by16 ? 0 : piece & 1;
-                    const uint8_t* src = (v ? v_pages : k_pages) + (long long)id * A.nkv * page_bytes;
+                    const uint8_t* src = (v ? v_pages : k_pages) + page;
                     src += n < NG ? ((long long)n * ps + slot) * 16 : (long long)ps * 16 * NG + slot * NG * 4;
                     const uint32_t to_smem = dst + (2 * (piece >> shift) + v) * HALF + (n < NG ? n * STEP * 16 + half * 128 : CODES + half * 8 * NG * 4);
                     bulk_copy(to_smem, src, n < NG ? keys * 16 : keys * NG * 4, bar);

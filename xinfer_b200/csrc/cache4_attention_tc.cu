@@ -24,7 +24,7 @@ using namespace xbtc;
 
 constexpr int RT = 128, ROWS = 2 * RT, KT = 64;
 constexpr int BLOCKS = 148, THREADS = 576, NS = 3;
-constexpr int COST_JOB = 3;                // a job's start and end take about as long as three tiles
+constexpr int COST_JOB = 6;                // a job's start and end take about as long as six tiles
 constexpr float RESCALE_STEP = 8.f;
 constexpr int JOB_WORDS = 8, INFOS = 8;    // (a tile's facts are read at most NS + 2 tiles after they are written)
 constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
@@ -32,13 +32,13 @@ constexpr float P_UP = 6.f;
 constexpr int RAW = 3;                     // tiles whose codes are on their way
 
 struct Line {
-    float* part_o;                 // [blocks][2][256][DP]: a block's first segment, if its job began before it, and its last, if its job goes on
+    float* part_o;                 // [blocks][2][DP / 4][256][4]: a block's first segment, if its job began before it, and its last, if its job goes on
     float* part_ml;                // [blocks][2][256][2]
     int* jobs;                     // [blocks][2][8]: parts (0: there is no such part), block of the first, first row, rows, key/value head, request
 };
 
 // What the softmax needs to know of a tile's keys and values.
-struct Info {
+struct __align__(16) Info {
     float k_back[4];               // what the scores of every 16 keys are multiplied by,
     float v_back[4];               // and what comes of every 16 values
     unsigned short there[4];       // keys that lie in a page
@@ -54,25 +54,40 @@ struct Walk {
     int i0, i1;
 };
 
-// First row, keys and tiles of a request's piece of rows.
+// Keys and tiles of a request's piece of rows, from the places of its first and its last token.
+__device__ __forceinline__ void set_tiles(const AttendArgs& A, Walk& w, int node0, int node1) {
+    w.tile0 = first_seen(A, w.r.first_pos + node0) / KT;
+    w.tiles = max(1, (min(w.r.first_pos + node1 + 1, w.r.keys) + KT - 1) / KT - w.tile0);       // (rows that see no key are written all the same)
+}
 __device__ __forceinline__ void set_piece(const AttendArgs& A, Walk& w) {
-    const int group = A.nh / A.nkv, row0 = w.piece * ROWS, rows = min(ROWS, w.r.nodes * group - row0);
-    const int pos0 = w.r.first_pos + row0 / group, pos1 = w.r.first_pos + (row0 + rows - 1) / group;
-    w.tile0 = first_seen(A, pos0) / KT;
-    w.tiles = max(1, (min(pos1 + 1, w.r.keys) + KT - 1) / KT - w.tile0);       // (rows that see no key are written all the same)
+    const int group = A.nh / A.nkv, row0 = w.piece * ROWS;
+    set_tiles(A, w, row0 / group, min(w.r.nodes - 1, (row0 + ROWS - 1) / group));
 }
 __device__ __forceinline__ void set_request(const AttendArgs& A, Walk& w, int b) {
     w.b = b;
     w.r = request_of(A, b);
     w.pieces = (w.r.nodes * (A.nh / A.nkv) + ROWS - 1) / ROWS;
 }
-__device__ __forceinline__ int head_units(const AttendArgs& A, Walk& w) {
-    int sum = 0;
+// The pieces one after another, until `f(piece)` is true: their tokens' places by sums.
+template <typename F>
+__device__ __forceinline__ void each_piece(const AttendArgs& A, Walk& w, F f) {
+    const int group = A.nh / A.nkv, quo = ROWS / group, rem = ROWS % group;
+    int node = 0, over = 0;        // (256 * piece) / group and the remainder
 #pragma unroll 1
     for (w.piece = 0; w.piece < w.pieces; ++w.piece) {
-        set_piece(A, w);
-        sum += w.tiles + COST_JOB;
+        int next = node + quo, left = over + rem;
+        if (left >= group) left -= group, ++next;
+        set_tiles(A, w, node, min(w.r.nodes - 1, left == 0 ? next - 1 : next));        // (the last row is one before the next piece's first)
+        if (f()) return;
+        node = next, over = left;
     }
+}
+__device__ __forceinline__ int head_units(const AttendArgs& A, Walk& w) {
+    int sum = 0;
+    each_piece(A, w, [&]() {
+        sum += w.tiles + COST_JOB;
+        return false;
+    });
     return sum;
 }
 
@@ -111,11 +126,11 @@ __device__ __forceinline__ bool place_in_line(const AttendArgs& A, Walk& w) {
     const int units = head_units(A, w);
     w.g = (w.from - before) / units;
     w.job = before + w.g * units;
-    for (w.piece = 0;; ++w.piece) {
-        set_piece(A, w);
-        if (w.from < w.job + w.tiles + COST_JOB) break;
+    each_piece(A, w, [&]() {
+        if (w.from < w.job + w.tiles + COST_JOB) return true;
         w.job += w.tiles + COST_JOB;
-    }
+        return false;
+    });
     return true;
 }
 
@@ -477,39 +492,55 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
             // Q: the last tile's scores of the last segment are there, so nothing reads what lies there
             float c1;
             {
-                const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(A.q) + t * A.q_stride + (long long)head * A.d;
-                auto load = [&](int c, float (&x)[8]) {
-                    if (q16 && c + 8 <= A.d) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(q + c);
-                        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+                // (VPR lanes have a row, eight channels each, so that lanes read what lies together; eight trips are on their way at a time)
+                constexpr int VPR = DP / 8, RPI = 32 / VPR, TRIPS = 32 / RPI;
+                const int c = (lane % VPR) * 8, sub = lane / VPR, warp_row = hd * RT + (warp & 3) * 32;
+                int e2 = 0, of = row0 + min(warp_row + sub, rows - 1), token = of / group, of_head = of - token * group;
+                const int last = row0 + rows - 1;
+#pragma unroll 1
+                for (int i0 = 0; i0 < TRIPS; i0 += 8) {
+                    uint4 u[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16);
-                    } else {
+                    for (int i = 0; i < 8; ++i) {
+                        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(A.q) + (w.r.first + token) * A.q_stride + (long long)(w.g * group + of_head) * A.d;
+                        for (int j = 0; j < RPI && of < last; ++j) {       // (rows behind the last repeat it)
+                            ++of;
+                            if (++of_head == group) of_head = 0, ++token;
+                        }
+                        uint32_t x[4] = {0, 0, 0, 0};
+                        if (q16) {
+                            if (c < A.d) {
+                                const uint4 v = *reinterpret_cast<const uint4*>(q + c);
+                                x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+                            }
+                        } else {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = c + e < A.d ? __bfloat162float(q[c + e]) : 0.f;
+                            for (int e = 0; e < 8; ++e)
+                                if (c + e < A.d) x[e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(q)[c + e] << (16 * (e & 1));
+                        }
+                        u[i] = make_uint4(x[0], x[1], x[2], x[3]);
                     }
-                };
-                float top = 0.f;
-#pragma unroll 4
-                for (int c = 0; c < DP; c += 8) {
-                    float x[8];
-                    load(c, x);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(x[e]));
-                }
-                // the power of two that brings the row's largest number to 2^13 .. 2^14
-                const int expo = (int)(__float_as_uint(top) >> 23), e2 = expo < 255 && expo > 0 ? 140 - expo : 0;
-                const float f1 = power_of_two(e2 / 2), f2 = power_of_two(e2 - e2 / 2);
-                c1 = scale_log2 / f1 / f2;
-#pragma unroll 2
-                for (int c = 0; c < DP; c += 8) {
-                    float x[8];
-                    load(c, x);
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t x[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+                        float top = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = x[e] * f1 * f2;
-                    store16(q_sm + hd * Q_ONE + (c >> 6) * (RT * 128) + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4), pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]),
-                            pack_f16(x[6], x[7]));
+                        for (int e = 0; e < 4; ++e) top = max3_nan(top, fabsf(scale_of(x[e])), fabsf(least_of(x[e])));
+#pragma unroll
+                        for (int o = 1; o < VPR; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        // the power of two that brings the row's largest number to 2^13 .. 2^14
+                        const int expo = (int)(__float_as_uint(top) >> 23), e = expo < 255 && expo > 0 ? 140 - expo : 0;
+                        const float f1 = power_of_two(e / 2), f2 = power_of_two(e - e / 2);
+                        uint32_t y[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) y[j] = pack_f16(scale_of(x[j]) * f1 * f2, least_of(x[j]) * f1 * f2);
+                        const int to = (warp & 3) * 32 + (i0 + i) * RPI + sub;
+                        store16(q_sm + hd * Q_ONE + (c >> 6) * (RT * 128) + to * 128 + ((((c >> 3) & 7) ^ (to & 7)) << 4), y[0], y[1], y[2], y[3]);
+                        const int mine = __shfl_sync(0xffffffffu, e, (lane % RPI) * VPR);          // of the row of this trip that the lane may have
+                        if (lane / RPI == i0 + i) e2 = mine;
+                    }
                 }
+                c1 = scale_log2 * power_of_two(-(e2 / 2)) * power_of_two(-(e2 - e2 / 2));
                 float zero[32];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) zero[i] = 0.f;
@@ -533,19 +564,20 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                     break;
                 }
                 tc_fence_after();
-                const volatile Info& info = infos[(T + it - w.i0) % INFOS];
                 const int vst = (T + it - w.i0) % NS;
                 if (!wait_warp(v_full0 + 8 * vst, ((T + it - w.i0) / NS) & 1, err)) {      // (what is known of the values)
                     alive = false;
                     break;
                 }
-                const unsigned t0 = info.there[0] | (unsigned)info.there[1] << 16, t1 = info.there[2] | (unsigned)info.there[3] << 16;
-                const unsigned o0 = info.odd[0] | (unsigned)info.odd[1] << 16, o1 = info.odd[2] | (unsigned)info.odd[3] << 16;
+                const uint32_t info_at = smem_u32(&infos[(T + it - w.i0) % INFOS]);
                 float cf[4], vf[4], v_most = v_back;
+                unsigned t0, t1, o0, o1;
+                asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(cf[0]), "=f"(cf[1]), "=f"(cf[2]), "=f"(cf[3]) : "r"(info_at) : "memory");
+                asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(vf[0]), "=f"(vf[1]), "=f"(vf[2]), "=f"(vf[3]) : "r"(info_at + 16) : "memory");
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(t0), "=r"(t1), "=r"(o0), "=r"(o1) : "r"(info_at + 32) : "memory");
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    cf[i] = fminf(fmaxf(c1 * info.k_back[i], 1.2e-38f), 3.0e38f);          // (a sum of zero stays one, and one of a key that is not seen)
-                    vf[i] = info.v_back[i];
+                    cf[i] = fminf(fmaxf(c1 * cf[i], 1.2e-38f), 3.0e38f);   // (a sum of zero stays one, and one of a key that is not seen)
                     v_most = fmaxf(v_most, vf[i]);
                 }
                 const bool edge = key0 < all0 || key0 + KT > all1 || (t0 & t1) != 0xffffffffu || (o0 | o1);
@@ -556,7 +588,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                     if (lo > key0) seen = lo - key0 < 64 ? seen & (~0ull << (lo - key0)) : 0ull;
                     unsigned long long odd = ((unsigned long long)o1 << 32 | o0) & seen;
                     while (odd) {
-                        poison |= info.groups[__ffsll((long long)odd) - 1];
+                        poison |= reinterpret_cast<volatile Info*>(infos)[(T + it - w.i0) % INFOS].groups[__ffsll((long long)odd) - 1];
                         odd &= odd - 1;
                     }
                 }
@@ -662,7 +694,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
             const bool whole = w.i0 == 0 && w.i1 == w.tiles;
             const size_t part = (size_t)blockIdx.x * 2 + (w.from > w.job ? 0 : 1);
             const float f = whole ? (l > 0.f || l != l ? v_back / l : 0.f) : v_back;
-            float* part_to = line.part_o + (part * ROWS + row) * DP;
+            float* part_to = line.part_o + (part * (DP / 4) * ROWS + row) * 4;
             __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + t * A.out_stride + (long long)head * A.d;
 #pragma unroll 1
             for (int c0 = 0; c0 < min(DP, NG * 32); c0 += 32) {
@@ -674,7 +706,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                 if (!valid) continue;
                 if (!whole) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(part_to + c0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(part_to + (size_t)(c0 + i) * ROWS) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 } else if (out16) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8)
@@ -715,10 +747,13 @@ cache4_attention_tc_join_kernel(const AttendArgs A, const Line line) {
     if (parts < 1) return;
     const int first = head.y, row0 = head.z, rows = head.w, g = job[4], group = A.nh / A.nkv;
     const Request r = request_of(A, job[5]);
-    const int mine = ((int)blockIdx.x / 2 - first) * JOIN_BLOCKS + (int)blockIdx.y, shares = parts * JOIN_BLOCKS, total = rows * FOURS;
+    // pieces of eight rows and sixteen channels, 32 lanes
+    const int mine = ((int)blockIdx.x / 2 - first) * JOIN_BLOCKS + (int)blockIdx.y, shares = parts * JOIN_BLOCKS, total = (rows + 7) / 8 * (FOURS / 4);
+    const int lane = threadIdx.x & 31;
     auto part_of = [&](int i) { return (size_t)(first + i) * 2 + (i == 0 ? 1 : 0); };     // (the first part is its block's last segment)
-    for (int i = (int)((long long)total * mine / shares) + (int)threadIdx.x; i < (int)((long long)total * (mine + 1) / shares); i += JOIN_THREADS) {
-        const int row = i / FOURS, c = i % FOURS * 4;
+    for (int i = total * mine / shares + (int)(threadIdx.x >> 5); i < total * (mine + 1) / shares; i += JOIN_THREADS / 32) {
+        const int row = i / (FOURS / 4) * 8 + (lane & 7), four = i % (FOURS / 4) * 4 + (lane >> 3), c = four * 4;
+        if (row >= rows) continue;
         float top = -INFINITY, sum = 0.f;
         for (int k = 0; k < parts; ++k) top = max_nan(top, line.part_ml[(part_of(k) * ROWS + row) * 2]);
         float4 v = {0.f, 0.f, 0.f, 0.f};
@@ -726,7 +761,7 @@ cache4_attention_tc_join_kernel(const AttendArgs A, const Line line) {
         for (int k = 0; k < parts; ++k) {
             const size_t at = part_of(k) * ROWS + row;
             const float2 ml = *reinterpret_cast<const float2*>(line.part_ml + at * 2);
-            const float4 u = *reinterpret_cast<const float4*>(line.part_o + at * DP + c);
+            const float4 u = *reinterpret_cast<const float4*>(line.part_o + ((part_of(k) * (DP / 4) + four) * ROWS + row) * 4);
             const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
             sum = fmaf(f, ml.y, sum);
             v.x = fmaf(f, u.x, v.x), v.y = fmaf(f, u.y, v.y), v.z = fmaf(f, u.z, v.z), v.w = fmaf(f, u.w, v.w);
