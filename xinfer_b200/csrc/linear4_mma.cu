@@ -6,9 +6,9 @@
 //   y += s (code . x) + m sum(x),   sum(x) by a product of the same x with ones; both in float32.
 // x may be up to 2^67 in size; below 2^-100 it loses digits.
 //
-// Bound by reading the weight once.  A block's warps and the blocks of a cluster take a range of the columns each, for R tiles of rows, whose codes they
-// fetch two stages ahead (before the kernel in front has ended: a weight is nobody's result); sums meet in shared memory, warp by warp and
-// block by block in their order.
+// Bound by reading the weight once.  A block's warps and the blocks of a cluster take a range of the columns each, for R tiles of rows at a time, and walk
+// over the rows' tiles; the codes are fetched two or four stages ahead, over the ends of the rows' tiles too (the first ones before the kernel in
+// front has ended: a weight is nobody's result).  Sums meet in shared memory, warp by warp and block by block in their order.
 #include "linear4.h"
 
 namespace {
@@ -20,14 +20,12 @@ constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u, ONES = 0x00010001u, ON
 constexpr uint32_t UP = 0x5d805d80u, UP16 = 0x5b805b80u;           // 2^60 and 2^56, twice
 constexpr float BACK = 0x1p73f;
 
-__host__ __device__ constexpr int tiles_at_once(int nt) { return nt == 1 ? 4 : 2; }
-__host__ __device__ constexpr int stages(int nt) { return nt == 1 ? 2 : 4; }
+constexpr int SLOTS = 2 * 148;             // blocks that the processors hold
+__host__ __device__ constexpr int stages(int r) { return r == 4 ? 2 : 4; }
 __host__ __device__ constexpr int tile_bytes(int per) { return TILE_CODES + TILE_ROWS * per * 4; }
-__host__ __device__ constexpr int sums_stride(int nt) { return tiles_at_once(nt) * TILE_ROWS + 4; }
-__host__ __device__ constexpr int smem_bytes(int nt, int per) {
-    const int ring = WARPS * stages(nt) * tiles_at_once(nt) * tile_bytes(per), sums = WARPS * nt * 8 * sums_stride(nt) * 4;
-    return ring > sums ? ring : sums;
-}
+__host__ __device__ constexpr int sums_stride(int r) { return r * TILE_ROWS + 4; }
+__host__ __device__ constexpr int ring_bytes(int r, int per) { return WARPS * stages(r) * r * tile_bytes(per); }
+__host__ __device__ constexpr int smem_bytes(int nt, int r, int per) { return ring_bytes(r, per) + WARPS * nt * 8 * sums_stride(r) * 4; }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -61,34 +59,45 @@ __device__ __forceinline__ float of_rank(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-template <int NT, int PER>
+template <int NT, int R, int PER>
 __global__ void __launch_bounds__(THREADS, 2)
 linear4_mma_kernel(const LinearArgs A, int cluster) {
     extern __shared__ __align__(128) char mem[];
-    constexpr int R = tiles_at_once(NT), STAGES = stages(NT), TILE = tile_bytes(PER), JOIN = 4 / PER;       // JOIN: words of a row's group
+    constexpr int STAGES = stages(R), TILE = tile_bytes(PER), JOIN = 4 / PER;       // JOIN: words of a row's group
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int row_tiles = (A.rows + TILE_ROWS - 1) / TILE_ROWS, col_tiles = (A.columns + TILE_COLS - 1) / TILE_COLS;
-    const int rank = cluster > 1 ? (int)cluster_rank() : 0, rt0 = (int)blockIdx.x / cluster * R;
-    const int parts = cluster * WARPS, part = rank * WARPS + warp;
+    const int rank = cluster > 1 ? (int)cluster_rank() : 0, parts = cluster * WARPS, part = rank * WARPS + warp;
     const int from = (int)((long long)col_tiles * part / parts), to = (int)((long long)col_tiles * (part + 1) / parts);
+    const int first = (int)blockIdx.x / cluster * R, stride = (int)gridDim.x / cluster * R;       // row tiles
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(mem) + warp * STAGES * R * TILE;
     const int t0 = blockIdx.y * NT * 8, many = min(NT * 8, A.tokens - t0);
 
-    int put = from;
+    int put = from, put_row = first, put_slot = 0, take_slot = 0;
+    const uint8_t* src[R];                                     // the next tile of each row of tiles
+    auto to_row = [&]() {
+#pragma unroll
+        for (int r = 0; r < R; ++r)                            // (behind the weight's rows: the last one's again, nobody stores what comes of them)
+            src[r] = A.weight + ((long long)min(put_row + r, row_tiles - 1) * col_tiles + from) * TILE + lane * 16;
+    };
+    to_row();
     auto fetch = [&]() {
-        if (put < to) {
+        if (put < to && put_row < row_tiles) {
+            const uint32_t dst = ring + put_slot * R * TILE + lane * 16;
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                // (tiles behind the weight's rows: the last one's again, nobody stores what comes of them)
-                const uint8_t* tile = A.weight + ((long long)min(rt0 + r, row_tiles - 1) * col_tiles + put) * TILE;
-                const uint32_t dst = ring + ((put - from) % STAGES * R + r) * TILE;
-                copy16(dst + lane * 16, tile + lane * 16);
-                copy16(dst + 512 + lane * 16, tile + 512 + lane * 16);
-                if (lane < PER * 4) copy16(dst + 1024 + lane * 16, tile + 1024 + lane * 16);
+                copy16(dst + r * TILE, src[r]);
+                copy16(dst + r * TILE + 512, src[r] + 512);
+                if (lane < PER * 4) copy16(dst + r * TILE + 1024, src[r] + 1024);
+                src[r] += TILE;
+            }
+            if (++put == to) {
+                put = from;
+                put_row += stride;
+                to_row();
             }
         }
         commit();
-        ++put;
+        put_slot = put_slot + 1 == STAGES ? 0 : put_slot + 1;
     };
 #pragma unroll
     for (int i = 0; i < STAGES; ++i) fetch();
@@ -97,32 +106,41 @@ linear4_mma_kernel(const LinearArgs A, int cluster) {
 
     const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(A.x) + t0 * A.x_stride;
     const bool on16 = ((uintptr_t)A.x & 15) == 0 && A.x_stride % 8 == 0;
-    auto load_x = [&](int token, int c) {
+    // columns c .. c + 7 of the lane's token of column tile n of the products, some of them beyond the matrix or off 16 bytes
+    auto load_x = [&](int n, int c) {
         uint32_t w[4] = {0, 0, 0, 0};
-        if (token < many) {
-            const __nv_bfloat16* row = x + token * A.x_stride;
-            if (on16 && c + 8 <= A.columns) {
-                const uint4 v = *reinterpret_cast<const uint4*>(row + c);
-                w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-            } else {
+        if (n * 8 + g < many) {
+            const uint16_t* row = reinterpret_cast<const uint16_t*>(x) + (n * 8 + g) * A.x_stride;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (c + e < A.columns) w[e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[c + e] << (16 * (e & 1));
-            }
+            for (int e = 0; e < 8; ++e)
+                if (c + e < A.columns) w[e / 2] |= (uint32_t)row[c + e] << (16 * (e & 1));
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     };
+    const uint4* x16[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) x16[n] = reinterpret_cast<const uint4*>(x + min(n * 8 + g, many - 1) * A.x_stride + t * 8);       // (columns without a token repeat the last one)
 
+    for (int rt0 = first; rt0 < row_tiles; rt0 += stride) {
     float acc[R][NT][4] = {};
     for (int ct = from; ct < to; ++ct) {
         uint4 xv[NT][4];
+        // (asked for before the codes are waited for)
+        if (on16 && (ct + 1) * TILE_COLS <= A.columns) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)                            // (asked for before the codes are waited for)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) xv[n][j] = load_x(n * 8 + g, ct * TILE_COLS + j * 32 + t * 8);
+                for (int n = 0; n < NT; ++n) xv[n][j] = x16[n][ct * (TILE_COLS / 8) + j * 4];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) xv[n][j] = load_x(n, ct * TILE_COLS + j * 32 + t * 8);
+        }
         wait_but<STAGES - 1>();
         __syncwarp();
-        const uint32_t at = ring + (ct - from) % STAGES * R * TILE;
+        const uint32_t at = ring + take_slot * R * TILE;
+        take_slot = take_slot + 1 == STAGES ? 0 : take_slot + 1;
         float d[R][NT][4], ones[NT][4];
         uint4 lo[R], hi[R];
 #pragma unroll
@@ -178,11 +196,9 @@ linear4_mma_kernel(const LinearArgs A, int cluster) {
         __syncwarp();                                          // (the stage has been read: the next codes may come)
         fetch();
     }
-    wait_but<0>();
-    __syncthreads();
     // ---- sums: [warp][token][row]
-    constexpr int STRIDE = sums_stride(NT), ROWS = R * TILE_ROWS;
-    float* sums = reinterpret_cast<float*>(mem);
+    constexpr int STRIDE = sums_stride(R), ROWS = R * TILE_ROWS;
+    float* sums = reinterpret_cast<float*>(mem + ring_bytes(R, PER));
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -200,28 +216,36 @@ linear4_mma_kernel(const LinearArgs A, int cluster) {
         if (cluster > 1) sums[token * STRIDE + row] = v;
         else if (n0 + row < A.rows) out[(t0 + token) * A.out_stride + n0 + row] = __float2bfloat16_rn(v);
     }
-    if (cluster == 1) return;
-    cluster_sync();
-    const uint32_t base = (uint32_t)__cvta_generic_to_shared(mem);
-    for (int i = total * rank / cluster + (int)threadIdx.x; i < total * (rank + 1) / cluster; i += THREADS) {
-        const int token = i / ROWS, row = i % ROWS;
-        float v = 0.f;
-        for (int k = 0; k < cluster; ++k) v += of_rank(base + (token * STRIDE + row) * 4, k);
-        if (n0 + row < A.rows) out[(t0 + token) * A.out_stride + n0 + row] = __float2bfloat16_rn(v);
+    if (cluster > 1) {
+        cluster_sync();
+        const uint32_t base = (uint32_t)__cvta_generic_to_shared(sums);
+        for (int i = total * rank / cluster + (int)threadIdx.x; i < total * (rank + 1) / cluster; i += THREADS) {
+            const int token = i / ROWS, row = i % ROWS;
+            float v = 0.f;
+            for (int k = 0; k < cluster; ++k) v += of_rank(base + (token * STRIDE + row) * 4, k);
+            if (n0 + row < A.rows) out[(t0 + token) * A.out_stride + n0 + row] = __float2bfloat16_rn(v);
+        }
+        cluster_sync();                                        // (nobody leaves, or forms other sums, while its sums are read)
+    } else {
+        __syncthreads();
     }
-    cluster_sync();                                            // (nobody leaves while its sums are read)
+    }
+    wait_but<0>();
 }
 
-template <int NT, int PER>
+template <int NT, int R, int PER>
 int launch(const LinearArgs& A, cudaStream_t stream) {
-    constexpr int R = tiles_at_once(NT), smem = smem_bytes(NT, PER);
+    constexpr int smem = smem_bytes(NT, R, PER);
     const int groups = ((A.rows + TILE_ROWS - 1) / TILE_ROWS + R - 1) / R, col_tiles = (A.columns + TILE_COLS - 1) / TILE_COLS, blocks_y = (A.tokens + NT * 8 - 1) / (NT * 8);
+    // Columns are shared out among a cluster's blocks while all blocks are on the processors at once and a warp has two tiles.  Measured with one, two,
+    // four and eight blocks: 4,096 x 4,096 (one row) 5.6, 4.9, 4.3, 7.4 us; 12,288 columns 19.2, 12.2, 8.9, 12.3; 4,096 x 6,144 6.6, 6.5, 8.0, 11.7.
     int cluster = 1;
-    while (cluster < 8 && (long long)groups * blocks_y * cluster < 2 * 148 && col_tiles >= 2 * WARPS * cluster) cluster *= 2;
+    while (cluster < 8 && (long long)groups * blocks_y * cluster * 2 <= SLOTS && col_tiles >= 2 * WARPS * cluster) cluster *= 2;
+    const int most = SLOTS / cluster / blocks_y, wide = groups < most ? groups : (most < 1 ? 1 : most);
     static unsigned long long roomy = 0;
-    if (const int rc = xb_more_smem(linear4_mma_kernel<NT, PER>, smem, &roomy)) return rc;
+    if (const int rc = xb_more_smem(linear4_mma_kernel<NT, R, PER>, smem, &roomy)) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(groups * cluster, blocks_y);
+    cfg.gridDim = dim3(wide * cluster, blocks_y);
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -234,13 +258,13 @@ int launch(const LinearArgs& A, cudaStream_t stream) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = xb_pdl_enabled() ? 2 : 1;
-    const cudaError_t rc = cudaLaunchKernelEx(&cfg, linear4_mma_kernel<NT, PER>, A, cluster);
+    const cudaError_t rc = cudaLaunchKernelEx(&cfg, linear4_mma_kernel<NT, R, PER>, A, cluster);
     return rc != cudaSuccess ? (int)rc : xb_launch_status();
 }
 
-template <int NT>
+template <int NT, int R>
 int with_group(const LinearArgs& A, cudaStream_t stream) {
-    return A.per_row == 4 ? launch<NT, 4>(A, stream) : (A.per_row == 2 ? launch<NT, 2>(A, stream) : launch<NT, 1>(A, stream));
+    return A.per_row == 4 ? launch<NT, R, 4>(A, stream) : (A.per_row == 2 ? launch<NT, R, 2>(A, stream) : launch<NT, R, 1>(A, stream));
 }
 
 }  // namespace
@@ -248,7 +272,11 @@ int with_group(const LinearArgs& A, cudaStream_t stream) {
 namespace xb4 {
 
 int linear4_mma(const LinearArgs& A, cudaStream_t stream) {
-    return A.tokens <= 8 ? with_group<1>(A, stream) : with_group<2>(A, stream);
+    if (A.tokens > 8) return with_group<2, 2>(A, stream);
+    // Four tiles of rows at a time take x out of memory half as often as two, but leave processors idle where they do not go round: whichever has less to do in
+    // its longest block, with a sixth more work for two.
+    const long long tiles = (A.rows + TILE_ROWS - 1) / TILE_ROWS, four = (((tiles + 3) / 4 + SLOTS - 1) / SLOTS) * 4 * 6, two = (((tiles + 1) / 2 + SLOTS - 1) / SLOTS) * 2 * 7;
+    return two < four ? with_group<1, 2>(A, stream) : with_group<1, 4>(A, stream);
 }
 
 }  // namespace xb4
