@@ -1,8 +1,9 @@
 // Products of many rows with a weight in 4 bits, in bfloat16 on the 5th-generation tensor cores (linear4.cu says what is computed and how a weight
 // lies).
 //
-// D[128 rows of the weight, up to 256 tokens] in tensor memory.  Sixteen warps take eight rows each of a column tile out of their codes, into the
-// shared-memory operand (128-byte swizzle); one thread fetches the tokens' columns by TMA, one issues the products.  A number of the weight
+// D[128 rows of the weight, up to 256 tokens] in tensor memory.  Two teams of eight warps take every other column tile each out of its codes, sixteen
+// rows a warp, into the shared-memory operand (128-byte swizzle): a tile is a chain of some 900 cycles from the stage that is free to the one that
+// is full, and two are at work.  One thread fetches the tokens' columns by TMA, one issues the products.  A number of the weight
 // becomes m + s code rounded to bfloat16 once, as a weight in bfloat16 would be: the bits of a code under a mask are the bfloat16 c 2^-133 (16 times that
 // in the next four bits), so that one multiply-add of two numbers, by s 2^64 and m 2^-69, gives them both times 2^-69, which the sums are
 // multiplied by at the end.  Scales may be up to 2^60.
@@ -16,9 +17,9 @@ namespace {
 using namespace xb4;
 using namespace xbtc;
 
-constexpr int ROWS = 128, CODE_WARPS = 16, THREADS = (CODE_WARPS + 2) * 32;
+constexpr int ROWS = 128, CODE_WARPS = 16, TEAM = CODE_WARPS / 2, THREADS = (CODE_WARPS + 2) * 32;
 constexpr int A_BYTES = ROWS * TILE_COLS * 2, ATOM = ROWS * 128;       // an atom: 64 columns
-constexpr int TOKENS_MOST = 256, STAGES_MOST = 4, AHEAD = 4;
+constexpr int TOKENS_MOST = 256, STAGES_MOST = 4, AHEAD = 2;
 constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
 constexpr uint32_t UP = 0x5f805f80u, UP16 = 0x5d805d80u, DOWN = 0x1d001d00u;       // 2^64, 2^60, 2^-69, twice
 constexpr float BACK = 0x1p69f;
@@ -58,11 +59,38 @@ __device__ __forceinline__ float of_rank(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-// What a lane takes of a column tile: 32 codes of a row, and the row's words.
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t e;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(e));
+    return e;
+}
+// Products issued by one lane of a warp that stays together: their operands are then values of the warp (in a branch of one lane every operand is
+// moved there, 100 cycles a product).
+__device__ __forceinline__ void umma_of(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
+}
+__device__ __forceinline__ void commit_of(uint32_t one, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(bar), "r"(one) : "memory");
+}
+
+// What a lane takes of a column tile: 32 codes of two rows, eight apart, and the rows' words.
 template <int PER>
 struct Codes {
-    uint4 c;
-    uint32_t w[PER];
+    uint4 c[2];
+    uint32_t w[2][PER];
 };
 
 // grid: (row blocks, splits, token blocks); cluster (1, splits, 1)
@@ -85,7 +113,7 @@ linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const TcArgs T) {
     const uint32_t tmem_cols = mp < 32 ? 32u : (uint32_t)mp;
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
-            mbar_init(full0 + 8 * s, CODE_WARPS + 1);
+            mbar_init(full0 + 8 * s, TEAM + 1);
             mbar_init(empty0 + 8 * s, 1);
         }
         mbar_init(accum, 1);
@@ -99,63 +127,68 @@ linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const TcArgs T) {
     pdl_launch_dependents();       // only now: see pdl_launch_dependents on tensor memory
 
     if (warp < CODE_WARPS) {
-        // ---- codes to numbers: row 16 (warp / 2) + 8 (warp % 2) + g of the block; a weight is nobody's result, so nothing is waited for
-        const int g = lane >> 2, t = lane & 3, half = warp & 1;
-        const uint8_t* line = A.weight + ((long long)min((int)blockIdx.x * 8 + (warp >> 1), row_tiles - 1) * col_tiles + from) * TILE;     // (behind the last row: it again)
-        auto fetch = [&](Codes<PER>& to, int it) {
-            const uint8_t* tile = line + (long long)min(it, iters - 1) * TILE;
-            to.c = *reinterpret_cast<const uint4*>(tile + half * 512 + lane * 16);
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(tile + TILE_CODES) + (half * 8 + g) * PER;
-            if constexpr (PER == 4) {
-                const uint4 v = *reinterpret_cast<const uint4*>(w);
-                to.w[0] = v.x, to.w[1] = v.y, to.w[2] = v.z, to.w[3] = v.w;
-            } else if constexpr (PER == 2) {
-                const uint2 v = *reinterpret_cast<const uint2*>(w);
-                to.w[0] = v.x, to.w[1] = v.y;
-            } else {
-                to.w[0] = *w;
+        // ---- codes to numbers: rows 16 (warp % 8) + g and + 8 of the block; a weight is nobody's result, so nothing is waited for
+        const int g = lane >> 2, t = lane & 3, team = warp / TEAM, tile_row = warp % TEAM;
+        const uint8_t* next = A.weight + ((long long)min((int)blockIdx.x * 8 + tile_row, row_tiles - 1) * col_tiles + from + team) * TILE;       // (behind the last row: it again)
+        int asked = team;
+        auto fetch = [&](Codes<PER>& to) {
+            if (asked < iters) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    to.c[h] = *reinterpret_cast<const uint4*>(next + h * 512 + lane * 16);
+                    const uint32_t* w = reinterpret_cast<const uint32_t*>(next + TILE_CODES) + (h * 8 + g) * PER;
+                    if constexpr (PER == 4) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(w);
+                        to.w[h][0] = v.x, to.w[h][1] = v.y, to.w[h][2] = v.z, to.w[h][3] = v.w;
+                    } else if constexpr (PER == 2) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(w);
+                        to.w[h][0] = v.x, to.w[h][1] = v.y;
+                    } else {
+                        to.w[h][0] = *w;
+                    }
+                }
             }
+            asked += 2;
+            next += 2 * TILE;
         };
         Codes<PER> have[AHEAD];
-        if (iters > 0) {
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) fetch(have[i], i);
-        }
+        for (int i = 0; i < AHEAD; ++i) fetch(have[i]);
         // where the lane's eight numbers of word j go: odd rows take the words of a pair the other way round, so that eight lanes meet all banks
         const int odd = g & 1;
-        const uint32_t row_at = (uint32_t)((warp >> 1) * 16 + half * 8 + g) * 128;
+        const uint32_t row_at = (uint32_t)(tile_row * 16 + g) * 128;
         const uint32_t first_at = row_at + (uint32_t)(((odd * 4 + t) ^ g) << 4), second_at = row_at + (uint32_t)((((odd ^ 1) * 4 + t) ^ g) << 4);
-        int s = 0;
-        uint32_t phase = 0;
+        int s = team % stages, laps = team / stages;           // the team's stage, and how often the ring has gone round
         bool ok = true;
-        for (int it0 = 0; it0 < iters && ok; it0 += AHEAD) {
+        for (int it0 = team; it0 < iters && ok; it0 += 2 * AHEAD) {
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
-                const int it = it0 + i;
+                const int it = it0 + 2 * i;
                 if (it >= iters || !ok) break;
-                if (it >= stages) ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, phase ^ 1u, T.err, true));
+                if (laps > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, (laps - 1) & 1, T.err, true));
                 if (!ok) break;
                 const uint32_t to = base + s * stage_bytes;
-                const uint32_t cw[4] = {have[i].c.x, have[i].c.y, have[i].c.z, have[i].c.w};
 #pragma unroll
-                for (int p = 0; p < 2; ++p)                // words 2 p and 2 p + 1: an atom
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t cw[4] = {have[i].c[h].x, have[i].c[h].y, have[i].c[h].z, have[i].c[h].w};
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const uint32_t u = (q ^ odd) ? cw[2 * p + 1] : cw[2 * p], u8 = u >> 8;
-                        const uint32_t w = PER == 4 ? ((q ^ odd) ? have[i].w[2 * p + 1 < PER ? 2 * p + 1 : 0] : have[i].w[2 * p < PER ? 2 * p : 0]) : have[i].w[PER == 2 ? p : 0];
-                        const uint32_t sc = __byte_perm(w, w, 0x1010), m = times(__byte_perm(w, w, 0x3232), DOWN), s1 = times(sc, UP), s16 = times(sc, UP16);
-                        uint4 v;
-                        v.x = fma_bf16(u & LOW, s1, m), v.y = fma_bf16(u & HIGH, s16, m), v.z = fma_bf16(u8 & LOW, s1, m), v.w = fma_bf16(u8 & HIGH, s16, m);
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + p * ATOM + (q == 0 ? first_at : second_at)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-                    }
+                    for (int p = 0; p < 2; ++p)            // words 2 p and 2 p + 1: an atom
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const uint32_t u = (q ^ odd) ? cw[2 * p + 1] : cw[2 * p], u8 = u >> 8;
+                            const uint32_t w = PER == 4 ? ((q ^ odd) ? have[i].w[h][2 * p + 1 < PER ? 2 * p + 1 : 0] : have[i].w[h][2 * p < PER ? 2 * p : 0]) : have[i].w[h][PER == 2 ? p : 0];
+                            const uint32_t sc = __byte_perm(w, w, 0x1010), m = times(__byte_perm(w, w, 0x3232), DOWN), s1 = times(sc, UP), s16 = times(sc, UP16);
+                            uint4 v;
+                            v.x = fma_bf16(u & LOW, s1, m), v.y = fma_bf16(u & HIGH, s16, m), v.z = fma_bf16(u8 & LOW, s1, m), v.w = fma_bf16(u8 & HIGH, s16, m);
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + h * 1024 + p * ATOM + (q == 0 ? first_at : second_at)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+                        }
+                }
+                fetch(have[i]);
                 fence_async_shared();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full0 + 8 * s);
-                fetch(have[i], it + AHEAD);
-                if (++s == stages) {
-                    s = 0;
-                    phase ^= 1u;
-                }
+                s += 2;
+                if (s >= stages) s -= stages, ++laps;
             }
         }
     } else if (threadIdx.x == CODE_WARPS * 32) {
@@ -174,31 +207,31 @@ linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const TcArgs T) {
                 phase ^= 1u;
             }
         }
-    } else if (threadIdx.x == (CODE_WARPS + 1) * 32) {
+    } else if (warp == CODE_WARPS + 1) {
         // ---- products
-        const uint32_t idesc = umma_idesc(mp);
+        const uint32_t one = elected(), tmem_u = __shfl_sync(0xffffffffu, tmem, 0), idesc = umma_idesc(mp);
+        const uint64_t adesc0 = umma_desc(base), bdesc0 = umma_desc(base + A_BYTES);
         int s = 0;
         uint32_t phase = 0;
         for (int it = 0; it < iters; ++it) {
-            if (!mbar_wait(full0 + 8 * s, phase, T.err)) {     // (reported; copies that are still on their way are waited for once more)
+            if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, phase, T.err, true))) {      // (reported; copies that are still on their way are waited for once more)
                 for (int i = 0; i < stages; ++i) mbar_wait(full0 + 8 * i, i < s ? phase ^ 1u : phase, T.err);
                 break;
             }
             tc_fence_after();
-            const uint32_t a = base + s * stage_bytes;
+            const uint64_t adesc = adesc0 + (uint64_t)((s * stage_bytes) >> 4), bdesc = bdesc0 + (uint64_t)((s * stage_bytes) >> 4);
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const uint64_t adesc = umma_desc(a + p * ATOM), bdesc = umma_desc(a + A_BYTES + p * x_atom);
+            for (int p = 0; p < 2; ++p)
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) umma_bf16(tmem, adesc + (uint64_t)(kk * 2), bdesc + (uint64_t)(kk * 2), idesc, (it | p | kk) ? 1u : 0u);
-            }
-            umma_commit(empty0 + 8 * s);
+                for (int kk = 0; kk < 4; ++kk)
+                    umma_of(one, tmem_u, adesc + (uint64_t)(p * (ATOM >> 4) + kk * 2), bdesc + (uint64_t)(p * (x_atom >> 4) + kk * 2), idesc, (it | p | kk) ? 1u : 0u);
+            commit_of(one, empty0 + 8 * s);
             if (++s == stages) {
                 s = 0;
                 phase ^= 1u;
             }
         }
-        umma_commit(accum);
+        commit_of(one, accum);
     }
     __syncwarp();
     pdl_wait();                    // nothing of the kernel before may still read what is written below
