@@ -1,12 +1,12 @@
 // Products of many rows with a weight in 4 bits, in bfloat16 on the 5th-generation tensor cores (linear4.cu says what is computed and how a weight
 // lies).
 //
-// D[128 rows of the weight, up to 256 tokens] in tensor memory.  Two teams of eight warps take every other column tile each out of its codes, sixteen
-// rows a warp, into the shared-memory operand (128-byte swizzle): a tile is a chain of some 900 cycles from the stage that is free to the one that
-// is full, and two are at work.  One thread fetches the tokens' columns by TMA, one issues the products.  A number of the weight
-// becomes m + s code rounded to bfloat16 once, as a weight in bfloat16 would be: the bits of a code under a mask are the bfloat16 c 2^-133 (16 times that
-// in the next four bits), so that one multiply-add of two numbers, by s 2^64 and m 2^-69, gives them both times 2^-69, which the sums are
-// multiplied by at the end.  Scales may be up to 2^60.
+// D[128 rows of the weight, up to 256 tokens] in tensor memory, and so is the weight's operand: a thread takes a row of a column tile out of its codes
+// into 64 registers and stores them to its lane.  (Through shared memory the operand is written and read again at 128 bytes a cycle, which bound the
+// kernel: 850 cycles a column tile with 64 tokens.)  Four teams of four warps take every fourth column tile each.  One thread fetches the tokens'
+// columns by TMA, one warp issues the products.  A number of the weight becomes m + s code rounded to bfloat16 once, as a weight in bfloat16
+// would be: the bits of a code under a mask are the bfloat16 c 2^-133 (16 times that in the next four bits), so that one multiply-add of two numbers, by
+// s 2^64 and m 2^-69, gives them both times 2^-69, which the sums are multiplied by at the end.  Scales may be up to 2^60.
 // K is split over a cluster's blocks where the row tiles alone do not fill the processors; their sums meet through distributed shared memory in
 // rank order.
 #include "linear4.h"
@@ -17,9 +17,9 @@ namespace {
 using namespace xb4;
 using namespace xbtc;
 
-constexpr int ROWS = 128, CODE_WARPS = 16, TEAM = CODE_WARPS / 2, THREADS = (CODE_WARPS + 2) * 32;
-constexpr int A_BYTES = ROWS * TILE_COLS * 2, ATOM = ROWS * 128;       // an atom: 64 columns
-constexpr int TOKENS_MOST = 256, STAGES_MOST = 4, AHEAD = 2;
+constexpr int ROWS = 128, CODE_WARPS = 16, TEAMS = CODE_WARPS / 4, THREADS = (CODE_WARPS + 2) * 32;
+constexpr int A_COLUMNS = TILE_COLS / 2;   // of tensor memory that a tile of the weight takes
+constexpr int TOKENS_MOST = 256, STAGES_MOST = 4;
 constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
 constexpr uint32_t UP = 0x5f805f80u, UP16 = 0x5d805d80u, DOWN = 0x1d001d00u;       // 2^64, 2^60, 2^-69, twice
 constexpr float BACK = 0x1p69f;
@@ -70,13 +70,13 @@ __device__ __forceinline__ uint32_t elected() {
 }
 // Products issued by one lane of a warp that stays together: their operands are then values of the warp (in a branch of one lane every operand is
 // moved there, 100 cycles a product).
-__device__ __forceinline__ void umma_of(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_of(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "setp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
 }
 __device__ __forceinline__ void commit_of(uint32_t one, uint32_t bar) {
     asm volatile(
@@ -86,11 +86,11 @@ __device__ __forceinline__ void commit_of(uint32_t one, uint32_t bar) {
         ::"r"(bar), "r"(one) : "memory");
 }
 
-// What a lane takes of a column tile: 32 codes of two rows, eight apart, and the rows' words.
+// A row's 128 codes in a column tile, and its words.
 template <int PER>
 struct Codes {
-    uint4 c[2];
-    uint32_t w[2][PER];
+    uint4 c[4];
+    uint32_t w[PER];
 };
 
 // grid: (row blocks, splits, token blocks); cluster (1, splits, 1)
@@ -98,24 +98,25 @@ template <int PER>
 __global__ void __launch_bounds__(THREADS, 1)
 linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const TcArgs T) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    __shared__ __align__(8) unsigned long long bars[2 * STAGES_MOST + 1];
+    __shared__ __align__(8) unsigned long long bars[2 * STAGES_MOST + 2 * TEAMS + 1];
     __shared__ uint32_t s_tmem;
     const LinearArgs& A = T.a;
     constexpr int TILE = TILE_CODES + TILE_ROWS * PER * 4;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;       // (the swizzle repeats every 1024 bytes)
     float* sums = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)));
-    const uint32_t x_atom = (uint32_t)T.mp * 128, stage_bytes = A_BYTES + 2 * x_atom;
+    const uint32_t x_atom = (uint32_t)T.mp * 128, stage_bytes = 2 * x_atom;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mp = T.mp, stages = T.stages;
     const int row_tiles = (A.rows + TILE_ROWS - 1) / TILE_ROWS, col_tiles = (A.columns + TILE_COLS - 1) / TILE_COLS;
     const int from = blockIdx.y * T.tiles_per_split, iters = max(0, min(col_tiles - from, T.tiles_per_split));
     const int t0 = blockIdx.z * mp, many = min(mp, A.tokens - t0);
-    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[STAGES_MOST]), accum = smem_u32(&bars[2 * STAGES_MOST]);
-    const uint32_t tmem_cols = mp < 32 ? 32u : (uint32_t)mp;
+    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[STAGES_MOST]), a_full0 = smem_u32(&bars[2 * STAGES_MOST]), a_empty0 = a_full0 + 8 * TEAMS, accum = a_empty0 + 8 * TEAMS;
+    const uint32_t tmem_cols = 512;        // D from the first on, the weight's tiles from 256 on
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
-            mbar_init(full0 + 8 * s, TEAM + 1);
+            mbar_init(full0 + 8 * s, 1);
             mbar_init(empty0 + 8 * s, 1);
         }
+        for (int i = 0; i < TEAMS; ++i) mbar_init(a_full0 + 8 * i, 4), mbar_init(a_empty0 + 8 * i, 1);
         mbar_init(accum, 1);
         mbar_init_fence();
     }
@@ -127,68 +128,65 @@ linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const TcArgs T) {
     pdl_launch_dependents();       // only now: see pdl_launch_dependents on tensor memory
 
     if (warp < CODE_WARPS) {
-        // ---- codes to numbers: rows 16 (warp % 8) + g and + 8 of the block; a weight is nobody's result, so nothing is waited for
-        const int g = lane >> 2, t = lane & 3, team = warp / TEAM, tile_row = warp % TEAM;
-        const uint8_t* next = A.weight + ((long long)min((int)blockIdx.x * 8 + tile_row, row_tiles - 1) * col_tiles + from + team) * TILE;       // (behind the last row: it again)
+        // ---- codes to numbers: row 32 (warp % 4) + lane of the block; a weight is nobody's result, so nothing is waited for
+        const int team = warp >> 2, in_tile = lane & 15;
+        const int row_tile = min((int)blockIdx.x * 8 + (warp & 3) * 2 + (lane >> 4), row_tiles - 1);       // (behind the last row: it again)
+        const uint8_t* next = A.weight + ((long long)row_tile * col_tiles + from + team) * TILE;
+        const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 256 + team * A_COLUMNS;
         int asked = team;
-        auto fetch = [&](Codes<PER>& to) {
+        auto fetch = [&](Codes<PER>& h) {
             if (asked < iters) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    to.c[h] = *reinterpret_cast<const uint4*>(next + h * 512 + lane * 16);
-                    const uint32_t* w = reinterpret_cast<const uint32_t*>(next + TILE_CODES) + (h * 8 + g) * PER;
-                    if constexpr (PER == 4) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(w);
-                        to.w[h][0] = v.x, to.w[h][1] = v.y, to.w[h][2] = v.z, to.w[h][3] = v.w;
-                    } else if constexpr (PER == 2) {
-                        const uint2 v = *reinterpret_cast<const uint2*>(w);
-                        to.w[h][0] = v.x, to.w[h][1] = v.y;
-                    } else {
-                        to.w[h][0] = *w;
-                    }
+                for (int t = 0; t < 4; ++t) h.c[t] = reinterpret_cast<const uint4*>(next + in_tile * 64)[t];       // (columns 32 j + 8 t + e of word j)
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(next + TILE_CODES) + in_tile * PER;
+                if constexpr (PER == 4) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(w);
+                    h.w[0] = v.x, h.w[1] = v.y, h.w[2] = v.z, h.w[3] = v.w;
+                } else if constexpr (PER == 2) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(w);
+                    h.w[0] = v.x, h.w[1] = v.y;
+                } else {
+                    h.w[0] = *w;
                 }
             }
-            asked += 2;
-            next += 2 * TILE;
+            asked += TEAMS;
+            next += TEAMS * TILE;
         };
-        Codes<PER> have[AHEAD];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) fetch(have[i]);
-        // where the lane's eight numbers of word j go: odd rows take the words of a pair the other way round, so that eight lanes meet all banks
-        const int odd = g & 1;
-        const uint32_t row_at = (uint32_t)(tile_row * 16 + g) * 128;
-        const uint32_t first_at = row_at + (uint32_t)(((odd * 4 + t) ^ g) << 4), second_at = row_at + (uint32_t)((((odd ^ 1) * 4 + t) ^ g) << 4);
-        int s = team % stages, laps = team / stages;           // the team's stage, and how often the ring has gone round
+        Codes<PER> have[2];
+        fetch(have[0]);
+        fetch(have[1]);
         bool ok = true;
-        for (int it0 = team; it0 < iters && ok; it0 += 2 * AHEAD) {
+        uint32_t laps = 0;
+        for (int it0 = team; it0 < iters && ok; it0 += 2 * TEAMS) {
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                const int it = it0 + 2 * i;
-                if (it >= iters || !ok) break;
-                if (laps > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, (laps - 1) & 1, T.err, true));
+            for (int i = 0; i < 2; ++i) {
+                if (it0 + i * TEAMS >= iters || !ok) break;
+                if (laps > 0) ok = __all_sync(0xffffffffu, mbar_wait(a_empty0 + 8 * team, (laps - 1) & 1, T.err, true));
                 if (!ok) break;
-                const uint32_t to = base + s * stage_bytes;
+                ++laps;
+                tc_fence_after();                          // (the products that read this part of tensor memory are done)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t cw[4] = {have[i].c[h].x, have[i].c[h].y, have[i].c[h].z, have[i].c[h].w};
+                for (int p = 0; p < 2; ++p) {              // columns 64 p .. 64 p + 63: words 2 p and 2 p + 1
+                    uint32_t v[32];
 #pragma unroll
-                    for (int p = 0; p < 2; ++p)            // words 2 p and 2 p + 1: an atom
+                    for (int q = 0; q < 2; ++q) {
+                        const uint32_t w = have[i].w[(2 * p + q) * PER / 4];
+                        const uint32_t sc = __byte_perm(w, w, 0x1010), m = times(__byte_perm(w, w, 0x3232), DOWN), s1 = times(sc, UP), s16 = times(sc, UP16);
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            const uint32_t u = (q ^ odd) ? cw[2 * p + 1] : cw[2 * p], u8 = u >> 8;
-                            const uint32_t w = PER == 4 ? ((q ^ odd) ? have[i].w[h][2 * p + 1 < PER ? 2 * p + 1 : 0] : have[i].w[h][2 * p < PER ? 2 * p : 0]) : have[i].w[h][PER == 2 ? p : 0];
-                            const uint32_t sc = __byte_perm(w, w, 0x1010), m = times(__byte_perm(w, w, 0x3232), DOWN), s1 = times(sc, UP), s16 = times(sc, UP16);
-                            uint4 v;
-                            v.x = fma_bf16(u & LOW, s1, m), v.y = fma_bf16(u & HIGH, s16, m), v.z = fma_bf16(u8 & LOW, s1, m), v.w = fma_bf16(u8 & HIGH, s16, m);
-                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + h * 1024 + p * ATOM + (q == 0 ? first_at : second_at)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+                        for (int t = 0; t < 4; ++t) {
+                            const uint4& c = have[i].c[t];
+                            const uint32_t u = p == 0 ? (q == 0 ? c.x : c.y) : (q == 0 ? c.z : c.w), u8 = u >> 8;
+                            v[q * 16 + t * 4] = fma_bf16(u & LOW, s1, m), v[q * 16 + t * 4 + 1] = fma_bf16(u & HIGH, s16, m);
+                            v[q * 16 + t * 4 + 2] = fma_bf16(u8 & LOW, s1, m), v[q * 16 + t * 4 + 3] = fma_bf16(u8 & HIGH, s16, m);
                         }
+                    }
+                    tmem_st32_u(to + p * 32, v);
                 }
                 fetch(have[i]);
-                fence_async_shared();
+                tmem_st_wait();
+                tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(full0 + 8 * s);
-                s += 2;
-                if (s >= stages) s -= stages, ++laps;
+                if (lane == 0) mbar_arrive(a_full0 + 8 * team);
             }
         }
     } else if (threadIdx.x == CODE_WARPS * 32) {
@@ -198,7 +196,7 @@ linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const TcArgs T) {
         uint32_t phase = 0;
         for (int it = 0; it < iters; ++it) {
             if (it >= stages && !mbar_wait(empty0 + 8 * s, phase ^ 1u, T.err)) break;
-            const uint32_t dst = base + s * stage_bytes + A_BYTES;
+            const uint32_t dst = base + s * stage_bytes;
             mbar_expect_tx(full0 + 8 * s, 2 * x_atom);
             tma_load_2d(dst, &map_x, (from + it) * TILE_COLS, t0, full0 + 8 * s);
             tma_load_2d(dst + x_atom, &map_x, (from + it) * TILE_COLS + 64, t0, full0 + 8 * s);
@@ -210,22 +208,25 @@ linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const TcArgs T) {
     } else if (warp == CODE_WARPS + 1) {
         // ---- products
         const uint32_t one = elected(), tmem_u = __shfl_sync(0xffffffffu, tmem, 0), idesc = umma_idesc(mp);
-        const uint64_t adesc0 = umma_desc(base), bdesc0 = umma_desc(base + A_BYTES);
+        const uint64_t bdesc0 = umma_desc(base);
         int s = 0;
         uint32_t phase = 0;
         for (int it = 0; it < iters; ++it) {
-            if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, phase, T.err, true))) {      // (reported; copies that are still on their way are waited for once more)
+            const int slot = it % TEAMS;
+            const bool ok = mbar_wait(a_full0 + 8 * slot, (it / TEAMS) & 1, T.err, true) && mbar_wait(full0 + 8 * s, phase, T.err, true);
+            if (!__all_sync(0xffffffffu, ok)) {            // (reported; copies that are still on their way are waited for once more)
                 for (int i = 0; i < stages; ++i) mbar_wait(full0 + 8 * i, i < s ? phase ^ 1u : phase, T.err);
                 break;
             }
             tc_fence_after();
-            const uint64_t adesc = adesc0 + (uint64_t)((s * stage_bytes) >> 4), bdesc = bdesc0 + (uint64_t)((s * stage_bytes) >> 4);
+            const uint64_t bdesc = bdesc0 + (uint64_t)((s * stage_bytes) >> 4);
 #pragma unroll
             for (int p = 0; p < 2; ++p)
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
-                    umma_of(one, tmem_u, adesc + (uint64_t)(p * (ATOM >> 4) + kk * 2), bdesc + (uint64_t)(p * (x_atom >> 4) + kk * 2), idesc, (it | p | kk) ? 1u : 0u);
+                    umma_of(one, tmem_u, tmem_u + 256 + slot * A_COLUMNS + p * 32 + kk * 8, bdesc + (uint64_t)(p * (x_atom >> 4) + kk * 2), idesc, (it | p | kk) ? 1u : 0u);
             commit_of(one, empty0 + 8 * s);
+            commit_of(one, a_empty0 + 8 * slot);
             if (++s == stages) {
                 s = 0;
                 phase ^= 1u;
@@ -296,9 +297,9 @@ int launch(const LinearArgs& A, int* err, cudaStream_t stream) {
     int splits = 1;
     while (splits < 8 && (long long)blocks * token_blocks * splits * 2 <= 148 && col_tiles / (splits * 2) >= 4) splits *= 2;
     T.tiles_per_split = (col_tiles + splits - 1) / splits;
-    const int stage_bytes = A_BYTES + 2 * T.mp * 128;
+    const int stage_bytes = 2 * T.mp * 128;
     T.stages = 200 * 1024 / stage_bytes < STAGES_MOST ? 200 * 1024 / stage_bytes : STAGES_MOST;
-    const int smem = T.stages * stage_bytes + 1024;        // (the sums, 512 bytes a token, fit the stages)
+    const int smem = (T.stages * stage_bytes > T.mp * ROWS * 4 ? T.stages * stage_bytes : T.mp * ROWS * 4) + 1024;        // (the sums lie where the stages did)
     CUtensorMap map;
     if (!map_of(&map, A, T.mp)) return (int)cudaErrorInvalidValue;
     static unsigned long long roomy = 0;
