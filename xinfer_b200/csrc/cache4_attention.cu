@@ -33,7 +33,7 @@ cache4_attention_any_kernel(const AttendArgs A, float* parts, int splits) {
     int* page = reinterpret_cast<int*>(alpha + RT);      // [KT]: a key's page, -1 without one
     int* place = page + KT;
     pdl_overlap_few();
-    const int b = blockIdx.y, g = blockIdx.x % A.nkv, group = A.nh / A.nkv, step = gridDim.x / A.nkv;
+    const int b = blockIdx.y, g = blockIdx.x % A.nkv, group = A.group, step = gridDim.x / A.nkv;
     const Request r = request_of(A, b);
     const int rows = r.nodes * group;
     for (int rt = blockIdx.x / A.nkv; rt * RT < rows; rt += step) {
@@ -236,7 +236,7 @@ static int cache4_attention(int dtype, void* out, const void* q, const uint8_t* 
     if (requests > REQUESTS_MAX || d < 1 || d > DIM_MOST || nkv < 1 || nh < nkv || nh % nkv || page_size < 1) return (int)cudaErrorInvalidValue;
     if ((long long)table_stride * page_size > KEYS_MOST || (long long)tokens * nh > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     AttendArgs A{out, q, k_cache, v_cache, lengths, token_start, block_table, out_stride, q_stride, tokens, requests, table_stride, nh, nkv, d, page_size,
-                       num_pages, window, 0, 0x7fffffff, scale, err};
+                       num_pages, window, nh / nkv, ((1ull << 32) + (unsigned)(nh / nkv) - 1) / (unsigned)(nh / nkv), 0, 0x7fffffff, scale, err};
     if (dtype == XB_BF16 && tc_takes(A, longest)) {
         // requests of few rows beside those of many have the kernel for few: 64 single tokens at up to 4,096 keys beside a portion of 512 (both forms read the lengths on the device)
         const bool both = mma_takes(A);

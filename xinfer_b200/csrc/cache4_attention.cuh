@@ -14,10 +14,16 @@ struct AttendArgs {
     const int* block_table;        // [requests, table_stride]
     long long out_stride, q_stride;
     int tokens, requests, table_stride, nh, nkv, d, page_size, num_pages, window;
+    int group;                     // query heads of a key/value head
+    unsigned long long group_inv;  // 2^32 / group, upwards
     int rows_from, rows_to;        // requests of other numbers of rows (tokens times query heads of a key/value head) are another kernel's
     float scale;
     int* err;
 };
+
+// The token that a row (token, query head of the group) of a request belongs to: row / group, right for rows below 2^32 / group.
+__device__ __forceinline__ int token_of(const AttendArgs& A, int row) { return (int)((unsigned)row * A.group_inv >> 32); }
+inline bool tokens_of_rows(const AttendArgs& A) { return (double)A.tokens * A.group * A.group < 4294967296.0; }
 
 constexpr int REQUESTS_MAX = 8192;
 constexpr long long KEYS_MOST = 0x7fff0000;      // keys that a row of the table may hold: their numbers, rounded up to tiles, are 32 bits
@@ -37,7 +43,7 @@ __device__ __forceinline__ Request request_of(const AttendArgs& A, int b) {
     if (len > most && r.nodes > 0) atomicOr(A.err, XB_ERR_BAD_PAGE);
     r.keys = len < 0 ? 0 : (int)(len > most ? most : len);
     r.first_pos = max(len, 0) - r.nodes;
-    const int rows = r.nodes * (A.nh / A.nkv);
+    const int rows = r.nodes * A.group;
     if (rows < A.rows_from || rows >= A.rows_to) r.nodes = 0;
     return r;
 }

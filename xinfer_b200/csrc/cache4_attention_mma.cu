@@ -40,7 +40,7 @@ __host__ __device__ constexpr int smem_bytes(int ng) { return WARPS * stages(ng)
 struct Line {
     float* part_o;                 // [warps][2][rows][d]: a warp's first segment, if its job began before it, and its last, if its job goes on
     float* part_ml;                // [warps][2][rows][2]: maximum and sum
-    int* jobs;                     // [warps][2][8]: parts (0: there is no such part), warp of the first, first row, rows, key/value head, request
+    int* jobs;                     // [warps][2][8]: parts (0: there is no such part), warp of the first, first row, rows, key/value head, the request's first token
 };
 
 struct Walk {
@@ -56,7 +56,7 @@ template <int ROWS>
 __device__ __forceinline__ void set_request(const AttendArgs& A, Walk& w, int b) {
     w.b = b;
     w.r = request_of(A, b);
-    w.pieces = (w.r.nodes * (A.nh / A.nkv) + ROWS - 1) / ROWS;
+    w.pieces = (w.r.nodes * A.group + ROWS - 1) / ROWS;
     w.tile0 = first_seen(A, w.r.first_pos) / KT;
     // (a request that sees no key has a tile all the same: its rows are written)
     w.tiles = max(1, (w.r.keys + KT - 1) / KT - w.tile0);
@@ -205,7 +205,7 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
     extern __shared__ __align__(128) char mem[];
     constexpr int ROWS = 8 * NT, STAGES = stages(NG), STAGE = stage_bytes(NG), HALF = 20 * NG * STEP, CODES = NG * STEP * 16, DP = 32 * NG;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gi = lane >> 2, ti = lane & 3;
-    const int group = A.nh / A.nkv, ps = A.page_size;
+    const int group = A.group, ps = A.page_size;
     const bool by16 = ps % STEP == 0;                      // a step's keys lie in one page; else in two
     const uint32_t ring = smem_u32(mem) + warp * STAGES * STAGE;
     const uint32_t bars = smem_u32(mem) + WARPS * STAGES * STAGE + warp * STAGES * 8;
@@ -230,7 +230,7 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
     bool failed = false;                                   // a copy never came: nothing is fetched any more
     for (bool first = true; next_segment<ROWS>(A, w, first); first = false) {
         const int row0 = w.piece * ROWS, rows = min(ROWS, w.r.nodes * group - row0);
-        const int pos0 = w.r.first_pos + row0 / group, pos1 = w.r.first_pos + (row0 + rows - 1) / group;
+        const int pos0 = w.r.first_pos + token_of(A, row0), pos1 = w.r.first_pos + token_of(A, row0 + rows - 1);
         // keys from `all0` on and below `all1` are seen by all rows
         const int all0 = first_seen(A, pos1), all1 = min(pos0 + 1, w.r.keys);
         // the segment's steps, of these the ones with keys that some row sees
@@ -297,8 +297,8 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int row = min(j * 8 + gi, rows - 1);     // (columns without a row repeat the last one's)
-            const long long t = w.r.first + (row0 + row) / group;
-            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(A.q) + t * A.q_stride + (long long)(w.g * group + (row0 + row) % group) * A.d;
+            const long long t = w.r.first + token_of(A, row0 + row);
+            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(A.q) + t * A.q_stride + (long long)(w.g * group + (row0 + row - token_of(A, row0 + row) * group)) * A.d;
             float x[NG][8], top = 0.f;
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
@@ -428,7 +428,7 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int key = key0 + gi + 8 * (e >> 1), row = min(j * 8 + 2 * ti + (e & 1), rows - 1), pos = w.r.first_pos + (row0 + row) / group;
+                            const int key = key0 + gi + 8 * (e >> 1), row = min(j * 8 + 2 * ti + (e & 1), rows - 1), pos = w.r.first_pos + token_of(A, row0 + row);
                             const bool is = !(lost >> (e >> 1) & 1) && key < w.r.keys && key <= pos && key >= first_seen(A, pos);
                             seen |= is ? 1u << (4 * j + e) : 0u;
                         }
@@ -567,8 +567,8 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
                 for (int s = 4; s < 32; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
                 sum *= DOWN;
                 const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
-                const long long t = w.r.first + (row0 + min(row, rows - 1)) / group;
-                __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + t * A.out_stride + (long long)(w.g * group + (row0 + row) % group) * A.d;
+                const long long t = w.r.first + token_of(A, row0 + min(row, rows - 1));
+                __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + t * A.out_stride + (long long)(w.g * group + (row0 + row - token_of(A, row0 + row) * group)) * A.d;
 #pragma unroll
                 for (int n = 0; n < NG; ++n) {
                     float r;
@@ -602,14 +602,14 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
         if (!whole && lane == 0) {
             int* job = line.jobs + part * JOB_WORDS;
             const int first_warp = w.job / w.share, last = (w.job + w.tiles - 1) / w.share;
-            job[1] = first_warp, job[2] = row0, job[3] = rows, job[4] = w.g, job[5] = w.b;
+            job[1] = first_warp, job[2] = row0, job[3] = rows, job[4] = w.g, job[5] = w.r.first;
             job[0] = last - first_warp + 1;
         }
     }
 }
 
-// A job's parts, joined in the order of the line: a warp for every part takes its share of the job's numbers, four to eight lanes each where the
-// parts are many.
+// A job's parts, joined in the order of the line: a warp for every part takes its share of the job's numbers, and as many lanes for a number as leave
+// one trip.
 template <int NT, int NG>
 __global__ void __launch_bounds__(THREADS)
 cache4_attention_join_kernel(const AttendArgs A, const Line line) {
@@ -619,36 +619,42 @@ cache4_attention_join_kernel(const AttendArgs A, const Line line) {
     const int lane = threadIdx.x & 31, entry = (int)blockIdx.x * WARPS + ((int)threadIdx.x >> 5);
     const int* job = line.jobs + (size_t)entry * JOB_WORDS;
     const int4 head = *reinterpret_cast<const int4*>(job);
+    const int2 more = *reinterpret_cast<const int2*>(job + 4);
     const int parts = head.x;
     if (parts < 1) return;
-    const int first = head.y, row0 = head.z, rows = head.w, g = job[4], group = A.nh / A.nkv;
-    const Request r = request_of(A, job[5]);
+    const int first = head.y, row0 = head.z, rows = head.w, g = more.x, group = A.group, first_token = more.y;
     const int mine = entry / 2 - first, total = rows * FOURS;
     auto part_of = [&](int i) { return (size_t)(first + i) * 2 + (i == 0 ? 1 : 0); };     // (the first part is its warp's last segment)
-    const int lanes = parts > 4 ? 8 : 1, sub = lane & (lanes - 1), lo = (int)((long long)total * mine / parts), hi = (int)((long long)total * (mine + 1) / parts);
+    const int lo = (int)((long long)total * mine / parts), hi = (int)((long long)total * (mine + 1) / parts);
+    int lanes = 1;
+    while (lanes < 16 && lanes * 2 * (hi - lo) <= 32 && lanes < parts) lanes *= 2;
+    const int sub = lane & (lanes - 1);
     for (int i0 = lo; i0 < hi; i0 += 32 / lanes) {
         const int i = min(i0 + lane / lanes, hi - 1), row = i / FOURS, c = i % FOURS * 4;
         float top = -INFINITY, sum = 0.f;
-        for (int k = sub; k < parts; k += lanes) top = max_nan(top, line.part_ml[(part_of(k) * ROWS + row) * 2]);
-        for (int s = 1; s < lanes; s <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, s));
         float4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int k = sub; k < parts; k += lanes) {
             const size_t at = part_of(k) * ROWS + row;
             const float2 ml = *reinterpret_cast<const float2*>(line.part_ml + at * 2);
             const float4 u = *reinterpret_cast<const float4*>(line.part_o + at * DP + c);
-            const float f = ml.x == -INFINITY ? 0.f : xbtc::ex2(ml.x - top);       // (parts of nothing hold zeros)
-            sum = fmaf(f, ml.y, sum);
-            v.x = fmaf(f, u.x, v.x), v.y = fmaf(f, u.y, v.y), v.z = fmaf(f, u.z, v.z), v.w = fmaf(f, u.w, v.w);
+            if (ml.x == -INFINITY) continue;                   // (a part of nothing)
+            const float now = max_nan(top, ml.x), a = xbtc::ex2(top - now), f = xbtc::ex2(ml.x - now);
+            top = now;
+            sum = fmaf(f, ml.y, sum * a);
+            v.x = fmaf(f, u.x, v.x * a), v.y = fmaf(f, u.y, v.y * a), v.z = fmaf(f, u.z, v.z * a), v.w = fmaf(f, u.w, v.w * a);
         }
         for (int s = 1; s < lanes; s <<= 1) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, s);
-            v.x += __shfl_xor_sync(0xffffffffu, v.x, s), v.y += __shfl_xor_sync(0xffffffffu, v.y, s);
-            v.z += __shfl_xor_sync(0xffffffffu, v.z, s), v.w += __shfl_xor_sync(0xffffffffu, v.w, s);
+            const float other = __shfl_xor_sync(0xffffffffu, top, s), now = max_nan(top, other);
+            const float a = now == -INFINITY ? 0.f : xbtc::ex2(top - now), f = now == -INFINITY ? 0.f : xbtc::ex2(other - now);
+            top = now;
+            sum = sum * a + __shfl_xor_sync(0xffffffffu, sum, s) * f;
+            v.x = v.x * a + __shfl_xor_sync(0xffffffffu, v.x, s) * f, v.y = v.y * a + __shfl_xor_sync(0xffffffffu, v.y, s) * f;
+            v.z = v.z * a + __shfl_xor_sync(0xffffffffu, v.z, s) * f, v.w = v.w * a + __shfl_xor_sync(0xffffffffu, v.w, s) * f;
         }
         if (sub || i0 + lane / lanes >= hi) continue;
-        const long long t = r.first + (row0 + row) / group;
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + t * A.out_stride + (long long)(g * group + (row0 + row) % group) * A.d;
+        const int token = token_of(A, row0 + row);
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + (long long)(first_token + token) * A.out_stride + (long long)(g * group + row0 + row - token * group) * A.d;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
 #pragma unroll
@@ -698,8 +704,8 @@ namespace xb4 {
 bool mma_takes(int d) { return groups_of(d) <= 4 || groups_of(d) == 8; }
 bool mma_takes(const AttendArgs& A) {
     // the longest line that these shapes allow is counted in 32 bits
-    const double jobs = (double)A.nkv * ((double)A.tokens * (A.nh / A.nkv) / 8 + A.requests), tiles = (double)A.table_stride * A.page_size / KT + 2;
-    return mma_takes(A.d) && A.page_size % 8 == 0 && A.num_pages > 0 && jobs * (tiles + COST_JOB) < 2147483648.0;
+    const double jobs = (double)A.nkv * ((double)A.tokens * A.group / 8 + A.requests), tiles = (double)A.table_stride * A.page_size / KT + 2;
+    return mma_takes(A.d) && tokens_of_rows(A) && A.page_size % 8 == 0 && A.num_pages > 0 && jobs * (tiles + COST_JOB) < 2147483648.0;
 }
 long long mma_scratch(int d, int rows) {
     return by_form(rows, groups_of(d), [](auto nt, auto ng) { return scratch_of<decltype(nt)::value, decltype(ng)::value>(); });

@@ -60,18 +60,18 @@ __device__ __forceinline__ void set_tiles(const AttendArgs& A, Walk& w, int node
     w.tiles = max(1, (min(w.r.first_pos + node1 + 1, w.r.keys) + KT - 1) / KT - w.tile0);       // (rows that see no key are written all the same)
 }
 __device__ __forceinline__ void set_piece(const AttendArgs& A, Walk& w) {
-    const int group = A.nh / A.nkv, row0 = w.piece * ROWS;
-    set_tiles(A, w, row0 / group, min(w.r.nodes - 1, (row0 + ROWS - 1) / group));
+    const int group = A.group, row0 = w.piece * ROWS;
+    set_tiles(A, w, token_of(A, row0), min(w.r.nodes - 1, token_of(A, row0 + ROWS - 1)));
 }
 __device__ __forceinline__ void set_request(const AttendArgs& A, Walk& w, int b) {
     w.b = b;
     w.r = request_of(A, b);
-    w.pieces = (w.r.nodes * (A.nh / A.nkv) + ROWS - 1) / ROWS;
+    w.pieces = (w.r.nodes * A.group + ROWS - 1) / ROWS;
 }
 // The pieces one after another, until `f(piece)` is true: their tokens' places by sums.
 template <typename F>
 __device__ __forceinline__ void each_piece(const AttendArgs& A, Walk& w, F f) {
-    const int group = A.nh / A.nkv, quo = ROWS / group, rem = ROWS % group;
+    const int group = A.group, quo = ROWS / group, rem = ROWS % group;
     int node = 0, over = 0;        // (256 * piece) / group and the remainder
 #pragma unroll 1
     for (w.piece = 0; w.piece < w.pieces; ++w.piece) {
@@ -272,7 +272,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, q_sm = base, kv_sm = base + 2 * Q_ONE, raw_sm = kv_sm + NS * STAGE_BYTES;
     const uint32_t bar0 = smem_u32(bars), k_full0 = bar0, k_empty0 = bar0 + 8 * NS, v_full0 = bar0 + 16 * NS, v_empty0 = bar0 + 24 * NS, rest = bar0 + 32 * NS;
     const uint32_t s_ready0 = rest, pv_done0 = rest + 32, p_ready0 = rest + 64, q_ready0 = rest + 96, drained0 = rest + 112;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = A.nh / A.nkv, ps = A.page_size;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = A.group, ps = A.page_size;
     int* const err = A.err;
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; ++i) mbar_init(k_full0 + 8 * i, 4), mbar_init(k_empty0 + 8 * i, 1), mbar_init(v_full0 + 8 * i, 4), mbar_init(v_empty0 + 8 * i, 1);
@@ -312,7 +312,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
         for (bool first = true; ok && next_segment(A, w, first); first = false) {
             const int* table = A.block_table + (long long)w.b * A.table_stride;
             const uint8_t* pages = (is_v ? A.v_cache : A.k_cache) + w.g * page_bytes;
-            const int first_key = first_seen(A, w.r.first_pos + w.piece * ROWS / group);       // (pages in front of it may have been given back)
+            const int first_key = first_seen(A, w.r.first_pos + token_of(A, w.piece * ROWS));       // (pages in front of it may have been given back)
             // the lane's key: its place in the table and in its page, kept up by sums
             int k = (w.tile0 + w.i0) * KT + key, at = k / ps, slot = k % ps, asked = w.i0, slot_in = 0, slot_out = 0;       // tiles asked for, their places in the ring
             unsigned have = 0;                     // whether the key is there, a bit a tile, the last asked for lowest
@@ -485,17 +485,17 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
             }
             const int row = hd * RT + r;
             const bool valid = row < rows;
-            const int of_request = row0 + min(row, rows - 1), pos = w.r.first_pos + of_request / group;
+            const int of_request = row0 + min(row, rows - 1), pos = w.r.first_pos + token_of(A, of_request);
             const int lo = first_seen(A, pos), hi = min(pos + 1, w.r.keys);              // the keys that the row sees
-            const long long t = w.r.first + of_request / group;
-            const int head = w.g * group + of_request % group;
+            const long long t = w.r.first + token_of(A, of_request);
+            const int head = w.g * group + of_request - token_of(A, of_request) * group;
             // Q: the last tile's scores of the last segment are there, so nothing reads what lies there
             float c1;
             {
                 // (VPR lanes have a row, eight channels each, so that lanes read what lies together; eight trips are on their way at a time)
                 constexpr int VPR = DP / 8, RPI = 32 / VPR, TRIPS = 32 / RPI;
                 const int c = (lane % VPR) * 8, sub = lane / VPR, warp_row = hd * RT + (warp & 3) * 32;
-                int e2 = 0, of = row0 + min(warp_row + sub, rows - 1), token = of / group, of_head = of - token * group;
+                int e2 = 0, of = row0 + min(warp_row + sub, rows - 1), token = token_of(A, of), of_head = of - token * group;
                 const int last = row0 + rows - 1;
 #pragma unroll 1
                 for (int i0 = 0; i0 < TRIPS; i0 += 8) {
@@ -555,7 +555,7 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
             float m_ref = -INFINITY, l = 0.f, v_back = 0.f, v_down = 0.f;
             unsigned poison = 0;                 // groups of channels that are no number
             // keys from all0 on and below all1 are seen by all rows of the job
-            const int pos0 = w.r.first_pos + row0 / group, pos1 = w.r.first_pos + (row0 + rows - 1) / group;
+            const int pos0 = w.r.first_pos + token_of(A, row0), pos1 = w.r.first_pos + token_of(A, row0 + rows - 1);
             const int all0 = first_seen(A, pos1), all1 = min(pos0 + 1, w.r.keys);
             for (int it = w.i0; it < w.i1; ++it, ++Th) {
                 const int sb = Th & 1, key0 = (w.tile0 + it) * KT;
@@ -745,7 +745,7 @@ cache4_attention_tc_join_kernel(const AttendArgs A, const Line line) {
     const int4 head = *reinterpret_cast<const int4*>(job);
     const int parts = head.x;
     if (parts < 1) return;
-    const int first = head.y, row0 = head.z, rows = head.w, g = job[4], group = A.nh / A.nkv;
+    const int first = head.y, row0 = head.z, rows = head.w, g = job[4], group = A.group;
     const Request r = request_of(A, job[5]);
     // pieces of eight rows and sixteen channels, 32 lanes
     const int mine = ((int)blockIdx.x / 2 - first) * JOIN_BLOCKS + (int)blockIdx.y, shares = parts * JOIN_BLOCKS, total = (rows + 7) / 8 * (FOURS / 4);
@@ -766,8 +766,8 @@ cache4_attention_tc_join_kernel(const AttendArgs A, const Line line) {
             sum = fmaf(f, ml.y, sum);
             v.x = fmaf(f, u.x, v.x), v.y = fmaf(f, u.y, v.y), v.z = fmaf(f, u.z, v.z), v.w = fmaf(f, u.w, v.w);
         }
-        const long long t = r.first + (row0 + row) / group;
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + t * A.out_stride + (long long)(g * group + (row0 + row) % group) * A.d;
+        const long long t = r.first + token_of(A, row0 + row);
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + t * A.out_stride + (long long)(g * group + (row0 + row - token_of(A, row0 + row) * group)) * A.d;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
 #pragma unroll
@@ -799,8 +799,8 @@ namespace xb4 {
 bool tc_takes(int nh, int nkv, int d, int longest) { return d <= 128 && (long long)longest * (nh / nkv) >= TC_ROWS; }
 bool tc_takes(const AttendArgs& A, int longest) {
     // the longest line that these shapes allow is counted in 32 bits
-    const double jobs = (double)A.nkv * ((double)A.tokens * (A.nh / A.nkv) / ROWS + A.requests), tiles = (double)A.table_stride * A.page_size / KT + 2;
-    return tc_takes(A.nh, A.nkv, A.d, longest) && A.scale > 0.f && A.num_pages > 0 && (long long)A.page_size * row_bytes(A.d) % 16 == 0 && jobs * (tiles + COST_JOB) < 2147483648.0;
+    const double jobs = (double)A.nkv * ((double)A.tokens * A.group / ROWS + A.requests), tiles = (double)A.table_stride * A.page_size / KT + 2;
+    return tc_takes(A.nh, A.nkv, A.d, longest) && tokens_of_rows(A) && A.scale > 0.f && A.num_pages > 0 && (long long)A.page_size * row_bytes(A.d) % 16 == 0 && jobs * (tiles + COST_JOB) < 2147483648.0;
 }
 long long tc_scratch(int d) { return (long long)BLOCKS * 2 * (ROWS * (dp_of(d) + 2) + JOB_WORDS); }
 int tc_launch(const AttendArgs& A, float* scratch, cudaStream_t stream) {
