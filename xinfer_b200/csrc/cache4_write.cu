@@ -98,7 +98,7 @@ cache4_write_any_kernel(const WriteArgs A) {
         }
         const uint32_t word = xb4::word_of(lo, hi);
         const float s = xb4::scale_of(word);
-        const uint32_t code = (uint32_t)xb4::code_of(v, s, xb4::least_of(word), xb4::reciprocal(s));
+        const uint32_t code = __float_as_uint(xb4::raised_code(v, s, xb4::least_of(word), xb4::reciprocal(s))) & 15u;
         if (values && c < d) values[c] = __float2bfloat16_rn(xb4::value_of(code, word));
         uint32_t eight = code << (4 * (lane & 7));
 #pragma unroll
@@ -142,7 +142,7 @@ __device__ __forceinline__ void store8(T* x, const float (&v)[8]) {
 
 constexpr int TURN_NONE = 0, TURN_HALVES = 1, TURN_PAIRS = 2;
 
-template <typename T, int LPH, int TURN>
+template <typename T, int LPH, int TURN, bool FULL>
 __global__ void __launch_bounds__(VEC_WARPS * 32, 4)
 cache4_write_kernel(const WriteArgs A, int each) {
     constexpr int HEADS = 32 / LPH;
@@ -153,7 +153,7 @@ cache4_write_kernel(const WriteArgs A, int each) {
     const unsigned job = blockIdx.x * VEC_WARPS + (threadIdx.x >> 5);
     const int t = (int)(job / (unsigned)(q_jobs + kv_jobs)), of_token = (int)(job % (unsigned)(q_jobs + kv_jobs));
     if (t >= A.tokens) return;
-    const bool is_q = of_token < q_jobs, active = li * 8 < d;
+    const bool is_q = of_token < q_jobs, active = FULL || li * 8 < d;      // FULL: every lane has channels
     const int count = is_q ? A.nh : 2 * A.nkv, h0 = (is_q ? of_token : of_token - q_jobs) * HEADS * each + sub;
     const int c0 = active ? li * 8 : 0, groups = xb4::groups_of(d);
     const T* heads = static_cast<const T*>(A.qkv) + t * A.row_stride + c0 + (is_q ? 0 : (long long)A.nh * d);
@@ -258,13 +258,13 @@ cache4_write_kernel(const WriteArgs A, int each) {
         }
         const uint32_t word = xb4::word_of(lo, hi);
         const float s = xb4::scale_of(word), m = xb4::least_of(word), inv = xb4::reciprocal(s);
-        uint32_t codes = 0;
+        uint32_t codes = 0u - 0x3f400000u;                     // (what the raised codes' upper bits come to, modulo 2^32)
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float c = xb4::code_of(v[e], s, m, inv);
-            codes |= (uint32_t)c << (4 * e);
-            y[e] = fmaf(s, c, m);
+            const float c = xb4::raised_code(v[e], s, m, inv);
+            codes += __float_as_uint(c) << (4 * e);
+            y[e] = fmaf(s, c - xb4::CODE_UP, m);
         }
         if (h >= count) continue;
         const int g = is_k ? h : h - A.nkv;
@@ -284,7 +284,12 @@ int launch_vec(const WriteArgs& A, cudaStream_t stream) {
     while (each < 8 && (long long)A.tokens * (A.nh + 2 * A.nkv) / (together * each * 2) >= 148 * 32) each *= 2;
     const long long jobs = (long long)A.tokens * ((A.nh + together * each - 1) / (together * each) + (2 * A.nkv + together * each - 1) / (together * each));
     auto go = [&](auto kernel) { return xb_launch_few(kernel, dim3((unsigned)((jobs + VEC_WARPS - 1) / VEC_WARPS)), dim3(VEC_WARPS * 32), 0, stream, A, each); };
-    return !A.cos_t ? go(cache4_write_kernel<T, LPH, TURN_NONE>) : (A.interleaved ? go(cache4_write_kernel<T, LPH, TURN_PAIRS>) : go(cache4_write_kernel<T, LPH, TURN_HALVES>));
+    auto form = [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        return !A.cos_t ? go(cache4_write_kernel<T, LPH, TURN_NONE, FULL>)
+                        : (A.interleaved ? go(cache4_write_kernel<T, LPH, TURN_PAIRS, FULL>) : go(cache4_write_kernel<T, LPH, TURN_HALVES, FULL>));
+    };
+    return A.d == 8 * LPH ? form(std::true_type()) : form(std::false_type());
 }
 
 template <typename T>

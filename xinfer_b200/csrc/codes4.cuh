@@ -53,12 +53,10 @@ __device__ __forceinline__ uint32_t word_of(float lo, float hi) {
     const uint32_t su = __bfloat16_as_ushort(s), mu = __bfloat16_as_ushort(m);
     return (su & 0x7f80u) == 0x7f80u || (mu & 0x7f80u) == 0x7f80u ? 0x7fff7fffu : su | (mu << 16);
 }
-// A number's code in a group of that scale and least value, as a whole float32 number; `inv` is the scale's reciprocal.  Where the scale is zero or no
-// number the quotient is no number, or none that counts, and the code is zero.
-__device__ __forceinline__ float code_of(float x, float s, float m, float inv) {
-    const float q = fminf(fmaxf(corrected(x - m, s, inv), 0.f), 15.f);
-    return (q + 12582912.f) - 12582912.f;          // 1.5 * 2^23: rounded to a whole number, halves to even
-}
+// A number's code in a group of that scale and least value, plus 1.5 * 2^23, which rounds it to a whole number (halves to even) and leaves it in the
+// lowest bits; `inv` is the scale's reciprocal.  Where the scale is zero or no number the quotient is no number, or none that counts, and the code is zero.
+constexpr float CODE_UP = 12582912.f;
+__device__ __forceinline__ float raised_code(float x, float s, float m, float inv) { return fminf(fmaxf(corrected(x - m, s, inv), 0.f), 15.f) + CODE_UP; }
 __device__ __forceinline__ float value_of(uint32_t code, uint32_t word) { return fmaf(scale_of(word), (float)code, least_of(word)); }
 
 }  // namespace xb4
