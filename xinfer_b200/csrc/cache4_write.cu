@@ -126,6 +126,30 @@ __device__ __forceinline__ void load8(const T* x, float (&v)[8]) {
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     }
 }
+// Eight numbers as they lie in memory.
+template <typename T>
+struct Eight {
+    uint4 u[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Eight<T> fetch8(const T* x) {
+    Eight<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(x)[i];
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void numbers(const Eight<T>& r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+        const uint32_t w[4] = {r.u[i].x, r.u[i].y, r.u[i].z, r.u[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (sizeof(T) == 2) v[2 * e] = __uint_as_float(w[e] << 16), v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+            else v[4 * i + e] = __uint_as_float(w[e]);
+        }
+    }
+}
 __device__ __forceinline__ uint32_t pack2bf(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
@@ -145,7 +169,7 @@ constexpr int TURN_NONE = 0, TURN_HALVES = 1, TURN_PAIRS = 2;
 template <typename T, int LPH, int TURN, bool FULL>
 __global__ void __launch_bounds__(VEC_WARPS * 32, 4)
 cache4_write_kernel(const WriteArgs A, int each) {
-    constexpr int HEADS = 32 / LPH;
+    constexpr int HEADS = 32 / LPH, AHEAD = 2;       // heads that are on their way
     pdl_overlap_few();
     const int lane = threadIdx.x & 31, li = lane & (LPH - 1), sub = lane / LPH, d = A.d;
     // a token's jobs: some for its query heads, then some for its keys and values
@@ -158,8 +182,9 @@ cache4_write_kernel(const WriteArgs A, int each) {
     const int c0 = active ? li * 8 : 0, groups = xb4::groups_of(d);
     const T* heads = static_cast<const T*>(A.qkv) + t * A.row_stride + c0 + (is_q ? 0 : (long long)A.nh * d);
     const int steps = min(each, (count - (h0 - sub) + HEADS - 1) / HEADS);
-    float next[8];
-    load8(heads + min(h0, count - 1) * d, next);
+    Eight<T> next[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) next[j] = fetch8(heads + min(h0 + j * HEADS, count - 1) * d);
     // the token's angles: of the vector's pair in the other half (the sine with its sign), or of its own four pairs
     const int half = A.rot / 16;                   // vectors of a half
     const bool turns = TURN != TURN_NONE && active && c0 < A.rot, upper = TURN == TURN_HALVES && li >= half;
@@ -219,15 +244,18 @@ cache4_write_kernel(const WriteArgs A, int each) {
     };
     if (is_q) {
         T* out = static_cast<T*>(A.q_out) + (long long)t * A.nh * d + c0;
-#pragma unroll 2
-        for (int i = 0; i < steps; ++i) {
-            const int h = h0 + i * HEADS;
-            float v[8];
+#pragma unroll 1
+        for (int i0 = 0; i0 < steps; i0 += AHEAD) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = next[e];
-            load8(heads + min(h + HEADS, count - 1) * d, next);
-            prepare(v, true);
-            if (h < count && active) store8(out + h * d, v);
+            for (int j = 0; j < AHEAD; ++j) {
+                if (i0 + j >= steps) break;
+                const int h = h0 + (i0 + j) * HEADS;
+                float v[8];
+                numbers(next[j], v);
+                if (i0 + AHEAD + j < steps) next[j] = fetch8(heads + min(h + AHEAD * HEADS, count - 1) * d);
+                prepare(v, true);
+                if (h < count && active) store8(out + h * d, v);
+            }
         }
         return;
     }
@@ -243,9 +271,10 @@ cache4_write_kernel(const WriteArgs A, int each) {
         const int h = h0 + i * HEADS;
         const bool is_k = h < A.nkv;
         float v[8];
+        numbers(next[0], v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = next[e];
-        load8(heads + min(h + HEADS, count - 1) * d, next);
+        for (int j = 0; j + 1 < AHEAD; ++j) next[j] = next[j + 1];
+        if (i + AHEAD < steps) next[AHEAD - 1] = fetch8(heads + min(h + AHEAD * HEADS, count - 1) * d);
         prepare(v, is_k);
         float lo = v[0], hi = v[0];
 #pragma unroll
@@ -278,10 +307,11 @@ cache4_write_kernel(const WriteArgs A, int each) {
 
 template <typename T, int LPH>
 int launch_vec(const WriteArgs& A, cudaStream_t stream) {
-    // as many heads a warp as leave every processor 32 warps
+    // As many heads a warp as leave every processor 32 warps, up to 16 times what lies side by side: a warp's angles and slot are a chain of trips.  8,192 tokens of
+    // 32 + 2 x 8 heads with 4, 8 and 16: 78, 65 and 51 us.
     const int together = 32 / LPH;
     int each = 1;
-    while (each < 8 && (long long)A.tokens * (A.nh + 2 * A.nkv) / (together * each * 2) >= 148 * 32) each *= 2;
+    while (each < 16 && (long long)A.tokens * (A.nh + 2 * A.nkv) / (together * each * 2) >= 148 * 32) each *= 2;
     const long long jobs = (long long)A.tokens * ((A.nh + together * each - 1) / (together * each) + (2 * A.nkv + together * each - 1) / (together * each));
     auto go = [&](auto kernel) { return xb_launch_few(kernel, dim3((unsigned)((jobs + VEC_WARPS - 1) / VEC_WARPS)), dim3(VEC_WARPS * 32), 0, stream, A, each); };
     auto form = [&](auto full) {
