@@ -17,7 +17,7 @@ __host__ __device__ constexpr int padded(int d) { return groups_of(d) * GROUP; }
 constexpr int smem_bytes(int dp) { return 4 * (RT * dp + KT * (dp + 4) + KT * dp + RT * (KT + 1) + KT * RT + 3 * RT + 2 * KT); }
 
 // Which rows of a job: row r is token r / group of the request, query head r % group.
-template <typename T>
+template <typename T, int NARROW>
 __global__ void __launch_bounds__(THREADS)
 cache4_attention_any_kernel(const AttendArgs A, float* parts, int splits) {
     extern __shared__ __align__(16) float mem[];
@@ -47,7 +47,10 @@ cache4_attention_any_kernel(const AttendArgs A, float* parts, int splits) {
             q[i] = y < many && c < d ? to_f32<T>(static_cast<const T*>(A.q)[row_of(y, A.q_stride) + c]) : 0.f;
         }
         if (tid < RT) m[tid] = -INFINITY, l[tid] = 0.f;
-        float acc[DIM_MOST / THREADS][RT] = {};
+        // sums: a thread has a channel and all rows, or (heads of up to 64 channels) half of the rows
+        constexpr int CHANNELS = NARROW ? 1 : DIM_MOST / THREADS, MINE = NARROW ? RT / 2 : RT;
+        const int own = NARROW ? tid % 64 : tid, rows0 = NARROW ? tid / 64 * MINE : 0;
+        float acc[CHANNELS][MINE] = {};
         __syncthreads();
         for (int tile = from; tile < to; ++tile) {
             if (tid < KT) {
@@ -64,6 +67,7 @@ cache4_attention_any_kernel(const AttendArgs A, float* parts, int splits) {
                 place[tid] = key % A.page_size;
             }
             __syncthreads();
+            bool strange = false;              // a value's group is no number: what does not see it must not add zero times that
             for (int i = tid; i < 2 * KT * groups; i += THREADS) {
                 const int key = i % KT, j = i / KT % groups;
                 const bool is_k = i < KT * groups;
@@ -75,6 +79,7 @@ cache4_attention_any_kernel(const AttendArgs A, float* parts, int splits) {
                     for (int e = 0; e < 4; ++e) code[e] = c4[e];
                     word = reinterpret_cast<const uint32_t*>(from_page + (long long)groups * A.page_size * GROUP_BYTES)[place[key] * groups + j];
                 }
+                strange |= !is_k && !(fabsf(scale_of(word)) < INFINITY && fabsf(least_of(word)) < INFINITY);
                 float* to_row = is_k ? k + key * (dp + 4) + j * GROUP : v + key * dp + j * GROUP;
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
@@ -89,7 +94,7 @@ cache4_attention_any_kernel(const AttendArgs A, float* parts, int splits) {
                     *reinterpret_cast<float4*>(to_row + e) = x;
                 }
             }
-            __syncthreads();
+            strange = __syncthreads_or(strange);
             {
                 const int key = tid % KT, y0 = tid / KT * (RT / 2);
                 float sum[RT / 2] = {};
@@ -123,7 +128,7 @@ cache4_attention_any_kernel(const AttendArgs A, float* parts, int splits) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const float w = expf(x[e] - base);
-                    p[(lane + 32 * e) * RT + y] = seen[e] ? w : -1.f;
+                    p[(lane + 32 * e) * RT + y] = seen[e] ? w : (strange ? -1.f : 0.f);
                     if (seen[e]) sum += w;
                 }
                 sum = warp_sum(sum);
@@ -137,35 +142,42 @@ cache4_attention_any_kernel(const AttendArgs A, float* parts, int splits) {
             }
             __syncthreads();
 #pragma unroll
-            for (int e = 0; e < DIM_MOST / THREADS; ++e) {
-                const int c = tid + e * THREADS;
+            for (int e = 0; e < CHANNELS; ++e) {
+                const int c = own + e * THREADS;
                 if (c >= dp) break;
 #pragma unroll
-                for (int y = 0; y < RT; ++y) acc[e][y] = alpha[y] == 0.f ? 0.f : acc[e][y] * alpha[y];
+                for (int y = 0; y < MINE; ++y) acc[e][y] = alpha[rows0 + y] == 0.f ? 0.f : acc[e][y] * alpha[rows0 + y];
+#pragma unroll 2
                 for (int key = 0; key < KT; ++key) {
                     const float x = v[key * dp + c];
-                    float w[RT];
+                    float w[MINE];
 #pragma unroll
-                    for (int y = 0; y < RT; y += 4) *reinterpret_cast<float4*>(w + y) = *reinterpret_cast<const float4*>(p + key * RT + y);
+                    for (int y = 0; y < MINE; y += 4) *reinterpret_cast<float4*>(w + y) = *reinterpret_cast<const float4*>(p + key * RT + rows0 + y);
+                    if (!strange) {
 #pragma unroll
-                    for (int y = 0; y < RT; ++y)
-                        if (!(w[y] < 0.f)) acc[e][y] = fmaf(w[y], x, acc[e][y]);      // (what is not seen adds nothing, whatever it is)
+                        for (int y = 0; y < MINE; ++y) acc[e][y] = fmaf(w[y], x, acc[e][y]);
+                    } else {
+#pragma unroll
+                        for (int y = 0; y < MINE; ++y)
+                            if (!(w[y] < 0.f)) acc[e][y] = fmaf(w[y], x, acc[e][y]);
+                    }
                 }
             }
             __syncthreads();
         }
 #pragma unroll
-        for (int e = 0; e < DIM_MOST / THREADS; ++e) {
-            const int c = tid + e * THREADS;
+        for (int e = 0; e < CHANNELS; ++e) {
+            const int c = own + e * THREADS;
             if (c >= d) break;
 #pragma unroll
-            for (int y = 0; y < RT; ++y) {
+            for (int j = 0; j < MINE; ++j) {
+                const int y = rows0 + j;
                 if (y >= many) break;
                 if (splits == 1) {
-                    static_cast<T*>(A.out)[row_of(y, A.out_stride) + c] = from_f32<T>(l[y] == 0.f ? 0.f : acc[e][y] / l[y]);
+                    static_cast<T*>(A.out)[row_of(y, A.out_stride) + c] = from_f32<T>(l[y] == 0.f ? 0.f : acc[e][j] / l[y]);
                 } else {
                     float* to_part = parts + ((long long)blockIdx.z * A.tokens * A.nh + row_of(y, (long long)A.nh * d) / d) * (d + 2);
-                    to_part[c] = acc[e][y];
+                    to_part[c] = acc[e][j];
                     if (c == 0) to_part[d] = m[y], to_part[d + 1] = l[y];
                 }
             }
@@ -219,9 +231,13 @@ AnyGrid any_grid(int requests, int nh, int nkv, int longest) {
 template <typename T>
 int launch_any(const AttendArgs& A, int longest, float* scratch, cudaStream_t stream) {
     const AnyGrid g = any_grid(A.requests, A.nh, A.nkv, longest);
-    static unsigned long long roomy = 0;
-    if (const int rc = xb_more_smem(cache4_attention_any_kernel<T>, smem_bytes(DIM_MOST), &roomy)) return rc;
-    int rc = xb_launch_few(cache4_attention_any_kernel<T>, dim3(g.row_tiles * A.nkv, A.requests, g.splits), dim3(THREADS), smem_bytes(padded(A.d)), stream, A, scratch, g.splits);
+    static unsigned long long roomy[2] = {0, 0};
+    const bool narrow = padded(A.d) <= 64;
+    auto go = [&](auto kernel, unsigned long long* done) {
+        if (const int rc = xb_more_smem(kernel, smem_bytes(DIM_MOST), done)) return rc;
+        return xb_launch_few(kernel, dim3(g.row_tiles * A.nkv, A.requests, g.splits), dim3(THREADS), smem_bytes(padded(A.d)), stream, A, scratch, g.splits);
+    };
+    const int rc = narrow ? go(cache4_attention_any_kernel<T, 1>, &roomy[0]) : go(cache4_attention_any_kernel<T, 0>, &roomy[1]);
     if (rc || g.splits == 1) return rc;
     const long long rows = (long long)A.tokens * A.nh;
     return xb_launch(cache4_attention_any_join_kernel<T>, dim3((unsigned)((rows + THREADS / 32 - 1) / (THREADS / 32))), dim3(THREADS), 0, stream, A, scratch, g.splits);
