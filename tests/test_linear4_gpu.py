@@ -116,6 +116,39 @@ def test_graphs_and_streams(tokens):
         assert torch.equal(out, want * 2)
 
 
+@pytest.mark.parametrize("tokens", [1, 12, 40])
+def test_weights_packed_here_or_laid_out_anew(tokens):
+    from xinfer_b200 import kernels as k
+    from xinfer_b200.weights import pack4
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randn((tokens, 1024), generator=gen, device=DEV).to(torch.bfloat16)
+    matrices = [torch.randn((512, 1024), generator=gen, device=DEV) for _ in range(3)]
+    wants = [product(x, pack4(m.cpu(), 64).to(DEV), 512) for m in matrices]
+    place = torch.zeros_like(pack4(matrices[0], 64))
+    for m, want in zip(matrices * 3, wants * 3):
+        out = torch.zeros_like(want)
+        k.linear4(out, x, pack4(m, 64))
+        assert torch.equal(out, want)
+        place.copy_(pack4(m, 64))
+        k.linear4(out.zero_(), x, place)
+        assert torch.equal(out, want)
+
+
+def test_calls_at_once():
+    from xinfer_b200 import kernels as k
+    cases = [case(tokens, 512, 2048, 64, torch.bfloat16) for tokens in (1, 16, 70, 300)]
+    wants = [product(x, w, 512) for x, w in cases]
+    outs, streams = [torch.zeros_like(y) for y in wants], [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (x, w), out, stream in zip(cases, outs, streams):
+            with torch.cuda.stream(stream):
+                out.zero_()
+                k.linear4(out, x, w)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, wants))
+
+
 def test_refusals():
     from xinfer_b200 import kernels as k
     from xinfer_b200.weights import pack4

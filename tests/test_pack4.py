@@ -5,6 +5,7 @@ import torch
 
 import fourbit
 from xinfer_b200 import kernels as k
+from xinfer_b200.native import wrap_module
 from xinfer_b200.weights import pack4
 
 
@@ -32,15 +33,18 @@ def test_groups_of_one_number():
 
 
 def test_refusals():
-    for bad in (torch.zeros(4), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(0, 4), torch.full((2, 2), float("nan")), torch.full((2, 2), float("inf"))):
+    for bad in (torch.zeros(4), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(0, 4), torch.full((2, 2), float("nan")), torch.full((2, 2), float("inf")),
+                torch.full((2, 2), -3.4e38), torch.tensor([[-3e38, 3e38]])):
         with pytest.raises(ValueError):
             pack4(bad)
+    # (the columns behind a weight are zeros, so a short group of numbers above zero has the least value 0, and 3.4e38 / 15 is an ordinary scale)
+    assert pack4(torch.full((2, 2), 3.4e38)).shape == (1, 1, 1280)
     for group in (0, 16, 48, 256):
         with pytest.raises(ValueError):
             pack4(torch.zeros(4, 4), group)
         with pytest.raises(k.KernelError):
             k.linear4_shape(4, 4, group)
-    for ps, d in ((0, 64), (16, 0), (16, 257)):
+    for ps, d in ((0, 64), (16, 0), (16, 257), (2 ** 27, 1), (2 ** 24, 256)):
         with pytest.raises(k.KernelError):
             k.cache4_page_bytes(ps, d)
     assert k.cache4_page_bytes(16, 128) == 1280 and k.cache4_page_bytes(8, 80) == 480
@@ -55,3 +59,12 @@ def test_tensors_on_the_host_are_refused():
         k.cache4_attention(x, x, cache, cache, i32(1), i32(2), i32(1, 2), 16, 1.0, i32(1))
     with pytest.raises(k.KernelError):
         k.linear4(torch.zeros(3, 8), torch.zeros(3, 64), pack4(torch.zeros(8, 64)))
+
+
+def test_the_first_tensor_of_another_device():
+    elsewhere = wrap_module().elsewhere
+    assert elsewhere(0) is None and elsewhere(0, None, None) is None
+    assert elsewhere(0, None, torch.zeros(1), torch.zeros(1)) == 1 and elsewhere(0, 3) == 0
+    for args in ((), ("x",), (None, torch.zeros(1))):
+        with pytest.raises(TypeError):
+            elsewhere(*args)

@@ -8,7 +8,7 @@
 //
 // Bound by reading the weight once.  A block's warps and the blocks of a cluster take a range of the columns each, for R tiles of rows at a time, and walk
 // over the rows' tiles; the codes are fetched two or four stages ahead, over the ends of the rows' tiles too (the first ones before the kernel in
-// front has ended: a weight is nobody's result).  Sums meet in shared memory, warp by warp and block by block in their order.
+// front has ended, which must not write the weight: waiting first takes 5.9 us instead of 5.1 for 4,096 x 4,096 and one row).  Sums meet in shared memory, warp by warp and block by block in their order.
 #include "linear4.h"
 
 namespace {

@@ -24,9 +24,14 @@ def pack4(weight: torch.Tensor, group: int = 32) -> torch.Tensor:
     g = full.view(rows * TILE_ROWS, -1, group)
     low = g.amin(2)
     scale, least = ((g.amax(2) - low) / 15).to(torch.bfloat16), low.to(torch.bfloat16)
+    if not bool(torch.isfinite(scale).all() & torch.isfinite(least).all()):
+        raise ValueError("a group of numbers that bfloat16 scales do not hold")
     s, m = scale.float().unsqueeze(2), least.float().unsqueeze(2)
     codes = torch.where(s > 0, torch.round((g - m) / torch.where(s > 0, s, 1.0)), 0.0).clamp_(0, 15).to(torch.uint8)
     # (tile, half, row, tile, word, lane, pair, place in the pair) -> (tile, tile, half, row, lane, word, place, pair)
     codes = codes.view(rows, 2, 8, cols, 4, 4, 4, 2).permute(0, 3, 1, 2, 5, 4, 7, 6).reshape(rows, cols, -1)
     words = torch.stack([scale, least], 2).view(torch.uint8).view(rows, TILE_ROWS, cols, -1).transpose(1, 2)
-    return torch.cat([codes[..., 0::2] | (codes[..., 1::2] << 4), words.reshape(rows, cols, -1)], 2)
+    packed = torch.cat([codes[..., 0::2] | (codes[..., 1::2] << 4), words.reshape(rows, cols, -1)], 2)
+    if packed.is_cuda:
+        torch.cuda.current_stream(packed.device).synchronize()       # (complete: products read a weight while the kernel ahead of them still runs)
+    return packed
