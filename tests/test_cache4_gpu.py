@@ -433,6 +433,61 @@ def test_graphs_and_streams(longest, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_calls_at_once(dtype):
+    """Calls on streams of their own, with scratch of their own: steps of single tokens, of portions, of both."""
+    from xinfer_b200 import kernels as k
+    calls = [Attend(news, contexts, 8, 2, 128, dtype, seed=i) for i, (news, contexts) in enumerate((([1] * 6, [700] * 6), ([130], [400]), ([1, 90, 1], [300, 20, 900]), ([40], [0])))]
+    wants, runs = [x.run().clone() for x in calls], []
+    for x in calls:
+        caches, lengths, start, table = x.tensors()
+        longest = max(x.news)
+        scratch = torch.zeros(max(1, k.cache4_attention_scratch(x.q.shape[0], len(x.news), 8, 2, 128, dtype, longest)), device=DEV)
+        runs.append(dict(out=x.out, q=x.q, k_cache=caches[0], v_cache=caches[1], lengths=lengths, token_start=start, block_table=table, page_size=x.ps, scale=x.scale, err=x.err,
+                         scratch=scratch, longest=longest))
+        x.out.fill_(9.0)
+    streams = [torch.cuda.Stream() for _ in runs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for run, stream in zip(runs, streams):
+            with torch.cuda.stream(stream):
+                k.cache4_attention(**run)
+    torch.cuda.synchronize()
+    for x, want in zip(calls, wants):
+        assert torch.equal(x.out, want) and int(x.err) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("news", [[3, 3], [70, 70]])
+def test_requests_of_the_same_pages(news, dtype):
+    a = Attend(news, [50, 50], 8, 2, 128, dtype)
+    a.table[1] = a.table[0]
+    a.run()
+    a.check()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("tokens", [1, 70])
+def test_batches_with_nobody_in_them(tokens, dtype):
+    """Requests without tokens (their lengths and rows of the table are anything), steps without tokens, steps without requests."""
+    from xinfer_b200 import kernels as k
+    a = Attend([tokens], [100], 8, 2, 128, dtype)
+    caches, _, _, table = a.tensors()
+    tables = torch.full((5, table.shape[1]), 2 ** 30, dtype=torch.int32, device=DEV)
+    tables[2] = table[0]
+    lengths, start = i32([0, 2 ** 31 - 1, a.lengths[0], -5, 77]), i32([0, 0, 0, tokens, tokens, tokens])
+    scratch = torch.zeros(max(1, k.cache4_attention_scratch(a.q.shape[0], 5, 8, 2, 128, dtype, tokens)), device=DEV)
+    a.out.fill_(9.0)
+    k.cache4_attention(a.out, a.q, *caches, lengths, start, tables, a.ps, a.scale, a.err, scratch=scratch, longest=tokens)
+    # (how often a row's keys are shared out goes by the number of requests, so the bits may be others than those of the request alone)
+    a.check()
+    assert bool((a.out[tokens:] == 9).all()) and int(a.err) == 0
+    k.cache4_attention(a.out[:0], a.q[:0], *caches, lengths, i32([0] * 6), tables, a.ps, a.scale, a.err, scratch=scratch)
+    k.cache4_attention(a.out.fill_(9.0), a.q, *caches, lengths[:0], start[:1], tables[:0], a.ps, a.scale, a.err, scratch=scratch)
+    k.cache4_attention(a.out, a.q, *caches, lengths, i32([0] * 6), tables, a.ps, a.scale, a.err, scratch=scratch)
+    assert bool((a.out == 9).all()) and int(a.err) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("news,d,ps", [([1, 2], 128, 8), ([1, 100], 128, 8), ([1, 100], 64, 16), ([3, 70], 48, 5)])
 def test_pages_that_a_window_has_left_behind(news, d, ps, dtype):
     """Their entries of the table are gone: nobody reads them and nothing is reported."""
@@ -503,7 +558,7 @@ def test_refusals():
     k.cache4_attention(**good)
     refused(out=a.out.float()), refused(q=a.q.half()), refused(k_cache=caches[0].int()), refused(v_cache=caches[1][:-1]), refused(lengths=lengths.long())
     refused(token_start=start[:-1]), refused(block_table=table[:1]), refused(page_size=8), refused(page_size=0), refused(window=0), refused(longest=0)
-    refused(q=a.q[:, :3], out=a.out[:, :3]), refused(scratch=torch.zeros(4, device=DEV)), refused(scratch=torch.zeros(room, device=DEV)[1:]), refused(err=a.err.long())
+    refused(q=a.q[:, :3], out=a.out[:, :3]), refused(scratch=torch.zeros(4, device=DEV)), refused(scratch=torch.zeros(room, device=DEV)[1:]), refused(err=a.err.long()), refused(err=a.err[:0]), refused(scale=float("nan")), refused(scale=float("inf"))
     refused(lengths=lengths.cpu()), refused(q=a.q.cpu()), refused(block_table=table.expand(2, table.shape[1])[:, ::2])
     w = Write(3, 4, 2, 64, BF, 16)
     base = dict(q_out=w.q_out, k_cache=w.caches[0], v_cache=w.caches[1], qkv=w.qkv, positions=w.positions, slots=w.slots, page_size=16, err=w.err, cos=w.cos, sin=w.sin)
@@ -516,7 +571,7 @@ def test_refusals():
     not_written(q_out=w.q_out.float()), not_written(k_cache=w.caches[0][:, :1]), not_written(qkv=w.qkv[:, :-1]), not_written(qkv=w.qkv.half()), not_written(slots=w.slots.int())
     not_written(positions=w.positions.long()), not_written(page_size=8), not_written(cos=None), not_written(sin=w.sin[:4]), not_written(q_norm=torch.ones(32, device=DEV))
     not_written(values=(w.values[0].float(), w.values[1])), not_written(cos=torch.zeros(5, 33, device=DEV), sin=torch.zeros(5, 33, device=DEV))
-    not_written(slots=w.slots.cpu()), not_written(positions=w.positions[:-1])
+    not_written(slots=w.slots.cpu()), not_written(positions=w.positions[:-1]), not_written(err=w.err[:0])
 
 
 # ---- a run of steps ---------------------------------------------------------------------------------------------------------

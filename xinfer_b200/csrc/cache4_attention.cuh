@@ -26,6 +26,7 @@ __device__ __forceinline__ int token_of(const AttendArgs& A, int row) { return (
 inline bool tokens_of_rows(const AttendArgs& A) { return (double)A.tokens * A.group * A.group < 4294967296.0; }
 
 constexpr int REQUESTS_MAX = 8192;
+constexpr int LINE_MOST = 0x70000000;            // tiles of a step's line of jobs (a share more is 32 bits still)
 constexpr long long KEYS_MOST = 0x7fff0000;      // keys that a row of the table may hold: their numbers, rounded up to tiles, are 32 bits
 
 // A request of the step.  Its token i stands at position first_pos + i and sees the keys up to there, of these the last `window`.
@@ -46,6 +47,23 @@ __device__ __forceinline__ Request request_of(const AttendArgs& A, int b) {
     const int rows = r.nodes * A.group;
     if (rows < A.rows_from || rows >= A.rows_to) r.nodes = 0;
     return r;
+}
+// The sum of the lanes' numbers up to each lane, and of all.  Requests whose tokens overlap can be more work than 32 bits count (others cannot, the
+// host has seen to that): reported, and nothing is done (-1).
+__device__ __forceinline__ int prefix_of_lanes(const AttendArgs& A, long long mine, int& incl) {
+    long long sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+        if ((int)(threadIdx.x & 31) >= o) sum += v;
+    }
+    incl = (int)sum;
+    const long long total = __shfl_sync(0xffffffffu, sum, 31);
+    if (total > LINE_MOST) {
+        atomicOr(A.err, XB_ERR_BAD_ROW);
+        return -1;
+    }
+    return (int)total;
 }
 // The first key that a token at `pos` sees.
 __device__ __forceinline__ int first_seen(const AttendArgs& A, int pos) { return A.window > 0 ? max(0, pos - A.window + 1) : 0; }

@@ -66,24 +66,20 @@ __device__ __forceinline__ void set_request(const AttendArgs& A, Walk& w, int b)
 template <int ROWS>
 __device__ __forceinline__ bool place_in_line(const AttendArgs& A, const Line& line, int me, int warps, Walk& w) {
     const int lane = threadIdx.x & 31, each = (A.requests + 31) / 32, b0 = lane * each, b1 = min(b0 + each, A.requests);
-    int mine = 0;
+    long long mine = 0;
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
         set_request<ROWS>(A, w, b);
-        mine += A.nkv * w.pieces * w.job_units();
+        mine += (long long)A.nkv * w.pieces * w.job_units();
     }
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-    }
-    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    int incl;
+    const int total = prefix_of_lanes(A, mine, incl);
+    if (total < 0) return false;
     w.share = (total + warps - 1) / warps;
     w.from = (int)min((long long)me * w.share, (long long)total);
     w.end = min(total, w.from + w.share);
     if (w.from >= w.end) return false;
-    int before = incl - mine, b = b0;
+    int before = incl - (int)mine, b = b0;
     const int owner = __ffs(__ballot_sync(0xffffffffu, w.from >= before && w.from < incl)) - 1;
     if (lane == owner) {
 #pragma unroll 1
@@ -705,7 +701,7 @@ bool mma_takes(int d) { return groups_of(d) <= 4 || groups_of(d) == 8; }
 bool mma_takes(const AttendArgs& A) {
     // the longest line that these shapes allow is counted in 32 bits
     const double jobs = (double)A.nkv * ((double)A.tokens * A.group / 8 + A.requests), tiles = (double)A.table_stride * A.page_size / KT + 2;
-    return mma_takes(A.d) && tokens_of_rows(A) && A.page_size % 8 == 0 && A.num_pages > 0 && jobs * (tiles + COST_JOB) < 2147483648.0;
+    return mma_takes(A.d) && tokens_of_rows(A) && A.page_size % 8 == 0 && A.num_pages > 0 && jobs * (tiles + COST_JOB) < LINE_MOST;
 }
 long long mma_scratch(int d, int rows) {
     return by_form(rows, groups_of(d), [](auto nt, auto ng) { return scratch_of<decltype(nt)::value, decltype(ng)::value>(); });

@@ -60,7 +60,7 @@ __device__ __forceinline__ void set_tiles(const AttendArgs& A, Walk& w, int node
     w.tiles = max(1, (min(w.r.first_pos + node1 + 1, w.r.keys) + KT - 1) / KT - w.tile0);       // (rows that see no key are written all the same)
 }
 __device__ __forceinline__ void set_piece(const AttendArgs& A, Walk& w) {
-    const int group = A.group, row0 = w.piece * ROWS;
+    const int row0 = w.piece * ROWS;
     set_tiles(A, w, token_of(A, row0), min(w.r.nodes - 1, token_of(A, row0 + ROWS - 1)));
 }
 __device__ __forceinline__ void set_request(const AttendArgs& A, Walk& w, int b) {
@@ -93,24 +93,20 @@ __device__ __forceinline__ int head_units(const AttendArgs& A, Walk& w) {
 
 __device__ __forceinline__ bool place_in_line(const AttendArgs& A, Walk& w) {
     const int lane = threadIdx.x & 31, each = (A.requests + 31) / 32, b0 = lane * each, b1 = min(b0 + each, A.requests);
-    int mine = 0;
+    long long mine = 0;
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
         set_request(A, w, b);
-        mine += A.nkv * head_units(A, w);
+        mine += (long long)A.nkv * head_units(A, w);
     }
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-    }
-    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    int incl;
+    const int total = prefix_of_lanes(A, mine, incl);
+    if (total < 0) return false;
     w.share = (total + (int)gridDim.x - 1) / (int)gridDim.x;
     w.from = (int)min((long long)blockIdx.x * w.share, (long long)total);
     w.end = min(total, w.from + w.share);
     if (w.from >= w.end) return false;
-    int before = incl - mine, b = b0;
+    int before = incl - (int)mine, b = b0;
     const int owner = __ffs(__ballot_sync(0xffffffffu, w.from >= before && w.from < incl)) - 1;
     if (lane == owner) {
 #pragma unroll 1
@@ -800,7 +796,7 @@ bool tc_takes(int nh, int nkv, int d, int longest) { return d <= 128 && (long lo
 bool tc_takes(const AttendArgs& A, int longest) {
     // the longest line that these shapes allow is counted in 32 bits
     const double jobs = (double)A.nkv * ((double)A.tokens * A.group / ROWS + A.requests), tiles = (double)A.table_stride * A.page_size / KT + 2;
-    return tc_takes(A.nh, A.nkv, A.d, longest) && tokens_of_rows(A) && A.scale > 0.f && A.num_pages > 0 && (long long)A.page_size * row_bytes(A.d) % 16 == 0 && jobs * (tiles + COST_JOB) < 2147483648.0;
+    return tc_takes(A.nh, A.nkv, A.d, longest) && tokens_of_rows(A) && A.scale > 0.f && A.num_pages > 0 && (long long)A.page_size * row_bytes(A.d) % 16 == 0 && jobs * (tiles + COST_JOB) < LINE_MOST;
 }
 long long tc_scratch(int d) { return (long long)BLOCKS * 2 * (ROWS * (dp_of(d) + 2) + JOB_WORDS); }
 int tc_launch(const AttendArgs& A, float* scratch, cudaStream_t stream) {

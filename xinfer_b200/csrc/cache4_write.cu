@@ -325,7 +325,7 @@ int launch_vec(const WriteArgs& A, cudaStream_t stream) {
 template <typename T>
 bool vec_takes(const WriteArgs& A) {
     auto on16 = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
-    return A.d % 8 == 0 && A.d <= 256 && (long long)A.page_size * xb4::row_bytes(A.d) < 0x7fffffffLL && A.row_stride * sizeof(T) % 16 == 0 && on16(A.qkv) && on16(A.q_out) && on16(A.q_w) && on16(A.k_w) && on16(A.k_values) && on16(A.v_values) &&
+    return A.d % 8 == 0 && A.d <= 256 && A.row_stride * sizeof(T) % 16 == 0 && on16(A.qkv) && on16(A.q_out) && on16(A.q_w) && on16(A.k_w) && on16(A.k_values) && on16(A.v_values) &&
            on16(A.cos_t) && on16(A.sin_t) && (!A.cos_t || A.rot % (A.interleaved ? 8 : 16) == 0);
 }
 
@@ -347,7 +347,7 @@ static int cache4_write(int dtype, void* q_out, uint8_t* k_cache, uint8_t* v_cac
                         long long row_stride, long long num_slots, int tokens, int nh, int nkv, int d, int rot, int interleaved, int page_size, int max_pos,
                         float eps, int* err, cudaStream_t stream) {
     if (tokens <= 0) return 0;
-    if (d < 1 || d > ANY_MOST || nh < 0 || nkv < 1 || page_size < 1 || rot < 0 || rot > d || rot % 2 || (cos_t && max_pos < 1)) return (int)cudaErrorInvalidValue;
+    if (d < 1 || d > ANY_MOST || nh < 0 || nkv < 1 || page_size < 1 || rot < 0 || rot > d || rot % 2 || (cos_t && max_pos < 1) || (long long)page_size * xb4::row_bytes(d) > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     if ((long long)tokens * (nh + 2 * nkv) > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     const WriteArgs A{q_out, k_cache, v_cache, qkv, q_w, k_w, rot ? cos_t : nullptr, sin_t, positions, slots, k_values, v_values, row_stride, num_slots, tokens, nh, nkv,
                       d, rot, interleaved, page_size, max_pos, eps, err};

@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import os
 from typing import Optional
 
@@ -2043,13 +2044,22 @@ def _here(*tensors) -> None:
         raise KernelError(f"a tensor on {tensors[at].device}: the call runs on the current device, cuda:{device}")
 
 
+def _word(err) -> None:
+    _check(err, "err", torch.int32, None)
+    if not err.numel():
+        raise KernelError("err: a word to report to")
+
+
 def cache4_page_bytes(page_size: int, d: int) -> int:
     """Bytes that a page of ``page_size`` tokens of one key/value head of ``d`` channels takes in 4 bits: 20 for every group of 32 channels of a
     token.  They are the codes of every group, 16 bytes for each slot (channel 2 i of the group in the low half of byte i), then for every slot the
     (s, m) pairs of its groups."""
     if not 1 <= d <= CACHE4_DIM_MAX or page_size < 1:
         raise KernelError(f"pages of {page_size} tokens with heads of {d} channels: of one token at least, and 1 to {CACHE4_DIM_MAX} channels")
-    return int(page_size) * 20 * (-(-int(d) // CACHE4_GROUP))
+    size = int(page_size) * 20 * (-(-int(d) // CACHE4_GROUP))
+    if size > 0x7fffffff:
+        raise KernelError(f"pages of {page_size} tokens with heads of {d} channels: {size} bytes, places in a page are counted in 32 bits")
+    return size
 
 
 def _cache4(k_cache, v_cache, page_size: int, nkv, d: int) -> tuple:
@@ -2083,7 +2093,7 @@ def cache4_write(q_out, k_cache, v_cache, qkv, positions, slots, page_size: int,
         raise KernelError(f"qkv: expected {dtype} CUDA rows {(T, (nh + 2 * nkv) * d)} with dense numbers, got {qkv.dtype} {tuple(qkv.shape)} with strides {qkv.stride()}")
     _check(positions, "positions", torch.int32, (T,))
     _check(slots, "slots", torch.int64, (T,))
-    _check(err, "err", torch.int32, None)
+    _word(err)
     for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
         if t is not None:
             _check(t, name, torch.float32, (d,))
@@ -2135,11 +2145,13 @@ def cache4_attention(out, q, k_cache, v_cache, lengths, token_start, block_table
         raise KernelError(f"{requests} requests; a call takes {TREE_REQUESTS_MAX}")
     _check(token_start, "token_start", torch.int32, (requests + 1,))
     _check(block_table, "block_table", torch.int32, (requests, None))
-    _check(err, "err", torch.int32, None)
+    _word(err)
     if block_table.shape[1] * page_size > 0x7fff0000:
         raise KernelError(f"a table of {block_table.shape[1]} pages of {page_size} tokens: keys are counted in 32 bits")
     if window is not None and window < 1:
         raise KernelError(f"a window of {window} keys")
+    if not math.isfinite(scale):
+        raise KernelError(f"a scale of {scale}")
     if longest is not None and longest < 1:
         raise KernelError(f"a longest request of {longest} tokens")
     longest = _longest(longest, T, 1)
@@ -2171,8 +2183,10 @@ def linear4_scratch(tokens: int, rows: int, columns: int, dtype) -> int:
 
 def linear4(out, x, weight, *, scratch=None):
     """``out[t, n] = sum_k x[t, k] * W[n, k]`` for rows ``x`` ``[T, columns]`` and a weight in 4 bits (``weights.pack4``); sums in float32, rounded once.
-    ``out`` is ``[T, rows]`` of x's type; rows of both may lie apart.  ``scratch``: float32, ``linear4_scratch`` numbers, contents undefined, not shared by calls that
-    may overlap."""
+    ``out`` is ``[T, rows]`` of x's type; rows of both may lie apart.  A weight is read before the kernel ahead in the stream has finished, so that kernel must
+    not write it (``pack4`` gives complete ones; a copy, a synchronisation or any other kernel in between will do).  bfloat16 holds its digits for x of up to 2^67 in
+    size (up to 16 rows), and scales of up to 2^60 (more rows); a row of x that is not finite gives a row that is not.  ``scratch``: float32, ``linear4_scratch``
+    numbers, contents undefined, not shared by calls that may overlap."""
     T, columns = x.shape
     rows = out.shape[1] if out.dim() == 2 else 0
     dtype = x.dtype
