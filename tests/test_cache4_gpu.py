@@ -502,7 +502,8 @@ def test_pages_that_a_window_has_left_behind(news, d, ps, dtype):
 
 @pytest.mark.parametrize("news,contexts,nh,nkv,d,window", [([200], [0], 4, 1, 128, None), ([64, 300], [700, 90], 8, 2, 128, None), ([130, 1, 70, 0, 2], [65, 500, 3, 8, 1000], 6, 2, 96, None),
                                                            ([90], [1000], 8, 8, 64, 100), ([257, 65], [31, 64], 3, 1, 32, 300), ([100, 5], [128, 900], 5, 1, 80, 77), ([80], [50], 2, 1, 256, None),
-                                                           ([500] * 3, [3000, 10, 600], 16, 8, 48, None)])
+                                                           ([500] * 3, [3000, 10, 600], 16, 8, 48, None), ([12, 3, 4, 15, 0], [200, 900, 31, 0, 9], 8, 2, 128, None),
+                                                           ([11, 4, 1], [70, 333, 800], 8, 2, 128, 100), ([3, 16, 2], [64, 40, 500], 16, 1, 64, None)])
 @pytest.mark.parametrize("ps", [16, 4, 24])
 def test_portions_of_prompts(news, contexts, nh, nkv, d, window, ps):
     a = Attend(news, contexts, nh, nkv, d, BF, ps=ps, window=window)

@@ -1,6 +1,10 @@
 // Attention of a step's tokens over a paged cache of 4-bit codes (codes4.cuh): token i of request b, at position lengths[b] - nodes + i, gets
 //   sum_j softmax_j(scale q . k_j) v_j   over the keys j up to its position, of these the last `window`; zeros if it sees none.
 // The step's own keys are in the cache already.  A page outside the pool is reported and its keys are not seen.
+//
+// Three kernels.  bfloat16, pages of a multiple of 8 tokens, heads of up to 128 channels or of 225 to 256: cache4_attention_mma.cu, which reads the keys once
+// for 8 or 16 rows.  Requests of TC_ROWS rows (tokens times query heads of a key/value head) and more, heads of up to 128 channels, a scale above zero, pages whose
+// bytes are a multiple of 16: cache4_attention_tc.cu, once for 256 rows.  Everything else, float32 first of all: the one below.
 #include "cache4_attention_mma.h"
 #include "cache4_attention_tc.h"
 
@@ -10,13 +14,15 @@ using namespace xb4;
 
 // ---- any type and size -----------------------------------------------------------------------------------------------------
 // A block per (16 rows, key/value head, request, share of the keys); the rows are (token, query head of the group) pairs.  A tile of 64 keys is
-// taken out of its codes once for the 16 rows; products in float32.
+// taken out of its codes once for the 16 rows; products in float32, whose multiply-adds and their operands in shared memory bound it.  Shares so
+// that two blocks have a processor; they are joined in their order by a second kernel.  Three requests of 13 tokens at up to 777 keys (window 256), 10 heads over 5 of 48
+// channels, float32: 21 us; with every thread holding all 16 rows of two channels (as heads of more than 64 channels have them) 31 us.
 constexpr int RT = 16, KT = 64, THREADS = 128, DIM_MOST = 256, SPLITS_MOST = 16, BLOCKS = 296;
 
 __host__ __device__ constexpr int padded(int d) { return groups_of(d) * GROUP; }
 constexpr int smem_bytes(int dp) { return 4 * (RT * dp + KT * (dp + 4) + KT * dp + RT * (KT + 1) + KT * RT + 3 * RT + 2 * KT); }
 
-// Which rows of a job: row r is token r / group of the request, query head r % group.
+// Row r is token r / group of the request, query head r % group.  NARROW: heads of up to 64 channels.
 template <typename T, int NARROW>
 __global__ void __launch_bounds__(THREADS)
 cache4_attention_any_kernel(const AttendArgs A, float* parts, int splits) {
@@ -254,14 +260,14 @@ static int cache4_attention(int dtype, void* out, const void* q, const uint8_t* 
     AttendArgs A{out, q, k_cache, v_cache, lengths, token_start, block_table, out_stride, q_stride, tokens, requests, table_stride, nh, nkv, d, page_size,
                        num_pages, window, nh / nkv, ((1ull << 32) + (unsigned)(nh / nkv) - 1) / (unsigned)(nh / nkv), 0, 0x7fffffff, scale, err};
     if (dtype == XB_BF16 && tc_takes(A, longest)) {
-        // requests of few rows beside those of many have the kernel for few: 64 single tokens at up to 4,096 keys beside a portion of 512 (both forms read the lengths on the device)
+        // requests of few rows beside those of many have the kernel for few (each reads on the device which requests are its own)
         const bool both = mma_takes(A);
         if (both) {
-            A.rows_from = TC_ROWS;
+            A.rows_from = OWN_ROWS;
             const int rc = tc_launch(A, scratch, stream);
             if (rc) return rc;
-            A.rows_from = 0, A.rows_to = TC_ROWS;
-            return mma_launch(A, TC_ROWS, scratch + tc_scratch(d), stream);
+            A.rows_from = 0, A.rows_to = OWN_ROWS;
+            return mma_launch(A, OWN_ROWS, scratch + tc_scratch(d), stream);
         }
         return tc_launch(A, scratch, stream);
     }

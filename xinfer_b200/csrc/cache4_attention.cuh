@@ -1,4 +1,4 @@
-// What the kernels of attention over a cache of 4-bit codes share (cache4_attention.cu says what they compute).
+// What the kernels of attention over a cache of 4-bit codes share (cache4_attention.cu says what they compute and which of them takes a call).
 #pragma once
 #include "codes4.cuh"
 

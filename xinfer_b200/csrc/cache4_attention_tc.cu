@@ -2,8 +2,8 @@
 // (cache4_attention.cu says what is computed).
 //
 // A job is (request, key/value head, up to two tiles of 128 rows): the rows are (token, query head of the group) pairs.  Warps 8..11 take tiles of 64
-// keys and values out of their codes, once for the 256 rows, into operands in shared memory (128-byte swizzle); S = Q K^T is issued by warp 12,
-// P = 2^(S - m) formed by a thread per row in warps 0..3 and 4..7, in the tensor memory of S, O += P V issued by warp 13.
+// keys and warps 12..15 tiles of 64 values out of their codes, once for the 256 rows, into operands in shared memory (128-byte swizzle); S = Q K^T is issued by
+// warp 16, P = 2^(S - m) formed by a thread per row in warps 0..3 and 4..7, in the tensor memory of S, O += P V issued by warp 17.
 //
 // All operands are float16: 11 digits of m + s code and of a probability, where bfloat16's 8 would each move the result as much as its own rounding
 // does.  float16's range is made up for by powers of two that are undone in float32: one per row of Q; one for every 16 keys of a tile, by which the
@@ -12,6 +12,9 @@
 // A group's word that is no number is zero in the operand; rows that see its key get no number in the group's channels at the end, the others nothing.
 //
 // The tiles of all jobs are one line cut into equal shares, one a block; parts of a job that blocks share are joined by a second kernel in their order.
+//
+// Bound by the softmax warps, 3,400 cycles for a tile of 64 keys and 256 rows (1,500 of them the exponentials), and by a job's start and end, 20,000 cycles.  Four
+// requests of up to 512 tokens at up to 4,096 keys, 32 heads over 8 of 128 channels: 104 us, a quarter of the products' rate.
 #include <cuda_fp16.h>
 
 #include "cache4_attention_tc.h"

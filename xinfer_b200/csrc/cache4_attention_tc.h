@@ -4,7 +4,11 @@
 
 namespace xb4 {
 
-constexpr int TC_ROWS = 64;        // from so many rows of a request's key/value head on
+// A step whose largest request has TC_ROWS rows of a key/value head has this kernel; in it, requests of fewer than OWN_ROWS are left to the one for few.  Few-row
+// kernel / this one (us, 32 heads over 8, up to 4,096 keys): 8 requests of up to 32 rows 34.4 / 34.1, 48 rows 38 / 34.5, 64 rows 45 / 34.8, 96 rows 55 / 36; 32 requests
+// of 48 91 / 83; one of 48 at 1,024 keys 18.3 / 20.1.  The 8 requests of 64 took 58 with those below 64 rows left to the other kernel: a second launch reads
+// lengths, places and parts again.
+constexpr int TC_ROWS = 48, OWN_ROWS = 16;
 
 bool tc_takes(int nh, int nkv, int d, int longest);                // whether it may, for a step's largest request
 bool tc_takes(const AttendArgs& A, int longest);
