@@ -4,13 +4,17 @@
 // Lane 4 g + t of a warp has rows g and g + 8 (two pieces of 16 bytes, 512 bytes apart) and in them the columns 32 j + 8 t + e of word j: as an
 // MMA's lanes take them, each word's columns in one group whatever the group's size.  Column e of a word lies in its half byte 4 (e & 1) +
 // e / 2, so that a mask takes out a pair of neighbours.  Rows and columns beyond the weight have codes and words of zeros.
+//
+// Three kernels: bfloat16 of up to 8 rows, up to 16 with small weights, and of any number off 16-byte boundaries, linear4_mma.cu; of more, linear4_tc.cu; float32
+// the one below.
 #include "linear4.h"
 
 namespace {
 
 using namespace xb4;
 
-// float32: a block per tile of rows and eight tokens, its warps take the column tiles in turn.  Products and sums in float32.
+// float32: a block per tile of rows and eight tokens, its warps take the column tiles in turn.  Products and sums in float32.  Few blocks of few trips:
+// five rows, 1,000 columns, 777 rows of the weight 5.8 us, a chain of codes, x, sums and launch.
 constexpr int ANY_WARPS = 8, ANY_TOKENS = 8;
 
 template <typename T>
@@ -77,14 +81,14 @@ int launch_any(const LinearArgs& A, cudaStream_t stream) {
 }  // namespace
 
 static int linear4(int dtype, void* out, const void* x, const uint8_t* weight, long long out_stride, long long x_stride, int tokens, int rows, int columns,
-                   int group, float* scratch, int* err, cudaStream_t stream) {
+                   int group, int* err, cudaStream_t stream) {
     if (tokens <= 0 || rows <= 0) return 0;
     if (columns < 1 || (group != 32 && group != 64 && group != 128) || tokens > 65535 * ANY_TOKENS) return (int)cudaErrorInvalidValue;
     const LinearArgs A{out, x, weight, out_stride, x_stride, tokens, rows, columns, TILE_COLS / group};
     if (dtype == XB_F32) return launch_any<float>(A, stream);
-    return A.tokens > 16 && linear4_tc_takes(A) ? linear4_tc(A, err, stream) : linear4_mma(A, stream);
+    // Few rows (us, few-row kernel / many-row kernel): 8 rows of 4,096 x 24,576 14.6 / 21, 9 rows 23.5 / 22.4, 16 rows of it 25.0 / 21.9, of 12,288 x 4,096 13.6 / 10.7, of
+    // 2,048 x 2,048 4.7 / 4.0, but of 1,024 x 1,024 2.7 / 3.9; 17 of that 4,096 x 24,576 43 / 22, of 4,096 x 4,096 8.7 / 6.8.
+    const bool many = A.tokens > 16 || (A.tokens > 8 && (long long)A.rows * A.columns > 1 << 20);
+    return many && linear4_tc_takes(A) ? linear4_tc(A, err, stream) : linear4_mma(A, stream);
 }
 XB_EXPORT int xb_linear4(const long long* words, int n) { return xb_by_words(linear4, words, n); }
-
-// float32 numbers of scratch for such a product
-XB_EXPORT long long xb_linear4_scratch(int dtype, int tokens, int rows, int columns) { return 0; }

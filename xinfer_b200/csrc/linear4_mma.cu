@@ -272,6 +272,7 @@ int with_group(const LinearArgs& A, cudaStream_t stream) {
 namespace xb4 {
 
 int linear4_mma(const LinearArgs& A, cudaStream_t stream) {
+    // (sixteen columns for eight rows or fewer: 4,096 x 24,576 23 us instead of 14.6)
     if (A.tokens > 8) return with_group<2, 2>(A, stream);
     // Four tiles of rows at a time take x out of memory half as often as two, but leave processors idle where they do not go round: whichever has less to do in
     // its longest block, with a sixth more work for two.

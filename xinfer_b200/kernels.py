@@ -2175,18 +2175,17 @@ def linear4_shape(rows: int, columns: int, group: int) -> tuple:
     return -(-int(rows) // 16), -(-int(columns) // 128), 1024 + 16 * (128 // group) * 4
 
 
-@functools.lru_cache(maxsize=4096)
 def linear4_scratch(tokens: int, rows: int, columns: int, dtype) -> int:
-    """float32 numbers of scratch that ``linear4`` takes for such a product; 0: none."""
-    return int(kernels_lib().xb_linear4_scratch(dtype_code(dtype), int(tokens), int(rows), int(columns)))
+    """float32 numbers of scratch that ``linear4`` takes for such a product: none for any, sums of shared columns meet in the processors' memory."""
+    return 0
 
 
 def linear4(out, x, weight, *, scratch=None):
     """``out[t, n] = sum_k x[t, k] * W[n, k]`` for rows ``x`` ``[T, columns]`` and a weight in 4 bits (``weights.pack4``); sums in float32, rounded once.
     ``out`` is ``[T, rows]`` of x's type; rows of both may lie apart.  A weight is read before the kernel ahead in the stream has finished, so that kernel must
     not write it (``pack4`` gives complete ones; a copy, a synchronisation or any other kernel in between will do).  bfloat16 holds its digits for x of up to 2^67 in
-    size (up to 16 rows), and scales of up to 2^60 (more rows); a row of x that is not finite gives a row that is not.  ``scratch``: float32, ``linear4_scratch``
-    numbers, contents undefined, not shared by calls that may overlap."""
+    size and scales of up to 2^60; a row of x that is not finite gives a row that is not.  ``scratch``: what
+    ``linear4_scratch`` asks for, which is nothing."""
     T, columns = x.shape
     rows = out.shape[1] if out.dim() == 2 else 0
     dtype = x.dtype
@@ -2201,13 +2200,5 @@ def linear4(out, x, weight, *, scratch=None):
         raise KernelError(f"weight: tiles of {weight.shape[2]} bytes belong to no group of 32, 64 or 128 columns")
     if weight.data_ptr() % 16:
         raise KernelError("weight: starts off a 16-byte boundary")
-    need = linear4_scratch(T, rows, columns, dtype)
-    if need:
-        _check(scratch, "scratch", torch.float32, None)
-        if scratch.numel() < need:
-            raise KernelError(f"scratch holds {scratch.numel()} numbers, {need} are needed")
-        if scratch.data_ptr() % 16:
-            raise KernelError("scratch starts off a 16-byte boundary")
     _here(out, x, weight, scratch)
-    _ok(_call(_entry("xb_linear4"), code, out, x, weight, at[1], at[0], T, rows, columns, group, scratch if need else None, own_err_word().data_ptr(),
-              _stream()), "linear4")
+    _ok(_call(_entry("xb_linear4"), code, out, x, weight, at[1], at[0], T, rows, columns, group, own_err_word().data_ptr(), _stream()), "linear4")

@@ -203,4 +203,3 @@ def _declare_kernels(lib):
          [P, P, P, P, P, P, P, P, I, I, I, I, I, I, L, I, I, I, F, F, F, P, F, I, I, I, I, P, I, P, P])
     _sig(lib, "xb_tree_attention_scratch", L, [I, I, I, I, I])
     _sig(lib, "xb_cache4_attention_scratch", L, [I, I, I, I, I, I, I])
-    _sig(lib, "xb_linear4_scratch", L, [I, I, I, I])
