@@ -6,7 +6,7 @@ namespace xb4 {
 
 bool mma_takes(int d);                        // whether it has a form for such heads
 bool mma_takes(const AttendArgs& A);
-// `rows`: of the request that has most, as far as it is known (64 of more)
+// `rows`: of the request that has most, as far as it is known (TC_ROWS of more)
 long long mma_scratch(int d, int rows);        // float32 numbers, on a 16-byte boundary
 int mma_launch(const AttendArgs& A, int rows, float* scratch, cudaStream_t stream);
 

@@ -1777,10 +1777,10 @@ TREE_REQUESTS_MAX = SLOT_REQUESTS_MAX = 8192
 # Checks and calls in native code, loaded at the first use (csrc/python/wrap.cpp): ``_check`` is ``_need``, ``_rows`` looks at rows that may
 # lie apart, ``_call`` calls an entry point of the kernels.
 def _load_wrap() -> None:
-    global _check, _rows, _call
+    global _check, _rows, _call, _elsewhere
     module = wrap_module()
     module.on_failure(_need_failed)
-    _check, _rows, _call = module.check, module.rows, module.call
+    _check, _rows, _call, _elsewhere = module.check, module.rows, module.call, module.elsewhere
 
 
 def _check(*args):
@@ -1796,6 +1796,11 @@ def _rows(*args):
 def _call(*args):
     _load_wrap()
     return _call(*args)
+
+
+def _elsewhere(*args):
+    _load_wrap()
+    return _elsewhere(*args)
 
 
 @functools.lru_cache(maxsize=None)
@@ -2039,7 +2044,7 @@ CACHE4_DIM_MAX = 256
 def _here(*tensors) -> None:
     """The kernels run on the current device: tensors of another one are an error."""
     device = torch.cuda.current_device() if _raw_stream is None else _device_index()
-    at = wrap_module().elsewhere(device, *tensors)
+    at = _elsewhere(device, *tensors)
     if at is not None:
         raise KernelError(f"a tensor on {tensors[at].device}: the call runs on the current device, cuda:{device}")
 
@@ -2062,13 +2067,15 @@ def cache4_page_bytes(page_size: int, d: int) -> int:
     return size
 
 
-def _cache4(k_cache, v_cache, page_size: int, nkv, d: int) -> tuple:
+def _cache4(k_cache, v_cache, page_size: int, d: int) -> tuple:
     """Checks the pages ``[pages, kv_heads, bytes]`` and gives (pages, kv_heads)."""
-    _check(k_cache, "k_cache", torch.uint8, (None, nkv, cache4_page_bytes(page_size, d)))
-    _check(v_cache, "v_cache", torch.uint8, tuple(k_cache.shape))
+    size = cache4_page_bytes(page_size, d)
+    _check(k_cache, "k_cache", torch.uint8, (None, None, size))
+    pages, nkv, _ = k_cache.shape
+    _check(v_cache, "v_cache", torch.uint8, (pages, nkv, size))
     if k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
         raise KernelError("a cache starts off a 16-byte boundary")
-    return k_cache.shape[0], k_cache.shape[1]
+    return pages, nkv
 
 
 def cache4_write(q_out, k_cache, v_cache, qkv, positions, slots, page_size: int, err, *, q_norm=None, k_norm=None, eps: float = 1e-6, cos=None, sin=None,
@@ -2084,7 +2091,7 @@ def cache4_write(q_out, k_cache, v_cache, qkv, positions, slots, page_size: int,
     T, nh, d = q_out.shape
     dtype = qkv.dtype
     code = dtype_code(dtype)
-    pages, nkv = _cache4(k_cache, v_cache, page_size, None, d)
+    pages, nkv = _cache4(k_cache, v_cache, page_size, d)
     if nkv < 1:
         raise KernelError("a cache without heads")
     _check(q_out, "q_out", dtype, (T, nh, d))
@@ -2102,8 +2109,9 @@ def cache4_write(q_out, k_cache, v_cache, qkv, positions, slots, page_size: int,
         raise KernelError("a rotation takes cosines and sines")
     if cos is not None:
         _check(cos, "cos", torch.float32, (None, None))
-        _check(sin, "sin", torch.float32, tuple(cos.shape))
-        most, rot = cos.shape[0], 2 * cos.shape[1]
+        most, half = cos.shape
+        _check(sin, "sin", torch.float32, (most, half))
+        rot = 2 * half
         if most < 1 or rot < 2 or rot > d:
             raise KernelError(f"a table of {most} positions and {rot} channels for heads of {d}")
     k_values = v_values = None
@@ -2134,7 +2142,7 @@ def cache4_attention(out, q, k_cache, v_cache, lengths, token_start, block_table
     T, nh, d = q.shape
     dtype = q.dtype
     code = dtype_code(dtype)
-    pages, nkv = _cache4(k_cache, v_cache, page_size, None, d)
+    pages, nkv = _cache4(k_cache, v_cache, page_size, d)
     if nkv < 1 or nh < 1 or nh % nkv:
         raise KernelError(f"{nh} query heads do not divide into {nkv} key/value heads")
     shape = (T, nh, d)
@@ -2175,6 +2183,9 @@ def linear4_shape(rows: int, columns: int, group: int) -> tuple:
     return -(-int(rows) // 16), -(-int(columns) // 128), 1024 + 16 * (128 // group) * 4
 
 
+_LINEAR4_GROUPS = {linear4_shape(1, 1, g)[2]: g for g in (32, 64, 128)}
+
+
 def linear4_scratch(tokens: int, rows: int, columns: int, dtype) -> int:
     """float32 numbers of scratch that ``linear4`` takes for such a product: none for any, sums of shared columns meet in the processors' memory."""
     return 0
@@ -2190,15 +2201,16 @@ def linear4(out, x, weight, *, scratch=None):
     rows = out.shape[1] if out.dim() == 2 else 0
     dtype = x.dtype
     code = dtype_code(dtype)
-    at = _rows(x, dtype, (T, columns)), _rows(out, dtype, (T, rows))
-    if None in at or rows < 1 or columns < 1:
+    x_row, out_row = _rows(x, dtype, (T, columns)), _rows(out, dtype, (T, rows))
+    if x_row is None or out_row is None or rows < 1 or columns < 1:
         raise KernelError(f"out and x: expected CUDA rows of one type with dense numbers, got {out.dtype} {tuple(out.shape)} with strides {out.stride()} and "
                           f"{x.dtype} {tuple(x.shape)} with strides {x.stride()}")
     _check(weight, "weight", torch.uint8, (-(-rows // 16), -(-columns // 128), None))
-    group = {1024 + 16 * (128 // g) * 4: g for g in (32, 64, 128)}.get(weight.shape[2])
+    tile = weight.shape[2]
+    group = _LINEAR4_GROUPS.get(tile)
     if group is None:
-        raise KernelError(f"weight: tiles of {weight.shape[2]} bytes belong to no group of 32, 64 or 128 columns")
+        raise KernelError(f"weight: tiles of {tile} bytes belong to no group of 32, 64 or 128 columns")
     if weight.data_ptr() % 16:
         raise KernelError("weight: starts off a 16-byte boundary")
     _here(out, x, weight, scratch)
-    _ok(_call(_entry("xb_linear4"), code, out, x, weight, at[1], at[0], T, rows, columns, group, own_err_word().data_ptr(), _stream()), "linear4")
+    _ok(_call(_entry("xb_linear4"), code, out, x, weight, out_row, x_row, T, rows, columns, group, own_err_word().data_ptr(), _stream()), "linear4")
