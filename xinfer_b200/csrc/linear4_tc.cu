@@ -20,6 +20,11 @@ using namespace xbtc;
 constexpr int ROWS = 128, CODE_WARPS = 16, TEAMS = CODE_WARPS / 4, THREADS = (CODE_WARPS + 2) * 32;
 constexpr int A_COLUMNS = TILE_COLS / 2;   // of tensor memory that a tile of the weight takes
 constexpr int TOKENS_MOST = 256, STAGES_MOST = 4;
+// Blocks of a cluster wait for each other while they hold all of their processors' tensor memory, and the waits for either have no limit: a block of
+// another kernel that does both (gemm_skinny_tc.cu, 37 KB of shared memory at least) on the same processor could hold columns that this one waits for while its
+// cluster waits for columns that this one's cluster holds elsewhere.  So a clustered launch takes so much of a processor's 228 KB of shared memory that no
+// block of that kernel, and none of this one, is there beside it.
+constexpr int SMEM_MOST = 201 * 1024, SMEM_CLUSTERED = SMEM_MOST;
 constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
 constexpr uint32_t UP = 0x5f805f80u, UP16 = 0x5d805d80u, DOWN = 0x1d001d00u;       // 2^64, 2^60, 2^-69, twice
 constexpr float BACK = 0x1p69f;
@@ -299,11 +304,12 @@ int launch(const LinearArgs& A, int* err, cudaStream_t stream) {
     T.tiles_per_split = (col_tiles + splits - 1) / splits;
     const int stage_bytes = 2 * T.mp * 128;
     T.stages = 200 * 1024 / stage_bytes < STAGES_MOST ? 200 * 1024 / stage_bytes : STAGES_MOST;
-    const int smem = (T.stages * stage_bytes > T.mp * ROWS * 4 ? T.stages * stage_bytes : T.mp * ROWS * 4) + 1024;        // (the sums lie where the stages did)
+    const int holds = (T.stages * stage_bytes > T.mp * ROWS * 4 ? T.stages * stage_bytes : T.mp * ROWS * 4) + 1024;        // (the sums lie where the stages did)
+    const int smem = splits > 1 && holds < SMEM_CLUSTERED ? SMEM_CLUSTERED : holds;
     CUtensorMap map;
     if (!map_of(&map, A, T.mp)) return (int)cudaErrorInvalidValue;
     static unsigned long long roomy = 0;
-    if (const int rc = xb_more_smem(linear4_tc_kernel<PER>, 201 * 1024, &roomy)) return rc;
+    if (const int rc = xb_more_smem(linear4_tc_kernel<PER>, SMEM_MOST, &roomy)) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks, splits, token_blocks);
     cfg.blockDim = dim3(THREADS);
