@@ -32,3 +32,38 @@ def test_products_on_two_streams_whose_blocks_hold_tensor_memory(tokens):
             k.gemm_skinny_tc(out16, x16, w16, err)
     torch.cuda.synchronize()
     assert torch.equal(out, want) and torch.equal(out16, want16) and int(err) == 0
+
+
+@pytest.mark.parametrize("tokens", [1, 12, 40])
+@pytest.mark.parametrize("between", [False, True])
+def test_a_weight_that_the_kernel_ahead_has_just_written(tokens, between):
+    """In front of the product a kernel writes the weight, or one that does and another that lets its successor start early; called and captured."""
+    from xinfer_b200 import kernels as k
+    from xinfer_b200.weights import pack4
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    x = torch.randn((tokens, 4096), generator=gen, device=DEV).to(BF)
+    weights = [pack4(torch.randn((2048, 4096), generator=gen, device=DEV), 64) for _ in range(2)]
+    wants = [product(x, w, 2048) for w in weights]
+    for w, want in zip(weights, wants):
+        assert torch.equal(product(x, w, 2048, weight_ready=True), want)
+    place, none, step = torch.zeros_like(weights[0]), torch.zeros_like(weights[0]), Write(1, 4, 2, 64, BF, 16)
+    outs = [torch.zeros_like(w) for w in wants]
+
+    def both():
+        for w, out in zip(weights, outs):
+            torch.bitwise_or(w, none, out=place)
+            if between:
+                step.run()
+            k.linear4(out, x, place)
+
+    for _ in range(20):
+        both()
+        assert all(torch.equal(a, b) for a, b in zip(outs, wants))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        both()
+    for _ in range(5):
+        for out in outs:
+            out.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs, wants))

@@ -81,10 +81,10 @@ int launch_any(const LinearArgs& A, cudaStream_t stream) {
 }  // namespace
 
 static int linear4(int dtype, void* out, const void* x, const uint8_t* weight, long long out_stride, long long x_stride, int tokens, int rows, int columns,
-                   int group, int* err, cudaStream_t stream) {
+                   int group, int early, int* err, cudaStream_t stream) {
     if (tokens <= 0 || rows <= 0) return 0;
     if (columns < 1 || (group != 32 && group != 64 && group != 128) || tokens > 65535 * ANY_TOKENS) return (int)cudaErrorInvalidValue;
-    const LinearArgs A{out, x, weight, out_stride, x_stride, tokens, rows, columns, TILE_COLS / group};
+    const LinearArgs A{out, x, weight, out_stride, x_stride, tokens, rows, columns, TILE_COLS / group, early};
     if (dtype == XB_F32) return launch_any<float>(A, stream);
     // Few rows (us, few-row kernel / many-row kernel): 8 rows of 4,096 x 24,576 14.9 / 22.4, 9 rows 23.5 / 22.4, 16 rows of it 25.0 / 21.9, of 12,288 x 4,096 13.6 / 10.7, of
     // 2,048 x 2,048 4.7 / 4.0, but of 1,024 x 1,024 2.7 / 3.9; 17 of that 4,096 x 24,576 43 / 22, of 4,096 x 4,096 8.7 / 6.8.

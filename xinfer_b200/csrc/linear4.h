@@ -10,6 +10,7 @@ struct LinearArgs {
     const uint8_t* weight;         // [row tiles, column tiles, tile bytes]
     long long out_stride, x_stride;
     int tokens, rows, columns, per_row;      // per_row: groups of a tile's row (4, 2, 1)
+    int early;                     // whatever wrote the weight has ended: it may be read before the kernel ahead has
 };
 
 int linear4_mma(const LinearArgs& A, cudaStream_t stream);                   // linear4_mma.cu

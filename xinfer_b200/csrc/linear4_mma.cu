@@ -7,8 +7,9 @@
 // x may be up to 2^67 in size; below 2^-100 it loses digits.
 //
 // Bound by reading the weight once.  A block's warps and the blocks of a cluster take a range of the columns each, for R tiles of rows at a time, and walk
-// over the rows' tiles; the codes are fetched two or four stages ahead, over the ends of the rows' tiles too (the first ones before the kernel in
-// front has ended, which must not write the weight: waiting first takes 5.9 us instead of 5.1 for 4,096 x 4,096 and one row).  Sums meet in shared memory, warp by warp and block by block in their order.
+// over the rows' tiles; the codes are fetched two or four stages ahead, over the ends of the rows' tiles too (where the caller says that the weight is
+// complete, the first ones before the kernel in front has ended: 5.1 us instead of 5.9 for 4,096 x 6,144 and one row).  Sums meet in shared memory, warp by
+// warp and block by block in their order.
 #include "linear4.h"
 
 namespace {
@@ -99,6 +100,7 @@ linear4_mma_kernel(const LinearArgs A, int cluster) {
         commit();
         put_slot = put_slot + 1 == STAGES ? 0 : put_slot + 1;
     };
+    if (!A.early) pdl_wait();
 #pragma unroll
     for (int i = 0; i < STAGES; ++i) fetch();
     pdl_launch_dependents();

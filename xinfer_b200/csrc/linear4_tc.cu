@@ -133,7 +133,8 @@ linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const TcArgs T) {
     pdl_launch_dependents();       // only now: see pdl_launch_dependents on tensor memory
 
     if (warp < CODE_WARPS) {
-        // ---- codes to numbers: row 32 (warp % 4) + lane of the block; the kernel in front must not write the weight, so nothing is waited for
+        // ---- codes to numbers: row 32 (warp % 4) + lane of the block
+        if (!A.early) pdl_wait();
         const int team = warp >> 2, in_tile = lane & 15;
         const int row_tile = min((int)blockIdx.x * 8 + (warp & 3) * 2 + (lane >> 4), row_tiles - 1);       // (behind the last row: it again)
         const uint8_t* next = A.weight + ((long long)row_tile * col_tiles + from + team) * TILE;

@@ -2191,10 +2191,11 @@ def linear4_scratch(tokens: int, rows: int, columns: int, dtype) -> int:
     return 0
 
 
-def linear4(out, x, weight, *, scratch=None):
+def linear4(out, x, weight, *, scratch=None, weight_ready: bool = False):
     """``out[t, n] = sum_k x[t, k] * W[n, k]`` for rows ``x`` ``[T, columns]`` and a weight in 4 bits (``weights.pack4``); sums in float32, rounded once.
-    ``out`` is ``[T, rows]`` of x's type; rows of both may lie apart.  A weight is read before the kernel ahead in the stream has finished, so that kernel must
-    not write it (``pack4`` gives complete ones; a copy, a synchronisation or any other kernel in between will do).  bfloat16 holds its digits for x of up to 2^67 in
+    ``out`` is ``[T, rows]`` of x's type; rows of both may lie apart.  ``weight_ready``: the caller's word that whatever wrote the weight had ended when the
+    call was made (a captured one: before its graph is launched), as it has for what ``pack4`` returns and for all that the host has waited for.  The weight is then read while the
+    kernels ahead in the stream still run; without it only behind them.  bfloat16 holds its digits for x of up to 2^67 in
     size and scales of up to 2^60; a row of x that is not finite gives a row that is not.  ``scratch``: what
     ``linear4_scratch`` asks for, which is nothing."""
     T, columns = x.shape
@@ -2213,4 +2214,4 @@ def linear4(out, x, weight, *, scratch=None):
     if weight.data_ptr() % 16:
         raise KernelError("weight: starts off a 16-byte boundary")
     _here(out, x, weight, scratch)
-    _ok(_call(_entry("xb_linear4"), code, out, x, weight, out_row, x_row, T, rows, columns, group, own_err_word().data_ptr(), _stream()), "linear4")
+    _ok(_call(_entry("xb_linear4"), code, out, x, weight, out_row, x_row, T, rows, columns, group, int(bool(weight_ready)), own_err_word().data_ptr(), _stream()), "linear4")
