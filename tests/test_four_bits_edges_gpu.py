@@ -67,3 +67,19 @@ def test_a_weight_that_the_kernel_ahead_has_just_written(tokens, between):
             out.zero_()
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(outs, wants))
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_products_report_to_the_word_they_are_given(tokens):
+    from xinfer_b200 import kernels as k
+    x, w = case(tokens, 128, 512, 64, BF)
+    out, err, own = torch.zeros((tokens, 128), dtype=BF, device=DEV), i32([0]), k.own_err_word()
+    own.value.value = k.ERR_WAIT                 # (as if a wait of an earlier call without a word had run out)
+    k.linear4(out, x, w, err=err)
+    assert int(err) == 0 and own.value.value == k.ERR_WAIT
+    with pytest.raises(k.KernelError):
+        k.linear4(out, x, w)
+    k.linear4(out, x, w)
+    for bad in (err.long(), err[:0], err.cpu(), 0):
+        with pytest.raises(k.KernelError):
+            k.linear4(out, x, w, err=bad)

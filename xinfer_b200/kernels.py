@@ -2191,12 +2191,13 @@ def linear4_scratch(tokens: int, rows: int, columns: int, dtype) -> int:
     return 0
 
 
-def linear4(out, x, weight, *, scratch=None, weight_ready: bool = False):
+def linear4(out, x, weight, *, scratch=None, weight_ready: bool = False, err=None):
     """``out[t, n] = sum_k x[t, k] * W[n, k]`` for rows ``x`` ``[T, columns]`` and a weight in 4 bits (``weights.pack4``); sums in float32, rounded once.
     ``out`` is ``[T, rows]`` of x's type; rows of both may lie apart.  ``weight_ready``: the caller's word that whatever wrote the weight had ended when the
     call was made (a captured one: before its graph is launched), as it has for what ``pack4`` returns and for all that the host has waited for.  The weight is then read while the
     kernels ahead in the stream still run; without it only behind them.  bfloat16 holds its digits for x of up to 2^67 in
-    size and scales of up to 2^60; a row of x that is not finite gives a row that is not.  ``scratch``: what
+    size and scales of up to 2^60; a row of x that is not finite gives a row that is not.  ``err``: the step's device error word, which says so where a wait has
+    run out (default: one that the next call without one looks at; a graph that is launched again and again has nobody who does).  ``scratch``: what
     ``linear4_scratch`` asks for, which is nothing."""
     T, columns = x.shape
     rows = out.shape[1] if out.dim() == 2 else 0
@@ -2213,5 +2214,8 @@ def linear4(out, x, weight, *, scratch=None, weight_ready: bool = False):
         raise KernelError(f"weight: tiles of {tile} bytes belong to no group of 32, 64 or 128 columns")
     if weight.data_ptr() % 16:
         raise KernelError("weight: starts off a 16-byte boundary")
-    _here(out, x, weight, scratch)
-    _ok(_call(_entry("xb_linear4"), code, out, x, weight, out_row, x_row, T, rows, columns, group, int(bool(weight_ready)), own_err_word().data_ptr(), _stream()), "linear4")
+    if err is not None:
+        _word(err)
+    _here(out, x, weight, scratch, err)
+    _ok(_call(_entry("xb_linear4"), code, out, x, weight, out_row, x_row, T, rows, columns, group, int(bool(weight_ready)),
+              err if err is not None else own_err_word().data_ptr(), _stream()), "linear4")
