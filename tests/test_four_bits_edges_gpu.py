@@ -83,3 +83,51 @@ def test_products_report_to_the_word_they_are_given(tokens):
     for bad in (err.long(), err[:0], err.cpu(), 0):
         with pytest.raises(k.KernelError):
             k.linear4(out, x, w, err=bad)
+
+
+@pytest.mark.parametrize("tokens,columns", [(1, 1100), (8, 1100), (12, 1100), (16, 1100), (40, 1100)])
+@pytest.mark.parametrize("x_size,w_size", [(1e-16, 1.0), (1e-22, 1.0), (1e-30, 1.0), (1e-35, 1.0), (1e20, 1.0), (1e30, 1e-3), (1.0, 1e-16), (1.0, 1e-25), (1.0, 1e30), (1e-30, 1e30), (1e30, 1e-25),
+                                           (1e-10, 1e-15)])
+def test_products_of_small_and_large_numbers(x_size, w_size, tokens, columns):
+    """The tolerance of test_linear4_gpu.check without its 1e-30: of each sum's terms, and of what is rounded; sums that bfloat16 holds as ordinary numbers."""
+    from xinfer_b200.weights import pack4
+    rows, group = 96, 64
+    gen = torch.Generator(device=DEV).manual_seed(tokens)
+    x = torch.randn((tokens, columns), generator=gen, device=DEV)
+    x = (x * x_size * 2.0 ** -torch.arange(tokens, device=DEV).remainder(4)[:, None].float()).to(BF)       # (rows of their own size)
+    x[tokens // 2, columns // 3:columns // 2] *= 2.0 ** -20
+    x[:, columns // 2:columns // 2 + 200] = 0
+    w = pack4(torch.randn((rows, columns), generator=gen, device=DEV) / columns ** 0.5 * w_size, group)
+    if tokens == 12:                       # (an odd start: the kernel for few rows reads x number by number)
+        x = torch.cat([torch.zeros_like(x[:, :1]), x], 1)[:, 1:]
+    got = product(x, w, rows)
+    value = torch.from_numpy(fourbit.weight_values(w.cpu().numpy(), group, rows, columns)).to(DEV)
+    want, size = x.double() @ value.T, x.double().abs() @ value.abs().T
+    allowed = 2.0 ** -8 * want.abs() + 3 * (columns / 16 + 64) * 2.0 ** -23 * size
+    if tokens > 16:
+        allowed = allowed + 2.0 ** -8 * torch.minimum(size, 6 * (x.double().square() @ value.square().T).sqrt())
+    off = (got.double() - want).abs()
+    assert bool((off <= allowed).all()), f"{(off / allowed).max().item():.2f} times what is allowed"
+
+
+@pytest.mark.parametrize("tokens,columns", [(1, 4096), (5, 4090), (8, 12288), (12, 1024), (40, 1100)])
+@pytest.mark.parametrize("low,high", [(1e-30, 1.0), (1.0, 1e30), (0.0, 1.0), (0.0, 1e-25), (1e-12, 1e2)])
+def test_products_of_rows_whose_numbers_grow(low, high, tokens, columns):
+    """Columns of one size in front of some of another, in every 512 columns and in the whole row; the rows beside such a row keep their bits."""
+    rows, group = 80, 32
+    x, w = case(tokens, rows, columns, group, BF)
+    clean = product(x, w, rows)
+    at, sizes = torch.arange(columns, device=DEV), torch.ones((tokens, columns), device=DEV)
+    sizes[0] = torch.where(at % 512 < 300, low, high)
+    sizes[tokens // 2] = torch.where(at < columns - 200, low, high)
+    x = (x.float() * sizes).to(BF)
+    got = product(x, w, rows)
+    value = torch.from_numpy(fourbit.weight_values(w.cpu().numpy(), group, rows, columns)).to(DEV)
+    want, size = x.double() @ value.T, x.double().abs() @ value.abs().T
+    allowed = 2.0 ** -8 * want.abs() + 3 * (columns / 16 + 64) * 2.0 ** -23 * size
+    if tokens > 16:
+        allowed = allowed + 2.0 ** -8 * torch.minimum(size, 6 * (x.double().square() @ value.square().T).sqrt())
+    off = (got.double() - want).abs()
+    assert bool((off <= allowed).all()), f"{(off / allowed).max().item():.2f} times what is allowed"
+    keep = [i for i in range(tokens) if i not in (0, tokens // 2)]
+    assert torch.equal(got[keep], clean[keep])

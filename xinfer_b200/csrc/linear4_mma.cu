@@ -2,9 +2,11 @@
 //
 // The weight's rows are the rows of the products, the tokens their columns.  The bits c of a code under a mask of four bits are the bfloat16
 // c 2^-133, in the next four bits 16 c 2^-133: a word of eight codes becomes eight operands by one shift and four masks, and nothing is subtracted.
-// x is scaled by 2^60 (2^56 in front of the 16-fold ones), so that sums are ordinary float32 numbers: 2^-73 of their value.  Per group of columns
+// Every warp scales each token's x by a power of two (and by a 16th of it in front of the 16-fold codes), by which its sums are divided before they meet the others', so
+// that they are ordinary float32 numbers whatever x's size is: the largest number of its first columns that are not all zero goes to 2^90 .. 2^91 (by 2^127 at
+// most).  Where a later one is more than 2^37 above it a product is not finite, and such a sum is formed again number by number.  (Eight rows of 4,096 x 24,576 take
+// 15.1 us, with one power for all 14.6, looking for the largest number of every 128 columns 16.0.)  Per group of columns
 //   y += s (code . x) + m sum(x),   sum(x) by a product of the same x with ones; both in float32.
-// x may be up to 2^67 in size; below 2^-100 it loses digits.
 //
 // Bound by reading the weight once.  A block's warps and the blocks of a cluster take a range of the columns each, for R tiles of rows at a time, and walk
 // over the rows' tiles; the codes are fetched two or four stages ahead, over the ends of the rows' tiles too (where the caller says that the weight is
@@ -18,8 +20,7 @@ using namespace xb4;
 
 constexpr int WARPS = 8, THREADS = WARPS * 32;
 constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u, ONES = 0x00010001u, ONES16 = 0x00100010u;      // ones of the scale of the codes
-constexpr uint32_t UP = 0x5d805d80u, UP16 = 0x5b805b80u;           // 2^60 and 2^56, twice
-constexpr float BACK = 0x1p73f;
+constexpr int X_TOP = 90, UP_MOST = 127;   // where a token's largest number goes, and the largest power of two in bfloat16
 
 constexpr int SLOTS = 2 * 148;             // blocks that the processors hold
 __host__ __device__ constexpr int stages(int r) { return r == 4 ? 2 : 4; }
@@ -46,6 +47,13 @@ __device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
+// The larger sizes of two pairs of numbers, whatever their signs; one that is no number wins.
+__device__ __forceinline__ uint32_t max_sizes(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }       // -126 <= e <= 127
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -58,6 +66,23 @@ __device__ __forceinline__ float of_rank(uint32_t addr, uint32_t rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
     return v;
+}
+
+// The sum of a token and a row of the weight, whose first tile `tile` is, number by number.
+template <int PER>
+__device__ __noinline__ float sum_by_number(const __nv_bfloat16* x, const uint8_t* tile, int row, int columns) {
+    float sum = 0.f;
+    for (int c0 = 0; c0 < columns && fabsf(sum) < INFINITY; c0 += TILE_COLS, tile += tile_bytes(PER)) {       // (what is not finite stays so)
+        float of_tile = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < min(TILE_COLS, columns - c0); ++c) {
+            const uint32_t codes = reinterpret_cast<const uint32_t*>(tile)[row * 16 + c % 32 / 8 * 4 + c / 32];
+            const int half = (c & 1) * 4 + (c & 7) / 2;                                            // (the half byte of the word)
+            of_tile = fmaf(__bfloat162float(x[c0 + c]), value_of(codes >> 4 * half & 15u, reinterpret_cast<const uint32_t*>(tile + TILE_CODES)[row * PER + c * PER / TILE_COLS]), of_tile);
+        }
+        sum += of_tile;
+    }
+    return sum;
 }
 
 template <int NT, int R, int PER>
@@ -123,11 +148,7 @@ linear4_mma_kernel(const LinearArgs A, int cluster) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) x16[n] = reinterpret_cast<const uint4*>(x + min(n * 8 + g, many - 1) * A.x_stride + t * 8);       // (columns without a token repeat the last one)
 
-    for (int rt0 = first; rt0 < row_tiles; rt0 += stride) {
-    float acc[R][NT][4] = {};
-    for (int ct = from; ct < to; ++ct) {
-        uint4 xv[NT][4];
-        // (asked for before the codes are waited for)
+    auto x_of = [&](int ct, uint4 (&xv)[NT][4]) {
         if (on16 && (ct + 1) * TILE_COLS <= A.columns) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -138,6 +159,32 @@ linear4_mma_kernel(const LinearArgs A, int cluster) {
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) xv[n][j] = load_x(n, ct * TILE_COLS + j * 32 + t * 8);
+        }
+    };
+    uint32_t up[NT];                                           // the power of two of the lane's token, twice
+#pragma unroll
+    for (int n = 0; n < NT; ++n) up[n] = (127 + UP_MOST) * 0x00800080u;
+    auto power_of = [&](int n) { return (int)(up[n] >> 23) - 127; };
+    unsigned known = 0;                                        // tokens that have theirs: those whose columns so far are not all zero
+    bool settled = false;
+    for (int rt0 = first; rt0 < row_tiles; rt0 += stride) {
+    float acc[R][NT][4] = {};
+    for (int ct = from; ct < to; ++ct) {
+        uint4 xv[NT][4];
+        x_of(ct, xv);                                          // (asked for before the codes are waited for)
+        if (!settled) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top = max_sizes(top, max_sizes(max_sizes(xv[n][j].x, xv[n][j].y), max_sizes(xv[n][j].z, xv[n][j].w)));
+                top = max_sizes(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max_sizes(top, __shfl_xor_sync(0xffffffffu, top, 2)) & 0x7fff7fffu;
+                const int size = (int)max(top & 0xffffu, top >> 16);             // (sizes of bfloat16 numbers compare as whole numbers)
+                if (size > 0 && !(known >> n & 1)) up[n] = (uint32_t)min(X_TOP + 254 - (size >> 7), 127 + UP_MOST) * 0x00800080u;
+                known |= (size > 0 || n * 8 + g >= many ? 1u : 0u) << n;
+            }
+            settled = __all_sync(0xffffffffu, known == (1u << NT) - 1);
         }
         wait_but<STAGES - 1>();
         __syncwarp();
@@ -163,7 +210,8 @@ linear4_mma_kernel(const LinearArgs A, int cluster) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const uint4 v = xv[n][j];
-                b[n][0] = times(v.x, UP), b[n][1] = times(v.y, UP16), b[n][2] = times(v.z, UP), b[n][3] = times(v.w, UP16);
+                const uint32_t up16 = up[n] - 4 * 0x00800080u;
+                b[n][0] = times(v.x, up[n]), b[n][1] = times(v.y, up16), b[n][2] = times(v.z, up[n]), b[n][3] = times(v.w, up16);
                 mma(ones[n], ONES, ONES, ONES16, ONES16, b[n][0], b[n][1]);
                 mma(ones[n], ONES, ONES, ONES16, ONES16, b[n][2], b[n][3]);
             }
@@ -202,21 +250,32 @@ linear4_mma_kernel(const LinearArgs A, int cluster) {
     constexpr int STRIDE = sums_stride(R), ROWS = R * TILE_ROWS;
     float* sums = reinterpret_cast<float*>(mem + ring_bytes(R, PER));
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int e = 0; e < 2; ++e) {
+            // (6 to 171, in two steps that both go up: nothing is lost or too large on the way)
+            const int of = 133 - __shfl_sync(0xffffffffu, power_of(n), (2 * t + e) * 4);
+            const float half = power_of_two(of / 2), rest = power_of_two(of - of / 2);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sums[(warp * NT * 8 + n * 8 + 2 * t + (e & 1)) * STRIDE + r * TILE_ROWS + g + 8 * (e >> 1)] = acc[r][n][e] * BACK;
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) sums[(warp * NT * 8 + n * 8 + 2 * t + e) * STRIDE + r * TILE_ROWS + g + 8 * h] = acc[r][n][2 * h + e] * half * rest;
+        }
     __syncthreads();
     const int n0 = rt0 * TILE_ROWS, total = many * ROWS;
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out);
+    auto store = [&](int token, int row, float v) {
+        if (n0 + row >= A.rows) return;
+        if (!(fabsf(v) < INFINITY)) v = sum_by_number<PER>(x + token * A.x_stride, A.weight + (long long)(rt0 + row / TILE_ROWS) * col_tiles * TILE, row % TILE_ROWS, A.columns);
+        out[(t0 + token) * A.out_stride + n0 + row] = __float2bfloat16_rn(v);
+    };
     for (int i = threadIdx.x; i < total; i += THREADS) {
         const int token = i / ROWS, row = i % ROWS;
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) v += sums[(w * NT * 8 + token) * STRIDE + row];
         if (cluster > 1) sums[token * STRIDE + row] = v;
-        else if (n0 + row < A.rows) out[(t0 + token) * A.out_stride + n0 + row] = __float2bfloat16_rn(v);
+        else store(token, row, v);
     }
     if (cluster > 1) {
         cluster_sync();
@@ -225,7 +284,7 @@ linear4_mma_kernel(const LinearArgs A, int cluster) {
             const int token = i / ROWS, row = i % ROWS;
             float v = 0.f;
             for (int k = 0; k < cluster; ++k) v += of_rank(base + (token * STRIDE + row) * 4, k);
-            if (n0 + row < A.rows) out[(t0 + token) * A.out_stride + n0 + row] = __float2bfloat16_rn(v);
+            store(token, row, v);
         }
         cluster_sync();                                        // (nobody leaves, or forms other sums, while its sums are read)
     } else {
