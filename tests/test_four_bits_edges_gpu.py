@@ -85,7 +85,7 @@ def test_products_report_to_the_word_they_are_given(tokens):
             k.linear4(out, x, w, err=bad)
 
 
-@pytest.mark.parametrize("tokens,columns", [(1, 1100), (8, 1100), (12, 1100), (16, 1100), (40, 1100)])
+@pytest.mark.parametrize("tokens,columns", [(1, 1100), (8, 1100), (12, 1100), (16, 1100), (40, 1100), (40, 1104), (300, 1104)])
 @pytest.mark.parametrize("x_size,w_size", [(1e-16, 1.0), (1e-22, 1.0), (1e-30, 1.0), (1e-35, 1.0), (1e20, 1.0), (1e30, 1e-3), (1.0, 1e-16), (1.0, 1e-25), (1.0, 1e30), (1e-30, 1e30), (1e30, 1e-25),
                                            (1e-10, 1e-15)])
 def test_products_of_small_and_large_numbers(x_size, w_size, tokens, columns):
@@ -110,7 +110,7 @@ def test_products_of_small_and_large_numbers(x_size, w_size, tokens, columns):
     assert bool((off <= allowed).all()), f"{(off / allowed).max().item():.2f} times what is allowed"
 
 
-@pytest.mark.parametrize("tokens,columns", [(1, 4096), (5, 4090), (8, 12288), (12, 1024), (40, 1100)])
+@pytest.mark.parametrize("tokens,columns", [(1, 4096), (5, 4090), (8, 12288), (12, 1024), (40, 1100), (40, 4096)])
 @pytest.mark.parametrize("low,high", [(1e-30, 1.0), (1.0, 1e30), (0.0, 1.0), (0.0, 1e-25), (1e-12, 1e2)])
 def test_products_of_rows_whose_numbers_grow(low, high, tokens, columns):
     """Columns of one size in front of some of another, in every 512 columns and in the whole row; the rows beside such a row keep their bits."""

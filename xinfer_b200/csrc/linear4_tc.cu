@@ -5,8 +5,8 @@
 // into 64 registers and stores them to its lane.  (Through shared memory the operand is written and read again at 128 bytes a cycle, which bound the
 // kernel: 850 cycles a column tile with 64 tokens.)  Four teams of four warps take every fourth column tile each.  One thread fetches the tokens'
 // columns by TMA, one warp issues the products.  A number of the weight becomes m + s code rounded to bfloat16 once, as a weight in bfloat16
-// would be: the bits of a code under a mask are the bfloat16 c 2^-133 (16 times that in the next four bits), so that one multiply-add of two numbers, by
-// s 2^64 and m 2^-69, gives them both times 2^-69, which the sums are multiplied by at the end.  Scales may be up to 2^60.
+// would be: the bits of a code under a mask are the bfloat16 c 2^-133 (16 times that in the next four bits), times 2^127 (2^123) they are c 2^-6, and a
+// multiply-add of two numbers with s 2^6 and m gives both.  Numbers and sums are what they stand for, whatever their size; scales may be up to 2^121.
 // K is split over a cluster's blocks where the row tiles alone do not fill the processors; their sums meet through distributed shared memory in
 // rank order.
 #include "linear4.h"
@@ -26,8 +26,7 @@ constexpr int TOKENS_MOST = 256, STAGES_MOST = 4;
 // block of that kernel, and none of this one, is there beside it.
 constexpr int SMEM_MOST = 201 * 1024, SMEM_CLUSTERED = SMEM_MOST;
 constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
-constexpr uint32_t UP = 0x5f805f80u, UP16 = 0x5d805d80u, DOWN = 0x1d001d00u;       // 2^64, 2^60, 2^-69, twice
-constexpr float BACK = 0x1p69f;
+constexpr uint32_t UP = 0x7f007f00u, UP16 = 0x7d007d00u, BACK = 0x42804280u;       // 2^127, 2^123, 2^6, twice
 
 struct TcArgs {
     LinearArgs a;
@@ -177,13 +176,13 @@ linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const TcArgs T) {
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const uint32_t w = have[i].w[(2 * p + q) * PER / 4];
-                        const uint32_t sc = __byte_perm(w, w, 0x1010), m = times(__byte_perm(w, w, 0x3232), DOWN), s1 = times(sc, UP), s16 = times(sc, UP16);
+                        const uint32_t sc = times(__byte_perm(w, w, 0x1010), BACK), m = __byte_perm(w, w, 0x3232);
 #pragma unroll
                         for (int t = 0; t < 4; ++t) {
                             const uint4& c = have[i].c[t];
                             const uint32_t u = p == 0 ? (q == 0 ? c.x : c.y) : (q == 0 ? c.z : c.w), u8 = u >> 8;
-                            v[q * 16 + t * 4] = fma_bf16(u & LOW, s1, m), v[q * 16 + t * 4 + 1] = fma_bf16(u & HIGH, s16, m);
-                            v[q * 16 + t * 4 + 2] = fma_bf16(u8 & LOW, s1, m), v[q * 16 + t * 4 + 3] = fma_bf16(u8 & HIGH, s16, m);
+                            v[q * 16 + t * 4] = fma_bf16(times(u & LOW, UP), sc, m), v[q * 16 + t * 4 + 1] = fma_bf16(times(u & HIGH, UP16), sc, m);
+                            v[q * 16 + t * 4 + 2] = fma_bf16(times(u8 & LOW, UP), sc, m), v[q * 16 + t * 4 + 3] = fma_bf16(times(u8 & HIGH, UP16), sc, m);
                         }
                     }
                     tmem_st32_u(to + p * 32, v);
@@ -261,10 +260,10 @@ linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const TcArgs T) {
             if (csize == 1) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (c0 + i < many && n0 + row < A.rows) out[(long long)(t0 + c0 + i) * A.out_stride + n0 + row] = __float2bfloat16_rn(v[i] * BACK);
+                    if (c0 + i < many && n0 + row < A.rows) out[(long long)(t0 + c0 + i) * A.out_stride + n0 + row] = __float2bfloat16_rn(v[i]);
             } else {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sums[(c0 + i) * ROWS + row] = v[i] * BACK;
+                for (int i = 0; i < 16; ++i) sums[(c0 + i) * ROWS + row] = v[i];
             }
         }
     }

@@ -2195,8 +2195,8 @@ def linear4(out, x, weight, *, scratch=None, weight_ready: bool = False, err=Non
     """``out[t, n] = sum_k x[t, k] * W[n, k]`` for rows ``x`` ``[T, columns]`` and a weight in 4 bits (``weights.pack4``); sums in float32, rounded once.
     ``out`` is ``[T, rows]`` of x's type; rows of both may lie apart.  ``weight_ready``: the caller's word that whatever wrote the weight had ended when the
     call was made (a captured one: before its graph is launched), as it has for what ``pack4`` returns and for all that the host has waited for.  The weight is then read while the
-    kernels ahead in the stream still run; without it only behind them.  bfloat16 holds its digits for x of up to 2^67 in
-    size and scales of up to 2^60; a row of x that is not finite gives a row that is not.  ``err``: the step's device error word, which says so where a wait has
+    kernels ahead in the stream still run; without it only behind them.  Numbers may have any size, scales up to 2^121 in
+    bfloat16; a row of x that is not finite gives a row that is not.  ``err``: the step's device error word, which says so where a wait has
     run out (default: one that the next call without one looks at; a graph that is launched again and again has nobody who does).  ``scratch``: what
     ``linear4_scratch`` asks for, which is nothing."""
     T, columns = x.shape
