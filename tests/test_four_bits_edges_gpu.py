@@ -131,3 +131,24 @@ def test_products_of_rows_whose_numbers_grow(low, high, tokens, columns):
     assert bool((off <= allowed).all()), f"{(off / allowed).max().item():.2f} times what is allowed"
     keep = [i for i in range(tokens) if i not in (0, tokens // 2)]
     assert torch.equal(got[keep], clean[keep])
+
+
+@pytest.mark.parametrize("dtype", [F32])
+@pytest.mark.parametrize("news,keys", [([1], 200), ([1], 3000), ([1] * 40, 500), ([70], 400)])
+def test_no_number_stays_where_later_scores_are_far_above(news, keys, dtype):
+    """A value's group of NaN that a row sees reaches its channels, however small the probability of its key is beside later ones."""
+    a = Attend(news, [keys] * len(news), 2, 1, 64, dtype, scale=1.0)
+    a.q.fill_(1.0)
+    level = torch.arange(a.pages, dtype=torch.float64)
+    for b in range(len(news)):             # pages in the order of the table: every 64 keys 160 above the last
+        for i, page in enumerate(a.table[b][:-(-a.lengths[b] // a.ps)]):
+            level[page] = 160.0 / 64 * (i * a.ps // 64)
+    a.data[0] = fourbit.page_bytes(np.broadcast_to(level.numpy()[:, None, None, None], (a.pages, 1, a.ps, 64)).copy(), a.ps)
+    clean = a.run().clone()
+    assert bool(torch.isfinite(clean).all())
+    words = a.data[1][..., 2 * a.ps * 16:].reshape(a.pages, 1, a.ps, 2, 4)
+    for b in range(len(news)):
+        words[a.table[b, 0], 0, 3, 1] = 0xFF               # key 3, the second group
+    got = a.run()
+    rows = sum(news)
+    assert bool(torch.isnan(got[:rows, :, 32:]).all()) and torch.equal(got[:rows, :, :32], clean[:rows, :, :32])

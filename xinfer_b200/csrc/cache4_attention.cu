@@ -152,7 +152,7 @@ cache4_attention_any_kernel(const AttendArgs A, float* parts, int splits) {
                 const int c = own + e * THREADS;
                 if (c >= dp) break;
 #pragma unroll
-                for (int y = 0; y < MINE; ++y) acc[e][y] = alpha[rows0 + y] == 0.f ? 0.f : acc[e][y] * alpha[rows0 + y];
+                for (int y = 0; y < MINE; ++y) acc[e][y] *= alpha[rows0 + y];         // (what is no number stays so, however far below a later score it is)
 #pragma unroll 2
                 for (int key = 0; key < KT; ++key) {
                     const float x = v[key * dp + c];
