@@ -133,7 +133,7 @@ def test_products_of_rows_whose_numbers_grow(low, high, tokens, columns):
     assert torch.equal(got[keep], clean[keep])
 
 
-@pytest.mark.parametrize("dtype", [F32])
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("news,keys", [([1], 200), ([1], 3000), ([1] * 40, 500), ([70], 400)])
 def test_no_number_stays_where_later_scores_are_far_above(news, keys, dtype):
     """A value's group of NaN that a row sees reaches its channels, however small the probability of its key is beside later ones."""
@@ -152,3 +152,57 @@ def test_no_number_stays_where_later_scores_are_far_above(news, keys, dtype):
     got = a.run()
     rows = sum(news)
     assert bool(torch.isnan(got[:rows, :, 32:]).all()) and torch.equal(got[:rows, :, :32], clean[:rows, :, :32])
+
+
+def with_values(a, sizes):
+    """The same request with new values, of a size for each page of the pool in the order of the tables."""
+    rng = np.random.default_rng(11)
+    nkv, d = a.sizes[1:]
+    level = np.ones(a.pages)
+    for b, length in enumerate(a.lengths):
+        held = -(-length // a.ps)
+        level[a.table[b, :held]] = sizes(np.arange(held) / max(1, held - 1))
+    a.data[1] = fourbit.page_bytes(rng.normal(size=(a.pages, nkv, a.ps, d)) * level[:, None, None, None], a.ps)
+    return a
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [128, 48, 256])
+@pytest.mark.parametrize("news,contexts", [([1, 6], [100, 37]), ([1], [3000]), ([100], [137])])
+@pytest.mark.parametrize("size", [1e-11, 1e-15, 1e-20, 1e-24, 1e10, 1e25])
+def test_values_of_any_size(size, news, contexts, d, dtype):
+    """Values' sizes apart from the keys', in each of the kernels."""
+    a = with_values(Attend(news, contexts, 8, 2, d, dtype), lambda at: size)
+    a.run()
+    a.check()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [128, 64])
+@pytest.mark.parametrize("news,contexts", [([1, 3], [700, 300]), ([1], [3000]), ([2] * 30, [400] * 30)])
+@pytest.mark.parametrize("first,last", [(1e-20, 1.0), (1.0, 1e-20), (1e-8, 1e8), (0.0, 1.0), (0.0, 1e-20)])
+def test_values_whose_sizes_change_from_page_to_page(first, last, news, contexts, d, dtype):
+    grow = lambda at: np.where(at < 0.4, 0.0, last) if first == 0 else first * (last / first) ** at  # noqa: E731
+    a = with_values(Attend(news, contexts, 8, 2, d, dtype), grow)
+    a.run()
+    a.check()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [128, 96, 256])
+@pytest.mark.parametrize("news,contexts", [([1, 1], [40, 700]), ([3], [500]), ([1], [3000]), ([60, 2], [100, 20])])
+def test_a_group_of_no_numbers_keeps_to_its_channels(news, contexts, d, dtype):
+    a = Attend(news, contexts, 4, 2, d, dtype)
+    clean = a.run().clone()
+    groups = d // 32
+    whole = a.data[1].copy()
+    words = a.data[1][..., groups * a.ps * 16:].reshape(a.pages, 2, a.ps, groups, 4)
+    for b in range(len(news)):
+        words[a.table[b, 1], 1, 3, 1] = 0xFF           # key 19, the second key/value head, channels 32 to 63
+    got, bad = a.run().clone(), torch.zeros_like(clean, dtype=torch.bool)
+    bad[:sum(news), 2:, 32:64] = True
+    assert bool(torch.isnan(got[bad]).all()) and torch.equal(got[:, :2], clean[:, :2])
+    # the other channels of these heads may have been summed up in another order: against 64 bits, like any sum
+    a.data[1] = whole
+    a.out.copy_(torch.where(bad, clean, got))
+    a.check()

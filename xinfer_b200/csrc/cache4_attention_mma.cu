@@ -11,6 +11,9 @@
 //   output: sum_keys (p s) (code - 8) + p (m + 8 s): p s is rounded to bfloat16 once, and around the middle of the codes that rounding is no
 //           larger than that of a probability times a value; the second sum is float32.  8 sum(p s) is a product with a constant operand.
 // The softmax's reference is a number per column that moves only when a score is more than 2^8 above it.
+// The products of values are ordinary float32 numbers for values from 2^-28 to 2^50 in size, beside which smaller ones count as part of a sum.  A segment whose
+// values are all smaller, that has larger ones, or a group that is no number, is known by its sums' sizes and done again number by number.  (A power of two
+// that follows the values instead: 64 single tokens 51 us instead of 48, the loop has no register for it.)
 //
 // The tiles (32 keys) of all jobs are one line cut into equal shares, one a warp, whatever the lengths are: warps of a block have nothing to do with each
 // other.  A warp fetches its keys and values into a ring of its own with bulk copies.  Parts of a job that several warps share are joined by a
@@ -199,9 +202,74 @@ __device__ __forceinline__ void load_query(const __nv_bfloat16* q, int c, int d,
     }
 }
 
+constexpr uint32_t VALUES_FROM = (127 - 28) << 7, VALUES_TO = (127 + 50) << 7, NO_NUMBER = 0x8000u;       // bits of bfloat16 sizes; above all of them
+
+// Bits of the largest scale or least value of a group's word, NO_NUMBER for one that is not finite.
+__device__ __forceinline__ uint32_t size_of_word(uint32_t word) {
+    const uint32_t size = max(word & 0x7fffu, word >> 16 & 0x7fffu);
+    return size >= 0x7f80u ? NO_NUMBER : size;
+}
+// The largest of some keys' values, out of the cache.
+template <int NG>
+__device__ __noinline__ uint32_t size_of_values(const AttendArgs& A, int b, int g, int from, int to) {
+    const int ps = A.page_size;
+    const long long page_bytes = (long long)ps * 20 * NG;
+    uint32_t most = 0;
+    for (int key = from + (int)(threadIdx.x & 31); key < to; key += 32) {
+        const int id = A.block_table[(long long)b * A.table_stride + key / ps];
+        if (id < 0 || id >= A.num_pages) continue;
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(A.v_cache + ((long long)id * A.nkv + g) * page_bytes + (long long)ps * 16 * NG) + key % ps * NG;
+        for (int n = 0; n < NG; ++n) most = max(most, size_of_word(words[n]));
+    }
+    return __reduce_max_sync(0xffffffffu, most);
+}
+// Keys `from` .. `to` of some rows, number by number: whole rows, or a part where `part_o` is given.
+template <int NG>
+__device__ __noinline__ void rows_by_number(const AttendArgs& A, int b, int g, int row0, int rows, int from, int to, float* part_o, float* part_ml) {
+    const int lane = threadIdx.x & 31, ps = A.page_size;
+    const Request r = request_of(A, b);
+    const long long page_bytes = (long long)ps * 20 * NG;
+    const int* table = A.block_table + (long long)b * A.table_stride;
+    for (int row = 0; row < rows; ++row) {
+        const int token = token_of(A, row0 + row), pos = r.first_pos + token;
+        const long long head = g * A.group + (row0 + row - token * A.group);
+        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(A.q) + (r.first + token) * A.q_stride + head * A.d;
+        float qv[NG], o[NG] = {}, top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < NG; ++n) qv[n] = 32 * n + lane < A.d ? __bfloat162float(q[32 * n + lane]) : 0.f;
+        for (int key = max(from, first_seen(A, pos)); key < min(min(to, pos + 1), r.keys); ++key) {
+            const int id = table[key / ps], slot = key % ps;
+            if (id < 0 || id >= A.num_pages) continue;             // (reported where it was to be fetched)
+            const uint8_t* page[2] = {A.k_cache + ((long long)id * A.nkv + g) * page_bytes, A.v_cache + ((long long)id * A.nkv + g) * page_bytes};
+            float x[2][NG], score = 0.f;
+#pragma unroll
+            for (int n = 0; n < NG; ++n)
+#pragma unroll
+                for (int v = 0; v < 2; ++v)                        // (channels behind the head have codes nobody wrote)
+                    x[v][n] = 32 * n + lane < A.d ? value_of(page[v][((long long)n * ps + slot) * 16 + lane / 2] >> 4 * (lane & 1) & 15u,
+                                                             reinterpret_cast<const uint32_t*>(page[v] + (long long)ps * 16 * NG)[slot * NG + n]) : 0.f;
+#pragma unroll
+            for (int n = 0; n < NG; ++n) score = fmaf(qv[n], x[0][n], score);
+            score = warp_sum(score) * (A.scale * 1.4426950408889634f);
+            const float now = max_nan(top, score), a = top == -INFINITY ? 0.f : xbtc::ex2(top - now), p = now == -INFINITY ? 0.f : xbtc::ex2(score - now);
+            top = now;
+            sum = fmaf(sum, a, p);
+#pragma unroll
+            for (int n = 0; n < NG; ++n) o[n] = fmaf(p, x[1][n], o[n] * a);
+        }
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(A.out) + (r.first + token) * A.out_stride + head * A.d;
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+            if (part_o) part_o[row * 32 * NG + 32 * n + lane] = o[n];
+            else if (32 * n + lane < A.d) out[32 * n + lane] = __float2bfloat16_rn(sum == 0.f ? 0.f : o[n] / sum);
+        }
+        if (part_o && lane == 0) *reinterpret_cast<float2*>(part_ml + row * 2) = make_float2(top, sum);
+    }
+}
+
 template <int NT, int NG>
 __global__ void __launch_bounds__(THREADS, per_sm(NT, NG))
-cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
+cache4_attention_mma_kernel(const __grid_constant__ AttendArgs A, const Line line) {
     extern __shared__ __align__(128) char mem[];
     constexpr int ROWS = 8 * NT, STAGES = stages(NG), STAGE = stage_bytes(NG), HALF = 20 * NG * STEP, CODES = NG * STEP * 16, DP = 32 * NG;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gi = lane >> 2, ti = lane & 3;
@@ -557,6 +625,27 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
         // ---- the segment's result: whole rows, or a part
         const bool whole = w.i0 == 0 && w.i1 == w.tiles;
         const size_t part = (size_t)me * 2 + (w.from > w.job ? 0 : 1);
+        // the sums' sizes: ordinary ones are finite, and not all below 2^-28 of the sum of probabilities (of which a lane has an eighth at least, if it has most)
+        uint32_t of_words = 0, of_codes = 0, of_p = 0;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                of_codes = max(of_codes, __float_as_uint(fabsf(eight[j][e])));
+                if constexpr (BY_WORDS) of_words = max(of_words, __float_as_uint(fabsf(both[j][e])));
+#pragma unroll
+                for (int n = 0; n < (BY_WORDS ? 0 : NG); ++n) of_words = max(of_words, __float_as_uint(fabsf(rest[j][n][e & 1])));
+                of_p = max(of_p, __float_as_uint(l[j][e & 1]) & 0x7fffffffu);
+            }
+        of_words = __reduce_max_sync(0xffffffffu, of_words), of_p = __reduce_max_sync(0xffffffffu, of_p);
+        const bool large = max(of_words, __reduce_max_sync(0xffffffffu, of_codes)) >= 0x7b800000u;       // (2^120: the lanes' parts are added up yet)
+        bool ordinary = true;
+        if (!failed && (large || (of_p > 0 && __uint_as_float(of_words) <= 0x1p-25f * __uint_as_float(of_p)))) {
+            const uint32_t most = size_of_values<NG>(A, w.b, w.g, max(from * STEP, first_key), min(min(to * STEP, pos1 + 1), w.r.keys));
+            ordinary = most == 0 || (most >= VALUES_FROM && most < VALUES_TO);         // (else it is the queries or keys, or signs that differ)
+        }
+        if (!ordinary) rows_by_number<NG>(A, w.b, w.g, row0, rows, max(from * STEP, first_key), to * STEP, whole ? nullptr : line.part_o + part * ROWS * DP, line.part_ml + part * ROWS * 2);
+        if (ordinary) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -599,6 +688,7 @@ cache4_attention_mma_kernel(const AttendArgs A, const Line line) {
                 // (minus infinity: there is nothing)
                 if (!whole && gi == 0 && row < rows) *reinterpret_cast<float2*>(line.part_ml + (part * ROWS + row) * 2) = make_float2(UP - base[j][e], sum);
             }
+        }
         if (!whole && lane == 0) {
             int* job = line.jobs + part * JOB_WORDS;
             const int first_warp = w.job / w.share, last = (w.job + w.tiles - 1) / w.share;
