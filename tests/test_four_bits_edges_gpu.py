@@ -206,3 +206,15 @@ def test_a_group_of_no_numbers_keeps_to_its_channels(news, contexts, d, dtype):
     a.data[1] = whole
     a.out.copy_(torch.where(bad, clean, got))
     a.check()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [128, 48, 7])
+@pytest.mark.parametrize("size", [1e-30, 1e-36, 1e-37, 1e-38, 1e-39, 1e30, 1e37])
+def test_write_numbers_of_any_size(size, d, dtype):
+    """Scales below the ordinary float32 numbers, whose reciprocals are infinite, and large ones: the definition's codes."""
+    w = Write(40, 2, 2, d, dtype, 16, norm=False, rot=0)
+    w.qkv.copy_((w.qkv.double() * size).to(dtype))
+    w.run()
+    w.check()
+    assert int(w.err) == 0

@@ -100,8 +100,8 @@ cache4_write_any_kernel(const WriteArgs A) {
             hi = xb4::max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
         const uint32_t word = xb4::word_of(lo, hi);
-        const float s = xb4::scale_of(word);
-        const uint32_t code = __float_as_uint(xb4::raised_code(v, s, xb4::least_of(word), xb4::reciprocal(s))) & 15u;
+        const float lift = xb4::scale_of(word) < xb4::TINY ? xb4::LIFT : 1.f, s = xb4::scale_of(word) * lift;
+        const uint32_t code = __float_as_uint(xb4::raised_code(v * lift, s, xb4::least_of(word) * lift, xb4::reciprocal(s))) & 15u;
         if (values && c < d) values[c] = __float2bfloat16_rn(xb4::value_of(code, word));
         uint32_t eight = code << (4 * (lane & 7));
 #pragma unroll
@@ -289,12 +289,19 @@ cache4_write_kernel(const WriteArgs A, int each) {
             hi = xb4::max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
         const uint32_t word = xb4::word_of(lo, hi);
-        const float s = xb4::scale_of(word), m = xb4::least_of(word), inv = xb4::reciprocal(s);
+        const float s = xb4::scale_of(word), m = xb4::least_of(word);
+        float of_s = s, of_m = m;
+        if (s < xb4::TINY) {
+            of_s *= xb4::LIFT, of_m *= xb4::LIFT;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= xb4::LIFT;
+        }
+        const float inv = xb4::reciprocal(of_s);
         uint32_t codes = 0u - 0x3f400000u;                     // (what the raised codes' upper bits come to, modulo 2^32)
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float c = xb4::raised_code(v[e], s, m, inv);
+            const float c = xb4::raised_code(v[e], of_s, of_m, inv);
             codes += __float_as_uint(c) << (4 * e);
             y[e] = fmaf(s, c - xb4::CODE_UP, m);
         }

@@ -55,7 +55,8 @@ __device__ __forceinline__ uint32_t word_of(float lo, float hi) {
 }
 // A number's code in a group of that scale and least value, plus 1.5 * 2^23, which rounds it to a whole number (halves to even) and leaves it in the
 // lowest bits; `inv` is the scale's reciprocal.  Where the scale is zero or no number the quotient is no number, or none that counts, and the code is zero.
-constexpr float CODE_UP = 12582912.f;
+// Below TINY a scale's reciprocal, or a remainder, is no ordinary number: scale, least value and numbers are taken LIFT times their size then, which is exact.
+constexpr float CODE_UP = 12582912.f, TINY = 0x1p-100f, LIFT = 0x1p100f;
 __device__ __forceinline__ float raised_code(float x, float s, float m, float inv) { return fminf(fmaxf(corrected(x - m, s, inv), 0.f), 15.f) + CODE_UP; }
 __device__ __forceinline__ float value_of(uint32_t code, uint32_t word) { return fmaf(scale_of(word), (float)code, least_of(word)); }
 
