@@ -218,3 +218,16 @@ def test_write_numbers_of_any_size(size, d, dtype):
     w.run()
     w.check()
     assert int(w.err) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 40 + 1])
+@pytest.mark.parametrize("news,contexts", [([1, 5], [150, 60]), ([70], [30])])
+def test_windows_and_longest_requests_that_32_bits_do_not_hold(news, contexts, window, dtype):
+    """A window of more keys than there are is none; a request brings no more tokens than the step has."""
+    a = Attend(news, contexts, 4, 2, 64, dtype)
+    want = a.run().clone()
+    a.window = window
+    assert torch.equal(a.run(), want)
+    a.run(longest=window)
+    a.check()

@@ -2127,7 +2127,7 @@ def cache4_write(q_out, k_cache, v_cache, qkv, positions, slots, page_size: int,
 @functools.lru_cache(maxsize=4096)
 def cache4_attention_scratch(tokens: int, requests: int, nh: int, nkv: int, d: int, dtype, longest: Optional[int] = None) -> int:
     """float32 numbers of scratch that ``cache4_attention`` takes for such a step; 0: none."""
-    longest = _longest(longest, tokens, 1)
+    longest = max(1, min(_longest(longest, tokens, 1), int(tokens)))
     return int(kernels_lib().xb_cache4_attention_scratch(dtype_code(dtype), int(tokens), int(requests), int(nh), int(nkv), int(d), longest))
 
 
@@ -2162,7 +2162,7 @@ def cache4_attention(out, q, k_cache, v_cache, lengths, token_start, block_table
         raise KernelError(f"a scale of {scale}")
     if longest is not None and longest < 1:
         raise KernelError(f"a longest request of {longest} tokens")
-    longest = _longest(longest, T, 1)
+    longest = max(1, min(_longest(longest, T, 1), T))
     need = cache4_attention_scratch(T, requests, nh, nkv, d, dtype, longest)
     if need:
         _check(scratch, "scratch", torch.float32, None)
@@ -2172,7 +2172,7 @@ def cache4_attention(out, q, k_cache, v_cache, lengths, token_start, block_table
             raise KernelError("scratch starts off a 16-byte boundary")
     _here(out, q, k_cache, v_cache, lengths, token_start, block_table, err, scratch)
     _ok(_call(_entry("xb_cache4_attention"), code, out, q, k_cache, v_cache, lengths, token_start, block_table, so, sq, T, requests, block_table.shape[1], nh, nkv,
-              d, int(page_size), pages, int(window or 0), longest, float(scale), scratch if need else None, err, _stream()), "cache4_attention")
+              d, int(page_size), pages, min(int(window or 0), 0x7fffffff), longest, float(scale), scratch if need else None, err, _stream()), "cache4_attention")
 
 
 def linear4_shape(rows: int, columns: int, group: int) -> tuple:
