@@ -256,7 +256,7 @@ static int cache4_attention(int dtype, void* out, const void* q, const uint8_t* 
                             int d, int page_size, int num_pages, int window, int longest, float scale, float* scratch, int* err, cudaStream_t stream) {
     if (tokens <= 0 || requests <= 0) return 0;
     if (requests > REQUESTS_MAX || d < 1 || d > DIM_MOST || nkv < 1 || nh < nkv || nh % nkv || page_size < 1 || (long long)page_size * row_bytes(d) > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-    if ((long long)table_stride * page_size > KEYS_MOST || (long long)tokens * nh > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+    if ((long long)table_stride * page_size > KEYS_MOST || (long long)tokens * nh > ROWS_MOST) return (int)cudaErrorInvalidValue;
     AttendArgs A{out, q, k_cache, v_cache, lengths, token_start, block_table, out_stride, q_stride, tokens, requests, table_stride, nh, nkv, d, page_size,
                        num_pages, window, nh / nkv, ((1ull << 32) + (unsigned)(nh / nkv) - 1) / (unsigned)(nh / nkv), 0, 0x7fffffff, scale, err};
     if (dtype == XB_BF16 && tc_takes(A, longest)) {

@@ -26,6 +26,7 @@ __device__ __forceinline__ int token_of(const AttendArgs& A, int row) { return (
 inline bool tokens_of_rows(const AttendArgs& A) { return (double)A.tokens * A.group * A.group < 4294967296.0; }
 
 constexpr int REQUESTS_MAX = 8192;
+constexpr int ROWS_MOST = 0x7ffff000;            // rows of a step: their numbers, rounded up to blocks, are 32 bits
 constexpr int LINE_MOST = 0x70000000;            // tiles of a step's line of jobs (a share more is 32 bits still)
 constexpr long long KEYS_MOST = 0x7fff0000;      // keys that a row of the table may hold: their numbers, rounded up to tiles, are 32 bits
 
