@@ -231,3 +231,35 @@ def test_windows_and_longest_requests_that_32_bits_do_not_hold(news, contexts, w
     assert torch.equal(a.run(), want)
     a.run(longest=window)
     a.check()
+
+
+@pytest.mark.parametrize("d,window", [(128, None), (64, 100), (96, None), (40, None)])
+@pytest.mark.parametrize("news,contexts", [([12, 3, 4, 15, 0], [200, 900, 31, 0, 9]), ([4, 13, 6], [640, 200, 77]), ([15], [1500])])
+def test_requests_of_16_to_63_rows_beside_larger_ones(news, contexts, d, window):
+    """Steps whose largest request has 48 rows and more: requests of 16 and more have the kernel for many, with float16 operands, and its bound: a probability and
+    a value are off by 2^-11 of themselves (values by 2^-25 of the largest at least), a key by that in every product of a score."""
+    nh, nkv = 8, 2
+    a = Attend(news, contexts, nh, nkv, d, BF, window=window)
+    got = a.run().double().cpu().numpy()
+    keys, vals = (fourbit.page_values(x, a.ps, d) for x in a.data)
+    q = a.q.double().cpu().numpy()
+    assert max(news) * (nh // nkv) >= 48
+    for b, n in enumerate(news):
+        if n * (nh // nkv) < 16:
+            continue
+        j = np.arange(a.lengths[b])
+        page = a.table[b][j // a.ps]
+        for i in range(n):
+            pos, t = a.lengths[b] - n + i, a.start[b] + i
+            seen = (j <= pos) & (j > pos - (window or 2 ** 31))
+            for h in range(nh):
+                kk, vv = keys[page, h // 4, j % a.ps][seen], vals[page, h // 4, j % a.ps][seen]
+                x = kk @ q[t, h] * a.scale
+                p = np.exp(x - x.max())
+                p /= p.sum()
+                want, size = p @ vv, p @ np.abs(vv)
+                steps = np.abs(kk).max() * np.abs(q[t, h]).sum() * a.scale
+                allowed = HALF[BF] * np.abs(want) + (2 * (d + 16) * 2.0 ** -23 * steps + (64 + seen.sum() / 16) * 2.0 ** -23) * size
+                allowed = allowed + (2 + 2 * float((p * (np.abs(kk) @ np.abs(q[t, h]))).sum() * a.scale)) * 2.0 ** -11 * size + 2.0 ** -25 * np.abs(vv).max()
+                off = np.abs(got[t, h] - want)
+                assert np.all(off <= allowed), (b, i, h, (off / allowed).max())

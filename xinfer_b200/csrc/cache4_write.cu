@@ -117,17 +117,9 @@ cache4_write_any_kernel(const WriteArgs A) {
 // token's angles.
 constexpr int VEC_WARPS = 8;
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* x, float (&v)[8]) {
-    if constexpr (sizeof(T) == 2) {
-        const uint4 u = *reinterpret_cast<const uint4*>(x);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
-    } else {
-        const float4 a = reinterpret_cast<const float4*>(x)[0], b = reinterpret_cast<const float4*>(x)[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    }
+__device__ __forceinline__ void load8(const float* x, float (&v)[8]) {
+    const float4 a = reinterpret_cast<const float4*>(x)[0], b = reinterpret_cast<const float4*>(x)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 // Eight numbers as they lie in memory.
 template <typename T>

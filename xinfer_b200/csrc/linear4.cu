@@ -15,20 +15,19 @@ using namespace xb4;
 
 // float32: a block per tile of rows and eight tokens, its warps take the column tiles in turn.  Products and sums in float32.  Few blocks of few trips:
 // five rows, 1,000 columns, 777 rows of the weight 5.8 us, a chain of codes, x, sums and launch.
-constexpr int ANY_WARPS = 8, ANY_TOKENS = 8;
+constexpr int F32_WARPS = 8, F32_TOKENS = 8;
 
-template <typename T>
-__global__ void __launch_bounds__(ANY_WARPS * 32)
-linear4_any_kernel(const LinearArgs A) {
-    __shared__ float part[ANY_WARPS][ANY_TOKENS][TILE_ROWS];
+__global__ void __launch_bounds__(F32_WARPS * 32)
+linear4_f32_kernel(const LinearArgs A) {
+    __shared__ float part[F32_WARPS][F32_TOKENS][TILE_ROWS];
     pdl_overlap_few();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int col_tiles = (A.columns + TILE_COLS - 1) / TILE_COLS, tile_bytes = TILE_CODES + TILE_ROWS * A.per_row * 4;
-    const int t0 = blockIdx.y * ANY_TOKENS, many = min(ANY_TOKENS, A.tokens - t0);
+    const int t0 = blockIdx.y * F32_TOKENS, many = min(F32_TOKENS, A.tokens - t0);
     const uint8_t* line = A.weight + (long long)blockIdx.x * col_tiles * tile_bytes;
-    const T* x = static_cast<const T*>(A.x) + t0 * A.x_stride;
-    float acc[ANY_TOKENS][2] = {};
-    for (int ct = warp; ct < col_tiles; ct += ANY_WARPS) {
+    const float* x = static_cast<const float*>(A.x) + t0 * A.x_stride;
+    float acc[F32_TOKENS][2] = {};
+    for (int ct = warp; ct < col_tiles; ct += F32_WARPS) {
         const uint8_t* tile = line + (long long)ct * tile_bytes;
         const uint32_t* words = reinterpret_cast<const uint32_t*>(tile + TILE_CODES);
         const uint4 a = reinterpret_cast<const uint4*>(tile)[lane], b = reinterpret_cast<const uint4*>(tile)[32 + lane];
@@ -44,9 +43,9 @@ linear4_any_kernel(const LinearArgs A) {
                 const int shift = 4 * ((e & 1) * 4 + e / 2);
                 const float w0 = value_of((lo[j] >> shift) & 15, wlo), w1 = value_of((hi[j] >> shift) & 15, whi);
 #pragma unroll
-                for (int i = 0; i < ANY_TOKENS; ++i)
+                for (int i = 0; i < F32_TOKENS; ++i)
                     if (i < many) {
-                        const float v = to_f32<T>(x[i * A.x_stride + c0 + e]);
+                        const float v = x[i * A.x_stride + c0 + e];
                         acc[i][0] = fmaf(v, w0, acc[i][0]);
                         acc[i][1] = fmaf(v, w1, acc[i][1]);
                     }
@@ -54,7 +53,7 @@ linear4_any_kernel(const LinearArgs A) {
         }
     }
 #pragma unroll
-    for (int i = 0; i < ANY_TOKENS; ++i)
+    for (int i = 0; i < F32_TOKENS; ++i)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             float v = acc[i][r];
@@ -63,19 +62,18 @@ linear4_any_kernel(const LinearArgs A) {
             if (t == 0) part[warp][i][g + 8 * r] = v;
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < many * TILE_ROWS; i += ANY_WARPS * 32) {
+    for (int i = threadIdx.x; i < many * TILE_ROWS; i += F32_WARPS * 32) {
         const int tok = i / TILE_ROWS, row = i % TILE_ROWS, n = blockIdx.x * TILE_ROWS + row;
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < ANY_WARPS; ++w) v += part[w][tok][row];
-        if (n < A.rows) static_cast<T*>(A.out)[(t0 + tok) * A.out_stride + n] = from_f32<T>(v);
+        for (int w = 0; w < F32_WARPS; ++w) v += part[w][tok][row];
+        if (n < A.rows) static_cast<float*>(A.out)[(t0 + tok) * A.out_stride + n] = v;
     }
 }
 
-template <typename T>
-int launch_any(const LinearArgs& A, cudaStream_t stream) {
-    const dim3 grid((A.rows + TILE_ROWS - 1) / TILE_ROWS, (A.tokens + ANY_TOKENS - 1) / ANY_TOKENS);
-    return xb_launch_few(linear4_any_kernel<T>, grid, dim3(ANY_WARPS * 32), 0, stream, A);
+int launch_f32(const LinearArgs& A, cudaStream_t stream) {
+    const dim3 grid((A.rows + TILE_ROWS - 1) / TILE_ROWS, (A.tokens + F32_TOKENS - 1) / F32_TOKENS);
+    return xb_launch_few(linear4_f32_kernel, grid, dim3(F32_WARPS * 32), 0, stream, A);
 }
 
 }  // namespace
@@ -83,9 +81,9 @@ int launch_any(const LinearArgs& A, cudaStream_t stream) {
 static int linear4(int dtype, void* out, const void* x, const uint8_t* weight, long long out_stride, long long x_stride, int tokens, int rows, int columns,
                    int group, int early, int* err, cudaStream_t stream) {
     if (tokens <= 0 || rows <= 0) return 0;
-    if (columns < 1 || (group != 32 && group != 64 && group != 128) || tokens > 65535 * ANY_TOKENS) return (int)cudaErrorInvalidValue;
+    if (columns < 1 || (group != 32 && group != 64 && group != 128) || tokens > 65535 * F32_TOKENS) return (int)cudaErrorInvalidValue;
     const LinearArgs A{out, x, weight, out_stride, x_stride, tokens, rows, columns, TILE_COLS / group, early};
-    if (dtype == XB_F32) return launch_any<float>(A, stream);
+    if (dtype == XB_F32) return launch_f32(A, stream);
     // Few rows (us, few-row kernel / many-row kernel): 8 rows of 4,096 x 24,576 14.9 / 22.4, 9 rows 23.5 / 22.4, 16 rows of it 25.0 / 21.9, of 12,288 x 4,096 13.6 / 10.7, of
     // 2,048 x 2,048 4.7 / 4.0, but of 1,024 x 1,024 2.7 / 3.9; 17 of that 4,096 x 24,576 43 / 22, of 4,096 x 4,096 8.7 / 6.8.
     const bool many = A.tokens > 16 || (A.tokens > 8 && (long long)A.rows * A.columns > 1 << 20);
