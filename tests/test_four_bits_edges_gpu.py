@@ -263,3 +263,17 @@ def test_requests_of_16_to_63_rows_beside_larger_ones(news, contexts, d, window)
                 allowed = allowed + (2 + 2 * float((p * (np.abs(kk) @ np.abs(q[t, h]))).sum() * a.scale)) * 2.0 ** -11 * size + 2.0 ** -25 * np.abs(vv).max()
                 off = np.abs(got[t, h] - want)
                 assert np.all(off <= allowed), (b, i, h, (off / allowed).max())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [128, 96, 256])
+@pytest.mark.parametrize("small", [1e-12, 1e-20, 1e-30])
+def test_small_values_beside_larger_ones_that_hardly_count(small, d, dtype):
+    """The second page's values are ordinary and its scores 200 below the others'."""
+    a = with_values(Attend([1, 2], [300, 90], 4, 1, d, dtype, scale=1.0), lambda at: np.where(np.arange(len(at)) == 1, 1.0, small))
+    a.q.fill_(1.0)
+    rng, level = np.random.default_rng(3), np.zeros(a.pages)
+    level[a.table[:, 1]] = -200.0 / d
+    a.data[0] = fourbit.page_bytes(rng.normal(size=(a.pages, 1, a.ps, d)) * 0.05 + level[:, None, None, None], a.ps)
+    a.run()
+    a.check()

@@ -11,9 +11,9 @@
 //   output: sum_keys (p s) (code - 8) + p (m + 8 s): p s is rounded to bfloat16 once, and around the middle of the codes that rounding is no
 //           larger than that of a probability times a value; the second sum is float32.  8 sum(p s) is a product with a constant operand.
 // The softmax's reference is a number per column that moves only when a score is more than 2^8 above it.
-// The products of values are ordinary float32 numbers for values from 2^-28 to 2^50 in size, beside which smaller ones count as part of a sum.  A segment whose
-// values are all smaller, that has larger ones, or a group that is no number, is known by its sums' sizes and done again number by number.  (A power of two
-// that follows the values instead: 64 single tokens 51 us instead of 48, the loop has no register for it.)
+// The products of values are ordinary float32 numbers for values of up to 2^50 and sums of 2^-28 and more.  A segment with smaller sums, larger values or a
+// group that is no number is known by its sums' sizes and done again number by number.  (A power of two that follows the values instead: 64 single tokens
+// 51 us instead of 48, the loop has no register for it.)
 //
 // The tiles (32 keys) of all jobs are one line cut into equal shares, one a warp, whatever the lengths are: warps of a block have nothing to do with each
 // other.  A warp fetches its keys and values into a ring of its own with bulk copies.  Parts of a job that several warps share are joined by a
@@ -202,7 +202,7 @@ __device__ __forceinline__ void load_query(const __nv_bfloat16* q, int c, int d,
     }
 }
 
-constexpr uint32_t VALUES_FROM = (127 - 28) << 7, VALUES_TO = (127 + 50) << 7, NO_NUMBER = 0x8000u;       // bits of bfloat16 sizes; above all of them
+constexpr uint32_t VALUES_TO = (127 + 50) << 7, NO_NUMBER = 0x8000u;       // bits of 2^50 in bfloat16; above those of all sizes
 
 // Bits of the largest scale or least value of a group's word, NO_NUMBER for one that is not finite.
 __device__ __forceinline__ uint32_t size_of_word(uint32_t word) {
@@ -642,7 +642,7 @@ cache4_attention_mma_kernel(const __grid_constant__ AttendArgs A, const Line lin
         bool ordinary = true;
         if (!failed && (large || (of_p > 0 && __uint_as_float(of_words) <= 0x1p-25f * __uint_as_float(of_p)))) {
             const uint32_t most = size_of_values<NG>(A, w.b, w.g, max(from * STEP, first_key), min(min(to * STEP, pos1 + 1), w.r.keys));
-            ordinary = most == 0 || (most >= VALUES_FROM && most < VALUES_TO);         // (else it is the queries or keys, or signs that differ)
+            ordinary = large ? most < VALUES_TO : most == 0;       // (if it is not the values it is the queries or keys)
         }
         if (!ordinary) rows_by_number<NG>(A, w.b, w.g, row0, rows, max(from * STEP, first_key), to * STEP, whole ? nullptr : line.part_o + part * ROWS * DP, line.part_ml + part * ROWS * 2);
         if (ordinary) {
