@@ -169,7 +169,7 @@ def with_values(a, sizes):
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("d", [128, 48, 256])
 @pytest.mark.parametrize("news,contexts", [([1, 6], [100, 37]), ([1], [3000]), ([100], [137])])
-@pytest.mark.parametrize("size", [1e-11, 1e-15, 1e-20, 1e-24, 1e10, 1e25])
+@pytest.mark.parametrize("size", [1e-11, 1e-15, 1e-20, 1e-24, 1e-31, 1e10, 1e25])
 def test_values_of_any_size(size, news, contexts, d, dtype):
     """Values' sizes apart from the keys', in each of the kernels."""
     a = with_values(Attend(news, contexts, 8, 2, d, dtype), lambda at: size)
@@ -277,3 +277,96 @@ def test_small_values_beside_larger_ones_that_hardly_count(small, d, dtype):
     a.data[0] = fourbit.page_bytes(rng.normal(size=(a.pages, 1, a.ps, d)) * 0.05 + level[:, None, None, None], a.ps)
     a.run()
     a.check()
+
+
+@pytest.mark.parametrize("d,ps", [(128, 16), (48, 8), (128, 4), (64, 12)])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("power", [10, 18, 24, 40, 60])
+@pytest.mark.parametrize("news,contexts", [([100], [137]), ([1, 40, 200, 20], [300, 90, 64, 10])])
+def test_portions_with_a_key_or_value_far_larger_than_the_others(news, contexts, power, which, d, ps):
+    """A token in the middle of a portion and its last one, whose key or value is 2^power times the others' size: rows that do not see it, and rows that see it with a
+    score far below the others', have their digits."""
+    nh, nkv = 8, 2
+    a = Attend(news, contexts, nh, nkv, d, BF, ps=ps)
+    rng = np.random.default_rng(5)
+    x = [rng.normal(size=(a.pages, nkv, ps, d)) for _ in range(2)]
+    b = len(news) // 2                       # the longest portion's request
+    for pos in (a.lengths[b] - 1, a.lengths[b] - news[b] // 2 - 1):
+        at = a.table[b, pos // ps], slice(None), pos % ps
+        x[which][at] *= 2.0 ** power
+        x[0][at] = -np.abs(x[0][at]) - (30 if which else 0)          # (queries of positive numbers give it a low score)
+    a.q.abs_()
+    a.data = [fourbit.page_bytes(y, ps) for y in x]
+    got = a.run().double().cpu().numpy()
+    keys, vals = (fourbit.page_values(y, ps, d) for y in a.data)
+    q = a.q.double().cpu().numpy()
+    for b, n in enumerate(news):
+        j = np.arange(a.lengths[b])
+        page = a.table[b][j // ps]
+        for i in range(n):
+            pos, t = a.lengths[b] - n + i, a.start[b] + i
+            seen = j <= pos
+            for h in (0, 5):
+                kk, vv = keys[page, h // 4, j % ps][seen], vals[page, h // 4, j % ps][seen]
+                s = kk @ q[t, h] * a.scale
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                want, size = p @ vv, p @ np.abs(vv)
+                # float16 operands (see above) or a bfloat16 probability times a scale; scores of the keys that count
+                steps = (p * (np.abs(kk) @ np.abs(q[t, h]))).sum() * a.scale
+                allowed = HALF[BF] * np.abs(want) + (4 * (d + 16) * 2.0 ** -23 * steps + (64 + seen.sum() / 16) * 2.0 ** -23 + (2 + 2 * steps) * 2.0 ** -11 + 2 * 3 * 2.0 ** -8) * size
+                off = np.abs(got[t, h] - want)
+                # values up to 2^18 times the others': 2^-31 of the largest for every key
+                allowed = allowed + (seen.sum() * 2.0 ** -31 * 2.0 ** power if which and power <= 18 else 0)
+                assert np.all(off <= allowed), (b, i, h, (off / allowed).max())
+
+
+def check_few_rows(a):
+    """Against 64 bits with the bound of the kernel for few rows: bfloat16 roundings of a probability, by itself and times a group's scale, for both parts of
+    m + s code, and float32 sums (test_cache4_gpu.Attend.check), which is also what requests that the kernel for many rows leaves get."""
+    nh, nkv, d = a.sizes
+    got, q = a.out.double().cpu().numpy(), a.q.double().cpu().numpy()
+    keys, vals = (fourbit.page_values(x, a.ps, d) for x in a.data)
+    codes, s, m = fourbit.page_parts(a.data[1], a.ps, d)
+    parts = np.abs(m)[..., np.arange(d) // 32] + s[..., np.arange(d) // 32] * codes
+    for b, n in enumerate(a.news):
+        j = np.arange(a.lengths[b])
+        page = a.table[b][j // a.ps]
+        for i in range(n):
+            seen, t = j <= a.lengths[b] - n + i, a.start[b] + i
+            for h in range(nh):
+                g = h // (nh // nkv)
+                kk, vv, pp = (x[page, :, j % a.ps][seen, g] for x in (keys, vals, parts))
+                x = kk @ q[t, h] * a.scale
+                p = np.exp(x - x.max())
+                p /= p.sum()
+                steps = np.abs(kk).max() * np.abs(q[t, h]).sum() * a.scale
+                allowed = HALF[BF] * np.abs(p @ vv) + (2 * (d + 16) * 2.0 ** -23 * steps + (64 + seen.sum() / 16) * 2.0 ** -23) * (p @ np.abs(vv)) + 2 * 2.0 ** -8 * (p @ pp)
+                assert np.all(np.abs(got[t, h] - p @ vv) <= allowed), (b, i, h)
+
+
+def test_a_captured_step_whose_values_come_to_differ():
+    """The same graph before and after a value grows: which kernel gives a request's rows is seen on the device."""
+    from xinfer_b200 import kernels as k
+    a = Attend([100, 30, 2], [137, 60, 500], 8, 2, 128, BF)
+    caches, lengths, start, table = a.tensors()
+    scratch = torch.zeros(k.cache4_attention_scratch(a.q.shape[0], 3, 8, 2, 128, BF, 100), device=DEV)
+
+    def call():
+        k.cache4_attention(a.out, a.q, *caches, lengths, start, table, a.ps, a.scale, a.err, scratch=scratch, longest=100)
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    plain = a.data[1].copy()
+    grown = with_values(a, lambda at: np.where(np.arange(len(at)) == 1, 2.0 ** 30, 1.0)).data[1].copy()
+    for data in (plain, grown, plain, grown):
+        a.data[1] = data
+        want = a.run().clone()
+        (a.check if data is plain else lambda: check_few_rows(a))()
+        for cache, part in zip(caches, a.data):
+            cache.copy_(torch.from_numpy(part))
+        a.out.fill_(9.0)
+        graph.replay()
+        assert torch.equal(a.out, want) and int(a.err) == 0

@@ -4,7 +4,8 @@
 //
 // Three kernels.  bfloat16, pages of a multiple of 8 tokens, heads of up to 128 channels or of 225 to 256: cache4_attention_mma.cu, which reads the keys once
 // for 8 or 16 rows.  Requests of TC_ROWS rows (tokens times query heads of a key/value head) and more, heads of up to 128 channels, a scale above zero, pages whose
-// bytes are a multiple of 16: cache4_attention_tc.cu, once for 256 rows.  Everything else, float32 first of all: the one below.
+// bytes are a multiple of 16: cache4_attention_tc.cu, once for 256 rows (beside the first or the last, which takes what it leaves).  Everything else, float32 first of
+// all: the one below.
 #include "cache4_attention_mma.h"
 #include "cache4_attention_tc.h"
 
@@ -40,7 +41,7 @@ cache4_attention_any_kernel(const AttendArgs A, float* parts, int splits) {
     int* place = page + KT;
     pdl_overlap_few();
     const int b = blockIdx.y, g = blockIdx.x % A.nkv, group = A.group, step = gridDim.x / A.nkv;
-    const Request r = request_of(A, b);
+    const Request r = request_of<true>(A, b);
     const int rows = r.nodes * group;
     for (int rt = blockIdx.x / A.nkv; rt * RT < rows; rt += step) {
         const int row0 = rt * RT, many = min(RT, rows - row0);
@@ -236,7 +237,8 @@ AnyGrid any_grid(int requests, int nh, int nkv, int longest) {
 
 template <typename T>
 int launch_any(const AttendArgs& A, int longest, float* scratch, cudaStream_t stream) {
-    const AnyGrid g = any_grid(A.requests, A.nh, A.nkv, longest);
+    AnyGrid g = any_grid(A.requests, A.nh, A.nkv, longest);
+    if (A.wide) g.splits = 1;                  // (for requests that another kernel has left: there is no scratch for shares)
     static unsigned long long roomy[2] = {0, 0};
     const bool narrow = padded(A.d) <= 64;
     auto go = [&](auto kernel, unsigned long long* done) {
@@ -258,18 +260,15 @@ static int cache4_attention(int dtype, void* out, const void* q, const uint8_t* 
     if (requests > REQUESTS_MAX || d < 1 || d > DIM_MOST || nkv < 1 || nh < nkv || nh % nkv || page_size < 1 || (long long)page_size * row_bytes(d) > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     if ((long long)table_stride * page_size > KEYS_MOST || (long long)tokens * nh > ROWS_MOST) return (int)cudaErrorInvalidValue;
     AttendArgs A{out, q, k_cache, v_cache, lengths, token_start, block_table, out_stride, q_stride, tokens, requests, table_stride, nh, nkv, d, page_size,
-                       num_pages, window, nh / nkv, ((1ull << 32) + (unsigned)(nh / nkv) - 1) / (unsigned)(nh / nkv), 0, 0x7fffffff, scale, err};
+                       num_pages, window, nh / nkv, ((1ull << 32) + (unsigned)(nh / nkv) - 1) / (unsigned)(nh / nkv), 0, 0x7fffffff, scale, err, nullptr};
     if (dtype == XB_BF16 && tc_takes(A, longest)) {
-        // requests of few rows beside those of many have the kernel for few (each reads on the device which requests are its own)
+        // requests of few rows beside those of many have the kernel for few (each reads on the device which requests are its own), which also takes what the
+        // one for many leaves; where it does not take such pages the general one does
         const bool both = mma_takes(A);
-        if (both) {
-            A.rows_from = OWN_ROWS;
-            const int rc = tc_launch(A, scratch, stream);
-            if (rc) return rc;
-            A.rows_from = 0, A.rows_to = OWN_ROWS;
-            return mma_launch(A, OWN_ROWS, scratch + tc_scratch(d), stream);
-        }
-        return tc_launch(A, scratch, stream);
+        A.rows_from = both ? OWN_ROWS : 0;
+        if (const int rc = tc_launch(A, scratch, stream)) return rc;
+        A.rows_from = 0, A.rows_to = both ? OWN_ROWS : 0, A.wide = tc_wide(d, scratch);
+        return both ? mma_launch(A, OWN_ROWS, scratch + tc_scratch(d), stream) : launch_any<__nv_bfloat16>(A, longest, nullptr, stream);
     }
     if (dtype == XB_BF16 && mma_takes(A)) return mma_launch(A, (nh / nkv) * (long long)longest > TC_ROWS ? TC_ROWS : (nh / nkv) * longest, scratch, stream);
     return dtype == XB_F32 ? launch_any<float>(A, longest, scratch, stream) : launch_any<__nv_bfloat16>(A, longest, scratch, stream);

@@ -19,7 +19,15 @@ struct AttendArgs {
     int rows_from, rows_to;        // requests of other numbers of rows (tokens times query heads of a key/value head) are another kernel's
     float scale;
     int* err;
+    const int* wide;               // null, or: whether the kernel for many rows has left requests to this one, then pairs of the first and the last of some (WIDE_PAIRS)
 };
+constexpr int WIDE_PAIRS = 148;            // a pair for each of its blocks; the first behind the last: none
+
+static __device__ __noinline__ bool in_wide_pairs(const int* wide, int b) {
+    for (int i = 0; i < WIDE_PAIRS; ++i)
+        if (b >= wide[2 + 2 * i] && b <= wide[3 + 2 * i]) return true;
+    return false;
+}
 
 // The token that a row (token, query head of the group) of a request belongs to: row / group, right for rows below 2^32 / group.
 __device__ __forceinline__ int token_of(const AttendArgs& A, int row) { return (int)((unsigned)row * A.group_inv >> 32); }
@@ -36,6 +44,8 @@ struct Request {
     int first_pos;
     int keys;                      // keys that lie in the table's row
 };
+// LEFT: with those that the kernel for many rows has left.
+template <bool LEFT>
 __device__ __forceinline__ Request request_of(const AttendArgs& A, int b) {
     Request r;
     r.first = min(max(A.token_start[b], 0), A.tokens);               // (starts outside the tokens count as the nearest bound)
@@ -46,7 +56,7 @@ __device__ __forceinline__ Request request_of(const AttendArgs& A, int b) {
     r.keys = len < 0 ? 0 : (int)(len > most ? most : len);
     r.first_pos = max(len, 0) - r.nodes;
     const int rows = r.nodes * A.group;
-    if (rows < A.rows_from || rows >= A.rows_to) r.nodes = 0;
+    if ((rows < A.rows_from || rows >= A.rows_to) && !(LEFT && A.wide && A.wide[0] && in_wide_pairs(A.wide, b))) r.nodes = 0;
     return r;
 }
 // The sum of the lanes' numbers up to each lane, and of all.  Requests whose tokens overlap can be more work than 32 bits count (others cannot, the

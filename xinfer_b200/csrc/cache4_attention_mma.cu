@@ -62,7 +62,7 @@ struct Walk {
 template <int ROWS>
 __device__ __forceinline__ void set_request(const AttendArgs& A, Walk& w, int b) {
     w.b = b;
-    w.r = request_of(A, b);
+    w.r = request_of<true>(A, b);
     w.pieces = (w.r.nodes * A.group + ROWS - 1) / ROWS;
     w.tile0 = first_seen(A, w.r.first_pos) / KT;
     // (a request that sees no key has a tile all the same: its rows are written)
@@ -227,7 +227,7 @@ __device__ __noinline__ uint32_t size_of_values(const AttendArgs& A, int b, int 
 template <int NG>
 __device__ __noinline__ void rows_by_number(const AttendArgs& A, int b, int g, int row0, int rows, int from, int to, float* part_o, float* part_ml) {
     const int lane = threadIdx.x & 31, ps = A.page_size;
-    const Request r = request_of(A, b);
+    const Request r = request_of<true>(A, b);
     const long long page_bytes = (long long)ps * 20 * NG;
     const int* table = A.block_table + (long long)b * A.table_stride;
     for (int row = 0; row < rows; ++row) {

@@ -8,7 +8,9 @@
 // All operands are float16: 11 digits of m + s code and of a probability, where bfloat16's 8 would each move the result as much as its own rounding
 // does.  float16's range is made up for by powers of two that are undone in float32: one per row of Q; one for every 16 keys of a tile, by which the
 // scores are multiplied; one for every 16 values, by which probabilities are multiplied, relative to the largest so far (which moves O as a new
-// maximum does).  Numbers 2^25 times smaller than the largest value lose digits.  Probabilities are held 2^6 times their size.
+// maximum does).  Probabilities are held 2^6 times their size.  Keys and values much smaller than others lose digits (keys beside ones of 2^24 times their size among
+// sixteen, values beside ones of 2^20), whoever sees those: a block whose keys or values differ by more says so, and its requests are done again by the kernel that
+// takes the rest of the step (cache4_attention.cu).
 // A group's word that is no number is zero in the operand; rows that see its key get no number in the group's channels at the end, the others nothing.
 //
 // The tiles of all jobs are one line cut into equal shares, one a block; parts of a job that blocks share are joined by a second kernel in their order.
@@ -38,7 +40,10 @@ struct Line {
     float* part_o;                 // [blocks][2][DP / 4][256][4]: a block's first segment, if its job began before it, and its last, if its job goes on
     float* part_ml;                // [blocks][2][256][2]
     int* jobs;                     // [blocks][2][8]: parts (0: there is no such part), block of the first, first row, rows, key/value head, request
+    int* wide;                     // AttendArgs::wide of the kernel that follows
 };
+// Exponents of the largest number that a key and a value holds may differ by that much among those that a block meets, and be that small (2^-100).
+constexpr int K_RANGE = 22, V_RANGE = 18, LEAST = 127 - 100;
 
 // What the softmax needs to know of a tile's keys and values.
 struct __align__(16) Info {
@@ -68,7 +73,7 @@ __device__ __forceinline__ void set_piece(const AttendArgs& A, Walk& w) {
 }
 __device__ __forceinline__ void set_request(const AttendArgs& A, Walk& w, int b) {
     w.b = b;
-    w.r = request_of(A, b);
+    w.r = request_of<false>(A, b);
     w.pieces = (w.r.nodes * A.group + ROWS - 1) / ROWS;
 }
 // The pieces one after another, until `f(piece)` is true: their tokens' places by sums.
@@ -267,6 +272,8 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
     __shared__ __align__(8) unsigned long long bars[4 * NS + 16];
     __shared__ uint32_t s_tmem;
     __shared__ Info infos[INFOS];
+    __shared__ unsigned sizes[4];                  // bits of the least and the largest number that a key holds, and a value
+    __shared__ int met[2];                         // the first and the last request
     constexpr uint32_t RAW_CODES = NG * KT * 16, RAW_BYTES = RAW_CODES + KT * NG * 4;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, q_sm = base, kv_sm = base + 2 * Q_ONE, raw_sm = kv_sm + NS * STAGE_BYTES;
     const uint32_t bar0 = smem_u32(bars), k_full0 = bar0, k_empty0 = bar0 + 8 * NS, v_full0 = bar0 + 16 * NS, v_empty0 = bar0 + 24 * NS, rest = bar0 + 32 * NS;
@@ -283,6 +290,8 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
         for (int i = 0; i < 2; ++i) mbar_init(q_ready0 + 8 * i, 4), mbar_init(drained0 + 8 * i, 1);
         mbar_init_fence();
     }
+    if (threadIdx.x < 4) sizes[threadIdx.x] = threadIdx.x & 1 ? 0u : 0x7f800000u;
+    if (threadIdx.x == 0) met[0] = 1, met[1] = 0;
     if (warp == 8) tmem_alloc(&s_tmem, 512);
     if (NG * 32 < DP)                              // channels that no group has: zeros for good (the products of Q and K go over them)
         for (uint32_t i = threadIdx.x * 16; i < NS * STAGE_BYTES; i += THREADS * 16) store16(kv_sm + i, 0, 0, 0, 0);
@@ -307,7 +316,9 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
         const int n0 = part * GP, n1 = min(NG, n0 + GP), quo = KT / ps, rem = KT % ps;
         int st = 0, done = 0;                      // ring stage, tiles
         uint32_t ph = 0;
+        unsigned least = 0x7f800000u, most = 0u;   // of the lane's keys or values that are not all zero
         bool ok = any;
+        if (any && threadIdx.x == 8 * 32) met[0] = w.b;
         for (bool first = true; ok && next_segment(A, w, first); first = false) {
             const int* table = A.block_table + (long long)w.b * A.table_stride;
             const uint8_t* pages = (is_v ? A.v_cache : A.k_cache) + w.g * page_bytes;
@@ -360,6 +371,8 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
                     top = fmaxf(top, strange ? 0.f : fmaf(15.f, fabsf(scale_of(words[n])), fabsf(least_of(words[n]))));
                     if (strange && is_v) odd |= 1u << n, words[n] = 0u;
                 }
+                most = max(most, __float_as_uint(top));
+                least = min(least, top > 0.f ? __float_as_uint(top) : 0x7f800000u);
                 const int expo = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), e = expo == 0 ? 100 : min(141 - expo, 100);
                 const float f = power_of_two(e);
                 const unsigned bits = __ballot_sync(0xffffffffu, is_v ? odd != 0 : there);
@@ -394,6 +407,9 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncwarp();
         }
+        if (any && threadIdx.x == 8 * 32) met[1] = w.b;
+        least = __reduce_min_sync(0xffffffffu, least), most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) atomicMin(&sizes[is_v ? 2 : 0], least), atomicMax(&sizes[is_v ? 3 : 1], most);
     } else if (warp == 16) {
         // ---- S = Q K^T of every tile
         const uint32_t one = elected(), tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
@@ -729,6 +745,11 @@ cache4_attention_tc_kernel(const AttendArgs A, const Line line, float scale_log2
     tc_fence_before();
     __syncthreads();
     if (warp == 8) tmem_free(tmem, 512);
+    if (threadIdx.x == 0) {
+        const int k0 = sizes[0] >> 23, v0 = sizes[2] >> 23;
+        const bool wide = (int)(sizes[1] >> 23) - k0 > K_RANGE || (int)(sizes[3] >> 23) - v0 > V_RANGE || min(k0, v0) < LEAST;
+        *reinterpret_cast<int2*>(line.wide + 2 + 2 * blockIdx.x) = wide ? make_int2(met[0], met[1]) : make_int2(1, 0);
+    }
 }
 
 // A job's parts, joined in the order of the line: every part's blocks take a share of the job's numbers.
@@ -740,12 +761,17 @@ cache4_attention_tc_join_kernel(const AttendArgs A, const Line line) {
     constexpr int DP = NG <= 2 ? 64 : 128, FOURS = NG * 8;
     pdl_launch_dependents();
     pdl_wait();
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+        const int2 met = threadIdx.x < BLOCKS ? *reinterpret_cast<const int2*>(line.wide + 2 + 2 * threadIdx.x) : make_int2(1, 0);
+        const int any = __syncthreads_or(met.x <= met.y);
+        if (threadIdx.x == 0) line.wide[0] = any;
+    }
     const int* job = line.jobs + (size_t)blockIdx.x * JOB_WORDS;
     const int4 head = *reinterpret_cast<const int4*>(job);
     const int parts = head.x;
     if (parts < 1) return;
     const int first = head.y, row0 = head.z, rows = head.w, g = job[4], group = A.group;
-    const Request r = request_of(A, job[5]);
+    const Request r = request_of<false>(A, job[5]);
     // pieces of eight rows and sixteen channels, 32 lanes
     const int mine = ((int)blockIdx.x / 2 - first) * JOIN_BLOCKS + (int)blockIdx.y, shares = parts * JOIN_BLOCKS, total = (rows + 7) / 8 * (FOURS / 4);
     const int lane = threadIdx.x & 31;
@@ -784,6 +810,7 @@ int launch(const AttendArgs& A, float* scratch, cudaStream_t stream) {
     line.part_o = scratch;
     line.part_ml = scratch + (size_t)BLOCKS * 2 * ROWS * DP;
     line.jobs = reinterpret_cast<int*>(line.part_ml + (size_t)BLOCKS * 2 * ROWS * 2);
+    line.wide = const_cast<int*>(xb4::tc_wide(A.d, scratch));
     static unsigned long long roomy = 0;
     if (const int rc = xb_more_smem(cache4_attention_tc_kernel<NG>, smem, &roomy)) return rc;
     const int rc = xb_launch(cache4_attention_tc_kernel<NG>, dim3(BLOCKS), dim3(THREADS), smem, stream, A, line, A.scale * 1.4426950408889634f);
@@ -801,7 +828,10 @@ bool tc_takes(const AttendArgs& A, int longest) {
     const double jobs = (double)A.nkv * ((double)A.tokens * A.group / ROWS + A.requests), tiles = (double)A.table_stride * A.page_size / KT + 2;
     return tc_takes(A.nh, A.nkv, A.d, longest) && tokens_of_rows(A) && A.scale > 0.f && A.num_pages > 0 && (long long)A.page_size * row_bytes(A.d) % 16 == 0 && jobs * (tiles + COST_JOB) < LINE_MOST;
 }
-long long tc_scratch(int d) { return (long long)BLOCKS * 2 * (ROWS * (dp_of(d) + 2) + JOB_WORDS); }
+static_assert(WIDE_PAIRS == BLOCKS && (2 + 2 * BLOCKS + 2) % 4 == 0 && BLOCKS <= JOIN_THREADS);
+static long long wide_at(int d) { return (long long)BLOCKS * 2 * (ROWS * (dp_of(d) + 2) + JOB_WORDS); }
+long long tc_scratch(int d) { return wide_at(d) + 2 + 2 * BLOCKS + 2; }
+const int* tc_wide(int d, const float* scratch) { return reinterpret_cast<const int*>(scratch + wide_at(d)); }
 int tc_launch(const AttendArgs& A, float* scratch, cudaStream_t stream) {
     switch (groups_of(A.d)) {
         case 1: return launch<1>(A, scratch, stream);

@@ -13,6 +13,7 @@ constexpr int TC_ROWS = 48, OWN_ROWS = 16;
 bool tc_takes(int nh, int nkv, int d, int longest);                // whether it may, for a step's largest request
 bool tc_takes(const AttendArgs& A, int longest);
 long long tc_scratch(int d);                                       // float32 numbers, on a 16-byte boundary
+const int* tc_wide(int d, const float* scratch);                   // where it says which requests it leaves to others (AttendArgs::wide)
 int tc_launch(const AttendArgs& A, float* scratch, cudaStream_t stream);
 
 }  // namespace xb4
