@@ -8,15 +8,16 @@
 // All operands are float16: 11 digits of m + s code and of a probability, where bfloat16's 8 would each move the result as much as its own rounding
 // does.  float16's range is made up for by powers of two that are undone in float32: one per row of Q; one for every 16 keys of a tile, by which the
 // scores are multiplied; one for every 16 values, by which probabilities are multiplied, relative to the largest so far (which moves O as a new
-// maximum does).  Probabilities are held 2^6 times their size.  Keys and values much smaller than others lose digits (keys beside ones of 2^24 times their size among
-// sixteen, values beside ones of 2^20), whoever sees those: a block whose keys or values differ by more says so, and its requests are done again by the kernel that
-// takes the rest of the step (cache4_attention.cu).
+// maximum does).  Probabilities are held 2^6 times their size.  Keys and values much smaller than others lose digits, whoever sees those: keys beside ones of 2^24 times
+// their size among sixteen; values beside ones of 2^r times theirs have probabilities that are off by 2^(r - 31) of the largest, which many small ones feel first
+// (2,000 of 2^-13.4 at r = 16: 5 % of the result).  A block whose keys or values differ by more than K_RANGE and V_RANGE says so, and its requests are done again by
+// the kernel that takes the rest of the step (cache4_attention.cu).
 // A group's word that is no number is zero in the operand; rows that see its key get no number in the group's channels at the end, the others nothing.
 //
 // The tiles of all jobs are one line cut into equal shares, one a block; parts of a job that blocks share are joined by a second kernel in their order.
 //
 // Bound by the softmax warps, 3,400 cycles for a tile of 64 keys and 256 rows (1,500 of them the exponentials), and by a job's start and end, 20,000 cycles.  Four
-// requests of up to 512 tokens at up to 4,096 keys, 32 heads over 8 of 128 channels: 104 us, a quarter of the products' rate.
+// requests of up to 512 tokens at up to 4,096 keys, 32 heads over 8 of 128 channels: 106 us, a quarter of the products' rate.
 #include <cuda_fp16.h>
 
 #include "cache4_attention_tc.h"
@@ -43,7 +44,7 @@ struct Line {
     int* wide;                     // AttendArgs::wide of the kernel that follows
 };
 // Exponents of the largest number that a key and a value holds may differ by that much among those that a block meets, and be that small (2^-100).
-constexpr int K_RANGE = 22, V_RANGE = 18, LEAST = 127 - 100;
+constexpr int K_RANGE = 22, V_RANGE = 12, LEAST = 127 - 100;
 
 // What the softmax needs to know of a tile's keys and values.
 struct __align__(16) Info {
