@@ -21,7 +21,7 @@
 //
 // Bound by issued instructions: 377 for 16 keys of 128 channels, 2.2 to 2.4 a cycle of a processor's 4, of which the matrix instructions are 2 cycles each; then
 // by what a segment costs to start and end (20,000 cycles) and by the join.  Bfloat16, 32 heads over 8 of 128 channels: 64 single tokens at up to 4,096 keys 48 us (2.5 TB/s of
-// codes), 24 at up to 32,768 103 us (3.7 TB/s); one token of 16 heads at 1,024 keys 11 us, of which the join is 4.
+// codes), 24 at up to 32,768 101 us (3.8 TB/s); one token of 16 heads at 1,024 keys 11 us, of which the join is 4.
 #include "cache4_attention_mma.h"
 #include "tc_common.cuh"
 

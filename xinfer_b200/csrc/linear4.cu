@@ -84,8 +84,8 @@ static int linear4(int dtype, void* out, const void* x, const uint8_t* weight, l
     if (columns < 1 || (group != 32 && group != 64 && group != 128) || tokens > 65535 * F32_TOKENS) return (int)cudaErrorInvalidValue;
     const LinearArgs A{out, x, weight, out_stride, x_stride, tokens, rows, columns, TILE_COLS / group, early};
     if (dtype == XB_F32) return launch_f32(A, stream);
-    // Few rows (us, few-row kernel / many-row kernel): 8 rows of 4,096 x 24,576 14.9 / 22.4, 9 rows 23.5 / 22.4, 16 rows of it 25.0 / 21.9, of 12,288 x 4,096 13.6 / 10.7, of
-    // 2,048 x 2,048 4.7 / 4.0, but of 1,024 x 1,024 2.7 / 3.9; 17 of that 4,096 x 24,576 43 / 22, of 4,096 x 4,096 8.7 / 6.8.
+    // Few rows (us, few-row kernel / many-row kernel, the weight ready): 8 rows of 4,096 x 24,576 15.1 / 23.0, 9 rows 25.5 / 23.1, 16 rows of it 27.4 / 22.9, of 12,288 x 4,096
+    // 14.4 / 11.2, of 2,048 x 2,048 5.0 / 4.1, but of 1,024 x 1,024 3.1 / 3.9; 17 of that 4,096 x 24,576 47 / 23, of 4,096 x 4,096 9.3 / 7.1.
     const bool many = A.tokens > 16 || (A.tokens > 8 && (long long)A.rows * A.columns > 1 << 20);
     return many && linear4_tc_takes(A) ? linear4_tc(A, err, stream) : linear4_mma(A, stream);
 }

@@ -10,7 +10,7 @@
 //
 // Bound by reading the weight once.  A block's warps and the blocks of a cluster take a range of the columns each, for R tiles of rows at a time, and walk
 // over the rows' tiles; the codes are fetched two or four stages ahead, over the ends of the rows' tiles too (where the caller says that the weight is
-// complete, the first ones before the kernel in front has ended: 5.1 us instead of 5.9 for 4,096 x 6,144 and one row).  Sums meet in shared memory, warp by
+// complete, the first ones before the kernel in front has ended: 5.2 us instead of 6.1 for 4,096 x 6,144 and one row).  Sums meet in shared memory, warp by
 // warp and block by block in their order.
 #include "linear4.h"
 
@@ -299,7 +299,7 @@ int launch(const LinearArgs& A, cudaStream_t stream) {
     constexpr int smem = smem_bytes(NT, R, PER);
     const int groups = ((A.rows + TILE_ROWS - 1) / TILE_ROWS + R - 1) / R, col_tiles = (A.columns + TILE_COLS - 1) / TILE_COLS, blocks_y = (A.tokens + NT * 8 - 1) / (NT * 8);
     // Columns are shared out among a cluster's blocks while all blocks are on the processors at once and a warp has two tiles.  Measured with one, two,
-    // four and eight blocks: 4,096 x 4,096 (one row) 5.6, 4.9, 4.3, 7.4 us; 12,288 columns 19.2, 12.2, 8.9, 12.3; 4,096 x 6,144 6.6, 6.5, 8.0, 11.7.
+    // four and eight blocks (the weight ready): 4,096 x 4,096 (one row) 4.8, 4.8, 7.2, 15.7 us; 12,288 columns 11.9, 8.4, 10.9, 21.4; 4,096 x 6,144 5.1, 7.7, 11.7, 23.7.
     int cluster = 1;
     while (cluster < 8 && (long long)groups * blocks_y * cluster * 2 <= SLOTS && col_tiles >= 2 * WARPS * cluster) cluster *= 2;
     const int most = SLOTS / cluster / blocks_y, wide = groups < most ? groups : (most < 1 ? 1 : most);
@@ -333,7 +333,7 @@ int with_group(const LinearArgs& A, cudaStream_t stream) {
 namespace xb4 {
 
 int linear4_mma(const LinearArgs& A, cudaStream_t stream) {
-    // (sixteen columns for eight rows or fewer: 4,096 x 24,576 23 us instead of 14.6)
+    // (sixteen columns for eight rows or fewer: 4,096 x 24,576 25 us instead of 15.1)
     if (A.tokens > 8) return with_group<2, 2>(A, stream);
     // Four tiles of rows at a time take x out of memory half as often as two, but leave processors idle where they do not go round: whichever has less to do in
     // its longest block, with a sixth more work for two.

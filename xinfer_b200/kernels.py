@@ -2138,7 +2138,9 @@ def cache4_attention(out, q, k_cache, v_cache, lengths, token_start, block_table
     sees the keys up to its own position, of these the last ``window``, by its request's row of ``block_table``.  One that sees nothing
     gets zeros; rows behind the last request's stay as they are.  ``out`` and ``q`` have dense heads, their tokens may lie apart.  ``scratch``: float32,
     ``cache4_attention_scratch`` numbers, contents undefined, not shared by calls that may overlap.  ``longest``: tokens of the request that
-    brings most, as far as the host knows it (1 for a decoding step); the form of the kernels goes by it, never what they compute."""
+    brings most, as far as the host knows it (1 for a decoding step); the form of the kernels goes by it, never what they compute.  Left out, it counts as all that one
+    request could bring: a decoding step of many requests then runs the kernels for portions of prompts first, which find little to do.  In bfloat16, values
+    that are all below 1e-8 or some above 1e15, and in portions of prompts keys or values of very different sizes (2^22 and 2^12 times), have their digits too but take longer."""
     T, nh, d = q.shape
     dtype = q.dtype
     code = dtype_code(dtype)
@@ -2193,7 +2195,8 @@ def linear4_scratch(tokens: int, rows: int, columns: int, dtype) -> int:
 
 def linear4(out, x, weight, *, scratch=None, weight_ready: bool = False, err=None):
     """``out[t, n] = sum_k x[t, k] * W[n, k]`` for rows ``x`` ``[T, columns]`` and a weight in 4 bits (``weights.pack4``); sums in float32, rounded once.
-    ``out`` is ``[T, rows]`` of x's type; rows of both may lie apart.  ``weight_ready``: the caller's word that whatever wrote the weight had ended when the
+    In bfloat16 the weight's numbers m + s code are exact up to 8 rows (16 with weights of up to 2^20 numbers, any with x off 16-byte rows); with more rows each is rounded to
+    bfloat16 first, as a bfloat16 weight would be.  ``out`` is ``[T, rows]`` of x's type; rows of both may lie apart.  ``weight_ready``: the caller's word that whatever wrote the weight had ended when the
     call was made (a captured one: before its graph is launched), as it has for what ``pack4`` returns and for all that the host has waited for.  The weight is then read while the
     kernels ahead in the stream still run; without it only behind them.  Numbers may have any size, scales up to 2^121 in
     bfloat16; a row of x that is not finite gives a row that is not.  ``err``: the step's device error word, which says so where a wait has

@@ -10,7 +10,8 @@ def pack4(weight: torch.Tensor, group: int = 32) -> torch.Tensor:
     """``weight`` ``[rows, columns]`` in groups of 32, 64 or 128 columns with a scale s and a least value m in bfloat16, as uint8
     ``[row tiles, column tiles, bytes]`` on the weight's device: s = (largest - least) / 15, code = round((w - m) / s), value m + s * code.  A tile of 16 rows and
     128 columns has 1,024 bytes of codes, then each row's (s, m) pairs.  Byte ``512 h + 64 r + 16 t + 4 j + b`` of the codes belongs to row 8 h + r and the columns
-    32 j + 8 t + 4 b .. : the low half is column e = 4 b for b < 2 and 4 b - 7 behind, the high half column e + 2.  Rows and columns behind the weight are zeros."""
+    32 j + 8 t + 4 b .. : the low half is column e = 4 b for b < 2 and 4 b - 7 behind, the high half column e + 2.  Rows and columns behind the weight are zeros,
+    which belong to the range of a last group that they fill up: a multiple of ``group`` columns keeps all codes for the weight's own numbers."""
     if weight.dim() != 2 or not weight.is_floating_point() or 0 in weight.shape:
         raise ValueError(f"pack4 takes a matrix of real numbers, not {weight.dtype} {tuple(weight.shape)}")
     if group not in (32, 64, 128):
