@@ -388,3 +388,28 @@ def test_portions_whose_many_small_probabilities_count(below, power):
     a.data = [fourbit.page_bytes(np.broadcast_to(level, values.shape).copy(), a.ps), fourbit.page_bytes(values, a.ps)]
     a.run()
     check_few_rows(a, heads=(0, 17, 36))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [128, 96, 256, 32])
+@pytest.mark.parametrize("news,contexts,times", [([1], [300], 1), ([1], [300], 1500), ([3, 1], [90, 700], 1), ([60], [100], 1)])
+def test_heads_of_a_group_that_count_values_of_different_sizes(news, contexts, times, d, dtype):
+    """Half of a group's heads give all their weight to a page of ordinary values, the other half to the small values of the other pages.  With so many requests
+    (of the same pages) that a request's keys are one segment, too."""
+    a = with_values(Attend(news, contexts, 4, 1, d, dtype, scale=1.0), lambda at: np.where(np.arange(len(at)) == 1, 1.0, 1e-18))
+    if times > 1:
+        a.news, a.lengths, a.table, a.start = a.news * times, a.lengths * times, np.repeat(a.table, times, 0), list(range(times + 1))
+        a.q, a.out = (torch.zeros((times + 2, 4, d), dtype=dtype, device=DEV) for _ in range(2))
+    a.q.fill_(1.0)
+    a.q[:, 1::2] = -1.0
+    rng, level = np.random.default_rng(4), np.zeros(a.pages)
+    level[a.table[:, 1]] = -200.0 / d
+    a.data[0] = fourbit.page_bytes(rng.normal(size=(a.pages, 1, a.ps, d)) * 0.02 + level[:, None, None, None], a.ps)
+    a.run()
+    if times > 1:                      # (all requests are the same one: twenty of them are looked at)
+        a.news, a.start = a.news[:20], a.start[:21]
+        a.out[20:] = 9.0
+    if dtype == F32:
+        a.check()
+    else:
+        check_few_rows(a)

@@ -11,8 +11,8 @@
 //   output: sum_keys (p s) (code - 8) + p (m + 8 s): p s is rounded to bfloat16 once, and around the middle of the codes that rounding is no
 //           larger than that of a probability times a value; the second sum is float32.  8 sum(p s) is a product with a constant operand.
 // The softmax's reference is a number per column that moves only when a score is more than 2^8 above it.
-// The products of values are ordinary float32 numbers for values of up to 2^50 and sums of 2^-28 and more.  A segment with smaller sums, larger values or a
-// group that is no number is known by its sums' sizes and done again number by number.  (A power of two that follows the values instead: 64 single tokens
+// The products of values are ordinary float32 numbers for values of up to 2^50 and sums of 2^-28 and more.  A segment with a row of smaller sums, with larger values or
+// a group that is no number is known by its sums' sizes and done again number by number.  (A power of two that follows the values instead: 64 single tokens
 // 51 us instead of 48, the loop has no register for it.)
 //
 // The tiles (32 keys) of all jobs are one line cut into equal shares, one a warp, whatever the lengths are: warps of a block have nothing to do with each
@@ -625,22 +625,25 @@ cache4_attention_mma_kernel(const __grid_constant__ AttendArgs A, const Line lin
         // ---- the segment's result: whole rows, or a part
         const bool whole = w.i0 == 0 && w.i1 == w.tiles;
         const size_t part = (size_t)me * 2 + (w.from > w.job ? 0 : 1);
-        // the sums' sizes: ordinary ones are finite, and not all below 2^-28 of the sum of probabilities (of which a lane has an eighth at least, if it has most)
-        uint32_t of_words = 0, of_codes = 0, of_p = 0;
+        // the sums' sizes: those of an ordinary column are finite, and not all below 2^-28 of its sum of probabilities
+        bool large = false, small = false;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                of_codes = max(of_codes, __float_as_uint(fabsf(eight[j][e])));
-                if constexpr (BY_WORDS) of_words = max(of_words, __float_as_uint(fabsf(both[j][e])));
+            for (int e = 0; e < 2; ++e) {
+                float of_words = 0.f, of_p = l[j][e];
+                if constexpr (BY_WORDS) of_words = max_nan(fabsf(both[j][e]), fabsf(both[j][e + 2]));
 #pragma unroll
-                for (int n = 0; n < (BY_WORDS ? 0 : NG); ++n) of_words = max(of_words, __float_as_uint(fabsf(rest[j][n][e & 1])));
-                of_p = max(of_p, __float_as_uint(l[j][e & 1]) & 0x7fffffffu);
+                for (int n = 0; n < (BY_WORDS ? 0 : NG); ++n) of_words = max_nan(of_words, fabsf(rest[j][n][e]));
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) of_words = max_nan(of_words, __shfl_xor_sync(0xffffffffu, of_words, o)), of_p += __shfl_xor_sync(0xffffffffu, of_p, o);
+                // (2^120: the lanes' parts are added up yet)
+                large |= !(max_nan(of_words, max_nan(fabsf(eight[j][e]), fabsf(eight[j][e + 2]))) < 0x1p120f);
+                small |= of_p > 0.f && of_words <= 0x1p-28f * of_p;
             }
-        of_words = __reduce_max_sync(0xffffffffu, of_words), of_p = __reduce_max_sync(0xffffffffu, of_p);
-        const bool large = max(of_words, __reduce_max_sync(0xffffffffu, of_codes)) >= 0x7b800000u;       // (2^120: the lanes' parts are added up yet)
+        large = __any_sync(0xffffffffu, large), small = __any_sync(0xffffffffu, small);
         bool ordinary = true;
-        if (!failed && (large || (of_p > 0 && __uint_as_float(of_words) <= 0x1p-25f * __uint_as_float(of_p)))) {
+        if (!failed && (large || small)) {
             const uint32_t most = size_of_values<NG>(A, w.b, w.g, max(from * STEP, first_key), min(min(to * STEP, pos1 + 1), w.r.keys));
             ordinary = large ? most < VALUES_TO : most == 0;       // (if it is not the values it is the queries or keys)
         }
