@@ -413,3 +413,16 @@ def test_heads_of_a_group_that_count_values_of_different_sizes(news, contexts, t
         a.check()
     else:
         check_few_rows(a)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [128, 48])
+@pytest.mark.parametrize("news,contexts", [([1, 6], [100, 37]), ([100], [137])])
+@pytest.mark.parametrize("k_size,q_size", [(1e-28, 1.0), (1e-20, 1.0), (1e12, 1.0), (1e20, 1.0), (1e30, 1.0), (1.0, 1e-30), (1.0, 1e-12), (1.0, 1e20), (1.0, 1e34), (1e-20, 1e20), (1e15, 1e-30)])
+def test_keys_and_queries_of_any_size(k_size, q_size, news, contexts, d, dtype):
+    a = Attend(news, contexts, 8, 2, d, dtype, scale=0.1 / (k_size * q_size))
+    rng = np.random.default_rng(6)
+    a.data[0] = fourbit.page_bytes(rng.normal(size=(a.pages, 2, a.ps, d)) * k_size, a.ps)
+    a.q.copy_((a.q.double() * q_size).to(dtype))
+    a.run()
+    a.check()
